@@ -449,6 +449,32 @@ int nmx_lin_mix_chunk(nmx_ctx *ctx, const nmx_lin_mix_args *a);
 int nmx_lin_chunk_ok(int dk, int dv, int conv_k, int heads);
 int nmx_attn_fused_chunk(nmx_ctx *ctx, const nmx_attn_args *p, int score_rows);
 
+/* ---- sampling -----------------------------------------------------------------------------
+ * A token for each of n rows of logits (row r at logits + r stride, vocab values), from a uniform
+ * number per row. The reference decodes greedily only; this stands where a program that samples has
+ * the argmax of nmx_head_accept. With w_i = exp((l_i - max l) / temperature), in 64 bits, and the
+ * row's tokens in descending order (equal logits: lower index first), the kept ones are the first
+ * top_k; of these the shortest run whose mass reaches top_p of theirs; of these the w_i >= min_p.
+ * The token is the first one in index order at which the running mass of the kept passes u times
+ * their whole. prob (may be NULL) receives its share of the kept mass.
+ * temperature <= 0 or NaN: the first maximum, prob 1. top_k <= 0 or >= vocab, top_p >= 1 or NaN,
+ * min_p <= 0 or NaN: no such filter; top_p <= 0 keeps the first token, min_p >= 1 the maxima. u
+ * below 0 or NaN counts as 0, from 1 on the last kept token is taken. A logit of -inf or NaN is
+ * never chosen, +inf is the largest finite value; a row that has nothing else gives token -1 and
+ * prob 0. Tokens 32 nats below the maximum of a filtered row have no mass (less than 2^-46 each).
+ * params and u are on the device (a captured call reads them at each replay): one record for all
+ * rows (per_row 0) or n of them. work: device scratch of nmx_sample_work_bytes(n, vocab) bytes (0
+ * for a shape that is refused), 16-byte aligned, used by one call at a time. n <= 4096, vocab <=
+ * 2^20. The same inputs give the same outputs on every call. */
+typedef struct {
+    float temperature, top_p, min_p;
+    int32_t top_k;
+} nmx_sample_params;
+size_t nmx_sample_work_bytes(int n, int vocab);
+int nmx_sample(nmx_ctx *ctx, const float *logits, int stride, int vocab, int n,
+               const nmx_sample_params *params, int per_row, const float *u, void *work, int32_t *tok,
+               float *prob);
+
 /* The reference's chain gate (engine/src/spec_adapt.c:56, spec.c:89-97) as a device op, for a
  * caller that drives the reference's own confidence-gated adaptive chain on this device layer;
  * the engine's own adaptive policy (pinfer_spec_params.adaptive) decides on the host and does

@@ -46,6 +46,21 @@ int nmx_fail(nmx_ctx *ctx, const char *fmt, ...) __attribute__((format(printf, 2
                             __LINE__);                                                      \
     } while (0)
 
+/* The context's device made current while a call enqueues its work, the caller's put back after. */
+struct nmx_on_device {
+    int before = -1;
+    explicit nmx_on_device(const nmx_ctx *ctx) {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess)
+            before = now;
+    }
+    ~nmx_on_device() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    nmx_on_device(const nmx_on_device &) = delete;
+    nmx_on_device &operator=(const nmx_on_device &) = delete;
+};
+
 /* Launch-error check after a kernel launch (hipGetLastError). */
 #define NMX_LAUNCHED(ctx, what)                                                             \
     do {                                                                                    \

@@ -1,0 +1,612 @@
+/* Sampling from rows of logits with temperature, top-k, top-p and min-p, from given uniform numbers
+ * (include/nmx.h nmx_sample).
+ *
+ * A row's weights are w_i = exp((l_i - max l) / T), in 64 bits. The kept tokens are a prefix of the
+ * row sorted by descending logit (ties: lower index first), the shortest of what the three filters
+ * allow; the token is the first one, in index order, at which the running mass of the kept weights
+ * passes u times their whole. So nothing is ever sorted: the filters need the logit at which the
+ * prefix ends, the draw a running sum.
+ *
+ * sample_scan_k, one workgroup per 8192 logits of a row, reads the logits once. Rows without a
+ * filter leave the chunk's maximum and its mass. Rows with one leave a histogram of the logits over
+ * bins of 1/8 nat on a grid that every chunk shares (bin B covers 8 l / T in [B, B + 1)), 256 bins
+ * down from the chunk's maximum: counts, masses, and the chunk's indices grouped by bin. What lies
+ * 32 nats below a maximum weighs less than 2^-46 of it and is taken as zero.
+ * sample_pick_k, one workgroup per row, adds the histograms, finds the bin where each filter ends,
+ * selects within that bin among its own members (fetched through the grouped indices), and rescans
+ * only the chunk that the draw falls into.
+ *
+ * Masses are whole numbers, the weight relative to its bin's lower edge (in [1, e^(1/8))) times
+ * 2^40: their sums do not depend on the order in which lanes add them, so a call's result is the
+ * same every time; between bins they are scaled and added in 64-bit floating point in a fixed
+ * order. Each weight is thereby right to 2^-41 of itself. */
+#include "nmx_internal.h"
+#include "nmx_lanes.h"
+
+namespace {
+
+constexpr int SM_CHUNK = 8192; /* logits of a workgroup of sample_scan_k */
+constexpr int SM_T1 = 512, SM_PER = SM_CHUNK / SM_T1;
+constexpr int SM_T2 = 1024, SM_RUN = SM_CHUNK / SM_T2; /* consecutive logits of a thread */
+constexpr int SM_BINS = 256;
+constexpr int SM_MAXC = (1 << 20) / SM_CHUNK; /* chunks of the longest row */
+constexpr int SM_LIST = 8192; /* members of a bin kept in LDS; a bin with more is read again */
+constexpr double SM_ONE = 0x1p40;
+
+/* What sample_scan_k leaves of one chunk. */
+struct Chunk {
+    unsigned long long mass[SM_BINS]; /* by bin, relative to the bin's lower edge, in 2^-40 */
+    double base;                      /* the top bin's number; without a filter the mass */
+    unsigned long long key;           /* greedy rows: the first maximum's key */
+    float max;                        /* -inf: nothing to choose in it */
+    uint32_t pad;
+    uint16_t start[SM_BINS + 8];      /* bin j's members: perm[start[j] .. start[j + 1]) */
+    uint16_t perm[SM_CHUNK];
+};
+
+/* A row's parameters with every value outside its range read as "no filter". */
+struct Par {
+    double T, top_p, min_p;
+    int top_k;
+    bool greedy, filter;
+};
+
+__device__ __forceinline__ Par sample_par(const nmx_sample_params *p, int vocab) {
+    Par r;
+    const float T = p->temperature, tp = p->top_p, mp = p->min_p;
+    r.greedy = !(T > 0.0f);
+    r.T = (double)T;
+    r.top_k = p->top_k > 0 && p->top_k < vocab ? p->top_k : 0;
+    r.top_p = tp < 1.0f ? fmaxf(tp, 0.0f) : 1.0;
+    r.min_p = mp > 0.0f ? fminf(mp, 1.0f) : 0.0;
+    if (!(T < INFINITY)) r.T = 0x1p1000; /* every finite logit alike */
+    r.filter = !r.greedy && (r.top_k || r.top_p < 1.0 || r.min_p > 0.0);
+    return r;
+}
+
+/* NaN is never chosen, +inf is the largest finite value (ties among several). */
+__device__ __forceinline__ float sample_value(float x) {
+    return x == x ? fminf(x, 3.40282347e+38f) : -INFINITY;
+}
+
+/* order-preserving bits of a value that is not NaN (-0 and 0 alike) */
+__device__ __forceinline__ uint32_t sample_key(float x) {
+    const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float sample_unkey(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+__device__ __forceinline__ double grid_pos(float x, double T) { return 8.0 * ((double)x / T); }
+
+/* the weight of x relative to the lower edge of its bin, in 2^-40 */
+__device__ __forceinline__ unsigned long long bin_mass(float x, double T) {
+    const double g = grid_pos(x, T);
+    return (unsigned long long)(exp((g - floor(g)) * 0.125) * SM_ONE + 0.5);
+}
+
+__device__ __forceinline__ float block_max(float v, float *red, int waves) {
+    v = nmx_max_f32_wave(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    for (int w = 0; w < waves; w++) v = fmaxf(v, red[w]);
+    return v;
+}
+
+/* inclusive running sums over the workgroup's threads, in thread order; *total is the last */
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V *red, V *total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const V o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 63) red[w] = v;
+    __syncthreads();
+    V before = 0, all = 0;
+    for (int i = 0; i < waves; i++) {
+        if (i < w) before += red[i];
+        all += red[i];
+    }
+    *total = all;
+    return before + v;
+}
+
+__global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__ logits, int stride,
+                                                       int vocab, Chunk *__restrict__ work,
+                                                       const nmx_sample_params *par, int par_step) {
+    __shared__ float redf[8];
+    __shared__ double redd[8];
+    __shared__ unsigned long long redk[8];
+    __shared__ uint32_t cnt[SM_BINS], wave_cnt[4];
+    __shared__ unsigned long long mass[SM_BINS];
+    __shared__ uint16_t perm[SM_CHUNK];
+    const int tid = threadIdx.x, c = blockIdx.x, row = blockIdx.y;
+    const Par p = sample_par(par + (size_t)row * par_step, vocab);
+    const float *l = logits + (size_t)row * stride + (size_t)c * SM_CHUNK;
+    const int len = vocab - c * SM_CHUNK < SM_CHUNK ? vocab - c * SM_CHUNK : SM_CHUNK;
+    Chunk *out = work + (size_t)row * gridDim.x + c;
+    float v[SM_PER];
+#pragma unroll
+    for (int u = 0; u < SM_PER; u++) {
+        const int i = u * SM_T1 + tid;
+        v[u] = i < len ? l[i] : -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < SM_PER; u++) {
+        v[u] = sample_value(v[u]);
+        mx = fmaxf(mx, v[u]);
+    }
+    if (p.greedy) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int u = 0; u < SM_PER; u++) {
+            const unsigned long long k = (unsigned long long)sample_key(v[u]) << 32 |
+                                         (0xffffffffu - (uint32_t)(c * SM_CHUNK + u * SM_T1 + tid));
+            if (v[u] > -INFINITY && k > best) best = k;
+        }
+        best = nmx_max_u64_wave(best);
+        if ((tid & 63) == 0) redk[tid >> 6] = best;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < SM_T1 / 64; w++) best = redk[w] > best ? redk[w] : best;
+            out->key = best;
+        }
+        return;
+    }
+    mx = block_max(mx, redf, SM_T1 / 64);
+    if (tid == 0) out->max = mx;
+    if (!(mx > -INFINITY)) {
+        if (tid == 0) out->base = 0.0;
+        return;
+    }
+    if (!p.filter) {
+        double s = 0.0;
+#pragma unroll
+        for (int u = 0; u < SM_PER; u++) s += exp(((double)v[u] - (double)mx) / p.T);
+        double total;
+        block_scan(s, redd, &total);
+        if (tid == 0) out->base = total;
+        return;
+    }
+    if (tid < SM_BINS) cnt[tid] = 0, mass[tid] = 0;
+    __syncthreads();
+    const double base = floor(grid_pos(mx, p.T));
+    uint32_t at[SM_PER]; /* bin << 16 | rank; all ones: no weight */
+#pragma unroll
+    for (int u = 0; u < SM_PER; u++) {
+        at[u] = 0xffffffffu;
+        const double d = base - floor(grid_pos(v[u], p.T)); /* inf for -inf */
+        if (d < (double)SM_BINS) {
+            const uint32_t j = (uint32_t)(int)d;
+            at[u] = j << 16 | atomicAdd(&cnt[j], 1u);
+            atomicAdd(&mass[j], bin_mass(v[u], p.T));
+        }
+    }
+    __syncthreads();
+    uint32_t first = 0; /* members of the bins above bin tid */
+    if (tid < SM_BINS) {
+        uint32_t x = cnt[tid];
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(x, d);
+            if ((tid & 63) >= d) x += o;
+        }
+        if ((tid & 63) == 63) wave_cnt[tid >> 6] = x;
+        first = x - cnt[tid];
+    }
+    __syncthreads();
+    if (tid < SM_BINS) {
+        for (int w = 0; w < tid >> 6; w++) first += wave_cnt[w];
+        out->start[tid] = (uint16_t)first;
+        out->mass[tid] = mass[tid];
+        if (tid == SM_BINS - 1) out->start[SM_BINS] = (uint16_t)(first + cnt[tid]);
+        cnt[tid] = first;
+    }
+    if (tid == 0) out->base = base;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < SM_PER; u++)
+        if (at[u] != 0xffffffffu) perm[cnt[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)(u * SM_T1 + tid);
+    __syncthreads();
+    uint32_t *po = (uint32_t *)out->perm;
+    for (int i = tid; i < SM_CHUNK / 2; i += SM_T1) po[i] = ((const uint32_t *)perm)[i];
+}
+
+/* The row's state in sample_pick_k. */
+struct Pick {
+    unsigned long long mass[SM_BINS];    /* the row's histogram, from its top bin down */
+    unsigned long long tally[SM_BINS];   /* masses of a selection's digit */
+    double chunk_mass[SM_MAXC];
+    double redd[16];
+    float redf[16];
+    uint32_t cnt[SM_BINS], digit[SM_BINS], redu[16];
+    int off[SM_MAXC];                    /* the chunk's top bin below the row's */
+    uint32_t seg[SM_MAXC + 1];           /* running sizes of a bin's segments */
+    uint32_t ties[SM_MAXC];
+    unsigned long long cand[SM_MAXC];    /* masses of a bin's kept members by chunk */
+    unsigned long long redk[16], sel_m;
+    double sel_d;
+    uint32_t sel_n;
+    int hit, last;
+    uint32_t list[SM_LIST];
+};
+
+/* What a row keeps: the keys above key, and of those equal to it the first `ties` in index order. */
+struct Cut {
+    uint32_t key, ties;
+};
+
+/* The members of row bin b as i = 0 .. S.seg[C] - 1: chunk and key of one. */
+__device__ __forceinline__ uint32_t member(const Pick &S, const Chunk *ch, const float *l, int C, int b,
+                                           uint32_t i, int *c_out) {
+    int lo = 0, hi = C; /* the last chunk whose segment starts at or before i */
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (S.seg[m] <= i) lo = m;
+        else hi = m;
+    }
+    *c_out = lo;
+    const Chunk &k = ch[lo];
+    const int at = k.perm[k.start[b - S.off[lo]] + (i - S.seg[lo])];
+    return sample_key(sample_value(l[(size_t)lo * SM_CHUNK + at]));
+}
+
+/* Running sizes of bin b's segments over the chunks; the keys into the list if they fit. */
+__device__ void open_bin(Pick &S, const Chunk *ch, const float *l, int C, int b) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    uint32_t x = 0;
+    if (tid < C) {
+        const int j = b - S.off[tid];
+        if (j >= 0 && j < SM_BINS) x = (uint32_t)ch[tid].start[j + 1] - ch[tid].start[j];
+    }
+    uint32_t total;
+    const uint32_t incl = block_scan(x, S.redu, &total);
+    if (tid < C) S.seg[tid] = incl - x;
+    if (tid == 0) S.seg[C] = total;
+    __syncthreads();
+    if (total <= SM_LIST)
+        for (uint32_t i = tid; i < total; i += SM_T2) {
+            int c;
+            S.list[i] = member(S, ch, l, C, b, i, &c);
+        }
+    __syncthreads();
+}
+
+/* Among the members of the opened bin b with keys of at least floor_key: the key at which the run in
+ * descending order reaches `want` members (by count) or the mass want_mass (in 2^-40 of the bin's
+ * lower edge). above / above_mass: what lies strictly above that key. Four digits of 8 bits. */
+__device__ uint32_t select_key(Pick &S, const Chunk *ch, const float *l, int C, int b, double T,
+                               bool by_count, uint32_t want, double want_mass, uint32_t floor_key,
+                               uint32_t *above, double *above_mass) {
+    const int tid = threadIdx.x;
+    const uint32_t total = S.seg[C];
+    uint32_t prefix = 0, n_above = 0;
+    unsigned long long m_above = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        if (tid < SM_BINS) S.digit[tid] = 0, S.tally[tid] = 0;
+        if (tid == 0) S.hit = -1, S.last = -1;
+        __syncthreads();
+        for (uint32_t i = tid; i < total; i += SM_T2) {
+            int c;
+            const uint32_t k = total <= SM_LIST ? S.list[i] : member(S, ch, l, C, b, i, &c);
+            if (k < floor_key || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
+            const uint32_t d = 255 - ((k >> shift) & 255);
+            atomicAdd(&S.digit[d], 1u);
+            if (!by_count) atomicAdd(&S.tally[d], bin_mass(sample_unkey(k), T));
+        }
+        __syncthreads();
+        const uint32_t n = tid < SM_BINS ? S.digit[tid] : 0;
+        const unsigned long long m = tid < SM_BINS ? S.tally[tid] : 0;
+        uint32_t n_all;
+        unsigned long long m_all;
+        const uint32_t n_to = n_above + block_scan(n, S.redu, &n_all);
+        const unsigned long long m_to = m_above + block_scan(m, S.redk, &m_all);
+        if (n) {
+            atomicMax(&S.last, tid);
+            const bool reached = by_count ? n_to >= want : (double)m_to >= want_mass;
+            const bool before = by_count ? n_to - n >= want : (double)(m_to - m) >= want_mass;
+            if (reached && !before) S.hit = tid; /* one digit at most */
+        }
+        __syncthreads();
+        /* a mass that a rounding keeps from being reached: the last digit. One that is reached at
+         * nothing (want_mass 0): the first */
+        int hit = S.hit;
+        if (hit < 0) hit = !by_count && want_mass <= (double)m_above ? -2 : S.last;
+        __syncthreads();
+        if (hit == -2 && n && n_to - n == n_above) S.hit = tid; /* the first digit with members */
+        if (hit >= 0 && tid == 0) S.hit = hit;
+        __syncthreads();
+        hit = S.hit;
+        if (tid == hit) S.sel_n = n_to - n, S.sel_m = m_to - m;
+        __syncthreads();
+        prefix = prefix << 8 | (uint32_t)(255 - hit);
+        n_above = S.sel_n;
+        m_above = S.sel_m;
+    }
+    *above = n_above;
+    *above_mass = (double)m_above;
+    return prefix;
+}
+
+/* The least logit whose weight is at least min_p of the largest: its key. */
+__device__ uint32_t min_p_key(float mx, double T, double min_p) {
+    auto in = [&](float x) { return exp(((double)x - (double)mx) / T) >= min_p; };
+    uint32_t k = sample_key(sample_value((float)fmax((double)mx + T * log(min_p), -3.40282346638528859e+38)));
+    const uint32_t top = sample_key(mx), low = sample_key(-3.40282347e+38f);
+    if (k > top) k = top;
+    while (k < top && !in(sample_unkey(k))) k++;
+    while (k > low && in(sample_unkey(k - 1))) k--;
+    return k;
+}
+
+__global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__ logits, int stride,
+                                                       int vocab, int C, const Chunk *__restrict__ work,
+                                                       const nmx_sample_params *par, int par_step,
+                                                       const float *__restrict__ uni,
+                                                       int32_t *__restrict__ tok,
+                                                       float *__restrict__ prob) {
+    __shared__ Pick S;
+    const int tid = threadIdx.x, row = blockIdx.x;
+    const Par p = sample_par(par + (size_t)row * par_step, vocab);
+    const float *l = logits + (size_t)row * stride;
+    const Chunk *ch = work + (size_t)row * C;
+    auto answer = [&](int t, double pr) {
+        tok[row] = t;
+        if (prob) prob[row] = (float)pr;
+    };
+    if (p.greedy) {
+        if (tid < 64) {
+            unsigned long long k = 0;
+            for (int c = tid; c < C; c += 64) k = ch[c].key > k ? ch[c].key : k;
+            k = nmx_max_u64_wave(k);
+            if (tid == 0) answer(k ? (int)(0xffffffffu - (uint32_t)k) : -1, k ? 1.0 : 0.0);
+        }
+        return;
+    }
+    const float u = uni[row];
+    const double ud = u > 0.0f ? (double)fminf(u, 1.0f) : 0.0;
+    const float mc = tid < C ? ch[tid].max : -INFINITY;
+    const float mx = block_max(mc, S.redf, SM_T2 / 64);
+    if (!(mx > -INFINITY)) { /* nothing to choose from */
+        if (tid == 0) answer(-1, 0.0);
+        return;
+    }
+    Cut cut = {0, 0xffffffffu};
+    double mass = 0.0; /* chunk tid's kept mass, the largest weight being 1 */
+    if (!p.filter) {
+        if (tid < C && mc > -INFINITY) mass = ch[tid].base * exp(((double)mc - (double)mx) / p.T);
+    } else {
+        const double g_top = grid_pos(mx, p.T), top = floor(g_top);
+        const double unit = exp((top - g_top) * 0.125) / SM_ONE; /* a mass of the top bin, as a weight */
+        if (tid < C) {
+            const double d = mc > -INFINITY ? top - ch[tid].base : (double)SM_BINS;
+            S.off[tid] = d < (double)SM_BINS ? (int)d : SM_BINS;
+            S.cand[tid] = 0, S.ties[tid] = 0;
+        }
+        if (tid < SM_BINS) S.cnt[tid] = 0, S.mass[tid] = 0;
+        __syncthreads();
+        const int b = tid & (SM_BINS - 1);
+        {
+            uint32_t n = 0;
+            unsigned long long m = 0;
+            for (int c = tid / SM_BINS; c < C; c += SM_T2 / SM_BINS) {
+                const int j = b - S.off[c];
+                if (j < 0) continue;
+                n += (uint32_t)ch[c].start[j + 1] - ch[c].start[j];
+                m += ch[c].mass[j];
+            }
+            if (n) atomicAdd(&S.cnt[b], n), atomicAdd(&S.mass[b], m);
+        }
+        __syncthreads();
+        const double edge = exp(-0.125 * b);
+        int kb = SM_BINS;     /* the bin that top-k ends in */
+        double k_mass = 0.0;  /* and the mass that it keeps of it, in 2^-40 of its lower edge */
+        if (p.top_k) {
+            const uint32_t k = (uint32_t)p.top_k, n = tid < SM_BINS ? S.cnt[tid] : 0;
+            uint32_t n_all;
+            const uint32_t n_to = block_scan(n, S.redu, &n_all);
+            if (n_all > k) {
+                if (n && n_to >= k && n_to - n < k) S.hit = tid, S.sel_n = k - (n_to - n);
+                __syncthreads();
+                kb = S.hit;
+                const uint32_t want = S.sel_n;
+                open_bin(S, ch, l, C, kb);
+                uint32_t above;
+                double unused;
+                cut.key = select_key(S, ch, l, C, kb, p.T, true, want, 0.0, 0, &above, &unused);
+                cut.ties = want - above;
+                unsigned long long kept = 0, whole;
+                for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
+                    int c;
+                    const uint32_t key = S.seg[C] <= SM_LIST ? S.list[i] : member(S, ch, l, C, kb, i, &c);
+                    if (key > cut.key) kept += bin_mass(sample_unkey(key), p.T);
+                }
+                block_scan(kept, S.redk, &whole);
+                k_mass = (double)whole + (double)cut.ties * (double)bin_mass(sample_unkey(cut.key), p.T);
+            }
+        }
+        if (p.top_p < 1.0) { /* over what top-k left */
+            double mine = 0.0, whole;
+            if (tid < SM_BINS) mine = (b < kb ? (double)S.mass[b] : b == kb ? k_mass : 0.0) * edge;
+            const double to = block_scan(mine, S.redd, &whole);
+            const double want = p.top_p * whole;
+            if (tid == 0) S.hit = SM_BINS, S.last = 0;
+            __syncthreads();
+            if (mine > 0.0) {
+                atomicMax(&S.last, tid);
+                if (to >= want) atomicMin(&S.hit, tid);
+            }
+            __syncthreads();
+            const int pb = S.hit < SM_BINS ? S.hit : S.last; /* a whole missed by a rounding */
+            if (tid == pb) S.sel_d = fmax(want - (to - mine), 0.0) / edge;
+            __syncthreads();
+            const double rest = S.sel_d;
+            if (pb != kb) open_bin(S, ch, l, C, pb);
+            uint32_t above;
+            double m_above;
+            const uint32_t key = select_key(S, ch, l, C, pb, p.T, false, 0, rest, pb == kb ? cut.key : 0,
+                                            &above, &m_above);
+            const double need = ceil((rest - m_above) / (double)bin_mass(sample_unkey(key), p.T));
+            uint32_t ties = need < 1.0 ? 1u : need < 4e9 ? (uint32_t)need : 0xffffffffu;
+            if (pb == kb && key == cut.key && cut.ties < ties) ties = cut.ties;
+            cut.key = key, cut.ties = ties;
+        }
+        if (p.min_p > 0.0) {
+            if (tid == 0) S.sel_n = min_p_key(mx, p.T, p.min_p);
+            __syncthreads();
+            if (S.sel_n > cut.key) cut.key = S.sel_n, cut.ties = 0xffffffffu;
+        }
+        /* the kept mass of each chunk: whole bins, then the members of the cut's own bin */
+        const double d = cut.key ? top - floor(grid_pos(sample_unkey(cut.key), p.T)) : (double)SM_BINS;
+        const int cb = d < (double)SM_BINS ? (int)d : SM_BINS;
+        if (cb < SM_BINS) {
+            open_bin(S, ch, l, C, cb);
+            for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
+                int c;
+                const uint32_t key = member(S, ch, l, C, cb, i, &c);
+                if (key == cut.key) atomicAdd(&S.ties[c], 1u);
+                else if (key > cut.key) atomicAdd(&S.cand[c], bin_mass(sample_unkey(key), p.T));
+            }
+        }
+        __syncthreads();
+        uint32_t all;
+        const uint32_t mine = tid < C ? S.ties[tid] : 0, to = block_scan(mine, S.redu, &all), before = to - mine;
+        const uint32_t ties = before >= cut.ties ? 0 : cut.ties - before < mine ? cut.ties - before : mine;
+        if (tid < C) S.ties[tid] = ties;
+        /* a chunk's whole bins: 8 lanes take every 8th, joined in a fixed order */
+        for (int c0 = 0; c0 < C; c0 += SM_T2 / 8) {
+            const int c = c0 + (tid >> 3);
+            double s = 0.0;
+            if (c < C) {
+                const int n = cb - S.off[c];
+                for (int j = tid & 7; j < n; j += 8) s += (double)ch[c].mass[j] * exp(-0.125 * (j + S.off[c]));
+            }
+            s += __shfl_xor(s, 1);
+            s += __shfl_xor(s, 2);
+            s += __shfl_xor(s, 4);
+            if (c < C && (tid & 7) == 0) S.chunk_mass[c] = s;
+        }
+        __syncthreads();
+        if (tid < C) {
+            mass = S.chunk_mass[tid];
+            if (cb < SM_BINS) {
+                double m = (double)S.cand[tid];
+                if (ties) m += (double)ties * (double)bin_mass(sample_unkey(cut.key), p.T);
+                mass += m * exp(-0.125 * cb);
+            }
+            mass *= unit;
+        }
+    }
+    /* the chunk that the draw falls into */
+    double whole;
+    const double to = block_scan(mass, S.redd, &whole), goal = ud * whole;
+    if (tid == 0) S.hit = SM_T2, S.last = 0;
+    __syncthreads();
+    if (mass > 0.0) {
+        atomicMax(&S.last, tid);
+        if (to > goal) atomicMin(&S.hit, tid);
+    }
+    __syncthreads();
+    const int c = S.hit < SM_T2 ? S.hit : S.last;
+    if (tid == c) S.sel_d = to - mass;
+    __syncthreads();
+    const double rest = goal - S.sel_d;
+    /* its logits, 8 consecutive ones to a thread */
+    const int len = vocab - c * SM_CHUNK < SM_CHUNK ? vocab - c * SM_CHUNK : SM_CHUNK, i0 = tid * SM_RUN;
+    const float *lc = l + (size_t)c * SM_CHUNK;
+    float x[SM_RUN];
+    uint32_t key[SM_RUN], same = 0;
+#pragma unroll
+    for (int e = 0; e < SM_RUN; e++) {
+        x[e] = i0 + e < len ? sample_value(lc[i0 + e]) : -INFINITY;
+        key[e] = sample_key(x[e]);
+        same += x[e] > -INFINITY && key[e] == cut.key;
+    }
+    uint32_t rank = 0xffffffffu, allowed = 0xffffffffu;
+    if (p.filter) {
+        uint32_t all;
+        rank = block_scan(same, S.redu, &all) - same;
+        allowed = S.ties[c];
+    }
+    double w[SM_RUN], s = 0.0;
+#pragma unroll
+    for (int e = 0; e < SM_RUN; e++) {
+        bool keep = x[e] > -INFINITY && key[e] >= cut.key;
+        if (p.filter && keep && key[e] == cut.key) keep = rank++ < allowed;
+        w[e] = keep ? exp(((double)x[e] - (double)mx) / p.T) : 0.0;
+        s += w[e];
+    }
+    double in_chunk;
+    double run = block_scan(s, S.redd, &in_chunk) - s;
+    if (tid == 0) S.hit = SM_CHUNK, S.last = 0;
+    __syncthreads();
+    int first = SM_CHUNK, final = -1;
+#pragma unroll
+    for (int e = 0; e < SM_RUN; e++) {
+        run += w[e];
+        if (w[e] > 0.0) {
+            final = i0 + e;
+            if (run > rest && first == SM_CHUNK) first = i0 + e;
+        }
+    }
+    if (final >= 0) {
+        atomicMax(&S.last, final);
+        if (first < SM_CHUNK) atomicMin(&S.hit, first);
+    }
+    __syncthreads();
+    const int at = S.hit < SM_CHUNK ? S.hit : S.last; /* a whole missed by a rounding: the last one */
+    if (at / SM_RUN == tid) {
+        double mine = 0.0;
+#pragma unroll
+        for (int e = 0; e < SM_RUN; e++) mine = e == at % SM_RUN ? w[e] : mine;
+        answer(c * SM_CHUNK + at, mine / whole);
+    }
+}
+
+} // namespace
+
+extern "C" {
+
+size_t nmx_sample_work_bytes(int n, int vocab) {
+    if (n < 1 || n > 4096 || vocab < 1 || vocab > (1 << 20)) return 0;
+    return (size_t)n * ((vocab + SM_CHUNK - 1) / SM_CHUNK) * sizeof(Chunk);
+}
+
+int nmx_sample(nmx_ctx *ctx, const float *logits, int stride, int vocab, int n,
+               const nmx_sample_params *params, int per_row, const float *u, void *work, int32_t *tok,
+               float *prob) {
+    if (!ctx) return -1;
+    if (n < 1 || n > 4096 || vocab < 1 || vocab > (1 << 20) || stride < vocab)
+        return nmx_fail(ctx, "nmx_sample: bad shape n=%d vocab=%d stride=%d", n, vocab, stride);
+    if (!logits || !params || !u || !work || !tok) return nmx_fail(ctx, "nmx_sample: NULL argument");
+    if ((uintptr_t)work % 16) return nmx_fail(ctx, "nmx_sample: work not 16-byte aligned");
+    const int C = (vocab + SM_CHUNK - 1) / SM_CHUNK;
+    const size_t lb = ((size_t)(n - 1) * stride + vocab) * 4, wb = nmx_sample_work_bytes(n, vocab);
+    const size_t pb = sizeof(nmx_sample_params) * (per_row ? (size_t)n : 1), ob = (size_t)n * 4;
+    const void *in[] = {logits, params, u};
+    const size_t ib[] = {lb, pb, ob};
+    for (int i = 0; i < 3; i++)
+        if (nmx_overlap(tok, ob, in[i], ib[i]) || nmx_overlap(work, wb, in[i], ib[i]) ||
+            (prob && nmx_overlap(prob, ob, in[i], ib[i])))
+            return nmx_fail(ctx, "nmx_sample: an output or the workspace overlaps an input");
+    if (nmx_overlap(tok, ob, work, wb) || (prob && (nmx_overlap(prob, ob, work, wb) || nmx_overlap(prob, ob, tok, ob))))
+        return nmx_fail(ctx, "nmx_sample: outputs overlap");
+    const nmx_on_device on(ctx);
+    sample_scan_k<<<dim3((unsigned)C, (unsigned)n), SM_T1, 0, ctx->stream>>>(
+        logits, stride, vocab, (Chunk *)work, params, per_row ? 1 : 0);
+    NMX_LAUNCHED(ctx, "sample_scan");
+    sample_pick_k<<<(unsigned)n, SM_T2, 0, ctx->stream>>>(logits, stride, vocab, C, (const Chunk *)work,
+                                                          params, per_row ? 1 : 0, u, tok, prob);
+    NMX_LAUNCHED(ctx, "sample_pick");
+    return 0;
+}
+
+} /* extern "C" */

@@ -24,6 +24,11 @@ class NmxError(RuntimeError):
     pass
 
 
+# nmx_sample_params: the records that Device.sample reads
+SAMPLE_PARAMS = np.dtype([("temperature", np.float32), ("top_p", np.float32),
+                          ("min_p", np.float32), ("top_k", np.int32)])
+
+
 class LinArgs(ctypes.Structure):
     """Mirror of nmx_lin_args (include/nmx.h)."""
 
@@ -158,6 +163,8 @@ _SIGS: dict[str, tuple[object, list[object]]] = {
     "nmx_attn_fused": (_i, [_vp, ctypes.POINTER(AttnArgs)]),
     "nmx_q4k_swiglu": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, ctypes.POINTER(NormIn),
                             _vp, A8, A8, _vp, _vp]),
+    "nmx_sample_work_bytes": (_sz, [_i, _i]),
+    "nmx_sample": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp]),
     "nmx_top1_gate": (_i, [_vp, _vp, _i, ctypes.c_float, _vp]),
     "nmx_kv_bytes": (_sz, [_i, _i, _i, _i]),
 }
@@ -539,6 +546,16 @@ class Device:
     def host_free(self, p: int) -> None:
         self.check(self.lib.nmx_host_free(self.ctx, p), "host_free")
 
+
+    def sample_work_bytes(self, n: int, vocab: int) -> int:
+        return int(self.lib.nmx_sample_work_bytes(n, vocab))
+
+    def sample(self, logits, stride: int, vocab: int, n: int, params, u, work, tok, prob=None,
+               per_row: bool = True) -> None:
+        """nmx_sample: a token for each of n rows of logits from the uniform numbers u; params: n
+        records of SAMPLE_PARAMS on the device, or one for all rows (per_row False)."""
+        self.check(self.lib.nmx_sample(self.ctx, _p(logits), stride, vocab, n, _p(params),
+                                       int(per_row), _p(u), _p(work), _p(tok), _p(prob)), "sample")
 
     def top1_gate(self, logits, n: int, tau: float, flag) -> None:
         """flag[0] = top-1 softmax probability of logits[0, n) >= tau (nmx_top1_gate)."""

@@ -1,0 +1,228 @@
+"""GPU: nmx_sample against its definition in 64 bits (numpy sort, cumulative sums).
+
+Bar: tokens equal, prob within 4e-7 relative. The token can only differ where the uniform number lies
+within the weights' error (2^-41 of the mass) of a boundary between two tokens, about 1e-8 of the
+draws below; prob is a quotient of weights right to 2^-41 rounded once to 32 bits (2^-24 = 6e-8),
+the reference's quotient is not rounded."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from nibblemac_amd.nmx import SAMPLE_PARAMS, NmxError
+
+CHUNK = 8192  # logits of one workgroup: sizes on both sides of its multiples
+
+
+def reference(l, T, top_k, top_p, min_p, u):
+    """One row: (token, prob)."""
+    l = np.where(np.isnan(l), -np.inf, np.minimum(l.astype(np.float64), np.float64(np.finfo(np.float32).max)))
+    if not (l > -np.inf).any():
+        return -1, 0.0
+    T, top_p, min_p, u = (float(np.float32(x)) for x in (T, top_p, min_p, u))
+    if not T > 0:
+        return int(np.argmax(l)), 1.0
+    order = np.lexsort((np.arange(len(l)), -l))
+    with np.errstate(over="ignore", under="ignore"):
+        w = np.exp((l - l.max()) / T) if T < np.inf else (l > -np.inf).astype(float)
+    if 0 < top_k < len(l):
+        order = order[:top_k]
+    if top_p < 1:
+        reach = np.cumsum(w[order])
+        order = order[:1 + min(np.searchsorted(reach, max(top_p, 0.0) * reach[-1]), len(order) - 1)]
+    if min_p > 0:
+        order = order[w[order] >= min(min_p, 1.0)]
+    order = np.sort(order[w[order] > 0])
+    reach = np.cumsum(w[order])
+    u = u if u > 0 else 0.0
+    i = min(np.searchsorted(reach, u * reach[-1], side="right"), len(order) - 1)
+    return int(order[i]), w[order[i]] / reach[-1]
+
+
+def records(n, T=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    r = np.zeros(n, SAMPLE_PARAMS)
+    r["temperature"], r["top_k"], r["top_p"], r["min_p"] = T, top_k, top_p, min_p
+    return r
+
+
+def sample(dev, logits, par, u, stride=None, times=1):
+    """The device's tokens and probs; the buffers hold 7s before."""
+    n, vocab = logits.shape
+    stride = stride or vocab
+    wide = np.full((n, stride), 1e30, np.float32)
+    wide[:, :vocab] = logits
+    bufs = [dev.to_device(x) for x in (wide, par, u.astype(np.float32), np.full(n + 1, 7, np.int32),
+                                       np.full(n + 1, 7, np.float32))]
+    work = dev.alloc(dev.sample_work_bytes(n, vocab))
+    for _ in range(times):
+        dev.sample(bufs[0], stride, vocab, n, bufs[1], bufs[2], work, bufs[3], prob=bufs[4],
+                   per_row=len(par) > 1 or n == 1)
+    dev.sync()
+    tok, prob = bufs[3].numpy(), bufs[4].numpy()
+    assert tok[n] == 7 and prob[n] == 7
+    for b in (*bufs, work):
+        b.free()
+    return tok[:n], prob[:n]
+
+
+def check(dev, logits, par, u, stride=None):
+    tok, prob = sample(dev, logits, par, u, stride, times=2)
+    for r in range(len(logits)):
+        p = par[r if len(par) > 1 else 0]
+        want = reference(logits[r], p["temperature"], p["top_k"], p["top_p"], p["min_p"], u[r])
+        assert tok[r] == want[0], (r, p, u[r], tok[r], want)
+        assert abs(prob[r] - want[1]) <= 4e-7 * want[1], (r, p, prob[r], want)
+
+
+def rows(rng, n, vocab, spread=2.0, peaks=20):
+    l = (rng.standard_normal((n, vocab)) * spread).astype(np.float32)
+    for r in range(n if peaks else 0):
+        l[r, rng.integers(0, vocab, peaks)] += rng.uniform(3, 12, peaks).astype(np.float32)
+    return l
+
+
+FILTERS = [dict(), dict(top_k=1), dict(top_k=50), dict(top_p=0.9), dict(top_p=0.999), dict(min_p=0.05),
+           dict(top_k=20, top_p=0.8), dict(top_k=3000, top_p=0.99, min_p=0.001), dict(T=0.0),
+           dict(T=0.3, top_p=0.95), dict(T=1.7, top_k=4000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1, 2, 63, 1000, CHUNK - 1, CHUNK, CHUNK + 1, 3 * CHUNK + 17, 248320])
+def test_filters(dev, vocab):
+    print(f"[case] sample filters vocab={vocab}", flush=True)
+    rng = np.random.default_rng(vocab)
+    par = np.concatenate([records(2, **f) for f in FILTERS])
+    u = rng.random(len(par), np.float32)
+    check(dev, rows(rng, len(par), vocab, peaks=min(20, vocab // 4)), par, u, stride=vocab + vocab % 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["equal", "two_values", "quantized", "far_apart", "huge", "zeros_of_both_signs", "steps"])
+def test_ties_and_ranges(dev, kind):
+    """Ties at the borders of every filter, more members in a bin than the list holds, magnitudes at
+    the ends of the type."""
+    print(f"[case] sample {kind}", flush=True)
+    rng = np.random.default_rng(len(kind))
+    par = np.concatenate([records(3, **f) for f in FILTERS + [dict(top_k=9001, top_p=0.5), dict(T=1e-30), dict(T=np.inf),
+                                                             dict(T=1e30, top_k=700), dict(T=1e-3, top_p=0.9)]])
+    n, vocab = len(par), 2 * CHUNK + 300
+    l = np.zeros((n, vocab), np.float32)
+    if kind == "equal":
+        l += 1.5
+    elif kind == "two_values":
+        l[:, ::3] = 0.25
+    elif kind == "quantized":
+        l = np.round(rng.standard_normal((n, vocab)) * 4).astype(np.float32) / 4
+    elif kind == "far_apart":
+        l = (rng.standard_normal((n, vocab)) * 40).astype(np.float32)
+    elif kind == "huge":
+        l = (rng.uniform(-1, 1, (n, vocab)) * 3e38).astype(np.float32)
+        l[:, 5] = l[:, 9000] = 3.4e38
+    elif kind == "zeros_of_both_signs":
+        l = np.where(rng.random((n, vocab)) < 0.5, np.float32(-0.0), np.float32(0.0))
+    else:       # one chunk 20 nats below the other, one 40
+        l = rng.standard_normal((n, vocab)).astype(np.float32)
+        l[:, :CHUNK] -= 20
+        l[:, 2 * CHUNK:] -= 40
+    check(dev, l, par, rng.random(n, np.float32))
+
+
+@pytest.mark.gpu
+def test_masked_values(dev):
+    """-inf, NaN, +inf and the lowest finite value as masks; rows that nothing is left of."""
+    print("[case] sample masks", flush=True)
+    rng = np.random.default_rng(3)
+    vocab = CHUNK + 100
+    for f in (dict(), dict(top_k=5), dict(top_p=0.7), dict(min_p=0.1), dict(T=0.0)):
+        l = rows(rng, 8, vocab)
+        l[0, :CHUNK] = -np.inf
+        l[1, 10:] = -np.inf
+        l[2] = -np.inf
+        l[3] = np.nan
+        l[4, rng.random(vocab) < 0.5] = np.nan
+        l[5, [7, CHUNK + 3]] = np.inf
+        l[6] = np.finfo(np.float32).min
+        l[7, 50:] = np.finfo(np.float32).min
+        check(dev, l, records(8, **f), rng.random(8, np.float32))
+
+
+@pytest.mark.gpu
+def test_uniform_numbers(dev):
+    """u at the ends of its range and outside it; one record for all rows."""
+    print("[case] sample u", flush=True)
+    rng = np.random.default_rng(4)
+    u = np.array([0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, -1.0, np.nan, 2.0 ** -24, 0.5], np.float32)
+    for f in (dict(), dict(top_p=0.9), dict(top_k=40, min_p=0.01)):
+        check(dev, rows(rng, 8, 20000), records(1, **f), u)
+
+
+@pytest.mark.gpu
+def test_parameters_outside_their_range(dev):
+    print("[case] sample odd parameters", flush=True)
+    rng = np.random.default_rng(5)
+    par = np.concatenate([records(1, **f) for f in (
+        dict(T=-1.0), dict(T=np.nan), dict(top_k=-3), dict(top_k=1 << 30), dict(top_p=0.0), dict(top_p=-1.0),
+        dict(top_p=np.nan), dict(top_p=7.0), dict(min_p=-1.0), dict(min_p=np.nan), dict(min_p=1.0), dict(min_p=3.0),
+        dict(top_k=1 << 30, top_p=0.5), dict(min_p=1e-40), dict(top_p=1e-40))])
+    check(dev, rows(rng, len(par), 9000), par, rng.random(len(par), np.float32))
+
+
+@pytest.mark.gpu
+def test_draws_follow_the_weights(dev):
+    """4096 draws of one row: counts within 6 sigma of the weights' shares."""
+    print("[case] sample counts", flush=True)
+    rng = np.random.default_rng(6)
+    l = np.tile(rng.standard_normal(40).astype(np.float32), (4096, 1))
+    u = ((np.arange(4096) + 0.5) / 4096).astype(np.float32)
+    tok, _ = sample(dev, l, records(1, T=0.9), u)
+    w = np.exp(l[0].astype(np.float64) / float(np.float32(0.9)))
+    assert np.abs(np.bincount(tok, minlength=40) - 4096 * w / w.sum()).max() <= 1.0  # u is a grid
+
+
+@pytest.mark.gpu
+def test_captured_call_reads_its_inputs_anew(dev):
+    """One captured call, replayed with other logits, parameters and numbers."""
+    print("[case] sample graph", flush=True)
+    rng = np.random.default_rng(7)
+    n, vocab = 5, 20000
+    bufs = [dev.empty((n, vocab), np.float32), dev.alloc(16 * n), dev.empty(n, np.float32)]
+    tok, prob = dev.empty(n, np.int32), dev.empty(n, np.float32)
+    work = dev.alloc(dev.sample_work_bytes(n, vocab))
+    dev.graph_begin()
+    dev.sample(bufs[0], vocab, vocab, n, bufs[1], bufs[2], work, tok, prob=prob)
+    g = dev.graph_end()
+    for f in (dict(), dict(top_p=0.8), dict(T=0.0), dict(top_k=30, T=0.6), dict()):
+        l, u, par = rows(rng, n, vocab), rng.random(n, np.float32), records(n, **f)
+        for b, x in zip(bufs, (l, par, u)):
+            dev.upload(b, x)
+        dev.graph_launch(g)
+        dev.sync()
+        want_t, want_p = sample(dev, l, par, u)
+        assert np.array_equal(tok.numpy(), want_t) and np.array_equal(prob.numpy(), want_p)
+        check(dev, l, par, u)
+    dev.graph_destroy(g)
+
+
+
+def test_work_bytes_of_refused_shapes():
+    from nibblemac_amd.nmx import load_library
+
+    f = load_library().nmx_sample_work_bytes
+    assert f(0, 100) == f(1, 0) == f(4097, 100) == f(1, (1 << 20) + 1) == f(-1, -1) == 0
+    assert 0 < f(1, 1) == f(1, CHUNK) and f(1, CHUNK + 1) == 2 * f(1, 1) and f(4096, 1 << 20) == 4096 * 128 * f(1, 1)
+
+
+@pytest.mark.gpu
+def test_refusals(dev):
+    print("[case] sample refusals", flush=True)
+    n, vocab = 2, 100
+    l, par, u = dev.zeros((n, vocab), np.float32), dev.zeros(4 * n, np.float32), dev.zeros(n, np.float32)
+    tok, prob, work = dev.zeros(n, np.int32), dev.zeros(n, np.float32), dev.zeros(dev.sample_work_bytes(n, vocab), np.uint8)
+    good = dict(logits=l, stride=vocab, vocab=vocab, n=n, params=par, u=u, work=work, tok=tok, prob=prob)
+    for bad in (dict(n=0), dict(n=4097), dict(vocab=0), dict(vocab=(1 << 20) + 1, stride=1 << 21), dict(stride=99),
+                dict(logits=None), dict(params=None), dict(u=None), dict(work=None), dict(tok=None),
+                dict(work=work.ptr + 8), dict(tok=u), dict(tok=work), dict(prob=tok), dict(prob=l), dict(work=l)):
+        with pytest.raises(NmxError, match="nmx_sample"):
+            dev.sample(**{**good, **bad})
+    dev.sync()
+    assert not tok.numpy().any() and not work.numpy().any()

@@ -449,6 +449,29 @@ int nmx_lin_mix_chunk(nmx_ctx *ctx, const nmx_lin_mix_args *a);
 int nmx_lin_chunk_ok(int dk, int dv, int conv_k, int heads);
 int nmx_attn_fused_chunk(nmx_ctx *ctx, const nmx_attn_args *p, int score_rows);
 
+/* ---- a tree of drafts -----------------------------------------------------------------------
+ * One verify pass over a tree of up to NMX_TREE_MAX tokens instead of a chain: node t's
+ * predecessor is parent[t] < t (device int32 [n], so parents stand before their children), or the
+ * last token of the context where it is -1; any other value is read as -1. Node 0 is the token that
+ * the round starts from. The reference verifies chains only (engine/src/spec.c:303-365). Node t's
+ * cache row is at slot *pos + pos_off + t, its position *pos + pos_off + depth(t); a node whose slot
+ * lies outside the cache has no row (its caller keeps *pos + n <= max_ctx).
+ * Results are right to 32-bit rounding but not equal bit for bit to those of a chain's calls, which
+ * add in the reference's order. */
+#define NMX_TREE_MAX 64
+
+/* nmx_attn_prep for a tree: q and k rows normed, RoPE at the node's position, K and V stored at its
+ * slot (a chain's rows equal nmx_attn_prep's bit for bit). */
+int nmx_attn_tree_prep(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent);
+/* nmx_attn over the context [0, *pos + pos_off) and the node's own ancestors, itself among them;
+ * other nodes' rows are not read. Uses n, nh, nkv, hd, max_ctx, q, scale, kc, vc, pos, pos_off, o, a8
+ * and kv_dtype of p (the others may be zero). hd a multiple of 64 up to 512, nh <= 1024, q and the
+ * caches 16-byte aligned. Cache rows that a node sees hold finite values. work: device scratch of
+ * nmx_attn_tree_work_bytes bytes (0 for a shape that is refused; enough for every kv_dtype and
+ * position), 16-byte aligned, used by one call at a time. */
+size_t nmx_attn_tree_work_bytes(int n, int nh, int nkv, int hd);
+int nmx_attn_tree(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent, void *work);
+
 /* ---- sampling -----------------------------------------------------------------------------
  * A token for each of n rows of logits (row r at logits + r stride, vocab values), from a uniform
  * number per row. The reference decodes greedily only; this stands where a program that samples has

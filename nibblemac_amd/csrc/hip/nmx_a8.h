@@ -29,6 +29,14 @@ __device__ __forceinline__ void nmx_a8_store(float x, int8_t *q, float *d, float
     }
 }
 
+/* ---- A8 of one 32-value block held by a 32-lane half-wave (lane = column within block),
+ * written as the block-major element (b, v) of an [nb][n] layout (nmx_a8.h). */
+__device__ __forceinline__ void a8_block(float x, int b, int v, int n, int8_t *q, float *d,
+                                         float *fs) {
+    const size_t u = (size_t)b * n + v;
+    nmx_a8_store(x, q + u * 32, d + u, fs + u);
+}
+
 /* Two blocks at once (one value of each per lane): both blocks' reductions and divides are
  * computed before any store, so the two dependent chains interleave. */
 __device__ __forceinline__ void nmx_a8_store2(float x1, int8_t *q1, float *d1, float *fs1,

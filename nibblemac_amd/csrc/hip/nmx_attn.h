@@ -77,6 +77,32 @@ __device__ __forceinline__ const float *kv_scales(const void *cache, const nmx_a
                         : nullptr;
 }
 
+/* Store one row element per thread (thread i of the row's hd); the int8 format first reduces
+ * the row's max |x| over the workgroup (hd threads, exact in any order). */
+template <int KVT>
+__device__ __forceinline__ void kv_store(void *cache, const nmx_attn_dev &a, size_t R, int i, float x,
+                                         float *red) {
+    const int hd = a.hd;
+    if constexpr (KVT == KV_F32) {
+        ((float *)cache)[R * hd + i] = x;
+    } else if constexpr (KVT == KV_F16) {
+        ((unsigned short *)cache)[R * hd + i] = (unsigned short)kv_half_bits(x);
+    } else {
+        float m = fabsf(x);
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+        __syncthreads(); /* red free */
+        if ((i & 63) == 0) red[i >> 6] = m;
+        __syncthreads();
+        float amax = 0.0f;
+        for (int w = 0; w < (hd >> 6); w++) amax = fmaxf(amax, red[w]);
+        /* inv stays finite: a row of subnormals codes to zeros like a zero row */
+        const float inv = amax > 127.0f / 3.40282347e+38f ? 127.0f / amax : 0.0f;
+        ((int8_t *)cache)[R * hd + i] = (int8_t)kv_i8_code(x, inv);
+        if (i == 0) ((float *)((int8_t *)cache + (size_t)a.nkv * a.max_ctx * hd))[R] = amax / 127.0f;
+    }
+}
+
 /* Scores, softmax and P.V of a prefill chunk (nmx_attnc.hip), on the queries and caches that
  * attn_prep_k left; sc: [n][nh][max_ctx] workspace (it ends holding the softmax weights).
  * hd a multiple of 64 up to 512. */

@@ -18,45 +18,6 @@
 
 namespace {
 
-/* ---- A8 of one 32-value block held by a 32-lane half-wave (lane = column within block),
- * written as the block-major element (b, v) of an [nb][n] layout (nmx_a8.h). */
-__device__ __forceinline__ void a8_block(float x, int b, int v, int n, int8_t *q, float *d,
-                                         float *fs) {
-    const size_t u = (size_t)b * n + v;
-    nmx_a8_store(x, q + u * 32, d + u, fs + u);
-}
-
-/* Sum in the reference's order (sumsq forward_ops.c:168-189, pf_softmax_exp :333-353):
- * partial l accumulates v[4m + l] for m ascending over the first cols/4*4 elements;
- * s = (c0 + c1) + (c2 + c3); the tail sequentially into t; result s + t. v[] is in LDS in
- * element order; four lanes run the four chains, reading 16 values per batch so the LDS
- * latency overlaps the dependent adds. Every thread of the block gets the result. */
-__device__ float ordered_sum4(const float *sq, int cols, float *red) {
-    const int tid = threadIdx.x, m4 = cols >> 2;
-    if (tid < 4) {
-        float c = 0.0f;
-        int m = 0;
-        for (; m + 16 <= m4; m += 16) {
-            float b[16];
-#pragma unroll
-            for (int u = 0; u < 16; u++) b[u] = sq[4 * (m + u) + tid];
-#pragma unroll
-            for (int u = 0; u < 16; u++) c = c + b[u];
-        }
-        for (; m < m4; m++) c = c + sq[4 * m + tid];
-        red[tid] = c;
-    } else if (tid == 4) {
-        float t = 0.0f;
-        for (int i = m4 * 4; i < cols; i++) t = t + sq[i];
-        red[4] = t;
-    }
-    __syncthreads();
-    const float s = (red[0] + red[1]) + (red[2] + red[3]);
-    const float r = s + red[4];
-    __syncthreads();
-    return r;
-}
-
 /* ---- embedding rows of a Q4K matrix (engine/src/kern_act.c:53-88) ---- */
 __global__ __launch_bounds__(256) void embed_k(const uint8_t *__restrict__ W, int cols,
                                                const int32_t *__restrict__ tok,
@@ -375,32 +336,6 @@ __global__ __launch_bounds__(256) void silu_mul_k(const float *__restrict__ gate
  * RoPE, K and V rows stored at position pos + t; every query head: RMSNorm + RoPE in place.
  * RoPE (forward_ops.c:149-165): pairs (i, i + rot/2), v_i = a c - b s, v_{i+h} = b c + a s. */
 using Attn = nmx_attn_dev;
-
-/* Store one row element per thread (thread i of the row's hd); the int8 format first reduces
- * the row's max |x| over the workgroup (hd threads, exact in any order). */
-template <int KVT>
-__device__ __forceinline__ void kv_store(void *cache, const Attn &a, size_t R, int i, float x,
-                                         float *red) {
-    const int hd = a.hd;
-    if constexpr (KVT == KV_F32) {
-        ((float *)cache)[R * hd + i] = x;
-    } else if constexpr (KVT == KV_F16) {
-        ((unsigned short *)cache)[R * hd + i] = (unsigned short)kv_half_bits(x);
-    } else {
-        float m = fabsf(x);
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-        __syncthreads(); /* red free */
-        if ((i & 63) == 0) red[i >> 6] = m;
-        __syncthreads();
-        float amax = 0.0f;
-        for (int w = 0; w < (hd >> 6); w++) amax = fmaxf(amax, red[w]);
-        /* inv stays finite: a row of subnormals codes to zeros like a zero row */
-        const float inv = amax > 127.0f / 3.40282347e+38f ? 127.0f / amax : 0.0f;
-        ((int8_t *)cache)[R * hd + i] = (int8_t)kv_i8_code(x, inv);
-        if (i == 0) ((float *)((int8_t *)cache + (size_t)a.nkv * a.max_ctx * hd))[R] = amax / 127.0f;
-    }
-}
 
 template <int KVT>
 __global__ __launch_bounds__(512) void attn_prep_k(Attn a) {

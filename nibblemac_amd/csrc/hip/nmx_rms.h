@@ -11,6 +11,37 @@
 #include "nmx_math.h"
 #include "nmx_lanes.h"
 
+/* Sum in the reference's order (sumsq forward_ops.c:168-189, pf_softmax_exp :333-353):
+ * partial l accumulates v[4m + l] for m ascending over the first cols/4*4 elements;
+ * s = (c0 + c1) + (c2 + c3); the tail sequentially into t; result s + t. v[] is in LDS in
+ * element order; four lanes run the four chains, reading 16 values per batch so the LDS
+ * latency overlaps the dependent adds. Every thread of the block gets the result. */
+__device__ inline float ordered_sum4(const float *sq, int cols, float *red) {
+    const int tid = threadIdx.x, m4 = cols >> 2;
+    if (tid < 4) {
+        float c = 0.0f;
+        int m = 0;
+        for (; m + 16 <= m4; m += 16) {
+            float b[16];
+#pragma unroll
+            for (int u = 0; u < 16; u++) b[u] = sq[4 * (m + u) + tid];
+#pragma unroll
+            for (int u = 0; u < 16; u++) c = c + b[u];
+        }
+        for (; m < m4; m++) c = c + sq[4 * m + tid];
+        red[tid] = c;
+    } else if (tid == 4) {
+        float t = 0.0f;
+        for (int i = m4 * 4; i < cols; i++) t = t + sq[i];
+        red[4] = t;
+    }
+    __syncthreads();
+    const float s = (red[0] + red[1]) + (red[2] + red[3]);
+    const float r = s + red[4];
+    __syncthreads();
+    return r;
+}
+
 /* The same sum over values stored chain-major: chain l's m-th value at cm[l * s4 + m]
  * (s4 a multiple of 4, so a chain is read as float4), the cols % 4 tail at cm[4 * s4 + k].
  * Two register sets of 32 values take turns: the next set is requested before the current

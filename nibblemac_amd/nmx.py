@@ -163,6 +163,9 @@ _SIGS: dict[str, tuple[object, list[object]]] = {
     "nmx_attn_fused": (_i, [_vp, ctypes.POINTER(AttnArgs)]),
     "nmx_q4k_swiglu": (_i, [_vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, ctypes.POINTER(NormIn),
                             _vp, A8, A8, _vp, _vp]),
+    "nmx_attn_tree_prep": (_i, [_vp, ctypes.POINTER(AttnArgs), _vp]),
+    "nmx_attn_tree_work_bytes": (_sz, [_i, _i, _i, _i]),
+    "nmx_attn_tree": (_i, [_vp, ctypes.POINTER(AttnArgs), _vp, _vp]),
     "nmx_sample_work_bytes": (_sz, [_i, _i]),
     "nmx_sample": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp]),
     "nmx_top1_gate": (_i, [_vp, _vp, _i, ctypes.c_float, _vp]),
@@ -457,6 +460,19 @@ class Device:
     def attn_fused(self, args: "AttnArgs") -> None:
         """nmx_attn_fused: nmx_attn_prep + nmx_attn in two launches."""
         self.check(self.lib.nmx_attn_fused(self.ctx, ctypes.byref(args)), "attn_fused")
+
+    def attn_tree_prep(self, args: "AttnArgs", parent) -> None:
+        """nmx_attn_tree_prep: attn_prep for the nodes of a tree (parent: device int32 [n])."""
+        self.check(self.lib.nmx_attn_tree_prep(self.ctx, ctypes.byref(args), _p(parent)),
+                   "attn_tree_prep")
+
+    def attn_tree_work_bytes(self, n: int, nh: int, nkv: int, hd: int) -> int:
+        return int(self.lib.nmx_attn_tree_work_bytes(n, nh, nkv, hd))
+
+    def attn_tree(self, args: "AttnArgs", parent, work) -> None:
+        """nmx_attn_tree: attention of a tree's nodes over the context and their ancestors."""
+        self.check(self.lib.nmx_attn_tree(self.ctx, ctypes.byref(args), _p(parent), _p(work)),
+                   "attn_tree")
 
     def lin_mix(self, args: "LinMixArgs") -> None:
         self.check(self.lib.nmx_lin_mix(self.ctx, ctypes.byref(args)), "lin_mix")

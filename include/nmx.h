@@ -472,6 +472,49 @@ int nmx_attn_tree_prep(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *pare
 size_t nmx_attn_tree_work_bytes(int n, int nh, int nkv, int hd);
 int nmx_attn_tree(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent, void *work);
 
+/* nmx_lin_mix for a tree: the conv window of node t is the node, its ancestors and then the state's
+ * rows; its recurrence starts from its parent's state. S advances by the keep pending rows only (as
+ * nmx_lin_apply) and the conv state not at all; log rows k | delta | decay [n][heads][dk + dv + 1] of
+ * every node are written (rule.log is required, log0 not used), and, when pre.xin is not NULL, the raw
+ * inputs [n][C] of every node: what nmx_tree_commit takes the accepted branch from. The intermediate
+ * buffers pre.out (16-byte aligned), pre.beta, pre.decay and rule.o are written; rule.qkv,
+ * rule.decay and rule.beta are not used. dk in {32, 64, 128, 256}, dv a multiple of 32 up to 512, any rep.
+ * The pend and conv rows, the state and the nodes above a node hold finite values; other branches may
+ * hold anything. */
+int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *a, const int32_t *parent);
+
+/* The end of a tree round: from node 0 on, the child whose token tok[child] equals the choice made
+ * after its parent (choice[node]: the argmax of nmx_head_accept, or the token of nmx_sample, at the
+ * node's logits) is accepted, the first one of several; a negative choice accepts none. With
+ * e >= 1 nodes on that path (node 0 among them):
+ *   out [2 + n]: e - 1 (accepted drafts), the choice after the last node (the next round's node 0),
+ *     the path's nodes, -1 behind them; ctl (may be NULL): ctl[1] = ctl[2] = e, ctl[0] as it is
+ *     (nmx_ctl_advance adds e to it); vt (may be NULL, may be tok): vt[0] = that choice;
+ *   layers (0: none) DeltaNet layers, arrays as in nmx_commit_args: state becomes the last
+ *     conv_k - 1 rows of [state; the path's xin rows], pend rows 0 .. e - 1 the path's log rows (the
+ *     keep = e rows of the next nmx_lin_mix_tree; rows behind them are left as they were);
+ *   caches (0: none) KV caches, host array of device pointers: the path's rows move to the slots
+ *     *pos + pos_off + i, i < e (nodes without a slot are left out).
+ * The path ends equal what a chain of its tokens would have left, as far as the rows themselves do. */
+#define NMX_TREE_KV_MAX 64
+typedef struct {
+    int n;
+    const int32_t *parent, *tok, *choice; /* [n] each */
+    int32_t *out, *ctl, *vt;
+    int layers, C, conv_k;
+    float *state;          /* [layers][conv_k-1][C] */
+    const float *xin;      /* [layers][cap][C] */
+    const float *log;      /* [layers][cap][row] */
+    float *pend;           /* [layers][cap][row] */
+    int cap, row;
+    int caches;
+    void *const *kv;       /* [caches]: nmx_kv_bytes(kv_dtype, nkv, max_ctx, hd) each, read by the call */
+    int nkv, max_ctx, hd, kv_dtype;
+    const int32_t *pos;
+    int pos_off;
+} nmx_tree_commit_args;
+int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p);
+
 /* ---- sampling -----------------------------------------------------------------------------
  * A token for each of n rows of logits (row r at logits + r stride, vocab values), from a uniform
  * number per row. The reference decodes greedily only; this stands where a program that samples has

@@ -1,0 +1,183 @@
+/* The commit of a verified tree (include/nmx.h nmx_tree_commit): the walk from the root along the
+ * drafts that were chosen, and the move of what it accepted to where a chain's pass would have left
+ * it. One launch: every workgroup redoes the walk (64 nodes: six shuffles and a ballot), so no second
+ * launch waits for it; the rest is a copy of a few rows, bound by the round trip to memory. */
+#include "nmx_internal.h"
+#include "nmx_lanes.h"
+#include "nmx_tree.h"
+
+namespace {
+
+struct Commit {
+    int n;
+    const int32_t *parent, *tok, *choice;
+    int32_t *out, *ctl, *vt;
+    int layers, C, S; /* S = conv_k - 1 rows of conv state */
+    float *state;
+    const float *xin, *log;
+    float *pend;
+    int cap, row;
+    int caches, nkv, max_ctx, row_bytes, scales;
+    const int32_t *pos;
+    int pos_off;
+    size_t scale_at; /* bytes from a cache's start to its row scales */
+    int conv_wgs, log_wgs, kv_wgs; /* workgroups of one layer's conv state, of its log rows, of one
+                                    * cache's head */
+    void *kv[NMX_TREE_KV_MAX];
+};
+
+/* The accepted path: path[i] for i < the result (path[0] = 0), known to every thread. */
+__device__ int walk(const Commit &a, int *path, int *bonus) {
+    __shared__ int s_e, s_bonus;
+    if (threadIdx.x < 64) {
+        const int lane = threadIdx.x;
+        int p;
+        const unsigned long long set = tree_ancestors(a.parent, a.n, &p);
+        const int tok = lane < a.n ? a.tok[lane] : -1, ch = lane < a.n ? a.choice[lane] : -1;
+        const int want = __shfl(ch, p < 0 ? 0 : p);
+        bool hit = lane < a.n && p >= 0 && want >= 0 && tok == want;
+        /* of several children with the chosen token the first counts */
+        for (unsigned long long m = __ballot(hit); m; m &= m - 1) {
+            const int k = __ffsll((long long)m) - 1;
+            if (__shfl(p, k) == p && k < lane) hit = false;
+        }
+        const unsigned long long good = __ballot(hit || lane == 0);
+        const bool on = lane < a.n && (set & 1) && !(set & ~good);
+        const unsigned long long chain = __ballot(on);
+        if (on) path[__popcll(chain & ((1ull << lane) - 1))] = lane;
+        const int last = 63 - __clzll((long long)chain);
+        const int b = __shfl(ch, last);
+        if (lane == 0) s_e = __popcll(chain), s_bonus = b;
+    }
+    __syncthreads();
+    *bonus = s_bonus;
+    return s_e;
+}
+
+__global__ __launch_bounds__(256) void tree_commit_k(Commit a) {
+    __shared__ int path[NMX_TREE_MAX];
+    int bonus;
+    const int e = walk(a, path, &bonus), tid = threadIdx.x;
+    int b = blockIdx.x;
+    if (b == 0) {
+        if (tid < a.n) a.out[2 + tid] = tid < e ? path[tid] : -1;
+        if (tid == 0) {
+            a.out[0] = e - 1;
+            a.out[1] = bonus;
+            if (a.ctl) a.ctl[1] = e, a.ctl[2] = e;
+            if (a.vt) a.vt[0] = bonus;
+        }
+        return;
+    }
+    b--;
+    if (b < a.layers * a.conv_wgs) { /* conv state: the last S of [state; raw inputs of the path] */
+        const int l = b / a.conv_wgs, c = b % a.conv_wgs * 256 + tid;
+        if (c >= a.C) return;
+        float *st = a.state + (size_t)l * a.S * a.C + c;
+        const float *xi = a.xin + (size_t)l * a.cap * a.C + c;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (j >= a.S) continue;
+            const int r = j + e;
+            v[j] = r < a.S ? st[(size_t)r * a.C] : xi[(size_t)path[r - a.S] * a.C];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (j < a.S) st[(size_t)j * a.C] = v[j];
+        return;
+    }
+    b -= a.layers * a.conv_wgs;
+    if (b < a.layers * a.log_wgs) { /* pending rows: the path's log rows */
+        const int l = b / a.log_wgs, w = b % a.log_wgs;
+        const float *lg = a.log + (size_t)l * a.cap * a.row;
+        float *pd = a.pend + (size_t)l * a.cap * a.row;
+        for (int x = w * 256 + tid; x < e * a.row; x += a.log_wgs * 256) {
+            const int i = x / a.row, k = x - i * a.row;
+            pd[x] = lg[(size_t)path[i] * a.row + k];
+        }
+        return;
+    }
+    b -= a.layers * a.log_wgs;
+    /* cache rows to consecutive slots. path[i] >= i and grows, so a thread that takes its own bytes of
+     * the rows in order reads each row before it writes one at or behind it. */
+    const int cache = b / (a.nkv * a.kv_wgs), g = b / a.kv_wgs % a.nkv, w = b % a.kv_wgs;
+    const long long p = (long long)*a.pos + a.pos_off;
+    const int words = a.row_bytes / 4 + (a.scales ? 1 : 0), x = w * 256 + tid;
+    if (x >= words) return;
+    char *c = (char *)a.kv[cache];
+    char *base;
+    size_t step;
+    if (x < a.row_bytes / 4) base = c + (size_t)g * a.max_ctx * a.row_bytes + 4 * x, step = a.row_bytes;
+    else base = c + a.scale_at + (size_t)g * a.max_ctx * 4, step = 4;
+    for (int i = 1; i < e; i++) {
+        const long long from = p + path[i], to = p + i;
+        if (from == to || to < 0 || from >= a.max_ctx) continue;
+        *(uint32_t *)(base + (size_t)to * step) = *(const uint32_t *)(base + (size_t)from * step);
+    }
+}
+
+} // namespace
+
+extern "C" {
+
+int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p) {
+    if (!ctx) return -1;
+    if (!p) return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
+    if (p->n < 1 || p->n > NMX_TREE_MAX) return nmx_fail(ctx, "nmx_tree_commit: n=%d", p->n);
+    if (!p->parent || !p->tok || !p->choice || !p->out) return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
+    const size_t nb = (size_t)p->n * 4, ob = nb + 8;
+    if (nmx_overlap(p->out, ob, p->parent, nb) || nmx_overlap(p->out, ob, p->tok, nb) || nmx_overlap(p->out, ob, p->choice, nb) ||
+        (p->ctl && (nmx_overlap(p->out, ob, p->ctl, 12) || nmx_overlap(p->ctl + 1, 8, p->parent, nb) ||
+                    nmx_overlap(p->ctl + 1, 8, p->tok, nb) || nmx_overlap(p->ctl + 1, 8, p->choice, nb))) ||
+        (p->vt && (nmx_overlap(p->out, ob, p->vt, 4) || nmx_overlap(p->vt, 4, p->parent, nb) ||
+                   nmx_overlap(p->vt, 4, p->choice, nb) || (p->vt != p->tok && nmx_overlap(p->vt, 4, p->tok, nb)))))
+        return nmx_fail(ctx, "nmx_tree_commit: out, ctl, vt and the tree overlap");
+    Commit a{};
+    a.n = p->n, a.parent = p->parent, a.tok = p->tok, a.choice = p->choice;
+    a.out = p->out, a.ctl = p->ctl, a.vt = p->vt;
+    if (p->layers) {
+        if (p->layers < 0 || p->layers > 1024 || p->C < 1 || p->C > (1 << 20) || p->conv_k < 1 || p->conv_k > 8 ||
+            p->cap < p->n || p->cap > 4096 || p->row < 1 || p->row > (1 << 24))
+            return nmx_fail(ctx, "nmx_tree_commit: bad shape layers=%d C=%d conv_k=%d cap=%d row=%d", p->layers, p->C,
+                            p->conv_k, p->cap, p->row);
+        if (!p->log || !p->pend || (p->conv_k > 1 && (!p->state || !p->xin)))
+            return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
+        const size_t lb = (size_t)p->layers * p->cap * p->row * 4, xb = (size_t)p->layers * p->cap * p->C * 4,
+                     sb = (size_t)p->layers * (p->conv_k - 1) * p->C * 4;
+        if (nmx_overlap(p->log, lb, p->pend, lb) || nmx_overlap(p->state, sb, p->xin, xb) ||
+            nmx_overlap(p->state, sb, p->pend, lb) || nmx_overlap(p->state, sb, p->log, lb) ||
+            nmx_overlap(p->pend, lb, p->xin, xb))
+            return nmx_fail(ctx, "nmx_tree_commit: the layers' arrays overlap");
+        a.layers = p->layers, a.C = p->C, a.S = p->conv_k - 1;
+        a.state = p->state, a.xin = p->xin, a.log = p->log, a.pend = p->pend, a.cap = p->cap, a.row = p->row;
+        a.conv_wgs = a.S ? (p->C + 255) / 256 : 0;
+        a.log_wgs = (p->row + 1023) / 1024;
+    }
+    if (p->caches) {
+        if (p->caches < 0 || p->caches > NMX_TREE_KV_MAX || p->nkv < 1 || p->nkv > 1024 || p->max_ctx < 1 ||
+            p->max_ctx > (1 << 20) || p->hd < 64 || p->hd > 512 || p->hd % 64 || p->kv_dtype < 0 || p->kv_dtype > 2)
+            return nmx_fail(ctx, "nmx_tree_commit: bad caches %d nkv=%d max_ctx=%d hd=%d kv_dtype=%d", p->caches, p->nkv,
+                            p->max_ctx, p->hd, p->kv_dtype);
+        if (!p->kv || !p->pos) return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
+        const size_t kb = nmx_kv_bytes(p->kv_dtype, p->nkv, p->max_ctx, p->hd);
+        for (int i = 0; i < p->caches; i++) {
+            if (!p->kv[i] || (uintptr_t)p->kv[i] % 4) return nmx_fail(ctx, "nmx_tree_commit: cache %d", i);
+            for (int k = 0; k < i; k++)
+                if (nmx_overlap(p->kv[i], kb, p->kv[k], kb)) return nmx_fail(ctx, "nmx_tree_commit: caches overlap");
+            a.kv[i] = p->kv[i];
+        }
+        a.caches = p->caches, a.nkv = p->nkv, a.max_ctx = p->max_ctx, a.pos = p->pos, a.pos_off = p->pos_off;
+        a.row_bytes = p->hd * (p->kv_dtype == 0 ? 4 : p->kv_dtype == 1 ? 2 : 1);
+        a.scales = p->kv_dtype == 2;
+        a.scale_at = (size_t)p->nkv * p->max_ctx * p->hd;
+        a.kv_wgs = (a.row_bytes / 4 + a.scales + 255) / 256;
+    }
+    const nmx_on_device on(ctx);
+    const size_t wgs = 1 + (size_t)a.layers * (a.conv_wgs + a.log_wgs) + (size_t)a.caches * a.nkv * a.kv_wgs;
+    tree_commit_k<<<(unsigned)wgs, 256, 0, ctx->stream>>>(a);
+    NMX_LAUNCHED(ctx, "tree_commit");
+    return 0;
+}
+
+} /* extern "C" */

@@ -94,6 +94,34 @@ class AttnArgs(ctypes.Structure):
                 ("o", _vp), ("a8", A8), ("scores", _vp), ("kv_dtype", _i)]
 
 
+class TreeCommitArgs(ctypes.Structure):
+    """Mirror of nmx_tree_commit_args (the commit of a verified tree)."""
+
+    _fields_ = [("n", _i), ("parent", _vp), ("tok", _vp), ("choice", _vp), ("out", _vp),
+                ("ctl", _vp), ("vt", _vp), ("layers", _i), ("C", _i), ("conv_k", _i),
+                ("state", _vp), ("xin", _vp), ("log", _vp), ("pend", _vp), ("cap", _i),
+                ("row", _i), ("caches", _i), ("kv", _vp), ("nkv", _i), ("max_ctx", _i),
+                ("hd", _i), ("kv_dtype", _i), ("pos", _vp), ("pos_off", _i)]
+
+
+def tree_commit_args(n: int, parent, tok, choice, out, *, ctl=None, vt=None, lin: dict | None = None,
+                     kv: dict | None = None) -> TreeCommitArgs:
+    """The arguments of Device.tree_commit. lin: layers, C, conv_k, state, xin, log, pend, cap, row;
+    kv: caches (device pointers), nkv, max_ctx, hd, kv_dtype, pos and, if not 0, pos_off."""
+    a = TreeCommitArgs(n=n, parent=_p(parent), tok=_p(tok), choice=_p(choice), out=_p(out),
+                       ctl=_p(ctl), vt=_p(vt))
+    for k, v in (lin or {}).items():
+        setattr(a, k, _p(v) if k in ("state", "xin", "log", "pend") else v)
+    for k, v in (kv or {}).items():
+        if k == "caches":
+            ptrs = (ctypes.c_void_p * max(1, len(v)))(*[_p(x) for x in v])
+            a.caches, a.kv = len(v), ctypes.addressof(ptrs)
+            a.keep_kv = ptrs  # the array lives as long as the arguments
+        else:
+            setattr(a, k, _p(v) if k == "pos" else v)
+    return a
+
+
 _SIGS: dict[str, tuple[object, list[object]]] = {
     "nmx_create": (_vp, [_i]),
     "nmx_create_error": (ctypes.c_char_p, []),
@@ -166,6 +194,8 @@ _SIGS: dict[str, tuple[object, list[object]]] = {
     "nmx_attn_tree_prep": (_i, [_vp, ctypes.POINTER(AttnArgs), _vp]),
     "nmx_attn_tree_work_bytes": (_sz, [_i, _i, _i, _i]),
     "nmx_attn_tree": (_i, [_vp, ctypes.POINTER(AttnArgs), _vp, _vp]),
+    "nmx_lin_mix_tree": (_i, [_vp, ctypes.POINTER(LinMixArgs), _vp]),
+    "nmx_tree_commit": (_i, [_vp, ctypes.POINTER(TreeCommitArgs)]),
     "nmx_sample_work_bytes": (_sz, [_i, _i]),
     "nmx_sample": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp]),
     "nmx_top1_gate": (_i, [_vp, _vp, _i, ctypes.c_float, _vp]),
@@ -476,6 +506,15 @@ class Device:
 
     def lin_mix(self, args: "LinMixArgs") -> None:
         self.check(self.lib.nmx_lin_mix(self.ctx, ctypes.byref(args)), "lin_mix")
+
+    def lin_mix_tree(self, args: "LinMixArgs", parent) -> None:
+        """nmx_lin_mix_tree: the DeltaNet mixer over a tree's nodes (parent: device int32 [n])."""
+        self.check(self.lib.nmx_lin_mix_tree(self.ctx, ctypes.byref(args), _p(parent)),
+                   "lin_mix_tree")
+
+    def tree_commit(self, args: "TreeCommitArgs") -> None:
+        """nmx_tree_commit: the accepted branch of a tree and the move of its rows."""
+        self.check(self.lib.nmx_tree_commit(self.ctx, ctypes.byref(args)), "tree_commit")
 
     def lin_apply(self, S, log, keep: int, heads: int, dk: int, dv: int) -> None:
         self.check(self.lib.nmx_lin_apply(self.ctx, _p(S), _p(log), keep, heads, dk, dv),

@@ -41,8 +41,8 @@ struct TreeAttn {
     int pos_off;
     float scale;
     float *part;   /* [splits][n nh][hd] weighted values, 2^12 high */
-    float4 *stat;  /* [splits][n nh]: maximum of the scores, of scores + value exponent (columns
-                    * below 256), sum, maximum of scores + value exponent (columns from 256) */
+    float4 *stat;  /* [splits][n nh]: maximum of the scores, the values' exponent (columns below 256),
+                    * sum, the values' exponent (columns from 256) */
     int splits, unit; /* a part is a whole number of units of positions */
     float *o;
     int8_t *aq;
@@ -72,6 +72,12 @@ __device__ __forceinline__ int row_exp(float amax) {
 __device__ __forceinline__ float pow2f(int e) { /* -149 < e < 128 */
     return e > -127 ? __uint_as_float((uint32_t)(e + 127) << 23) : ldexpf(1.0f, e);
 }
+
+/* lane and wave as the hardware knows them: no register kept for them, the wave's in a scalar */
+__device__ __forceinline__ int lane_id() {
+    return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+}
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
 __device__ __forceinline__ float4v mfma16(half8 a, half8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -119,309 +125,575 @@ __global__ __launch_bounds__(512) void attn_tree_prep_k(nmx_attn_dev a, const in
     }
 }
 
-/* ---- the context ------------------------------------------------------------------------ */
+/* ---- the context ------------------------------------------------------------------------
+ * Scores are made transposed (positions x rows: keys are the first matrix operand, the query rows the
+ * second), so a lane holds its own row's weights of 8 positions in exactly the order in which the
+ * second product (values transposed x weights) wants its second operand: nothing moves between
+ * lanes, and a row's running maximum, sum and rescale are its lane's own. */
 
-/* A tile of PT positions in LDS: HDP binary16 values per position (a second plane of low parts for
- * fp32 caches), 16-byte chunks moved by an XOR so that the matrix operands' reads (16 positions of
- * one chunk for the keys, 4 positions of two chunks for the values) meet no bank twice; columns past
- * hd and positions past the part hold zeros. */
-template <int HDP>
+/* A row's 16-byte chunks of binary16 in LDS, moved by an XOR so that the operands' reads (16
+ * positions of one chunk for the keys, 4 positions of two chunks for the values) meet no bank twice. */
+template <int W>
 __device__ __forceinline__ int k_at(int p, int chunk) {
-    return p * HDP + ((chunk ^ (p & 7)) << 3);
+    return p * W + ((chunk ^ (p & 7)) << 3);
 }
-template <int HDP>
+template <int W>
 __device__ __forceinline__ int v_at(int p, int chunk) {
-    return p * HDP + ((chunk ^ ((p & 3) << 1)) << 3);
+    return p * W + ((chunk ^ ((p & 3) << 1)) << 3);
 }
 
-/* 8 values of row R, columns col .. col + 7, as floats (int8: the codes) */
+/* 8 values of a cache row as they lie in it */
 template <int KVT>
-__device__ __forceinline__ void load8(const void *cache, size_t R, int hd, int col, uint4 (&raw)[2]) {
+struct Raw8 {
+    uint4 a, b;
+};
+template <>
+struct Raw8<KV_F16> {
+    uint4 a;
+};
+template <>
+struct Raw8<KV_I8> {
+    uint2 a;
+};
+
+template <int KVT>
+__device__ __forceinline__ Raw8<KVT> load8(const void *cache, size_t R, int hd, int col) {
+    Raw8<KVT> r;
     if constexpr (KVT == KV_F32) {
         const uint4 *s = (const uint4 *)((const float *)cache + R * hd + col);
-        raw[0] = s[0], raw[1] = s[1];
+        r.a = s[0], r.b = s[1];
     } else if constexpr (KVT == KV_F16) {
-        raw[0] = *(const uint4 *)((const unsigned short *)cache + R * hd + col);
+        r.a = *(const uint4 *)((const unsigned short *)cache + R * hd + col);
     } else {
-        const uint2 w = *(const uint2 *)((const int8_t *)cache + R * hd + col);
-        raw[0].x = w.x, raw[0].y = w.y;
+        r.a = *(const uint2 *)((const int8_t *)cache + R * hd + col);
+    }
+    return r;
+}
+template <int KVT>
+__device__ __forceinline__ float scale_of(const TreeAttn &a, const void *cache, size_t R) {
+    if constexpr (KVT == KV_I8) return ((const float *)((const int8_t *)cache + (size_t)a.nkv * a.max_ctx * a.hd))[R];
+    return 1.0f;
+}
+__device__ __forceinline__ half8 codes8(uint2 w) {
+    half8 h;
+#pragma unroll
+    for (int i = 0; i < 8; i++) h[i] = (_Float16)(float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+    return h;
+}
+__device__ __forceinline__ void floats8(const Raw8<KV_F32> &r, float (&x)[8]) {
+    x[0] = __uint_as_float(r.a.x), x[1] = __uint_as_float(r.a.y), x[2] = __uint_as_float(r.a.z), x[3] = __uint_as_float(r.a.w);
+    x[4] = __uint_as_float(r.b.x), x[5] = __uint_as_float(r.b.y), x[6] = __uint_as_float(r.b.z), x[7] = __uint_as_float(r.b.w);
+}
+__device__ __forceinline__ float amax8(const Raw8<KV_F32> &r) {
+    float x[8];
+    floats8(r, x);
+    return fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))),
+                 fmaxf(fmaxf(fabsf(x[4]), fabsf(x[5])), fmaxf(fabsf(x[6]), fabsf(x[7]))));
+}
+/* x up as a binary16 and the binary16 rest */
+__device__ __forceinline__ void split8(const float (&x)[8], float up, half8 &h, half8 &r) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float v = x[i] * up;
+        h[i] = (_Float16)v;
+        r[i] = (_Float16)(v - (float)h[i]);
     }
 }
 
-/* Rows pt .. pt + PT - 1 of a cache (zeros from row p1 on), columns c0 .. c0 + W - 1, into a tile.
- * Keys: aux0 the factor of a row's scores. Values: aux0, aux1 exponent and fraction of a row's factor.
- * W / 8 lanes stage a row, 8 columns each. */
-template <int W, int KVT, int PT, bool VALUES>
-__device__ __forceinline__ void stage(const TreeAttn &a, size_t R0, int pt, int p1, int c0, _Float16 *dst,
-                                      float *aux0, float *aux1) {
-    constexpr int CH = W / 8, TURNS = PT * CH / 256, BATCH = TURNS < 8 ? TURNS : 8;
-    static_assert(PT * CH % 256 == 0, "whole turns");
-    const void *cache = VALUES ? a.vc : a.kc;
-    const int tid = threadIdx.x, hd = a.hd;
-    for (int t0 = 0; t0 < TURNS; t0 += BATCH) {
-        uint4 raw[BATCH][2];
-        float sc[BATCH];
+/* Lane c of 16 (quarter gq) takes its query row's chunks 4 k + gq, split; the result is the factor that
+ * turns a product of parts into a score in powers of two. Columns past hd are zeros. */
+template <int KS>
+__device__ __forceinline__ float load_q(const float *qp, bool live, int hd, int gq, float scale, half8 (&qh)[KS], half8 (&ql)[KS]) {
+    constexpr int HELD = KS <= 4 ? KS : 1; /* a longer row is read again instead of held */
+    float4 x[HELD][2];
+    auto get = [&](int k, float4 (&y)[2]) {
+        const int col = k * 32 + gq * 8;
+        y[0] = y[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (live && col < hd) y[0] = *(const float4 *)(qp + col), y[1] = *(const float4 *)(qp + col + 4);
+    };
+    float am = 0.0f;
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int f = (t0 + u) * 256 + tid, p = f / CH, col = c0 + f % CH * 8;
-            raw[u][0] = raw[u][1] = uint4{0, 0, 0, 0};
-            sc[u] = 0.0f;
-            if (pt + p < p1 && col < hd) load8<KVT>(cache, R0 + pt + p, hd, col, raw[u]);
-            if constexpr (KVT == KV_I8)
-                if (pt + p < p1)
-                    sc[u] = ((const float *)((const int8_t *)cache + (size_t)a.nkv * a.max_ctx * hd))[R0 + pt + p];
-        }
+    for (int k = 0; k < KS; k++) {
+        float4(&y)[2] = x[k % HELD];
+        get(k, y);
+        am = fmaxf(am, fmaxf(fmaxf(fabsf(y[0].x), fabsf(y[0].y)), fmaxf(fabsf(y[0].z), fabsf(y[0].w))));
+        am = fmaxf(am, fmaxf(fmaxf(fabsf(y[1].x), fabsf(y[1].y)), fmaxf(fabsf(y[1].z), fabsf(y[1].w))));
+    }
+    am = fmaxf(am, __shfl_xor(am, 16));
+    am = fmaxf(am, __shfl_xor(am, 32));
+    const int e = row_exp(am);
+    const float up = pow2f(12 - e);
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int f = (t0 + u) * 256 + tid, p = f / CH, chunk = f % CH;
-            const int at = VALUES ? v_at<W>(p, chunk) : k_at<W>(p, chunk);
-            if constexpr (KVT == KV_F16) {
-                *(uint4 *)(dst + at) = raw[u][0];
-            } else if constexpr (KVT == KV_I8) {
-                half8 h;
+    for (int k = 0; k < KS; k++) {
+        float4(&y)[2] = x[k % HELD];
+        if (HELD < KS) get(k, y);
+        const float z[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
+        split8(z, up, qh[k], ql[k]);
+    }
+    return pow2f(e - 12) * (scale * AT_LOG2E);
+}
+
+/* A row's running state: weights are 2^(score - m); a value's factor 2^(its exponent - ve), where ve
+ * grows so that no weight times value leaves binary16; l is this lane's share of the sum. */
+template <int DT>
+struct Running {
+    float4v o[DT];
+    float m = -INFINITY, l = 0.0f;
+    int ve = -1000;
+    __device__ __forceinline__ Running() {
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    h[i] = (_Float16)(float)(int8_t)((i < 4 ? raw[u][0].x : raw[u][0].y) >> (8 * (i & 3)));
-                *(half8 *)(dst + at) = h;
-                if (chunk == 0) {
-                    if constexpr (VALUES) {
-                        const int e = row_exp(sc[u]);
-                        aux0[p] = (float)e;
-                        aux1[p] = sc[u] * pow2f(-e);
-                    } else {
-                        aux0[p] = sc[u];
-                    }
-                }
-            } else {
-                const float *x = (const float *)&raw[u][0];
-                float am = 0.0f;
+        for (int d = 0; d < DT; d++) o[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+};
+
+/* One tile of 32 positions: x[8] the lane's scores (-inf: no position), e / f their values' exponents
+ * and fractions (int8 and fp32 caches), vb the value operand's bases, OD columns, `plane` halves to
+ * the low parts. */
+template <int OD, int KVT>
+__device__ __forceinline__ void add_tile(Running<OD / 16> &r, const float (&x)[8], const int (&e)[8], const float (&f)[8],
+                                         const _Float16 *const (&vb)[4], int plane) {
+    constexpr int DT = OD / 16;
+    float mx = x[0];
 #pragma unroll
-                for (int i = 0; i < 8; i++) am = fmaxf(am, fabsf(x[i]));
+    for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(r.m, fmaxf(mx, __shfl_xor(mx, 32)));
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    int ve = 0;
+    if constexpr (KVT != KV_F16) { /* the largest of score + exponent, above the largest score, rounded up */
+        float t = -INFINITY;
 #pragma unroll
-                for (int w = 1; w < CH; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
-                const int e = row_exp(am);
-                const float up = pow2f(12 - e);
-                half8 h, r;
+        for (int i = 0; i < 8; i++) t = fmaxf(t, (x[i] - ref) + (float)e[i]);
+        t = fmaxf(t, __shfl_xor(t, 16));
+        t = fmaxf(t, __shfl_xor(t, 32));
+        /* the old values' bound moves with the maximum */
+        t = fmaxf(t, (r.m - ref) + (float)r.ve);
+        ve = (int)ceilf(fmaxf(t, -500.0f));
+    }
+    if (__any(mx > r.m || ve != (KVT == KV_F16 ? 0 : r.ve))) {
+        const float down = __builtin_amdgcn_exp2f(r.m - ref);
+        r.l *= down;
+        const float dv = KVT == KV_F16 ? down : ldexpf(down, r.ve - ve < -300 ? -300 : r.ve - ve);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float v = x[i] * up;
-                    h[i] = (_Float16)v;
-                    r[i] = (_Float16)(v - (float)h[i]);
-                }
-                *(half8 *)(dst + at) = h;
-                *(half8 *)(dst + PT * W + at) = r;
-                if (chunk == 0) {
-                    if constexpr (VALUES) aux0[p] = (float)(e - 12), aux1[p] = 1.0f;
-                    else aux0[p] = pow2f(e - 12);
-                }
-            }
+        for (int d = 0; d < DT; d++) r.o[d] *= dv;
+        r.m = mx, r.ve = ve;
+    }
+    half8 ph, pl;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float w = __builtin_amdgcn_exp2f(x[i] - ref);
+        r.l += w;
+        float v;
+        if constexpr (KVT == KV_F16) v = w * 4096.0f;
+        else v = ldexpf(w * f[i], e[i] - ve + 12);
+        ph[i] = (_Float16)v;
+        pl[i] = (_Float16)(v - (float)ph[i]);
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        /* values of column c of the tile's 16, positions in the weights' order */
+        const _Float16 *at = vb[d & 3] + 16 * d;
+        half8 y;
+        const half4 y0 = lds_tr(at), y1 = lds_tr(at + 16 * OD);
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] = y0[i], y[4 + i] = y1[i];
+        r.o[d] = mfma16(y, ph, r.o[d]);
+        r.o[d] = mfma16(y, pl, r.o[d]);
+        if constexpr (KVT == KV_F32) {
+            const half4 z0 = lds_tr(at + plane), z1 = lds_tr(at + plane + 16 * OD);
+            half8 z;
+#pragma unroll
+            for (int i = 0; i < 4; i++) z[i] = z0[i], z[4 + i] = z1[i];
+            r.o[d] = mfma16(z, ph, r.o[d]);
         }
     }
 }
 
-template <int HDP, int KVT, int PW>
-__global__ __launch_bounds__(256) void attn_tree_ctx_k(TreeAttn a) {
-    constexpr int PT = AT_P * PW, RW = 4 / PW, OD = HDP > 256 ? 256 : HDP, KS = HDP / 32, DT = OD / 16;
+/* This part's result of a row: columns d0 .. of the weighted values, maximum, exponent and sum. */
+template <int DT>
+__device__ __forceinline__ void store_part(const TreeAttn &a, const Running<DT> &r, int s, int hrow, int d0, int gq) {
+    const size_t at = (size_t)s * a.n * a.nh + hrow;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+        if (d0 + 16 * d < a.hd) *(float4v *)(a.part + at * a.hd + d0 + 16 * d + 4 * gq) = r.o[d];
+    if (gq == 0) { /* the halves of 512 columns have value exponents of their own */
+        if (d0) a.stat[at].w = (float)r.ve;
+        else a.stat[at].x = r.m, a.stat[at].y = (float)r.ve, a.stat[at].z = r.l;
+    }
+}
+
+/* Many rows: 8 waves of 16 rows (4 where a row has 512 columns) share a tile of 32 positions. The next
+ * tile is on its way into registers while the matrix cores work on the current one (two tiles in
+ * LDS; one for 512 columns). */
+template <int HDP>
+constexpr int ctx_waves() {
+    return HDP > 256 ? 4 : 8;
+}
+template <int HDP, int KVT>
+__global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAttn a) {
+    constexpr int TH = 64 * ctx_waves<HDP>();
+    constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32, DT = OD / 16, NB = HDP > 256 ? 1 : 2;
     constexpr int PL = KVT == KV_F32 ? 2 : 1; /* planes */
+    constexpr int KC = HDP / 8, VC = OD / 8;  /* lanes that stage a row, 8 columns each */
+    constexpr int KU = AT_P * KC / TH ? AT_P * KC / TH : 1, VU = AT_P * VC / TH ? AT_P * VC / TH : 1;
+    constexpr int TILE = PL * AT_P * (HDP + OD);
     extern __shared__ uint4 smem[];
-    _Float16 *sk = (_Float16 *)smem, *sv = sk + PL * PT * HDP;
-    float *kscale = (float *)(sv + PL * PT * OD), *vexp = kscale + PT, *vfrac = vexp + PT;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, gq = lane >> 4;
+    _Float16 *tiles = (_Float16 *)smem;
+    float *aux = (float *)(tiles + NB * TILE); /* per tile: the keys' factors, the values' exponents and fractions */
+    const int lane = lane_id(), wave = wave_id(), tid = 64 * wave + lane, c = lane & 15, gq = lane >> 4;
     const int s = blockIdx.x % a.splits, g = blockIdx.x / a.splits % a.nkv, mt = blockIdx.x / a.splits / a.nkv;
     const int d0 = blockIdx.y * OD; /* the output columns: of 512, half */
     const int len = ctx_len(a), per = part_len(a, len), hd = a.hd, rep = a.nh / a.nkv, rows = a.n * rep;
     const int p0 = s * per;
     if (per == 0 || p0 >= len) return;
     const int p1 = p0 + per < len ? p0 + per : len;
-    const int pw = wave % PW, row0 = (mt * RW + wave / PW) * 16, row = row0 + c;
-    const int hrow = (row / rep) * a.nh + g * rep + row % rep; /* (node, head) */
-    const bool live = row < rows;
+    const int row0 = (mt * ctx_waves<HDP>() + wave) * 16, row = row0 + c;
+    const int hrow = row < rows ? (row / rep) * a.nh + g * rep + row % rep : -1; /* (node, head) */
+    const bool busy = row0 < rows;
     const size_t R0 = (size_t)g * a.max_ctx;
 
-    /* the query row of this lane's column, split; its factor goes to the scores */
-    half8 qh[KS], ql[KS];
-    float qfac;
-    {
-        const float *qp = a.q + (size_t)(live ? hrow : 0) * 2 * hd;
-        float am = 0.0f;
+    /* staging: columns and rows past the end repeat ones inside (finite, and their weight is 0) */
+    Raw8<KVT> rk[KU], rv[VU];
+    float sk[KU], sv[VU];
+    auto fetch_k = [&](int pt) {
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const int col = k * 32 + gq * 8;
-            if (!live || col >= hd) continue;
-            const float4 x = *(const float4 *)(qp + col), y = *(const float4 *)(qp + col + 4);
-            am = fmaxf(am, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-            am = fmaxf(am, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+        for (int u = 0; u < KU; u++) {
+            const int f = u * TH + tid, p = f / KC & (AT_P - 1), col = f % KC * 8;
+            const size_t R = R0 + (pt + p < p1 ? pt + p : p1 - 1);
+            rk[u] = load8<KVT>(a.kc, R, hd, col < hd ? col : 0);
+            sk[u] = scale_of<KVT>(a, a.kc, R);
         }
-        am = fmaxf(am, __shfl_xor(am, 16));
-        am = fmaxf(am, __shfl_xor(am, 32));
-        const int e = row_exp(am);
-        const float up = pow2f(12 - e);
-        qfac = pow2f(e - 12) * (a.scale * AT_LOG2E);
+    };
+    auto fetch_v = [&](int pt) {
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const int col = k * 32 + gq * 8;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y = x;
-            if (live && col < hd) x = *(const float4 *)(qp + col), y = *(const float4 *)(qp + col + 4);
-            const float z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        for (int u = 0; u < VU; u++) {
+            const int f = u * TH + tid, p = f / VC & (AT_P - 1), col = d0 + f % VC * 8;
+            const size_t R = R0 + (pt + p < p1 ? pt + p : p1 - 1);
+            rv[u] = load8<KVT>(a.vc, R, hd, col < hd ? col : 0);
+            sv[u] = scale_of<KVT>(a, a.vc, R);
+        }
+    };
+    auto put_k = [&](int buf) {
+        _Float16 *tk = tiles + buf * TILE;
+        float *kf = aux + buf * 3 * AT_P;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float v = z[i] * up;
-                qh[k][i] = (_Float16)v;
-                ql[k][i] = (_Float16)(v - (float)qh[k][i]);
+        for (int u = 0; u < KU; u++) {
+            const int f = u * TH + tid, p = f / KC, ch = f % KC, at = k_at<HDP>(p, ch);
+            if (AT_P * KC < TH && p >= AT_P) break;
+            if constexpr (KVT == KV_F16) {
+                *(uint4 *)(tk + at) = rk[u].a;
+            } else if constexpr (KVT == KV_I8) {
+                *(half8 *)(tk + at) = codes8(rk[u].a);
+                if (ch == 0) kf[p] = sk[u];
+            } else {
+                float am = amax8(rk[u]), x[8];
+#pragma unroll
+                for (int w = 1; w < KC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
+                const int e = row_exp(am);
+                half8 h, r;
+                floats8(rk[u], x);
+                split8(x, pow2f(12 - e), h, r);
+                *(half8 *)(tk + at) = h;
+                *(half8 *)(tk + AT_P * HDP + at) = r;
+                if (ch == 0) kf[p] = pow2f(e - 12);
             }
         }
-    }
-
-    /* this lane's operand addresses in its wave's part of a tile: the XORs leave two bases for the
-     * keys (chunk 4 k + gq by k's parity) and four for the values (by d mod 4), the rest is constant */
-    const int kp = pw * AT_P + c, vp = pw * AT_P + 4 * gq + (c >> 2);
-    const _Float16 *kb[2], *vb[4];
+    };
+    auto put_v = [&](int buf) {
+        _Float16 *tv = tiles + buf * TILE + PL * AT_P * HDP;
+        float *vf = aux + buf * 3 * AT_P + AT_P;
+        int *ve = (int *)(vf + AT_P);
 #pragma unroll
-    for (int i = 0; i < 2; i++) kb[i] = sk + k_at<HDP>(kp, 4 * i + gq) - 32 * i;
+        for (int u = 0; u < VU; u++) {
+            const int f = u * TH + tid, p = f / VC, ch = f % VC, at = v_at<OD>(p, ch);
+            if (AT_P * VC < TH && p >= AT_P) break;
+            if constexpr (KVT == KV_F16) {
+                *(uint4 *)(tv + at) = rv[u].a;
+            } else if constexpr (KVT == KV_I8) {
+                *(half8 *)(tv + at) = codes8(rv[u].a);
+                if (ch == 0) {
+                    const int e = row_exp(sv[u]);
+                    ve[p] = e, vf[p] = sv[u] * pow2f(-e);
+                }
+            } else {
+                float am = amax8(rv[u]), x[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) vb[i] = sv + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
-
-    float4v o[DT];
+                for (int w = 1; w < VC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
+                const int e = row_exp(am);
+                half8 h, r;
+                floats8(rv[u], x);
+                split8(x, pow2f(12 - e), h, r);
+                *(half8 *)(tv + at) = h;
+                *(half8 *)(tv + AT_P * OD + at) = r;
+                if (ch == 0) ve[p] = e - 12, vf[p] = 1.0f;
+            }
+        }
+    };
+    if constexpr (NB == 2) fetch_k(p0), fetch_v(p0);
+    half8 qh[KS], ql[KS];
+    const float qfac = load_q<KS>(a.q + (size_t)(hrow < 0 ? 0 : hrow) * 2 * hd, hrow >= 0, hd, gq, a.scale, qh, ql);
+    Running<DT> r;
+    if (NB == 2) put_k(0), put_v(0);
+    /* this lane's operand addresses in a tile: the XORs leave two bases for the keys (chunk 4 k + gq by
+     * k's parity) and four for the values (by d mod 4), the rest is constant */
+    const int vp = 4 * gq + (c >> 2);
+    int kb[2], vo[4];
 #pragma unroll
-    for (int d = 0; d < DT; d++) o[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, mo = -INFINITY, l = 0.0f;
-
-    for (int pt = p0; pt < p1; pt += PT) {
-        __syncthreads(); /* the last tile has been read */
-        stage<HDP, KVT, PT, false>(a, R0, pt, p1, 0, sk, kscale, nullptr);
-        stage<OD, KVT, PT, true>(a, R0, pt, p1, d0, sv, vexp, vfrac);
+    for (int i = 0; i < 2; i++) kb[i] = k_at<HDP>(c, 4 * i + gq) - 32 * i;
+#pragma unroll
+    for (int i = 0; i < 4; i++) vo[i] = PL * AT_P * HDP + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
+    int buf = 0;
+    for (int pt = p0; pt < p1; pt += AT_P) {
+        const bool more = NB == 2 && pt + AT_P < p1;
+        if (NB == 1) { /* one tile: no registers to hold the next one either */
+            __syncthreads();
+            fetch_k(pt), put_k(0);
+            fetch_v(pt), put_v(0);
+        }
         __syncthreads();
-        const int b = pw * AT_P; /* this wave's positions of the tile */
-        if (pt + b >= p1) continue;
-        /* scores: positions 16 i + 4 gq + j of the wave's tile against row c */
+        if (more) fetch_k(pt + AT_P), fetch_v(pt + AT_P);
+        if (busy) {
+            const _Float16 *tk = tiles + buf * TILE;
+            const float *kf = aux + buf * 3 * AT_P, *vf = kf + AT_P;
+            const int *ve = (const int *)(vf + AT_P);
+            float4v sc[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const _Float16 *at = tk + kb[k & 1] + 16 * i * HDP + 32 * k;
+                    const half8 x = *(const half8 *)at;
+                    sc[i] = mfma16(x, qh[k], sc[i]);
+                    sc[i] = mfma16(x, ql[k], sc[i]);
+                    if constexpr (KVT == KV_F32) sc[i] = mfma16(*(const half8 *)(at + AT_P * HDP), qh[k], sc[i]);
+                }
+            float x[8], f[8];
+            int e[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) { /* position 16 (i / 4) + 4 gq + i % 4 */
+                const int p = 16 * (i >> 2) + 4 * gq + (i & 3);
+                float y = sc[i >> 2][i & 3];
+                if constexpr (KVT != KV_F16) y *= qfac * kf[p], e[i] = ve[p], f[i] = vf[p];
+                else y *= qfac, e[i] = 0, f[i] = 1.0f;
+                x[i] = pt + p < p1 ? y : -INFINITY;
+            }
+            const _Float16 *const vb[4] = {tk + vo[0], tk + vo[1], tk + vo[2], tk + vo[3]};
+            add_tile<OD, KVT>(r, x, e, f, vb, AT_P * OD);
+        }
+        if (more) put_k(buf ^ 1), put_v(buf ^ 1);
+        if (NB == 2) buf ^= 1;
+    }
+    r.l += __shfl_xor(r.l, 16);
+    r.l += __shfl_xor(r.l, 32);
+    if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);
+}
+
+/* Few rows: the time is that of the cache's bytes, so each of 4 waves takes tiles of its own, its
+ * keys straight into matrix operands, its values through a piece of LDS of its own (a binary16
+ * cache's without a register between), requested together; two workgroups to a CU keep the requests
+ * coming. The waves' results are joined at the end. */
+template <int HDP, int KVT>
+__global__ __launch_bounds__(256, HDP <= 128 || (HDP == 256 && KVT == KV_F16) ? 2 : 1) void attn_tree_few_k(TreeAttn a) {
+    constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32, DT = OD / 16;
+    constexpr int PL = KVT == KV_F32 ? 2 : 1, VC = OD / 8, VR = 64 / VC; /* rows of a wave's request */
+    constexpr int VU = AT_P / VR, VB = KVT == KV_F16 ? 1 : 2; /* requests of a tile, taken in VB batches */
+    extern __shared__ uint4 smem[];
+    const int lane = lane_id(), wave = wave_id(), c = lane & 15, gq = lane >> 4;
+    _Float16 *tv = (_Float16 *)smem + wave * PL * AT_P * OD;
+    float *aux = (float *)((_Float16 *)smem + 4 * PL * AT_P * OD) + wave * 3 * AT_P, *kf = aux, *vf = aux + AT_P;
+    int *ve = (int *)(aux + 2 * AT_P);
+    const int s = blockIdx.x % a.splits, g = blockIdx.x / a.splits % a.nkv, mt = blockIdx.x / a.splits / a.nkv;
+    const int d0 = blockIdx.y * OD, hd = a.hd, rep = a.nh / a.nkv, row = mt * 16 + c;
+    const int hrow = row < a.n * rep ? (row / rep) * a.nh + g * rep + row % rep : -1; /* (node, head) */
+    const size_t R0 = (size_t)g * a.max_ctx;
+    half8 qh[KS], ql[KS];
+    const float qfac = load_q<KS>(a.q + (size_t)(hrow < 0 ? 0 : hrow) * 2 * hd, hrow >= 0, hd, gq, a.scale, qh, ql);
+    const int len = ctx_len(a), per = part_len(a, len), p0 = s * per;
+    if (per == 0 || p0 >= len) return;
+    const int p1 = p0 + per < len ? p0 + per : len;
+    Running<DT> r;
+    const int vp = 4 * gq + (c >> 2);
+    const _Float16 *vb[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) vb[i] = tv + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
+    for (int pt = p0 + wave * AT_P; pt < p1; pt += 4 * AT_P) {
+        /* rows and columns past the end repeat ones inside (finite, and their weight is 0) */
+        auto row_at = [&](int p) { return R0 + (pt + p < p1 ? pt + p : p1 - 1); };
+        Raw8<KVT> rk[KS], rv[VU / VB];
+        float vs[VU / VB];
         float4v sc[2];
+        auto ask_v = [&](int b) {
+#pragma unroll
+            for (int u = 0; u < VU / VB; u++) {
+                const int p = (b * (VU / VB) + u) * VR + lane / VC, ch = lane % VC;
+                if constexpr (KVT == KV_F16) { /* chunk ch of the LDS row is the row's chunk ch ^ ... */
+                    const int col = d0 + ((ch ^ ((p & 3) << 1)) << 3);
+                    const unsigned short *src = (const unsigned short *)a.vc + row_at(p) * hd + (col < hd ? col : 0);
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)(uintptr_t)src,
+                                                     (__attribute__((address_space(3))) uint32_t *)(uintptr_t)(tv + u * VR * OD), 16, 0, 0);
+                } else {
+                    const int col = d0 + ch * 8;
+                    rv[u] = load8<KVT>(a.vc, row_at(p), hd, col < hd ? col : 0);
+                    vs[u] = scale_of<KVT>(a, a.vc, row_at(p));
+                }
+            }
+        };
+        auto put_v = [&](int b) {
+#pragma unroll
+            for (int u = 0; u < VU / VB; u++) {
+                const int p = (b * (VU / VB) + u) * VR + lane / VC, ch = lane % VC, at = v_at<OD>(p, ch);
+                if constexpr (KVT == KV_I8) {
+                    *(half8 *)(tv + at) = codes8(rv[u].a);
+                    if (ch == 0) {
+                        const int e = row_exp(vs[u]);
+                        ve[p] = e, vf[p] = vs[u] * pow2f(-e);
+                    }
+                } else if constexpr (KVT == KV_F32) {
+                    float am = amax8(rv[u]), x[8];
+#pragma unroll
+                    for (int w = 1; w < VC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
+                    const int e = row_exp(am);
+                    half8 h, y;
+                    floats8(rv[u], x);
+                    split8(x, pow2f(12 - e), h, y);
+                    *(half8 *)(tv + at) = h;
+                    *(half8 *)(tv + AT_P * OD + at) = y;
+                    if (ch == 0) ve[p] = e - 12, vf[p] = 1.0f;
+                }
+            }
+        };
+        nmx_lds_wave_sync(); /* the last tile's values have been read */
+        ask_v(0);
+        /* scores: positions 16 i + 4 gq + j against row c */
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            const size_t R = row_at(16 * i + c);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const _Float16 *at = kb[k & 1] + 16 * i * HDP + 32 * k;
-                const half8 x = *(const half8 *)at;
+                const int col = 32 * k + 8 * gq;
+                rk[k] = load8<KVT>(a.kc, R, hd, col < hd ? col : 0);
+            }
+            float ks = scale_of<KVT>(a, a.kc, R), up = 1.0f;
+            if (VB == 2 && i == 1) put_v(0), ask_v(1);
+            sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (KVT == KV_F32) {
+                float am = amax8(rk[0]);
+#pragma unroll
+                for (int k = 1; k < KS; k++) am = fmaxf(am, amax8(rk[k]));
+                am = fmaxf(am, __shfl_xor(am, 16));
+                am = fmaxf(am, __shfl_xor(am, 32));
+                const int e = row_exp(am);
+                up = pow2f(12 - e), ks = pow2f(e - 12);
+            }
+            if (KVT != KV_F16 && gq == 0) kf[16 * i + c] = ks;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                half8 x, y;
+                if constexpr (KVT == KV_F16) {
+                    x = __builtin_bit_cast(half8, rk[k].a);
+                } else if constexpr (KVT == KV_I8) {
+                    x = codes8(rk[k].a);
+                } else {
+                    float z[8];
+                    floats8(rk[k], z);
+                    split8(z, up, x, y);
+                }
                 sc[i] = mfma16(x, qh[k], sc[i]);
                 sc[i] = mfma16(x, ql[k], sc[i]);
-                if constexpr (KVT == KV_F32) sc[i] = mfma16(*(const half8 *)(at + PT * HDP), qh[k], sc[i]);
+                if constexpr (KVT == KV_F32) sc[i] = mfma16(y, qh[k], sc[i]);
             }
         }
-        float x[8], xv[8], vf[8], mx = -INFINITY, mxo = -INFINITY;
+        if constexpr (KVT == KV_F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* the values are in LDS */
+        else put_v(VB - 1);
+        nmx_lds_wave_sync();
+        float x[8], f[8];
+        int e[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int p = b + 16 * (i >> 2) + 4 * gq + (i & 3);
-            float y = sc[i >> 2][i & 3] * qfac;
-            if constexpr (KVT != KV_F16) y *= kscale[p];
+            const int p = 16 * (i >> 2) + 4 * gq + (i & 3);
+            float y = sc[i >> 2][i & 3];
+            if constexpr (KVT != KV_F16) y *= qfac * kf[p], e[i] = ve[p], f[i] = vf[p];
+            else y *= qfac, e[i] = 0, f[i] = 1.0f;
             x[i] = pt + p < p1 ? y : -INFINITY;
-            mx = fmaxf(mx, x[i]);
-            if constexpr (KVT != KV_F16) {
-                xv[i] = x[i] + vexp[p];
-                vf[i] = vfrac[p];
-                mxo = fmaxf(mxo, xv[i]);
-            }
         }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
-        if constexpr (KVT != KV_F16) {
-            mxo = fmaxf(mxo, __shfl_xor(mxo, 16));
-            mxo = fmaxf(mo, fmaxf(mxo, __shfl_xor(mxo, 32)));
-        } else {
-            mxo = mx;
-        }
-        const float ref = mx == -INFINITY ? 0.0f : mx, refo = mxo == -INFINITY ? 0.0f : mxo;
-        l *= exp2f(m - ref);
-        const float down = exp2f(mo - refo);
-        m = mx, mo = mxo;
-        half8 ph, pl;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float w = exp2f(x[i] - ref);
-            l += w;
-            const float v = KVT == KV_F16 ? w * 4096.0f : exp2f(xv[i] - refo) * (vf[i] * 4096.0f);
-            ph[i] = (_Float16)v;
-            pl[i] = (_Float16)(v - (float)ph[i]);
-        }
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            o[d] *= down;
-            /* values of column c of the tile's 16, positions in the weights' order */
-            const _Float16 *at = vb[d & 3] + 16 * d;
-            half8 y, z;
-            const half4 y0 = lds_tr(at), y1 = lds_tr(at + 16 * OD);
-#pragma unroll
-            for (int i = 0; i < 4; i++) y[i] = y0[i], y[4 + i] = y1[i];
-            o[d] = mfma16(y, ph, o[d]);
-            o[d] = mfma16(y, pl, o[d]);
-            if constexpr (KVT == KV_F32) {
-                const half4 z0 = lds_tr(at + PT * OD), z1 = lds_tr(at + PT * OD + 16 * OD);
-#pragma unroll
-                for (int i = 0; i < 4; i++) z[i] = z0[i], z[4 + i] = z1[i];
-                o[d] = mfma16(z, ph, o[d]);
-            }
-        }
+        add_tile<OD, KVT>(r, x, e, f, vb, AT_P * OD);
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-
-    if constexpr (PW > 1) { /* the waves' positions joined: wave pw 0 of a row group adds the others' */
-        __syncthreads();
-        float *xo = (float *)smem; /* [RW][PW - 1][64][DT 4 + 4] would not fit: one wave at a time */
-        for (int w = 1; w < PW; w++) {
-            float *my = xo + (size_t)(wave / PW) * 64 * (4 * DT + 4) + lane;
-            if (pw == w) {
+    /* the waves' results joined, one after the other into wave 0's; 4 DT + 3 words of a lane each */
+    constexpr int XW = 64 * (4 * DT + 4);
+    float *xo = (float *)smem + lane;
+    r.l += __shfl_xor(r.l, 16);
+    r.l += __shfl_xor(r.l, 32);
+    __syncthreads();
+    if (wave) {
+        float *my = xo + (wave - 1) * XW;
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) my[(4 * d + j) * 64] = o[d][j];
-                my[4 * DT * 64] = m, my[(4 * DT + 1) * 64] = mo, my[(4 * DT + 2) * 64] = l;
-            }
-            __syncthreads();
-            if (pw == 0) {
-                const float m2 = my[4 * DT * 64], mo2 = my[(4 * DT + 1) * 64], l2 = my[(4 * DT + 2) * 64];
-                const float mn = fmaxf(m, m2), mon = fmaxf(mo, mo2);
-                const float ref = mn == -INFINITY ? 0.0f : mn, refo = mon == -INFINITY ? 0.0f : mon;
-                const float f1 = exp2f(mo - refo), f2 = exp2f(mo2 - refo);
-                l = l * exp2f(m - ref) + l2 * exp2f(m2 - ref);
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) o[d][j] = o[d][j] * f1 + my[(4 * d + j) * 64] * f2;
-                m = mn, mo = mon;
-            }
-            __syncthreads();
-        }
-        if (pw) return;
+            for (int j = 0; j < 4; j++) my[(4 * d + j) * 64] = r.o[d][j];
+        my[4 * DT * 64] = r.m, my[(4 * DT + 1) * 64] = r.l, my[(4 * DT + 2) * 64] = (float)r.ve;
     }
-    if (!live) return;
-    const size_t at = (size_t)s * a.n * a.nh + hrow;
+    __syncthreads();
+    if (wave) return;
+    float m = r.m;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-        if (d0 + 16 * d < hd) *(float4v *)(a.part + at * hd + d0 + 16 * d + 4 * gq) = o[d];
-    if (gq == 0) { /* the halves of 512 columns have value exponents of their own */
-        if (d0) a.stat[at].w = mo;
-        else a.stat[at].x = m, a.stat[at].y = mo, a.stat[at].z = l;
+    for (int w = 0; w < 3; w++) m = fmaxf(m, xo[w * XW + 4 * DT * 64]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    /* exponents count from a row's own maximum: the common one covers them all */
+    float top = (r.m - ref) + (float)r.ve;
+#pragma unroll
+    for (int w = 0; w < 3; w++) top = fmaxf(top, (xo[w * XW + 4 * DT * 64] - ref) + xo[w * XW + (4 * DT + 2) * 64]);
+    const int vn = KVT == KV_F16 ? 0 : (int)ceilf(fmaxf(top, -500.0f));
+    auto shift = [&](float f, float v) { /* f 2^(v - vn) */
+        const float d = v - (float)vn;
+        return KVT == KV_F16 ? f : ldexpf(f, d < -300.0f ? -300 : (int)d);
+    };
+    const float f0 = __builtin_amdgcn_exp2f(r.m - ref), g0 = shift(f0, (float)r.ve);
+    r.l *= f0;
+#pragma unroll
+    for (int d = 0; d < DT; d++) r.o[d] *= g0;
+#pragma unroll 1
+    for (int w = 0; w < 3; w++) {
+        const float *o = xo + w * XW;
+        const float fw = __builtin_amdgcn_exp2f(o[4 * DT * 64] - ref), gw = shift(fw, o[(4 * DT + 2) * 64]);
+        r.l += o[(4 * DT + 1) * 64] * fw;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) r.o[d][j] += o[(4 * d + j) * 64] * gw;
     }
+    r.m = m, r.ve = vn;
+    if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);
 }
 
 /* ---- the node's ancestors, and the join ---------------------------------------------------- */
+constexpr int JT = 1024; /* threads of a join */
+
 template <int KVT>
-__global__ __launch_bounds__(256) void attn_tree_join_k(TreeAttn a) {
-    constexpr int ND = 8; /* columns lane + 64 i, hd <= 512 */
-    __shared__ float sc[64], red[8], acc_s[4][512], w_s[2][AT_MAXS];
+__global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
+    __shared__ float sc[64], red[32], acc_s[JT * 4], w_s[2][AT_MAXS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int hrow = blockIdx.x, t = hrow / a.nh, h = hrow % a.nh, hd = a.hd, nd = hd >> 6;
     const int g = h / (a.nh / a.nkv), rows = a.n * a.nh;
     const int len = ctx_len(a), per = part_len(a, len), parts = per ? (len + per - 1) / per : 0;
     const size_t R0 = (size_t)g * a.max_ctx;
     const float *qp = a.q + (size_t)hrow * 2 * hd;
-    const float *ksc = KVT == KV_I8 ? (const float *)((const int8_t *)a.kc + (size_t)a.nkv * a.max_ctx * hd) : nullptr;
-    const float *vsc = KVT == KV_I8 ? (const float *)((const int8_t *)a.vc + (size_t)a.nkv * a.max_ctx * hd) : nullptr;
-    float q[ND];
+    /* slots of hd / 4 threads: a thread takes 4 columns of every slots-th row of a sum */
+    const int per_slot = hd >> 2, slots = JT / per_slot, slot = tid / per_slot, col = tid % per_slot * 4;
+    constexpr int PB = 8; /* rows of a slot requested at once */
+    float4 pr[PB];
 #pragma unroll
-    for (int i = 0; i < ND; i++) q[i] = i < nd ? qp[lane + 64 * i] : 0.0f;
-    float4 st = make_float4(-INFINITY, -INFINITY, 0.0f, 0.0f); /* thread = part */
+    for (int u = 0; u < PB; u++) {
+        const int s = slot + u * slots;
+        pr[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (slot < slots && s < parts) pr[u] = *(const float4 *)(a.part + ((size_t)s * rows + hrow) * hd + col);
+    }
+    float4 st = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f); /* thread = part */
     if (tid < parts) st = a.stat[(size_t)tid * rows + hrow];
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = i < nd ? qp[lane + 64 * i] : 0.0f;
     /* the ancestors' rows inside the cache */
     const int p0 = tree_slot0(a.pos, a.pos_off, a.max_ctx);
     unsigned long long set = __shfl(tree_ancestors(a.parent, a.n, nullptr), t);
@@ -431,24 +703,27 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(TreeAttn a) {
         set &= ~0ull << lo;
         if (hi < 64) set &= (1ull << hi) - 1;
     }
-    auto value = [&](const void *cache, const float *scales, size_t R, int col) -> float {
-        if constexpr (KVT == KV_F32) return ((const float *)cache)[R * hd + col];
-        else if constexpr (KVT == KV_F16) return kv_half_value(((const unsigned short *)cache)[R * hd + col]);
-        else return (float)((const int8_t *)cache)[R * hd + col] * scales[R];
-    };
     const int na = __popcll(set);
     auto nth = [&](int i) { /* the i-th node of the set */
         unsigned long long x = set;
         for (int k = 0; k < i; k++) x &= x - 1;
         return __ffsll((long long)x) - 1;
     };
+    /* scores: a wave for each ancestor */
     float mt = -INFINITY;
-    for (int i = wave; i < na; i += 4) {
+    for (int i = wave; i < na; i += JT / 64) {
         const size_t R = R0 + p0 + nth(i);
+        const float rs = scale_of<KVT>(a, a.kc, R);
         float d = 0.0f;
 #pragma unroll
-        for (int k = 0; k < ND; k++)
-            if (k < nd) d = __builtin_fmaf(q[k], value(a.kc, ksc, R, lane + 64 * k), d);
+        for (int k = 0; k < 8; k++)
+            if (k < nd) {
+                float x;
+                if constexpr (KVT == KV_F32) x = ((const float *)a.kc)[R * hd + lane + 64 * k];
+                else if constexpr (KVT == KV_F16) x = kv_half_value(((const unsigned short *)a.kc)[R * hd + lane + 64 * k]);
+                else x = (float)((const int8_t *)a.kc)[R * hd + lane + 64 * k] * rs;
+                d = __builtin_fmaf(q[k], x, d);
+            }
 #pragma unroll
         for (int x = 32; x >= 1; x >>= 1) d += __shfl_xor(d, x);
         d *= a.scale * AT_LOG2E;
@@ -458,114 +733,112 @@ __global__ __launch_bounds__(256) void attn_tree_join_k(TreeAttn a) {
     mt = fmaxf(mt, nmx_max_f32_wave(st.x));
     if (lane == 0) red[wave] = mt;
     __syncthreads();
-    const float m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), ref = m == -INFINITY ? 0.0f : m;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < JT / 64; w++) m = fmaxf(m, red[w]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    if (tid < parts) { /* a part's weight, for its sum and for its 2^12 high values */
+        const float w = __builtin_amdgcn_exp2f(st.x - ref);
+        st.z *= w;
+        w_s[0][tid] = ldexpf(w, (int)st.y - 12);
+        w_s[1][tid] = hd > 256 ? ldexpf(w, (int)st.w - 12) : 0.0f;
+    }
+    float l = tid < na ? __builtin_amdgcn_exp2f(sc[tid] - ref) : 0.0f;
     __syncthreads();
-    float l = st.z * exp2f(st.x - ref); /* a part's sum */
-    if (tid < parts) {
-        w_s[0][tid] = exp2f(st.y - ref - 12.0f);
-        if (hd > 256) w_s[1][tid] = exp2f(st.w - ref - 12.0f);
-    }
-    __syncthreads();
-    float acc[ND];
-#pragma unroll
-    for (int i = 0; i < ND; i++) acc[i] = 0.0f;
-    for (int s = wave; s < parts; s += 4) {
-        const float w0 = w_s[0][s], w1 = hd > 256 ? w_s[1][s] : 0.0f;
-        const float *pp = a.part + ((size_t)s * rows + hrow) * hd + lane;
-#pragma unroll
-        for (int i = 0; i < ND; i++)
-            if (i < nd) acc[i] = __builtin_fmaf(i < 4 ? w0 : w1, pp[64 * i], acc[i]);
-    }
-    float lt = 0.0f;
-    for (int i = wave; i < na; i += 4) {
-        const float w = exp2f(sc[i] - ref);
-        const size_t R = R0 + p0 + nth(i);
-        lt += w;
-#pragma unroll
-        for (int k = 0; k < ND; k++)
-            if (k < nd) acc[k] = __builtin_fmaf(w, value(a.vc, vsc, R, lane + 64 * k), acc[k]);
-    }
+    if (tid < na) sc[tid] = l;
+    l += st.z;
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x);
-    if (lane == 0) red[4 + wave] = l + lt;
-#pragma unroll
-    for (int i = 0; i < ND; i++)
-        if (i < nd) acc_s[wave][lane + 64 * i] = acc[i];
+    if (lane == 0) red[16 + wave] = l;
     __syncthreads();
-    const float sum = (red[4] + red[5]) + (red[6] + red[7]);
-    for (int d = tid; d < hd; d += 256) {
-        float v = (acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d]);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](float w, float4 x) {
+        acc.x = __builtin_fmaf(w, x.x, acc.x), acc.y = __builtin_fmaf(w, x.y, acc.y);
+        acc.z = __builtin_fmaf(w, x.z, acc.z), acc.w = __builtin_fmaf(w, x.w, acc.w);
+    };
+    if (slot < slots) {
+        const float *ws = w_s[col >> 8];
+#pragma unroll
+        for (int u = 0; u < PB; u++) {
+            const int s = slot + u * slots;
+            if (s < parts) add(ws[s], pr[u]);
+        }
+        for (int s = slot + PB * slots; s < parts; s += slots)
+            add(ws[s], *(const float4 *)(a.part + ((size_t)s * rows + hrow) * hd + col));
+        for (int i = slot; i < na; i += slots)
+            add(sc[i], kv_load4<KVT>(a.vc, R0 + p0 + nth(i), hd, col,
+                                     KVT == KV_I8 ? (const float *)((const int8_t *)a.vc + (size_t)a.nkv * a.max_ctx * hd) : nullptr));
+        *(float4 *)(acc_s + slot * hd + col) = acc;
+    }
+    __syncthreads();
+    if (tid < hd) {
+        float sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JT / 64; w++) sum += red[16 + w];
+        for (int w = 0; w < slots; w++) v += acc_s[w * hd + tid];
         v = sum > 0.0f || !(sum == sum) ? v / sum : 0.0f; /* no row at all in sight: 0 */
-        v = v * nmx_sigmoid(qp[hd + d]);
-        const int col = h * hd + d;
-        a.o[(size_t)t * a.nh * hd + col] = v;
-        if (a.aq) a8_block(v, col >> 5, t, a.n, a.aq, a.ad, a.afs); /* hd % 64 == 0: whole blocks */
+        v = v * nmx_sigmoid(qp[hd + tid]);
+        const int at = h * hd + tid;
+        a.o[(size_t)t * a.nh * hd + at] = v;
+        if (a.aq) a8_block(v, at >> 5, t, a.n, a.aq, a.ad, a.afs); /* hd % 64 == 0: whole blocks */
     }
 }
 
-/* How the context is divided among workgroups: PW of a workgroup's 4 waves side by side over the
- * positions, the others over rows; `splits` parts. */
+/* How the context is divided among workgroups. */
 struct Plan {
-    int hdp, pw, mtiles, splits, unit, halves;
+    int hdp, mtiles, splits, unit, halves;
+    bool few; /* attn_tree_few_k, else attn_tree_ctx_k */
     size_t part_bytes, bytes, lds;
 };
-
-/* positions side by side that a tile of the format fits the LDS with */
-int max_pw(int hdp, int kv_dtype) {
-    const int planes = kv_dtype == KV_F32 ? 2 : 1;
-    const int fit = hdp > 256 ? 1 : (128 << 10) / (2 * planes * AT_P * hdp * 2);
-    return fit >= 4 ? 4 : fit >= 2 ? 2 : 1;
-}
 
 Plan make_plan(int n, int nh, int nkv, int hd, int kv_dtype) {
     Plan p;
     p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
-    const int tiles = (n * (nh / nkv) + 15) / 16;
-    const int most = max_pw(p.hdp, kv_dtype);
-    p.pw = tiles == 1 ? most : tiles == 2 ? (most < 2 ? most : 2) : 1;
-    const int rw = 4 / p.pw;
-    p.mtiles = (tiles + rw - 1) / rw;
-    const int target = p.pw == 4 ? 256 : 512;
-    int s = target / (nkv * p.mtiles);
-    p.splits = s < 1 ? 1 : s > AT_MAXS ? AT_MAXS : s;
-    p.unit = AT_P * p.pw;
+    const int tiles = (n * (nh / nkv) + 15) / 16, od = p.hdp > 256 ? 256 : p.hdp;
     const int planes = kv_dtype == KV_F32 ? 2 : 1;
-    const int od = p.hdp > 256 ? 256 : p.hdp;
+    p.few = tiles <= 2 && !(p.hdp > 256 && kv_dtype == KV_F32); /* too many registers */
+    const int waves = p.hdp > 256 ? 4 : 8;
+    p.mtiles = p.few ? tiles : (tiles + waves - 1) / waves;
     p.halves = p.hdp / od;
-    p.lds = (size_t)p.unit * (p.hdp + od) * 2 * planes + (size_t)3 * p.unit * 4;
-    const size_t join = p.pw > 1 ? (size_t)rw * 64 * (od / 4 + 4) * 4 : 0;
-    if (join > p.lds) p.lds = join;
+    /* the many-row kernel has a CU for itself; of the other's workgroups two share one */
+    const int s = (p.few ? 512 : 256) / (nkv * p.mtiles * p.halves);
+    p.splits = s < 1 ? 1 : s > AT_MAXS ? AT_MAXS : s;
+    p.unit = p.few ? 4 * AT_P : AT_P;
+    if (p.few) {
+        p.lds = (size_t)4 * planes * AT_P * od * 2 + 4 * 3 * AT_P * 4;
+        const size_t join = (size_t)3 * 64 * (od / 4 + 4) * 4;
+        if (join > p.lds) p.lds = join;
+    } else {
+        p.lds = (size_t)(p.hdp > 256 ? 1 : 2) * (planes * AT_P * (p.hdp + od) * 2 + 3 * AT_P * 4);
+    }
     p.part_bytes = (size_t)p.splits * n * nh * hd * 4;
     p.bytes = p.part_bytes + (size_t)p.splits * n * nh * sizeof(float4);
     return p;
 }
 
-template <int HDP, int KVT, int PW>
+template <int HDP, int KVT>
 int launch_ctx(nmx_ctx *ctx, const TreeAttn &a, const Plan &p) {
-    static std::atomic<uint64_t> set;
-    if (nmx_dyn_lds(ctx, (const void *)attn_tree_ctx_k<HDP, KVT, PW>, p.lds, set)) return -1;
-    attn_tree_ctx_k<HDP, KVT, PW><<<dim3((unsigned)(p.splits * a.nkv * p.mtiles), (unsigned)p.halves), 256, p.lds,
-                                        ctx->stream>>>(a);
+    const dim3 grid((unsigned)(p.splits * a.nkv * p.mtiles), (unsigned)p.halves);
+    static std::atomic<uint64_t> set0, set1;
+    if (p.few) {
+        if constexpr (HDP <= 256 || KVT != KV_F32) {
+            if (nmx_dyn_lds(ctx, (const void *)attn_tree_few_k<HDP, KVT>, p.lds, set1)) return -1;
+            attn_tree_few_k<HDP, KVT><<<grid, 256, p.lds, ctx->stream>>>(a);
+        }
+    } else {
+        if (nmx_dyn_lds(ctx, (const void *)attn_tree_ctx_k<HDP, KVT>, p.lds, set0)) return -1;
+        attn_tree_ctx_k<HDP, KVT><<<grid, 64 * ctx_waves<HDP>(), p.lds, ctx->stream>>>(a);
+    }
     NMX_LAUNCHED(ctx, "attn_tree_ctx");
     return 0;
 }
 
-template <int HDP, int KVT>
-int launch_pw(nmx_ctx *ctx, const TreeAttn &a, const Plan &p) {
-    constexpr int planes = KVT == KV_F32 ? 2 : 1, fit = HDP > 256 ? 1 : (128 << 10) / (2 * planes * AT_P * HDP * 2);
-    if constexpr (fit >= 4)
-        if (p.pw == 4) return launch_ctx<HDP, KVT, 4>(ctx, a, p);
-    if constexpr (fit >= 2)
-        if (p.pw == 2) return launch_ctx<HDP, KVT, 2>(ctx, a, p);
-    return launch_ctx<HDP, KVT, 1>(ctx, a, p);
-}
-
 template <int KVT>
 int launch_tree(nmx_ctx *ctx, const TreeAttn &a, const Plan &p) {
-    int rc = p.hdp == 64 ? launch_pw<64, KVT>(ctx, a, p) : p.hdp == 128 ? launch_pw<128, KVT>(ctx, a, p) :
-             p.hdp == 256 ? launch_pw<256, KVT>(ctx, a, p) : launch_pw<512, KVT>(ctx, a, p);
+    const int rc = p.hdp == 64 ? launch_ctx<64, KVT>(ctx, a, p) : p.hdp == 128 ? launch_ctx<128, KVT>(ctx, a, p) :
+                   p.hdp == 256 ? launch_ctx<256, KVT>(ctx, a, p) : launch_ctx<512, KVT>(ctx, a, p);
     if (rc) return rc;
-    attn_tree_join_k<KVT><<<(unsigned)(a.n * a.nh), 256, 0, ctx->stream>>>(a);
+    attn_tree_join_k<KVT><<<(unsigned)(a.n * a.nh), JT, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "attn_tree_join");
     return 0;
 }

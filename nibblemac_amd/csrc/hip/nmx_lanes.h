@@ -4,6 +4,7 @@
  * within each 32-lane group (ds_swizzle). nmx_max32 / nmx_sum32 reduce over each 32-lane
  * half-wave (every lane of the half active): DPP quad permutes and row mirrors inside the
  * 16-lane rows, one swizzle across them; max and integer sums are exact in any order.
+ * nmx_scan_wave: running sums over the wave's lanes.
  * nmx_quad_chain: a left-to-right fp32 sum over a quad of lanes, lane c holding the c-th
  * quarter of the terms; the running sum moves to the next lane by a DPP broadcast of lane c
  * (quad_perm [c, c, c, c]), so the adds are one sequential chain. nmx_lds_wave_sync: between
@@ -51,6 +52,33 @@ __device__ __forceinline__ int nmx_sum32(int v) {
     v += nmx_dpp<NMX_DPP_HALF_MIRROR>(v);
     v += nmx_dpp<NMX_DPP_MIRROR>(v);
     return v + nmx_swz16(v);
+}
+
+/* Inclusive running sums over the wave's lanes (every lane active; V u32, u64 or double): DPP shifts
+ * within the 16-lane rows, then the rows' ends broadcast to the rows behind them. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t nmx_dpp_or0(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V nmx_dpp_or0_of(V v) {
+    if constexpr (sizeof(V) == 4) {
+        return __builtin_bit_cast(V, nmx_dpp_or0<CTRL, ROWS>(__builtin_bit_cast(uint32_t, v)));
+    } else {
+        const uint64_t x = __builtin_bit_cast(uint64_t, v);
+        const uint64_t lo = nmx_dpp_or0<CTRL, ROWS>((uint32_t)x), hi = nmx_dpp_or0<CTRL, ROWS>((uint32_t)(x >> 32));
+        return __builtin_bit_cast(V, hi << 32 | lo);
+    }
+}
+template <typename V>
+__device__ __forceinline__ V nmx_scan_wave(V v) {
+    v += nmx_dpp_or0_of<0x111, 0xF>(v); /* row_shr 1, 2, 4, 8 */
+    v += nmx_dpp_or0_of<0x112, 0xF>(v);
+    v += nmx_dpp_or0_of<0x114, 0xF>(v);
+    v += nmx_dpp_or0_of<0x118, 0xF>(v);
+    v += nmx_dpp_or0_of<0x142, 0xA>(v); /* row_bcast 15 into rows 1 and 3 */
+    v += nmx_dpp_or0_of<0x143, 0xC>(v); /* row_bcast 31 into rows 2 and 3 */
+    return v;
 }
 
 /* Maximum of a float over the wave (every lane active; exact in any order), returned to

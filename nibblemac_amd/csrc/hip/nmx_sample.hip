@@ -26,16 +26,19 @@
 namespace {
 
 constexpr int SM_CHUNK = 8192; /* logits of a workgroup of sample_scan_k */
-constexpr int SM_T1 = 512, SM_PER = SM_CHUNK / SM_T1;
-constexpr int SM_T2 = 1024, SM_RUN = SM_CHUNK / SM_T2; /* consecutive logits of a thread */
+constexpr int SM_T1 = 512, SM_PER = SM_CHUNK / SM_T1, SM_SLICE = SM_CHUNK / (SM_T1 / 64);
+constexpr int SM_T2 = 1024, SM_W2 = SM_T2 / 64, SM_RUN = SM_CHUNK / SM_T2; /* consecutive logits of a thread */
 constexpr int SM_BINS = 256;
 constexpr int SM_MAXC = (1 << 20) / SM_CHUNK; /* chunks of the longest row */
 constexpr int SM_LIST = 8192; /* members of a bin kept in LDS; a bin with more is read again */
-constexpr double SM_ONE = 0x1p40;
+constexpr int SM_RANK = 256;  /* members ranked by comparing all with all */
+constexpr int SM_DIGIT = SM_T2; /* values of a selection's digit */
+static_assert(SM_SLICE == SM_T2, "a wave's slice of a chunk is one logit a thread of sample_pick_k");
 
 /* What sample_scan_k leaves of one chunk. */
 struct Chunk {
-    unsigned long long mass[SM_BINS]; /* by bin, relative to the bin's lower edge, in 2^-40 */
+    unsigned long long mass[SM_BINS]; /* by bin, relative to the bin's lower edge, in 2^-40 (without a
+                                       * filter: the slices' masses, in 64-bit floating point) */
     double base;                      /* the top bin's number; without a filter the mass */
     unsigned long long key;           /* greedy rows: the first maximum's key */
     float max;                        /* -inf: nothing to choose in it */
@@ -46,7 +49,7 @@ struct Chunk {
 
 /* A row's parameters with every value outside its range read as "no filter". */
 struct Par {
-    double T, top_p, min_p;
+    double inv, min_p, top_p; /* inv = 8 / T */
     int top_k;
     bool greedy, filter;
 };
@@ -55,11 +58,10 @@ __device__ __forceinline__ Par sample_par(const nmx_sample_params *p, int vocab)
     Par r;
     const float T = p->temperature, tp = p->top_p, mp = p->min_p;
     r.greedy = !(T > 0.0f);
-    r.T = (double)T;
+    r.inv = T < INFINITY ? 8.0 / (double)T : 0x1p-1000; /* infinite: every finite logit alike */
     r.top_k = p->top_k > 0 && p->top_k < vocab ? p->top_k : 0;
     r.top_p = tp < 1.0f ? fmaxf(tp, 0.0f) : 1.0;
     r.min_p = mp > 0.0f ? fminf(mp, 1.0f) : 0.0;
-    if (!(T < INFINITY)) r.T = 0x1p1000; /* every finite logit alike */
     r.filter = !r.greedy && (r.top_k || r.top_p < 1.0 || r.min_p > 0.0);
     return r;
 }
@@ -78,12 +80,50 @@ __device__ __forceinline__ float sample_unkey(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-__device__ __forceinline__ double grid_pos(float x, double T) { return 8.0 * ((double)x / T); }
+__device__ __forceinline__ double grid_pos(float x, double inv) { return (double)x * inv; }
 
-/* the weight of x relative to the lower edge of its bin, in 2^-40 */
-__device__ __forceinline__ unsigned long long bin_mass(float x, double T) {
-    const double g = grid_pos(x, T);
-    return (unsigned long long)(exp((g - floor(g)) * 0.125) * SM_ONE + 0.5);
+/* e^z for z <= 0, right to 2^-43 (2^(k + f), |f| <= 1/2, by the Taylor polynomial of degree 10 of
+ * e^(f ln 2): the next term is below 2.1e-13 2^-1; the reduced argument's error is |z| 2^-52). What
+ * lies below e^-700 is 0. */
+__device__ __forceinline__ double exp_neg(double z) {
+    const double t = z * 1.4426950408889634074, k = rint(t), x = (t - k) * 0.69314718055994530942;
+    double p = 1.0 / 3628800;
+    p = __builtin_fma(p, x, 1.0 / 362880);
+    p = __builtin_fma(p, x, 1.0 / 40320);
+    p = __builtin_fma(p, x, 1.0 / 5040);
+    p = __builtin_fma(p, x, 1.0 / 720);
+    p = __builtin_fma(p, x, 1.0 / 120);
+    p = __builtin_fma(p, x, 1.0 / 24);
+    p = __builtin_fma(p, x, 1.0 / 6);
+    p = __builtin_fma(p, x, 0.5);
+    p = __builtin_fma(p, x, 1.0);
+    p = __builtin_fma(p, x, 1.0);
+    return z > -700.0 ? ldexp(p, (int)k) : 0.0;
+}
+/* the weight of v where the largest logit is mx */
+__device__ __forceinline__ double weight(float v, float mx, double inv) {
+    return exp_neg(((double)v - (double)mx) * inv * 0.125);
+}
+
+/* The weight of grid position g relative to the lower edge of its bin, in 2^-40, for fr = g - floor(g):
+ * 2^40 e^(fr / 8) about the bin's middle, degree 7 (the next term is below 6e-15), rounded to a whole
+ * number by the addition of 2^52. */
+__device__ __forceinline__ unsigned long long bin_mass_at(double fr) {
+    constexpr double M = 0x1p40 * 1.0644944589178594296; /* e^(1/16) */
+    const double x = (fr - 0.5) * 0.125;
+    double p = M / 5040;
+    p = __builtin_fma(p, x, M / 720);
+    p = __builtin_fma(p, x, M / 120);
+    p = __builtin_fma(p, x, M / 24);
+    p = __builtin_fma(p, x, M / 6);
+    p = __builtin_fma(p, x, M / 2);
+    p = __builtin_fma(p, x, M);
+    p = __builtin_fma(p, x, M);
+    return (unsigned long long)__double_as_longlong(p + 0x1p52) & 0xfffffffffffffull;
+}
+__device__ __forceinline__ unsigned long long bin_mass(float x, double inv) {
+    const double g = grid_pos(x, inv);
+    return bin_mass_at(g - floor(g));
 }
 
 __device__ __forceinline__ float block_max(float v, float *red, int waves) {
@@ -95,21 +135,18 @@ __device__ __forceinline__ float block_max(float v, float *red, int waves) {
     return v;
 }
 
-/* inclusive running sums over the workgroup's threads, in thread order; *total is the last */
+/* inclusive running sums over the SM_T2 threads, in thread order; *total is the last */
 template <typename V>
 __device__ __forceinline__ V block_scan(V v, V *red, V *total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const V o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+    const int w = threadIdx.x >> 6;
+    v = nmx_scan_wave(v);
     __syncthreads();
-    if (lane == 63) red[w] = v;
+    if ((threadIdx.x & 63) == 63) red[w] = v;
     __syncthreads();
     V before = 0, all = 0;
-    for (int i = 0; i < waves; i++) {
-        if (i < w) before += red[i];
+#pragma unroll
+    for (int i = 0; i < SM_W2; i++) {
+        if (i == w) before = all;
         all += red[i];
     }
     *total = all;
@@ -119,23 +156,33 @@ __device__ __forceinline__ V block_scan(V v, V *red, V *total) {
 __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__ logits, int stride,
                                                        int vocab, Chunk *__restrict__ work,
                                                        const nmx_sample_params *par, int par_step) {
-    __shared__ float redf[8];
-    __shared__ double redd[8];
-    __shared__ unsigned long long redk[8];
+    __shared__ float redf[SM_T1 / 64];
+    __shared__ double redd[SM_T1 / 64];
+    __shared__ unsigned long long redk[SM_T1 / 64];
     __shared__ uint32_t cnt[SM_BINS], wave_cnt[4];
     __shared__ unsigned long long mass[SM_BINS];
-    __shared__ uint16_t perm[SM_CHUNK];
-    const int tid = threadIdx.x, c = blockIdx.x, row = blockIdx.y;
-    const Par p = sample_par(par + (size_t)row * par_step, vocab);
+    __shared__ uint32_t perm2[SM_CHUNK / 2];
+    uint16_t *perm = (uint16_t *)perm2;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
     const float *l = logits + (size_t)row * stride + (size_t)c * SM_CHUNK;
     const int len = vocab - c * SM_CHUNK < SM_CHUNK ? vocab - c * SM_CHUNK : SM_CHUNK;
     Chunk *out = work + (size_t)row * gridDim.x + c;
+    /* a wave takes a slice of consecutive logits, 16 bytes a lane where the row allows it */
+    const bool vec = len == SM_CHUNK && ((uintptr_t)l & 15) == 0;
+    const int i0 = wave * SM_SLICE + (vec ? 4 * lane : lane);
+    auto index = [&](int u) { return i0 + (vec ? (u >> 2) * 256 + (u & 3) : u * 64); };
     float v[SM_PER];
+    if (vec) {
 #pragma unroll
-    for (int u = 0; u < SM_PER; u++) {
-        const int i = u * SM_T1 + tid;
-        v[u] = i < len ? l[i] : -INFINITY;
+        for (int u = 0; u < SM_PER; u += 4) {
+            const float4 x = *(const float4 *)(l + index(u));
+            v[u] = x.x, v[u + 1] = x.y, v[u + 2] = x.z, v[u + 3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < SM_PER; u++) v[u] = index(u) < len ? l[index(u)] : -INFINITY;
     }
+    const Par p = sample_par(par + (size_t)row * par_step, vocab);
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < SM_PER; u++) {
@@ -147,11 +194,11 @@ __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__
 #pragma unroll
         for (int u = 0; u < SM_PER; u++) {
             const unsigned long long k = (unsigned long long)sample_key(v[u]) << 32 |
-                                         (0xffffffffu - (uint32_t)(c * SM_CHUNK + u * SM_T1 + tid));
+                                         (0xffffffffu - (uint32_t)(c * SM_CHUNK + index(u)));
             if (v[u] > -INFINITY && k > best) best = k;
         }
         best = nmx_max_u64_wave(best);
-        if ((tid & 63) == 0) redk[tid >> 6] = best;
+        if (lane == 0) redk[wave] = best;
         __syncthreads();
         if (tid == 0) {
             for (int w = 1; w < SM_T1 / 64; w++) best = redk[w] > best ? redk[w] : best;
@@ -168,41 +215,41 @@ __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__
     if (!p.filter) {
         double s = 0.0;
 #pragma unroll
-        for (int u = 0; u < SM_PER; u++) s += exp(((double)v[u] - (double)mx) / p.T);
-        double total;
-        block_scan(s, redd, &total);
-        if (tid == 0) out->base = total;
+        for (int u = 0; u < SM_PER; u++) s += weight(v[u], mx, p.inv);
+        s = nmx_scan_wave(s);
+        if (lane == 63) redd[wave] = s, ((double *)out->mass)[wave] = s;
+        __syncthreads();
+        if (tid == 0) {
+            double total = 0.0;
+            for (int w = 0; w < SM_T1 / 64; w++) total += redd[w];
+            out->base = total;
+        }
         return;
     }
     if (tid < SM_BINS) cnt[tid] = 0, mass[tid] = 0;
     __syncthreads();
-    const double base = floor(grid_pos(mx, p.T));
+    const double base = floor(grid_pos(mx, p.inv));
     uint32_t at[SM_PER]; /* bin << 16 | rank; all ones: no weight */
 #pragma unroll
     for (int u = 0; u < SM_PER; u++) {
         at[u] = 0xffffffffu;
-        const double d = base - floor(grid_pos(v[u], p.T)); /* inf for -inf */
+        const double g = grid_pos(v[u], p.inv), fl = floor(g), d = base - fl; /* inf for -inf */
         if (d < (double)SM_BINS) {
             const uint32_t j = (uint32_t)(int)d;
             at[u] = j << 16 | atomicAdd(&cnt[j], 1u);
-            atomicAdd(&mass[j], bin_mass(v[u], p.T));
+            atomicAdd(&mass[j], bin_mass_at(g - fl));
         }
     }
     __syncthreads();
     uint32_t first = 0; /* members of the bins above bin tid */
     if (tid < SM_BINS) {
-        uint32_t x = cnt[tid];
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(x, d);
-            if ((tid & 63) >= d) x += o;
-        }
-        if ((tid & 63) == 63) wave_cnt[tid >> 6] = x;
+        const uint32_t x = nmx_scan_wave(cnt[tid]);
+        if (lane == 63) wave_cnt[wave] = x;
         first = x - cnt[tid];
     }
     __syncthreads();
     if (tid < SM_BINS) {
-        for (int w = 0; w < tid >> 6; w++) first += wave_cnt[w];
+        for (int w = 0; w < wave; w++) first += wave_cnt[w];
         out->start[tid] = (uint16_t)first;
         out->mass[tid] = mass[tid];
         if (tid == SM_BINS - 1) out->start[SM_BINS] = (uint16_t)(first + cnt[tid]);
@@ -212,27 +259,26 @@ __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < SM_PER; u++)
-        if (at[u] != 0xffffffffu) perm[cnt[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)(u * SM_T1 + tid);
+        if (at[u] != 0xffffffffu) perm[cnt[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)index(u);
     __syncthreads();
-    uint32_t *po = (uint32_t *)out->perm;
-    for (int i = tid; i < SM_CHUNK / 2; i += SM_T1) po[i] = ((const uint32_t *)perm)[i];
+    uint2 *po = (uint2 *)out->perm;
+    for (int i = tid; i < SM_CHUNK / 4; i += SM_T1) po[i] = ((const uint2 *)perm2)[i];
 }
 
 /* The row's state in sample_pick_k. */
 struct Pick {
     unsigned long long mass[SM_BINS];    /* the row's histogram, from its top bin down */
-    unsigned long long tally[SM_BINS];   /* masses of a selection's digit */
-    double chunk_mass[SM_MAXC];
-    double redd[16];
-    float redf[16];
-    uint32_t cnt[SM_BINS], digit[SM_BINS], redu[16];
+    unsigned long long tally[SM_DIGIT];  /* masses of a selection's digit */
+    unsigned long long cand[SM_MAXC];    /* masses of a bin's kept members by chunk */
+    unsigned long long redk[SM_W2], small_mass[SM_RANK], sel_m;
+    double edge[SM_BINS];                /* e^(-b / 8): bin b's lower edge, the top bin's being 1 */
+    double chunk_mass[SM_MAXC], redd[SM_W2], sel_d;
+    float redf[SM_W2];
+    uint32_t cnt[SM_BINS], digit[SM_DIGIT], redu[SM_W2];
     int off[SM_MAXC];                    /* the chunk's top bin below the row's */
     uint32_t seg[SM_MAXC + 1];           /* running sizes of a bin's segments */
     uint32_t ties[SM_MAXC];
-    unsigned long long cand[SM_MAXC];    /* masses of a bin's kept members by chunk */
-    unsigned long long redk[16], sel_m;
-    double sel_d;
-    uint32_t sel_n;
+    uint32_t small[SM_RANK], sel_n, sel_k;
     int hit, last;
     uint32_t list[SM_LIST];
 };
@@ -242,104 +288,153 @@ struct Cut {
     uint32_t key, ties;
 };
 
+/* A row as sample_pick_k sees it. */
+struct Row {
+    const Chunk *ch;
+    const float *l;
+    int C;
+    double inv, top; /* top: the row's top bin */
+};
+
 /* The members of row bin b as i = 0 .. S.seg[C] - 1: chunk and key of one. */
-__device__ __forceinline__ uint32_t member(const Pick &S, const Chunk *ch, const float *l, int C, int b,
-                                           uint32_t i, int *c_out) {
-    int lo = 0, hi = C; /* the last chunk whose segment starts at or before i */
+__device__ __forceinline__ uint32_t member(const Pick &S, const Row &r, int b, uint32_t i, int *c_out) {
+    int lo = 0, hi = r.C; /* the last chunk whose segment starts at or before i */
     while (hi - lo > 1) {
         const int m = (lo + hi) >> 1;
         if (S.seg[m] <= i) lo = m;
         else hi = m;
     }
     *c_out = lo;
-    const Chunk &k = ch[lo];
+    const Chunk &k = r.ch[lo];
     const int at = k.perm[k.start[b - S.off[lo]] + (i - S.seg[lo])];
-    return sample_key(sample_value(l[(size_t)lo * SM_CHUNK + at]));
+    return sample_key(sample_value(r.l[(size_t)lo * SM_CHUNK + at]));
 }
 
 /* Running sizes of bin b's segments over the chunks; the keys into the list if they fit. */
-__device__ void open_bin(Pick &S, const Chunk *ch, const float *l, int C, int b) {
+__device__ void open_bin(Pick &S, const Row &r, int b) {
     const int tid = threadIdx.x;
     __syncthreads();
     uint32_t x = 0;
-    if (tid < C) {
+    if (tid < r.C) {
         const int j = b - S.off[tid];
-        if (j >= 0 && j < SM_BINS) x = (uint32_t)ch[tid].start[j + 1] - ch[tid].start[j];
+        if (j >= 0 && j < SM_BINS) x = (uint32_t)r.ch[tid].start[j + 1] - r.ch[tid].start[j];
     }
     uint32_t total;
     const uint32_t incl = block_scan(x, S.redu, &total);
-    if (tid < C) S.seg[tid] = incl - x;
-    if (tid == 0) S.seg[C] = total;
+    if (tid < r.C) S.seg[tid] = incl - x;
+    if (tid == 0) S.seg[r.C] = total;
     __syncthreads();
     if (total <= SM_LIST)
         for (uint32_t i = tid; i < total; i += SM_T2) {
             int c;
-            S.list[i] = member(S, ch, l, C, b, i, &c);
+            S.list[i] = member(S, r, b, i, &c);
         }
     __syncthreads();
 }
 
 /* Among the members of the opened bin b with keys of at least floor_key: the key at which the run in
  * descending order reaches `want` members (by count) or the mass want_mass (in 2^-40 of the bin's
- * lower edge). above / above_mass: what lies strictly above that key. Four digits of 8 bits. */
-__device__ uint32_t select_key(Pick &S, const Chunk *ch, const float *l, int C, int b, double T,
-                               bool by_count, uint32_t want, double want_mass, uint32_t floor_key,
-                               uint32_t *above, double *above_mass) {
+ * lower edge). above / above_mass: what lies strictly above that key. Digits of 10 bits of the keys
+ * that the bin spans, until few enough are left to compare all with all. */
+__device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint32_t want, double want_mass,
+                               uint32_t floor_key, uint32_t *above, double *above_mass) {
     const int tid = threadIdx.x;
-    const uint32_t total = S.seg[C];
-    uint32_t prefix = 0, n_above = 0;
+    const uint32_t total = S.seg[r.C];
+    /* the bin's keys lie between those of its edges (one bin wider: the product's rounding) */
+    const double lo_x = (r.top - b - 1.0) / r.inv, hi_x = (r.top - b + 2.0) / r.inv, most = 3.40282346638528859e+38;
+    uint32_t klo = sample_key((float)fmin(fmax(lo_x, -most), most)), khi = sample_key((float)fmin(fmax(hi_x, -most), most));
+    klo = klo < floor_key ? floor_key : klo;
+    uint32_t n_above = 0, left = total;
     unsigned long long m_above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    auto key_of = [&](uint32_t i) {
+        int c;
+        return total <= SM_LIST ? S.list[i] : member(S, r, b, i, &c);
+    };
+    while (left > SM_RANK && klo < khi) {
+        const int bits = 32 - __clz((int)(khi - klo)), shift = bits > 10 ? bits - 10 : 0;
         __syncthreads();
-        if (tid < SM_BINS) S.digit[tid] = 0, S.tally[tid] = 0;
-        if (tid == 0) S.hit = -1, S.last = -1;
+        S.digit[tid] = 0, S.tally[tid] = 0;
+        if (tid == 0) S.hit = SM_DIGIT, S.last = 0;
         __syncthreads();
         for (uint32_t i = tid; i < total; i += SM_T2) {
-            int c;
-            const uint32_t k = total <= SM_LIST ? S.list[i] : member(S, ch, l, C, b, i, &c);
-            if (k < floor_key || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
-            const uint32_t d = 255 - ((k >> shift) & 255);
+            const uint32_t k = key_of(i);
+            if (k < klo || k > khi) continue;
+            const uint32_t d = (khi - k) >> shift;
             atomicAdd(&S.digit[d], 1u);
-            if (!by_count) atomicAdd(&S.tally[d], bin_mass(sample_unkey(k), T));
+            if (!by_count) atomicAdd(&S.tally[d], bin_mass(sample_unkey(k), r.inv));
         }
         __syncthreads();
-        const uint32_t n = tid < SM_BINS ? S.digit[tid] : 0;
-        const unsigned long long m = tid < SM_BINS ? S.tally[tid] : 0;
+        const uint32_t n = S.digit[tid];
+        const unsigned long long m = S.tally[tid];
         uint32_t n_all;
-        unsigned long long m_all;
+        unsigned long long m_all = 0, m_to = 0;
         const uint32_t n_to = n_above + block_scan(n, S.redu, &n_all);
-        const unsigned long long m_to = m_above + block_scan(m, S.redk, &m_all);
-        if (n) {
+        if (!by_count) m_to = m_above + block_scan(m, S.redk, &m_all);
+        if (n) { /* the first digit that reaches the want; the last one where a rounding keeps it from any */
             atomicMax(&S.last, tid);
-            const bool reached = by_count ? n_to >= want : (double)m_to >= want_mass;
-            const bool before = by_count ? n_to - n >= want : (double)(m_to - m) >= want_mass;
-            if (reached && !before) S.hit = tid; /* one digit at most */
+            if (by_count ? n_to >= want : (double)m_to >= want_mass) atomicMin(&S.hit, tid);
         }
         __syncthreads();
-        /* a mass that a rounding keeps from being reached: the last digit. One that is reached at
-         * nothing (want_mass 0): the first */
-        int hit = S.hit;
-        if (hit < 0) hit = !by_count && want_mass <= (double)m_above ? -2 : S.last;
+        const int hit = S.hit < SM_DIGIT ? S.hit : S.last;
+        if (tid == hit) S.sel_n = n_to - n, S.sel_k = n, S.sel_m = m_to - m;
         __syncthreads();
-        if (hit == -2 && n && n_to - n == n_above) S.hit = tid; /* the first digit with members */
-        if (hit >= 0 && tid == 0) S.hit = hit;
-        __syncthreads();
-        hit = S.hit;
-        if (tid == hit) S.sel_n = n_to - n, S.sel_m = m_to - m;
-        __syncthreads();
-        prefix = prefix << 8 | (uint32_t)(255 - hit);
-        n_above = S.sel_n;
-        m_above = S.sel_m;
+        n_above = S.sel_n, left = S.sel_k, m_above = S.sel_m;
+        khi -= (uint32_t)hit << shift;
+        const uint32_t low = shift ? khi - ((1u << shift) - 1) : khi;
+        klo = low > klo && low <= khi ? low : klo;
     }
-    *above = n_above;
-    *above_mass = (double)m_above;
-    return prefix;
+    __syncthreads();
+    if (klo == khi) { /* all that is left are ties */
+        *above = n_above, *above_mass = (double)m_above;
+        return khi;
+    }
+    if (tid == 0) S.sel_n = 0, S.last = -1;
+    __syncthreads();
+    for (uint32_t i = tid; i < total; i += SM_T2) {
+        const uint32_t k = key_of(i);
+        if (k < klo || k > khi) continue;
+        const uint32_t at = atomicAdd(&S.sel_n, 1u);
+        S.small[at] = k; /* at < left <= SM_RANK */
+        S.small_mass[at] = by_count ? 0 : bin_mass(sample_unkey(k), r.inv);
+    }
+    __syncthreads();
+    const uint32_t N = S.sel_n;
+    uint32_t k = 0, gt = 0, eq = 0;
+    unsigned long long gm = 0, em = 0;
+    if ((uint32_t)tid < N) {
+        k = S.small[tid];
+#pragma unroll 8
+        for (uint32_t i = 0; i < N; i++) {
+            const uint32_t o = S.small[i];
+            const unsigned long long w = S.small_mass[i];
+            if (o > k) gt++, gm += w;
+            if (o == k) eq++, em += w;
+        }
+    }
+    /* the greatest key whose run reaches the want; the least where none does */
+    if (tid == 0) S.sel_k = 0;
+    __syncthreads();
+    if ((uint32_t)tid < N && (by_count ? n_above + gt + eq >= want : (double)(m_above + gm + em) >= want_mass)) atomicMax(&S.sel_k, k);
+    __syncthreads();
+    uint32_t key = S.sel_k;
+    __syncthreads();
+    if (key == 0) {
+        if (tid == 0) S.sel_k = 0xffffffffu;
+        __syncthreads();
+        if ((uint32_t)tid < N) atomicMin(&S.sel_k, k);
+        __syncthreads();
+        key = S.sel_k;
+    }
+    if ((uint32_t)tid < N && k == key) S.sel_n = n_above + gt, S.sel_m = m_above + gm; /* the same of each tie */
+    __syncthreads();
+    *above = S.sel_n, *above_mass = (double)S.sel_m;
+    return key;
 }
 
 /* The least logit whose weight is at least min_p of the largest: its key. */
-__device__ uint32_t min_p_key(float mx, double T, double min_p) {
-    auto in = [&](float x) { return exp(((double)x - (double)mx) / T) >= min_p; };
-    uint32_t k = sample_key(sample_value((float)fmax((double)mx + T * log(min_p), -3.40282346638528859e+38)));
+__device__ uint32_t min_p_key(float mx, double inv, double min_p) {
+    auto in = [&](float x) { return weight(x, mx, inv) >= min_p; };
+    uint32_t k = sample_key(sample_value((float)fmax((double)mx + 8.0 * log(min_p) / inv, -3.40282346638528859e+38)));
     const uint32_t top = sample_key(mx), low = sample_key(-3.40282347e+38f);
     if (k > top) k = top;
     while (k < top && !in(sample_unkey(k))) k++;
@@ -354,10 +449,13 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
                                                        int32_t *__restrict__ tok,
                                                        float *__restrict__ prob) {
     __shared__ Pick S;
-    const int tid = threadIdx.x, row = blockIdx.x;
-    const Par p = sample_par(par + (size_t)row * par_step, vocab);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
     const float *l = logits + (size_t)row * stride;
     const Chunk *ch = work + (size_t)row * C;
+    const float mc = tid < C ? ch[tid].max : -INFINITY; /* garbage in a greedy row, and not used there */
+    const double bc = tid < C ? ch[tid].base : 0.0;
+    const float u = uni[row];
+    const Par p = sample_par(par + (size_t)row * par_step, vocab);
     auto answer = [&](int t, double pr) {
         tok[row] = t;
         if (prob) prob[row] = (float)pr;
@@ -371,10 +469,8 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
         }
         return;
     }
-    const float u = uni[row];
     const double ud = u > 0.0f ? (double)fminf(u, 1.0f) : 0.0;
-    const float mc = tid < C ? ch[tid].max : -INFINITY;
-    const float mx = block_max(mc, S.redf, SM_T2 / 64);
+    const float mx = block_max(mc, S.redf, SM_W2);
     if (!(mx > -INFINITY)) { /* nothing to choose from */
         if (tid == 0) answer(-1, 0.0);
         return;
@@ -382,31 +478,36 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
     Cut cut = {0, 0xffffffffu};
     double mass = 0.0; /* chunk tid's kept mass, the largest weight being 1 */
     if (!p.filter) {
-        if (tid < C && mc > -INFINITY) mass = ch[tid].base * exp(((double)mc - (double)mx) / p.T);
+        if (tid < C && mc > -INFINITY) mass = bc * weight(mc, mx, p.inv);
     } else {
-        const double g_top = grid_pos(mx, p.T), top = floor(g_top);
-        const double unit = exp((top - g_top) * 0.125) / SM_ONE; /* a mass of the top bin, as a weight */
+        const double g_top = grid_pos(mx, p.inv), top = floor(g_top);
+        const Row r = {ch, l, C, p.inv, top};
         if (tid < C) {
-            const double d = mc > -INFINITY ? top - ch[tid].base : (double)SM_BINS;
+            const double d = mc > -INFINITY ? top - bc : (double)SM_BINS;
             S.off[tid] = d < (double)SM_BINS ? (int)d : SM_BINS;
             S.cand[tid] = 0, S.ties[tid] = 0;
         }
-        if (tid < SM_BINS) S.cnt[tid] = 0, S.mass[tid] = 0;
+        if (tid < SM_BINS) S.cnt[tid] = 0, S.mass[tid] = 0, S.edge[tid] = exp_neg(-0.125 * tid);
         __syncthreads();
-        const int b = tid & (SM_BINS - 1);
-        {
-            uint32_t n = 0;
-            unsigned long long m = 0;
-            for (int c = tid / SM_BINS; c < C; c += SM_T2 / SM_BINS) {
-                const int j = b - S.off[c];
-                if (j < 0) continue;
-                n += (uint32_t)ch[c].start[j + 1] - ch[c].start[j];
-                m += ch[c].mass[j];
+#pragma unroll 2
+        for (int c = wave; c < C; c += SM_W2) { /* a wave adds a chunk's histogram */
+            const int off = S.off[c];
+            uint32_t n[4];
+            unsigned long long m[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int j = lane + 64 * q;
+                const bool in = j + off < SM_BINS;
+                n[q] = in ? (uint32_t)ch[c].start[j + 1] - ch[c].start[j] : 0;
+                m[q] = in ? ch[c].mass[j] : 0;
             }
-            if (n) atomicAdd(&S.cnt[b], n), atomicAdd(&S.mass[b], m);
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                if (n[q]) atomicAdd(&S.cnt[lane + 64 * q + off], n[q]), atomicAdd(&S.mass[lane + 64 * q + off], m[q]);
         }
         __syncthreads();
-        const double edge = exp(-0.125 * b);
+        const int b = tid & (SM_BINS - 1);
+        const double edge = S.edge[b];
         int kb = SM_BINS;     /* the bin that top-k ends in */
         double k_mass = 0.0;  /* and the mass that it keeps of it, in 2^-40 of its lower edge */
         if (p.top_k) {
@@ -418,21 +519,24 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
                 __syncthreads();
                 kb = S.hit;
                 const uint32_t want = S.sel_n;
-                open_bin(S, ch, l, C, kb);
+                open_bin(S, r, kb);
                 uint32_t above;
                 double unused;
-                cut.key = select_key(S, ch, l, C, kb, p.T, true, want, 0.0, 0, &above, &unused);
+                cut.key = select_key(S, r, kb, true, want, 0.0, 0, &above, &unused);
                 cut.ties = want - above;
-                unsigned long long kept = 0, whole;
-                for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
-                    int c;
-                    const uint32_t key = S.seg[C] <= SM_LIST ? S.list[i] : member(S, ch, l, C, kb, i, &c);
-                    if (key > cut.key) kept += bin_mass(sample_unkey(key), p.T);
+                if (p.top_p < 1.0) {
+                    unsigned long long kept = 0, whole;
+                    for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
+                        int c;
+                        const uint32_t key = S.seg[C] <= SM_LIST ? S.list[i] : member(S, r, kb, i, &c);
+                        if (key > cut.key) kept += bin_mass(sample_unkey(key), p.inv);
+                    }
+                    block_scan(kept, S.redk, &whole);
+                    k_mass = (double)whole + (double)cut.ties * (double)bin_mass(sample_unkey(cut.key), p.inv);
                 }
-                block_scan(kept, S.redk, &whole);
-                k_mass = (double)whole + (double)cut.ties * (double)bin_mass(sample_unkey(cut.key), p.T);
             }
         }
+        int opened = kb;
         if (p.top_p < 1.0) { /* over what top-k left */
             double mine = 0.0, whole;
             if (tid < SM_BINS) mine = (b < kb ? (double)S.mass[b] : b == kb ? k_mass : 0.0) * edge;
@@ -449,60 +553,58 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
             if (tid == pb) S.sel_d = fmax(want - (to - mine), 0.0) / edge;
             __syncthreads();
             const double rest = S.sel_d;
-            if (pb != kb) open_bin(S, ch, l, C, pb);
+            if (pb != kb) open_bin(S, r, pb);
+            opened = pb;
             uint32_t above;
             double m_above;
-            const uint32_t key = select_key(S, ch, l, C, pb, p.T, false, 0, rest, pb == kb ? cut.key : 0,
-                                            &above, &m_above);
-            const double need = ceil((rest - m_above) / (double)bin_mass(sample_unkey(key), p.T));
+            const uint32_t key = select_key(S, r, pb, false, 0, rest, pb == kb ? cut.key : 0, &above, &m_above);
+            const double need = ceil((rest - m_above) / (double)bin_mass(sample_unkey(key), p.inv));
             uint32_t ties = need < 1.0 ? 1u : need < 4e9 ? (uint32_t)need : 0xffffffffu;
             if (pb == kb && key == cut.key && cut.ties < ties) ties = cut.ties;
             cut.key = key, cut.ties = ties;
         }
         if (p.min_p > 0.0) {
-            if (tid == 0) S.sel_n = min_p_key(mx, p.T, p.min_p);
+            __syncthreads();
+            if (tid == 0) S.sel_n = min_p_key(mx, p.inv, p.min_p);
             __syncthreads();
             if (S.sel_n > cut.key) cut.key = S.sel_n, cut.ties = 0xffffffffu;
         }
         /* the kept mass of each chunk: whole bins, then the members of the cut's own bin */
-        const double d = cut.key ? top - floor(grid_pos(sample_unkey(cut.key), p.T)) : (double)SM_BINS;
+        const double d = cut.key ? top - floor(grid_pos(sample_unkey(cut.key), p.inv)) : (double)SM_BINS;
         const int cb = d < (double)SM_BINS ? (int)d : SM_BINS;
         if (cb < SM_BINS) {
-            open_bin(S, ch, l, C, cb);
+            if (cb != opened) open_bin(S, r, cb);
             for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
                 int c;
-                const uint32_t key = member(S, ch, l, C, cb, i, &c);
+                const uint32_t key = member(S, r, cb, i, &c);
                 if (key == cut.key) atomicAdd(&S.ties[c], 1u);
-                else if (key > cut.key) atomicAdd(&S.cand[c], bin_mass(sample_unkey(key), p.T));
+                else if (key > cut.key) atomicAdd(&S.cand[c], bin_mass(sample_unkey(key), p.inv));
             }
+        }
+        for (int c = wave; c < C; c += SM_W2) { /* a wave adds a chunk's whole bins, in a fixed order */
+            const int n = cb - S.off[c];
+            double s = 0.0;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int j = lane + 64 * q;
+                if (j < n) s += (double)ch[c].mass[j] * S.edge[j + S.off[c]];
+            }
+            s = nmx_scan_wave(s);
+            if (lane == 63) S.chunk_mass[c] = s;
         }
         __syncthreads();
         uint32_t all;
         const uint32_t mine = tid < C ? S.ties[tid] : 0, to = block_scan(mine, S.redu, &all), before = to - mine;
         const uint32_t ties = before >= cut.ties ? 0 : cut.ties - before < mine ? cut.ties - before : mine;
-        if (tid < C) S.ties[tid] = ties;
-        /* a chunk's whole bins: 8 lanes take every 8th, joined in a fixed order */
-        for (int c0 = 0; c0 < C; c0 += SM_T2 / 8) {
-            const int c = c0 + (tid >> 3);
-            double s = 0.0;
-            if (c < C) {
-                const int n = cb - S.off[c];
-                for (int j = tid & 7; j < n; j += 8) s += (double)ch[c].mass[j] * exp(-0.125 * (j + S.off[c]));
-            }
-            s += __shfl_xor(s, 1);
-            s += __shfl_xor(s, 2);
-            s += __shfl_xor(s, 4);
-            if (c < C && (tid & 7) == 0) S.chunk_mass[c] = s;
-        }
-        __syncthreads();
         if (tid < C) {
+            S.ties[tid] = ties;
             mass = S.chunk_mass[tid];
             if (cb < SM_BINS) {
                 double m = (double)S.cand[tid];
-                if (ties) m += (double)ties * (double)bin_mass(sample_unkey(cut.key), p.T);
-                mass += m * exp(-0.125 * cb);
+                if (ties) m += (double)ties * (double)bin_mass(sample_unkey(cut.key), p.inv);
+                mass += m * S.edge[cb];
             }
-            mass *= unit;
+            mass *= exp_neg((top - g_top) * 0.125) * 0x1p-40; /* a mass of the top bin, as a weight */
         }
     }
     /* the chunk that the draw falls into */
@@ -510,7 +612,7 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
     const double to = block_scan(mass, S.redd, &whole), goal = ud * whole;
     if (tid == 0) S.hit = SM_T2, S.last = 0;
     __syncthreads();
-    if (mass > 0.0) {
+    if (mass > 1e-296) { /* so that one of its slices has 1e-297, and one logit a weight of 1e-300 */
         atomicMax(&S.last, tid);
         if (to > goal) atomicMin(&S.hit, tid);
     }
@@ -518,15 +620,32 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
     const int c = S.hit < SM_T2 ? S.hit : S.last;
     if (tid == c) S.sel_d = to - mass;
     __syncthreads();
-    const double rest = goal - S.sel_d;
-    /* its logits, 8 consecutive ones to a thread */
-    const int len = vocab - c * SM_CHUNK < SM_CHUNK ? vocab - c * SM_CHUNK : SM_CHUNK, i0 = tid * SM_RUN;
+    double rest = goal - S.sel_d;
+    const int len = vocab - c * SM_CHUNK < SM_CHUNK ? vocab - c * SM_CHUNK : SM_CHUNK;
     const float *lc = l + (size_t)c * SM_CHUNK;
+    /* without a filter the scan left the masses of the chunk's slices: one logit to a thread; else 8
+     * consecutive ones of the chunk */
+    const int per = p.filter ? SM_RUN : 1;
+    int i0 = tid * per;
+    if (!p.filter) {
+        const float mcc = ch[c].max;
+        const double up = weight(mcc, mx, p.inv);
+        double at = -1.0, run = 0.0;
+        int slice = 0;
+#pragma unroll
+        for (int w = 0; w < SM_CHUNK / SM_SLICE; w++) { /* every thread the same few sums */
+            const double m = ((const double *)ch[c].mass)[w] * up;
+            if (m > 1e-297 && (run <= rest || at < 0.0)) slice = w, at = run; /* the last one that starts at or before */
+            run += m;
+        }
+        rest -= at;
+        i0 += slice * SM_SLICE;
+    }
     float x[SM_RUN];
     uint32_t key[SM_RUN], same = 0;
 #pragma unroll
     for (int e = 0; e < SM_RUN; e++) {
-        x[e] = i0 + e < len ? sample_value(lc[i0 + e]) : -INFINITY;
+        x[e] = e < per && i0 + e < len ? sample_value(lc[i0 + e]) : -INFINITY;
         key[e] = sample_key(x[e]);
         same += x[e] > -INFINITY && key[e] == cut.key;
     }
@@ -539,9 +658,11 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
     double w[SM_RUN], s = 0.0;
 #pragma unroll
     for (int e = 0; e < SM_RUN; e++) {
+        w[e] = 0.0;
+        if (e >= per) continue;
         bool keep = x[e] > -INFINITY && key[e] >= cut.key;
         if (p.filter && keep && key[e] == cut.key) keep = rank++ < allowed;
-        w[e] = keep ? exp(((double)x[e] - (double)mx) / p.T) : 0.0;
+        if (keep) w[e] = weight(x[e], mx, p.inv);
         s += w[e];
     }
     double in_chunk;
@@ -563,10 +684,10 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
     }
     __syncthreads();
     const int at = S.hit < SM_CHUNK ? S.hit : S.last; /* a whole missed by a rounding: the last one */
-    if (at / SM_RUN == tid) {
+    if (at >= i0 && at < i0 + per) {
         double mine = 0.0;
 #pragma unroll
-        for (int e = 0; e < SM_RUN; e++) mine = e == at % SM_RUN ? w[e] : mine;
+        for (int e = 0; e < SM_RUN; e++) mine = e == at - i0 ? w[e] : mine;
         answer(c * SM_CHUNK + at, mine / whole);
     }
 }

@@ -30,8 +30,9 @@ constexpr int SM_T1 = 512, SM_PER = SM_CHUNK / SM_T1, SM_SLICE = SM_CHUNK / (SM_
 constexpr int SM_T2 = 1024, SM_W2 = SM_T2 / 64, SM_RUN = SM_CHUNK / SM_T2; /* consecutive logits of a thread */
 constexpr int SM_BINS = 256;
 constexpr int SM_MAXC = (1 << 20) / SM_CHUNK; /* chunks of the longest row */
-constexpr int SM_LIST = 8192; /* members of a bin kept in LDS; a bin with more is read again */
-constexpr int SM_RANK = 256;  /* members ranked by comparing all with all */
+constexpr int SM_LIST = 16384; /* members of a bin kept in LDS; a bin with more is read again */
+constexpr int SM_RANK = 256;   /* members of a bin ranked by comparing all with all */
+constexpr int SM_FEW = 512;    /* tokens among which a row is decided in LDS altogether */
 constexpr int SM_DIGIT = SM_T2; /* values of a selection's digit */
 static_assert(SM_SLICE == SM_T2, "a wave's slice of a chunk is one logit a thread of sample_pick_k");
 
@@ -43,8 +44,8 @@ struct Chunk {
     unsigned long long key;           /* greedy rows: the first maximum's key */
     float max;                        /* -inf: nothing to choose in it */
     uint32_t pad;
-    uint16_t start[SM_BINS + 8];      /* bin j's members: perm[start[j] .. start[j + 1]) */
-    uint16_t perm[SM_CHUNK];
+    uint32_t seg[SM_BINS];            /* bin j's members: perm[seg & 0xffff ..], seg >> 16 of them */
+    uint16_t perm[SM_CHUNK];          /* the chunk's indices, from its top bin down */
 };
 
 /* A row's parameters with every value outside its range read as "no filter". */
@@ -135,10 +136,12 @@ __device__ __forceinline__ float block_max(float v, float *red, int waves) {
     return v;
 }
 
-/* inclusive running sums over the SM_T2 threads, in thread order; *total is the last */
+/* inclusive running sums over the SM_T2 threads, in thread order; *total is the last. red: SM_W2 words
+ * that nothing else uses meanwhile. */
 template <typename V>
-__device__ __forceinline__ V block_scan(V v, V *red, V *total) {
+__device__ __forceinline__ V block_scan(V v, unsigned long long *red8, V *total) {
     const int w = threadIdx.x >> 6;
+    V *red = (V *)red8;
     v = nmx_scan_wave(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) red[w] = v;
@@ -153,6 +156,22 @@ __device__ __forceinline__ V block_scan(V v, V *red, V *total) {
     return before + v;
 }
 
+/* The first and the last thread for which a truth holds (SM_T2 and -1: none), known to all. */
+__device__ __forceinline__ void block_find(bool first_of, bool last_of, unsigned long long *red1,
+                                           unsigned long long *red2, int *first, int *last) {
+    const unsigned long long a = __ballot(first_of), b = __ballot(last_of);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red1[threadIdx.x >> 6] = a, red2[threadIdx.x >> 6] = b;
+    __syncthreads();
+    /* lane w of every wave looks at wave w's word */
+    const int lane = threadIdx.x & 63, at = lane & (SM_W2 - 1);
+    const unsigned long long x = red1[at], y = red2[at], low = (1ull << SM_W2) - 1;
+    const unsigned long long mx = __ballot(x != 0) & low, my = __ballot(y != 0) & low;
+    const int f = __ffsll((long long)x) - 1, l = 63 - __clzll((long long)y);
+    *first = mx ? 64 * (__ffsll((long long)mx) - 1) + __builtin_amdgcn_readlane(f, __ffsll((long long)mx) - 1) : SM_T2;
+    *last = my ? 64 * (63 - __clzll((long long)my)) + __builtin_amdgcn_readlane(l, 63 - __clzll((long long)my)) : -1;
+}
+
 __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__ logits, int stride,
                                                        int vocab, Chunk *__restrict__ work,
                                                        const nmx_sample_params *par, int par_step) {
@@ -162,6 +181,7 @@ __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__
     __shared__ uint32_t cnt[SM_BINS], wave_cnt[4];
     __shared__ unsigned long long mass[SM_BINS];
     __shared__ uint32_t perm2[SM_CHUNK / 2];
+    __shared__ float val[SM_CHUNK / 16 * 17]; /* the logits in grouped order, a word skipped every 16 */
     uint16_t *perm = (uint16_t *)perm2;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
     const float *l = logits + (size_t)row * stride + (size_t)c * SM_CHUNK;
@@ -180,7 +200,9 @@ __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__
         }
     } else {
 #pragma unroll
-        for (int u = 0; u < SM_PER; u++) v[u] = index(u) < len ? l[index(u)] : -INFINITY;
+        for (int u = 0; u < SM_PER; u++) v[u] = l[index(u) < len ? index(u) : len - 1]; /* no branch around a request */
+#pragma unroll
+        for (int u = 0; u < SM_PER; u++) v[u] = index(u) < len ? v[u] : -INFINITY;
     }
     const Par p = sample_par(par + (size_t)row * par_step, vocab);
     float mx = -INFINITY;
@@ -233,54 +255,87 @@ __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__
 #pragma unroll
     for (int u = 0; u < SM_PER; u++) {
         at[u] = 0xffffffffu;
-        const double g = grid_pos(v[u], p.inv), fl = floor(g), d = base - fl; /* inf for -inf */
+        const double d = base - floor(grid_pos(v[u], p.inv)); /* inf for -inf */
         if (d < (double)SM_BINS) {
             const uint32_t j = (uint32_t)(int)d;
             at[u] = j << 16 | atomicAdd(&cnt[j], 1u);
-            atomicAdd(&mass[j], bin_mass_at(g - fl));
         }
     }
     __syncthreads();
-    uint32_t first = 0; /* members of the bins above bin tid */
+    uint32_t first = 0, mine = 0; /* members of the bins above bin tid, and of it */
     if (tid < SM_BINS) {
-        const uint32_t x = nmx_scan_wave(cnt[tid]);
+        mine = cnt[tid];
+        const uint32_t x = nmx_scan_wave(mine);
         if (lane == 63) wave_cnt[wave] = x;
-        first = x - cnt[tid];
+        first = x - mine;
     }
     __syncthreads();
+    const uint32_t members = wave_cnt[0] + wave_cnt[1] + wave_cnt[2] + wave_cnt[3];
     if (tid < SM_BINS) {
         for (int w = 0; w < wave; w++) first += wave_cnt[w];
-        out->start[tid] = (uint16_t)first;
-        out->mass[tid] = mass[tid];
-        if (tid == SM_BINS - 1) out->start[SM_BINS] = (uint16_t)(first + cnt[tid]);
+        out->seg[tid] = first | mine << 16;
         cnt[tid] = first;
     }
     if (tid == 0) out->base = base;
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < SM_PER; u++)
-        if (at[u] != 0xffffffffu) perm[cnt[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)index(u);
+    for (int u = 0; u < SM_PER; u++) {
+        if (at[u] == 0xffffffffu) continue;
+        const uint32_t to = cnt[at[u] >> 16] + (at[u] & 0xffffu);
+        perm[to] = (uint16_t)index(u);
+        val[to + (to >> 4)] = v[u];
+    }
     __syncthreads();
     uint2 *po = (uint2 *)out->perm;
-    for (int i = tid; i < SM_CHUNK / 4; i += SM_T1) po[i] = ((const uint2 *)perm2)[i];
+    for (uint32_t i = tid; 4 * i < members; i += SM_T1) po[i] = ((const uint2 *)perm2)[i];
+    /* masses: neighbours in the grouped order mostly share a bin, so a thread of 16 consecutive ones adds
+     * to the bins' sums once or twice instead of 16 times */
+    unsigned long long sum = 0;
+    int bin = -1;
+#pragma unroll
+    for (int u = 0; u < SM_PER; u++) {
+        const uint32_t i = (uint32_t)tid * SM_PER + u;
+        if (i >= members) break;
+        const double g = grid_pos(val[17 * tid + u], p.inv), fl = floor(g);
+        const int j = (int)(base - fl);
+        if (j != bin) {
+            if (bin >= 0) atomicAdd(&mass[bin], sum);
+            sum = 0, bin = j;
+        }
+        sum += bin_mass_at(g - fl);
+    }
+    if (bin >= 0) atomicAdd(&mass[bin], sum);
+    __syncthreads();
+    if (tid < SM_BINS) out->mass[tid] = mass[tid];
 }
 
 /* The row's state in sample_pick_k. */
 struct Pick {
     unsigned long long mass[SM_BINS];    /* the row's histogram, from its top bin down */
-    unsigned long long tally[SM_DIGIT];  /* masses of a selection's digit */
     unsigned long long cand[SM_MAXC];    /* masses of a bin's kept members by chunk */
-    unsigned long long redk[SM_W2], small_mass[SM_RANK], sel_m;
+    unsigned long long red1[SM_W2], red2[SM_W2], sel_m;
     double edge[SM_BINS];                /* e^(-b / 8): bin b's lower edge, the top bin's being 1 */
-    double chunk_mass[SM_MAXC], redd[SM_W2], sel_d;
+    double chunk_mass[SM_MAXC], sel_d;
     float redf[SM_W2];
-    uint32_t cnt[SM_BINS], digit[SM_DIGIT], redu[SM_W2];
+    uint32_t cnt[SM_BINS];
     int off[SM_MAXC];                    /* the chunk's top bin below the row's */
-    uint32_t seg[SM_MAXC + 1];           /* running sizes of a bin's segments */
+    uint32_t seg[SM_MAXC + 1];           /* running sizes of the segments of the members in hand */
+    uint32_t at[SM_MAXC];                /* where a chunk's segment begins in its order */
     uint32_t ties[SM_MAXC];
-    uint32_t small[SM_RANK], sel_n, sel_k;
-    int hit, last;
-    uint32_t list[SM_LIST];
+    uint32_t sel_n, sel_k;
+    int hit;
+    union {
+        struct {
+            unsigned long long tally[SM_DIGIT], part_m[3][SM_BINS]; /* masses of a selection's digit */
+            unsigned long long small_mass[SM_RANK];
+            uint32_t digit[SM_DIGIT], small[SM_RANK], part_n[3][SM_BINS];
+            uint32_t list[SM_LIST];
+        };
+        struct {
+            unsigned long long order[SM_FEW], w[SM_FEW]; /* greater order: earlier in the sorted row */
+            uint32_t index[SM_FEW];
+        } few;
+    };
 };
 
 /* What a row keeps: the keys above key, and of those equal to it the first `ties` in index order. */
@@ -296,40 +351,55 @@ struct Row {
     double inv, top; /* top: the row's top bin */
 };
 
-/* The members of row bin b as i = 0 .. S.seg[C] - 1: chunk and key of one. */
-__device__ __forceinline__ uint32_t member(const Pick &S, const Row &r, int b, uint32_t i, int *c_out) {
+/* Member i of those in hand (S.seg, S.at): its chunk, its index there, its logit. */
+__device__ __forceinline__ float member(const Pick &S, const Row &r, uint32_t i, int *c_out, int *at_out) {
     int lo = 0, hi = r.C; /* the last chunk whose segment starts at or before i */
     while (hi - lo > 1) {
         const int m = (lo + hi) >> 1;
         if (S.seg[m] <= i) lo = m;
         else hi = m;
     }
-    *c_out = lo;
-    const Chunk &k = r.ch[lo];
-    const int at = k.perm[k.start[b - S.off[lo]] + (i - S.seg[lo])];
-    return sample_key(sample_value(r.l[(size_t)lo * SM_CHUNK + at]));
+    const int at = r.ch[lo].perm[S.at[lo] + (i - S.seg[lo])];
+    *c_out = lo, *at_out = at;
+    return sample_value(r.l[(size_t)lo * SM_CHUNK + at]);
 }
 
-/* Running sizes of bin b's segments over the chunks; the keys into the list if they fit. */
-__device__ void open_bin(Pick &S, const Row &r, int b) {
+/* Takes in hand the members of the row's bins b0 .. b1; a chunk's lie together. The number of them. */
+__device__ uint32_t take_bins(Pick &S, const Row &r, int b0, int b1) {
     const int tid = threadIdx.x;
-    __syncthreads();
-    uint32_t x = 0;
+    uint32_t x = 0, from = 0;
     if (tid < r.C) {
-        const int j = b - S.off[tid];
-        if (j >= 0 && j < SM_BINS) x = (uint32_t)r.ch[tid].start[j + 1] - r.ch[tid].start[j];
+        int j0 = b0 - S.off[tid], j1 = b1 - S.off[tid];
+        j0 = j0 < 0 ? 0 : j0, j1 = j1 < SM_BINS - 1 ? j1 : SM_BINS - 1;
+        if (j0 <= j1) {
+            const uint32_t s0 = r.ch[tid].seg[j0], s1 = r.ch[tid].seg[j1];
+            from = s0 & 0xffff, x = (s1 & 0xffff) + (s1 >> 16) - from;
+        }
     }
     uint32_t total;
-    const uint32_t incl = block_scan(x, S.redu, &total);
-    if (tid < r.C) S.seg[tid] = incl - x;
+    const uint32_t incl = block_scan(x, S.red1, &total);
+    if (tid < r.C) S.seg[tid] = incl - x, S.at[tid] = from;
     if (tid == 0) S.seg[r.C] = total;
     __syncthreads();
-    if (total <= SM_LIST)
-        for (uint32_t i = tid; i < total; i += SM_T2) {
-            int c;
-            S.list[i] = member(S, r, b, i, &c);
-        }
+    return total;
+}
+
+/* take_bins of bin b alone, and its keys into the list if they fit. */
+__device__ void open_bin(Pick &S, const Row &r, int b) {
     __syncthreads();
+    const uint32_t total = take_bins(S, r, b, b);
+    if (total <= SM_LIST) {
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < total; i += SM_T2) {
+            int c, at;
+            S.list[i] = sample_key(member(S, r, i, &c, &at));
+        }
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ uint32_t key_of(const Pick &S, const Row &r, uint32_t i) {
+    int c, at;
+    return S.seg[r.C] <= SM_LIST ? S.list[i] : sample_key(member(S, r, i, &c, &at));
 }
 
 /* Among the members of the opened bin b with keys of at least floor_key: the key at which the run in
@@ -346,18 +416,13 @@ __device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint
     klo = klo < floor_key ? floor_key : klo;
     uint32_t n_above = 0, left = total;
     unsigned long long m_above = 0;
-    auto key_of = [&](uint32_t i) {
-        int c;
-        return total <= SM_LIST ? S.list[i] : member(S, r, b, i, &c);
-    };
     while (left > SM_RANK && klo < khi) {
         const int bits = 32 - __clz((int)(khi - klo)), shift = bits > 10 ? bits - 10 : 0;
         __syncthreads();
         S.digit[tid] = 0, S.tally[tid] = 0;
-        if (tid == 0) S.hit = SM_DIGIT, S.last = 0;
         __syncthreads();
         for (uint32_t i = tid; i < total; i += SM_T2) {
-            const uint32_t k = key_of(i);
+            const uint32_t k = key_of(S, r, i);
             if (k < klo || k > khi) continue;
             const uint32_t d = (khi - k) >> shift;
             atomicAdd(&S.digit[d], 1u);
@@ -368,14 +433,12 @@ __device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint
         const unsigned long long m = S.tally[tid];
         uint32_t n_all;
         unsigned long long m_all = 0, m_to = 0;
-        const uint32_t n_to = n_above + block_scan(n, S.redu, &n_all);
-        if (!by_count) m_to = m_above + block_scan(m, S.redk, &m_all);
-        if (n) { /* the first digit that reaches the want; the last one where a rounding keeps it from any */
-            atomicMax(&S.last, tid);
-            if (by_count ? n_to >= want : (double)m_to >= want_mass) atomicMin(&S.hit, tid);
-        }
-        __syncthreads();
-        const int hit = S.hit < SM_DIGIT ? S.hit : S.last;
+        const uint32_t n_to = n_above + block_scan(n, S.red1, &n_all);
+        if (!by_count) m_to = m_above + block_scan(m, S.red1, &m_all);
+        /* the first digit that reaches the want; the last one where a rounding keeps it from any */
+        int hit, last;
+        block_find(n && (by_count ? n_to >= want : (double)m_to >= want_mass), n, S.red1, S.red2, &hit, &last);
+        hit = hit < SM_DIGIT ? hit : last < 0 ? 0 : last;
         if (tid == hit) S.sel_n = n_to - n, S.sel_k = n, S.sel_m = m_to - m;
         __syncthreads();
         n_above = S.sel_n, left = S.sel_k, m_above = S.sel_m;
@@ -388,10 +451,10 @@ __device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint
         *above = n_above, *above_mass = (double)m_above;
         return khi;
     }
-    if (tid == 0) S.sel_n = 0, S.last = -1;
+    if (tid == 0) S.sel_n = 0;
     __syncthreads();
     for (uint32_t i = tid; i < total; i += SM_T2) {
-        const uint32_t k = key_of(i);
+        const uint32_t k = key_of(S, r, i);
         if (k < klo || k > khi) continue;
         const uint32_t at = atomicAdd(&S.sel_n, 1u);
         S.small[at] = k; /* at < left <= SM_RANK */
@@ -442,13 +505,83 @@ __device__ uint32_t min_p_key(float mx, double inv, double min_p) {
     return k;
 }
 
+/* A row whose kept tokens are among the S.seg[C] <= SM_FEW in hand: all of it in LDS, by comparing all
+ * with all (two lanes to a token, each half of the others). Masses are in 2^-52 of the largest weight.
+ * whole: the mass that top-p counts against where there is no top-k. */
+__device__ void pick_few(Pick &S, const Row &r, const Par &p, float mx, double whole, double ud, int32_t *tok, float *prob) {
+    const int tid = threadIdx.x, i = tid >> 1, half = tid & 1;
+    const uint32_t N = S.seg[r.C];
+    float x = -INFINITY;
+    uint32_t index = 0;
+    if ((uint32_t)i < N) {
+        int c, at;
+        x = member(S, r, i, &c, &at);
+        index = (uint32_t)(c * SM_CHUNK + at);
+    }
+    const double wd = (uint32_t)i < N ? weight(x, mx, r.inv) : 0.0;
+    const unsigned long long mine = (unsigned long long)(wd * 0x1p52 + 0.5), ord = (unsigned long long)sample_key(x) << 32 | ~index;
+    __syncthreads();
+    if (half == 0) S.few.order[i] = (uint32_t)i < N ? ord : 0, S.few.w[i] = mine, S.few.index[i] = (uint32_t)i < N ? index : 0xffffffffu;
+    __syncthreads();
+    uint32_t rank = 0;
+    unsigned long long before = 0;
+    const uint32_t n2 = (N + 1) / 2;
+#pragma unroll 8
+    for (uint32_t k = 0; k < n2; k++) {
+        const uint32_t j = 2 * k + half; /* j = N has no order */
+        if (S.few.order[j] > ord) rank++, before += S.few.w[j];
+    }
+    rank += (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)rank);
+    before += (unsigned long long)(uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)(before >> 32)) << 32 |
+              (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)before);
+    bool keep = (uint32_t)i < N && wd > 0.0;
+    if (p.top_k) {
+        const uint32_t k = (uint32_t)p.top_k < N ? (uint32_t)p.top_k : N;
+        if (rank == k - 1 && (uint32_t)i < N && half == 0) S.sel_m = before + mine;
+        __syncthreads();
+        whole = (double)S.sel_m;
+        keep = keep && rank < k;
+    } else {
+        whole *= 0x1p52;
+    }
+    if (p.top_p < 1.0) keep = keep && (rank == 0 || (double)before < p.top_p * whole);
+    if (p.min_p > 0.0) keep = keep && wd >= p.min_p;
+    __syncthreads(); /* the masses have been read */
+    if (half == 0) S.few.w[i] = keep ? mine : 0;
+    __syncthreads();
+    unsigned long long upto = 0, all = 0;
+    uint32_t last = 0;
+#pragma unroll 8
+    for (uint32_t k = 0; k < n2; k++) {
+        const uint32_t j = 2 * k + half;
+        const unsigned long long w = j < N ? S.few.w[j] : 0;
+        all += w;
+        if (S.few.index[j] < index) upto += w;
+        if (w && S.few.index[j] >= last) last = S.few.index[j];
+    }
+    auto other = [&](unsigned long long v) {
+        return (unsigned long long)(uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)(v >> 32)) << 32 | (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)v);
+    };
+    all += other(all), upto += other(upto);
+    const uint32_t lo = (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)last);
+    last = lo > last ? lo : last;
+    const double goal = ud * (double)all;
+    /* the token whose share of the running mass holds the goal; past the whole the last one */
+    const bool hit = goal < (double)all ? (double)upto <= goal && (double)(upto + mine) > goal : index == last;
+    if (keep && hit && half == 0) {
+        tok[blockIdx.x] = (int)index;
+        if (prob) prob[blockIdx.x] = (float)(wd / ((double)all * 0x1p-52));
+    }
+}
+
 __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__ logits, int stride,
                                                        int vocab, int C, const Chunk *__restrict__ work,
                                                        const nmx_sample_params *par, int par_step,
                                                        const float *__restrict__ uni,
                                                        int32_t *__restrict__ tok,
                                                        float *__restrict__ prob) {
-    __shared__ Pick S;
+    extern __shared__ uint4 smem[];
+    Pick &S = *(Pick *)smem;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
     const float *l = logits + (size_t)row * stride;
     const Chunk *ch = work + (size_t)row * C;
@@ -487,69 +620,98 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
             S.off[tid] = d < (double)SM_BINS ? (int)d : SM_BINS;
             S.cand[tid] = 0, S.ties[tid] = 0;
         }
-        if (tid < SM_BINS) S.cnt[tid] = 0, S.mass[tid] = 0, S.edge[tid] = exp_neg(-0.125 * tid);
         __syncthreads();
-#pragma unroll 2
-        for (int c = wave; c < C; c += SM_W2) { /* a wave adds a chunk's histogram */
-            const int off = S.off[c];
-            uint32_t n[4];
-            unsigned long long m[4];
+        const int b = tid & (SM_BINS - 1), quarter = tid / SM_BINS;
+        {
+            uint32_t n = 0; /* a thread adds its bin over every 4th chunk, 8 requests at a time */
+            unsigned long long m = 0;
+            for (int c0 = quarter; c0 < C; c0 += 32) {
+                uint32_t ns[8];
+                unsigned long long ms[8];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int j = lane + 64 * q;
-                const bool in = j + off < SM_BINS;
-                n[q] = in ? (uint32_t)ch[c].start[j + 1] - ch[c].start[j] : 0;
-                m[q] = in ? ch[c].mass[j] : 0;
+                for (int q = 0; q < 8; q++) {
+                    const int c = c0 + 4 * q < C ? c0 + 4 * q : C - 1, j = b - S.off[c]; /* no branch around a request */
+                    ns[q] = ch[c].seg[j < 0 ? 0 : j] >> 16;
+                    ms[q] = ch[c].mass[j < 0 ? 0 : j];
+                }
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const int c = c0 + 4 * q;
+                    if (c < C && b >= S.off[c]) n += ns[q], m += ms[q];
+                }
             }
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (n[q]) atomicAdd(&S.cnt[lane + 64 * q + off], n[q]), atomicAdd(&S.mass[lane + 64 * q + off], m[q]);
+            if (quarter) S.part_n[quarter - 1][b] = n, S.part_m[quarter - 1][b] = m;
+            __syncthreads();
+            if (!quarter) {
+                S.cnt[b] = n + S.part_n[0][b] + S.part_n[1][b] + S.part_n[2][b];
+                S.mass[b] = m + S.part_m[0][b] + S.part_m[1][b] + S.part_m[2][b];
+                S.edge[b] = exp_neg(-0.125 * b);
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        const int b = tid & (SM_BINS - 1);
         const double edge = S.edge[b];
+        const double unit = exp_neg((top - g_top) * 0.125) * 0x1p-40; /* a mass of the top bin, as a weight */
+        /* a bin that the kept tokens do not reach below: of top-k's or top-p's end, of min-p's border (one
+         * lower, for its rounding). Few tokens down to it: they decide among themselves */
+        uint32_t n_all;
+        const uint32_t n_mine = tid < SM_BINS ? S.cnt[tid] : 0, n_upto = block_scan(n_mine, S.red1, &n_all);
+        const bool by_k = p.top_k && (uint32_t)p.top_k < n_all;
+        double m_all = 0.0;
+        int reach = SM_BINS, none;
+        if (by_k) {
+            block_find(tid < SM_BINS && n_upto >= (uint32_t)p.top_k, false, S.red1, S.red2, &reach, &none);
+        } else if (p.top_p < 1.0) {
+            const double m_upto = block_scan(tid < SM_BINS ? (double)S.mass[b] * edge : 0.0, S.red1, &m_all);
+            block_find(tid < SM_BINS && m_upto >= p.top_p * m_all, false, S.red1, S.red2, &reach, &none);
+        }
+        if (p.min_p > 0.0 && !(by_k && p.top_p < 1.0)) {
+            const double d = top - floor(g_top + 8.0 * log(p.min_p)) + 1.0;
+            if (d < (double)reach) reach = (int)d;
+        }
+        if (reach < SM_BINS) {
+            if (tid == reach) S.sel_n = n_upto;
+            __syncthreads();
+            if (S.sel_n <= SM_FEW) {
+                Par q = p;
+                if (!by_k) q.top_k = 0;
+                take_bins(S, r, 0, reach);
+                pick_few(S, r, q, mx, m_all * unit, ud, tok, prob);
+                return;
+            }
+        }
         int kb = SM_BINS;     /* the bin that top-k ends in */
         double k_mass = 0.0;  /* and the mass that it keeps of it, in 2^-40 of its lower edge */
-        if (p.top_k) {
-            const uint32_t k = (uint32_t)p.top_k, n = tid < SM_BINS ? S.cnt[tid] : 0;
-            uint32_t n_all;
-            const uint32_t n_to = block_scan(n, S.redu, &n_all);
-            if (n_all > k) {
-                if (n && n_to >= k && n_to - n < k) S.hit = tid, S.sel_n = k - (n_to - n);
-                __syncthreads();
-                kb = S.hit;
-                const uint32_t want = S.sel_n;
-                open_bin(S, r, kb);
-                uint32_t above;
-                double unused;
-                cut.key = select_key(S, r, kb, true, want, 0.0, 0, &above, &unused);
-                cut.ties = want - above;
-                if (p.top_p < 1.0) {
-                    unsigned long long kept = 0, whole;
-                    for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
-                        int c;
-                        const uint32_t key = S.seg[C] <= SM_LIST ? S.list[i] : member(S, r, kb, i, &c);
-                        if (key > cut.key) kept += bin_mass(sample_unkey(key), p.inv);
-                    }
-                    block_scan(kept, S.redk, &whole);
-                    k_mass = (double)whole + (double)cut.ties * (double)bin_mass(sample_unkey(cut.key), p.inv);
+        if (by_k) {
+            const uint32_t k = (uint32_t)p.top_k;
+            __syncthreads();
+            if (n_mine && n_upto >= k && n_upto - n_mine < k) S.hit = tid, S.sel_n = k - (n_upto - n_mine);
+            __syncthreads();
+            kb = S.hit;
+            const uint32_t want = S.sel_n;
+            open_bin(S, r, kb);
+            uint32_t above;
+            double unused;
+            cut.key = select_key(S, r, kb, true, want, 0.0, 0, &above, &unused);
+            cut.ties = want - above;
+            if (p.top_p < 1.0) {
+                unsigned long long kept = 0, whole;
+                for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
+                    const uint32_t key = key_of(S, r, i);
+                    if (key > cut.key) kept += bin_mass(sample_unkey(key), p.inv);
                 }
+                block_scan(kept, S.red1, &whole);
+                k_mass = (double)whole + (double)cut.ties * (double)bin_mass(sample_unkey(cut.key), p.inv);
             }
         }
         int opened = kb;
         if (p.top_p < 1.0) { /* over what top-k left */
             double mine = 0.0, whole;
             if (tid < SM_BINS) mine = (b < kb ? (double)S.mass[b] : b == kb ? k_mass : 0.0) * edge;
-            const double to = block_scan(mine, S.redd, &whole);
+            const double to = block_scan(mine, S.red1, &whole);
             const double want = p.top_p * whole;
-            if (tid == 0) S.hit = SM_BINS, S.last = 0;
-            __syncthreads();
-            if (mine > 0.0) {
-                atomicMax(&S.last, tid);
-                if (to >= want) atomicMin(&S.hit, tid);
-            }
-            __syncthreads();
-            const int pb = S.hit < SM_BINS ? S.hit : S.last; /* a whole missed by a rounding */
+            int pb, last;
+            block_find(mine > 0.0 && to >= want, mine > 0.0, S.red1, S.red2, &pb, &last);
+            pb = pb < SM_BINS ? pb : last; /* a whole missed by a rounding */
             if (tid == pb) S.sel_d = fmax(want - (to - mine), 0.0) / edge;
             __syncthreads();
             const double rest = S.sel_d;
@@ -574,11 +736,20 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
         const int cb = d < (double)SM_BINS ? (int)d : SM_BINS;
         if (cb < SM_BINS) {
             if (cb != opened) open_bin(S, r, cb);
-            for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
-                int c;
-                const uint32_t key = member(S, r, cb, i, &c);
-                if (key == cut.key) atomicAdd(&S.ties[c], 1u);
-                else if (key > cut.key) atomicAdd(&S.cand[c], bin_mass(sample_unkey(key), p.inv));
+            const uint32_t total = S.seg[C];
+            for (int c = wave; c < C; c += SM_W2) { /* a wave adds a chunk's */
+                uint32_t n = 0;
+                unsigned long long m = 0;
+                const uint32_t end = S.seg[c + 1];
+                for (uint32_t i = S.seg[c] + lane; i < end; i += 64) {
+                    uint32_t key;
+                    if (total <= SM_LIST) key = S.list[i];
+                    else key = sample_key(sample_value(l[(size_t)c * SM_CHUNK + ch[c].perm[S.at[c] + (i - S.seg[c])]]));
+                    n += key == cut.key;
+                    if (key > cut.key) m += bin_mass(sample_unkey(key), p.inv);
+                }
+                n = nmx_scan_wave(n), m = nmx_scan_wave(m);
+                if (lane == 63) S.ties[c] = n, S.cand[c] = m;
             }
         }
         for (int c = wave; c < C; c += SM_W2) { /* a wave adds a chunk's whole bins, in a fixed order */
@@ -587,14 +758,15 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const int j = lane + 64 * q;
-                if (j < n) s += (double)ch[c].mass[j] * S.edge[j + S.off[c]];
+                const unsigned long long m = ch[c].mass[j];
+                if (j < n) s += (double)m * S.edge[j + S.off[c]];
             }
             s = nmx_scan_wave(s);
             if (lane == 63) S.chunk_mass[c] = s;
         }
         __syncthreads();
         uint32_t all;
-        const uint32_t mine = tid < C ? S.ties[tid] : 0, to = block_scan(mine, S.redu, &all), before = to - mine;
+        const uint32_t mine = tid < C ? S.ties[tid] : 0, to = block_scan(mine, S.red1, &all), before = to - mine;
         const uint32_t ties = before >= cut.ties ? 0 : cut.ties - before < mine ? cut.ties - before : mine;
         if (tid < C) {
             S.ties[tid] = ties;
@@ -604,20 +776,16 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
                 if (ties) m += (double)ties * (double)bin_mass(sample_unkey(cut.key), p.inv);
                 mass += m * S.edge[cb];
             }
-            mass *= exp_neg((top - g_top) * 0.125) * 0x1p-40; /* a mass of the top bin, as a weight */
+            mass *= unit;
         }
     }
     /* the chunk that the draw falls into */
     double whole;
-    const double to = block_scan(mass, S.redd, &whole), goal = ud * whole;
-    if (tid == 0) S.hit = SM_T2, S.last = 0;
-    __syncthreads();
-    if (mass > 1e-296) { /* so that one of its slices has 1e-297, and one logit a weight of 1e-300 */
-        atomicMax(&S.last, tid);
-        if (to > goal) atomicMin(&S.hit, tid);
-    }
-    __syncthreads();
-    const int c = S.hit < SM_T2 ? S.hit : S.last;
+    const double to = block_scan(mass, S.red1, &whole), goal = ud * whole;
+    const bool some = mass > 1e-296; /* so that one of its slices has 1e-297, and one logit a weight of 1e-300 */
+    int c, c_last;
+    block_find(some && to > goal, some, S.red1, S.red2, &c, &c_last);
+    c = c < SM_T2 ? c : c_last;
     if (tid == c) S.sel_d = to - mass;
     __syncthreads();
     double rest = goal - S.sel_d;
@@ -643,16 +811,28 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
     }
     float x[SM_RUN];
     uint32_t key[SM_RUN], same = 0;
+    if (p.filter && len == SM_CHUNK && ((uintptr_t)lc & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < SM_RUN; e += 4) {
+            const float4 y = *(const float4 *)(lc + i0 + e);
+            x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < SM_RUN; e++) x[e] = lc[e < per && i0 + e < len ? i0 + e : len - 1];
+#pragma unroll
+        for (int e = 0; e < SM_RUN; e++) x[e] = e < per && i0 + e < len ? x[e] : -INFINITY;
+    }
 #pragma unroll
     for (int e = 0; e < SM_RUN; e++) {
-        x[e] = e < per && i0 + e < len ? sample_value(lc[i0 + e]) : -INFINITY;
+        x[e] = sample_value(x[e]);
         key[e] = sample_key(x[e]);
         same += x[e] > -INFINITY && key[e] == cut.key;
     }
     uint32_t rank = 0xffffffffu, allowed = 0xffffffffu;
     if (p.filter) {
         uint32_t all;
-        rank = block_scan(same, S.redu, &all) - same;
+        rank = block_scan(same, S.red1, &all) - same;
         allowed = S.ties[c];
     }
     double w[SM_RUN], s = 0.0;
@@ -666,29 +846,23 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
         s += w[e];
     }
     double in_chunk;
-    double run = block_scan(s, S.redd, &in_chunk) - s;
-    if (tid == 0) S.hit = SM_CHUNK, S.last = 0;
-    __syncthreads();
-    int first = SM_CHUNK, final = -1;
+    double run = block_scan(s, S.red1, &in_chunk) - s;
+    double wf = 0.0, wl = 0.0; /* the thread's first token past the goal, and its last one */
+    int first = -1, final = -1;
 #pragma unroll
     for (int e = 0; e < SM_RUN; e++) {
         run += w[e];
         if (w[e] > 0.0) {
-            final = i0 + e;
-            if (run > rest && first == SM_CHUNK) first = i0 + e;
+            final = i0 + e, wl = w[e];
+            if (run > rest && first < 0) first = i0 + e, wf = w[e];
         }
     }
-    if (final >= 0) {
-        atomicMax(&S.last, final);
-        if (first < SM_CHUNK) atomicMin(&S.hit, first);
-    }
-    __syncthreads();
-    const int at = S.hit < SM_CHUNK ? S.hit : S.last; /* a whole missed by a rounding: the last one */
-    if (at >= i0 && at < i0 + per) {
-        double mine = 0.0;
-#pragma unroll
-        for (int e = 0; e < SM_RUN; e++) mine = e == at - i0 ? w[e] : mine;
-        answer(c * SM_CHUNK + at, mine / whole);
+    int who, who_last;
+    block_find(first >= 0, final >= 0, S.red1, S.red2, &who, &who_last);
+    if (who < SM_T2) {
+        if (tid == who) answer(c * SM_CHUNK + first, wf / whole);
+    } else if (tid == who_last) { /* a whole missed by a rounding: the last one */
+        answer(c * SM_CHUNK + final, wl / whole);
     }
 }
 
@@ -724,7 +898,9 @@ int nmx_sample(nmx_ctx *ctx, const float *logits, int stride, int vocab, int n,
     sample_scan_k<<<dim3((unsigned)C, (unsigned)n), SM_T1, 0, ctx->stream>>>(
         logits, stride, vocab, (Chunk *)work, params, per_row ? 1 : 0);
     NMX_LAUNCHED(ctx, "sample_scan");
-    sample_pick_k<<<(unsigned)n, SM_T2, 0, ctx->stream>>>(logits, stride, vocab, C, (const Chunk *)work,
+    static std::atomic<uint64_t> lds_set;
+    if (nmx_dyn_lds(ctx, (const void *)sample_pick_k, sizeof(Pick), lds_set)) return -1;
+    sample_pick_k<<<(unsigned)n, SM_T2, sizeof(Pick), ctx->stream>>>(logits, stride, vocab, C, (const Chunk *)work,
                                                           params, per_row ? 1 : 0, u, tok, prob);
     NMX_LAUNCHED(ctx, "sample_pick");
     return 0;

@@ -28,7 +28,8 @@ namespace {
 constexpr int SM_CHUNK = 8192; /* logits of a workgroup of sample_scan_k */
 constexpr int SM_T1 = 512, SM_PER = SM_CHUNK / SM_T1, SM_SLICE = SM_CHUNK / (SM_T1 / 64);
 constexpr int SM_T2 = 1024, SM_W2 = SM_T2 / 64, SM_RUN = SM_CHUNK / SM_T2; /* consecutive logits of a thread */
-constexpr int SM_BINS = 256;
+constexpr int SM_BINS = 256, SM_COPY = 4;
+static_assert(2 * SM_BINS == SM_T1, "two threads of sample_scan_k to a bin");
 constexpr int SM_MAXC = (1 << 20) / SM_CHUNK; /* chunks of the longest row */
 constexpr int SM_LIST = 16384; /* members of a bin kept in LDS; a bin with more is read again */
 constexpr int SM_RANK = 256;   /* members of a bin ranked by comparing all with all */
@@ -172,16 +173,15 @@ __device__ __forceinline__ void block_find(bool first_of, bool last_of, unsigned
     *last = my ? 64 * (63 - __clzll((long long)my)) + __builtin_amdgcn_readlane(l, 63 - __clzll((long long)my)) : -1;
 }
 
-__global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__ logits, int stride,
+__global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restrict__ logits, int stride,
                                                        int vocab, Chunk *__restrict__ work,
                                                        const nmx_sample_params *par, int par_step) {
     __shared__ float redf[SM_T1 / 64];
     __shared__ double redd[SM_T1 / 64];
     __shared__ unsigned long long redk[SM_T1 / 64];
-    __shared__ uint32_t cnt[SM_BINS], wave_cnt[4];
-    __shared__ unsigned long long mass[SM_BINS];
+    __shared__ uint32_t cnt[SM_BINS * SM_COPY], wave_cnt[SM_T1 / 64];
+    __shared__ unsigned long long mass[SM_BINS * SM_COPY];
     __shared__ uint32_t perm2[SM_CHUNK / 2];
-    __shared__ float val[SM_CHUNK / 16 * 17]; /* the logits in grouped order, a word skipped every 16 */
     uint16_t *perm = (uint16_t *)perm2;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
     const float *l = logits + (size_t)row * stride + (size_t)c * SM_CHUNK;
@@ -248,65 +248,56 @@ __global__ __launch_bounds__(SM_T1) void sample_scan_k(const float *__restrict__
         }
         return;
     }
-    if (tid < SM_BINS) cnt[tid] = 0, mass[tid] = 0;
+    /* SM_COPY copies of each bin, by lane: neighbouring lanes of one bin do not wait for each other */
+#pragma unroll
+    for (int i = 0; i < SM_BINS * SM_COPY; i += SM_T1) cnt[i + tid] = 0, mass[i + tid] = 0;
     __syncthreads();
     const double base = floor(grid_pos(mx, p.inv));
-    uint32_t at[SM_PER]; /* bin << 16 | rank; all ones: no weight */
+    const int copy = lane & (SM_COPY - 1);
+    uint32_t at[SM_PER]; /* bin copy << 16 | rank; all ones: no weight */
 #pragma unroll
     for (int u = 0; u < SM_PER; u++) {
         at[u] = 0xffffffffu;
-        const double d = base - floor(grid_pos(v[u], p.inv)); /* inf for -inf */
+        const double g = grid_pos(v[u], p.inv), fl = floor(g), d = base - fl; /* inf for -inf */
         if (d < (double)SM_BINS) {
-            const uint32_t j = (uint32_t)(int)d;
+            const uint32_t j = (uint32_t)(int)d * SM_COPY + copy;
             at[u] = j << 16 | atomicAdd(&cnt[j], 1u);
+            atomicAdd(&mass[j], bin_mass_at(g - fl));
         }
     }
     __syncthreads();
-    uint32_t first = 0, mine = 0; /* members of the bins above bin tid, and of it */
-    if (tid < SM_BINS) {
-        mine = cnt[tid];
-        const uint32_t x = nmx_scan_wave(mine);
-        if (lane == 63) wave_cnt[wave] = x;
-        first = x - mine;
-    }
+    /* thread: SM_COPY / 2 copies of a bin */
+    constexpr int PT = SM_BINS * SM_COPY / SM_T1;
+    uint32_t mine[PT], n = 0;
+    unsigned long long m = 0;
+#pragma unroll
+    for (int i = 0; i < PT; i++) mine[i] = cnt[tid * PT + i], n += mine[i], m += mass[tid * PT + i];
+    const uint32_t upto = nmx_scan_wave(n);
+    if (lane == 63) wave_cnt[wave] = upto;
     __syncthreads();
-    const uint32_t members = wave_cnt[0] + wave_cnt[1] + wave_cnt[2] + wave_cnt[3];
-    if (tid < SM_BINS) {
-        for (int w = 0; w < wave; w++) first += wave_cnt[w];
-        out->seg[tid] = first | mine << 16;
-        cnt[tid] = first;
+    uint32_t first = upto - n, members = 0;
+#pragma unroll
+    for (int w = 0; w < SM_T1 / 64; w++) {
+        if (w < wave) first += wave_cnt[w];
+        members += wave_cnt[w];
     }
+    {
+        uint32_t f = first;
+#pragma unroll
+        for (int i = 0; i < PT; i++) cnt[tid * PT + i] = f, f += mine[i];
+    }
+    /* the two threads of a bin together */
+    const uint32_t n2 = n + (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)n);
+    m += (unsigned long long)(uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)(m >> 32)) << 32 | (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)m);
+    if (!(tid & 1)) out->seg[tid >> 1] = first | n2 << 16, out->mass[tid >> 1] = m;
     if (tid == 0) out->base = base;
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < SM_PER; u++) {
-        if (at[u] == 0xffffffffu) continue;
-        const uint32_t to = cnt[at[u] >> 16] + (at[u] & 0xffffu);
-        perm[to] = (uint16_t)index(u);
-        val[to + (to >> 4)] = v[u];
-    }
+    for (int u = 0; u < SM_PER; u++)
+        if (at[u] != 0xffffffffu) perm[cnt[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)index(u);
     __syncthreads();
     uint2 *po = (uint2 *)out->perm;
     for (uint32_t i = tid; 4 * i < members; i += SM_T1) po[i] = ((const uint2 *)perm2)[i];
-    /* masses: neighbours in the grouped order mostly share a bin, so a thread of 16 consecutive ones adds
-     * to the bins' sums once or twice instead of 16 times */
-    unsigned long long sum = 0;
-    int bin = -1;
-#pragma unroll
-    for (int u = 0; u < SM_PER; u++) {
-        const uint32_t i = (uint32_t)tid * SM_PER + u;
-        if (i >= members) break;
-        const double g = grid_pos(val[17 * tid + u], p.inv), fl = floor(g);
-        const int j = (int)(base - fl);
-        if (j != bin) {
-            if (bin >= 0) atomicAdd(&mass[bin], sum);
-            sum = 0, bin = j;
-        }
-        sum += bin_mass_at(g - fl);
-    }
-    if (bin >= 0) atomicAdd(&mass[bin], sum);
-    __syncthreads();
-    if (tid < SM_BINS) out->mass[tid] = mass[tid];
 }
 
 /* The row's state in sample_pick_k. */
@@ -656,13 +647,16 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
         uint32_t n_all;
         const uint32_t n_mine = tid < SM_BINS ? S.cnt[tid] : 0, n_upto = block_scan(n_mine, S.red1, &n_all);
         const bool by_k = p.top_k && (uint32_t)p.top_k < n_all;
-        double m_all = 0.0;
-        int reach = SM_BINS, none;
+        double m_all = 0.0, m_mine = 0.0, m_upto = 0.0; /* the masses that top-p counts, top-k aside */
+        int reach = SM_BINS, pb = SM_BINS, last;
         if (by_k) {
-            block_find(tid < SM_BINS && n_upto >= (uint32_t)p.top_k, false, S.red1, S.red2, &reach, &none);
+            block_find(tid < SM_BINS && n_upto >= (uint32_t)p.top_k, false, S.red1, S.red2, &reach, &last);
         } else if (p.top_p < 1.0) {
-            const double m_upto = block_scan(tid < SM_BINS ? (double)S.mass[b] * edge : 0.0, S.red1, &m_all);
-            block_find(tid < SM_BINS && m_upto >= p.top_p * m_all, false, S.red1, S.red2, &reach, &none);
+            if (tid < SM_BINS) m_mine = (double)S.mass[b] * edge;
+            m_upto = block_scan(m_mine, S.red1, &m_all);
+            block_find(m_mine > 0.0 && m_upto >= p.top_p * m_all, m_mine > 0.0, S.red1, S.red2, &pb, &last);
+            pb = pb < SM_BINS ? pb : last; /* a whole missed by a rounding */
+            reach = pb;
         }
         if (p.min_p > 0.0 && !(by_k && p.top_p < 1.0)) {
             const double d = top - floor(g_top + 8.0 * log(p.min_p)) + 1.0;
@@ -705,14 +699,13 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
         }
         int opened = kb;
         if (p.top_p < 1.0) { /* over what top-k left */
-            double mine = 0.0, whole;
-            if (tid < SM_BINS) mine = (b < kb ? (double)S.mass[b] : b == kb ? k_mass : 0.0) * edge;
-            const double to = block_scan(mine, S.red1, &whole);
-            const double want = p.top_p * whole;
-            int pb, last;
-            block_find(mine > 0.0 && to >= want, mine > 0.0, S.red1, S.red2, &pb, &last);
-            pb = pb < SM_BINS ? pb : last; /* a whole missed by a rounding */
-            if (tid == pb) S.sel_d = fmax(want - (to - mine), 0.0) / edge;
+            if (by_k) {
+                m_mine = tid < SM_BINS ? (b < kb ? (double)S.mass[b] : b == kb ? k_mass : 0.0) * edge : 0.0;
+                m_upto = block_scan(m_mine, S.red1, &m_all);
+                block_find(m_mine > 0.0 && m_upto >= p.top_p * m_all, m_mine > 0.0, S.red1, S.red2, &pb, &last);
+                pb = pb < SM_BINS ? pb : last;
+            }
+            if (tid == pb) S.sel_d = fmax(p.top_p * m_all - (m_upto - m_mine), 0.0) / edge;
             __syncthreads();
             const double rest = S.sel_d;
             if (pb != kb) open_bin(S, r, pb);
@@ -752,17 +745,25 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
                 if (lane == 63) S.ties[c] = n, S.cand[c] = m;
             }
         }
-        for (int c = wave; c < C; c += SM_W2) { /* a wave adds a chunk's whole bins, in a fixed order */
-            const int n = cb - S.off[c];
-            double s = 0.0;
+        for (int c0 = wave; c0 < C; c0 += 2 * SM_W2) { /* a wave adds two chunks' whole bins, in a fixed order */
+            unsigned long long m[2][4];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const int j = lane + 64 * q;
-                const unsigned long long m = ch[c].mass[j];
-                if (j < n) s += (double)m * S.edge[j + S.off[c]];
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) m[i][q] = ch[c0 + i * SM_W2 < C ? c0 + i * SM_W2 : C - 1].mass[lane + 64 * q];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int c = c0 + i * SM_W2;
+                if (c >= C) break;
+                double s = 0.0;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int k = lane + 64 * q + S.off[c];
+                    if (k < cb) s += (double)m[i][q] * S.edge[k];
+                }
+                s = nmx_scan_wave(s);
+                if (lane == 63) S.chunk_mass[c] = s;
             }
-            s = nmx_scan_wave(s);
-            if (lane == 63) S.chunk_mass[c] = s;
         }
         __syncthreads();
         uint32_t all;

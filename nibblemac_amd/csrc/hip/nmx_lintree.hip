@@ -14,6 +14,7 @@
  * A node's sums run over its own ancestors alone (no product with a masked zero), so whatever
  * another branch holds, NaN or infinity, does not reach it. */
 #include "nmx_internal.h"
+#include "nmx_a8.h"
 #include "nmx_lanes.h"
 #include "nmx_math.h"
 #include "nmx_tree.h"
@@ -44,76 +45,96 @@ struct TreePre {
 
 constexpr int TP_N = 8; /* nodes of a workgroup */
 
+/* Partial sum l of 4 interleaved ones over the dk squares of a row (v: element l of it, dk / 4 elements 4
+ * apart), in element order: the adds of lin_pre_k. */
+__device__ __forceinline__ float square_chain(const float *v, int m4) {
+    float c = 0.0f;
+    int m = 0;
+    for (; m + 8 <= m4; m += 8) {
+        float b[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) b[u] = v[4 * (m + u)];
+#pragma unroll
+        for (int u = 0; u < 8; u++) c = c + b[u] * b[u];
+    }
+    for (; m < m4; m++) c = c + v[4 * m] * v[4 * m];
+    return c;
+}
+__device__ __forceinline__ float tree_beta(const float b) { return 1.0f / (1.0f + nmx_gate_expf(-b)); }
+__device__ __forceinline__ float tree_decay(const TreePre &a, float av, int h) {
+    const float A = a.A ? a.A[h] : -nmx_gate_expf(a.A_log[h]);
+    float sp = av + a.dt_bias[h];
+    sp = sp > 20.0f ? sp : nmx_gate_log1pf(nmx_gate_expf(sp));
+    return nmx_gate_expf(A * sp);
+}
+
+template <int KT>
 __global__ __launch_bounds__(256) void lin_tree_pre_k(TreePre a) {
-    extern __shared__ float sq[]; /* [TP_N][dk] squares */
+    extern __shared__ float sq[]; /* [TP_N][dk + 4] */
     __shared__ float red[4 * TP_N];
+    __shared__ int par[NMX_TREE_MAX];
     const int groups = (a.C + a.dk - 1) / a.dk, tid = threadIdx.x;
     const int t0 = blockIdx.y * TP_N, nb = a.n - t0 < TP_N ? a.n - t0 : TP_N;
     if ((int)blockIdx.x == groups) { /* gates */
         for (int u = tid; u < nb * a.heads; u += blockDim.x) {
             const int t = t0 + u / a.heads, h = u % a.heads;
-            const float b = a.b_in[(size_t)t * a.g_stride + h], av = a.a_in[(size_t)t * a.g_stride + h];
-            a.beta[t * a.heads + h] = 1.0f / (1.0f + nmx_gate_expf(-b));
-            const float A = a.A ? a.A[h] : -nmx_gate_expf(a.A_log[h]);
-            float sp = av + a.dt_bias[h];
-            sp = sp > 20.0f ? sp : nmx_gate_log1pf(nmx_gate_expf(sp));
-            a.decay[t * a.heads + h] = nmx_gate_expf(A * sp);
+            a.beta[t * a.heads + h] = tree_beta(a.b_in[(size_t)t * a.g_stride + h]);
+            a.decay[t * a.heads + h] = tree_decay(a, a.a_in[(size_t)t * a.g_stride + h], h);
         }
         return;
     }
-    const int ch = blockIdx.x * a.dk + tid, S = a.K - 1;
+    for (int t = tid; t < a.n; t += blockDim.x) par[t] = tree_parent(a.parent, t);
+    const int ch = blockIdx.x * a.dk + tid, K = KT ? KT : a.K, S = K - 1;
     const bool live = tid < a.dk && ch < a.C;
     const int cc = live ? ch : 0;
-    float wc[8], y[TP_N];
+    constexpr int KM = KT ? KT : 8;
+    float wc[KM], y[TP_N], win[TP_N][KM];
 #pragma unroll
-    for (int r = 0; r < 8; r++) wc[r] = r < a.K ? a.conv_w[(size_t)cc * a.K + r] : 0.0f;
+    for (int r = 0; r < KM; r++) wc[r] = r < K ? a.conv_w[(size_t)cc * K + r] : 0.0f;
+    __syncthreads();
+    /* win[u][j]: tap j's input, the newest (the node itself) at K - 1, then its ancestors, then the state's
+     * rows from the newest down; nodes past the end repeat the last one */
 #pragma unroll
     for (int u = 0; u < TP_N; u++) {
-        y[u] = 0.0f;
-        if (u >= nb) continue;
-        /* win[j]: tap j's input, the newest (the node itself) at K - 1, then its ancestors, then the
-         * state's rows from the newest down */
-        float win[8];
-        int at = t0 + u, row = S; /* row: the state row above, once the path is over */
+        int at = t0 + (u < nb ? u : nb - 1), row = S; /* row: the state row above, once the path is over */
 #pragma unroll
-        for (int r = 0; r < 8; r++) {
-            const int j = a.K - 1 - r; /* the r-th newest */
-            if (j < 0) continue;
-            float x;
-            if (at >= 0) {
-                x = a.raw[(size_t)at * a.raw_stride + cc];
-                at = tree_parent(a.parent, at);
-            } else {
-                row--;
-                x = a.state[(size_t)row * a.C + cc];
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (k == j) win[k] = x;
-            if (r == 0 && a.xin && live) a.xin[(size_t)(t0 + u) * a.C + ch] = x;
+        for (int r = 0; r < KM; r++) {
+            if (!KT && r >= K) break;
+            const bool node = at >= 0;
+            row -= !node;
+            const float *src = node ? a.raw + (size_t)at * a.raw_stride : a.state + (size_t)row * a.C;
+            win[u][r] = src[cc]; /* the r-th newest */
+            at = node ? par[at] : at;
         }
-        float acc = wc[0] * win[0];
+    }
 #pragma unroll
-        for (int j = 1; j < 8; j++)
-            if (j < a.K) acc = acc + wc[j] * win[j];
+    for (int u = 0; u < TP_N; u++) {
+        /* taps in order, the oldest first */
+        float acc = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KM; j++) {
+            if (!KT && j >= K) break;
+            float x = win[u][KT ? KT - 1 - j : 0];
+            if constexpr (!KT) {
+#pragma unroll
+                for (int r = 0; r < KM; r++) x = r == K - 1 - j ? win[u][r] : x;
+            }
+            acc = j ? acc + wc[j] * x : wc[0] * x;
+        }
         y[u] = nmx_silu(acc);
+        if (a.xin && live && u < nb) a.xin[(size_t)(t0 + u) * a.C + ch] = win[u][0];
     }
     if ((int)(blockIdx.x * a.dk) < 2 * a.kd) { /* a q or k head: L2 norm, chains of 4 per node */
         const float scale = (int)(blockIdx.x * a.dk) < a.kd ? a.qscale : 1.0f;
+        const int rs = a.dk + 4;
 #pragma unroll
         for (int u = 0; u < TP_N; u++)
-            if (u < nb && tid < a.dk) sq[u * a.dk + tid] = live ? y[u] * y[u] : 0.0f;
+            if (tid < a.dk) sq[u * rs + tid] = live ? y[u] : 0.0f;
         __syncthreads();
-        if (tid < 4 * nb) {
-            const float *v = sq + (tid >> 2) * a.dk + (tid & 3);
-            float c = 0.0f;
-            for (int m = 0; m < a.dk >> 2; m++) c = c + v[4 * m];
-            red[tid] = c;
-        }
+        if (tid < 4 * TP_N) red[tid] = square_chain(sq + (tid >> 2) * rs + (tid & 3), a.dk >> 2);
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < TP_N; u++) {
-            if (u >= nb) continue;
             const float ss = ((red[4 * u] + red[4 * u + 1]) + (red[4 * u + 2] + red[4 * u + 3])) + 0.0f;
             const float r = 1.0f / sqrtf(ss + a.l2eps);
             y[u] = (y[u] * r) * scale;
@@ -139,19 +160,115 @@ struct TreeRule {
 
 constexpr int TR_B = 8; /* pending rows staged at a time */
 
-/* One workgroup per head and 16 value columns (a group of the state's layout), a wave per 16 nodes.
- * The state's columns are a matrix operand as they lie: lane (column c, quarter gq) holds the float4
- * slots of keys gq dk/4 .. of its column, and the rows of k and q are read in the same order. */
+/* The tree as a wave's lanes see it, into LDS: sets of ancestors, decays over 2^k steps up, decays from
+ * the state (lane t; d, bt: its decay and beta). Every lane of the wave. */
+struct TreeTables {
+    unsigned long long sets[NMX_TREE_MAX];
+    float dec[NMX_TREE_MAX], bet[NMX_TREE_MAX], gs[NMX_TREE_MAX], run[6][NMX_TREE_MAX];
+    int up[6][NMX_TREE_MAX];
+    int levels;
+};
+__device__ __forceinline__ void tree_tables(TreeTables &s, const int32_t *parent, int n, float d, float bt) {
+    const int lane = threadIdx.x & 63;
+    int p;
+    const unsigned long long set = tree_ancestors(parent, n, &p);
+    s.sets[lane] = set, s.dec[lane] = d, s.bet[lane] = bt;
+    float r = d;
+    int q = p;
+#pragma unroll
+    for (int k = 0; k < 6; k++) {
+        s.run[k][lane] = r, s.up[k][lane] = q;
+        const int from = q < 0 ? lane : q;
+        const float ro = __shfl(r, from);
+        const int qo = __shfl(q, from);
+        if (q >= 0) r *= ro, q = qo;
+    }
+    s.gs[lane] = r; /* every node is at most 63 steps from the state */
+    int deep = lane < n ? __popcll(set) : 0;
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) deep = max(deep, __shfl_xor(deep, x));
+    if (lane == 0) s.levels = deep;
+}
+/* D(t, a), the product of the decays after ancestor a up to t */
+__device__ __forceinline__ float tree_gap(const TreeTables &s, int t, int a) {
+    const int steps = __popcll(s.sets[t]) - __popcll(s.sets[a]);
+    float d = 1.0f;
+    int at = t;
+#pragma unroll
+    for (int k = 0; k < 6; k++)
+        if (steps >> k & 1) d *= s.run[k][at], at = s.up[k][at];
+    return d;
+}
+
+/* A lane's 16 x 16 piece of x y^T over DK4 4 columns: rows of x and y in LDS, quarter gq of the columns
+ * to a lane (the state's order of keys). */
+template <int NS>
+__device__ __forceinline__ f32x4 row_products(const float *x, const float *y) {
+    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < NS; k++) {
+        const float4 u = *(const float4 *)(x + 4 * k), v = *(const float4 *)(y + 4 * k);
+        r = mfma4(u.x, v.x, r), r = mfma4(u.y, v.y, r), r = mfma4(u.z, v.z, r), r = mfma4(u.w, v.w, r);
+    }
+    return r;
+}
+
+/* Pending rows u0 .. of head h into the state's columns held in s, as nmx_lin_apply makes them. */
+template <int DK4>
+__device__ __forceinline__ void replay(float4 (&s)[DK4 / 4], const float *pend, int keep, int heads, int h, size_t logw, int dv,
+                                       int j0, float (*pk)[4 * DK4 + 16], float *pdec, bool owner) {
+    constexpr int DK = 4 * DK4;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, gq = lane >> 4;
+    for (int u0 = 0; u0 < keep; u0 += TR_B) {
+        const int nb = keep - u0 < TR_B ? keep - u0 : TR_B;
+        float w[TR_B];
+        __syncthreads();
+        for (int x = tid; x < nb * DK; x += blockDim.x) {
+            const int u = x / DK, i = x % DK;
+            pk[u][i + 4 * (i / DK4)] = pend[((size_t)(u0 + u) * heads + h) * logw + i];
+        }
+        if (tid < nb) pdec[tid] = pend[((size_t)(u0 + tid) * heads + h) * logw + DK + dv];
+#pragma unroll
+        for (int u = 0; u < TR_B; u++) w[u] = pend[((size_t)(u0 + (u < nb ? u : nb - 1)) * heads + h) * logw + DK + (owner ? j0 + c : 0)];
+        __syncthreads();
+        for (int u = 0; u < TR_B; u++) {
+            if (u >= nb) break;
+            const float d = pdec[u];
+            float wu = w[0];
+#pragma unroll
+            for (int i = 1; i < TR_B; i++) wu = i == u ? w[i] : wu;
+            const float *k = &pk[u][gq * (DK4 + 4)];
+#pragma unroll
+            for (int i = 0; i < DK4 / 4; i++) {
+                const float4 x = *(const float4 *)(k + 4 * i);
+                s[i].x = s[i].x * d, s[i].y = s[i].y * d, s[i].z = s[i].z * d, s[i].w = s[i].w * d;
+                s[i].x = s[i].x + x.x * wu, s[i].y = s[i].y + x.y * wu, s[i].z = s[i].z + x.z * wu, s[i].w = s[i].w + x.w * wu;
+            }
+        }
+    }
+}
+__device__ __forceinline__ int keep_of(int keep, const int32_t *keep_dev) {
+    if (!keep_dev) return keep;
+    const int d = *keep_dev;
+    return d < keep ? d : keep;
+}
+
+/* More than 16 nodes: one workgroup per head and 16 value columns (a group of the state's layout), a wave
+ * per 16 nodes. The state's columns are a matrix operand as they lie: lane (column c, quarter gq)
+ * holds the float4 slots of keys gq dk/4 .. of its column, and the rows of k and q are read in the
+ * same order. */
 template <int DK4>
 __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
-    constexpr int DK = 4 * DK4, NS = DK4 / 4;
-    __shared__ float kk[NMX_TREE_MAX][NMX_TREE_MAX + 1], qk[NMX_TREE_MAX][NMX_TREE_MAX + 1];
-    __shared__ float del[NMX_TREE_MAX][16], pk[TR_B][DK], pdel[TR_B][16], pdec[TR_B];
-    __shared__ float dec[NMX_TREE_MAX], bet[NMX_TREE_MAX], run[6][NMX_TREE_MAX], gs[NMX_TREE_MAX];
-    __shared__ int up[6][NMX_TREE_MAX];
-    __shared__ unsigned long long sets[NMX_TREE_MAX];
-    const int h = blockIdx.x, j0 = blockIdx.y * 16, tid = threadIdx.x, lane = tid & 63, T = tid >> 6;
-    const int c = lane & 15, gq = lane >> 4, n = a.n, heads = a.heads, dv = a.dv;
+    constexpr int DK = 4 * DK4, NS = DK4 / 4, RS = DK + 4;
+    extern __shared__ float4 smem4[];
+    __shared__ TreeTables tt;
+    __shared__ float del[2][NMX_TREE_MAX][16], pdec[TR_B];
+    const int h = blockIdx.x, j0 = blockIdx.y * 16, tid = threadIdx.x, lane = tid & 63, T = tid >> 6, waves = blockDim.x >> 6;
+    const int c = lane & 15, gq = lane >> 4, n = a.n, heads = a.heads, dv = a.dv, n16 = 16 * waves;
+    constexpr bool QL = DK4 < 64;                   /* rows of q in LDS too; of 256 keys read where they lie */
+    float *ks = (float *)smem4, *qs = ks + n16 * RS; /* [n16][RS] rows of k, then of q */
+    float2 *co = (float2 *)(QL ? qs + n16 * RS : qs); /* [n16][n16 + 1]: D k.k, D q.k */
+    float(*pk)[DK + 16] = (float(*)[DK + 16])co;                /* pending keys, before the products */
     const size_t logw = (size_t)DK + dv + 1;
     const int kh = h / a.rep;
 
@@ -159,138 +276,113 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
     float *Sp = a.S + ((size_t)h * dv + j0) * DK + (4 * c + gq) * 4;
 #pragma unroll
     for (int k = 0; k < NS; k++) s[k] = *(const float4 *)(Sp + k * 256);
-
-    /* operands of this wave's nodes: row 16 T + c, keys gq DK4 + 4 k + e */
-    const int tn = 16 * T + c;
-    const float *row = a.qkv + (size_t)(tn < n ? tn : n - 1) * a.C + kh * DK + gq * DK4;
-    float4 kf[NS], qf[NS];
+    /* rows past the end repeat the last one: their products are not used */
+    for (int x0 = 0; x0 < n16 * (DK / 4); x0 += 4 * blockDim.x) {
+        float4 kb[4], qb[4];
 #pragma unroll
-    for (int k = 0; k < NS; k++) kf[k] = *(const float4 *)(row + a.kd + 4 * k), qf[k] = *(const float4 *)(row + 4 * k);
-
-    if (T == 0) { /* the tree: sets, decays over 2^k steps, the decays from the state */
-        int p;
-        const unsigned long long set = tree_ancestors(a.parent, n, &p);
-        sets[lane] = set;
-        const float d = lane < n ? a.decay[lane * heads + h] : 1.0f;
-        dec[lane] = d;
-        bet[lane] = lane < n ? a.beta[lane * heads + h] : 0.0f;
-        float r = d;
-        int q = p;
-#pragma unroll
-        for (int k = 0; k < 6; k++) {
-            run[k][lane] = r, up[k][lane] = q;
-            const int from = q < 0 ? lane : q;
-            const float ro = __shfl(r, from);
-            const int qo = __shfl(q, from);
-            if (q >= 0) r *= ro, q = qo;
+        for (int u = 0; u < 4; u++) {
+            const int x = x0 + u * (int)blockDim.x + tid, t = x / (DK / 4), i = x % (DK / 4) * 4;
+            const float *row = a.qkv + (size_t)(t < n ? t : n - 1) * a.C + kh * DK + i;
+            qb[u] = *(const float4 *)row, kb[u] = *(const float4 *)(row + a.kd);
         }
-        gs[lane] = r; /* every node is at most 63 steps from the state */
-    }
-
-    /* the updates of the last commit, as nmx_lin_apply makes them */
-    int keep = a.keep;
-    if (a.keep_dev) {
-        const int kd = *a.keep_dev;
-        keep = kd < keep ? kd : keep;
-    }
-    for (int u0 = 0; u0 < keep; u0 += TR_B) {
-        const int nb = keep - u0 < TR_B ? keep - u0 : TR_B;
-        __syncthreads();
-        for (int x = tid; x < nb * DK; x += blockDim.x) pk[x / DK][x % DK] = a.pend[((size_t)(u0 + x / DK) * heads + h) * logw + x % DK];
-        for (int x = tid; x < nb * 16; x += blockDim.x) pdel[x >> 4][x & 15] = a.pend[((size_t)(u0 + (x >> 4)) * heads + h) * logw + DK + j0 + (x & 15)];
-        if (tid < nb) pdec[tid] = a.pend[((size_t)(u0 + tid) * heads + h) * logw + DK + dv];
-        __syncthreads();
-        for (int u = 0; u < nb; u++) {
-            const float d = pdec[u], w = pdel[u][c];
-            const float *k = &pk[u][gq * DK4];
 #pragma unroll
-            for (int i = 0; i < NS; i++) {
-                const float4 x = *(const float4 *)(k + 4 * i);
-                s[i].x = s[i].x * d, s[i].y = s[i].y * d, s[i].z = s[i].z * d, s[i].w = s[i].w * d;
-                s[i].x = s[i].x + x.x * w, s[i].y = s[i].y + x.y * w, s[i].z = s[i].z + x.z * w, s[i].w = s[i].w + x.w * w;
-            }
+        for (int u = 0; u < 4; u++) {
+            const int x = x0 + u * (int)blockDim.x + tid, t = x / (DK / 4), i = x % (DK / 4) * 4;
+            if (t >= n16) continue;
+            *(float4 *)(ks + t * RS + i) = kb[u];
+            if (QL) *(float4 *)(qs + t * RS + i) = qb[u];
         }
     }
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int t = 16 * T + 4 * gq + j;
+        v[j] = a.qkv[(size_t)(t < n ? t : n - 1) * a.C + 2 * a.kd + h * dv + j0 + c];
+    }
+    if (T == waves - 1) tree_tables(tt, a.parent, n, lane < n ? a.decay[lane * heads + h] : 1.0f, lane < n ? a.beta[lane * heads + h] : 0.0f);
+    const int keep = keep_of(a.keep, a.keep_dev);
+    replay<DK4>(s, a.pend, keep, heads, h, logw, dv, j0, pk, pdec, true);
     if (keep > 0 && T == 0) {
 #pragma unroll
         for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
     }
+    __syncthreads();
 
+    auto q_row = [&](int t) { /* quarter gq of node t's q */
+        if constexpr (QL) return (const float *)(qs + t * RS + gq * DK4);
+        else return a.qkv + (size_t)(t < n ? t : n - 1) * a.C + kh * DK + gq * DK4;
+    };
     /* S^T k and S^T q of the wave's nodes: element j is node 16 T + 4 gq + j, column c */
-    f32x4 ks = {0.0f, 0.0f, 0.0f, 0.0f}, qs = ks;
-#pragma unroll
-    for (int k = 0; k < NS; k++) {
-        ks = mfma4(kf[k].x, s[k].x, ks), qs = mfma4(qf[k].x, s[k].x, qs);
-        ks = mfma4(kf[k].y, s[k].y, ks), qs = mfma4(qf[k].y, s[k].y, qs);
-        ks = mfma4(kf[k].z, s[k].z, ks), qs = mfma4(qf[k].z, s[k].z, qs);
-        ks = mfma4(kf[k].w, s[k].w, ks), qs = mfma4(qf[k].w, s[k].w, qs);
-    }
-    __syncthreads(); /* the tree's tables */
-    /* D(t, a) (k_t . k_a) and D(t, a) (q_t . k_a), t of this wave, a of tile U */
-    for (int U = 0; U <= T; U++) {
-        const int an = 16 * U + c;
-        const float *ar = a.qkv + (size_t)(an < n ? an : n - 1) * a.C + a.kd + kh * DK + gq * DK4;
-        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+    f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
+    {
+        const float *kr = ks + (16 * T + c) * RS + gq * DK4, *qr = q_row(16 * T + c);
 #pragma unroll
         for (int k = 0; k < NS; k++) {
-            const float4 b = *(const float4 *)(ar + 4 * k);
-            x = mfma4(kf[k].x, b.x, x), y = mfma4(qf[k].x, b.x, y);
-            x = mfma4(kf[k].y, b.y, x), y = mfma4(qf[k].y, b.y, y);
-            x = mfma4(kf[k].z, b.z, x), y = mfma4(qf[k].z, b.z, y);
-            x = mfma4(kf[k].w, b.w, x), y = mfma4(qf[k].w, b.w, y);
+            const float4 x = *(const float4 *)(kr + 4 * k), y = *(const float4 *)(qr + 4 * k);
+            sk = mfma4(x.x, s[k].x, sk), sq = mfma4(y.x, s[k].x, sq);
+            sk = mfma4(x.y, s[k].y, sk), sq = mfma4(y.y, s[k].y, sq);
+            sk = mfma4(x.z, s[k].z, sk), sq = mfma4(y.z, s[k].z, sq);
+            sk = mfma4(x.w, s[k].w, sk), sq = mfma4(y.w, s[k].w, sq);
         }
+    }
+    /* D(t, a) (k_t . k_a) and D(t, a) (q_t . k_a): the tiles (t, a) on and below the diagonal, in turn */
+    for (int job = T, X = 0; X < waves; job -= X + 1, X++) {
+        for (; job <= X; job += waves) {
+            const int U = job;
+            const float *ar = ks + (16 * U + c) * RS + gq * DK4;
+            const f32x4 x = row_products<NS>(ks + (16 * X + c) * RS + gq * DK4, ar);
+            const f32x4 y = row_products<NS>(q_row(16 * X + c), ar);
+            const int an = 16 * U + c;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 16 * T + 4 * gq + j;
-            if (t >= n || !(sets[t] >> an & 1)) continue;
-            const int steps = __popcll(sets[t]) - __popcll(sets[an]);
-            float d = 1.0f;
-            int at = t;
-#pragma unroll
-            for (int k = 0; k < 6; k++)
-                if (steps >> k & 1) d *= run[k][at], at = up[k][at];
-            kk[t][an] = x[j] * d, qk[t][an] = y[j] * d;
+            for (int j = 0; j < 4; j++) {
+                const int t = 16 * X + 4 * gq + j;
+                if (t >= n || !(tt.sets[t] >> an & 1)) continue;
+                const float d = tree_gap(tt, t, an);
+                co[t * (n16 + 1) + an] = make_float2(x[j] * d, y[j] * d);
+            }
         }
     }
     __syncthreads();
-    /* the deltas, level by level */
+    /* the deltas, level by level; a level's ancestor and coefficients are at hand before its deltas are */
     unsigned long long left[4];
-    float r[4], o[4];
-    int depth[4], levels = 0;
+    float r[4], o[4], bt[4];
+    float2 cf[4];
+    int depth[4], an[4];
+    const int levels = tt.levels;
+    auto next = [&](int j) {
+        an[j] = left[j] ? __ffsll((long long)left[j]) - 1 : 0; /* ancestors in order of depth */
+        left[j] &= left[j] - 1;
+        const int t = 16 * T + 4 * gq + j;
+        cf[j] = co[t * (n16 + 1) + an[j]];
+    };
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int t = 16 * T + 4 * gq + j;
-        left[j] = t < n ? sets[t] : 0;
-        depth[j] = t < n ? __popcll(sets[t]) - 1 : -1;
-        const float v = t < n ? a.qkv[(size_t)t * a.C + 2 * a.kd + h * dv + j0 + c] : 0.0f;
-        const float g = t < n ? gs[t] : 0.0f;
-        r[j] = v - g * ks[j], o[j] = g * qs[j];
-    }
-    for (int t = 0; t < n; t++) { /* uniform: the deepest node */
-        const int d = __popcll(sets[t]);
-        levels = d > levels ? d : levels;
+        const bool in = t < n;
+        left[j] = in ? tt.sets[t] : 0;
+        depth[j] = in ? __popcll(left[j]) - 1 : -1;
+        const float g = in ? tt.gs[t] : 0.0f;
+        bt[j] = in ? tt.bet[t] : 0.0f;
+        r[j] = v[j] - g * sk[j], o[j] = g * sq[j];
+        next(j);
     }
     for (int d = 0; d < levels; d++) {
+        float(*dl)[16] = del[d & 1]; /* read in this level while the next one is written */
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 16 * T + 4 * gq + j;
+        for (int j = 0; j < 4; j++)
             if (depth[j] == d) {
-                r[j] = r[j] * bet[t];
-                del[t][c] = r[j];
+                r[j] = r[j] * bt[j];
+                dl[16 * T + 4 * gq + j][c] = r[j];
             }
-        }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 16 * T + 4 * gq + j;
+        for (int j = 0; j < 4; j++)
             if (depth[j] >= d) {
-                const int an = __ffsll((long long)left[j]) - 1; /* ancestors in order of depth */
-                left[j] &= left[j] - 1;
-                const float x = del[an][c];
-                o[j] = o[j] + qk[t][an] * x;
-                if (depth[j] > d) r[j] = r[j] - kk[t][an] * x;
+                const float x = dl[an[j]][c];
+                o[j] = o[j] + cf[j].y * x;
+                if (depth[j] > d) r[j] = r[j] - cf[j].x * x;
+                next(j);
             }
-        }
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -301,16 +393,243 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
         }
     }
     if (j0 == 0) { /* the log rows' keys and decays */
-        for (int x = tid; x < n * DK; x += blockDim.x)
-            a.log[((size_t)(x / DK) * heads + h) * logw + x % DK] = a.qkv[(size_t)(x / DK) * a.C + a.kd + kh * DK + x % DK];
-        if (tid < n) a.log[((size_t)tid * heads + h) * logw + DK + dv] = dec[tid];
+        for (int x = tid; x < n * DK; x += blockDim.x) a.log[((size_t)(x / DK) * heads + h) * logw + x % DK] = ks[x / DK * RS + x % DK];
+        if (tid < n) a.log[((size_t)tid * heads + h) * logw + DK + dv] = tt.dec[tid];
+    }
+}
+
+/* Up to 16 nodes: the whole mixer of a head in one workgroup and one launch, a wave per 16 value columns.
+ * The raw rows lie in LDS, where each channel's thread reads its windows and then puts its outputs in
+ * their place (the last node first: nodes read their ancestors' raw values, which lie before them);
+ * o replaces v there in turn, for the gated norm over the head. */
+constexpr int TO_N = 16, TO_ROWS = TO_N + 7; /* nodes, then the conv state's rows */
+
+struct TreeOne {
+    TreePre p;
+    TreeRule r;
+    const float *z, *norm_w;
+    int z_stride, y_stride;
+    float eps;
+    float *y;
+    int8_t *aq;
+    float *ad, *afs;
+};
+
+template <int DK4>
+__global__ __launch_bounds__(1024) void lin_tree_one_k(TreeOne a) {
+    constexpr int DK = 4 * DK4, NS = DK4 / 4;
+    extern __shared__ float4 smem4[];
+    __shared__ TreeTables tt;
+    __shared__ float2 co[TO_N][TO_N + 1];
+    __shared__ float pk[TR_B][DK + 16], pdec[TR_B], red[4 * 2 * TO_N];
+    __shared__ int par[TO_N];
+    const TreePre &p = a.p;
+    const TreeRule &q = a.r;
+    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, gq = lane >> 4;
+    const int n = p.n, heads = q.heads, dv = q.dv, K = p.K, S = K - 1, kh = h / q.rep, T = blockDim.x;
+    const int CH = 2 * DK + dv, RS = CH + 4, j0 = 16 * w;
+    const size_t logw = (size_t)DK + dv + 1;
+    float *xs = (float *)smem4; /* [TO_ROWS][RS]: q | k | v of a row */
+    const bool owner = j0 < dv; /* the wave has value columns */
+
+    /* requests: the channel's raw rows, conv rows and taps, the wave's state columns */
+    const bool chan = tid < CH;
+    const int ch = !chan ? 0 : tid < DK ? kh * DK + tid : tid < 2 * DK ? p.kd + kh * DK + tid - DK : 2 * p.kd + h * dv + tid - 2 * DK;
+    float x[TO_N], st[7], wc[8];
+#pragma unroll
+    for (int t = 0; t < TO_N; t++) x[t] = p.raw[(size_t)(t < n ? t : n - 1) * p.raw_stride + ch];
+#pragma unroll
+    for (int r = 0; r < 7; r++) st[r] = r < S ? p.state[(size_t)r * p.C + ch] : 0.0f;
+#pragma unroll
+    for (int r = 0; r < 8; r++) wc[r] = r < K ? p.conv_w[(size_t)ch * K + r] : 0.0f;
+    if (tid < n) par[tid] = tree_parent(p.parent, tid);
+    float4 s[NS];
+    float *Sp = q.S + ((size_t)h * dv + (owner ? j0 : 0)) * DK + (4 * c + gq) * 4;
+#pragma unroll
+    for (int k = 0; k < NS; k++) s[k] = *(const float4 *)(Sp + k * 256);
+    if (chan) {
+#pragma unroll
+        for (int t = 0; t < TO_N; t++) xs[t * RS + tid] = x[t];
+#pragma unroll
+        for (int r = 0; r < 7; r++)
+            if (r < S) xs[(TO_N + r) * RS + tid] = st[r];
+        if (p.xin) {
+#pragma unroll
+            for (int t = 0; t < TO_N; t++)
+                if (t < n) p.xin[(size_t)t * p.C + ch] = x[t];
+        }
+    }
+    if (w == (T >> 6) - 1) { /* the last wave, which has no channels: gates and the tree */
+        float bt = 0.0f, d = 1.0f;
+        if (lane < n) {
+            bt = tree_beta(p.b_in[(size_t)lane * p.g_stride + h]);
+            d = tree_decay(p, p.a_in[(size_t)lane * p.g_stride + h], h);
+            p.beta[lane * heads + h] = bt, p.decay[lane * heads + h] = d;
+        }
+        tree_tables(tt, p.parent, n, d, bt);
+    }
+    __syncthreads();
+    if (chan) { /* conv + SiLU, 4 nodes at a time from the last down */
+        for (int t1 = n - 1; t1 >= 0; t1 -= 4) {
+            float acc[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                int at = t1 - u < 0 ? 0 : t1 - u, row = S;
+                float win[8];
+#pragma unroll
+                for (int r = 0; r < 8; r++) { /* the r-th newest */
+                    if (r >= K) break;
+                    const bool node = at >= 0;
+                    row -= !node;
+                    win[r] = xs[(node ? at : TO_N + row) * RS + tid];
+                    at = node ? par[at] : at;
+                }
+                float y = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) { /* taps in order, the oldest first */
+                    if (j >= K) break;
+                    float v = win[0];
+#pragma unroll
+                    for (int r = 1; r < 8; r++) v = r == K - 1 - j ? win[r] : v;
+                    y = j ? y + wc[j] * v : wc[0] * v;
+                }
+                acc[u] = nmx_silu(y);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                if (t1 - u >= 0) xs[(t1 - u) * RS + tid] = acc[u];
+        }
+    }
+    const int keep = keep_of(q.keep, q.keep_dev);
+    replay<DK4>(s, q.pend, keep, heads, h, logw, dv, j0, pk, pdec, owner);
+    if (keep > 0 && owner) {
+#pragma unroll
+        for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
+    }
+    __syncthreads();
+    /* L2 norms of the q and k rows: 4 chains each */
+    for (int i = tid; i < 8 * n; i += T) red[i] = square_chain(xs + (i >> 3) * RS + (i >> 2 & 1) * DK + (i & 3), DK >> 2);
+    __syncthreads();
+    for (int i = tid; i < n * 2 * DK; i += T) {
+        const int t = i / (2 * DK), e = i % (2 * DK);
+        const float *rd = red + 8 * t + (e < DK ? 0 : 4);
+        const float ss = ((rd[0] + rd[1]) + (rd[2] + rd[3])) + 0.0f, r = 1.0f / sqrtf(ss + p.l2eps);
+        xs[t * RS + e] = (xs[t * RS + e] * r) * (e < DK ? p.qscale : 1.0f);
+    }
+    __syncthreads();
+    for (int i = tid; i < n * CH; i += T) { /* what is kept of the pass: conv outputs, the log rows' keys */
+        const int t = i / CH, e = i % CH;
+        const float v = xs[t * RS + e];
+        p.out[(size_t)t * p.C + (e < DK ? kh * DK + e : e < 2 * DK ? p.kd + kh * DK + e - DK : 2 * p.kd + h * dv + e - 2 * DK)] = v;
+        if (e >= DK && e < 2 * DK) q.log[((size_t)t * heads + h) * logw + e - DK] = v;
+    }
+    if (tid < n) q.log[((size_t)tid * heads + h) * logw + DK + dv] = tt.dec[tid];
+    /* products: rows past the end hold raw values, and are not used */
+    const float *qr = xs + c * RS + gq * DK4, *kr = qr + DK;
+    f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
+    if (owner) {
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+            const float4 x4 = *(const float4 *)(kr + 4 * k), y4 = *(const float4 *)(qr + 4 * k);
+            sk = mfma4(x4.x, s[k].x, sk), sq = mfma4(y4.x, s[k].x, sq);
+            sk = mfma4(x4.y, s[k].y, sk), sq = mfma4(y4.y, s[k].y, sq);
+            sk = mfma4(x4.z, s[k].z, sk), sq = mfma4(y4.z, s[k].z, sq);
+            sk = mfma4(x4.w, s[k].w, sk), sq = mfma4(y4.w, s[k].w, sq);
+        }
+    }
+    for (int job = w; job < 2; job += T >> 6) { /* D k.k and D q.k */
+        const f32x4 x4 = row_products<NS>(job ? qr : kr, kr);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int t = 4 * gq + j;
+            if (t >= n || !(tt.sets[t] >> c & 1)) continue;
+            const float d = x4[j] * tree_gap(tt, t, c);
+            if (job) co[t][c].y = d;
+            else co[t][c].x = d;
+        }
+    }
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = owner ? xs[(4 * gq + j) * RS + 2 * DK + j0 + c] : 0.0f;
+    __syncthreads();
+    float *del = xs + 2 * DK + j0 + c; /* this lane's column: deltas where v was, then o */
+    if (owner) {
+        unsigned long long left[4];
+        float r[4], o[4];
+        int depth[4];
+        const int levels = tt.levels;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int t = 4 * gq + j;
+            left[j] = t < n ? tt.sets[t] : 0;
+            depth[j] = t < n ? __popcll(left[j]) - 1 : -1;
+            const float g = t < n ? tt.gs[t] : 0.0f;
+            r[j] = v[j] - g * sk[j], o[j] = g * sq[j];
+        }
+        for (int d = 0; d < levels; d++) { /* the wave's columns are its own: no barrier */
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (depth[j] == d) {
+                    r[j] = r[j] * tt.bet[4 * gq + j];
+                    del[(4 * gq + j) * RS] = r[j];
+                }
+            nmx_lds_wave_sync();
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (depth[j] >= d) {
+                    const int an = __ffsll((long long)left[j]) - 1; /* ancestors in order of depth */
+                    left[j] &= left[j] - 1;
+                    const float xd = del[an * RS];
+                    const float2 cf = co[4 * gq + j][an];
+                    o[j] = o[j] + cf.y * xd;
+                    if (depth[j] > d) r[j] = r[j] - cf.x * xd;
+                }
+        }
+        nmx_lds_wave_sync();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int t = 4 * gq + j;
+            if (t >= n) continue;
+            del[t * RS] = o[j];
+            q.o[(size_t)t * q.o_stride + h * dv + j0 + c] = o[j];
+            q.log[((size_t)t * heads + h) * logw + DK + j0 + c] = r[j];
+        }
+    }
+    __syncthreads();
+    /* the gated RMSNorm over the head, as lin_post_k makes it */
+    for (int i = tid; i < 4 * n; i += T) red[i] = square_chain(xs + (i >> 2) * RS + 2 * DK + (i & 3), dv >> 2);
+    __syncthreads();
+    const int nd = n * dv; /* whole half-waves: dv % 32 == 0 */
+    for (int i = tid; i < nd; i += T) {
+        const int t = i / dv, j = i % dv, col = h * dv + j;
+        const float *rd = red + 4 * t;
+        const float ss = ((rd[0] + rd[1]) + (rd[2] + rd[3])) + 0.0f, r = 1.0f / sqrtf(ss / (float)dv + a.eps);
+        float y = (xs[t * RS + 2 * DK + j] * r) * a.norm_w[j];
+        y = y * nmx_silu(a.z[(size_t)t * a.z_stride + col]);
+        if (a.y) a.y[(size_t)t * a.y_stride + col] = y;
+        if (a.aq) a8_block(y, col >> 5, t, n, a.aq, a.ad, a.afs);
     }
 }
 
 template <int DK4>
+int launch_one(nmx_ctx *ctx, const TreeOne &a, int threads, size_t lds) {
+    static std::atomic<uint64_t> set;
+    if (nmx_dyn_lds(ctx, (const void *)lin_tree_one_k<DK4>, (size_t)TO_ROWS * (8 * DK4 + 256 + 4) * 4, set)) return -1;
+    lin_tree_one_k<DK4><<<(unsigned)a.r.heads, (unsigned)threads, lds, ctx->stream>>>(a);
+    NMX_LAUNCHED(ctx, "lin_tree_one");
+    return 0;
+}
+
+template <int DK4>
 int launch_rule(nmx_ctx *ctx, const TreeRule &a) {
-    lin_tree_rule_k<DK4><<<dim3((unsigned)a.heads, (unsigned)(a.dv / 16)), (unsigned)((a.n + 15) / 16 * 64), 0,
-                           ctx->stream>>>(a);
+    const int n16 = (a.n + 15) / 16 * 16;
+    auto bytes = [](int m) {
+        const size_t co = (size_t)m * (m + 1) * 8, pk = (size_t)TR_B * (4 * DK4 + 16) * 4;
+        return (size_t)(DK4 < 64 ? 2 : 1) * m * (4 * DK4 + 4) * 4 + (co > pk ? co : pk);
+    };
+    static std::atomic<uint64_t> set;
+    if (nmx_dyn_lds(ctx, (const void *)lin_tree_rule_k<DK4>, bytes(64), set)) return -1;
+    lin_tree_rule_k<DK4><<<dim3((unsigned)a.heads, (unsigned)(a.dv / 16)), (unsigned)(4 * n16), bytes(n16), ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "lin_tree_rule");
     return 0;
 }
@@ -361,11 +680,21 @@ int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *m, const int32_t *par
     const nmx_on_device on(ctx);
     const TreePre a{n, p.C, p.conv_k, dk, p.kd, p.raw, p.raw_stride, p.out, p.state, p.conv_w, p.xin, p.qscale, p.l2eps,
                     p.b_in, p.a_in, p.g_stride, heads, p.A_log, p.A, p.dt_bias, p.beta, p.decay, parent};
-    lin_tree_pre_k<<<dim3((unsigned)((p.C + dk - 1) / dk + 1), (unsigned)((n + TP_N - 1) / TP_N)),
-                     (unsigned)(dk < 64 ? 64 : dk), (size_t)TP_N * dk * 4, ctx->stream>>>(a);
-    NMX_LAUNCHED(ctx, "lin_tree_pre");
     const TreeRule t{n, heads, r.rep, dv, p.kd, p.C, p.out, p.beta, p.decay, r.S, r.o, r.o_stride, r.log, r.pend, r.keep,
                      r.keep_dev, parent};
+    const int ch_waves = (2 * dk + dv + 63) / 64 + 1, waves = dv / 16 > ch_waves ? dv / 16 : ch_waves;
+    if (n <= TO_N && dk <= 128 && waves <= 16) {
+        const TreeOne o{a, t, m->z, m->norm_w, m->z_stride, m->y_stride, m->eps, m->y, m->a8.q, m->a8.d, m->a8.fs};
+        const size_t lds = (size_t)TO_ROWS * (2 * dk + dv + 4) * 4;
+        return dk == 32 ? launch_one<8>(ctx, o, 64 * waves, lds) : dk == 64 ? launch_one<16>(ctx, o, 64 * waves, lds) :
+                          launch_one<32>(ctx, o, 64 * waves, lds);
+    }
+    const dim3 grid((unsigned)((p.C + dk - 1) / dk + 1), (unsigned)((n + TP_N - 1) / TP_N));
+    const unsigned threads = dk < 64 ? 64 : (unsigned)dk;
+    const size_t lds = (size_t)TP_N * (dk + 4) * 4;
+    if (p.conv_k == 4) lin_tree_pre_k<4><<<grid, threads, lds, ctx->stream>>>(a);
+    else lin_tree_pre_k<0><<<grid, threads, lds, ctx->stream>>>(a);
+    NMX_LAUNCHED(ctx, "lin_tree_pre");
     const int rc = dk == 32 ? launch_rule<8>(ctx, t) : dk == 64 ? launch_rule<16>(ctx, t) :
                    dk == 128 ? launch_rule<32>(ctx, t) : launch_rule<64>(ctx, t);
     if (rc) return rc;

@@ -156,6 +156,7 @@ struct TreeRule {
     const float *pend;
     int keep;
     const int32_t *keep_dev, *parent;
+    float qscale;
 };
 
 constexpr int TR_B = 8; /* pending rows staged at a time */
@@ -200,53 +201,73 @@ __device__ __forceinline__ float tree_gap(const TreeTables &s, int t, int a) {
     return d;
 }
 
-/* A lane's 16 x 16 piece of x y^T over DK4 4 columns: rows of x and y in LDS, quarter gq of the columns
- * to a lane (the state's order of keys). */
-template <int NS>
-__device__ __forceinline__ f32x4 row_products(const float *x, const float *y) {
-    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int k = 0; k < NS; k++) {
-        const float4 u = *(const float4 *)(x + 4 * k), v = *(const float4 *)(y + 4 * k);
-        r = mfma4(u.x, v.x, r), r = mfma4(u.y, v.y, r), r = mfma4(u.z, v.z, r), r = mfma4(u.w, v.w, r);
-    }
-    return r;
+/* Rows of k and q for the products of nodes: as two binary16 parts each, which together hold 22 bits of
+ * the row's largest element (k has norm 1, q norm qscale: brought to 2^6 first), so that a product of rows
+ * is three 16-bit matrix instructions per 32 keys in place of 32 32-bit ones; the low-low part, 2^-22, is
+ * left out. */
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ void split4(float4 x, float up, _Float16 *hi, _Float16 *lo) {
+    const float v[4] = {x.x * up, x.y * up, x.z * up, x.w * up};
+    half4 h, l;
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = (_Float16)v[i], l[i] = (_Float16)(v[i] - (float)h[i]);
+    *(half4 *)hi = h, *(half4 *)lo = l;
+}
+constexpr float TR_UP = 64.0f;
 
-/* Pending rows u0 .. of head h into the state's columns held in s, as nmx_lin_apply makes them. */
-template <int DK4>
-__device__ __forceinline__ void replay(float4 (&s)[DK4 / 4], const float *pend, int keep, int heads, int h, size_t logw, int dv,
-                                       int j0, float (*pk)[4 * DK4 + 16], float *pdec, bool owner) {
-    constexpr int DK = 4 * DK4;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, gq = lane >> 4;
-    for (int u0 = 0; u0 < keep; u0 += TR_B) {
+/* The pending rows of head h, TR_B at a time: keys and decays to LDS (pk, pdec), the deltas of column
+ * col to registers. The first batch is requested at the kernel's entry, among its other requests. */
+template <int DK4, int TMIN>
+struct Replay {
+    static constexpr int DK = 4 * DK4, NP = (TR_B * DK + TMIN - 1) / TMIN; /* TMIN: the least threads of a workgroup */
+    float k[NP], w[TR_B], d;
+    __device__ __forceinline__ void ask(const float *pend, int u0, int keep, int heads, int h, size_t logw, int col) {
         const int nb = keep - u0 < TR_B ? keep - u0 : TR_B;
-        float w[TR_B];
-        __syncthreads();
-        for (int x = tid; x < nb * DK; x += blockDim.x) {
-            const int u = x / DK, i = x % DK;
-            pk[u][i + 4 * (i / DK4)] = pend[((size_t)(u0 + u) * heads + h) * logw + i];
+        if (nb <= 0) return;
+        auto row = [&](int u) { return pend + ((size_t)(u0 + (u < nb ? u : nb - 1)) * heads + h) * logw; };
+#pragma unroll
+        for (int e = 0; e < NP; e++) {
+            const int x = e * (int)blockDim.x + (int)threadIdx.x;
+            k[e] = row(x / DK)[x % DK];
         }
-        if (tid < nb) pdec[tid] = pend[((size_t)(u0 + tid) * heads + h) * logw + DK + dv];
 #pragma unroll
-        for (int u = 0; u < TR_B; u++) w[u] = pend[((size_t)(u0 + (u < nb ? u : nb - 1)) * heads + h) * logw + DK + (owner ? j0 + c : 0)];
-        __syncthreads();
-        for (int u = 0; u < TR_B; u++) {
-            if (u >= nb) break;
-            const float d = pdec[u];
-            float wu = w[0];
+        for (int u = 0; u < TR_B; u++) w[u] = row(u)[DK + col];
+        d = row(threadIdx.x < TR_B ? threadIdx.x : 0)[logw - 1];
+    }
+    /* into the state's columns held in s, as nmx_lin_apply makes them */
+    __device__ __forceinline__ void run(float4 (&s)[DK4 / 4], const float *pend, int asked, int keep, int heads, int h, size_t logw,
+                                        int col, float (*pk)[DK + 16], float *pdec) {
+        const int tid = threadIdx.x, gq = (tid & 63) >> 4;
+        for (int u0 = 0; u0 < keep; u0 += TR_B) {
+            if (u0) ask(pend, u0, asked, heads, h, logw, col);
+            const int nb = keep - u0 < TR_B ? keep - u0 : TR_B;
+            __syncthreads();
 #pragma unroll
-            for (int i = 1; i < TR_B; i++) wu = i == u ? w[i] : wu;
-            const float *k = &pk[u][gq * (DK4 + 4)];
+            for (int e = 0; e < NP; e++) {
+                const int x = e * (int)blockDim.x + tid, i = x % DK;
+                if (x < TR_B * DK) pk[x / DK][i + 4 * (i / DK4)] = k[e];
+            }
+            if (tid < TR_B) pdec[tid] = d;
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < DK4 / 4; i++) {
-                const float4 x = *(const float4 *)(k + 4 * i);
-                s[i].x = s[i].x * d, s[i].y = s[i].y * d, s[i].z = s[i].z * d, s[i].w = s[i].w * d;
-                s[i].x = s[i].x + x.x * wu, s[i].y = s[i].y + x.y * wu, s[i].z = s[i].z + x.z * wu, s[i].w = s[i].w + x.w * wu;
+            for (int u = 0; u < TR_B; u++) {
+                if (u >= nb) continue;
+                const float dc = pdec[u];
+                const float *kr = &pk[u][gq * (DK4 + 4)];
+#pragma unroll
+                for (int i = 0; i < DK4 / 4; i++) {
+                    const float4 x = *(const float4 *)(kr + 4 * i);
+                    s[i].x = s[i].x * dc, s[i].y = s[i].y * dc, s[i].z = s[i].z * dc, s[i].w = s[i].w * dc;
+                    s[i].x = s[i].x + x.x * w[u], s[i].y = s[i].y + x.y * w[u], s[i].z = s[i].z + x.z * w[u], s[i].w = s[i].w + x.w * w[u];
+                }
             }
         }
     }
-}
+};
 __device__ __forceinline__ int keep_of(int keep, const int32_t *keep_dev) {
     if (!keep_dev) return keep;
     const int d = *keep_dev;
@@ -255,44 +276,34 @@ __device__ __forceinline__ int keep_of(int keep, const int32_t *keep_dev) {
 
 /* More than 16 nodes: one workgroup per head and 16 value columns (a group of the state's layout), a wave
  * per 16 nodes. The state's columns are a matrix operand as they lie: lane (column c, quarter gq)
- * holds the float4 slots of keys gq dk/4 .. of its column, and the rows of k and q are read in the
- * same order. */
+ * holds the float4 slots of keys gq dk/4 .. of its column, and the wave's rows of k and q are read in
+ * the same order. */
 template <int DK4>
 __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
-    constexpr int DK = 4 * DK4, NS = DK4 / 4, RS = DK + 4;
+    constexpr int DK = 4 * DK4, NS = DK4 / 4, HS = DK + 8; /* halves of a row in LDS: 16 bytes on, no bank twice */
     extern __shared__ float4 smem4[];
     __shared__ TreeTables tt;
     __shared__ float del[2][NMX_TREE_MAX][16], pdec[TR_B];
     const int h = blockIdx.x, j0 = blockIdx.y * 16, tid = threadIdx.x, lane = tid & 63, T = tid >> 6, waves = blockDim.x >> 6;
     const int c = lane & 15, gq = lane >> 4, n = a.n, heads = a.heads, dv = a.dv, n16 = 16 * waves;
-    constexpr bool QL = DK4 < 64;                   /* rows of q in LDS too; of 256 keys read where they lie */
-    float *ks = (float *)smem4, *qs = ks + n16 * RS; /* [n16][RS] rows of k, then of q */
-    float2 *co = (float2 *)(QL ? qs + n16 * RS : qs); /* [n16][n16 + 1]: D k.k, D q.k */
-    float(*pk)[DK + 16] = (float(*)[DK + 16])co;                /* pending keys, before the products */
+    _Float16 *kh2 = (_Float16 *)smem4, *qh2 = kh2 + 2 * n16 * HS;   /* [2][n16][HS]: high, low parts */
+    constexpr bool QL = DK4 < 64; /* 256 keys: the parts of q are made when they are used, LDS has no room */
+    float2 *co = (float2 *)(QL ? qh2 + 2 * n16 * HS : qh2);         /* [n16][n16 + 1]: D k.k, D q.k */
+    float(*pk)[DK + 16] = (float(*)[DK + 16])co;                    /* pending keys, before the products */
     const size_t logw = (size_t)DK + dv + 1;
     const int kh = h / a.rep;
 
-    float4 s[NS];
+    Replay<DK4, 128> rp;
+    rp.ask(a.pend, 0, a.keep, heads, h, logw, j0 + c);
+    float4 s[NS], kf[NS], qf[NS];
     float *Sp = a.S + ((size_t)h * dv + j0) * DK + (4 * c + gq) * 4;
 #pragma unroll
     for (int k = 0; k < NS; k++) s[k] = *(const float4 *)(Sp + k * 256);
     /* rows past the end repeat the last one: their products are not used */
-    for (int x0 = 0; x0 < n16 * (DK / 4); x0 += 4 * blockDim.x) {
-        float4 kb[4], qb[4];
+    const int tn = 16 * T + c;
+    const float *row = a.qkv + (size_t)(tn < n ? tn : n - 1) * a.C + kh * DK + gq * DK4;
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int x = x0 + u * (int)blockDim.x + tid, t = x / (DK / 4), i = x % (DK / 4) * 4;
-            const float *row = a.qkv + (size_t)(t < n ? t : n - 1) * a.C + kh * DK + i;
-            qb[u] = *(const float4 *)row, kb[u] = *(const float4 *)(row + a.kd);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int x = x0 + u * (int)blockDim.x + tid, t = x / (DK / 4), i = x % (DK / 4) * 4;
-            if (t >= n16) continue;
-            *(float4 *)(ks + t * RS + i) = kb[u];
-            if (QL) *(float4 *)(qs + t * RS + i) = qb[u];
-        }
-    }
+    for (int k = 0; k < NS; k++) kf[k] = *(const float4 *)(row + a.kd + 4 * k), qf[k] = *(const float4 *)(row + 4 * k);
     float v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -300,45 +311,62 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
         v[j] = a.qkv[(size_t)(t < n ? t : n - 1) * a.C + 2 * a.kd + h * dv + j0 + c];
     }
     if (T == waves - 1) tree_tables(tt, a.parent, n, lane < n ? a.decay[lane * heads + h] : 1.0f, lane < n ? a.beta[lane * heads + h] : 0.0f);
+    const float q_up = a.qscale != 0.0f ? TR_UP / a.qscale : 0.0f, q_down = a.qscale / (TR_UP * TR_UP);
+#pragma unroll
+    for (int k = 0; k < NS; k++) {
+        const int at = tn * HS + gq * DK4 + 4 * k;
+        split4(kf[k], TR_UP, kh2 + at, kh2 + n16 * HS + at);
+        if (QL) split4(qf[k], q_up, qh2 + at, qh2 + n16 * HS + at);
+    }
     const int keep = keep_of(a.keep, a.keep_dev);
-    replay<DK4>(s, a.pend, keep, heads, h, logw, dv, j0, pk, pdec, true);
+    rp.run(s, a.pend, a.keep, keep, heads, h, logw, j0 + c, pk, pdec);
     if (keep > 0 && T == 0) {
 #pragma unroll
         for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
     }
-    __syncthreads();
-
-    auto q_row = [&](int t) { /* quarter gq of node t's q */
-        if constexpr (QL) return (const float *)(qs + t * RS + gq * DK4);
-        else return a.qkv + (size_t)(t < n ? t : n - 1) * a.C + kh * DK + gq * DK4;
-    };
     /* S^T k and S^T q of the wave's nodes: element j is node 16 T + 4 gq + j, column c */
     f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
-    {
-        const float *kr = ks + (16 * T + c) * RS + gq * DK4, *qr = q_row(16 * T + c);
 #pragma unroll
-        for (int k = 0; k < NS; k++) {
-            const float4 x = *(const float4 *)(kr + 4 * k), y = *(const float4 *)(qr + 4 * k);
-            sk = mfma4(x.x, s[k].x, sk), sq = mfma4(y.x, s[k].x, sq);
-            sk = mfma4(x.y, s[k].y, sk), sq = mfma4(y.y, s[k].y, sq);
-            sk = mfma4(x.z, s[k].z, sk), sq = mfma4(y.z, s[k].z, sq);
-            sk = mfma4(x.w, s[k].w, sk), sq = mfma4(y.w, s[k].w, sq);
-        }
+    for (int k = 0; k < NS; k++) {
+        sk = mfma4(kf[k].x, s[k].x, sk), sq = mfma4(qf[k].x, s[k].x, sq);
+        sk = mfma4(kf[k].y, s[k].y, sk), sq = mfma4(qf[k].y, s[k].y, sq);
+        sk = mfma4(kf[k].z, s[k].z, sk), sq = mfma4(qf[k].z, s[k].z, sq);
+        sk = mfma4(kf[k].w, s[k].w, sk), sq = mfma4(qf[k].w, s[k].w, sq);
     }
+    __syncthreads(); /* the rows, the tables; the pending keys have been read */
     /* D(t, a) (k_t . k_a) and D(t, a) (q_t . k_a): the tiles (t, a) on and below the diagonal, in turn */
     for (int job = T, X = 0; X < waves; job -= X + 1, X++) {
         for (; job <= X; job += waves) {
-            const int U = job;
-            const float *ar = ks + (16 * U + c) * RS + gq * DK4;
-            const f32x4 x = row_products<NS>(ks + (16 * X + c) * RS + gq * DK4, ar);
-            const f32x4 y = row_products<NS>(q_row(16 * X + c), ar);
-            const int an = 16 * U + c;
+            const int U = job, an = 16 * U + c;
+            const _Float16 *ar = kh2 + an * HS + 8 * gq, *tr = kh2 + (16 * X + c) * HS + 8 * gq, *ur = qh2 + (16 * X + c) * HS + 8 * gq;
+            const int lo = n16 * HS;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+#pragma unroll
+            for (int k = 0; k < DK; k += 32) {
+                const half8 ah = *(const half8 *)(ar + k), al = *(const half8 *)(ar + lo + k);
+                const half8 th = *(const half8 *)(tr + k), tl = *(const half8 *)(tr + lo + k);
+                half8 uh, ul;
+                if constexpr (QL) {
+                    uh = *(const half8 *)(ur + k), ul = *(const half8 *)(ur + lo + k);
+                } else {
+                    const int t = 16 * X + c < n ? 16 * X + c : n - 1;
+                    const float *src = a.qkv + (size_t)t * a.C + kh * DK + k + 8 * gq;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float v = src[i] * q_up;
+                        uh[i] = (_Float16)v, ul[i] = (_Float16)(v - (float)uh[i]);
+                    }
+                }
+                x = mfma16(th, ah, x), y = mfma16(uh, ah, y);
+                x = mfma16(tl, ah, x), y = mfma16(ul, ah, y);
+                x = mfma16(th, al, x), y = mfma16(uh, al, y);
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int t = 16 * X + 4 * gq + j;
                 if (t >= n || !(tt.sets[t] >> an & 1)) continue;
                 const float d = tree_gap(tt, t, an);
-                co[t * (n16 + 1) + an] = make_float2(x[j] * d, y[j] * d);
+                co[t * (n16 + 1) + an] = make_float2(x[j] * (d * (1.0f / (TR_UP * TR_UP))), y[j] * (d * q_down));
             }
         }
     }
@@ -369,20 +397,21 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
     for (int d = 0; d < levels; d++) {
         float(*dl)[16] = del[d & 1]; /* read in this level while the next one is written */
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (depth[j] == d) {
-                r[j] = r[j] * bt[j];
-                dl[16 * T + 4 * gq + j][c] = r[j];
-            }
+        for (int j = 0; j < 4; j++) {
+            const bool now = depth[j] == d;
+            r[j] = now ? r[j] * bt[j] : r[j];
+            if (now) dl[16 * T + 4 * gq + j][c] = r[j];
+        }
         __syncthreads();
+        float x[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (depth[j] >= d) {
-                const float x = dl[an[j]][c];
-                o[j] = o[j] + cf[j].y * x;
-                if (depth[j] > d) r[j] = r[j] - cf[j].x * x;
-                next(j);
-            }
+        for (int j = 0; j < 4; j++) x[j] = dl[an[j]][c];
+#pragma unroll
+        for (int j = 0; j < 4; j++) { /* chosen, not multiplied away: a node past its depth reads anything */
+            o[j] = depth[j] >= d ? o[j] + cf[j].y * x[j] : o[j];
+            r[j] = depth[j] > d ? r[j] - cf[j].x * x[j] : r[j];
+            next(j);
+        }
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -392,9 +421,12 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
             a.log[((size_t)t * heads + h) * logw + DK + j0 + c] = r[j];
         }
     }
-    if (j0 == 0) { /* the log rows' keys and decays */
-        for (int x = tid; x < n * DK; x += blockDim.x) a.log[((size_t)(x / DK) * heads + h) * logw + x % DK] = ks[x / DK * RS + x % DK];
-        if (tid < n) a.log[((size_t)tid * heads + h) * logw + DK + dv] = tt.dec[tid];
+    /* the log rows' keys and decays, a share of them each */
+    for (int t = blockIdx.y; t < n; t += gridDim.y) {
+        const float *src = a.qkv + (size_t)t * a.C + a.kd + kh * DK;
+        float *dst = a.log + ((size_t)t * heads + h) * logw;
+        for (int i = tid; i < DK; i += blockDim.x) dst[i] = src[i];
+        if (tid == 0) dst[DK + dv] = tt.dec[t];
     }
 }
 
@@ -403,6 +435,7 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
  * their place (the last node first: nodes read their ancestors' raw values, which lie before them);
  * o replaces v there in turn, for the gated norm over the head. */
 constexpr int TO_N = 16, TO_ROWS = TO_N + 7; /* nodes, then the conv state's rows */
+constexpr int TO_WAVES = 8;                  /* more would leave a wave 128 registers, too few */
 
 struct TreeOne {
     TreePre p;
@@ -416,37 +449,57 @@ struct TreeOne {
 };
 
 template <int DK4>
-__global__ __launch_bounds__(1024) void lin_tree_one_k(TreeOne a) {
+__global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
     constexpr int DK = 4 * DK4, NS = DK4 / 4;
     extern __shared__ float4 smem4[];
     __shared__ TreeTables tt;
     __shared__ float2 co[TO_N][TO_N + 1];
-    __shared__ float pk[TR_B][DK + 16], pdec[TR_B], red[4 * 2 * TO_N];
-    __shared__ int par[TO_N];
+    __shared__ alignas(16) float pk[TR_B][DK + 16];
+    __shared__ float gap[TO_N][TO_N + 1], pdec[TR_B], red[4 * 2 * TO_N];
+    __shared__ alignas(16) int win[TO_N][8]; /* the LDS rows of a node's window, the newest first */
     const TreePre &p = a.p;
     const TreeRule &q = a.r;
     const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, gq = lane >> 4;
-    const int n = p.n, heads = q.heads, dv = q.dv, K = p.K, S = K - 1, kh = h / q.rep, T = blockDim.x;
+    const int n = p.n, heads = q.heads, dv = q.dv, K = p.K, S = K - 1, kh = h / q.rep, T = blockDim.x, waves = T >> 6;
     const int CH = 2 * DK + dv, RS = CH + 4, j0 = 16 * w;
     const size_t logw = (size_t)DK + dv + 1;
     float *xs = (float *)smem4; /* [TO_ROWS][RS]: q | k | v of a row */
     const bool owner = j0 < dv; /* the wave has value columns */
 
-    /* requests: the channel's raw rows, conv rows and taps, the wave's state columns */
+    /* requests: the channel's raw rows, conv rows and taps, the wave's state columns, the pending rows */
     const bool chan = tid < CH;
     const int ch = !chan ? 0 : tid < DK ? kh * DK + tid : tid < 2 * DK ? p.kd + kh * DK + tid - DK : 2 * p.kd + h * dv + tid - 2 * DK;
     float x[TO_N], st[7], wc[8];
 #pragma unroll
     for (int t = 0; t < TO_N; t++) x[t] = p.raw[(size_t)(t < n ? t : n - 1) * p.raw_stride + ch];
 #pragma unroll
-    for (int r = 0; r < 7; r++) st[r] = r < S ? p.state[(size_t)r * p.C + ch] : 0.0f;
+    for (int r = 0; r < 7; r++) st[r] = S ? p.state[(size_t)(r < S ? r : S - 1) * p.C + ch] : 0.0f;
 #pragma unroll
-    for (int r = 0; r < 8; r++) wc[r] = r < K ? p.conv_w[(size_t)ch * K + r] : 0.0f;
-    if (tid < n) par[tid] = tree_parent(p.parent, tid);
+    for (int r = 0; r < 8; r++) wc[r] = p.conv_w[(size_t)ch * K + (r < K ? r : K - 1)];
+    Replay<DK4, 192> rp;
+    rp.ask(q.pend, 0, q.keep, heads, h, logw, owner ? j0 + c : 0);
     float4 s[NS];
     float *Sp = q.S + ((size_t)h * dv + (owner ? j0 : 0)) * DK + (4 * c + gq) * 4;
 #pragma unroll
     for (int k = 0; k < NS; k++) s[k] = *(const float4 *)(Sp + k * 256);
+    if (w == waves - 1) { /* the last wave, which has no channels: the tree, the gates */
+        if (lane < n) {
+            int at = lane, row = S;
+            for (int r = 0; r < K; r++) {
+                const bool node = at >= 0;
+                row -= !node;
+                win[lane][r] = node ? at : TO_N + row;
+                at = node ? tree_parent(p.parent, at) : at;
+            }
+        }
+        float bt = 0.0f, d = 1.0f;
+        if (lane < n) {
+            bt = tree_beta(p.b_in[(size_t)lane * p.g_stride + h]);
+            d = tree_decay(p, p.a_in[(size_t)lane * p.g_stride + h], h);
+            p.beta[lane * heads + h] = bt, p.decay[lane * heads + h] = d;
+        }
+        tree_tables(tt, p.parent, n, d, bt);
+    }
     if (chan) {
 #pragma unroll
         for (int t = 0; t < TO_N; t++) xs[t * RS + tid] = x[t];
@@ -459,49 +512,51 @@ __global__ __launch_bounds__(1024) void lin_tree_one_k(TreeOne a) {
                 if (t < n) p.xin[(size_t)t * p.C + ch] = x[t];
         }
     }
-    if (w == (T >> 6) - 1) { /* the last wave, which has no channels: gates and the tree */
-        float bt = 0.0f, d = 1.0f;
-        if (lane < n) {
-            bt = tree_beta(p.b_in[(size_t)lane * p.g_stride + h]);
-            d = tree_decay(p, p.a_in[(size_t)lane * p.g_stride + h], h);
-            p.beta[lane * heads + h] = bt, p.decay[lane * heads + h] = d;
-        }
-        tree_tables(tt, p.parent, n, d, bt);
-    }
     __syncthreads();
-    if (chan) { /* conv + SiLU, 4 nodes at a time from the last down */
-        for (int t1 = n - 1; t1 >= 0; t1 -= 4) {
-            float acc[4];
+    if (w == waves - 1) { /* while the others convolve */
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                int at = t1 - u < 0 ? 0 : t1 - u, row = S;
-                float win[8];
+        for (int j = 0; j < 4; j++) {
+            const int t = 4 * gq + j;
+            if (t < n && (tt.sets[t] >> c & 1)) gap[t][c] = tree_gap(tt, t, c);
+        }
+    }
+    if (chan) { /* conv + SiLU: the channel's column is this thread's own, all windows read before any output */
+        if (K == 4) {
+            float b[TO_N][3];
 #pragma unroll
-                for (int r = 0; r < 8; r++) { /* the r-th newest */
-                    if (r >= K) break;
-                    const bool node = at >= 0;
-                    row -= !node;
-                    win[r] = xs[(node ? at : TO_N + row) * RS + tid];
-                    at = node ? par[at] : at;
-                }
-                float y = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) { /* taps in order, the oldest first */
-                    if (j >= K) break;
-                    float v = win[0];
-#pragma unroll
-                    for (int r = 1; r < 8; r++) v = r == K - 1 - j ? win[r] : v;
-                    y = j ? y + wc[j] * v : wc[0] * v;
-                }
-                acc[u] = nmx_silu(y);
+            for (int t = 0; t < TO_N; t++) {
+                const int4 at = *(const int4 *)win[t < n ? t : 0];
+                b[t][0] = xs[at.y * RS + tid], b[t][1] = xs[at.z * RS + tid], b[t][2] = xs[at.w * RS + tid];
             }
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                if (t1 - u >= 0) xs[(t1 - u) * RS + tid] = acc[u];
+            for (int t = 0; t < TO_N; t++) {
+                if (t >= n) continue;
+                float y = wc[0] * b[t][2]; /* taps in order, the oldest first */
+                y = y + wc[1] * b[t][1];
+                y = y + wc[2] * b[t][0];
+                y = y + wc[3] * x[t];
+                xs[t * RS + tid] = nmx_silu(y);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < TO_N; t++) {
+                if (t >= n) continue;
+                float y = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (j >= K) continue;
+                    const float v = xs[win[t][K - 1 - j] * RS + tid];
+                    y = j ? y + wc[j] * v : wc[0] * v;
+                }
+                x[t] = nmx_silu(y);
+            }
+#pragma unroll
+            for (int t = 0; t < TO_N; t++)
+                if (t < n) xs[t * RS + tid] = x[t];
         }
     }
     const int keep = keep_of(q.keep, q.keep_dev);
-    replay<DK4>(s, q.pend, keep, heads, h, logw, dv, j0, pk, pdec, owner);
+    rp.run(s, q.pend, q.keep, keep, heads, h, logw, owner ? j0 + c : 0, pk, pdec);
     if (keep > 0 && owner) {
 #pragma unroll
         for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
@@ -517,15 +572,35 @@ __global__ __launch_bounds__(1024) void lin_tree_one_k(TreeOne a) {
         xs[t * RS + e] = (xs[t * RS + e] * r) * (e < DK ? p.qscale : 1.0f);
     }
     __syncthreads();
-    for (int i = tid; i < n * CH; i += T) { /* what is kept of the pass: conv outputs, the log rows' keys */
-        const int t = i / CH, e = i % CH;
-        const float v = xs[t * RS + e];
-        p.out[(size_t)t * p.C + (e < DK ? kh * DK + e : e < 2 * DK ? p.kd + kh * DK + e - DK : 2 * p.kd + h * dv + e - 2 * DK)] = v;
-        if (e >= DK && e < 2 * DK) q.log[((size_t)t * heads + h) * logw + e - DK] = v;
+    if (chan) { /* what is kept of the pass: conv outputs, the log rows' keys */
+#pragma unroll 4
+        for (int t = 0; t < n; t++) {
+            const float v = xs[t * RS + tid];
+            p.out[(size_t)t * p.C + ch] = v;
+            if (tid >= DK && tid < 2 * DK) q.log[((size_t)t * heads + h) * logw + tid - DK] = v;
+        }
     }
     if (tid < n) q.log[((size_t)tid * heads + h) * logw + DK + dv] = tt.dec[tid];
-    /* products: rows past the end hold raw values, and are not used */
+    /* products: rows past the end hold raw values, and are not used. D k.k and D q.k by two waves (the
+     * last ones, which have no channels' rows to store), their sums in two chains */
     const float *qr = xs + c * RS + gq * DK4, *kr = qr + DK;
+    for (int job = waves - 1 - w; job < 2; job += waves) {
+        const float *l = job ? qr : kr;
+        f32x4 u = {0.0f, 0.0f, 0.0f, 0.0f}, v = u;
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+            const float4 b = *(const float4 *)(kr + 4 * k), e = *(const float4 *)(l + 4 * k);
+            u = mfma4(e.x, b.x, u), v = mfma4(e.y, b.y, v), u = mfma4(e.z, b.z, u), v = mfma4(e.w, b.w, v);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int t = 4 * gq + j;
+            if (t >= n || !(tt.sets[t] >> c & 1)) continue;
+            const float d = (u[j] + v[j]) * gap[t][c];
+            if (job) co[t][c].y = d;
+            else co[t][c].x = d;
+        }
+    }
     f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
     if (owner) {
 #pragma unroll
@@ -537,17 +612,6 @@ __global__ __launch_bounds__(1024) void lin_tree_one_k(TreeOne a) {
             sk = mfma4(x4.w, s[k].w, sk), sq = mfma4(y4.w, s[k].w, sq);
         }
     }
-    for (int job = w; job < 2; job += T >> 6) { /* D k.k and D q.k */
-        const f32x4 x4 = row_products<NS>(job ? qr : kr, kr);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 4 * gq + j;
-            if (t >= n || !(tt.sets[t] >> c & 1)) continue;
-            const float d = x4[j] * tree_gap(tt, t, c);
-            if (job) co[t][c].y = d;
-            else co[t][c].x = d;
-        }
-    }
     float v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = owner ? xs[(4 * gq + j) * RS + 2 * DK + j0 + c] : 0.0f;
@@ -555,35 +619,42 @@ __global__ __launch_bounds__(1024) void lin_tree_one_k(TreeOne a) {
     float *del = xs + 2 * DK + j0 + c; /* this lane's column: deltas where v was, then o */
     if (owner) {
         unsigned long long left[4];
-        float r[4], o[4];
-        int depth[4];
+        float r[4], o[4], bt[4];
+        float2 cf[4];
+        int depth[4], an[4];
         const int levels = tt.levels;
+        auto next = [&](int j) {
+            an[j] = left[j] ? __ffsll((long long)left[j]) - 1 : 0; /* ancestors in order of depth */
+            left[j] &= left[j] - 1;
+            cf[j] = co[4 * gq + j][an[j]];
+        };
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int t = 4 * gq + j;
             left[j] = t < n ? tt.sets[t] : 0;
             depth[j] = t < n ? __popcll(left[j]) - 1 : -1;
             const float g = t < n ? tt.gs[t] : 0.0f;
+            bt[j] = tt.bet[t];
             r[j] = v[j] - g * sk[j], o[j] = g * sq[j];
+            next(j);
         }
         for (int d = 0; d < levels; d++) { /* the wave's columns are its own: no barrier */
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (depth[j] == d) {
-                    r[j] = r[j] * tt.bet[4 * gq + j];
-                    del[(4 * gq + j) * RS] = r[j];
-                }
+            for (int j = 0; j < 4; j++) {
+                const bool now = depth[j] == d;
+                r[j] = now ? r[j] * bt[j] : r[j];
+                if (now) del[(4 * gq + j) * RS] = r[j];
+            }
             nmx_lds_wave_sync();
+            float xd[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (depth[j] >= d) {
-                    const int an = __ffsll((long long)left[j]) - 1; /* ancestors in order of depth */
-                    left[j] &= left[j] - 1;
-                    const float xd = del[an * RS];
-                    const float2 cf = co[4 * gq + j][an];
-                    o[j] = o[j] + cf.y * xd;
-                    if (depth[j] > d) r[j] = r[j] - cf.x * xd;
-                }
+            for (int j = 0; j < 4; j++) xd[j] = del[an[j] * RS];
+#pragma unroll
+            for (int j = 0; j < 4; j++) { /* chosen, not multiplied away: a node past its depth reads anything */
+                o[j] = depth[j] >= d ? o[j] + cf[j].y * xd[j] : o[j];
+                r[j] = depth[j] > d ? r[j] - cf[j].x * xd[j] : r[j];
+                next(j);
+            }
         }
         nmx_lds_wave_sync();
 #pragma unroll
@@ -595,17 +666,27 @@ __global__ __launch_bounds__(1024) void lin_tree_one_k(TreeOne a) {
             q.log[((size_t)t * heads + h) * logw + DK + j0 + c] = r[j];
         }
     }
+    const int nd = n * dv; /* whole half-waves: dv % 32 == 0 */
+    constexpr int ZB = 4; /* turns of the gated norm: n dv <= 16 dv values, T >= 4 dv threads */
+    float zb[ZB], nb[ZB];
+#pragma unroll
+    for (int u = 0; u < ZB; u++) {
+        const int i = tid + u * T < nd ? tid + u * T : tid % dv, t = i / dv, j = i % dv;
+        zb[u] = a.z[(size_t)t * a.z_stride + h * dv + j], nb[u] = a.norm_w[j];
+    }
     __syncthreads();
     /* the gated RMSNorm over the head, as lin_post_k makes it */
     for (int i = tid; i < 4 * n; i += T) red[i] = square_chain(xs + (i >> 2) * RS + 2 * DK + (i & 3), dv >> 2);
     __syncthreads();
-    const int nd = n * dv; /* whole half-waves: dv % 32 == 0 */
-    for (int i = tid; i < nd; i += T) {
+#pragma unroll
+    for (int u = 0; u < ZB; u++) {
+        const int i = tid + u * T;
+        if (i >= nd) continue;
         const int t = i / dv, j = i % dv, col = h * dv + j;
         const float *rd = red + 4 * t;
         const float ss = ((rd[0] + rd[1]) + (rd[2] + rd[3])) + 0.0f, r = 1.0f / sqrtf(ss / (float)dv + a.eps);
-        float y = (xs[t * RS + 2 * DK + j] * r) * a.norm_w[j];
-        y = y * nmx_silu(a.z[(size_t)t * a.z_stride + col]);
+        float y = (xs[t * RS + 2 * DK + j] * r) * nb[u];
+        y = y * nmx_silu(zb[u]);
         if (a.y) a.y[(size_t)t * a.y_stride + col] = y;
         if (a.aq) a8_block(y, col >> 5, t, n, a.aq, a.ad, a.afs);
     }
@@ -625,7 +706,7 @@ int launch_rule(nmx_ctx *ctx, const TreeRule &a) {
     const int n16 = (a.n + 15) / 16 * 16;
     auto bytes = [](int m) {
         const size_t co = (size_t)m * (m + 1) * 8, pk = (size_t)TR_B * (4 * DK4 + 16) * 4;
-        return (size_t)(DK4 < 64 ? 2 : 1) * m * (4 * DK4 + 4) * 4 + (co > pk ? co : pk);
+        return (size_t)(DK4 < 64 ? 4 : 2) * m * (4 * DK4 + 8) * 2 + (co > pk ? co : pk);
     };
     static std::atomic<uint64_t> set;
     if (nmx_dyn_lds(ctx, (const void *)lin_tree_rule_k<DK4>, bytes(64), set)) return -1;
@@ -681,9 +762,9 @@ int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *m, const int32_t *par
     const TreePre a{n, p.C, p.conv_k, dk, p.kd, p.raw, p.raw_stride, p.out, p.state, p.conv_w, p.xin, p.qscale, p.l2eps,
                     p.b_in, p.a_in, p.g_stride, heads, p.A_log, p.A, p.dt_bias, p.beta, p.decay, parent};
     const TreeRule t{n, heads, r.rep, dv, p.kd, p.C, p.out, p.beta, p.decay, r.S, r.o, r.o_stride, r.log, r.pend, r.keep,
-                     r.keep_dev, parent};
+                     r.keep_dev, parent, p.qscale};
     const int ch_waves = (2 * dk + dv + 63) / 64 + 1, waves = dv / 16 > ch_waves ? dv / 16 : ch_waves;
-    if (n <= TO_N && dk <= 128 && waves <= 16) {
+    if (n <= TO_N && dk <= 128 && waves <= TO_WAVES) {
         const TreeOne o{a, t, m->z, m->norm_w, m->z_stride, m->y_stride, m->eps, m->y, m->a8.q, m->a8.d, m->a8.fs};
         const size_t lds = (size_t)TO_ROWS * (2 * dk + dv + 4) * 4;
         return dk == 32 ? launch_one<8>(ctx, o, 64 * waves, lds) : dk == 64 ? launch_one<16>(ctx, o, 64 * waves, lds) :

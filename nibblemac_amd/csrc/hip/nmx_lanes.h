@@ -25,6 +25,14 @@ __device__ __forceinline__ void nmx_lds_wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
+/* A workgroup's barrier that orders its LDS accesses alone: __syncthreads also waits until every global
+ * store and load in flight has arrived, about a microsecond after a store. */
+__device__ __forceinline__ void nmx_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <int CTRL>
 __device__ __forceinline__ int nmx_dpp(int v) {
     return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);

@@ -43,7 +43,7 @@ struct TreePre {
     const int32_t *parent;
 };
 
-constexpr int TP_N = 8; /* nodes of a workgroup */
+constexpr int TP_N = 4; /* nodes of a workgroup */
 
 /* Partial sum l of 4 interleaved ones over the dk squares of a row (v: element l of it, dk / 4 elements 4
  * apart), in element order: the adds of lin_pre_k. */
@@ -60,6 +60,12 @@ __device__ __forceinline__ float square_chain(const float *v, int m4) {
     for (; m < m4; m++) c = c + v[4 * m] * v[4 * m];
     return c;
 }
+/* (c0 + c1) + (c2 + c3) of a quad's lanes, in each of them */
+__device__ __forceinline__ float quad_sum(float c) {
+    const float o = __int_as_float(nmx_dpp<NMX_DPP_XOR1>(__float_as_int(c)));
+    const float s = c + o;
+    return s + __int_as_float(nmx_dpp<NMX_DPP_XOR2>(__float_as_int(s)));
+}
 __device__ __forceinline__ float tree_beta(const float b) { return 1.0f / (1.0f + nmx_gate_expf(-b)); }
 __device__ __forceinline__ float tree_decay(const TreePre &a, float av, int h) {
     const float A = a.A ? a.A[h] : -nmx_gate_expf(a.A_log[h]);
@@ -71,7 +77,7 @@ __device__ __forceinline__ float tree_decay(const TreePre &a, float av, int h) {
 template <int KT>
 __global__ __launch_bounds__(256) void lin_tree_pre_k(TreePre a) {
     extern __shared__ float sq[]; /* [TP_N][dk + 4] */
-    __shared__ float red[4 * TP_N];
+    __shared__ float red[TP_N];
     __shared__ int par[NMX_TREE_MAX];
     const int groups = (a.C + a.dk - 1) / a.dk, tid = threadIdx.x;
     const int t0 = blockIdx.y * TP_N, nb = a.n - t0 < TP_N ? a.n - t0 : TP_N;
@@ -91,7 +97,7 @@ __global__ __launch_bounds__(256) void lin_tree_pre_k(TreePre a) {
     float wc[KM], y[TP_N], win[TP_N][KM];
 #pragma unroll
     for (int r = 0; r < KM; r++) wc[r] = r < K ? a.conv_w[(size_t)cc * K + r] : 0.0f;
-    __syncthreads();
+    nmx_lds_sync();
     /* win[u][j]: tap j's input, the newest (the node itself) at K - 1, then its ancestors, then the state's
      * rows from the newest down; nodes past the end repeat the last one */
 #pragma unroll
@@ -130,15 +136,14 @@ __global__ __launch_bounds__(256) void lin_tree_pre_k(TreePre a) {
 #pragma unroll
         for (int u = 0; u < TP_N; u++)
             if (tid < a.dk) sq[u * rs + tid] = live ? y[u] : 0.0f;
-        __syncthreads();
-        if (tid < 4 * TP_N) red[tid] = square_chain(sq + (tid >> 2) * rs + (tid & 3), a.dk >> 2);
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < TP_N; u++) {
-            const float ss = ((red[4 * u] + red[4 * u + 1]) + (red[4 * u + 2] + red[4 * u + 3])) + 0.0f;
-            const float r = 1.0f / sqrtf(ss + a.l2eps);
-            y[u] = (y[u] * r) * scale;
+        nmx_lds_sync();
+        if (tid < 4 * TP_N) {
+            const float c = square_chain(sq + (tid >> 2) * rs + (tid & 3), a.dk >> 2);
+            red[tid >> 2] = 1.0f / sqrtf((quad_sum(c) + 0.0f) + a.l2eps);
         }
+        nmx_lds_sync();
+#pragma unroll
+        for (int u = 0; u < TP_N; u++) y[u] = (y[u] * red[u]) * scale;
     }
 #pragma unroll
     for (int u = 0; u < TP_N; u++)
@@ -161,44 +166,40 @@ struct TreeRule {
 
 constexpr int TR_B = 8; /* pending rows staged at a time */
 
-/* The tree as a wave's lanes see it, into LDS: sets of ancestors, decays over 2^k steps up, decays from
- * the state (lane t; d, bt: its decay and beta). Every lane of the wave. */
+/* The tree in LDS, for N nodes at most: of node t, in order of depth, its ancestors (itself the last) and
+ * the product of the decays after each of them up to t; the product of all of them from the state. */
+template <int N>
 struct TreeTables {
-    unsigned long long sets[NMX_TREE_MAX];
-    float dec[NMX_TREE_MAX], bet[NMX_TREE_MAX], gs[NMX_TREE_MAX], run[6][NMX_TREE_MAX];
-    int up[6][NMX_TREE_MAX];
+    unsigned long long sets[N];
+    float dec[N], bet[N], gs[N], gap[N][N + 1];
+    uint8_t depth[N];
+    alignas(16) uint8_t anc[N][N]; /* past a node's depth: itself */
     int levels;
 };
-__device__ __forceinline__ void tree_tables(TreeTables &s, const int32_t *parent, int n, float d, float bt) {
+/* One wave; lane t < n: its parent p, decay d and beta bt. */
+template <int N>
+__device__ __forceinline__ void tree_tables(TreeTables<N> &s, int n, unsigned long long set, int p, float d, float bt) {
     const int lane = threadIdx.x & 63;
-    int p;
-    const unsigned long long set = tree_ancestors(parent, n, &p);
-    s.sets[lane] = set, s.dec[lane] = d, s.bet[lane] = bt;
-    float r = d;
-    int q = p;
-#pragma unroll
-    for (int k = 0; k < 6; k++) {
-        s.run[k][lane] = r, s.up[k][lane] = q;
-        const int from = q < 0 ? lane : q;
-        const float ro = __shfl(r, from);
-        const int qo = __shfl(q, from);
-        if (q >= 0) r *= ro, q = qo;
-    }
-    s.gs[lane] = r; /* every node is at most 63 steps from the state */
-    int deep = lane < n ? __popcll(set) : 0;
+    const bool in = lane < n;
+    int at = in ? __popcll(set) - 1 : -1, cur = lane;
+    int deep = at;
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) deep = max(deep, __shfl_xor(deep, x));
-    if (lane == 0) s.levels = deep;
-}
-/* D(t, a), the product of the decays after ancestor a up to t */
-__device__ __forceinline__ float tree_gap(const TreeTables &s, int t, int a) {
-    const int steps = __popcll(s.sets[t]) - __popcll(s.sets[a]);
-    float d = 1.0f;
-    int at = t;
-#pragma unroll
-    for (int k = 0; k < 6; k++)
-        if (steps >> k & 1) d *= s.run[k][at], at = s.up[k][at];
-    return d;
+    if (lane < N) {
+        s.sets[lane] = set, s.dec[lane] = d, s.bet[lane] = bt, s.depth[lane] = (uint8_t)(at < 0 ? 0 : at);
+        for (int k = at < 0 ? 0 : at; k <= deep; k++) s.anc[lane][k] = (uint8_t)lane;
+    }
+    float g = 1.0f;
+    for (int k = 0; k <= deep; k++) { /* up the path, every lane at once */
+        if (at >= 0) s.gap[lane][at] = g, s.anc[lane][at] = (uint8_t)cur;
+        const float dc = __shfl(d, cur);
+        const int up = __shfl(p, cur);
+        if (at >= 0) g *= dc;
+        at--;
+        cur = up < 0 ? cur : up;
+    }
+    if (lane < N) s.gs[lane] = g;
+    if (lane == 0) s.levels = deep + 1;
 }
 
 /* Rows of k and q for the products of nodes: as two binary16 parts each, which together hold 22 bits of
@@ -245,14 +246,14 @@ struct Replay {
         for (int u0 = 0; u0 < keep; u0 += TR_B) {
             if (u0) ask(pend, u0, asked, heads, h, logw, col);
             const int nb = keep - u0 < TR_B ? keep - u0 : TR_B;
-            __syncthreads();
+            nmx_lds_sync();
 #pragma unroll
             for (int e = 0; e < NP; e++) {
                 const int x = e * (int)blockDim.x + tid, i = x % DK;
                 if (x < TR_B * DK) pk[x / DK][i + 4 * (i / DK4)] = k[e];
             }
             if (tid < TR_B) pdec[tid] = d;
-            __syncthreads();
+            nmx_lds_sync();
 #pragma unroll
             for (int u = 0; u < TR_B; u++) {
                 if (u >= nb) continue;
@@ -274,26 +275,32 @@ __device__ __forceinline__ int keep_of(int keep, const int32_t *keep_dev) {
     return d < keep ? d : keep;
 }
 
+/* A wave of its own for the tree's tables; of 256 keys the four waves of 64 nodes need the registers. */
+template <int DK4>
+constexpr int tree_wave() {
+    return DK4 < 64 ? 1 : 0;
+}
+
 /* More than 16 nodes: one workgroup per head and 16 value columns (a group of the state's layout), a wave
  * per 16 nodes. The state's columns are a matrix operand as they lie: lane (column c, quarter gq)
  * holds the float4 slots of keys gq dk/4 .. of its column, and the wave's rows of k and q are read in
  * the same order. */
 template <int DK4>
-__global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
+__global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(TreeRule a) {
     constexpr int DK = 4 * DK4, NS = DK4 / 4, HS = DK + 8; /* halves of a row in LDS: 16 bytes on, no bank twice */
     extern __shared__ float4 smem4[];
-    __shared__ TreeTables tt;
+    __shared__ TreeTables<NMX_TREE_MAX> tt;
     __shared__ float del[2][NMX_TREE_MAX][16], pdec[TR_B];
-    const int h = blockIdx.x, j0 = blockIdx.y * 16, tid = threadIdx.x, lane = tid & 63, T = tid >> 6, waves = blockDim.x >> 6;
+    const int h = blockIdx.x, j0 = blockIdx.y * 16, tid = threadIdx.x, lane = tid & 63, T = tid >> 6, waves = (int)(blockDim.x >> 6) - tree_wave<DK4>();
     const int c = lane & 15, gq = lane >> 4, n = a.n, heads = a.heads, dv = a.dv, n16 = 16 * waves;
     _Float16 *kh2 = (_Float16 *)smem4, *qh2 = kh2 + 2 * n16 * HS;   /* [2][n16][HS]: high, low parts */
     constexpr bool QL = DK4 < 64; /* 256 keys: the parts of q are made when they are used, LDS has no room */
-    float2 *co = (float2 *)(QL ? qh2 + 2 * n16 * HS : qh2);         /* [n16][n16 + 1]: D k.k, D q.k */
+    float2 *co = (float2 *)(QL ? qh2 + 2 * n16 * HS : qh2);         /* [n16][n16 + 1]: D k.k, D q.k of a node's ancestors by depth */
     float(*pk)[DK + 16] = (float(*)[DK + 16])co;                    /* pending keys, before the products */
     const size_t logw = (size_t)DK + dv + 1;
     const int kh = h / a.rep;
 
-    Replay<DK4, 128> rp;
+    Replay<DK4, DK4 < 64 ? 128 : 64> rp;
     rp.ask(a.pend, 0, a.keep, heads, h, logw, j0 + c);
     float4 s[NS], kf[NS], qf[NS];
     float *Sp = a.S + ((size_t)h * dv + j0) * DK + (4 * c + gq) * 4;
@@ -310,10 +317,17 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
         const int t = 16 * T + 4 * gq + j;
         v[j] = a.qkv[(size_t)(t < n ? t : n - 1) * a.C + 2 * a.kd + h * dv + j0 + c];
     }
-    if (T == waves - 1) tree_tables(tt, a.parent, n, lane < n ? a.decay[lane * heads + h] : 1.0f, lane < n ? a.beta[lane * heads + h] : 0.0f);
+    const bool nodes = T < waves; /* the last wave has the tree instead */
+    if (T == (int)(blockDim.x >> 6) - 1) {
+        const float dc = lane < n ? a.decay[lane * heads + h] : 1.0f, bt = lane < n ? a.beta[lane * heads + h] : 0.0f;
+        int p;
+        const unsigned long long set = tree_ancestors(a.parent, n, &p);
+        tree_tables(tt, n, set, p, dc, bt);
+    }
     const float q_up = a.qscale != 0.0f ? TR_UP / a.qscale : 0.0f, q_down = a.qscale / (TR_UP * TR_UP);
 #pragma unroll
     for (int k = 0; k < NS; k++) {
+        if (!nodes) continue;
         const int at = tn * HS + gq * DK4 + 4 * k;
         split4(kf[k], TR_UP, kh2 + at, kh2 + n16 * HS + at);
         if (QL) split4(qf[k], q_up, qh2 + at, qh2 + n16 * HS + at);
@@ -333,9 +347,9 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
         sk = mfma4(kf[k].z, s[k].z, sk), sq = mfma4(qf[k].z, s[k].z, sq);
         sk = mfma4(kf[k].w, s[k].w, sk), sq = mfma4(qf[k].w, s[k].w, sq);
     }
-    __syncthreads(); /* the rows, the tables; the pending keys have been read */
+    nmx_lds_sync(); /* the rows, the tables; the pending keys have been read */
     /* D(t, a) (k_t . k_a) and D(t, a) (q_t . k_a): the tiles (t, a) on and below the diagonal, in turn */
-    for (int job = T, X = 0; X < waves; job -= X + 1, X++) {
+    for (int job = nodes ? T : waves * waves, X = 0; X < waves; job -= X + 1, X++) {
         for (; job <= X; job += waves) {
             const int U = job, an = 16 * U + c;
             const _Float16 *ar = kh2 + an * HS + 8 * gq, *tr = kh2 + (16 * X + c) * HS + 8 * gq, *ur = qh2 + (16 * X + c) * HS + 8 * gq;
@@ -361,38 +375,34 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
                 x = mfma16(tl, ah, x), y = mfma16(ul, ah, y);
                 x = mfma16(th, al, x), y = mfma16(uh, al, y);
             }
+            const int dp = tt.depth[an];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int t = 16 * X + 4 * gq + j;
                 if (t >= n || !(tt.sets[t] >> an & 1)) continue;
-                const float d = tree_gap(tt, t, an);
-                co[t * (n16 + 1) + an] = make_float2(x[j] * (d * (1.0f / (TR_UP * TR_UP))), y[j] * (d * q_down));
+                const float d = tt.gap[t][dp];
+                co[t * (n16 + 1) + dp] = make_float2(x[j] * (d * (1.0f / (TR_UP * TR_UP))), y[j] * (d * q_down));
             }
         }
     }
-    __syncthreads();
-    /* the deltas, level by level; a level's ancestor and coefficients are at hand before its deltas are */
-    unsigned long long left[4];
+    nmx_lds_sync();
+    /* the deltas, level by level; four levels' ancestors and the next level's coefficients are at hand */
     float r[4], o[4], bt[4];
     float2 cf[4];
-    int depth[4], an[4];
+    int depth[4], tj[4];
+    uint32_t an[4];
     const int levels = tt.levels;
-    auto next = [&](int j) {
-        an[j] = left[j] ? __ffsll((long long)left[j]) - 1 : 0; /* ancestors in order of depth */
-        left[j] &= left[j] - 1;
-        const int t = 16 * T + 4 * gq + j;
-        cf[j] = co[t * (n16 + 1) + an[j]];
-    };
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int t = 16 * T + 4 * gq + j;
-        const bool in = t < n;
-        left[j] = in ? tt.sets[t] : 0;
-        depth[j] = in ? __popcll(left[j]) - 1 : -1;
-        const float g = in ? tt.gs[t] : 0.0f;
-        bt[j] = in ? tt.bet[t] : 0.0f;
+        const bool in = nodes && t < n;
+        tj[j] = in ? t : n - 1;
+        depth[j] = in ? tt.depth[t] : -1;
+        const float g = tt.gs[tj[j]];
+        bt[j] = tt.bet[tj[j]];
         r[j] = v[j] - g * sk[j], o[j] = g * sq[j];
-        next(j);
+        an[j] = *(const uint32_t *)tt.anc[tj[j]];
+        cf[j] = co[tj[j] * (n16 + 1)];
     }
     for (int d = 0; d < levels; d++) {
         float(*dl)[16] = del[d & 1]; /* read in this level while the next one is written */
@@ -400,23 +410,29 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
         for (int j = 0; j < 4; j++) {
             const bool now = depth[j] == d;
             r[j] = now ? r[j] * bt[j] : r[j];
-            if (now) dl[16 * T + 4 * gq + j][c] = r[j];
+            if (now) dl[tj[j]][c] = r[j];
         }
-        __syncthreads();
+        nmx_lds_sync();
         float x[4];
+        float2 cn[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = dl[an[j]][c];
+        for (int j = 0; j < 4; j++) x[j] = dl[an[j] & 255][c];
+#pragma unroll
+        for (int j = 0; j < 4; j++) cn[j] = co[tj[j] * (n16 + 1) + d + 1];
 #pragma unroll
         for (int j = 0; j < 4; j++) { /* chosen, not multiplied away: a node past its depth reads anything */
             o[j] = depth[j] >= d ? o[j] + cf[j].y * x[j] : o[j];
             r[j] = depth[j] > d ? r[j] - cf[j].x * x[j] : r[j];
-            next(j);
+            an[j] >>= 8, cf[j] = cn[j];
         }
+        if ((d & 3) == 3)
+#pragma unroll
+            for (int j = 0; j < 4; j++) an[j] = *(const uint32_t *)(tt.anc[tj[j]] + ((d + 1) & 63));
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int t = 16 * T + 4 * gq + j;
-        if (t < n) {
+        if (nodes && t < n) {
             a.o[(size_t)t * a.o_stride + h * dv + j0 + c] = o[j];
             a.log[((size_t)t * heads + h) * logw + DK + j0 + c] = r[j];
         }
@@ -435,7 +451,7 @@ __global__ __launch_bounds__(256) void lin_tree_rule_k(TreeRule a) {
  * their place (the last node first: nodes read their ancestors' raw values, which lie before them);
  * o replaces v there in turn, for the gated norm over the head. */
 constexpr int TO_N = 16, TO_ROWS = TO_N + 7; /* nodes, then the conv state's rows */
-constexpr int TO_WAVES = 8;                  /* more would leave a wave 128 registers, too few */
+constexpr int TO_WAVES = 10;                 /* 8 of value columns, two more for the tree and the products of nodes */
 
 struct TreeOne {
     TreePre p;
@@ -452,10 +468,10 @@ template <int DK4>
 __global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
     constexpr int DK = 4 * DK4, NS = DK4 / 4;
     extern __shared__ float4 smem4[];
-    __shared__ TreeTables tt;
-    __shared__ float2 co[TO_N][TO_N + 1];
+    __shared__ TreeTables<TO_N> tt;
+    __shared__ float2 co[TO_N][TO_N + 1]; /* D k.k, D q.k of a node's ancestors by depth */
     __shared__ alignas(16) float pk[TR_B][DK + 16];
-    __shared__ float gap[TO_N][TO_N + 1], pdec[TR_B], red[4 * 2 * TO_N];
+    __shared__ float pdec[TR_B], rr[2 * TO_N];
     __shared__ alignas(16) int win[TO_N][8]; /* the LDS rows of a node's window, the newest first */
     const TreePre &p = a.p;
     const TreeRule &q = a.r;
@@ -476,29 +492,27 @@ __global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
     for (int r = 0; r < 7; r++) st[r] = S ? p.state[(size_t)(r < S ? r : S - 1) * p.C + ch] : 0.0f;
 #pragma unroll
     for (int r = 0; r < 8; r++) wc[r] = p.conv_w[(size_t)ch * K + (r < K ? r : K - 1)];
-    Replay<DK4, 192> rp;
+    Replay<DK4, 256> rp;
     rp.ask(q.pend, 0, q.keep, heads, h, logw, owner ? j0 + c : 0);
     float4 s[NS];
     float *Sp = q.S + ((size_t)h * dv + (owner ? j0 : 0)) * DK + (4 * c + gq) * 4;
 #pragma unroll
     for (int k = 0; k < NS; k++) s[k] = *(const float4 *)(Sp + k * 256);
-    if (w == waves - 1) { /* the last wave, which has no channels: the tree, the gates */
-        if (lane < n) {
-            int at = lane, row = S;
-            for (int r = 0; r < K; r++) {
-                const bool node = at >= 0;
-                row -= !node;
-                win[lane][r] = node ? at : TO_N + row;
-                at = node ? tree_parent(p.parent, at) : at;
-            }
+    /* the last two waves, which have no channels: the windows, the gates; behind the barrier the tree */
+    if (w == waves - 1) {
+        const int up = lane < n ? tree_parent(p.parent, lane) : -1;
+        int at = lane, row = S;
+        for (int r = 0; r < K; r++) {
+            const bool node = at >= 0;
+            row -= !node;
+            if (lane < n) win[lane][r] = node ? at : TO_N + row;
+            const int next = __shfl(up, node ? at : 0);
+            at = node ? next : at;
         }
-        float bt = 0.0f, d = 1.0f;
-        if (lane < n) {
-            bt = tree_beta(p.b_in[(size_t)lane * p.g_stride + h]);
-            d = tree_decay(p, p.a_in[(size_t)lane * p.g_stride + h], h);
-            p.beta[lane * heads + h] = bt, p.decay[lane * heads + h] = d;
-        }
-        tree_tables(tt, p.parent, n, d, bt);
+    } else if (w == waves - 2 && lane < n) {
+        const float bt = tree_beta(p.b_in[(size_t)lane * p.g_stride + h]), d = tree_decay(p, p.a_in[(size_t)lane * p.g_stride + h], h);
+        p.beta[lane * heads + h] = bt, p.decay[lane * heads + h] = d;
+        tt.bet[lane] = bt, tt.dec[lane] = d;
     }
     if (chan) {
 #pragma unroll
@@ -512,13 +526,11 @@ __global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
                 if (t < n) p.xin[(size_t)t * p.C + ch] = x[t];
         }
     }
-    __syncthreads();
+    nmx_lds_sync();
     if (w == waves - 1) { /* while the others convolve */
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 4 * gq + j;
-            if (t < n && (tt.sets[t] >> c & 1)) gap[t][c] = tree_gap(tt, t, c);
-        }
+        int up;
+        const unsigned long long set = tree_ancestors(p.parent, n, &up);
+        tree_tables(tt, n, set, up, lane < n ? tt.dec[lane] : 1.0f, lane < n ? tt.bet[lane] : 0.0f);
     }
     if (chan) { /* conv + SiLU: the channel's column is this thread's own, all windows read before any output */
         if (K == 4) {
@@ -561,17 +573,19 @@ __global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
 #pragma unroll
         for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
     }
-    __syncthreads();
-    /* L2 norms of the q and k rows: 4 chains each */
-    for (int i = tid; i < 8 * n; i += T) red[i] = square_chain(xs + (i >> 3) * RS + (i >> 2 & 1) * DK + (i & 3), DK >> 2);
-    __syncthreads();
+    nmx_lds_sync();
+    /* L2 norms of the q and k rows: 4 chains each, in a quad of lanes */
+    for (int i = tid; i < 8 * TO_N; i += T) {
+        const int t = i >> 3 < n ? i >> 3 : n - 1;
+        const float ch4 = square_chain(xs + t * RS + (i >> 2 & 1) * DK + (i & 3), DK >> 2);
+        rr[i >> 2] = 1.0f / sqrtf((quad_sum(ch4) + 0.0f) + p.l2eps);
+    }
+    nmx_lds_sync();
     for (int i = tid; i < n * 2 * DK; i += T) {
         const int t = i / (2 * DK), e = i % (2 * DK);
-        const float *rd = red + 8 * t + (e < DK ? 0 : 4);
-        const float ss = ((rd[0] + rd[1]) + (rd[2] + rd[3])) + 0.0f, r = 1.0f / sqrtf(ss + p.l2eps);
-        xs[t * RS + e] = (xs[t * RS + e] * r) * (e < DK ? p.qscale : 1.0f);
+        xs[t * RS + e] = (xs[t * RS + e] * rr[2 * t + (e >= DK)]) * (e < DK ? p.qscale : 1.0f);
     }
-    __syncthreads();
+    nmx_lds_sync();
     if (chan) { /* what is kept of the pass: conv outputs, the log rows' keys */
 #pragma unroll 4
         for (int t = 0; t < n; t++) {
@@ -592,13 +606,14 @@ __global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
             const float4 b = *(const float4 *)(kr + 4 * k), e = *(const float4 *)(l + 4 * k);
             u = mfma4(e.x, b.x, u), v = mfma4(e.y, b.y, v), u = mfma4(e.z, b.z, u), v = mfma4(e.w, b.w, v);
         }
+        const int dp = c < n ? tt.depth[c] : 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int t = 4 * gq + j;
             if (t >= n || !(tt.sets[t] >> c & 1)) continue;
-            const float d = (u[j] + v[j]) * gap[t][c];
-            if (job) co[t][c].y = d;
-            else co[t][c].x = d;
+            const float d = (u[j] + v[j]) * tt.gap[t][dp];
+            if (job) co[t][dp].y = d;
+            else co[t][dp].x = d;
         }
     }
     f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
@@ -615,45 +630,46 @@ __global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
     float v[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) v[j] = owner ? xs[(4 * gq + j) * RS + 2 * DK + j0 + c] : 0.0f;
-    __syncthreads();
+    nmx_lds_sync();
     float *del = xs + 2 * DK + j0 + c; /* this lane's column: deltas where v was, then o */
     if (owner) {
-        unsigned long long left[4];
         float r[4], o[4], bt[4];
         float2 cf[4];
-        int depth[4], an[4];
+        int depth[4], tj[4];
+        uint4 anc[4];
         const int levels = tt.levels;
-        auto next = [&](int j) {
-            an[j] = left[j] ? __ffsll((long long)left[j]) - 1 : 0; /* ancestors in order of depth */
-            left[j] &= left[j] - 1;
-            cf[j] = co[4 * gq + j][an[j]];
-        };
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int t = 4 * gq + j;
-            left[j] = t < n ? tt.sets[t] : 0;
-            depth[j] = t < n ? __popcll(left[j]) - 1 : -1;
-            const float g = t < n ? tt.gs[t] : 0.0f;
-            bt[j] = tt.bet[t];
+            tj[j] = t < n ? t : n - 1;
+            depth[j] = t < n ? tt.depth[t] : -1;
+            const float g = tt.gs[tj[j]];
+            bt[j] = tt.bet[tj[j]];
             r[j] = v[j] - g * sk[j], o[j] = g * sq[j];
-            next(j);
+            anc[j] = *(const uint4 *)tt.anc[tj[j]];
+            cf[j] = co[tj[j]][0];
         }
         for (int d = 0; d < levels; d++) { /* the wave's columns are its own: no barrier */
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const bool now = depth[j] == d;
                 r[j] = now ? r[j] * bt[j] : r[j];
-                if (now) del[(4 * gq + j) * RS] = r[j];
+                if (now) del[tj[j] * RS] = r[j];
             }
             nmx_lds_wave_sync();
             float xd[4];
+            float2 cn[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) xd[j] = del[an[j] * RS];
+            for (int j = 0; j < 4; j++) xd[j] = del[(anc[j].x & 255) * RS];
+#pragma unroll
+            for (int j = 0; j < 4; j++) cn[j] = co[tj[j]][d + 1];
 #pragma unroll
             for (int j = 0; j < 4; j++) { /* chosen, not multiplied away: a node past its depth reads anything */
                 o[j] = depth[j] >= d ? o[j] + cf[j].y * xd[j] : o[j];
                 r[j] = depth[j] > d ? r[j] - cf[j].x * xd[j] : r[j];
-                next(j);
+                cf[j] = cn[j];
+                anc[j].x >>= 8;
+                if ((d & 3) == 3) anc[j].x = anc[j].y, anc[j].y = anc[j].z, anc[j].z = anc[j].w;
             }
         }
         nmx_lds_wave_sync();
@@ -674,18 +690,19 @@ __global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
         const int i = tid + u * T < nd ? tid + u * T : tid % dv, t = i / dv, j = i % dv;
         zb[u] = a.z[(size_t)t * a.z_stride + h * dv + j], nb[u] = a.norm_w[j];
     }
-    __syncthreads();
+    nmx_lds_sync();
     /* the gated RMSNorm over the head, as lin_post_k makes it */
-    for (int i = tid; i < 4 * n; i += T) red[i] = square_chain(xs + (i >> 2) * RS + 2 * DK + (i & 3), dv >> 2);
-    __syncthreads();
+    for (int i = tid; i < 4 * TO_N; i += T) {
+        const float ch4 = square_chain(xs + (i >> 2 < n ? i >> 2 : n - 1) * RS + 2 * DK + (i & 3), dv >> 2);
+        rr[i >> 2] = 1.0f / sqrtf((quad_sum(ch4) + 0.0f) / (float)dv + a.eps);
+    }
+    nmx_lds_sync();
 #pragma unroll
     for (int u = 0; u < ZB; u++) {
         const int i = tid + u * T;
         if (i >= nd) continue;
         const int t = i / dv, j = i % dv, col = h * dv + j;
-        const float *rd = red + 4 * t;
-        const float ss = ((rd[0] + rd[1]) + (rd[2] + rd[3])) + 0.0f, r = 1.0f / sqrtf(ss / (float)dv + a.eps);
-        float y = (xs[t * RS + 2 * DK + j] * r) * nb[u];
+        float y = (xs[t * RS + 2 * DK + j] * rr[t]) * nb[u];
         y = y * nmx_silu(zb[u]);
         if (a.y) a.y[(size_t)t * a.y_stride + col] = y;
         if (a.aq) a8_block(y, col >> 5, t, n, a.aq, a.ad, a.afs);
@@ -710,7 +727,8 @@ int launch_rule(nmx_ctx *ctx, const TreeRule &a) {
     };
     static std::atomic<uint64_t> set;
     if (nmx_dyn_lds(ctx, (const void *)lin_tree_rule_k<DK4>, bytes(64), set)) return -1;
-    lin_tree_rule_k<DK4><<<dim3((unsigned)a.heads, (unsigned)(a.dv / 16)), (unsigned)(4 * n16), bytes(n16), ctx->stream>>>(a);
+    lin_tree_rule_k<DK4><<<dim3((unsigned)a.heads, (unsigned)(a.dv / 16)), (unsigned)(4 * n16 + 64 * tree_wave<DK4>()),
+                           bytes(n16), ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "lin_tree_rule");
     return 0;
 }
@@ -763,8 +781,8 @@ int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *m, const int32_t *par
                     p.b_in, p.a_in, p.g_stride, heads, p.A_log, p.A, p.dt_bias, p.beta, p.decay, parent};
     const TreeRule t{n, heads, r.rep, dv, p.kd, p.C, p.out, p.beta, p.decay, r.S, r.o, r.o_stride, r.log, r.pend, r.keep,
                      r.keep_dev, parent, p.qscale};
-    const int ch_waves = (2 * dk + dv + 63) / 64 + 1, waves = dv / 16 > ch_waves ? dv / 16 : ch_waves;
-    if (n <= TO_N && dk <= 128 && waves <= TO_WAVES) {
+    const int ch_waves = (2 * dk + dv + 63) / 64, waves = (dv / 16 > ch_waves ? dv / 16 : ch_waves) + 2;
+    if (n <= TO_N && dk <= 128 && waves <= TO_WAVES) { /* 10 waves of at most 168 registers fit a CU at once */
         const TreeOne o{a, t, m->z, m->norm_w, m->z_stride, m->y_stride, m->eps, m->y, m->a8.q, m->a8.d, m->a8.fs};
         const size_t lds = (size_t)TO_ROWS * (2 * dk + dv + 4) * 4;
         return dk == 32 ? launch_one<8>(ctx, o, 64 * waves, lds) : dk == 64 ? launch_one<16>(ctx, o, 64 * waves, lds) :

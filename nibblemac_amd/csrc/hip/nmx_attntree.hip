@@ -44,6 +44,7 @@ struct TreeAttn {
     float4 *stat;  /* [splits][n nh]: maximum of the scores, the values' exponent (columns below 256),
                     * sum, the values' exponent (columns from 256) */
     int splits, unit; /* a part is a whole number of units of positions */
+    int jcols;        /* columns of a join's workgroup: hd over a divisor of hd / 64 */
     float *o;
     int8_t *aq;
     float *ad, *afs;
@@ -508,38 +509,42 @@ __global__ __launch_bounds__(256, HDP <= 128 || (HDP == 256 && KVT == KV_F16) ? 
     const int d0 = blockIdx.y * OD, hd = a.hd, rep = a.nh / a.nkv, row = mt * 16 + c;
     const int hrow = row < a.n * rep ? (row / rep) * a.nh + g * rep + row % rep : -1; /* (node, head) */
     const size_t R0 = (size_t)g * a.max_ctx;
+    const int len = ctx_len(a), per = part_len(a, len);
+    if (per == 0 || s * per >= len) return;
+    /* a quarter of the part for each wave */
+    const int w0 = s * per + wave * (per >> 2);
+    const int p1 = w0 + (per >> 2) < len ? w0 + (per >> 2) : len;
+    /* rows and columns past the end repeat ones inside (finite, and their weight is 0) */
+    auto row_at = [&](int p) { return R0 + (p < p1 ? p : p1 - 1); };
+    Raw8<KVT> rv[VU / VB];
+    float vs[VU / VB];
+    auto ask_v = [&](int pt, int b) {
+#pragma unroll
+        for (int u = 0; u < VU / VB; u++) {
+            const int p = (b * (VU / VB) + u) * VR + lane / VC, ch = lane % VC;
+            if constexpr (KVT == KV_F16) { /* chunk ch of the LDS row is the row's chunk ch ^ ... */
+                const int col = d0 + ((ch ^ ((p & 3) << 1)) << 3);
+                const unsigned short *src = (const unsigned short *)a.vc + row_at(pt + p) * hd + (col < hd ? col : 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)(uintptr_t)src,
+                                                 (__attribute__((address_space(3))) uint32_t *)(uintptr_t)(tv + u * VR * OD), 16, 0, 0);
+            } else {
+                const int col = d0 + ch * 8;
+                rv[u] = load8<KVT>(a.vc, row_at(pt + p), hd, col < hd ? col : 0);
+                vs[u] = scale_of<KVT>(a, a.vc, row_at(pt + p));
+            }
+        }
+    };
+    if (KVT == KV_F16 && w0 < p1) ask_v(w0, 0); /* on its way while the query rows are split */
     half8 qh[KS], ql[KS];
     const float qfac = load_q<KS>(a.q + (size_t)(hrow < 0 ? 0 : hrow) * 2 * hd, hrow >= 0, hd, gq, a.scale, qh, ql);
-    const int len = ctx_len(a), per = part_len(a, len), p0 = s * per;
-    if (per == 0 || p0 >= len) return;
-    const int p1 = p0 + per < len ? p0 + per : len;
     Running<DT> r;
     const int vp = 4 * gq + (c >> 2);
     const _Float16 *vb[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) vb[i] = tv + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
-    for (int pt = p0 + wave * AT_P; pt < p1; pt += 4 * AT_P) {
-        /* rows and columns past the end repeat ones inside (finite, and their weight is 0) */
-        auto row_at = [&](int p) { return R0 + (pt + p < p1 ? pt + p : p1 - 1); };
-        Raw8<KVT> rk[KS], rv[VU / VB];
-        float vs[VU / VB];
+    for (int pt = w0; pt < p1; pt += AT_P) {
+        Raw8<KVT> rk[KS];
         float4v sc[2];
-        auto ask_v = [&](int b) {
-#pragma unroll
-            for (int u = 0; u < VU / VB; u++) {
-                const int p = (b * (VU / VB) + u) * VR + lane / VC, ch = lane % VC;
-                if constexpr (KVT == KV_F16) { /* chunk ch of the LDS row is the row's chunk ch ^ ... */
-                    const int col = d0 + ((ch ^ ((p & 3) << 1)) << 3);
-                    const unsigned short *src = (const unsigned short *)a.vc + row_at(p) * hd + (col < hd ? col : 0);
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)(uintptr_t)src,
-                                                     (__attribute__((address_space(3))) uint32_t *)(uintptr_t)(tv + u * VR * OD), 16, 0, 0);
-                } else {
-                    const int col = d0 + ch * 8;
-                    rv[u] = load8<KVT>(a.vc, row_at(p), hd, col < hd ? col : 0);
-                    vs[u] = scale_of<KVT>(a, a.vc, row_at(p));
-                }
-            }
-        };
         auto put_v = [&](int b) {
 #pragma unroll
             for (int u = 0; u < VU / VB; u++) {
@@ -565,18 +570,18 @@ __global__ __launch_bounds__(256, HDP <= 128 || (HDP == 256 && KVT == KV_F16) ? 
             }
         };
         nmx_lds_wave_sync(); /* the last tile's values have been read */
-        ask_v(0);
+        if (KVT != KV_F16 || pt != w0) ask_v(pt, 0);
         /* scores: positions 16 i + 4 gq + j against row c */
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const size_t R = row_at(16 * i + c);
+            const size_t R = row_at(pt + 16 * i + c);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 const int col = 32 * k + 8 * gq;
                 rk[k] = load8<KVT>(a.kc, R, hd, col < hd ? col : 0);
             }
             float ks = scale_of<KVT>(a, a.kc, R), up = 1.0f;
-            if (VB == 2 && i == 1) put_v(0), ask_v(1);
+            if (VB == 2 && i == 1) put_v(0), ask_v(pt, 1);
             sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
             if constexpr (KVT == KV_F32) {
                 float am = amax8(rk[0]);
@@ -620,99 +625,101 @@ __global__ __launch_bounds__(256, HDP <= 128 || (HDP == 256 && KVT == KV_F16) ? 
         }
         add_tile<OD, KVT>(r, x, e, f, vb, AT_P * OD);
     }
-    /* the waves' results joined, one after the other into wave 0's; 4 DT + 3 words of a lane each */
-    constexpr int XW = 64 * (4 * DT + 4);
-    float *xo = (float *)smem + lane;
+    /* the waves' results joined, a wave taking a quarter of the columns of all four */
+    constexpr int XW = 64 * DT, QD = DT / 4;
+    float4v *xo = (float4v *)smem + lane;
+    float4 *xs = (float4 *)((float4v *)smem + 4 * XW) + c;
     r.l += __shfl_xor(r.l, 16);
     r.l += __shfl_xor(r.l, 32);
     __syncthreads();
-    if (wave) {
-        float *my = xo + (wave - 1) * XW;
 #pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) my[(4 * d + j) * 64] = r.o[d][j];
-        my[4 * DT * 64] = r.m, my[(4 * DT + 1) * 64] = r.l, my[(4 * DT + 2) * 64] = (float)r.ve;
-    }
+    for (int d = 0; d < DT; d++) xo[wave * XW + d * 64] = r.o[d];
+    if (gq == 0) xs[wave * 16] = make_float4(r.m, (float)r.ve, r.l, 0.0f);
     __syncthreads();
-    if (wave) return;
-    float m = r.m;
+    float4 st[4];
+    float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 3; w++) m = fmaxf(m, xo[w * XW + 4 * DT * 64]);
+    for (int w = 0; w < 4; w++) st[w] = xs[w * 16], m = fmaxf(m, st[w].x);
     const float ref = m == -INFINITY ? 0.0f : m;
-    /* exponents count from a row's own maximum: the common one covers them all */
-    float top = (r.m - ref) + (float)r.ve;
+    /* exponents count from a wave's own maximum: the common one covers them all */
+    float top = -500.0f, l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 3; w++) top = fmaxf(top, (xo[w * XW + 4 * DT * 64] - ref) + xo[w * XW + (4 * DT + 2) * 64]);
-    const int vn = KVT == KV_F16 ? 0 : (int)ceilf(fmaxf(top, -500.0f));
-    auto shift = [&](float f, float v) { /* f 2^(v - vn) */
-        const float d = v - (float)vn;
-        return KVT == KV_F16 ? f : ldexpf(f, d < -300.0f ? -300 : (int)d);
-    };
-    const float f0 = __builtin_amdgcn_exp2f(r.m - ref), g0 = shift(f0, (float)r.ve);
-    r.l *= f0;
+    for (int w = 0; w < 4; w++) top = fmaxf(top, (st[w].x - ref) + st[w].y);
+    const int vn = KVT == KV_F16 ? 0 : (int)ceilf(top);
+    float4v o[QD];
 #pragma unroll
-    for (int d = 0; d < DT; d++) r.o[d] *= g0;
-#pragma unroll 1
-    for (int w = 0; w < 3; w++) {
-        const float *o = xo + w * XW;
-        const float fw = __builtin_amdgcn_exp2f(o[4 * DT * 64] - ref), gw = shift(fw, o[(4 * DT + 2) * 64]);
-        r.l += o[(4 * DT + 1) * 64] * fw;
+    for (int d = 0; d < QD; d++) o[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+    for (int w = 0; w < 4; w++) {
+        const float f = __builtin_amdgcn_exp2f(st[w].x - ref), up = st[w].y - (float)vn;
+        const float fv = KVT == KV_F16 ? f : ldexpf(f, up < -300.0f ? -300 : (int)up);
+        l += st[w].z * f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) r.o[d][j] += o[(4 * d + j) * 64] * gw;
+        for (int d = 0; d < QD; d++) {
+            const float4v y = xo[w * XW + (QD * wave + d) * 64];
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[d][j] = __builtin_fmaf(y[j], fv, o[d][j]);
+        }
     }
-    r.m = m, r.ve = vn;
-    if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);
+    if (hrow < 0) return;
+    const size_t at = (size_t)s * a.n * a.nh + hrow;
+#pragma unroll
+    for (int d = 0; d < QD; d++) {
+        const int col = d0 + 16 * (QD * wave + d) + 4 * gq;
+        if (col < hd) *(float4v *)(a.part + at * hd + col) = o[d];
+    }
+    if (wave == 0 && gq == 0) {
+        if (d0) a.stat[at].w = (float)vn;
+        else a.stat[at].x = m, a.stat[at].y = (float)vn, a.stat[at].z = l;
+    }
 }
 
 /* ---- the node's ancestors, and the join ---------------------------------------------------- */
-constexpr int JT = 1024; /* threads of a join */
+constexpr int JT = 512; /* threads of a join */
 
+/* Workgroup: a node and head, blockIdx.y a group of a.jcols columns of it. */
 template <int KVT>
 __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
-    __shared__ float sc[64], red[32], acc_s[JT * 4], w_s[2][AT_MAXS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ float sc[64], red[2 * (JT / 64)], acc_s[JT * 4], w_s[2][AT_MAXS];
+    __shared__ int anc_s[64];
+    const int lane = lane_id(), wave = wave_id(), tid = 64 * wave + lane;
     const int hrow = blockIdx.x, t = hrow / a.nh, h = hrow % a.nh, hd = a.hd, nd = hd >> 6;
-    const int g = h / (a.nh / a.nkv), rows = a.n * a.nh;
-    const int len = ctx_len(a), per = part_len(a, len), parts = per ? (len + per - 1) / per : 0;
-    const size_t R0 = (size_t)g * a.max_ctx;
+    const int g = h / (a.nh / a.nkv), rows = a.n * a.nh, c0 = blockIdx.y * a.jcols;
     const float *qp = a.q + (size_t)hrow * 2 * hd;
-    /* slots of hd / 4 threads: a thread takes 4 columns of every slots-th row of a sum */
-    const int per_slot = hd >> 2, slots = JT / per_slot, slot = tid / per_slot, col = tid % per_slot * 4;
-    constexpr int PB = 8; /* rows of a slot requested at once */
-    float4 pr[PB];
-#pragma unroll
-    for (int u = 0; u < PB; u++) {
-        const int s = slot + u * slots;
-        pr[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (slot < slots && s < parts) pr[u] = *(const float4 *)(a.part + ((size_t)s * rows + hrow) * hd + col);
-    }
-    float4 st = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f); /* thread = part */
-    if (tid < parts) st = a.stat[(size_t)tid * rows + hrow];
+    /* requested at entry, whatever the context's length: a part's numbers past the last one are not used */
+    const int above = lane < a.n ? tree_parent(a.parent, lane) : -1;
+    float4 st = a.stat[(size_t)(tid < a.splits ? tid : 0) * rows + hrow]; /* thread = part */
     float q[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) q[i] = i < nd ? qp[lane + 64 * i] : 0.0f;
-    /* the ancestors' rows inside the cache */
-    const int p0 = tree_slot0(a.pos, a.pos_off, a.max_ctx);
-    unsigned long long set = __shfl(tree_ancestors(a.parent, a.n, nullptr), t);
-    const int lo = p0 < 0 ? -p0 : 0, hi = a.max_ctx - p0; /* nodes lo .. hi - 1 have a slot */
-    if (lo > 63 || hi <= 0) set = 0;
-    else {
-        set &= ~0ull << lo;
-        if (hi < 64) set &= (1ull << hi) - 1;
-    }
-    const int na = __popcll(set);
-    auto nth = [&](int i) { /* the i-th node of the set */
-        unsigned long long x = set;
-        for (int k = 0; k < i; k++) x &= x - 1;
-        return __ffsll((long long)x) - 1;
+    for (int i = 0; i < 8; i++) q[i] = qp[i < nd ? lane + 64 * i : lane];
+    const float gate = qp[hd + c0 + (tid < a.jcols ? tid : 0)];
+    const int len = ctx_len(a), per = part_len(a, len), parts = per ? (len + per - 1) / per : 0;
+    /* slots of jcols / 4 threads: a thread takes 4 columns of every slots-th row of a sum */
+    const int per_slot = a.jcols >> 2, slots = JT / per_slot, slot = tid / per_slot, col = c0 + tid % per_slot * 4;
+    constexpr int PB = 8; /* rows of a slot requested at once */
+    float4 pr[PB];
+    auto ask = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < PB; u++) {
+            const int s = s0 + u * slots;
+            if (s < parts) pr[u] = *(const float4 *)(a.part + ((size_t)s * rows + hrow) * hd + col);
+        }
     };
+    if (slot < slots) ask(slot);
+    /* the ancestors' rows inside the cache, from the node up: lane i keeps the i-th */
+    const int p0 = tree_slot0(a.pos, a.pos_off, a.max_ctx);
+    int na = 0, mine = 0;
+    for (int x = t; x >= 0; x = __builtin_amdgcn_readlane(above, x)) {
+        if (p0 + x < 0 || p0 + x >= a.max_ctx) continue;
+        mine = lane == na ? x : mine;
+        na++;
+    }
+    if (wave == 0) anc_s[lane] = mine;
+    const size_t R0 = (size_t)g * a.max_ctx + p0;
     /* scores: a wave for each ancestor */
     float mt = -INFINITY;
     for (int i = wave; i < na; i += JT / 64) {
-        const size_t R = R0 + p0 + nth(i);
+        const size_t R = R0 + __builtin_amdgcn_readlane(mine, i);
         const float rs = scale_of<KVT>(a, a.kc, R);
         float d = 0.0f;
 #pragma unroll
@@ -730,27 +737,30 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
         if (lane == 0) sc[i] = d;
         mt = fmaxf(mt, d);
     }
+    if (tid >= parts) st = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
     mt = fmaxf(mt, nmx_max_f32_wave(st.x));
     if (lane == 0) red[wave] = mt;
-    __syncthreads();
+    nmx_lds_sync();
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < JT / 64; w++) m = fmaxf(m, red[w]);
     const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
     if (tid < parts) { /* a part's weight, for its sum and for its 2^12 high values */
         const float w = __builtin_amdgcn_exp2f(st.x - ref);
-        st.z *= w;
+        l = st.z * w;
         w_s[0][tid] = ldexpf(w, (int)st.y - 12);
         w_s[1][tid] = hd > 256 ? ldexpf(w, (int)st.w - 12) : 0.0f;
     }
-    float l = tid < na ? __builtin_amdgcn_exp2f(sc[tid] - ref) : 0.0f;
-    __syncthreads();
-    if (tid < na) sc[tid] = l;
-    l += st.z;
+    if (tid < na) {
+        const float w = __builtin_amdgcn_exp2f(sc[tid] - ref);
+        sc[tid] = w; /* no other thread reads it before the next barrier */
+        l += w;
+    }
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x);
-    if (lane == 0) red[16 + wave] = l;
-    __syncthreads();
+    if (lane == 0) red[JT / 64 + wave] = l;
+    nmx_lds_sync();
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto add = [&](float w, float4 x) {
         acc.x = __builtin_fmaf(w, x.x, acc.x), acc.y = __builtin_fmaf(w, x.y, acc.y);
@@ -758,35 +768,36 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
     };
     if (slot < slots) {
         const float *ws = w_s[col >> 8];
+        for (int s0 = slot; s0 < parts; s0 += PB * slots) {
+            if (s0 != slot) ask(s0);
 #pragma unroll
-        for (int u = 0; u < PB; u++) {
-            const int s = slot + u * slots;
-            if (s < parts) add(ws[s], pr[u]);
+            for (int u = 0; u < PB; u++) {
+                const int s = s0 + u * slots;
+                if (s < parts) add(ws[s], pr[u]);
+            }
         }
-        for (int s = slot + PB * slots; s < parts; s += slots)
-            add(ws[s], *(const float4 *)(a.part + ((size_t)s * rows + hrow) * hd + col));
         for (int i = slot; i < na; i += slots)
-            add(sc[i], kv_load4<KVT>(a.vc, R0 + p0 + nth(i), hd, col,
+            add(sc[i], kv_load4<KVT>(a.vc, R0 + anc_s[i], hd, col,
                                      KVT == KV_I8 ? (const float *)((const int8_t *)a.vc + (size_t)a.nkv * a.max_ctx * hd) : nullptr));
-        *(float4 *)(acc_s + slot * hd + col) = acc;
+        *(float4 *)(acc_s + slot * a.jcols + col - c0) = acc;
     }
-    __syncthreads();
-    if (tid < hd) {
+    nmx_lds_sync();
+    if (tid < a.jcols) {
         float sum = 0.0f, v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < JT / 64; w++) sum += red[16 + w];
-        for (int w = 0; w < slots; w++) v += acc_s[w * hd + tid];
+        for (int w = 0; w < JT / 64; w++) sum += red[JT / 64 + w];
+        for (int w = 0; w < slots; w++) v += acc_s[w * a.jcols + tid];
         v = sum > 0.0f || !(sum == sum) ? v / sum : 0.0f; /* no row at all in sight: 0 */
-        v = v * nmx_sigmoid(qp[hd + tid]);
-        const int at = h * hd + tid;
+        v = v * nmx_sigmoid(gate);
+        const int at = h * hd + c0 + tid;
         a.o[(size_t)t * a.nh * hd + at] = v;
-        if (a.aq) a8_block(v, at >> 5, t, a.n, a.aq, a.ad, a.afs); /* hd % 64 == 0: whole blocks */
+        if (a.aq) a8_block(v, at >> 5, t, a.n, a.aq, a.ad, a.afs); /* jcols % 64 == 0: whole blocks */
     }
 }
 
 /* How the context is divided among workgroups. */
 struct Plan {
-    int hdp, mtiles, splits, unit, halves;
+    int hdp, mtiles, splits, unit, halves, jcols;
     bool few; /* attn_tree_few_k, else attn_tree_ctx_k */
     size_t part_bytes, bytes, lds;
 };
@@ -803,14 +814,19 @@ Plan make_plan(int n, int nh, int nkv, int hd, int kv_dtype) {
     /* the many-row kernel has a CU for itself; of the other's workgroups two share one */
     const int s = (p.few ? 512 : 256) / (nkv * p.mtiles * p.halves);
     p.splits = s < 1 ? 1 : s > AT_MAXS ? AT_MAXS : s;
-    p.unit = p.few ? 4 * AT_P : AT_P;
+    p.unit = p.few ? 16 : AT_P;
     if (p.few) {
         p.lds = (size_t)4 * planes * AT_P * od * 2 + 4 * 3 * AT_P * 4;
-        const size_t join = (size_t)3 * 64 * (od / 4 + 4) * 4;
+        const size_t join = (size_t)4 * (64 * od / 16 + 16) * 16;
         if (join > p.lds) p.lds = join;
     } else {
         p.lds = (size_t)(p.hdp > 256 ? 1 : 2) * (planes * AT_P * (p.hdp + od) * 2 + 3 * AT_P * 4);
     }
+    /* with few rows their columns are shared out too, while the chip holds the workgroups in one round */
+    int groups = 1;
+    for (int k = 2; k <= hd / 64; k++)
+        if (hd / 64 % k == 0 && n * nh * k <= 512) groups = k;
+    p.jcols = hd / groups;
     p.part_bytes = (size_t)p.splits * n * nh * hd * 4;
     p.bytes = p.part_bytes + (size_t)p.splits * n * nh * sizeof(float4);
     return p;
@@ -838,7 +854,7 @@ int launch_tree(nmx_ctx *ctx, const TreeAttn &a, const Plan &p) {
     const int rc = p.hdp == 64 ? launch_ctx<64, KVT>(ctx, a, p) : p.hdp == 128 ? launch_ctx<128, KVT>(ctx, a, p) :
                    p.hdp == 256 ? launch_ctx<256, KVT>(ctx, a, p) : launch_ctx<512, KVT>(ctx, a, p);
     if (rc) return rc;
-    attn_tree_join_k<KVT><<<(unsigned)(a.n * a.nh), JT, 0, ctx->stream>>>(a);
+    attn_tree_join_k<KVT><<<dim3((unsigned)(a.n * a.nh), (unsigned)(a.hd / a.jcols)), JT, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "attn_tree_join");
     return 0;
 }
@@ -907,7 +923,7 @@ int nmx_attn_tree(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent, v
         return nmx_fail(ctx, "nmx_attn_tree: o, work and the inputs overlap");
     const TreeAttn a{p->n, p->nh, p->nkv, p->hd, p->max_ctx, p->q, p->kc, p->vc, p->pos, parent, p->pos_off,
                      p->scale, (float *)work, (float4 *)((char *)work + pl.part_bytes), pl.splits, pl.unit,
-                     p->o, p->a8.q, p->a8.d, p->a8.fs};
+                     pl.jcols, p->o, p->a8.q, p->a8.d, p->a8.fs};
     const nmx_on_device on(ctx);
     if (p->kv_dtype == KV_F16) return launch_tree<KV_F16>(ctx, a, pl);
     if (p->kv_dtype == KV_I8) return launch_tree<KV_I8>(ctx, a, pl);

@@ -157,24 +157,31 @@ struct Raw8<KV_I8> {
     uint2 a;
 };
 
+/* One head of a cache: its rows and, int8, their scales. A head has at most 2^20 rows of 512 values, so
+ * a byte offset in it has 32 bits and an address is a scalar base plus one register. */
 template <int KVT>
-__device__ __forceinline__ Raw8<KVT> load8(const void *cache, size_t R, int hd, int col) {
-    Raw8<KVT> r;
-    if constexpr (KVT == KV_F32) {
-        const uint4 *s = (const uint4 *)((const float *)cache + R * hd + col);
-        r.a = s[0], r.b = s[1];
-    } else if constexpr (KVT == KV_F16) {
-        r.a = *(const uint4 *)((const unsigned short *)cache + R * hd + col);
-    } else {
-        r.a = *(const uint2 *)((const int8_t *)cache + R * hd + col);
+struct Head {
+    const char *rows;
+    const float *scales;
+    int hd;
+    static constexpr int SIZE = KVT == KV_F32 ? 4 : KVT == KV_F16 ? 2 : 1;
+    __device__ __forceinline__ Head(const TreeAttn &a, const void *cache, int g)
+        : rows((const char *)cache + (size_t)g * a.max_ctx * a.hd * SIZE),
+          scales((const float *)((const char *)cache + (size_t)a.nkv * a.max_ctx * a.hd) + (size_t)g * a.max_ctx), hd(a.hd) {}
+    __device__ __forceinline__ const char *at(int p, int col) const { return rows + (uint32_t)(p * hd + col) * SIZE; }
+    __device__ __forceinline__ Raw8<KVT> load8(int p, int col) const {
+        Raw8<KVT> r;
+        const char *s = at(p, col);
+        if constexpr (KVT == KV_F32) r.a = *(const uint4 *)s, r.b = *(const uint4 *)(s + 16);
+        else if constexpr (KVT == KV_F16) r.a = *(const uint4 *)s;
+        else r.a = *(const uint2 *)s;
+        return r;
     }
-    return r;
-}
-template <int KVT>
-__device__ __forceinline__ float scale_of(const TreeAttn &a, const void *cache, size_t R) {
-    if constexpr (KVT == KV_I8) return ((const float *)((const int8_t *)cache + (size_t)a.nkv * a.max_ctx * a.hd))[R];
-    return 1.0f;
-}
+    __device__ __forceinline__ float scale(int p) const {
+        if constexpr (KVT == KV_I8) return scales[(uint32_t)p];
+        return 1.0f;
+    }
+};
 __device__ __forceinline__ half8 codes8(uint2 w) {
     half8 h;
 #pragma unroll
@@ -201,38 +208,51 @@ __device__ __forceinline__ void split8(const float (&x)[8], float up, half8 &h, 
     }
 }
 
-/* Lane c of 16 (quarter gq) takes its query row's chunks 4 k + gq, split; the result is the factor that
- * turns a product of parts into a score in powers of two. Columns past hd are zeros. */
+/* Lane c of 16 (quarter gq) takes its query row's chunks 4 k + gq: requested first, split when the
+ * cache's first rows have been requested too. Columns past hd are zeros. */
 template <int KS>
-__device__ __forceinline__ float load_q(const float *qp, bool live, int hd, int gq, float scale, half8 (&qh)[KS], half8 (&ql)[KS]) {
-    constexpr int HELD = KS <= 4 ? KS : 1; /* a longer row is read again instead of held */
+struct QueryRow {
+    static constexpr int HELD = KS <= 8 ? KS : 1; /* a longer row is read again instead of held */
+    const float *qp;
+    bool live;
+    int hd, gq;
     float4 x[HELD][2];
-    auto get = [&](int k, float4 (&y)[2]) {
-        const int col = k * 32 + gq * 8;
-        y[0] = y[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (live && col < hd) y[0] = *(const float4 *)(qp + col), y[1] = *(const float4 *)(qp + col + 4);
-    };
-    float am = 0.0f;
-#pragma unroll
-    for (int k = 0; k < KS; k++) {
-        float4(&y)[2] = x[k % HELD];
-        get(k, y);
-        am = fmaxf(am, fmaxf(fmaxf(fabsf(y[0].x), fabsf(y[0].y)), fmaxf(fabsf(y[0].z), fabsf(y[0].w))));
-        am = fmaxf(am, fmaxf(fmaxf(fabsf(y[1].x), fabsf(y[1].y)), fmaxf(fabsf(y[1].z), fabsf(y[1].w))));
+    __device__ __forceinline__ void get(int k) {
+        const int col = k * 32 + gq * 8, at = live && col < hd ? col : 0; /* qp is in bounds for every lane */
+        x[k % HELD][0] = *(const float4 *)(qp + at), x[k % HELD][1] = *(const float4 *)(qp + at + 4);
     }
-    am = fmaxf(am, __shfl_xor(am, 16));
-    am = fmaxf(am, __shfl_xor(am, 32));
-    const int e = row_exp(am);
-    const float up = pow2f(12 - e);
+    __device__ __forceinline__ QueryRow(const float *qp, bool live, int hd, int gq) : qp(qp), live(live), hd(hd), gq(gq) {
+        if constexpr (HELD == KS)
 #pragma unroll
-    for (int k = 0; k < KS; k++) {
-        float4(&y)[2] = x[k % HELD];
-        if (HELD < KS) get(k, y);
-        const float z[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
-        split8(z, up, qh[k], ql[k]);
+            for (int k = 0; k < KS; k++) get(k);
     }
-    return pow2f(e - 12) * (scale * AT_LOG2E);
-}
+    /* the parts; the result is the factor that turns a product of parts into a score in powers of two */
+    __device__ __forceinline__ float split(float scale, half8 (&qh)[KS], half8 (&ql)[KS]) {
+        float am = 0.0f;
+        auto in = [&](int k) { return live && k * 32 + gq * 8 < hd; };
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            if (HELD < KS) get(k);
+            float4(&y)[2] = x[k % HELD];
+            float b = fmaxf(fmaxf(fmaxf(fabsf(y[0].x), fabsf(y[0].y)), fmaxf(fabsf(y[0].z), fabsf(y[0].w))),
+                            fmaxf(fmaxf(fabsf(y[1].x), fabsf(y[1].y)), fmaxf(fabsf(y[1].z), fabsf(y[1].w))));
+            am = fmaxf(am, in(k) ? b : 0.0f);
+        }
+        am = fmaxf(am, __shfl_xor(am, 16));
+        am = fmaxf(am, __shfl_xor(am, 32));
+        const int e = row_exp(am);
+        const float up = pow2f(12 - e);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            if (HELD < KS) get(k);
+            float4(&y)[2] = x[k % HELD];
+            const float z[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
+            split8(z, up, qh[k], ql[k]);
+            if (!in(k)) qh[k] = ql[k] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+        return pow2f(e - 12) * (scale * AT_LOG2E);
+    }
+};
 
 /* A row's running state: weights are 2^(score - m); a value's factor 2^(its exponent - ve), where ve
  * grows so that no weight times value leaves binary16; l is this lane's share of the sum. */
@@ -344,14 +364,15 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
     const int lane = lane_id(), wave = wave_id(), tid = 64 * wave + lane, c = lane & 15, gq = lane >> 4;
     const int s = blockIdx.x % a.splits, g = blockIdx.x / a.splits % a.nkv, mt = blockIdx.x / a.splits / a.nkv;
     const int d0 = blockIdx.y * OD; /* the output columns: of 512, half */
-    const int len = ctx_len(a), per = part_len(a, len), hd = a.hd, rep = a.nh / a.nkv, rows = a.n * rep;
-    const int p0 = s * per;
-    if (per == 0 || p0 >= len) return;
-    const int p1 = p0 + per < len ? p0 + per : len;
+    const int hd = a.hd, rep = a.nh / a.nkv, rows = a.n * rep;
     const int row0 = (mt * ctx_waves<HDP>() + wave) * 16, row = row0 + c;
     const int hrow = row < rows ? (row / rep) * a.nh + g * rep + row % rep : -1; /* (node, head) */
     const bool busy = row0 < rows;
-    const size_t R0 = (size_t)g * a.max_ctx;
+    QueryRow<KS> qr(a.q + (size_t)(hrow < 0 ? 0 : hrow) * 2 * hd, hrow >= 0, hd, gq);
+    const Head<KVT> kh(a, a.kc, g), vh(a, a.vc, g);
+    const int len = ctx_len(a), per = part_len(a, len), p0 = s * per;
+    if (per == 0 || p0 >= len) return;
+    const int p1 = p0 + per < len ? p0 + per : len;
 
     /* staging: columns and rows past the end repeat ones inside (finite, and their weight is 0) */
     Raw8<KVT> rk[KU], rv[VU];
@@ -360,18 +381,18 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
 #pragma unroll
         for (int u = 0; u < KU; u++) {
             const int f = u * TH + tid, p = f / KC & (AT_P - 1), col = f % KC * 8;
-            const size_t R = R0 + (pt + p < p1 ? pt + p : p1 - 1);
-            rk[u] = load8<KVT>(a.kc, R, hd, col < hd ? col : 0);
-            sk[u] = scale_of<KVT>(a, a.kc, R);
+            const int at = pt + p < p1 ? pt + p : p1 - 1;
+            rk[u] = kh.load8(at, col < hd ? col : 0);
+            sk[u] = kh.scale(at);
         }
     };
     auto fetch_v = [&](int pt) {
 #pragma unroll
         for (int u = 0; u < VU; u++) {
             const int f = u * TH + tid, p = f / VC & (AT_P - 1), col = d0 + f % VC * 8;
-            const size_t R = R0 + (pt + p < p1 ? pt + p : p1 - 1);
-            rv[u] = load8<KVT>(a.vc, R, hd, col < hd ? col : 0);
-            sv[u] = scale_of<KVT>(a, a.vc, R);
+            const int at = pt + p < p1 ? pt + p : p1 - 1;
+            rv[u] = vh.load8(at, col < hd ? col : 0);
+            sv[u] = vh.scale(at);
         }
     };
     auto put_k = [&](int buf) {
@@ -432,7 +453,7 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
     };
     if constexpr (NB == 2) fetch_k(p0), fetch_v(p0);
     half8 qh[KS], ql[KS];
-    const float qfac = load_q<KS>(a.q + (size_t)(hrow < 0 ? 0 : hrow) * 2 * hd, hrow >= 0, hd, gq, a.scale, qh, ql);
+    const float qfac = qr.split(a.scale, qh, ql);
     Running<DT> r;
     if (NB == 2) put_k(0), put_v(0);
     /* this lane's operand addresses in a tile: the XORs leave two bases for the keys (chunk 4 k + gq by
@@ -491,136 +512,197 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
     if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);
 }
 
-/* Few rows: the time is that of the cache's bytes, so each of 4 waves takes tiles of its own, its
- * keys straight into matrix operands, its values through a piece of LDS of its own (a binary16
- * cache's without a register between), requested together; two workgroups to a CU keep the requests
- * coming. The waves' results are joined at the end. */
+/* Few rows: the time is that of the cache's bytes, so each of 4 waves takes positions of its own, the
+ * keys straight into matrix operands, the values through a piece of LDS of its own (a binary16 cache's
+ * without a register between), all of a tile requested together and before the query rows have come;
+ * the split query rows are the waves' common operand in LDS. Two workgroups to a CU keep the requests
+ * coming (80 KB of LDS each up to 256 columns; an fp32 cache's has a CU for itself). The waves' results
+ * are joined at the end. */
 template <int HDP, int KVT>
-__global__ __launch_bounds__(256, HDP <= 128 || (HDP == 256 && KVT == KV_F16) ? 2 : 1) void attn_tree_few_k(TreeAttn a) {
+constexpr int few_lds() {
+    return 4 * (KVT == KV_F32 ? 2 : 1) * AT_P * (HDP > 256 ? 256 : HDP) * 2 /* values */ + 2 * 16 * HDP * 2 /* query rows */ +
+           (KVT == KV_F32 ? 4 * 2 * AT_P * 4 : 0) /* the values' exponents and fractions */;
+}
+template <int HDP, int KVT>
+__global__ __launch_bounds__(256, (few_lds<HDP, KVT>() <= 80 * 1024 ? 2 : 1)) void attn_tree_few_k(TreeAttn a) {
     constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32, DT = OD / 16;
     constexpr int PL = KVT == KV_F32 ? 2 : 1, VC = OD / 8, VR = 64 / VC; /* rows of a wave's request */
-    constexpr int VU = AT_P / VR, VB = KVT == KV_F16 ? 1 : 2; /* requests of a tile, taken in VB batches */
+    constexpr int VU = AT_P / VR;
     extern __shared__ uint4 smem[];
     const int lane = lane_id(), wave = wave_id(), c = lane & 15, gq = lane >> 4;
-    _Float16 *tv = (_Float16 *)smem + wave * PL * AT_P * OD;
-    float *aux = (float *)((_Float16 *)smem + 4 * PL * AT_P * OD) + wave * 3 * AT_P, *kf = aux, *vf = aux + AT_P;
-    int *ve = (int *)(aux + 2 * AT_P);
+    _Float16 *tv = (_Float16 *)smem + wave * PL * AT_P * OD, *tq = (_Float16 *)smem + 4 * PL * AT_P * OD;
+    float *vf = (float *)(tq + 2 * 16 * HDP) + wave * 2 * AT_P; /* fp32 */
+    int *ve = (int *)(vf + AT_P);
     const int s = blockIdx.x % a.splits, g = blockIdx.x / a.splits % a.nkv, mt = blockIdx.x / a.splits / a.nkv;
-    const int d0 = blockIdx.y * OD, hd = a.hd, rep = a.nh / a.nkv, row = mt * 16 + c;
-    const int hrow = row < a.n * rep ? (row / rep) * a.nh + g * rep + row % rep : -1; /* (node, head) */
-    const size_t R0 = (size_t)g * a.max_ctx;
+    const int d0 = blockIdx.y * OD, hd = a.hd, rep = a.nh / a.nkv, rows = a.n * rep;
+    auto head_row = [&](int row) { return row < rows ? (row / rep) * a.nh + g * rep + row % rep : -1; }; /* (node, head) */
+    /* the query rows: 16 lanes each, chunks of 8 columns */
+    const int qr = 4 * wave + gq, qrow = head_row(mt * 16 + qr);
+    constexpr int QU = HDP > 128 ? HDP / 128 : 1;
+    const float *qp = a.q + (size_t)(qrow < 0 ? 0 : qrow) * 2 * hd;
+    float4 qx[QU][2];
+#pragma unroll
+    for (int u = 0; u < QU; u++) {
+        const int col = (16 * u + c) * 8, at = col < hd ? col : 0;
+        qx[u][0] = *(const float4 *)(qp + at), qx[u][1] = *(const float4 *)(qp + at + 4);
+    }
+    const Head<KVT> kh(a, a.kc, g), vh(a, a.vc, g);
     const int len = ctx_len(a), per = part_len(a, len);
     if (per == 0 || s * per >= len) return;
     /* a quarter of the part for each wave */
     const int w0 = s * per + wave * (per >> 2);
     const int p1 = w0 + (per >> 2) < len ? w0 + (per >> 2) : len;
     /* rows and columns past the end repeat ones inside (finite, and their weight is 0) */
-    auto row_at = [&](int p) { return R0 + (p < p1 ? p : p1 - 1); };
-    Raw8<KVT> rv[VU / VB];
-    float vs[VU / VB];
-    auto ask_v = [&](int pt, int b) {
-#pragma unroll
-        for (int u = 0; u < VU / VB; u++) {
-            const int p = (b * (VU / VB) + u) * VR + lane / VC, ch = lane % VC;
-            if constexpr (KVT == KV_F16) { /* chunk ch of the LDS row is the row's chunk ch ^ ... */
-                const int col = d0 + ((ch ^ ((p & 3) << 1)) << 3);
-                const unsigned short *src = (const unsigned short *)a.vc + row_at(pt + p) * hd + (col < hd ? col : 0);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)(uintptr_t)src,
-                                                 (__attribute__((address_space(3))) uint32_t *)(uintptr_t)(tv + u * VR * OD), 16, 0, 0);
-            } else {
-                const int col = d0 + ch * 8;
-                rv[u] = load8<KVT>(a.vc, row_at(pt + p), hd, col < hd ? col : 0);
-                vs[u] = scale_of<KVT>(a, a.vc, row_at(pt + p));
-            }
-        }
-    };
-    if (KVT == KV_F16 && w0 < p1) ask_v(w0, 0); /* on its way while the query rows are split */
-    half8 qh[KS], ql[KS];
-    const float qfac = load_q<KS>(a.q + (size_t)(hrow < 0 ? 0 : hrow) * 2 * hd, hrow >= 0, hd, gq, a.scale, qh, ql);
-    Running<DT> r;
-    const int vp = 4 * gq + (c >> 2);
-    const _Float16 *vb[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) vb[i] = tv + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
-    for (int pt = w0; pt < p1; pt += AT_P) {
-        Raw8<KVT> rk[KS];
-        float4v sc[2];
-        auto put_v = [&](int b) {
-#pragma unroll
-            for (int u = 0; u < VU / VB; u++) {
-                const int p = (b * (VU / VB) + u) * VR + lane / VC, ch = lane % VC, at = v_at<OD>(p, ch);
-                if constexpr (KVT == KV_I8) {
-                    *(half8 *)(tv + at) = codes8(rv[u].a);
-                    if (ch == 0) {
-                        const int e = row_exp(vs[u]);
-                        ve[p] = e, vf[p] = vs[u] * pow2f(-e);
-                    }
-                } else if constexpr (KVT == KV_F32) {
-                    float am = amax8(rv[u]), x[8];
-#pragma unroll
-                    for (int w = 1; w < VC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
-                    const int e = row_exp(am);
-                    half8 h, y;
-                    floats8(rv[u], x);
-                    split8(x, pow2f(12 - e), h, y);
-                    *(half8 *)(tv + at) = h;
-                    *(half8 *)(tv + AT_P * OD + at) = y;
-                    if (ch == 0) ve[p] = e - 12, vf[p] = 1.0f;
-                }
-            }
-        };
-        nmx_lds_wave_sync(); /* the last tile's values have been read */
-        if (KVT != KV_F16 || pt != w0) ask_v(pt, 0);
-        /* scores: positions 16 i + 4 gq + j against row c */
+    auto row_at = [&](int p) { return p < p1 ? p : p1 - 1; };
+    Raw8<KVT> rk[2][KS], rv[VU];
+    float ks[2], vs[2]; /* int8: the scales of positions c and 16 + c */
+    auto ask = [&](int pt) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const size_t R = row_at(pt + 16 * i + c);
+            const int p = row_at(pt + 16 * i + c);
+            ks[i] = kh.scale(p), vs[i] = vh.scale(p);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 const int col = 32 * k + 8 * gq;
-                rk[k] = load8<KVT>(a.kc, R, hd, col < hd ? col : 0);
+                rk[i][k] = kh.load8(p, col < hd ? col : 0);
             }
-            float ks = scale_of<KVT>(a, a.kc, R), up = 1.0f;
-            if (VB == 2 && i == 1) put_v(0), ask_v(pt, 1);
-            sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (KVT == KV_F32) {
-                float am = amax8(rk[0]);
+        }
 #pragma unroll
-                for (int k = 1; k < KS; k++) am = fmaxf(am, amax8(rk[k]));
+        for (int u = 0; u < VU; u++) {
+            const int p = u * VR + lane / VC, ch = lane % VC;
+            if constexpr (KVT == KV_F16) { /* chunk ch of the LDS row is the row's chunk ch ^ ... */
+                const int col = d0 + ((ch ^ ((p & 3) << 1)) << 3);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)(uintptr_t)vh.at(row_at(pt + p), col < hd ? col : 0),
+                                                 (__attribute__((address_space(3))) uint32_t *)(uintptr_t)(tv + u * VR * OD), 16, 0, 0);
+            } else {
+                const int col = d0 + ch * 8;
+                rv[u] = vh.load8(row_at(pt + p), col < hd ? col : 0);
+            }
+        }
+    };
+    auto put_v = [&]() {
+#pragma unroll
+        for (int u = 0; u < VU; u++) {
+            const int p = u * VR + lane / VC, ch = lane % VC, at = v_at<OD>(p, ch);
+            if constexpr (KVT == KV_I8) {
+                *(half8 *)(tv + at) = codes8(rv[u].a);
+            } else if constexpr (KVT == KV_F32) {
+                float am = amax8(rv[u]), x[8];
+#pragma unroll
+                for (int w = 1; w < VC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
+                const int e = row_exp(am);
+                half8 h, y;
+                floats8(rv[u], x);
+                split8(x, pow2f(12 - e), h, y);
+                *(half8 *)(tv + at) = h;
+                *(half8 *)(tv + AT_P * OD + at) = y;
+                if (ch == 0) ve[p] = e - 12, vf[p] = 1.0f;
+            }
+        }
+    };
+    if (w0 < p1) ask(w0); /* on its way while the query rows are split */
+    float qfac;
+    {
+        float am = 0.0f;
+        auto in = [&](int u) { return qrow >= 0 && (16 * u + c) * 8 < hd; };
+#pragma unroll
+        for (int u = 0; u < QU; u++) {
+            float4(&y)[2] = qx[u];
+            const float b = fmaxf(fmaxf(fmaxf(fabsf(y[0].x), fabsf(y[0].y)), fmaxf(fabsf(y[0].z), fabsf(y[0].w))),
+                                  fmaxf(fmaxf(fabsf(y[1].x), fabsf(y[1].y)), fmaxf(fabsf(y[1].z), fabsf(y[1].w))));
+            am = fmaxf(am, in(u) ? b : 0.0f);
+        }
+#pragma unroll
+        for (int w = 1; w < 16; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
+        const int e = row_exp(am);
+        const float up = pow2f(12 - e);
+        /* the rows' factors go round through the place of their parts */
+        float *fac = (float *)tq;
+        if (c == 0) fac[qr] = pow2f(e - 12) * (a.scale * AT_LOG2E);
+        nmx_lds_sync();
+        qfac = fac[c];
+        nmx_lds_sync();
+#pragma unroll
+        for (int u = 0; u < QU; u++) {
+            float4(&y)[2] = qx[u];
+            const float z[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
+            half8 h, r;
+            split8(z, up, h, r);
+            if (!in(u)) h = r = half8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (HDP >= 128 || c * 8 < HDP) {
+                const int at = k_at<HDP>(qr, 16 * u + c);
+                *(half8 *)(tq + at) = h;
+                *(half8 *)(tq + 16 * HDP + at) = r;
+            }
+        }
+        nmx_lds_sync();
+    }
+    Running<DT> r;
+    const int vp = 4 * gq + (c >> 2);
+    const _Float16 *vb[4], *qb[2];
+#pragma unroll
+    for (int i = 0; i < 4; i++) vb[i] = tv + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
+#pragma unroll
+    for (int i = 0; i < 2; i++) qb[i] = tq + k_at<HDP>(c, 4 * i + gq) - 32 * i;
+    for (int pt = w0; pt < p1; pt += AT_P) {
+        if (pt != w0) {
+            nmx_lds_wave_sync(); /* the last tile's values have been read */
+            ask(pt);
+        }
+        /* scores: positions 16 i + 4 gq + j against row c */
+        float4v sc[2];
+        float kfac[2], up[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f}, kfac[i] = ks[i], up[i] = 1.0f;
+            if constexpr (KVT == KV_F32) {
+                float am = amax8(rk[i][0]);
+#pragma unroll
+                for (int k = 1; k < KS; k++) am = fmaxf(am, amax8(rk[i][k]));
                 am = fmaxf(am, __shfl_xor(am, 16));
                 am = fmaxf(am, __shfl_xor(am, 32));
                 const int e = row_exp(am);
-                up = pow2f(12 - e), ks = pow2f(e - 12);
+                up[i] = pow2f(12 - e), kfac[i] = pow2f(e - 12);
             }
-            if (KVT != KV_F16 && gq == 0) kf[16 * i + c] = ks;
+        }
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < KS; k++) {
+            const half8 qh = *(const half8 *)(qb[k & 1] + 32 * k), ql = *(const half8 *)(qb[k & 1] + 16 * HDP + 32 * k);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
                 half8 x, y;
                 if constexpr (KVT == KV_F16) {
-                    x = __builtin_bit_cast(half8, rk[k].a);
+                    x = __builtin_bit_cast(half8, rk[i][k].a);
                 } else if constexpr (KVT == KV_I8) {
-                    x = codes8(rk[k].a);
+                    x = codes8(rk[i][k].a);
                 } else {
                     float z[8];
-                    floats8(rk[k], z);
-                    split8(z, up, x, y);
+                    floats8(rk[i][k], z);
+                    split8(z, up[i], x, y);
                 }
-                sc[i] = mfma16(x, qh[k], sc[i]);
-                sc[i] = mfma16(x, ql[k], sc[i]);
-                if constexpr (KVT == KV_F32) sc[i] = mfma16(y, qh[k], sc[i]);
+                sc[i] = mfma16(x, qh, sc[i]);
+                sc[i] = mfma16(x, ql, sc[i]);
+                if constexpr (KVT == KV_F32) sc[i] = mfma16(y, qh, sc[i]);
             }
         }
         if constexpr (KVT == KV_F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* the values are in LDS */
-        else put_v(VB - 1);
+        else put_v();
         nmx_lds_wave_sync();
         float x[8], f[8];
         int e[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int p = 16 * (i >> 2) + 4 * gq + (i & 3);
-            float y = sc[i >> 2][i & 3];
-            if constexpr (KVT != KV_F16) y *= qfac * kf[p], e[i] = ve[p], f[i] = vf[p];
-            else y *= qfac, e[i] = 0, f[i] = 1.0f;
+            const int j = 4 * gq + (i & 3), p = 16 * (i >> 2) + j;
+            float y = sc[i >> 2][i & 3] * qfac;
+            if constexpr (KVT != KV_F16) y *= __shfl(kfac[i >> 2], j); /* a position's number is with lane j */
+            if constexpr (KVT == KV_I8) {
+                const float v = __shfl(vs[i >> 2], j);
+                e[i] = row_exp(v), f[i] = v * pow2f(-e[i]);
+            } else if constexpr (KVT == KV_F32) {
+                e[i] = ve[p], f[i] = vf[p];
+            } else {
+                e[i] = 0, f[i] = 1.0f;
+            }
             x[i] = pt + p < p1 ? y : -INFINITY;
         }
         add_tile<OD, KVT>(r, x, e, f, vb, AT_P * OD);
@@ -661,6 +743,7 @@ __global__ __launch_bounds__(256, HDP <= 128 || (HDP == 256 && KVT == KV_F16) ? 
             for (int j = 0; j < 4; j++) o[d][j] = __builtin_fmaf(y[j], fv, o[d][j]);
         }
     }
+    const int hrow = head_row(mt * 16 + c);
     if (hrow < 0) return;
     const size_t at = (size_t)s * a.n * a.nh + hrow;
 #pragma unroll
@@ -715,20 +798,21 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
         na++;
     }
     if (wave == 0) anc_s[lane] = mine;
-    const size_t R0 = (size_t)g * a.max_ctx + p0;
+    const Head<KVT> kh(a, a.kc, g);
     /* scores: a wave for each ancestor */
     float mt = -INFINITY;
     for (int i = wave; i < na; i += JT / 64) {
-        const size_t R = R0 + __builtin_amdgcn_readlane(mine, i);
-        const float rs = scale_of<KVT>(a, a.kc, R);
+        const int p = p0 + __builtin_amdgcn_readlane(mine, i);
+        const float rs = kh.scale(p);
         float d = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; k++)
             if (k < nd) {
+                const char *at = kh.at(p, lane + 64 * k);
                 float x;
-                if constexpr (KVT == KV_F32) x = ((const float *)a.kc)[R * hd + lane + 64 * k];
-                else if constexpr (KVT == KV_F16) x = kv_half_value(((const unsigned short *)a.kc)[R * hd + lane + 64 * k]);
-                else x = (float)((const int8_t *)a.kc)[R * hd + lane + 64 * k] * rs;
+                if constexpr (KVT == KV_F32) x = *(const float *)at;
+                else if constexpr (KVT == KV_F16) x = kv_half_value(*(const unsigned short *)at);
+                else x = (float)*(const int8_t *)at * rs;
                 d = __builtin_fmaf(q[k], x, d);
             }
 #pragma unroll
@@ -777,7 +861,7 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
             }
         }
         for (int i = slot; i < na; i += slots)
-            add(sc[i], kv_load4<KVT>(a.vc, R0 + anc_s[i], hd, col,
+            add(sc[i], kv_load4<KVT>(a.vc, (size_t)g * a.max_ctx + p0 + anc_s[i], hd, col,
                                      KVT == KV_I8 ? (const float *)((const int8_t *)a.vc + (size_t)a.nkv * a.max_ctx * hd) : nullptr));
         *(float4 *)(acc_s + slot * a.jcols + col - c0) = acc;
     }
@@ -799,14 +883,13 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
 struct Plan {
     int hdp, mtiles, splits, unit, halves, jcols;
     bool few; /* attn_tree_few_k, else attn_tree_ctx_k */
-    size_t part_bytes, bytes, lds;
+    size_t part_bytes, bytes;
 };
 
 Plan make_plan(int n, int nh, int nkv, int hd, int kv_dtype) {
     Plan p;
     p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
     const int tiles = (n * (nh / nkv) + 15) / 16, od = p.hdp > 256 ? 256 : p.hdp;
-    const int planes = kv_dtype == KV_F32 ? 2 : 1;
     p.few = tiles <= 2 && !(p.hdp > 256 && kv_dtype == KV_F32); /* too many registers */
     const int waves = p.hdp > 256 ? 4 : 8;
     p.mtiles = p.few ? tiles : (tiles + waves - 1) / waves;
@@ -815,13 +898,6 @@ Plan make_plan(int n, int nh, int nkv, int hd, int kv_dtype) {
     const int s = (p.few ? 512 : 256) / (nkv * p.mtiles * p.halves);
     p.splits = s < 1 ? 1 : s > AT_MAXS ? AT_MAXS : s;
     p.unit = p.few ? 16 : AT_P;
-    if (p.few) {
-        p.lds = (size_t)4 * planes * AT_P * od * 2 + 4 * 3 * AT_P * 4;
-        const size_t join = (size_t)4 * (64 * od / 16 + 16) * 16;
-        if (join > p.lds) p.lds = join;
-    } else {
-        p.lds = (size_t)(p.hdp > 256 ? 1 : 2) * (planes * AT_P * (p.hdp + od) * 2 + 3 * AT_P * 4);
-    }
     /* with few rows their columns are shared out too, while the chip holds the workgroups in one round */
     int groups = 1;
     for (int k = 2; k <= hd / 64; k++)
@@ -838,12 +914,17 @@ int launch_ctx(nmx_ctx *ctx, const TreeAttn &a, const Plan &p) {
     static std::atomic<uint64_t> set0, set1;
     if (p.few) {
         if constexpr (HDP <= 256 || KVT != KV_F32) {
-            if (nmx_dyn_lds(ctx, (const void *)attn_tree_few_k<HDP, KVT>, p.lds, set1)) return -1;
-            attn_tree_few_k<HDP, KVT><<<grid, 256, p.lds, ctx->stream>>>(a);
+            /* the join of the waves takes the place of the tiles */
+            constexpr int od = HDP > 256 ? 256 : HDP, join = 4 * (64 * od / 16 + 16) * 16;
+            constexpr int tiles = few_lds<HDP, KVT>(), lds = tiles > join ? tiles : join;
+            if (nmx_dyn_lds(ctx, (const void *)attn_tree_few_k<HDP, KVT>, lds, set1)) return -1;
+            attn_tree_few_k<HDP, KVT><<<grid, 256, lds, ctx->stream>>>(a);
         }
     } else {
-        if (nmx_dyn_lds(ctx, (const void *)attn_tree_ctx_k<HDP, KVT>, p.lds, set0)) return -1;
-        attn_tree_ctx_k<HDP, KVT><<<grid, 64 * ctx_waves<HDP>(), p.lds, ctx->stream>>>(a);
+        constexpr int od = HDP > 256 ? 256 : HDP, planes = KVT == KV_F32 ? 2 : 1;
+        constexpr int lds = (HDP > 256 ? 1 : 2) * (planes * AT_P * (HDP + od) * 2 + 3 * AT_P * 4);
+        if (nmx_dyn_lds(ctx, (const void *)attn_tree_ctx_k<HDP, KVT>, lds, set0)) return -1;
+        attn_tree_ctx_k<HDP, KVT><<<grid, 64 * ctx_waves<HDP>(), lds, ctx->stream>>>(a);
     }
     NMX_LAUNCHED(ctx, "attn_tree_ctx");
     return 0;

@@ -110,22 +110,31 @@ __device__ __forceinline__ double weight(float v, float mx, double inv) {
 /* The weight of grid position g relative to the lower edge of its bin, in 2^-40, for fr = g - floor(g):
  * 2^40 e^(fr / 8) about the bin's middle, degree 7 (the next term is below 6e-15), rounded to a whole
  * number by the addition of 2^52. */
-__device__ __forceinline__ unsigned long long bin_mass_at(double fr) {
-    constexpr double M = 0x1p40 * 1.0644944589178594296; /* e^(1/16) */
-    const double x = (fr - 0.5) * 0.125;
-    double p = M / 5040;
-    p = __builtin_fma(p, x, M / 720);
-    p = __builtin_fma(p, x, M / 120);
-    p = __builtin_fma(p, x, M / 24);
-    p = __builtin_fma(p, x, M / 6);
-    p = __builtin_fma(p, x, M / 2);
-    p = __builtin_fma(p, x, M);
-    p = __builtin_fma(p, x, M);
-    return (unsigned long long)__double_as_longlong(p + 0x1p52) & 0xfffffffffffffull;
-}
+struct BinPoly { /* the coefficients, in scalars: a lane's fma takes one from there without a move */
+    double c[8];
+    __device__ __forceinline__ BinPoly() {
+        constexpr double M = 0x1p40 * 1.0644944589178594296; /* e^(1/16) */
+        const double k[8] = {M, M / 8, M / (2 * 0x1p6), M / (6 * 0x1p9), M / (24 * 0x1p12), M / (120 * 0x1p15),
+                             M / (720 * 0x1p18), M / (5040 * 0x1p21)};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            c[i] = k[i];
+            asm("" : "+s"(c[i]));
+        }
+    }
+    /* the bits of 2^52 + the mass: 0x433 << 52 | mass */
+    __device__ __forceinline__ unsigned long long bits(double fr) const {
+        const double x = fr - 0.5;
+        double p = c[7];
+#pragma unroll
+        for (int i = 6; i >= 0; i--) p = __builtin_fma(p, x, c[i]);
+        return (unsigned long long)__double_as_longlong(p + 0x1p52);
+    }
+    __device__ __forceinline__ unsigned long long at(double fr) const { return bits(fr) & 0xfffffffffffffull; }
+};
 __device__ __forceinline__ unsigned long long bin_mass(float x, double inv) {
     const double g = grid_pos(x, inv);
-    return bin_mass_at(g - floor(g));
+    return BinPoly().at(g - floor(g));
 }
 
 __device__ __forceinline__ float block_max(float v, float *red, int waves) {
@@ -179,8 +188,8 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
     __shared__ float redf[SM_T1 / 64];
     __shared__ double redd[SM_T1 / 64];
     __shared__ unsigned long long redk[SM_T1 / 64];
-    __shared__ uint32_t cnt[SM_BINS * SM_COPY], wave_cnt[SM_T1 / 64];
-    __shared__ unsigned long long mass[SM_BINS * SM_COPY];
+    __shared__ uint32_t wave_cnt[SM_T1 / 64], first_s[SM_BINS * SM_COPY];
+    __shared__ unsigned long long bins[SM_BINS * SM_COPY]; /* members << 52 | mass */
     __shared__ uint32_t perm2[SM_CHUNK / 2];
     uint16_t *perm = (uint16_t *)perm2;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x, row = blockIdx.y;
@@ -248,12 +257,16 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
         }
         return;
     }
-    /* SM_COPY copies of each bin, by lane: neighbouring lanes of one bin do not wait for each other */
+    /* SM_COPY copies of each bin, by lane: neighbouring lanes of one bin do not wait for each other. A
+     * copy has at most SM_CHUNK / SM_COPY members of less than 1.14 2^40 each: 12 bits for them and 52
+     * for their mass, one addition for both */
+    static_assert(SM_CHUNK / SM_COPY * 1.14 * 0x1p40 < 0x1p52 && SM_CHUNK / SM_COPY < 4096, "a copy's word");
 #pragma unroll
-    for (int i = 0; i < SM_BINS * SM_COPY; i += SM_T1) cnt[i + tid] = 0, mass[i + tid] = 0;
+    for (int i = 0; i < SM_BINS * SM_COPY; i += SM_T1) bins[i + tid] = 0;
     __syncthreads();
     const double base = floor(grid_pos(mx, p.inv));
     const int copy = lane & (SM_COPY - 1);
+    const BinPoly poly;
     uint32_t at[SM_PER]; /* bin copy << 16 | rank; all ones: no weight */
 #pragma unroll
     for (int u = 0; u < SM_PER; u++) {
@@ -261,8 +274,7 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
         const double g = grid_pos(v[u], p.inv), fl = floor(g), d = base - fl; /* inf for -inf */
         if (d < (double)SM_BINS) {
             const uint32_t j = (uint32_t)(int)d * SM_COPY + copy;
-            at[u] = j << 16 | atomicAdd(&cnt[j], 1u);
-            atomicAdd(&mass[j], bin_mass_at(g - fl));
+            at[u] = j << 16 | (uint32_t)(atomicAdd(&bins[j], poly.bits(g - fl) - (0x432ull << 52)) >> 52);
         }
     }
     __syncthreads();
@@ -271,7 +283,10 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
     uint32_t mine[PT], n = 0;
     unsigned long long m = 0;
 #pragma unroll
-    for (int i = 0; i < PT; i++) mine[i] = cnt[tid * PT + i], n += mine[i], m += mass[tid * PT + i];
+    for (int i = 0; i < PT; i++) {
+        const unsigned long long x = bins[tid * PT + i];
+        mine[i] = (uint32_t)(x >> 52), n += mine[i], m += x & 0xfffffffffffffull;
+    }
     const uint32_t upto = nmx_scan_wave(n);
     if (lane == 63) wave_cnt[wave] = upto;
     __syncthreads();
@@ -284,7 +299,7 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
     {
         uint32_t f = first;
 #pragma unroll
-        for (int i = 0; i < PT; i++) cnt[tid * PT + i] = f, f += mine[i];
+        for (int i = 0; i < PT; i++) first_s[tid * PT + i] = f, f += mine[i];
     }
     /* the two threads of a bin together */
     const uint32_t n2 = n + (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)n);
@@ -294,7 +309,7 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < SM_PER; u++)
-        if (at[u] != 0xffffffffu) perm[cnt[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)index(u);
+        if (at[u] != 0xffffffffu) perm[first_s[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)index(u);
     __syncthreads();
     uint2 *po = (uint2 *)out->perm;
     for (uint32_t i = tid; 4 * i < members; i += SM_T1) po[i] = ((const uint2 *)perm2)[i];

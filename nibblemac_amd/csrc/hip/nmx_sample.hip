@@ -117,17 +117,19 @@ struct BinPoly { /* the coefficients, in scalars: a lane's fma takes one from th
         const double k[8] = {M, M / 8, M / (2 * 0x1p6), M / (6 * 0x1p9), M / (24 * 0x1p12), M / (120 * 0x1p15),
                              M / (720 * 0x1p18), M / (5040 * 0x1p21)};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            c[i] = k[i];
+        for (int i = 0; i < 8; i++) { /* the same polynomial, in powers of fr */
+            double b = 0.0, w = 1.0; /* w: binomial(j, i) (-1/2)^(j - i) */
+#pragma unroll
+            for (int j = i; j < 8; j++) b += k[j] * w, w *= -0.5 * (j + 1) / (j + 1 - i);
+            c[i] = b;
             asm("" : "+s"(c[i]));
         }
     }
     /* the bits of 2^52 + the mass: 0x433 << 52 | mass */
     __device__ __forceinline__ unsigned long long bits(double fr) const {
-        const double x = fr - 0.5;
         double p = c[7];
 #pragma unroll
-        for (int i = 6; i >= 0; i--) p = __builtin_fma(p, x, c[i]);
+        for (int i = 6; i >= 0; i--) p = __builtin_fma(p, fr, c[i]);
         return (unsigned long long)__double_as_longlong(p + 0x1p52);
     }
     __device__ __forceinline__ unsigned long long at(double fr) const { return bits(fr) & 0xfffffffffffffull; }
@@ -265,16 +267,18 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
     for (int i = 0; i < SM_BINS * SM_COPY; i += SM_T1) bins[i + tid] = 0;
     __syncthreads();
     const double base = floor(grid_pos(mx, p.inv));
-    const int copy = lane & (SM_COPY - 1);
+    const uint32_t copy = (lane & (SM_COPY - 1)) * 8;
     const BinPoly poly;
-    uint32_t at[SM_PER]; /* bin copy << 16 | rank; all ones: no weight */
+    uint32_t at[SM_PER]; /* byte offset of a copy's word << 12 | rank in it; all ones: no weight */
 #pragma unroll
     for (int u = 0; u < SM_PER; u++) {
         at[u] = 0xffffffffu;
         const double g = grid_pos(v[u], p.inv), fl = floor(g), d = base - fl; /* inf for -inf */
         if (d < (double)SM_BINS) {
-            const uint32_t j = (uint32_t)(int)d * SM_COPY + copy;
-            at[u] = j << 16 | (uint32_t)(atomicAdd(&bins[j], poly.bits(g - fl) - (0x432ull << 52)) >> 52);
+            const uint32_t j = (uint32_t)(int)d * (SM_COPY * 8) + copy;
+            unsigned long long *w = (unsigned long long *)((char *)bins + j);
+            const unsigned long long old = atomicAdd(w, poly.bits(g - fl) - (0x432ull << 52));
+            at[u] = __builtin_amdgcn_alignbit(j, (uint32_t)(old >> 32), 20);
         }
     }
     __syncthreads();
@@ -309,7 +313,7 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < SM_PER; u++)
-        if (at[u] != 0xffffffffu) perm[first_s[at[u] >> 16] + (at[u] & 0xffffu)] = (uint16_t)index(u);
+        if (at[u] != 0xffffffffu) perm[*(const uint32_t *)((const char *)first_s + (at[u] >> 13)) + (at[u] & 0xfffu)] = (uint16_t)index(u);
     __syncthreads();
     uint2 *po = (uint2 *)out->perm;
     for (uint32_t i = tid; 4 * i < members; i += SM_T1) po[i] = ((const uint2 *)perm2)[i];

@@ -8,6 +8,8 @@
 
 namespace {
 
+constexpr int TC_ROWS = 8; /* rows of a thread on their way at once */
+
 struct Commit {
     int n;
     const int32_t *parent, *tok, *choice;
@@ -89,18 +91,23 @@ __global__ __launch_bounds__(256) void tree_commit_k(Commit a) {
     }
     b -= a.layers * a.conv_wgs;
     if (b < a.layers * a.log_wgs) { /* pending rows: the path's log rows */
-        const int l = b / a.log_wgs, w = b % a.log_wgs;
-        const float *lg = a.log + (size_t)l * a.cap * a.row;
-        float *pd = a.pend + (size_t)l * a.cap * a.row;
-        for (int x = w * 256 + tid; x < e * a.row; x += a.log_wgs * 256) {
-            const int i = x / a.row, k = x - i * a.row;
-            pd[x] = lg[(size_t)path[i] * a.row + k];
+        const int l = b / a.log_wgs, x = b % a.log_wgs * 256 + tid;
+        if (x >= a.row) return;
+        const float *lg = a.log + (size_t)l * a.cap * a.row + x;
+        float *pd = a.pend + (size_t)l * a.cap * a.row + x;
+        for (int i0 = 0; i0 < e; i0 += TC_ROWS) {
+            float v[TC_ROWS];
+#pragma unroll
+            for (int k = 0; k < TC_ROWS; k++) v[k] = lg[(size_t)path[i0 + k < e ? i0 + k : e - 1] * a.row];
+#pragma unroll
+            for (int k = 0; k < TC_ROWS; k++)
+                if (i0 + k < e) pd[(size_t)(i0 + k) * a.row] = v[k];
         }
         return;
     }
     b -= a.layers * a.log_wgs;
-    /* cache rows to consecutive slots. path[i] >= i and grows, so a thread that takes its own bytes of
-     * the rows in order reads each row before it writes one at or behind it. */
+    /* cache rows to consecutive slots. path[i] >= i and grows: no row is written before it is read where
+     * a thread takes its own bytes of the rows in order, or some rows' in order before any of theirs */
     const int cache = b / (a.nkv * a.kv_wgs), g = b / a.kv_wgs % a.nkv, w = b % a.kv_wgs;
     const long long p = (long long)*a.pos + a.pos_off;
     const int words = a.row_bytes / 4 + (a.scales ? 1 : 0), x = w * 256 + tid;
@@ -110,10 +117,20 @@ __global__ __launch_bounds__(256) void tree_commit_k(Commit a) {
     size_t step;
     if (x < a.row_bytes / 4) base = c + (size_t)g * a.max_ctx * a.row_bytes + 4 * x, step = a.row_bytes;
     else base = c + a.scale_at + (size_t)g * a.max_ctx * 4, step = 4;
-    for (int i = 1; i < e; i++) {
-        const long long from = p + path[i], to = p + i;
-        if (from == to || to < 0 || from >= a.max_ctx) continue;
-        *(uint32_t *)(base + (size_t)to * step) = *(const uint32_t *)(base + (size_t)from * step);
+    for (int i0 = 1; i0 < e; i0 += TC_ROWS) {
+        uint32_t v[TC_ROWS];
+#pragma unroll
+        for (int k = 0; k < TC_ROWS; k++) { /* a row outside the cache is not moved: any row inside stands for it */
+            const long long from = p + path[i0 + k < e ? i0 + k : e - 1];
+            v[k] = *(const uint32_t *)(base + (size_t)(from >= 0 && from < a.max_ctx ? from : 0) * step);
+        }
+#pragma unroll
+        for (int k = 0; k < TC_ROWS; k++) {
+            if (i0 + k >= e) continue;
+            const long long from = p + path[i0 + k], to = p + i0 + k;
+            if (from == to || to < 0 || from >= a.max_ctx) continue;
+            *(uint32_t *)(base + (size_t)to * step) = v[k];
+        }
     }
 }
 
@@ -152,7 +169,7 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p) {
         a.layers = p->layers, a.C = p->C, a.S = p->conv_k - 1;
         a.state = p->state, a.xin = p->xin, a.log = p->log, a.pend = p->pend, a.cap = p->cap, a.row = p->row;
         a.conv_wgs = a.S ? (p->C + 255) / 256 : 0;
-        a.log_wgs = (p->row + 1023) / 1024;
+        a.log_wgs = (p->row + 255) / 256;
     }
     if (p->caches) {
         if (p->caches < 0 || p->caches > NMX_TREE_KV_MAX || p->nkv < 1 || p->nkv > 1024 || p->max_ctx < 1 ||
@@ -160,6 +177,9 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p) {
             return nmx_fail(ctx, "nmx_tree_commit: bad caches %d nkv=%d max_ctx=%d hd=%d kv_dtype=%d", p->caches, p->nkv,
                             p->max_ctx, p->hd, p->kv_dtype);
         if (!p->kv || !p->pos) return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
+        if (nmx_overlap(p->out, ob, p->pos, 4) || (p->ctl && nmx_overlap(p->ctl + 1, 8, p->pos, 4)) ||
+            (p->vt && nmx_overlap(p->vt, 4, p->pos, 4)))
+            return nmx_fail(ctx, "nmx_tree_commit: pos overlaps an output");
         const size_t kb = nmx_kv_bytes(p->kv_dtype, p->nkv, p->max_ctx, p->hd);
         for (int i = 0; i < p->caches; i++) {
             if (!p->kv[i] || (uintptr_t)p->kv[i] % 4) return nmx_fail(ctx, "nmx_tree_commit: cache %d", i);

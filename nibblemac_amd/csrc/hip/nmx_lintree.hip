@@ -202,10 +202,12 @@ __device__ __forceinline__ void tree_tables(TreeTables<N> &s, int n, unsigned lo
     if (lane == 0) s.levels = deep + 1;
 }
 
-/* Rows of k and q for the products of nodes: as two binary16 parts each, which together hold 22 bits of
- * the row's largest element (k has norm 1, q norm qscale: brought to 2^6 first), so that a product of rows
- * is three 16-bit matrix instructions per 32 keys in place of 32 32-bit ones; the low-low part, 2^-22, is
- * left out. */
+/* Rows of k and q for the products of nodes: an element, brought to norm 2^12 (k has norm 1, q norm
+ * qscale), as its nearest whole number and the rest, both binary16. Products of whole numbers add up
+ * to no more than 2^24: exact in the accumulator, whose additions are not rounded to the nearest (their
+ * bias, 2^-23 of a sum, would be the largest error of o where q.k nearly cancels). The products of a
+ * whole number and a rest are 2^-12 of that and have an accumulator of their own; those of two rests,
+ * random and 2^-24, are left out. Three 16-bit instructions per 32 keys in place of 32 32-bit ones. */
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
@@ -215,10 +217,10 @@ __device__ __forceinline__ void split4(float4 x, float up, _Float16 *hi, _Float1
     const float v[4] = {x.x * up, x.y * up, x.z * up, x.w * up};
     half4 h, l;
 #pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = (_Float16)v[i], l[i] = (_Float16)(v[i] - (float)h[i]);
+    for (int i = 0; i < 4; i++) h[i] = (_Float16)rintf(v[i]), l[i] = (_Float16)(v[i] - (float)h[i]);
     *(half4 *)hi = h, *(half4 *)lo = l;
 }
-constexpr float TR_UP = 64.0f;
+constexpr float TR_UP = 4096.0f;
 
 /* The pending rows of head h, TR_B at a time: keys and decays to LDS (pk, pdec), the deltas of column
  * col to registers. The first batch is requested at the kernel's entry, among its other requests. */
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
             const int U = job, an = 16 * U + c;
             const _Float16 *ar = kh2 + an * HS + 8 * gq, *tr = kh2 + (16 * X + c) * HS + 8 * gq, *ur = qh2 + (16 * X + c) * HS + 8 * gq;
             const int lo = n16 * HS;
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x, xr = x, yr = x;
 #pragma unroll
             for (int k = 0; k < DK; k += 32) {
                 const half8 ah = *(const half8 *)(ar + k), al = *(const half8 *)(ar + lo + k);
@@ -368,13 +370,14 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const float v = src[i] * q_up;
-                        uh[i] = (_Float16)v, ul[i] = (_Float16)(v - (float)uh[i]);
+                        uh[i] = (_Float16)rintf(v), ul[i] = (_Float16)(v - (float)uh[i]);
                     }
                 }
                 x = mfma16(th, ah, x), y = mfma16(uh, ah, y);
-                x = mfma16(tl, ah, x), y = mfma16(ul, ah, y);
-                x = mfma16(th, al, x), y = mfma16(uh, al, y);
+                xr = mfma16(tl, ah, xr), yr = mfma16(ul, ah, yr);
+                xr = mfma16(th, al, xr), yr = mfma16(uh, al, yr);
             }
+            x += xr, y += yr;
             const int dp = tt.depth[an];
 #pragma unroll
             for (int j = 0; j < 4; j++) {

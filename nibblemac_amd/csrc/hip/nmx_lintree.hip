@@ -341,14 +341,15 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
         for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
     }
     /* S^T k and S^T q of the wave's nodes: element j is node 16 T + 4 gq + j, column c */
-    f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
+    f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk, sk2 = sk, sq2 = sk; /* two chains each: shorter ones round less */
 #pragma unroll
     for (int k = 0; k < NS; k++) {
         sk = mfma4(kf[k].x, s[k].x, sk), sq = mfma4(qf[k].x, s[k].x, sq);
-        sk = mfma4(kf[k].y, s[k].y, sk), sq = mfma4(qf[k].y, s[k].y, sq);
+        sk2 = mfma4(kf[k].y, s[k].y, sk2), sq2 = mfma4(qf[k].y, s[k].y, sq2);
         sk = mfma4(kf[k].z, s[k].z, sk), sq = mfma4(qf[k].z, s[k].z, sq);
-        sk = mfma4(kf[k].w, s[k].w, sk), sq = mfma4(qf[k].w, s[k].w, sq);
+        sk2 = mfma4(kf[k].w, s[k].w, sk2), sq2 = mfma4(qf[k].w, s[k].w, sq2);
     }
+    sk += sk2, sq += sq2;
     nmx_lds_sync(); /* the rows, the tables; the pending keys have been read */
     /* D(t, a) (k_t . k_a) and D(t, a) (q_t . k_a): the tiles (t, a) on and below the diagonal, in turn */
     for (int job = nodes ? T : waves * waves, X = 0; X < waves; job -= X + 1, X++) {

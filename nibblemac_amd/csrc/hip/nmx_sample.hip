@@ -33,7 +33,7 @@ static_assert(2 * SM_BINS == SM_T1, "two threads of sample_scan_k to a bin");
 constexpr int SM_MAXC = (1 << 20) / SM_CHUNK; /* chunks of the longest row */
 constexpr int SM_LIST = 16384; /* members of a bin kept in LDS; a bin with more is read again */
 constexpr int SM_RANK = 256;   /* members of a bin ranked by comparing all with all */
-constexpr int SM_FEW = 512;    /* tokens among which a row is decided in LDS altogether */
+constexpr int SM_FEW = SM_T2;  /* tokens among which a row is decided one to a thread */
 constexpr int SM_DIGIT = SM_T2; /* values of a selection's digit */
 static_assert(SM_SLICE == SM_T2, "a wave's slice of a chunk is one logit a thread of sample_pick_k");
 
@@ -341,10 +341,7 @@ struct Pick {
             uint32_t digit[SM_DIGIT], small[SM_RANK], part_n[3][SM_BINS];
             uint32_t list[SM_LIST];
         };
-        struct {
-            unsigned long long order[SM_FEW], w[SM_FEW]; /* greater order: earlier in the sorted row */
-            uint32_t index[SM_FEW];
-        } few;
+        unsigned long long few[SM_FEW];
     };
 };
 
@@ -515,72 +512,142 @@ __device__ uint32_t min_p_key(float mx, double inv, double min_p) {
     return k;
 }
 
-/* A row whose kept tokens are among the S.seg[C] <= SM_FEW in hand: all of it in LDS, by comparing all
- * with all (two lanes to a token, each half of the others). Masses are in 2^-52 of the largest weight.
- * whole: the mass that top-p counts against where there is no top-k. */
-__device__ void pick_few(Pick &S, const Row &r, const Par &p, float mx, double whole, double ud, int32_t *tok, float *prob) {
-    const int tid = threadIdx.x, i = tid >> 1, half = tid & 1;
-    const uint32_t N = S.seg[r.C];
-    float x = -INFINITY;
-    uint32_t index = 0;
-    if ((uint32_t)i < N) {
+/* A step of a bitonic network: this lane and lane ^ J, the greater with the lower one where up holds. J < 16
+ * goes without LDS. */
+template <int CTRL>
+__device__ __forceinline__ unsigned long long dpp64(unsigned long long v) {
+    return (unsigned long long)(uint32_t)nmx_dpp<CTRL>((int)(v >> 32)) << 32 | (uint32_t)nmx_dpp<CTRL>((int)v);
+}
+template <int J>
+__device__ __forceinline__ void sort_step(unsigned long long &v, bool up) {
+    unsigned long long o;
+    if constexpr (J == 1) o = dpp64<NMX_DPP_XOR1>(v);
+    else if constexpr (J == 2) o = dpp64<NMX_DPP_XOR2>(v);
+    else if constexpr (J == 4) o = dpp64<NMX_DPP_HALF_MIRROR>(dpp64<0x1B>(v)); /* lane ^ 3, then ^ 7 */
+    else if constexpr (J == 8) o = dpp64<0x128>(v);                            /* row_ror:8 */
+    else o = __shfl_xor(v, J);
+    const bool low = (threadIdx.x & J) == 0;
+    if ((o > v) == (low == up)) v = o;
+}
+__device__ __forceinline__ unsigned long long readlane64(unsigned long long v, int l) {
+    return (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
+
+/* The threads' values below P (a power of two from 64 on) in descending order, thread 0's the largest: a bitonic
+ * network, in a wave by shuffles, across waves through buf. Threads from P on keep what they have. */
+__device__ unsigned long long sort_down(unsigned long long v, int P, unsigned long long *buf) {
+    const int tid = threadIdx.x;
+    const bool in = tid < P;
+    for (int k = 2; k <= P; k <<= 1) {
+        for (int j = k >> 1; j >= 64; j >>= 1) {
+            __syncthreads();
+            if (in) buf[tid] = v;
+            __syncthreads();
+            const unsigned long long o = buf[in ? tid ^ j : 0];
+            if (in && (o > v) == (((tid & j) == 0) == ((tid & k) == 0))) v = o;
+        }
+        if ((tid & ~63) >= P) continue; /* a wave without values */
+        const bool up = (tid & k) == 0;
+        if (k >= 64) sort_step<32>(v, up);
+        if (k >= 32) sort_step<16>(v, up);
+        if (k >= 16) sort_step<8>(v, up);
+        if (k >= 8) sort_step<4>(v, up);
+        if (k >= 4) sort_step<2>(v, up);
+        sort_step<1>(v, up);
+    }
+    return v;
+}
+
+/* pick_few for up to 64 tokens: the first wave's lanes, each compared with all through scalars. */
+__device__ void pick_wave(const Pick &S, const Row &r, const Par &p, float mx, double whole, double ud, int32_t *tok, float *prob) {
+    const int i = threadIdx.x, N = (int)S.seg[r.C];
+    if (i >= 64) return;
+    unsigned long long v = 0;
+    double w = 0.0;
+    uint32_t index = 0xffffffffu;
+    if (i < N) {
         int c, at;
-        x = member(S, r, i, &c, &at);
+        const float x = member(S, r, i, &c, &at);
         index = (uint32_t)(c * SM_CHUNK + at);
+        v = (unsigned long long)sample_key(x) << 32 | ~index;
+        w = weight(x, mx, r.inv);
     }
-    const double wd = (uint32_t)i < N ? weight(x, mx, r.inv) : 0.0;
-    const unsigned long long mine = (unsigned long long)(wd * 0x1p52 + 0.5), ord = (unsigned long long)sample_key(x) << 32 | ~index;
-    __syncthreads();
-    if (half == 0) S.few.order[i] = (uint32_t)i < N ? ord : 0, S.few.w[i] = mine, S.few.index[i] = (uint32_t)i < N ? index : 0xffffffffu;
-    __syncthreads();
-    uint32_t rank = 0;
-    unsigned long long before = 0;
-    const uint32_t n2 = (N + 1) / 2;
-#pragma unroll 8
-    for (uint32_t k = 0; k < n2; k++) {
-        const uint32_t j = 2 * k + half; /* j = N has no order */
-        if (S.few.order[j] > ord) rank++, before += S.few.w[j];
+    unsigned long long mine = (unsigned long long)(w * 0x1p52 + 0.5), before = 0;
+    int rank = 0;
+    for (int j = 0; j < N; j++) {
+        const unsigned long long o = readlane64(v, j), m = readlane64(mine, j);
+        if (o > v) rank++, before += m;
     }
-    rank += (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)rank);
-    before += (unsigned long long)(uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)(before >> 32)) << 32 |
-              (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)before);
-    bool keep = (uint32_t)i < N && wd > 0.0;
+    bool keep = i < N && w > 0.0;
     if (p.top_k) {
-        const uint32_t k = (uint32_t)p.top_k < N ? (uint32_t)p.top_k : N;
-        if (rank == k - 1 && (uint32_t)i < N && half == 0) S.sel_m = before + mine;
-        __syncthreads();
-        whole = (double)S.sel_m;
+        const int k = p.top_k < N ? p.top_k : N;
+        whole = (double)readlane64(before + mine, __ffsll((long long)__ballot(i < N && rank == k - 1)) - 1);
         keep = keep && rank < k;
     } else {
         whole *= 0x1p52;
     }
     if (p.top_p < 1.0) keep = keep && (rank == 0 || (double)before < p.top_p * whole);
-    if (p.min_p > 0.0) keep = keep && wd >= p.min_p;
-    __syncthreads(); /* the masses have been read */
-    if (half == 0) S.few.w[i] = keep ? mine : 0;
-    __syncthreads();
-    unsigned long long upto = 0, all = 0;
+    if (p.min_p > 0.0) keep = keep && w >= p.min_p;
+    mine = keep ? mine : 0;
+    unsigned long long upto = mine, all = 0;
     uint32_t last = 0;
-#pragma unroll 8
-    for (uint32_t k = 0; k < n2; k++) {
-        const uint32_t j = 2 * k + half;
-        const unsigned long long w = j < N ? S.few.w[j] : 0;
-        all += w;
-        if (S.few.index[j] < index) upto += w;
-        if (w && S.few.index[j] >= last) last = S.few.index[j];
+    for (int j = 0; j < N; j++) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)index, j);
+        const unsigned long long m = readlane64(mine, j);
+        all += m;
+        if (o < index) upto += m;
+        last = m && o > last ? o : last;
     }
-    auto other = [&](unsigned long long v) {
-        return (unsigned long long)(uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)(v >> 32)) << 32 | (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)v);
-    };
-    all += other(all), upto += other(upto);
-    const uint32_t lo = (uint32_t)nmx_dpp<NMX_DPP_XOR1>((int)last);
-    last = lo > last ? lo : last;
+    const double goal = ud * (double)all;
+    const bool hit = goal < (double)all ? (double)(upto - mine) <= goal && (double)upto > goal : index == last;
+    if (keep && hit) {
+        tok[blockIdx.x] = (int)index;
+        if (prob) prob[blockIdx.x] = (float)(w / ((double)all * 0x1p-52));
+    }
+}
+
+/* A row whose kept tokens are among the S.seg[C] <= SM_FEW in hand, one to a thread: sorted by order for
+ * the filters, then what they keep by index for the draw. Masses are in 2^-52 of the largest weight.
+ * whole: the mass that top-p counts against where there is no top-k. */
+__device__ void pick_few(Pick &S, const Row &r, const Par &p, float mx, double whole, double ud, int32_t *tok, float *prob) {
+    const int tid = threadIdx.x, N = (int)S.seg[r.C]; /* > 64 */
+    const int P = 1 << (32 - __clz(N - 1));
+    unsigned long long v = 0; /* greater: earlier in the sorted row */
+    if (tid < N) {
+        int c, at;
+        const float x = member(S, r, tid, &c, &at);
+        v = (unsigned long long)sample_key(x) << 32 | ~(uint32_t)(c * SM_CHUNK + at);
+    }
+    auto mass_of = [&](double w) { return (unsigned long long)(w * 0x1p52 + 0.5); };
+    v = sort_down(v, P, S.few);
+    const uint32_t key = (uint32_t)(v >> 32);
+    double w = tid < N ? weight(sample_unkey(key), mx, r.inv) : 0.0;
+    unsigned long long mine = mass_of(w), all;
+    const unsigned long long before = block_scan(mine, S.red1, &all) - mine;
+    bool keep = tid < N && w > 0.0;
+    if (p.top_k) {
+        const int k = p.top_k < N ? p.top_k : N;
+        if (tid == k - 1) S.sel_m = before + mine;
+        __syncthreads();
+        whole = (double)S.sel_m;
+        keep = keep && tid < k;
+    } else {
+        whole *= 0x1p52;
+    }
+    if (p.top_p < 1.0) keep = keep && (tid == 0 || (double)before < p.top_p * whole);
+    if (p.min_p > 0.0) keep = keep && w >= p.min_p;
+    v = sort_down(keep ? v << 32 | key : 0, P, S.few); /* the kept ones by index: ~index on top */
+    const bool kept = v != 0;
+    w = kept ? weight(sample_unkey((uint32_t)v), mx, r.inv) : 0.0, mine = mass_of(w);
+    const unsigned long long upto = block_scan(mine, S.red2, &all);
     const double goal = ud * (double)all;
     /* the token whose share of the running mass holds the goal; past the whole the last one */
-    const bool hit = goal < (double)all ? (double)upto <= goal && (double)(upto + mine) > goal : index == last;
-    if (keep && hit && half == 0) {
-        tok[blockIdx.x] = (int)index;
-        if (prob) prob[blockIdx.x] = (float)(wd / ((double)all * 0x1p-52));
+    int hit, last;
+    block_find(kept && (double)upto > goal, kept, S.red1, S.red2, &hit, &last);
+    if (tid == (hit < SM_T2 ? hit : last)) {
+        tok[blockIdx.x] = (int)~(uint32_t)(v >> 32);
+        if (prob) prob[blockIdx.x] = (float)(w / ((double)all * 0x1p-52));
     }
 }
 
@@ -688,7 +755,8 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
                 Par q = p;
                 if (!by_k) q.top_k = 0;
                 take_bins(S, r, 0, reach);
-                pick_few(S, r, q, mx, m_all * unit, ud, tok, prob);
+                if (S.seg[C] <= 64) pick_wave(S, r, q, mx, m_all * unit, ud, tok, prob);
+                else pick_few(S, r, q, mx, m_all * unit, ud, tok, prob);
                 return;
             }
         }

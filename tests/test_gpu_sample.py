@@ -128,6 +128,37 @@ def test_ties_and_ranges(dev, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ties", [False, True])
+def test_few_and_more_tokens(dev, ties):
+    """Prefixes about the sizes at which a row is decided by one wave, by one workgroup's threads, and
+    by its bins: by count, by mass and by border, over one chunk and over three."""
+    print(f"[case] sample few tokens ties={ties}", flush=True)
+    rng = np.random.default_rng(11 + ties)
+    ks = [2, 33, 63, 64, 65, 127, 128, 129, 255, 256, 500, 511, 512, 513, 1000, 1023, 1024, 1025, 2000]
+    for vocab in (2777, 2 * CHUNK + 300):
+        par = np.concatenate([records(1, **f) for k in ks for f in (dict(top_k=k), dict(top_k=k, top_p=0.97),
+                                                                   dict(top_k=k, min_p=0.003, T=1.5))] +
+                             [records(1, top_p=p, T=t) for p in (0.3, 0.6, 0.8, 0.9, 0.95, 0.99) for t in (0.5, 1.0, 2.0)] +
+                             [records(1, min_p=m, T=t) for m in (0.3, 0.03, 0.003) for t in (0.5, 1.0, 2.0)])
+        l = (rng.standard_normal((len(par), vocab)) * 2.5).astype(np.float32)
+        if ties:
+            l = np.round(l * 8) / 8
+        u = rng.random(len(par), np.float32)
+        u[::7] = 0.0
+        u[3::7] = 1.0 - 2.0 ** -24
+        check(dev, l.astype(np.float32), par, u)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, vocab", [(4096, 33), (3, 1 << 20)])
+def test_largest_sizes(dev, n, vocab):
+    print(f"[case] sample {n} x {vocab}", flush=True)
+    rng = np.random.default_rng(vocab)
+    par = np.concatenate([records(1, **FILTERS[r % len(FILTERS)]) for r in range(n)])
+    check(dev, rows(rng, n, vocab, peaks=4), par, rng.random(n, np.float32), stride=vocab + 1)
+
+
+@pytest.mark.gpu
 def test_masked_values(dev):
     """-inf, NaN, +inf and the lowest finite value as masks; rows that nothing is left of."""
     print("[case] sample masks", flush=True)

@@ -43,7 +43,7 @@ struct TreeAttn {
     float *part;   /* [splits][n nh][hd] weighted values, 2^12 high */
     float4 *stat;  /* [splits][n nh]: maximum of the scores, the values' exponent (columns below 256),
                     * sum, the values' exponent (columns from 256) */
-    int splits, unit; /* a part is a whole number of units of positions */
+    int splits; /* a part is a whole number of tiles */
     int jcols;        /* columns of a join's workgroup: hd over a divisor of hd / 64 */
     float *o;
     int8_t *aq;
@@ -61,7 +61,7 @@ __device__ __forceinline__ int ctx_len(const TreeAttn &a) {
 }
 __device__ __forceinline__ int part_len(const TreeAttn &a, int len) {
     const int per = (len + a.splits - 1) / a.splits;
-    return (per + a.unit - 1) / a.unit * a.unit;
+    return (per + AT_P - 1) / AT_P * AT_P;
 }
 
 /* Exponent e with |x| < 2^e for the largest |x| of a row (0 for a row of zeros), clamped so that
@@ -198,14 +198,16 @@ __device__ __forceinline__ float amax8(const Raw8<KV_F32> &r) {
     return fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))),
                  fmaxf(fmaxf(fabsf(x[4]), fabsf(x[5])), fmaxf(fabsf(x[6]), fabsf(x[7]))));
 }
-/* x up as a binary16 and the binary16 rest */
+/* x as a binary16 (towards zero, two at a time: the rest is exact either way) and the binary16 rest */
+typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void split2(float a, float b, half8 &h, half8 &r, int i) {
+    const fp16x2 p = __builtin_amdgcn_cvt_pkrtz(a, b);
+    h[i] = (_Float16)p.x, h[i + 1] = (_Float16)p.y;
+    r[i] = (_Float16)__builtin_fmaf((float)h[i], -1.0f, a), r[i + 1] = (_Float16)__builtin_fmaf((float)h[i + 1], -1.0f, b);
+}
 __device__ __forceinline__ void split8(const float (&x)[8], float up, half8 &h, half8 &r) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float v = x[i] * up;
-        h[i] = (_Float16)v;
-        r[i] = (_Float16)(v - (float)h[i]);
-    }
+    for (int i = 0; i < 8; i += 2) split2(x[i] * up, x[i + 1] * up, h, r, i);
 }
 
 /* Lane c of 16 (quarter gq) takes its query row's chunks 4 k + gq: requested first, split when the
@@ -300,16 +302,16 @@ __device__ __forceinline__ void add_tile(Running<OD / 16> &r, const float (&x)[8
         r.m = mx, r.ve = ve;
     }
     half8 ph, pl;
+    float wv[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const float w = __builtin_amdgcn_exp2f(x[i] - ref);
         r.l += w;
-        float v;
-        if constexpr (KVT == KV_F16) v = w * 4096.0f;
-        else v = ldexpf(w * f[i], e[i] - ve + 12);
-        ph[i] = (_Float16)v;
-        pl[i] = (_Float16)(v - (float)ph[i]);
+        if constexpr (KVT == KV_F16) wv[i] = w * 4096.0f;
+        else wv[i] = ldexpf(w * f[i], e[i] - ve + 12);
     }
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) split2(wv[i], wv[i + 1], ph, pl, i);
 #pragma unroll
     for (int d = 0; d < DT; d++) {
         /* values of column c of the tile's 16, positions in the weights' order */
@@ -351,9 +353,13 @@ constexpr int ctx_waves() {
     return HDP > 256 ? 4 : 8;
 }
 template <int HDP, int KVT>
+constexpr int ctx_bufs() {
+    return HDP > 256 && KVT == KV_F32 ? 1 : 2;
+}
+template <int HDP, int KVT>
 __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAttn a) {
     constexpr int TH = 64 * ctx_waves<HDP>();
-    constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32, DT = OD / 16, NB = HDP > 256 ? 1 : 2;
+    constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32, DT = OD / 16, NB = ctx_bufs<HDP, KVT>();
     constexpr int PL = KVT == KV_F32 ? 2 : 1; /* planes */
     constexpr int KC = HDP / 8, VC = OD / 8;  /* lanes that stage a row, 8 columns each */
     constexpr int KU = AT_P * KC / TH ? AT_P * KC / TH : 1, VU = AT_P * VC / TH ? AT_P * VC / TH : 1;
@@ -512,251 +518,6 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
     if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);
 }
 
-/* Few rows: the time is that of the cache's bytes, so each of 4 waves takes positions of its own, the
- * keys straight into matrix operands, the values through a piece of LDS of its own (a binary16 cache's
- * without a register between), all of a tile requested together and before the query rows have come;
- * the split query rows are the waves' common operand in LDS. Two workgroups to a CU keep the requests
- * coming (80 KB of LDS each up to 256 columns; an fp32 cache's has a CU for itself). The waves' results
- * are joined at the end. */
-template <int HDP, int KVT>
-constexpr int few_lds() {
-    return 4 * (KVT == KV_F32 ? 2 : 1) * AT_P * (HDP > 256 ? 256 : HDP) * 2 /* values */ + 2 * 16 * HDP * 2 /* query rows */ +
-           (KVT == KV_F32 ? 4 * 2 * AT_P * 4 : 0) /* the values' exponents and fractions */;
-}
-template <int HDP, int KVT>
-__global__ __launch_bounds__(256, (few_lds<HDP, KVT>() <= 80 * 1024 ? 2 : 1)) void attn_tree_few_k(TreeAttn a) {
-    constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32, DT = OD / 16;
-    constexpr int PL = KVT == KV_F32 ? 2 : 1, VC = OD / 8, VR = 64 / VC; /* rows of a wave's request */
-    constexpr int VU = AT_P / VR;
-    extern __shared__ uint4 smem[];
-    const int lane = lane_id(), wave = wave_id(), c = lane & 15, gq = lane >> 4;
-    _Float16 *tv = (_Float16 *)smem + wave * PL * AT_P * OD, *tq = (_Float16 *)smem + 4 * PL * AT_P * OD;
-    float *vf = (float *)(tq + 2 * 16 * HDP) + wave * 2 * AT_P; /* fp32 */
-    int *ve = (int *)(vf + AT_P);
-    const int s = blockIdx.x % a.splits, g = blockIdx.x / a.splits % a.nkv, mt = blockIdx.x / a.splits / a.nkv;
-    const int d0 = blockIdx.y * OD, hd = a.hd, rep = a.nh / a.nkv, rows = a.n * rep;
-    auto head_row = [&](int row) { return row < rows ? (row / rep) * a.nh + g * rep + row % rep : -1; }; /* (node, head) */
-    /* the query rows: 16 lanes each, chunks of 8 columns */
-    const int qr = 4 * wave + gq, qrow = head_row(mt * 16 + qr);
-    constexpr int QU = HDP > 128 ? HDP / 128 : 1;
-    const float *qp = a.q + (size_t)(qrow < 0 ? 0 : qrow) * 2 * hd;
-    float4 qx[QU][2];
-#pragma unroll
-    for (int u = 0; u < QU; u++) {
-        const int col = (16 * u + c) * 8, at = col < hd ? col : 0;
-        qx[u][0] = *(const float4 *)(qp + at), qx[u][1] = *(const float4 *)(qp + at + 4);
-    }
-    const Head<KVT> kh(a, a.kc, g), vh(a, a.vc, g);
-    const int len = ctx_len(a), per = part_len(a, len);
-    if (per == 0 || s * per >= len) return;
-    /* a quarter of the part for each wave */
-    const int w0 = s * per + wave * (per >> 2);
-    const int p1 = w0 + (per >> 2) < len ? w0 + (per >> 2) : len;
-    /* rows and columns past the end repeat ones inside (finite, and their weight is 0) */
-    auto row_at = [&](int p) { return p < p1 ? p : p1 - 1; };
-    Raw8<KVT> rk[2][KS], rv[VU];
-    float ks[2], vs[2]; /* int8: the scales of positions c and 16 + c */
-    auto ask = [&](int pt) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int p = row_at(pt + 16 * i + c);
-            ks[i] = kh.scale(p), vs[i] = vh.scale(p);
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const int col = 32 * k + 8 * gq;
-                rk[i][k] = kh.load8(p, col < hd ? col : 0);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < VU; u++) {
-            const int p = u * VR + lane / VC, ch = lane % VC;
-            if constexpr (KVT == KV_F16) { /* chunk ch of the LDS row is the row's chunk ch ^ ... */
-                const int col = d0 + ((ch ^ ((p & 3) << 1)) << 3);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)(uintptr_t)vh.at(row_at(pt + p), col < hd ? col : 0),
-                                                 (__attribute__((address_space(3))) uint32_t *)(uintptr_t)(tv + u * VR * OD), 16, 0, 0);
-            } else {
-                const int col = d0 + ch * 8;
-                rv[u] = vh.load8(row_at(pt + p), col < hd ? col : 0);
-            }
-        }
-    };
-    auto put_v = [&]() {
-#pragma unroll
-        for (int u = 0; u < VU; u++) {
-            const int p = u * VR + lane / VC, ch = lane % VC, at = v_at<OD>(p, ch);
-            if constexpr (KVT == KV_I8) {
-                *(half8 *)(tv + at) = codes8(rv[u].a);
-            } else if constexpr (KVT == KV_F32) {
-                float am = amax8(rv[u]), x[8];
-#pragma unroll
-                for (int w = 1; w < VC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
-                const int e = row_exp(am);
-                half8 h, y;
-                floats8(rv[u], x);
-                split8(x, pow2f(12 - e), h, y);
-                *(half8 *)(tv + at) = h;
-                *(half8 *)(tv + AT_P * OD + at) = y;
-                if (ch == 0) ve[p] = e - 12, vf[p] = 1.0f;
-            }
-        }
-    };
-    if (w0 < p1) ask(w0); /* on its way while the query rows are split */
-    float qfac;
-    {
-        float am = 0.0f;
-        auto in = [&](int u) { return qrow >= 0 && (16 * u + c) * 8 < hd; };
-#pragma unroll
-        for (int u = 0; u < QU; u++) {
-            float4(&y)[2] = qx[u];
-            const float b = fmaxf(fmaxf(fmaxf(fabsf(y[0].x), fabsf(y[0].y)), fmaxf(fabsf(y[0].z), fabsf(y[0].w))),
-                                  fmaxf(fmaxf(fabsf(y[1].x), fabsf(y[1].y)), fmaxf(fabsf(y[1].z), fabsf(y[1].w))));
-            am = fmaxf(am, in(u) ? b : 0.0f);
-        }
-#pragma unroll
-        for (int w = 1; w < 16; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
-        const int e = row_exp(am);
-        const float up = pow2f(12 - e);
-        /* the rows' factors go round through the place of their parts */
-        float *fac = (float *)tq;
-        if (c == 0) fac[qr] = pow2f(e - 12) * (a.scale * AT_LOG2E);
-        nmx_lds_sync();
-        qfac = fac[c];
-        nmx_lds_sync();
-#pragma unroll
-        for (int u = 0; u < QU; u++) {
-            float4(&y)[2] = qx[u];
-            const float z[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
-            half8 h, r;
-            split8(z, up, h, r);
-            if (!in(u)) h = r = half8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (HDP >= 128 || c * 8 < HDP) {
-                const int at = k_at<HDP>(qr, 16 * u + c);
-                *(half8 *)(tq + at) = h;
-                *(half8 *)(tq + 16 * HDP + at) = r;
-            }
-        }
-        nmx_lds_sync();
-    }
-    Running<DT> r;
-    const int vp = 4 * gq + (c >> 2);
-    const _Float16 *vb[4], *qb[2];
-#pragma unroll
-    for (int i = 0; i < 4; i++) vb[i] = tv + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
-#pragma unroll
-    for (int i = 0; i < 2; i++) qb[i] = tq + k_at<HDP>(c, 4 * i + gq) - 32 * i;
-    for (int pt = w0; pt < p1; pt += AT_P) {
-        if (pt != w0) {
-            nmx_lds_wave_sync(); /* the last tile's values have been read */
-            ask(pt);
-        }
-        /* scores: positions 16 i + 4 gq + j against row c */
-        float4v sc[2];
-        float kfac[2], up[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f}, kfac[i] = ks[i], up[i] = 1.0f;
-            if constexpr (KVT == KV_F32) {
-                float am = amax8(rk[i][0]);
-#pragma unroll
-                for (int k = 1; k < KS; k++) am = fmaxf(am, amax8(rk[i][k]));
-                am = fmaxf(am, __shfl_xor(am, 16));
-                am = fmaxf(am, __shfl_xor(am, 32));
-                const int e = row_exp(am);
-                up[i] = pow2f(12 - e), kfac[i] = pow2f(e - 12);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const half8 qh = *(const half8 *)(qb[k & 1] + 32 * k), ql = *(const half8 *)(qb[k & 1] + 16 * HDP + 32 * k);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                half8 x, y;
-                if constexpr (KVT == KV_F16) {
-                    x = __builtin_bit_cast(half8, rk[i][k].a);
-                } else if constexpr (KVT == KV_I8) {
-                    x = codes8(rk[i][k].a);
-                } else {
-                    float z[8];
-                    floats8(rk[i][k], z);
-                    split8(z, up[i], x, y);
-                }
-                sc[i] = mfma16(x, qh, sc[i]);
-                sc[i] = mfma16(x, ql, sc[i]);
-                if constexpr (KVT == KV_F32) sc[i] = mfma16(y, qh, sc[i]);
-            }
-        }
-        if constexpr (KVT == KV_F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* the values are in LDS */
-        else put_v();
-        nmx_lds_wave_sync();
-        float x[8], f[8];
-        int e[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int j = 4 * gq + (i & 3), p = 16 * (i >> 2) + j;
-            float y = sc[i >> 2][i & 3] * qfac;
-            if constexpr (KVT != KV_F16) y *= __shfl(kfac[i >> 2], j); /* a position's number is with lane j */
-            if constexpr (KVT == KV_I8) {
-                const float v = __shfl(vs[i >> 2], j);
-                e[i] = row_exp(v), f[i] = v * pow2f(-e[i]);
-            } else if constexpr (KVT == KV_F32) {
-                e[i] = ve[p], f[i] = vf[p];
-            } else {
-                e[i] = 0, f[i] = 1.0f;
-            }
-            x[i] = pt + p < p1 ? y : -INFINITY;
-        }
-        add_tile<OD, KVT>(r, x, e, f, vb, AT_P * OD);
-    }
-    /* the waves' results joined, a wave taking a quarter of the columns of all four */
-    constexpr int XW = 64 * DT, QD = DT / 4;
-    float4v *xo = (float4v *)smem + lane;
-    float4 *xs = (float4 *)((float4v *)smem + 4 * XW) + c;
-    r.l += __shfl_xor(r.l, 16);
-    r.l += __shfl_xor(r.l, 32);
-    __syncthreads();
-#pragma unroll
-    for (int d = 0; d < DT; d++) xo[wave * XW + d * 64] = r.o[d];
-    if (gq == 0) xs[wave * 16] = make_float4(r.m, (float)r.ve, r.l, 0.0f);
-    __syncthreads();
-    float4 st[4];
-    float m = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; w++) st[w] = xs[w * 16], m = fmaxf(m, st[w].x);
-    const float ref = m == -INFINITY ? 0.0f : m;
-    /* exponents count from a wave's own maximum: the common one covers them all */
-    float top = -500.0f, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) top = fmaxf(top, (st[w].x - ref) + st[w].y);
-    const int vn = KVT == KV_F16 ? 0 : (int)ceilf(top);
-    float4v o[QD];
-#pragma unroll
-    for (int d = 0; d < QD; d++) o[d] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float f = __builtin_amdgcn_exp2f(st[w].x - ref), up = st[w].y - (float)vn;
-        const float fv = KVT == KV_F16 ? f : ldexpf(f, up < -300.0f ? -300 : (int)up);
-        l += st[w].z * f;
-#pragma unroll
-        for (int d = 0; d < QD; d++) {
-            const float4v y = xo[w * XW + (QD * wave + d) * 64];
-#pragma unroll
-            for (int j = 0; j < 4; j++) o[d][j] = __builtin_fmaf(y[j], fv, o[d][j]);
-        }
-    }
-    const int hrow = head_row(mt * 16 + c);
-    if (hrow < 0) return;
-    const size_t at = (size_t)s * a.n * a.nh + hrow;
-#pragma unroll
-    for (int d = 0; d < QD; d++) {
-        const int col = d0 + 16 * (QD * wave + d) + 4 * gq;
-        if (col < hd) *(float4v *)(a.part + at * hd + col) = o[d];
-    }
-    if (wave == 0 && gq == 0) {
-        if (d0) a.stat[at].w = (float)vn;
-        else a.stat[at].x = m, a.stat[at].y = (float)vn, a.stat[at].z = l;
-    }
-}
-
 /* ---- the node's ancestors, and the join ---------------------------------------------------- */
 constexpr int JT = 512; /* threads of a join */
 
@@ -881,23 +642,20 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
 
 /* How the context is divided among workgroups. */
 struct Plan {
-    int hdp, mtiles, splits, unit, halves, jcols;
-    bool few; /* attn_tree_few_k, else attn_tree_ctx_k */
+    int hdp, mtiles, splits, halves, jcols;
     size_t part_bytes, bytes;
 };
 
-Plan make_plan(int n, int nh, int nkv, int hd, int kv_dtype) {
+Plan make_plan(int n, int nh, int nkv, int hd) {
     Plan p;
     p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
     const int tiles = (n * (nh / nkv) + 15) / 16, od = p.hdp > 256 ? 256 : p.hdp;
-    p.few = tiles <= 2 && !(p.hdp > 256 && kv_dtype == KV_F32); /* too many registers */
     const int waves = p.hdp > 256 ? 4 : 8;
-    p.mtiles = p.few ? tiles : (tiles + waves - 1) / waves;
+    p.mtiles = (tiles + waves - 1) / waves;
     p.halves = p.hdp / od;
-    /* the many-row kernel has a CU for itself; of the other's workgroups two share one */
-    const int s = (p.few ? 512 : 256) / (nkv * p.mtiles * p.halves);
+    /* a workgroup to a CU */
+    const int s = 256 / (nkv * p.mtiles * p.halves);
     p.splits = s < 1 ? 1 : s > AT_MAXS ? AT_MAXS : s;
-    p.unit = p.few ? 16 : AT_P;
     /* with few rows their columns are shared out too, while the chip holds the workgroups in one round */
     int groups = 1;
     for (int k = 2; k <= hd / 64; k++)
@@ -911,21 +669,12 @@ Plan make_plan(int n, int nh, int nkv, int hd, int kv_dtype) {
 template <int HDP, int KVT>
 int launch_ctx(nmx_ctx *ctx, const TreeAttn &a, const Plan &p) {
     const dim3 grid((unsigned)(p.splits * a.nkv * p.mtiles), (unsigned)p.halves);
-    static std::atomic<uint64_t> set0, set1;
-    if (p.few) {
-        if constexpr (HDP <= 256 || KVT != KV_F32) {
-            /* the join of the waves takes the place of the tiles */
-            constexpr int od = HDP > 256 ? 256 : HDP, join = 4 * (64 * od / 16 + 16) * 16;
-            constexpr int tiles = few_lds<HDP, KVT>(), lds = tiles > join ? tiles : join;
-            if (nmx_dyn_lds(ctx, (const void *)attn_tree_few_k<HDP, KVT>, lds, set1)) return -1;
-            attn_tree_few_k<HDP, KVT><<<grid, 256, lds, ctx->stream>>>(a);
-        }
-    } else {
-        constexpr int od = HDP > 256 ? 256 : HDP, planes = KVT == KV_F32 ? 2 : 1;
-        constexpr int lds = (HDP > 256 ? 1 : 2) * (planes * AT_P * (HDP + od) * 2 + 3 * AT_P * 4);
-        if (nmx_dyn_lds(ctx, (const void *)attn_tree_ctx_k<HDP, KVT>, lds, set0)) return -1;
-        attn_tree_ctx_k<HDP, KVT><<<grid, 64 * ctx_waves<HDP>(), lds, ctx->stream>>>(a);
-    }
+    static std::atomic<uint64_t> set0;
+    constexpr int nb = ctx_bufs<HDP, KVT>();
+    constexpr int od = HDP > 256 ? 256 : HDP, planes = KVT == KV_F32 ? 2 : 1;
+    constexpr int lds = nb * (planes * AT_P * (HDP + od) * 2 + 3 * AT_P * 4);
+    if (nmx_dyn_lds(ctx, (const void *)attn_tree_ctx_k<HDP, KVT>, lds, set0)) return -1;
+    attn_tree_ctx_k<HDP, KVT><<<grid, 64 * ctx_waves<HDP>(), lds, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "attn_tree_ctx");
     return 0;
 }
@@ -983,12 +732,7 @@ int nmx_attn_tree_prep(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *pare
 size_t nmx_attn_tree_work_bytes(int n, int nh, int nkv, int hd) {
     if (n < 1 || n > NMX_TREE_MAX || nkv < 1 || nh < nkv || nh % nkv || nh > 1024 || hd < 64 || hd > 512 || hd % 64)
         return 0;
-    size_t most = 0;
-    for (int t = KV_F32; t <= KV_I8; t++) {
-        const size_t b = make_plan(n, nh, nkv, hd, t).bytes;
-        most = b > most ? b : most;
-    }
-    return most;
+    return make_plan(n, nh, nkv, hd).bytes;
 }
 
 int nmx_attn_tree(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent, void *work) {
@@ -996,14 +740,14 @@ int nmx_attn_tree(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent, v
     if (tree_shape(ctx, p, parent, "nmx_attn_tree")) return -1;
     if (!p->o || !work || (p->a8.q && (!p->a8.d || !p->a8.fs))) return nmx_fail(ctx, "nmx_attn_tree: NULL argument");
     if ((uintptr_t)work % 16) return nmx_fail(ctx, "nmx_attn_tree: work not 16-byte aligned");
-    const Plan pl = make_plan(p->n, p->nh, p->nkv, p->hd, p->kv_dtype);
+    const Plan pl = make_plan(p->n, p->nh, p->nkv, p->hd);
     const size_t kb = nmx_kv_bytes(p->kv_dtype, p->nkv, p->max_ctx, p->hd), ob = (size_t)p->n * p->nh * p->hd * 4;
     if (nmx_overlap(work, pl.bytes, p->q, 2 * ob) || nmx_overlap(work, pl.bytes, p->kc, kb) ||
         nmx_overlap(work, pl.bytes, p->vc, kb) || nmx_overlap(work, pl.bytes, p->o, ob) ||
         nmx_overlap(p->o, ob, p->q, 2 * ob) || nmx_overlap(p->o, ob, p->kc, kb) || nmx_overlap(p->o, ob, p->vc, kb))
         return nmx_fail(ctx, "nmx_attn_tree: o, work and the inputs overlap");
     const TreeAttn a{p->n, p->nh, p->nkv, p->hd, p->max_ctx, p->q, p->kc, p->vc, p->pos, parent, p->pos_off,
-                     p->scale, (float *)work, (float4 *)((char *)work + pl.part_bytes), pl.splits, pl.unit,
+                     p->scale, (float *)work, (float4 *)((char *)work + pl.part_bytes), pl.splits,
                      pl.jcols, p->o, p->a8.q, p->a8.d, p->a8.fs};
     const nmx_on_device on(ctx);
     if (p->kv_dtype == KV_F16) return launch_tree<KV_F16>(ctx, a, pl);

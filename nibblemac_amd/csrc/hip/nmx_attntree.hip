@@ -13,7 +13,14 @@
  * row's scale are first brought to a power of two of their own, so that neither part leaves
  * binary16's range, and the softmax weights are taken 2^12 high. A binary16 cache's rows and int8
  * codes are exact as they are: two products per pair (q or weight high, low); an fp32 row has
- * two parts itself: three products, the low-low one left out (2^-22 of the row). */
+ * two parts itself: three products, the low-low one left out (2^-22 of the row).
+ *
+ * Times of both kernels (context + join) on MI355X, 8 heads on 2 of 256: 64 nodes over 100000 binary16
+ * positions 124 us (110 + 14), 423 TFLOP/s of the definition's products and twice that of the matrix
+ * cores', which a large binary16 product runs at 1068; 37 nodes over 4001 int8 26.1 us (17.8 + 9.4);
+ * 9 nodes over 600 fp32 17.0 us (10.9 + 6.1) and one node over 20000 binary16 17.9 us (12 + 6.1): the
+ * latter 41 MB, 8 us as a copy; the others are chains of round trips to memory (position, rows, barrier,
+ * parts, position, parts, rows). */
 #include "nmx_internal.h"
 #include "nmx_a8.h"
 #include "nmx_attn.h"
@@ -198,16 +205,21 @@ __device__ __forceinline__ float amax8(const Raw8<KV_F32> &r) {
     return fmaxf(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))),
                  fmaxf(fmaxf(fabsf(x[4]), fabsf(x[5])), fmaxf(fabsf(x[6]), fabsf(x[7]))));
 }
-/* x as a binary16 (towards zero, two at a time: the rest is exact either way) and the binary16 rest */
+/* x up as a binary16 and the binary16 rest: 2^-22 of x is left */
+__device__ __forceinline__ void split8(const float (&x)[8], float up, half8 &h, half8 &r) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float v = x[i] * up;
+        h[i] = (_Float16)v;
+        r[i] = (_Float16)__builtin_fmaf((float)h[i], -1.0f, v);
+    }
+}
+/* two weights, the first part towards zero in one instruction: 2^-21 is left */
 typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void split2(float a, float b, half8 &h, half8 &r, int i) {
     const fp16x2 p = __builtin_amdgcn_cvt_pkrtz(a, b);
     h[i] = (_Float16)p.x, h[i + 1] = (_Float16)p.y;
     r[i] = (_Float16)__builtin_fmaf((float)h[i], -1.0f, a), r[i + 1] = (_Float16)__builtin_fmaf((float)h[i + 1], -1.0f, b);
-}
-__device__ __forceinline__ void split8(const float (&x)[8], float up, half8 &h, half8 &r) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) split2(x[i] * up, x[i + 1] * up, h, r, i);
 }
 
 /* Lane c of 16 (quarter gq) takes its query row's chunks 4 k + gq: requested first, split when the
@@ -345,9 +357,12 @@ __device__ __forceinline__ void store_part(const TreeAttn &a, const Running<DT> 
     }
 }
 
-/* Many rows: 8 waves of 16 rows (4 where a row has 512 columns) share a tile of 32 positions. The next
- * tile is on its way into registers while the matrix cores work on the current one (two tiles in
- * LDS; one for 512 columns). */
+/* 8 waves of 16 rows (4 where a row has 512 columns) share a tile of 32 positions. The next tile is on its
+ * way into registers while the matrix cores work on the current one, with two tiles in LDS (one for
+ * 512 columns of fp32, which have neither the registers nor the room). The same kernel serves few rows,
+ * whose waves without rows only bring tiles: waves with tiles of their own, each staging for itself, took
+ * as long over 20000 binary16 positions and much longer otherwise (5 nodes over 30000 fp32 positions 86
+ * against 46 us, 2 over 16 int8 17 against 12). */
 template <int HDP>
 constexpr int ctx_waves() {
     return HDP > 256 ? 4 : 8;
@@ -519,7 +534,7 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
 }
 
 /* ---- the node's ancestors, and the join ---------------------------------------------------- */
-constexpr int JT = 512; /* threads of a join */
+constexpr int JT = 512; /* threads of a join: of 1024, two workgroups do not fit a CU's registers (64 nodes 21 against 14 us) */
 
 /* Workgroup: a node and head, blockIdx.y a group of a.jcols columns of it. */
 template <int KVT>

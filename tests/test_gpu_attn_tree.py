@@ -14,7 +14,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from nibblemac_amd.nmx import A8, AttnArgs, NmxError
+from nibblemac_amd.nmx import A8, AttnArgs, Device, NmxError
 from tests.test_gpu_q4k import assert_bits_equal
 
 KV_F32, KV_F16, KV_I8 = 0, 1, 2
@@ -366,3 +366,42 @@ def test_refusals(dev):
     assert dev.lib.nmx_attn_tree_prep(dev.ctx, None, par.ptr) == -1
     dev.sync()
     assert not b["o"].numpy().any() and not b["kc"].numpy().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_F16, KV_I8])
+@pytest.mark.parametrize("n,nh,nkv,hd,pos", [(1, 8, 1, 512, 9001), (23, 4, 1, 448, 12300), (1, 4, 2, 64, 20011), (3, 4, 2, 192, 20000),
+                                             (20, 8, 2, 320, 5000), (2, 16, 2, 256, 13000)])
+def test_several_tiles_to_a_part(dev, n, nh, nkv, hd, pos, kv):
+    print(f"[case] attn tree tiles n={n} hd={hd} pos={pos} kv={kv}", flush=True)
+    check(dev, np.random.default_rng(n + hd + kv), (n, nh, nkv, hd, pos + n + 3, kv, pos), poison=False)
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once(dev):
+    """Two devices' streams with workspaces of their own, calls queued in turn without a wait."""
+    print("[case] attn tree two streams", flush=True)
+    rng = np.random.default_rng(31)
+    n, nh, nkv, hd, ctx, pos = 19, 4, 2, 128, 2100, 2000
+    shape = (n, nh, nkv, hd, ctx)
+    other = Device(0)
+    jobs = []
+    for d, kv in ((dev, KV_F16), (other, KV_F32)):
+        q, parent = rng.standard_normal((n, nh, 2 * hd)).astype(np.float32), tree(rng, n, "random")
+        (kc, _), (vc, _) = (make_cache(rng, kv, nkv, ctx, hd) for _ in range(2))
+        want = run(d, q, kc, vc, parent, pos, shape, kv)
+        b = [d.to_device(x) for x in (q, kc, vc, parent, np.array([pos], np.int32))]
+        outs = [d.zeros((n, nh * hd), np.float32) for _ in range(6)]
+        w = d.alloc(d.attn_tree_work_bytes(n, nh, nkv, hd))
+        d.sync()
+        jobs.append((d, kv, b, outs, w, want))
+    for r in range(6):
+        for d, kv, b, outs, w, _ in jobs:
+            a = AttnArgs(n=n, nh=nh, nkv=nkv, hd=hd, max_ctx=ctx, q=b[0].ptr, scale=np.float32(1 / np.sqrt(hd)), kc=b[1].ptr,
+                         vc=b[2].ptr, pos=b[4].ptr, o=outs[r].ptr, a8=A8(None, None, None), kv_dtype=kv)
+            d.attn_tree(a, b[3].ptr, w.ptr)
+    for d, _, _, outs, _, want in jobs:
+        d.sync()
+        for o in outs:
+            assert_bits_equal(o.numpy(), want, "beside another stream's calls")
+    other.close()

@@ -287,3 +287,62 @@ def test_rounds_equal_the_accepted_chain(dev, kv):
         for x in (*b, choice, work, out, S, L.par):
             x.free()
     assert accepted >= 4
+
+
+@pytest.mark.gpu
+def test_position_among_the_outputs_is_refused(dev):
+    print("[case] tree commit pos refusals", flush=True)
+    n = 4
+    i = {k: dev.zeros(32, np.int32) for k in ("parent", "tok", "choice", "out", "ctl", "vt")}
+    kv = dev.zeros((1, 16, 64), np.float32)
+    for pos in (i["out"].ptr, i["out"].ptr + 4 * (n + 1), i["vt"].ptr, i["ctl"].ptr + 4, i["ctl"].ptr + 8):
+        with pytest.raises(NmxError, match="nmx_tree_commit"):
+            dev.tree_commit(tree_commit_args(n, i["parent"], i["tok"], i["choice"], i["out"], ctl=i["ctl"], vt=i["vt"],
+                                             kv=dict(caches=[kv], nkv=1, max_ctx=16, hd=64, kv_dtype=0, pos=pos)))
+    dev.sync()
+    assert not any(x.numpy().any() for x in (*i.values(), kv))
+
+
+@pytest.mark.gpu
+def test_captured_call(dev):
+    """One captured commit, replayed over other choices and positions, against the eager call's check."""
+    print("[case] tree commit graph", flush=True)
+    rng = np.random.default_rng(21)
+    n, ctx, nkv, hd, cap, C, row = 12, 64, 2, 64, 16, 96, 70
+    parent = np.array([-1] + [int(rng.integers(0, t)) for t in range(1, n)], np.int32)
+    i = dict(parent=dev.to_device(parent), tok=dev.zeros(n, np.int32), choice=dev.zeros(n, np.int32), out=dev.zeros(n + 2, np.int32),
+             ctl=dev.zeros(16, np.int32))
+    f = dict(state=dev.zeros((2, 3, C), np.float32), xin=dev.zeros((2, cap, C), np.float32), log=dev.zeros((2, cap, row), np.float32),
+             pend=dev.zeros((2, cap, row), np.float32))
+    kv = dev.zeros((nkv, ctx, hd), np.float32)
+    a = tree_commit_args(n, i["parent"], i["tok"], i["choice"], i["out"], ctl=i["ctl"],
+                         lin=dict(layers=2, C=C, conv_k=4, cap=cap, row=row, **f),
+                         kv=dict(caches=[kv], nkv=nkv, max_ctx=ctx, hd=hd, kv_dtype=0, pos=i["ctl"]))
+
+    def fill():
+        tok = rng.integers(0, 3, n).astype(np.int32)
+        x = {k: rng.standard_normal(b.numpy().shape).astype(np.float32) for k, b in (*f.items(), ("kv", kv))}
+        new = dict(tok=tok, choice=rng.integers(0, 3, n).astype(np.int32), ctl=np.array([int(rng.integers(0, 40))] + [0] * 15, np.int32), **x)
+        return new
+
+    def put(new):
+        for k, v in new.items():
+            dev.upload(kv if k == "kv" else f[k] if k in f else i[k], v)
+
+    def outputs():
+        dev.sync()
+        return [x.numpy() for x in (i["out"], i["ctl"], f["state"], f["pend"], kv)]
+
+    dev.graph_begin()
+    dev.tree_commit(a)
+    g = dev.graph_end()
+    for _ in range(4):
+        new = fill()
+        put(new)
+        dev.graph_launch(g)
+        got = outputs()
+        put(new)
+        dev.tree_commit(a)
+        for x, y in zip(got, outputs()):
+            assert_bits_equal(x, y, "replay")
+    dev.graph_destroy(g)

@@ -336,9 +336,11 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
     }
     const int keep = keep_of(a.keep, a.keep_dev);
     rp.run(s, a.pend, a.keep, keep, heads, h, logw, j0 + c, pk, pdec);
-    if (keep > 0 && T == 0) {
+    if (keep > 0) {
+        __syncthreads(); /* every wave's request of these columns has come: one of them writes */
+        if (T == 0)
 #pragma unroll
-        for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
+            for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
     }
     /* S^T k and S^T q of the wave's nodes: element j is node 16 T + 4 gq + j, column c */
     f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk, sk2 = sk, sq2 = sk; /* two chains each: shorter ones round less */

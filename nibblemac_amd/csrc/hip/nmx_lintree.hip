@@ -12,7 +12,13 @@
  * and only the deltas remain to be solved, one level of the tree after the other.
  *
  * A node's sums run over its own ancestors alone (no product with a masked zero), so whatever
- * another branch holds, NaN or infinity, does not reach it. */
+ * another branch holds, NaN or infinity, does not reach it.
+ *
+ * On MI355X, 16 heads of 128 x 128: 9 nodes 15.8 us (3.0 MB, 0.6 us as a copy), 64 nodes 28 us (7.6 MB,
+ * 1.5 us; pre 5.1, rule 22.2, post 4.5). Both are chains of phases behind barriers, not bytes: the
+ * requests' round trip (3 us), the conv, the norms in their order, the products, then the levels of the
+ * tree, one round through LDS each (0.2 us). The whole mixer of a head in one workgroup, for up to 16
+ * nodes, took longer (9 nodes 18.0, 16 nodes 20.8 against 16.9 us). */
 #include "nmx_internal.h"
 #include "nmx_a8.h"
 #include "nmx_lanes.h"
@@ -166,10 +172,10 @@ struct TreeRule {
 
 constexpr int TR_B = 8; /* pending rows staged at a time */
 
-/* The tree in LDS, for N nodes at most: of node t, in order of depth, its ancestors (itself the last) and
+/* The tree in LDS: of node t, in order of depth, its ancestors (itself the last) and
  * the product of the decays after each of them up to t; the product of all of them from the state. */
-template <int N>
 struct TreeTables {
+    static constexpr int N = NMX_TREE_MAX;
     unsigned long long sets[N];
     float dec[N], bet[N], gs[N], gap[N][N + 1];
     uint8_t depth[N];
@@ -177,18 +183,15 @@ struct TreeTables {
     int levels;
 };
 /* One wave; lane t < n: its parent p, decay d and beta bt. */
-template <int N>
-__device__ __forceinline__ void tree_tables(TreeTables<N> &s, int n, unsigned long long set, int p, float d, float bt) {
+__device__ __forceinline__ void tree_tables(TreeTables &s, int n, unsigned long long set, int p, float d, float bt) {
     const int lane = threadIdx.x & 63;
     const bool in = lane < n;
     int at = in ? __popcll(set) - 1 : -1, cur = lane;
     int deep = at;
 #pragma unroll
     for (int x = 32; x >= 1; x >>= 1) deep = max(deep, __shfl_xor(deep, x));
-    if (lane < N) {
-        s.sets[lane] = set, s.dec[lane] = d, s.bet[lane] = bt, s.depth[lane] = (uint8_t)(at < 0 ? 0 : at);
-        for (int k = at < 0 ? 0 : at; k <= deep; k++) s.anc[lane][k] = (uint8_t)lane;
-    }
+    s.sets[lane] = set, s.dec[lane] = d, s.bet[lane] = bt, s.depth[lane] = (uint8_t)(at < 0 ? 0 : at);
+    for (int k = at < 0 ? 0 : at; k <= deep; k++) s.anc[lane][k] = (uint8_t)lane;
     float g = 1.0f;
     for (int k = 0; k <= deep; k++) { /* up the path, every lane at once */
         if (at >= 0) s.gap[lane][at] = g, s.anc[lane][at] = (uint8_t)cur;
@@ -198,7 +201,7 @@ __device__ __forceinline__ void tree_tables(TreeTables<N> &s, int n, unsigned lo
         at--;
         cur = up < 0 ? cur : up;
     }
-    if (lane < N) s.gs[lane] = g;
+    s.gs[lane] = g;
     if (lane == 0) s.levels = deep + 1;
 }
 
@@ -283,15 +286,14 @@ constexpr int tree_wave() {
     return DK4 < 64 ? 1 : 0;
 }
 
-/* More than 16 nodes: one workgroup per head and 16 value columns (a group of the state's layout), a wave
- * per 16 nodes. The state's columns are a matrix operand as they lie: lane (column c, quarter gq)
- * holds the float4 slots of keys gq dk/4 .. of its column, and the wave's rows of k and q are read in
- * the same order. */
+/* One workgroup per head and 16 value columns (a group of the state's layout), a wave per 16 nodes. The
+ * state's columns are a matrix operand as they lie: lane (column c, quarter gq) holds the float4 slots of
+ * keys gq dk/4 .. of its column, and the wave's rows of k and q are read in the same order. */
 template <int DK4>
 __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(TreeRule a) {
     constexpr int DK = 4 * DK4, NS = DK4 / 4, HS = DK + 8; /* halves of a row in LDS: 16 bytes on, no bank twice */
     extern __shared__ float4 smem4[];
-    __shared__ TreeTables<NMX_TREE_MAX> tt;
+    __shared__ TreeTables tt;
     __shared__ float del[2][NMX_TREE_MAX][16], pdec[TR_B];
     const int h = blockIdx.x, j0 = blockIdx.y * 16, tid = threadIdx.x, lane = tid & 63, T = tid >> 6, waves = (int)(blockDim.x >> 6) - tree_wave<DK4>();
     const int c = lane & 15, gq = lane >> 4, n = a.n, heads = a.heads, dv = a.dv, n16 = 16 * waves;
@@ -452,278 +454,6 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
     }
 }
 
-/* Up to 16 nodes: the whole mixer of a head in one workgroup and one launch, a wave per 16 value columns.
- * The raw rows lie in LDS, where each channel's thread reads its windows and then puts its outputs in
- * their place (the last node first: nodes read their ancestors' raw values, which lie before them);
- * o replaces v there in turn, for the gated norm over the head. */
-constexpr int TO_N = 16, TO_ROWS = TO_N + 7; /* nodes, then the conv state's rows */
-constexpr int TO_WAVES = 10;                 /* 8 of value columns, two more for the tree and the products of nodes */
-
-struct TreeOne {
-    TreePre p;
-    TreeRule r;
-    const float *z, *norm_w;
-    int z_stride, y_stride;
-    float eps;
-    float *y;
-    int8_t *aq;
-    float *ad, *afs;
-};
-
-template <int DK4>
-__global__ __launch_bounds__(64 * TO_WAVES) void lin_tree_one_k(TreeOne a) {
-    constexpr int DK = 4 * DK4, NS = DK4 / 4;
-    extern __shared__ float4 smem4[];
-    __shared__ TreeTables<TO_N> tt;
-    __shared__ float2 co[TO_N][TO_N + 1]; /* D k.k, D q.k of a node's ancestors by depth */
-    __shared__ alignas(16) float pk[TR_B][DK + 16];
-    __shared__ float pdec[TR_B], rr[2 * TO_N];
-    __shared__ alignas(16) int win[TO_N][8]; /* the LDS rows of a node's window, the newest first */
-    const TreePre &p = a.p;
-    const TreeRule &q = a.r;
-    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6, c = lane & 15, gq = lane >> 4;
-    const int n = p.n, heads = q.heads, dv = q.dv, K = p.K, S = K - 1, kh = h / q.rep, T = blockDim.x, waves = T >> 6;
-    const int CH = 2 * DK + dv, RS = CH + 4, j0 = 16 * w;
-    const size_t logw = (size_t)DK + dv + 1;
-    float *xs = (float *)smem4; /* [TO_ROWS][RS]: q | k | v of a row */
-    const bool owner = j0 < dv; /* the wave has value columns */
-
-    /* requests: the channel's raw rows, conv rows and taps, the wave's state columns, the pending rows */
-    const bool chan = tid < CH;
-    const int ch = !chan ? 0 : tid < DK ? kh * DK + tid : tid < 2 * DK ? p.kd + kh * DK + tid - DK : 2 * p.kd + h * dv + tid - 2 * DK;
-    float x[TO_N], st[7], wc[8];
-#pragma unroll
-    for (int t = 0; t < TO_N; t++) x[t] = p.raw[(size_t)(t < n ? t : n - 1) * p.raw_stride + ch];
-#pragma unroll
-    for (int r = 0; r < 7; r++) st[r] = S ? p.state[(size_t)(r < S ? r : S - 1) * p.C + ch] : 0.0f;
-#pragma unroll
-    for (int r = 0; r < 8; r++) wc[r] = p.conv_w[(size_t)ch * K + (r < K ? r : K - 1)];
-    Replay<DK4, 256> rp;
-    rp.ask(q.pend, 0, q.keep, heads, h, logw, owner ? j0 + c : 0);
-    float4 s[NS];
-    float *Sp = q.S + ((size_t)h * dv + (owner ? j0 : 0)) * DK + (4 * c + gq) * 4;
-#pragma unroll
-    for (int k = 0; k < NS; k++) s[k] = *(const float4 *)(Sp + k * 256);
-    /* the last two waves, which have no channels: the windows, the gates; behind the barrier the tree */
-    if (w == waves - 1) {
-        const int up = lane < n ? tree_parent(p.parent, lane) : -1;
-        int at = lane, row = S;
-        for (int r = 0; r < K; r++) {
-            const bool node = at >= 0;
-            row -= !node;
-            if (lane < n) win[lane][r] = node ? at : TO_N + row;
-            const int next = __shfl(up, node ? at : 0);
-            at = node ? next : at;
-        }
-    } else if (w == waves - 2 && lane < n) {
-        const float bt = tree_beta(p.b_in[(size_t)lane * p.g_stride + h]), d = tree_decay(p, p.a_in[(size_t)lane * p.g_stride + h], h);
-        p.beta[lane * heads + h] = bt, p.decay[lane * heads + h] = d;
-        tt.bet[lane] = bt, tt.dec[lane] = d;
-    }
-    if (chan) {
-#pragma unroll
-        for (int t = 0; t < TO_N; t++) xs[t * RS + tid] = x[t];
-#pragma unroll
-        for (int r = 0; r < 7; r++)
-            if (r < S) xs[(TO_N + r) * RS + tid] = st[r];
-        if (p.xin) {
-#pragma unroll
-            for (int t = 0; t < TO_N; t++)
-                if (t < n) p.xin[(size_t)t * p.C + ch] = x[t];
-        }
-    }
-    nmx_lds_sync();
-    if (w == waves - 1) { /* while the others convolve */
-        int up;
-        const unsigned long long set = tree_ancestors(p.parent, n, &up);
-        tree_tables(tt, n, set, up, lane < n ? tt.dec[lane] : 1.0f, lane < n ? tt.bet[lane] : 0.0f);
-    }
-    if (chan) { /* conv + SiLU: the channel's column is this thread's own, all windows read before any output */
-        if (K == 4) {
-            float b[TO_N][3];
-#pragma unroll
-            for (int t = 0; t < TO_N; t++) {
-                const int4 at = *(const int4 *)win[t < n ? t : 0];
-                b[t][0] = xs[at.y * RS + tid], b[t][1] = xs[at.z * RS + tid], b[t][2] = xs[at.w * RS + tid];
-            }
-#pragma unroll
-            for (int t = 0; t < TO_N; t++) {
-                if (t >= n) continue;
-                float y = wc[0] * b[t][2]; /* taps in order, the oldest first */
-                y = y + wc[1] * b[t][1];
-                y = y + wc[2] * b[t][0];
-                y = y + wc[3] * x[t];
-                xs[t * RS + tid] = nmx_silu(y);
-            }
-        } else {
-#pragma unroll
-            for (int t = 0; t < TO_N; t++) {
-                if (t >= n) continue;
-                float y = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (j >= K) continue;
-                    const float v = xs[win[t][K - 1 - j] * RS + tid];
-                    y = j ? y + wc[j] * v : wc[0] * v;
-                }
-                x[t] = nmx_silu(y);
-            }
-#pragma unroll
-            for (int t = 0; t < TO_N; t++)
-                if (t < n) xs[t * RS + tid] = x[t];
-        }
-    }
-    const int keep = keep_of(q.keep, q.keep_dev);
-    rp.run(s, q.pend, q.keep, keep, heads, h, logw, owner ? j0 + c : 0, pk, pdec);
-    if (keep > 0 && owner) {
-#pragma unroll
-        for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
-    }
-    nmx_lds_sync();
-    /* L2 norms of the q and k rows: 4 chains each, in a quad of lanes */
-    for (int i = tid; i < 8 * TO_N; i += T) {
-        const int t = i >> 3 < n ? i >> 3 : n - 1;
-        const float ch4 = square_chain(xs + t * RS + (i >> 2 & 1) * DK + (i & 3), DK >> 2);
-        rr[i >> 2] = 1.0f / sqrtf((quad_sum(ch4) + 0.0f) + p.l2eps);
-    }
-    nmx_lds_sync();
-    for (int i = tid; i < n * 2 * DK; i += T) {
-        const int t = i / (2 * DK), e = i % (2 * DK);
-        xs[t * RS + e] = (xs[t * RS + e] * rr[2 * t + (e >= DK)]) * (e < DK ? p.qscale : 1.0f);
-    }
-    nmx_lds_sync();
-    if (chan) { /* what is kept of the pass: conv outputs, the log rows' keys */
-#pragma unroll 4
-        for (int t = 0; t < n; t++) {
-            const float v = xs[t * RS + tid];
-            p.out[(size_t)t * p.C + ch] = v;
-            if (tid >= DK && tid < 2 * DK) q.log[((size_t)t * heads + h) * logw + tid - DK] = v;
-        }
-    }
-    if (tid < n) q.log[((size_t)tid * heads + h) * logw + DK + dv] = tt.dec[tid];
-    /* products: rows past the end hold raw values, and are not used. D k.k and D q.k by two waves (the
-     * last ones, which have no channels' rows to store), their sums in two chains */
-    const float *qr = xs + c * RS + gq * DK4, *kr = qr + DK;
-    for (int job = waves - 1 - w; job < 2; job += waves) {
-        const float *l = job ? qr : kr;
-        f32x4 u = {0.0f, 0.0f, 0.0f, 0.0f}, v = u;
-#pragma unroll
-        for (int k = 0; k < NS; k++) {
-            const float4 b = *(const float4 *)(kr + 4 * k), e = *(const float4 *)(l + 4 * k);
-            u = mfma4(e.x, b.x, u), v = mfma4(e.y, b.y, v), u = mfma4(e.z, b.z, u), v = mfma4(e.w, b.w, v);
-        }
-        const int dp = c < n ? tt.depth[c] : 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 4 * gq + j;
-            if (t >= n || !(tt.sets[t] >> c & 1)) continue;
-            const float d = (u[j] + v[j]) * tt.gap[t][dp];
-            if (job) co[t][dp].y = d;
-            else co[t][dp].x = d;
-        }
-    }
-    f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk;
-    if (owner) {
-#pragma unroll
-        for (int k = 0; k < NS; k++) {
-            const float4 x4 = *(const float4 *)(kr + 4 * k), y4 = *(const float4 *)(qr + 4 * k);
-            sk = mfma4(x4.x, s[k].x, sk), sq = mfma4(y4.x, s[k].x, sq);
-            sk = mfma4(x4.y, s[k].y, sk), sq = mfma4(y4.y, s[k].y, sq);
-            sk = mfma4(x4.z, s[k].z, sk), sq = mfma4(y4.z, s[k].z, sq);
-            sk = mfma4(x4.w, s[k].w, sk), sq = mfma4(y4.w, s[k].w, sq);
-        }
-    }
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = owner ? xs[(4 * gq + j) * RS + 2 * DK + j0 + c] : 0.0f;
-    nmx_lds_sync();
-    float *del = xs + 2 * DK + j0 + c; /* this lane's column: deltas where v was, then o */
-    if (owner) {
-        float r[4], o[4], bt[4];
-        float2 cf[4];
-        int depth[4], tj[4];
-        uint4 anc[4];
-        const int levels = tt.levels;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 4 * gq + j;
-            tj[j] = t < n ? t : n - 1;
-            depth[j] = t < n ? tt.depth[t] : -1;
-            const float g = tt.gs[tj[j]];
-            bt[j] = tt.bet[tj[j]];
-            r[j] = v[j] - g * sk[j], o[j] = g * sq[j];
-            anc[j] = *(const uint4 *)tt.anc[tj[j]];
-            cf[j] = co[tj[j]][0];
-        }
-        for (int d = 0; d < levels; d++) { /* the wave's columns are its own: no barrier */
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const bool now = depth[j] == d;
-                r[j] = now ? r[j] * bt[j] : r[j];
-                if (now) del[tj[j] * RS] = r[j];
-            }
-            nmx_lds_wave_sync();
-            float xd[4];
-            float2 cn[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) xd[j] = del[(anc[j].x & 255) * RS];
-#pragma unroll
-            for (int j = 0; j < 4; j++) cn[j] = co[tj[j]][d + 1];
-#pragma unroll
-            for (int j = 0; j < 4; j++) { /* chosen, not multiplied away: a node past its depth reads anything */
-                o[j] = depth[j] >= d ? o[j] + cf[j].y * xd[j] : o[j];
-                r[j] = depth[j] > d ? r[j] - cf[j].x * xd[j] : r[j];
-                cf[j] = cn[j];
-                anc[j].x >>= 8;
-                if ((d & 3) == 3) anc[j].x = anc[j].y, anc[j].y = anc[j].z, anc[j].z = anc[j].w;
-            }
-        }
-        nmx_lds_wave_sync();
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int t = 4 * gq + j;
-            if (t >= n) continue;
-            del[t * RS] = o[j];
-            q.o[(size_t)t * q.o_stride + h * dv + j0 + c] = o[j];
-            q.log[((size_t)t * heads + h) * logw + DK + j0 + c] = r[j];
-        }
-    }
-    const int nd = n * dv; /* whole half-waves: dv % 32 == 0 */
-    constexpr int ZB = 4; /* turns of the gated norm: n dv <= 16 dv values, T >= 4 dv threads */
-    float zb[ZB], nb[ZB];
-#pragma unroll
-    for (int u = 0; u < ZB; u++) {
-        const int i = tid + u * T < nd ? tid + u * T : tid % dv, t = i / dv, j = i % dv;
-        zb[u] = a.z[(size_t)t * a.z_stride + h * dv + j], nb[u] = a.norm_w[j];
-    }
-    nmx_lds_sync();
-    /* the gated RMSNorm over the head, as lin_post_k makes it */
-    for (int i = tid; i < 4 * TO_N; i += T) {
-        const float ch4 = square_chain(xs + (i >> 2 < n ? i >> 2 : n - 1) * RS + 2 * DK + (i & 3), dv >> 2);
-        rr[i >> 2] = 1.0f / sqrtf((quad_sum(ch4) + 0.0f) / (float)dv + a.eps);
-    }
-    nmx_lds_sync();
-#pragma unroll
-    for (int u = 0; u < ZB; u++) {
-        const int i = tid + u * T;
-        if (i >= nd) continue;
-        const int t = i / dv, j = i % dv, col = h * dv + j;
-        float y = (xs[t * RS + 2 * DK + j] * rr[t]) * nb[u];
-        y = y * nmx_silu(zb[u]);
-        if (a.y) a.y[(size_t)t * a.y_stride + col] = y;
-        if (a.aq) a8_block(y, col >> 5, t, n, a.aq, a.ad, a.afs);
-    }
-}
-
-template <int DK4>
-int launch_one(nmx_ctx *ctx, const TreeOne &a, int threads, size_t lds) {
-    static std::atomic<uint64_t> set;
-    if (nmx_dyn_lds(ctx, (const void *)lin_tree_one_k<DK4>, (size_t)TO_ROWS * (8 * DK4 + 256 + 4) * 4, set)) return -1;
-    lin_tree_one_k<DK4><<<(unsigned)a.r.heads, (unsigned)threads, lds, ctx->stream>>>(a);
-    NMX_LAUNCHED(ctx, "lin_tree_one");
-    return 0;
-}
-
 template <int DK4>
 int launch_rule(nmx_ctx *ctx, const TreeRule &a) {
     const int n16 = (a.n + 15) / 16 * 16;
@@ -787,13 +517,6 @@ int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *m, const int32_t *par
                     p.b_in, p.a_in, p.g_stride, heads, p.A_log, p.A, p.dt_bias, p.beta, p.decay, parent};
     const TreeRule t{n, heads, r.rep, dv, p.kd, p.C, p.out, p.beta, p.decay, r.S, r.o, r.o_stride, r.log, r.pend, r.keep,
                      r.keep_dev, parent, p.qscale};
-    const int ch_waves = (2 * dk + dv + 63) / 64, waves = (dv / 16 > ch_waves ? dv / 16 : ch_waves) + 2;
-    if (n <= TO_N && dk <= 128 && waves <= TO_WAVES) { /* 10 waves of at most 168 registers fit a CU at once */
-        const TreeOne o{a, t, m->z, m->norm_w, m->z_stride, m->y_stride, m->eps, m->y, m->a8.q, m->a8.d, m->a8.fs};
-        const size_t lds = (size_t)TO_ROWS * (2 * dk + dv + 4) * 4;
-        return dk == 32 ? launch_one<8>(ctx, o, 64 * waves, lds) : dk == 64 ? launch_one<16>(ctx, o, 64 * waves, lds) :
-                          launch_one<32>(ctx, o, 64 * waves, lds);
-    }
     const dim3 grid((unsigned)((p.C + dk - 1) / dk + 1), (unsigned)((n + TP_N - 1) / TP_N));
     const unsigned threads = dk < 64 ? 64 : (unsigned)dk;
     const size_t lds = (size_t)TP_N * (dk + 4) * 4;

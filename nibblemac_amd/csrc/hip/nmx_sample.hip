@@ -19,7 +19,14 @@
  * Masses are whole numbers, the weight relative to its bin's lower edge (in [1, e^(1/8))) times
  * 2^40: their sums do not depend on the order in which lanes add them, so a call's result is the
  * same every time; between bins they are scaled and added in 64-bit floating point in a fixed
- * order. Each weight is thereby right to 2^-41 of itself. */
+ * order. Each weight is thereby right to 2^-40 of itself (half a unit of rounding, and the polynomial's
+ * next term).
+ *
+ * On MI355X (scan + pick): a row of 248320 with top-k and top-p 16.3 us (6.2 + 10.1), of 32768 with min-p
+ * 13.4 (5.9 + 7.5), 5 rows at the temperature alone 12.1 (5.5 + 7.9), 64 rows of 248320 with top-p
+ * 0.95 and no peaks 51 (26.6 + 25): 63.6 MB, 12.3 us as a copy. The scan of 64 rows issues 40 vector
+ * instructions a logit, the weight's polynomial and the bin among them (86 % of its cycles; neither more
+ * copies of the bins nor two additions for one changed it). A pick is one workgroup's chain of phases. */
 #include "nmx_internal.h"
 #include "nmx_lanes.h"
 
@@ -33,7 +40,8 @@ static_assert(2 * SM_BINS == SM_T1, "two threads of sample_scan_k to a bin");
 constexpr int SM_MAXC = (1 << 20) / SM_CHUNK; /* chunks of the longest row */
 constexpr int SM_LIST = 16384; /* members of a bin kept in LDS; a bin with more is read again */
 constexpr int SM_RANK = 256;   /* members of a bin ranked by comparing all with all */
-constexpr int SM_FEW = SM_T2;  /* tokens among which a row is decided one to a thread */
+constexpr int SM_FEW = SM_T2;  /* tokens among which a row is decided one to a thread (500 of them 15 us against 22
+                                * through the bins; up to 64 by one wave, 9.9 against 12.6) */
 constexpr int SM_DIGIT = SM_T2; /* values of a selection's digit */
 static_assert(SM_SLICE == SM_T2, "a wave's slice of a chunk is one logit a thread of sample_pick_k");
 

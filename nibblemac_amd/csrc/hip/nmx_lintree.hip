@@ -14,11 +14,11 @@
  * A node's sums run over its own ancestors alone (no product with a masked zero), so whatever
  * another branch holds, NaN or infinity, does not reach it.
  *
- * On MI355X, 16 heads of 128 x 128: 9 nodes 15.8 us (3.0 MB, 0.6 us as a copy), 64 nodes 28 us (7.6 MB,
- * 1.5 us; pre 5.1, rule 22.2, post 4.5). Both are chains of phases behind barriers, not bytes: the
- * requests' round trip (3 us), the conv, the norms in their order, the products, then the levels of the
- * tree, one round through LDS each (0.2 us). The whole mixer of a head in one workgroup, for up to 16
- * nodes, took longer (9 nodes 18.0, 16 nodes 20.8 against 16.9 us). */
+ * On MI355X, 16 heads of 128 x 128: 9 nodes 15.5 us (3.0 MB, 0.6 us as a copy), 64 nodes 26 us (7.6 MB,
+ * 1.5 us; pre 5.5, rule 19.7, post 4.5). Both are chains of phases behind barriers, not bytes; of the rule's
+ * at 64 nodes the requests take 2.1 us, parts of the rows 1.6, 5 pending rows 2.2, the state's products
+ * and the tree's tables 2.2, the products of nodes 2.3, 15 levels 3.5. The whole mixer of a head in one
+ * workgroup, for up to 16 nodes, took longer (9 nodes 18.0, 16 nodes 20.8 against 16.9 us). */
 #include "nmx_internal.h"
 #include "nmx_a8.h"
 #include "nmx_lanes.h"
@@ -244,9 +244,10 @@ struct Replay {
         for (int u = 0; u < TR_B; u++) w[u] = row(u)[DK + col];
         d = row(threadIdx.x < TR_B ? threadIdx.x : 0)[logw - 1];
     }
-    /* into the state's columns held in s, as nmx_lin_apply makes them */
+    /* into the state's columns held in s, as nmx_lin_apply makes them; a wave without columns only helps to
+     * stage */
     __device__ __forceinline__ void run(float4 (&s)[DK4 / 4], const float *pend, int asked, int keep, int heads, int h, size_t logw,
-                                        int col, float (*pk)[DK + 16], float *pdec) {
+                                        int col, float (*pk)[DK + 16], float *pdec, bool has) {
         const int tid = threadIdx.x, gq = (tid & 63) >> 4;
         for (int u0 = 0; u0 < keep; u0 += TR_B) {
             if (u0) ask(pend, u0, asked, heads, h, logw, col);
@@ -261,7 +262,7 @@ struct Replay {
             nmx_lds_sync();
 #pragma unroll
             for (int u = 0; u < TR_B; u++) {
-                if (u >= nb) continue;
+                if (u >= nb || !has) continue;
                 const float dc = pdec[u];
                 const float *kr = &pk[u][gq * (DK4 + 4)];
 #pragma unroll
@@ -322,11 +323,13 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
         v[j] = a.qkv[(size_t)(t < n ? t : n - 1) * a.C + 2 * a.kd + h * dv + j0 + c];
     }
     const bool nodes = T < waves; /* the last wave has the tree instead */
-    if (T == (int)(blockDim.x >> 6) - 1) {
-        const float dc = lane < n ? a.decay[lane * heads + h] : 1.0f, bt = lane < n ? a.beta[lane * heads + h] : 0.0f;
-        int p;
-        const unsigned long long set = tree_ancestors(a.parent, n, &p);
-        tree_tables(tt, n, set, p, dc, bt);
+    const bool tree = T == (int)(blockDim.x >> 6) - 1;
+    float dc = 1.0f, bt1 = 0.0f;
+    int up = -1;
+    unsigned long long set = 0;
+    if (tree) {
+        dc = lane < n ? a.decay[lane * heads + h] : 1.0f, bt1 = lane < n ? a.beta[lane * heads + h] : 0.0f;
+        set = tree_ancestors(a.parent, n, &up);
     }
     const float q_up = a.qscale != 0.0f ? TR_UP / a.qscale : 0.0f, q_down = a.qscale / (TR_UP * TR_UP);
 #pragma unroll
@@ -337,13 +340,8 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
         if (QL) split4(qf[k], q_up, qh2 + at, qh2 + n16 * HS + at);
     }
     const int keep = keep_of(a.keep, a.keep_dev);
-    rp.run(s, a.pend, a.keep, keep, heads, h, logw, j0 + c, pk, pdec);
-    if (keep > 0) {
-        __syncthreads(); /* every wave's request of these columns has come: one of them writes */
-        if (T == 0)
-#pragma unroll
-            for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
-    }
+    rp.run(s, a.pend, a.keep, keep, heads, h, logw, j0 + c, pk, pdec, nodes);
+    if (tree) tree_tables(tt, n, set, up, dc, bt1); /* while the others multiply */
     /* S^T k and S^T q of the wave's nodes: element j is node 16 T + 4 gq + j, column c */
     f32x4 sk = {0.0f, 0.0f, 0.0f, 0.0f}, sq = sk, sk2 = sk, sq2 = sk; /* two chains each: shorter ones round less */
 #pragma unroll
@@ -354,10 +352,19 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
         sk2 = mfma4(kf[k].w, s[k].w, sk2), sq2 = mfma4(qf[k].w, s[k].w, sq2);
     }
     sk += sk2, sq += sq2;
-    nmx_lds_sync(); /* the rows, the tables; the pending keys have been read */
+    /* the rows, the tables; the pending keys have been read */
+    if (keep > 0) {
+        __syncthreads(); /* and every wave's request of the state's columns has come: one of them writes */
+        if (T == 0)
+#pragma unroll
+            for (int k = 0; k < NS; k++) *(float4 *)(Sp + k * 256) = s[k];
+    } else {
+        nmx_lds_sync();
+    }
     /* D(t, a) (k_t . k_a) and D(t, a) (q_t . k_a): the tiles (t, a) on and below the diagonal, in turn */
-    for (int job = nodes ? T : waves * waves, X = 0; X < waves; job -= X + 1, X++) {
-        for (; job <= X; job += waves) {
+    const int all = (int)(blockDim.x >> 6);
+    for (int job = T, X = 0; X < waves; job -= X + 1, X++) {
+        for (; job <= X; job += all) {
             const int U = job, an = 16 * U + c;
             const _Float16 *ar = kh2 + an * HS + 8 * gq, *tr = kh2 + (16 * X + c) * HS + 8 * gq, *ur = qh2 + (16 * X + c) * HS + 8 * gq;
             const int lo = n16 * HS;
@@ -412,6 +419,19 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
         an[j] = *(const uint32_t *)tt.anc[tj[j]];
         cf[j] = co[tj[j] * (n16 + 1)];
     }
+    /* the log rows' keys and decays: a share of the nodes for each workgroup of the head */
+    constexpr int LB = 4; /* values of a thread on their way at once */
+    const int mine = (n - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y * DK, TH = (int)blockDim.x; /* blockIdx.y >= n: none */
+    float lk[LB];
+    auto node_of = [&](int x) { return (int)blockIdx.y + x / DK * (int)gridDim.y; };
+    auto ask_keys = [&](int x0) {
+#pragma unroll
+        for (int u = 0; u < LB; u++) {
+            const int x = x0 + u * TH < mine ? x0 + u * TH : 0, t = node_of(x);
+            lk[u] = a.qkv[(size_t)(t < n ? t : n - 1) * a.C + a.kd + kh * DK + x % DK];
+        }
+    };
+    ask_keys(tid); /* there when the deltas are */
     for (int d = 0; d < levels; d++) {
         float(*dl)[16] = del[d & 1]; /* read in this level while the next one is written */
 #pragma unroll
@@ -445,13 +465,15 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
             a.log[((size_t)t * heads + h) * logw + DK + j0 + c] = r[j];
         }
     }
-    /* the log rows' keys and decays, a share of them each */
-    for (int t = blockIdx.y; t < n; t += gridDim.y) {
-        const float *src = a.qkv + (size_t)t * a.C + a.kd + kh * DK;
-        float *dst = a.log + ((size_t)t * heads + h) * logw;
-        for (int i = tid; i < DK; i += blockDim.x) dst[i] = src[i];
-        if (tid == 0) dst[DK + dv] = tt.dec[t];
+    for (int x0 = tid; x0 < mine; x0 += LB * TH) {
+        if (x0 != tid) ask_keys(x0);
+#pragma unroll
+        for (int u = 0; u < LB; u++) {
+            const int x = x0 + u * TH;
+            if (x < mine) a.log[((size_t)node_of(x) * heads + h) * logw + x % DK] = lk[u];
+        }
     }
+    if (tid * DK < mine) a.log[((size_t)node_of(tid * DK) * heads + h) * logw + DK + dv] = tt.dec[node_of(tid * DK)];
 }
 
 template <int DK4>

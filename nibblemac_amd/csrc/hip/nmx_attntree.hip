@@ -269,11 +269,12 @@ struct QueryRow {
 };
 
 /* A row's running state: weights are 2^(score - m); a value's factor 2^(its exponent - ve), where ve
- * grows so that no weight times value leaves binary16; l is this lane's share of the sum. */
+ * grows so that no weight times value leaves binary16; l is this lane's share of the sum, lc what its
+ * roundings have added to it (a part may have a thousand tiles, and equal weights round alike). */
 template <int DT>
 struct Running {
     float4v o[DT];
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f, lc = 0.0f;
     int ve = -1000;
     __device__ __forceinline__ Running() {
 #pragma unroll
@@ -307,21 +308,23 @@ __device__ __forceinline__ void add_tile(Running<OD / 16> &r, const float (&x)[8
     }
     if (__any(mx > r.m || ve != (KVT == KV_F16 ? 0 : r.ve))) {
         const float down = __builtin_amdgcn_exp2f(r.m - ref);
-        r.l *= down;
+        r.l *= down, r.lc *= down;
         const float dv = KVT == KV_F16 ? down : ldexpf(down, r.ve - ve < -300 ? -300 : r.ve - ve);
 #pragma unroll
         for (int d = 0; d < DT; d++) r.o[d] *= dv;
         r.m = mx, r.ve = ve;
     }
     half8 ph, pl;
-    float wv[8];
+    float wv[8], sum;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const float w = __builtin_amdgcn_exp2f(x[i] - ref);
-        r.l += w;
+        sum = i ? sum + w : w;
         if constexpr (KVT == KV_F16) wv[i] = w * 4096.0f;
         else wv[i] = ldexpf(w * f[i], e[i] - ve + 12);
     }
+    const float more = sum - r.lc, all = r.l + more;
+    r.lc = (all - r.l) - more, r.l = all;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) split2(wv[i], wv[i + 1], ph, pl, i);
 #pragma unroll
@@ -528,6 +531,7 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
         if (more) put_k(buf ^ 1), put_v(buf ^ 1);
         if (NB == 2) buf ^= 1;
     }
+    r.l -= r.lc;
     r.l += __shfl_xor(r.l, 16);
     r.l += __shfl_xor(r.l, 32);
     if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);

@@ -14,7 +14,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
-from nibblemac_amd.nmx import A8, AttnArgs, Device, NmxError
+from nibblemac_amd.nmx import A8, AttnArgs, Device, NmxError, tree_commit_args
 from tests.test_gpu_q4k import assert_bits_equal
 
 KV_F32, KV_F16, KV_I8 = 0, 1, 2
@@ -405,3 +405,74 @@ def test_two_contexts_at_once(dev):
         for o in outs:
             assert_bits_equal(o.numpy(), want, "beside another stream's calls")
     other.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,nkv,hd", [(KV_F32, 5, 256), (KV_F16, 5, 512), (KV_I8, 9, 512)])
+def test_offsets_past_32_bits(dev, kv, nkv, hd):
+    """Caches of more than 4 GiB: zeros but for a few rows of each head, which hold their query's
+    direction at scores near the logarithm of the positions; then the commit's move in the same caches."""
+    print(f"[case] attn tree long caches kv={kv}", flush=True)
+    rng = np.random.default_rng(41 + kv)
+    ctx, n = 1 << 20, 3
+    pos, parent = ctx - 7, np.array([-1, 0, 0], np.int32)
+    size = {KV_F32: 4, KV_F16: 2, KV_I8: 1}[kv]
+    total = nkv * ctx * hd * size + (nkv * ctx * 4 if kv == KV_I8 else 0)
+    assert nkv * ctx * hd * size > 1 << 32
+    caches = [dev.zeros(total, np.uint8) for _ in range(2)]
+
+    def move(b, g, slot, codes, scale, up):
+        """a row to (up) or from the cache"""
+        f = dev.lib.nmx_upload if up else dev.lib.nmx_download
+        for arr, off in ((codes, ((g * ctx) + slot) * hd * size), (scale, nkv * ctx * hd + (g * ctx + slot) * 4)):
+            if arr is not None:
+                dev.check(f(dev.ctx, *((b.ptr + off, arr.ctypes.data) if up else (arr.ctypes.data, b.ptr + off)), arr.nbytes))
+
+    def parts(enc):
+        return (enc[:hd].copy(), enc[hd:].copy()) if kv == KV_I8 else (enc.ravel().copy(), None)
+
+    q = rng.standard_normal((n, nkv, 2 * hd)).astype(np.float32)
+    scale = float(np.float32(1 / np.sqrt(hd)))
+    slots = [3, 777777, pos - 1, pos, pos + 1, pos + 2]
+    want, tol, rows = np.zeros((n, nkv, hd)), 0.0, {}
+    for g in range(nkv):
+        K, V = [], []
+        for i, s in enumerate(slots):
+            toward = q[i % n, g, :hd].astype(np.float64)
+            k = (toward * rng.uniform(12, 15) / (toward @ toward * scale)).astype(np.float32)
+            for b, x, out in ((caches[0], k, K), (caches[1], rng.standard_normal(hd).astype(np.float32), V)):
+                enc, val = encode(x[None, None], kv)
+                codes, sc = parts(enc)
+                move(b, g, s, codes, sc, True)
+                out.append(val[0, 0])
+                rows[b.ptr, g, s] = codes, sc
+        K, V = np.array(K), np.array(V)
+        for t in range(n):
+            at = [0, 1, 2] + [3 + a for a in range(n) if a == t or a == 0]
+            qt = q[t, g, :hd].astype(np.float64)
+            s = K[at] @ qt * scale
+            w = np.exp(s)
+            want[t, g] = w @ V[at] / (w.sum() + pos - 3) / (1 + np.exp(-q[t, g, hd:].astype(np.float64)))
+            ds = np.linalg.norm(qt) * np.linalg.norm(K, axis=1).max() * scale * (4 * 2.0 ** -22 + (hd / 32 + 8) * 2.0 ** -24)
+            tol = max(tol, (2 * ds + 2.0 ** -18) * np.abs(V).max())
+    i = dict(parent=dev.to_device(parent), pos=dev.to_device(np.array([pos], np.int32)), q=dev.to_device(q), o=dev.zeros((n, nkv * hd), np.float32),
+             tok=dev.to_device(np.array([5, 6, 7], np.int32)), choice=dev.to_device(np.array([7, 0, 8], np.int32)), out=dev.zeros(n + 2, np.int32))
+    work = dev.alloc(dev.attn_tree_work_bytes(n, nkv, nkv, hd))
+    dev.attn_tree(AttnArgs(n=n, nh=nkv, nkv=nkv, hd=hd, max_ctx=ctx, q=i["q"].ptr, scale=np.float32(scale), kc=caches[0].ptr,
+                           vc=caches[1].ptr, pos=i["pos"].ptr, o=i["o"].ptr, a8=A8(None, None, None), kv_dtype=kv), i["parent"], work)
+    dev.sync()
+    got = i["o"].numpy().reshape(n, nkv, hd)
+    assert np.abs(got - want).max() <= tol, (np.abs(got - want).max(), tol)
+    dev.tree_commit(tree_commit_args(n, i["parent"], i["tok"], i["choice"], i["out"],
+                                     kv=dict(caches=caches, nkv=nkv, max_ctx=ctx, hd=hd, kv_dtype=kv, pos=i["pos"])))
+    dev.sync()
+    assert i["out"].numpy().tolist() == [1, 8, 0, 2, -1]
+    for b in caches:
+        for g in range(nkv):
+            for s in (*slots[:4], pos + 1, pos + 2):
+                codes, sc = (x if x is None else np.empty_like(x) for x in rows[b.ptr, g, s])
+                move(b, g, s, codes, sc, False)
+                for x, y in zip((codes, sc), rows[b.ptr, g, pos + 2 if s == pos + 1 else s]):
+                    assert x is None or np.array_equal(x, y), (g, s)
+    for b in (*caches, work, *i.values()):
+        b.free()

@@ -87,6 +87,38 @@ __device__ __forceinline__ int lane_id() {
 }
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
+/* v of this lane and of those 16, 32 and 48 on, combined by f, in all four: exchanges of rows of lanes
+ * between two registers, not through LDS */
+template <typename F>
+__device__ __forceinline__ float over_quarters(float v, F f) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const uint32_t y = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float max_quarters(float v) {
+    return over_quarters(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_quarters(float v) {
+    return over_quarters(v, [](float a, float b) { return a + b; });
+}
+/* the largest of W neighbouring lanes, in each of them (W a power of two) */
+template <int W>
+__device__ __forceinline__ float max_lanes(float v) {
+    auto with = [&](int o) { v = fmaxf(v, __int_as_float(o)); };
+    if (W >= 2) with(nmx_dpp<NMX_DPP_XOR1>(__float_as_int(v)));
+    if (W >= 4) with(nmx_dpp<NMX_DPP_XOR2>(__float_as_int(v)));
+    if (W >= 8) with(nmx_dpp<NMX_DPP_HALF_MIRROR>(__float_as_int(v)));
+    if (W >= 16) with(nmx_dpp<NMX_DPP_MIRROR>(__float_as_int(v)));
+    if (W == 64) return max_quarters(v);
+    if (W == 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    return v;
+}
+
 __device__ __forceinline__ float4v mfma16(half8 a, half8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -226,19 +258,17 @@ __device__ __forceinline__ void split2(float a, float b, half8 &h, half8 &r, int
  * cache's first rows have been requested too. Columns past hd are zeros. */
 template <int KS>
 struct QueryRow {
-    static constexpr int HELD = KS <= 8 ? KS : 1; /* a longer row is read again instead of held */
     const float *qp;
     bool live;
     int hd, gq;
-    float4 x[HELD][2];
+    float4 x[KS][2];
     __device__ __forceinline__ void get(int k) {
         const int col = k * 32 + gq * 8, at = live && col < hd ? col : 0; /* qp is in bounds for every lane */
-        x[k % HELD][0] = *(const float4 *)(qp + at), x[k % HELD][1] = *(const float4 *)(qp + at + 4);
+        x[k][0] = *(const float4 *)(qp + at), x[k][1] = *(const float4 *)(qp + at + 4);
     }
     __device__ __forceinline__ QueryRow(const float *qp, bool live, int hd, int gq) : qp(qp), live(live), hd(hd), gq(gq) {
-        if constexpr (HELD == KS)
 #pragma unroll
-            for (int k = 0; k < KS; k++) get(k);
+        for (int k = 0; k < KS; k++) get(k);
     }
     /* the parts; the result is the factor that turns a product of parts into a score in powers of two */
     __device__ __forceinline__ float split(float scale, half8 (&qh)[KS], half8 (&ql)[KS]) {
@@ -246,20 +276,17 @@ struct QueryRow {
         auto in = [&](int k) { return live && k * 32 + gq * 8 < hd; };
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            if (HELD < KS) get(k);
-            float4(&y)[2] = x[k % HELD];
+            float4(&y)[2] = x[k];
             float b = fmaxf(fmaxf(fmaxf(fabsf(y[0].x), fabsf(y[0].y)), fmaxf(fabsf(y[0].z), fabsf(y[0].w))),
                             fmaxf(fmaxf(fabsf(y[1].x), fabsf(y[1].y)), fmaxf(fabsf(y[1].z), fabsf(y[1].w))));
             am = fmaxf(am, in(k) ? b : 0.0f);
         }
-        am = fmaxf(am, __shfl_xor(am, 16));
-        am = fmaxf(am, __shfl_xor(am, 32));
+        am = max_quarters(am);
         const int e = row_exp(am);
         const float up = pow2f(12 - e);
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            if (HELD < KS) get(k);
-            float4(&y)[2] = x[k % HELD];
+            float4(&y)[2] = x[k];
             const float z[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
             split8(z, up, qh[k], ql[k]);
             if (!in(k)) qh[k] = ql[k] = half8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -292,16 +319,14 @@ __device__ __forceinline__ void add_tile(Running<OD / 16> &r, const float (&x)[8
     float mx = x[0];
 #pragma unroll
     for (int i = 1; i < 8; i++) mx = fmaxf(mx, x[i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(r.m, fmaxf(mx, __shfl_xor(mx, 32)));
+    mx = fmaxf(r.m, max_quarters(mx));
     const float ref = mx == -INFINITY ? 0.0f : mx;
     int ve = 0;
     if constexpr (KVT != KV_F16) { /* the largest of score + exponent, above the largest score, rounded up */
         float t = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; i++) t = fmaxf(t, (x[i] - ref) + (float)e[i]);
-        t = fmaxf(t, __shfl_xor(t, 16));
-        t = fmaxf(t, __shfl_xor(t, 32));
+        t = max_quarters(t);
         /* the old values' bound moves with the maximum */
         t = fmaxf(t, (r.m - ref) + (float)r.ve);
         ve = (int)ceilf(fmaxf(t, -500.0f));
@@ -432,10 +457,8 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
                 *(half8 *)(tk + at) = codes8(rk[u].a);
                 if (ch == 0) kf[p] = sk[u];
             } else {
-                float am = amax8(rk[u]), x[8];
-#pragma unroll
-                for (int w = 1; w < KC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
-                const int e = row_exp(am);
+                float x[8];
+                const int e = row_exp(max_lanes<KC>(amax8(rk[u])));
                 half8 h, r;
                 floats8(rk[u], x);
                 split8(x, pow2f(12 - e), h, r);
@@ -462,10 +485,8 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
                     ve[p] = e, vf[p] = sv[u] * pow2f(-e);
                 }
             } else {
-                float am = amax8(rv[u]), x[8];
-#pragma unroll
-                for (int w = 1; w < VC; w <<= 1) am = fmaxf(am, __shfl_xor(am, w));
-                const int e = row_exp(am);
+                float x[8];
+                const int e = row_exp(max_lanes<VC>(amax8(rv[u])));
                 half8 h, r;
                 floats8(rv[u], x);
                 split8(x, pow2f(12 - e), h, r);
@@ -532,8 +553,7 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
         if (NB == 2) buf ^= 1;
     }
     r.l -= r.lc;
-    r.l += __shfl_xor(r.l, 16);
-    r.l += __shfl_xor(r.l, 32);
+    r.l = sum_quarters(r.l);
     if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);
 }
 

@@ -16,9 +16,9 @@
  * two parts itself: three products, the low-low one left out (2^-22 of the row).
  *
  * Times of both kernels (context + join) on MI355X, 8 heads on 2 of 256: 64 nodes over 100000 binary16
- * positions 124 us (110 + 14), 423 TFLOP/s of the definition's products and twice that of the matrix
- * cores', which a large binary16 product runs at 1068; 37 nodes over 4001 int8 26.1 us (17.8 + 9.4);
- * 9 nodes over 600 fp32 17.0 us (10.9 + 6.1) and one node over 20000 binary16 17.9 us (12 + 6.1): the
+ * positions 126 us (112 + 14), 415 TFLOP/s of the definition's products and twice that of the matrix
+ * cores', which a large binary16 product runs at 1068; 37 nodes over 4001 int8 25.9 us (17 + 8.8);
+ * 9 nodes over 600 fp32 16.4 us (10.7 + 5.7) and one node over 20000 binary16 17.6 us (12 + 5.6): the
  * latter 41 MB, 8 us as a copy; the others are chains of round trips to memory (position, rows, barrier,
  * parts, position, parts, rows). */
 #include "nmx_internal.h"
@@ -117,6 +117,14 @@ __device__ __forceinline__ float max_lanes(float v) {
         v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
     }
     return v;
+}
+/* the sum over a wave, in each lane */
+__device__ __forceinline__ float sum_lanes(float v) {
+    v += __int_as_float(nmx_dpp<NMX_DPP_XOR1>(__float_as_int(v)));
+    v += __int_as_float(nmx_dpp<NMX_DPP_XOR2>(__float_as_int(v)));
+    v += __int_as_float(nmx_dpp<NMX_DPP_HALF_MIRROR>(__float_as_int(v)));
+    v += __int_as_float(nmx_dpp<NMX_DPP_MIRROR>(__float_as_int(v)));
+    return sum_quarters(v);
 }
 
 __device__ __forceinline__ float4v mfma16(half8 a, half8 b, float4v c) {
@@ -390,7 +398,7 @@ __device__ __forceinline__ void store_part(const TreeAttn &a, const Running<DT> 
  * 512 columns of fp32, which have neither the registers nor the room). The same kernel serves few rows,
  * whose waves without rows only bring tiles: waves with tiles of their own, each staging for itself, took
  * as long over 20000 binary16 positions and much longer otherwise (5 nodes over 30000 fp32 positions 86
- * against 46 us, 2 over 16 int8 17 against 12). */
+ * against 41 us, 2 over 16 int8 17 against 12). */
 template <int HDP>
 constexpr int ctx_waves() {
     return HDP > 256 ? 4 : 8;
@@ -615,9 +623,7 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
                 else x = (float)*(const int8_t *)at * rs;
                 d = __builtin_fmaf(q[k], x, d);
             }
-#pragma unroll
-        for (int x = 32; x >= 1; x >>= 1) d += __shfl_xor(d, x);
-        d *= a.scale * AT_LOG2E;
+        d = sum_lanes(d) * (a.scale * AT_LOG2E);
         if (lane == 0) sc[i] = d;
         mt = fmaxf(mt, d);
     }
@@ -641,8 +647,7 @@ __global__ __launch_bounds__(JT) void attn_tree_join_k(TreeAttn a) {
         sc[tid] = w; /* no other thread reads it before the next barrier */
         l += w;
     }
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x);
+    l = sum_lanes(l);
     if (lane == 0) red[JT / 64 + wave] = l;
     nmx_lds_sync();
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

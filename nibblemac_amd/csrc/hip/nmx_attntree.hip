@@ -547,12 +547,18 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
             float x[8], f[8];
             int e[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) { /* position 16 (i / 4) + 4 gq + i % 4 */
-                const int p = 16 * (i >> 2) + 4 * gq + (i & 3);
-                float y = sc[i >> 2][i & 3];
-                if constexpr (KVT != KV_F16) y *= qfac * kf[p], e[i] = ve[p], f[i] = vf[p];
-                else y *= qfac, e[i] = 0, f[i] = 1.0f;
-                x[i] = pt + p < p1 ? y : -INFINITY;
+            for (int h = 0; h < 2; h++) { /* positions 16 h + 4 gq + j */
+                const int p = 16 * h + 4 * gq;
+                float4v k4{1.0f, 1.0f, 1.0f, 1.0f}, f4 = k4;
+                int4 e4 = make_int4(0, 0, 0, 0);
+                if constexpr (KVT != KV_F16) k4 = *(const float4v *)(kf + p), f4 = *(const float4v *)(vf + p), e4 = *(const int4 *)(ve + p);
+                const int ej[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float y = sc[h][j] * qfac;
+                    if constexpr (KVT != KV_F16) y *= k4[j];
+                    x[4 * h + j] = pt + p + j < p1 ? y : -INFINITY, f[4 * h + j] = f4[j], e[4 * h + j] = ej[j];
+                }
             }
             const _Float16 *const vb[4] = {tk + vo[0], tk + vo[1], tk + vo[2], tk + vo[3]};
             add_tile<OD, KVT>(r, x, e, f, vb, AT_P * OD);

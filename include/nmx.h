@@ -524,7 +524,9 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p);
  * The token is the first one in index order at which the running mass of the kept passes u times
  * their whole. prob (may be NULL) receives its share of the kept mass.
  * temperature <= 0 or NaN: the first maximum, prob 1. top_k <= 0 or >= vocab, top_p >= 1 or NaN,
- * min_p <= 0 or NaN: no such filter; top_p <= 0 keeps the first token, min_p >= 1 the maxima. u
+ * min_p <= 0 or NaN: no such filter; top_p <= 0 keeps the first token, min_p >= 1 those of the
+ * largest weight (the maxima, and what is so near to them that its w_i is 1 in 64 bits: at an
+ * infinite temperature every finite logit). u
  * below 0 or NaN counts as 0, from 1 on the last kept token is taken. A logit of -inf or NaN is
  * never chosen, +inf is the largest finite value; a row that has nothing else gives token -1 and
  * prob 0. Tokens 32 nats below the maximum of a filtered row have no mass (less than 2^-46 each).

@@ -509,15 +509,22 @@ __device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint
     return key;
 }
 
-/* The least logit whose weight is at least min_p of the largest: its key. */
+/* The least logit whose weight is at least min_p of the largest: its key. Weights grow with the key, so a
+ * wave cuts the span of keys that the border may lie in to a 64th at a time: 6 rounds for 32 bits, where
+ * weights are alike over millions of keys too (logits next to 0, a high temperature, min_p of 1). The
+ * upper end always holds a key that is in. */
 __device__ uint32_t min_p_key(float mx, double inv, double min_p) {
-    auto in = [&](float x) { return weight(x, mx, inv) >= min_p; };
-    uint32_t k = sample_key(sample_value((float)fmax((double)mx + 8.0 * log(min_p) / inv, -3.40282346638528859e+38)));
-    const uint32_t top = sample_key(mx), low = sample_key(-3.40282347e+38f);
-    if (k > top) k = top;
-    while (k < top && !in(sample_unkey(k))) k++;
-    while (k > low && in(sample_unkey(k - 1))) k--;
-    return k;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = sample_key(-3.40282347e+38f), hi = sample_key(mx);
+    for (int round = 0; lo < hi && round < 7; round++) {
+        const uint32_t step = (hi - lo + 63) >> 6;
+        const uint32_t k = lo + lane * step < hi ? lo + lane * step : hi;
+        const unsigned long long in = __ballot(k == hi || weight(sample_unkey(k), mx, inv) >= min_p);
+        const int f = in ? __ffsll((long long)in) - 1 : 64; /* the first key that is in */
+        if (f < 64) hi = lo + f * step < hi ? lo + f * step : hi;
+        if (f > 0) lo += (f - 1) * step + 1;
+    }
+    return hi;
 }
 
 /* A step of a bitonic network: this lane and lane ^ J, the greater with the lower one where up holds. J < 16
@@ -814,10 +821,8 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
             cut.key = key, cut.ties = ties;
         }
         if (p.min_p > 0.0) {
-            __syncthreads();
-            if (tid == 0) S.sel_n = min_p_key(mx, p.inv, p.min_p);
-            __syncthreads();
-            if (S.sel_n > cut.key) cut.key = S.sel_n, cut.ties = 0xffffffffu;
+            const uint32_t key = min_p_key(mx, p.inv, p.min_p); /* the same of every wave */
+            if (key > cut.key) cut.key = key, cut.ties = 0xffffffffu;
         }
         /* the kept mass of each chunk: whole bins, then the members of the cut's own bin */
         const double d = cut.key ? top - floor(grid_pos(sample_unkey(cut.key), p.inv)) : (double)SM_BINS;

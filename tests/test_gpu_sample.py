@@ -257,3 +257,42 @@ def test_refusals(dev):
             dev.sample(**{**good, **bad})
     dev.sync()
     assert not tok.numpy().any() and not work.numpy().any()
+
+
+MIN_P_ROWS = [  # T, min_p, the maximum
+    (1.0, 1.0, 0.0), (1.0, 1.0, 1.5), (np.inf, 1.0, 1.5), (np.inf, 0.5, -2.0), (1e17, 1.0, 10.0), (1e17, 3.0, 0.0), (1e30, 0.5, 3.0),
+    (1.0, float(np.exp(-1)), 1.0), (1.0, 0.5, float(np.log(2))), (2.0, 0.3, 0.0), (0.7, 0.999, 0.0), (1.0, 1.0, 3.4e38),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["zeros", "zeros_of_both_signs", "next_to_zero", "tiny", "spread"])
+def test_min_p_border_over_many_tokens(dev, kind):
+    """More tokens than are decided among themselves, min-p alone and beside the other filters, where the
+    border lies among logits next to 0 (floats are dense there), or the weights are alike over billions
+    of floats (a high temperature, a min_p of 1 or more). No weight lies within 2^-40 of min_p of the
+    border: a kernel's weight is right to 2^-43."""
+    print(f"[case] sample min_p border {kind}", flush=True)
+    rng = np.random.default_rng(len(kind))
+    vocab = CHUNK + 3000
+    par = np.concatenate([records(1, T=T, min_p=m, **f) for T, m, _ in MIN_P_ROWS for f in (dict(), dict(top_k=5000), dict(top_p=0.97))])
+    n = len(par)
+    l = np.zeros((n, vocab), np.float32)
+    if kind == "zeros_of_both_signs":
+        l = np.where(rng.random((n, vocab)) < 0.5, np.float32(-0.0), np.float32(0.0))
+    elif kind == "next_to_zero":
+        l = (10.0 ** rng.uniform(-12, -2, (n, vocab)) * rng.choice([-1, 1], (n, vocab))).astype(np.float32)
+    elif kind == "tiny":    # down to the subnormals: all of one weight
+        l = (10.0 ** rng.uniform(-44, -20, (n, vocab)) * rng.choice([-1, 1], (n, vocab))).astype(np.float32)
+    elif kind == "spread":
+        l = (rng.standard_normal((n, vocab)) * 0.3).astype(np.float32)
+    if not kind.startswith("zeros"):
+        l = np.minimum(l, np.repeat([m for _, _, m in MIN_P_ROWS], 3)[:, None]).astype(np.float32)
+    l[np.arange(n), rng.integers(0, vocab, n)] = np.repeat([m for _, _, m in MIN_P_ROWS], 3)
+    for r in range(n):
+        x, m = l[r].astype(np.float64), float(par["min_p"][r])
+        T = float(par["temperature"][r])
+        w = np.exp((x - x.max()) / T) if T < np.inf else np.ones(vocab)
+        near = np.abs(w / min(m, 1.0) - 1)
+        assert not ((near < 2.0 ** -40) & (near > 0) & (m < 1)).any()
+    check(dev, l, par, rng.random(n, np.float32))

@@ -87,21 +87,8 @@ __device__ __forceinline__ int lane_id() {
 }
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
-/* v of this lane and of those 16, 32 and 48 on, combined by f, in all four: exchanges of rows of lanes
- * between two registers, not through LDS */
-template <typename F>
-__device__ __forceinline__ float over_quarters(float v, F f) {
-    const uint32_t x = __float_as_uint(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    const uint32_t y = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
-    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
-    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
 __device__ __forceinline__ float max_quarters(float v) {
-    return over_quarters(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float sum_quarters(float v) {
-    return over_quarters(v, [](float a, float b) { return a + b; });
+    return nmx_over_quarters(v, [](float a, float b) { return fmaxf(a, b); });
 }
 /* the largest of W neighbouring lanes, in each of them (W a power of two) */
 template <int W>
@@ -124,7 +111,7 @@ __device__ __forceinline__ float sum_lanes(float v) {
     v += __int_as_float(nmx_dpp<NMX_DPP_XOR2>(__float_as_int(v)));
     v += __int_as_float(nmx_dpp<NMX_DPP_HALF_MIRROR>(__float_as_int(v)));
     v += __int_as_float(nmx_dpp<NMX_DPP_MIRROR>(__float_as_int(v)));
-    return sum_quarters(v);
+    return nmx_sum_quarters(v);
 }
 
 __device__ __forceinline__ float4v mfma16(half8 a, half8 b, float4v c) {
@@ -567,7 +554,7 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_tree_ctx_k(TreeAtt
         if (NB == 2) buf ^= 1;
     }
     r.l -= r.lc;
-    r.l = sum_quarters(r.l);
+    r.l = nmx_sum_quarters(r.l);
     if (hrow >= 0) store_part(a, r, s, hrow, d0, gq);
 }
 

@@ -89,6 +89,20 @@ __device__ __forceinline__ V nmx_scan_wave(V v) {
     return v;
 }
 
+/* v of this lane and of those 16, 32 and 48 on, combined by f, in all four (every lane active): exchanges of
+ * rows of lanes between two registers, not through LDS */
+template <typename F>
+__device__ __forceinline__ float nmx_over_quarters(float v, F f) {
+    const uint32_t x = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const uint32_t y = __float_as_uint(f(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float nmx_sum_quarters(float v) {
+    return nmx_over_quarters(v, [](float a, float b) { return a + b; });
+}
+
 /* Maximum of a float over the wave (every lane active; exact in any order), returned to
  * every lane: nmx_max32 within each half, then the halves through readlane. */
 __device__ __forceinline__ float nmx_max_f32_wave(float v) {

@@ -167,7 +167,6 @@ struct TreeRule {
     const float *pend;
     int keep;
     const int32_t *keep_dev, *parent;
-    float qscale;
 };
 
 constexpr int TR_B = 8; /* pending rows staged at a time */
@@ -205,13 +204,13 @@ __device__ __forceinline__ void tree_tables(TreeTables &s, int n, unsigned long 
     if (lane == 0) s.levels = deep + 1;
 }
 
-/* Rows of k and q for the products of nodes: an element, brought to norm 2^12 (k has norm 1, q norm
- * qscale), as its nearest whole number and the rest, both binary16. Products of whole numbers add up
- * to no more than 2^24: exact in the accumulator. The products of a whole number and a rest are 2^-12 of that
- * and have an accumulator of their own: beside a larger sum the matrix instruction drops what lies below
- * 2^-26 of it from every product, which was the largest error of o where q.k nearly cancels. The products
- * of two rests, random and 2^-24, are left out. Three 16-bit instructions per 32 keys in place of 32
- * 32-bit ones. */
+/* Rows of k and q for the products of nodes: a row is brought to a norm about 2^12 by a power of two of its
+ * own (the norm's epsilon leaves small conv rows far below 1), an element then taken as its nearest
+ * whole number and the rest, both binary16. Products of whole numbers add up to no more than about 2^24: exact in
+ * the accumulator. The products of a whole number and a rest are 2^-12 of that and have an accumulator of
+ * their own: beside a larger sum the matrix instruction drops what lies below 2^-26 of it from every
+ * product, which was the largest error of o where q.k nearly cancels. The products of two rests, random
+ * and 2^-24, are left out. Three 16-bit instructions per 32 keys in place of 32 32-bit ones. */
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
@@ -224,7 +223,22 @@ __device__ __forceinline__ void split4(float4 x, float up, _Float16 *hi, _Float1
     for (int i = 0; i < 4; i++) h[i] = (_Float16)rintf(v[i]), l[i] = (_Float16)(v[i] - (float)h[i]);
     *(half4 *)hi = h, *(half4 *)lo = l;
 }
-constexpr float TR_UP = 4096.0f;
+__device__ __forceinline__ float sum_squares(const float4 *x, int n) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < n; i++) {
+        s.x = __builtin_fmaf(x[i].x, x[i].x, s.x), s.y = __builtin_fmaf(x[i].y, x[i].y, s.y);
+        s.z = __builtin_fmaf(x[i].z, x[i].z, s.z), s.w = __builtin_fmaf(x[i].w, x[i].w, s.w);
+    }
+    return nmx_sum_quarters((s.x + s.y) + (s.z + s.w));
+}
+/* The power of two that a row scaled for its products is brought back by, from its sum of squares: 2^(e - 12)
+ * for the least e with ss < 2^(2 e), e from -63 on (below, a product has no 32-bit value either) up to 65. */
+__device__ __forceinline__ float row_down(float ss) {
+    const int e = ((int)(__float_as_uint(ss) >> 23 & 255) - 125) >> 1;
+    return __uint_as_float((uint32_t)(e - 12 + 127) << 23);
+}
+__device__ __forceinline__ float inverse_pow2(float x) { return __uint_as_float(0x7f000000u - __float_as_uint(x)); }
 
 /* The pending rows of head h, TR_B at a time: keys and decays to LDS (pk, pdec), the deltas of column
  * col to registers. The first batch is requested at the kernel's entry, among its other requests. */
@@ -297,6 +311,7 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
     extern __shared__ float4 smem4[];
     __shared__ TreeTables tt;
     __shared__ float del[2][NMX_TREE_MAX][16], pdec[TR_B];
+    __shared__ float2 down[NMX_TREE_MAX]; /* of a node's k and q: what their scaled products are multiplied by */
     const int h = blockIdx.x, j0 = blockIdx.y * 16, tid = threadIdx.x, lane = tid & 63, T = tid >> 6, waves = (int)(blockDim.x >> 6) - tree_wave<DK4>();
     const int c = lane & 15, gq = lane >> 4, n = a.n, heads = a.heads, dv = a.dv, n16 = 16 * waves;
     _Float16 *kh2 = (_Float16 *)smem4, *qh2 = kh2 + 2 * n16 * HS;   /* [2][n16][HS]: high, low parts */
@@ -332,13 +347,18 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
         dc = lane < n ? a.decay[lane * heads + h] : 1.0f, bt1 = lane < n ? a.beta[lane * heads + h] : 0.0f;
         set = tree_ancestors(a.parent, n, &up);
     }
-    const float q_up = a.qscale != 0.0f ? TR_UP / a.qscale : 0.0f, q_down = a.qscale / (TR_UP * TR_UP);
+    if (nodes) {
+        /* a little less than the squares: a norm of 1, give or take a rounding, stays 2^12; half of q's, whose
+         * norm of dk^-1/2 then goes to 2^12 or 2^12.5 */
+        const float kdown = row_down(sum_squares(kf, NS) * 0.998f), qdown = row_down(sum_squares(qf, NS) * 0.499f);
+        const float k_up = inverse_pow2(kdown), q_up = inverse_pow2(qdown);
+        if (gq == 0) down[tn] = make_float2(kdown, qdown);
 #pragma unroll
-    for (int k = 0; k < NS; k++) {
-        if (!nodes) continue;
-        const int at = tn * HS + gq * DK4 + 4 * k;
-        split4(kf[k], TR_UP, kh2 + at, kh2 + n16 * HS + at);
-        if (QL) split4(qf[k], q_up, qh2 + at, qh2 + n16 * HS + at);
+        for (int k = 0; k < NS; k++) {
+            const int at = tn * HS + gq * DK4 + 4 * k;
+            split4(kf[k], k_up, kh2 + at, kh2 + n16 * HS + at);
+            if (QL) split4(qf[k], q_up, qh2 + at, qh2 + n16 * HS + at);
+        }
     }
     const int keep = keep_of(a.keep, a.keep_dev);
     rp.run(s, a.pend, a.keep, keep, heads, h, logw, j0 + c, pk, pdec, nodes);
@@ -369,6 +389,7 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
             const int U = job, an = 16 * U + c;
             const _Float16 *ar = kh2 + an * HS + 8 * gq, *tr = kh2 + (16 * X + c) * HS + 8 * gq, *ur = qh2 + (16 * X + c) * HS + 8 * gq;
             const int lo = n16 * HS;
+            const float q_up = QL ? 0.0f : inverse_pow2(down[16 * X + c].y);
             f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x, xr = x, yr = x;
 #pragma unroll
             for (int k = 0; k < DK; k += 32) {
@@ -392,12 +413,14 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
             }
             x += xr, y += yr;
             const int dp = tt.depth[an];
+            const float down_a = down[an].x;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int t = 16 * X + 4 * gq + j;
                 if (t >= n || !(tt.sets[t] >> an & 1)) continue;
-                const float d = tt.gap[t][dp];
-                co[t * (n16 + 1) + dp] = make_float2(x[j] * (d * (1.0f / (TR_UP * TR_UP))), y[j] * (d * q_down));
+                const float d = tt.gap[t][dp] * down_a;
+                const float2 dt = down[t];
+                co[t * (n16 + 1) + dp] = make_float2(x[j] * dt.x * d, y[j] * dt.y * d);
             }
         }
     }
@@ -539,7 +562,7 @@ int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *m, const int32_t *par
     const TreePre a{n, p.C, p.conv_k, dk, p.kd, p.raw, p.raw_stride, p.out, p.state, p.conv_w, p.xin, p.qscale, p.l2eps,
                     p.b_in, p.a_in, p.g_stride, heads, p.A_log, p.A, p.dt_bias, p.beta, p.decay, parent};
     const TreeRule t{n, heads, r.rep, dv, p.kd, p.C, p.out, p.beta, p.decay, r.S, r.o, r.o_stride, r.log, r.pend, r.keep,
-                     r.keep_dev, parent, p.qscale};
+                     r.keep_dev, parent};
     const dim3 grid((unsigned)((p.C + dk - 1) / dk + 1), (unsigned)((n + TP_N - 1) / TP_N));
     const unsigned threads = dk < 64 ? 64 : (unsigned)dk;
     const size_t lds = (size_t)TP_N * (dk + 4) * 4;

@@ -289,3 +289,89 @@ def test_refusals(dev):
     for k, v in r.b.items():
         assert_bits_equal(v.numpy(), before[k], k)
     r.free()
+
+
+def bounded(cv, beta, decay, S0, parent, heads, rep, dk, dv, kd, rests=True):
+    """o and delta [n][heads][dv] in 64 bits, as sums over a node's ancestors, and what each element may be
+    off by. u = 2^-24. A product of a row with the state is dk / 8 chained instructions of 4 terms in each of
+    two chains, each off by at most two roundings of its sum: (dk / 4 + 2) u of the sum of magnitudes. A
+    product of nodes: rows scaled to a norm of at least 2^11 (q 2^11.5), an element as a whole number of 11
+    bits and a rest of at most 1/2 + 2^-11 of the element in 11 bits, so with s = sqrt(dk) / 2 the rests
+    have a norm of at most s + 1 for every 2^11 of the row's: without the products of two rests it is
+    off by ((s + 1)^2 + 2 (s + 1) + 1) 2^-22 of the norms' product. A factor of decays has one rounding a level; every
+    product and sum one more. rests False: the same sums with the rests left out (a mistake to be noticed)."""
+    n, u = len(parent), 2.0 ** -24
+    q = cv[:, :kd].reshape(n, -1, dk).astype(np.float64).repeat(rep, 1)
+    k = cv[:, kd:2 * kd].reshape(n, -1, dk).astype(np.float64).repeat(rep, 1)
+    v = cv[:, 2 * kd:].reshape(n, heads, dv).astype(np.float64)
+    nq, nk = np.linalg.norm(q, axis=2), np.linalg.norm(k, axis=2)
+    qq, kk = q, k
+    if not rests:
+        up = lambda x, nx: 2.0 ** (11 - np.floor(np.log2(np.maximum(nx, 1e-300))))[..., None]  # noqa: E731
+        qq, kk = (np.rint(x * up(x, nx)) / up(x, nx) for x, nx in ((q, nq), (k, nk)))
+    KK, QK = (np.einsum("thd,ahd->tah", x, kk) for x in (kk, qq))
+    s = np.sqrt(dk) / 2
+    eta = ((s + 1) ** 2 + 2 * (s + 1) + 1) * 2.0 ** -22
+    o, d, eo, ed = (np.zeros((n, heads, dv)) for _ in range(4))
+    for t in range(n):
+        g, D, a, path = np.ones(heads), {}, t, []
+        while a >= 0:
+            D[a] = g
+            path.append(a)
+            g = g * decay[a]
+            a = parent[a] if 0 <= parent[a] < a else -1
+        L = len(path)
+        state = ((dk / 4 + 2) + (L + 2)) * u
+        for x, out, err, prod, nx in ((k, d, ed, KK, nk), (q, o, eo, QK, nq)):
+            first = x is k
+            S = g[:, None] * (S0 @ x[t][:, :, None])[..., 0]
+            val, mag = (v[t] - S, np.abs(v[t]) + np.abs(S)) if first else (S, np.abs(S))
+            e = state * g[:, None] * (np.abs(S0) @ np.abs(x[t])[:, :, None])[..., 0]
+            for b in (path[1:] if first else path):
+                c = (D[b] * prod[t, b])[:, None]
+                val = val + (-c if first else c) * d[b]
+                mag = mag + np.abs(c * d[b])
+                e = e + (D[b] * (eta * nx[t] * nk[b] + (L + 4) * u * np.abs(prod[t, b])))[:, None] * np.abs(d[b]) + np.abs(c) * ed[b]
+            e = e + (L + 1) * u * mag
+            w = beta[t].astype(np.float64)[:, None] if first else 1.0
+            out[t], err[t] = val * w, (e * w + u * np.abs(val * w)) * 1.001 + 1e-40
+    return o, d, eo, ed
+
+
+def bushes(rng, n):
+    """Roots at nodes 0, 16, 32, 48, every other node below one of those before it: pairs in every block
+    of 16 x 16 nodes, no depth to hide in."""
+    return np.array([-1 if t % 16 == 0 else 16 * rng.integers(0, t // 16 + 1) for t in range(n)], np.int32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["chain", "bushes"])
+@pytest.mark.parametrize("scale", [1.0, 1e-3, 1e-4, 1e-5, 1e-6, 1e-8, 1e-12])
+@pytest.mark.parametrize("dk", [32, 64, 128, 256])
+def test_small_keys_and_queries(dev, dk, scale, kind):
+    """Conv rows of q and k small against the norm's epsilon keep norms far below 1 (1e-6 normalises to
+    1e-3): products of nodes are right relative to their rows, whatever those measure. The state is zero,
+    so o is nothing but such products."""
+    print(f"[case] lin tree small rows dk={dk} scale={scale} {kind}", flush=True)
+    rng = np.random.default_rng(dk)
+    n, heads, dv = (9, 2, 64) if kind == "chain" else (64, 2, 64)
+    parent = tree(rng, n, "chain") if kind == "chain" else bushes(rng, n)
+    host = make(rng, n, heads, 1, dk, dv, 4, 0)
+    kd = heads * dk
+    host["rec"][:] = 0
+    host["b"][:] = 2
+    for x in (host["raw"], host["conv"]):
+        x[:, :2 * kd] *= np.float32(scale)
+    host["raw"][n // 2, :kd] *= np.float32(1e-3)     # one query and one key smaller than the others
+    host["raw"][n // 3, kd:2 * kd] *= np.float32(1e-2)
+    r = Run(dev, host, n, heads, 1, dk, dv, 4, 0)
+    got = r(parent)
+    r.free()
+    args = (got["cv"], got["beta"], got["decay"], np.zeros((heads, dv, dk)), parent, heads, 1, dk, dv, kd)
+    o, d, eo, ed = bounded(*args)
+    assert eo.max() <= 1e-3 * np.abs(o).max() and ed.max() <= 1e-3 * np.abs(d).max()
+    off = bounded(*args, rests=False)
+    assert (np.abs(off[0] - o) > eo).any()      # the bound would notice the rests
+    err, errd = np.abs(got["o"].reshape(o.shape) - o), np.abs(got["log"][:n, :, dk:dk + dv] - d)
+    assert (err <= eo).all(), (err.max(), (err / eo).max(), np.abs(o).max())
+    assert (errd <= ed).all(), (errd.max(), (errd / ed).max())

@@ -71,11 +71,12 @@ __device__ __forceinline__ int part_len(const TreeAttn &a, int len) {
     return (per + AT_P - 1) / AT_P * AT_P;
 }
 
-/* Exponent e with |x| < 2^e for the largest |x| of a row (0 for a row of zeros), clamped so that
- * 2^(12 - e) and 2^(e - 12) are finite; bits of anything not finite give the upper end. */
+/* Exponent e with |x| < 2^e for the largest |x| of a row, clamped so that 2^(12 - e) and 2^(e - 12) are
+ * finite; bits of anything not finite give the upper end. A row of zeros has the lower end: of the value
+ * rows of a tile the weights follow the largest, which a row of zeros must not be. */
 __device__ __forceinline__ int row_exp(float amax) {
     const int e = (int)(__float_as_uint(amax) >> 23) - 126;
-    return amax == 0.0f ? 0 : e < -100 ? -100 : e > 128 ? 128 : e;
+    return e < -100 ? -100 : e > 128 ? 128 : e;
 }
 __device__ __forceinline__ float pow2f(int e) { /* -149 < e < 128 */
     return e > -127 ? __uint_as_float((uint32_t)(e + 127) << 23) : ldexpf(1.0f, e);

@@ -476,3 +476,28 @@ def test_offsets_past_32_bits(dev, kv, nkv, hd):
                     assert x is None or np.array_equal(x, y), (g, s)
     for b in (*caches, work, *i.values()):
         b.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_I8])
+@pytest.mark.parametrize("n,nh,nkv,hd,pos", [(1, 2, 1, 64, 400), (6, 4, 2, 128, 400), (40, 4, 1, 256, 70), (5, 2, 1, 512, 9000)])
+def test_zero_value_rows_beside_small_ones(dev, kv, n, nh, nkv, hd, pos):
+    """Value rows of zeros (an int8 row's scale is 0) at the highest scores, the others small: a row of
+    zeros says nothing about the magnitude of the rest."""
+    print(f"[case] attn tree zero values n={n} hd={hd} kv={kv}", flush=True)
+    for vstd in (1e-2, 1e-4, 1e-8, 1e-16, 1e-30):
+        rng = np.random.default_rng(n + hd)
+        shape = (n, nh, nkv, hd, pos + n)
+        q = rng.standard_normal((n, nh, 2 * hd)).astype(np.float32)
+        parent = tree(rng, n, "random")
+        kc, K = make_cache(rng, kv, nkv, pos + n, hd)
+        rows = (rng.standard_normal((nkv, pos + n, hd)) * vstd).astype(np.float32)
+        for g in range(nkv):    # a third of the rows, the highest score of every query row among them
+            s = q[:, g * (nh // nkv):(g + 1) * (nh // nkv), :hd].reshape(-1, hd) @ K[g].T.astype(np.float32)
+            rows[g, s.argmax(1)] = 0
+            rows[g, rng.random(pos + n) < 0.3] = 0
+        vc, V = encode(rows, kv)
+        want, tol = reference(q, K, V, parent, pos, shape)
+        assert tol < 1e-3 * np.abs(V).max()
+        got = run(dev, q, kc, vc, parent, pos, shape, kv)
+        assert np.abs(got - want).max() <= tol, (vstd, np.abs(got - want).max(), tol)

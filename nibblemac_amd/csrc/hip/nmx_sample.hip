@@ -882,7 +882,8 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
     }
     /* the chunk that the draw falls into */
     double whole;
-    const double to = block_scan(mass, S.red1, &whole), goal = ud * whole;
+    const double to = block_scan(mass, S.red1, &whole);
+    const double goal = ud < 1.0 ? ud * whole : INFINITY; /* from 1 on: past every sum, however it was rounded */
     const bool some = mass > 1e-296; /* so that one of its slices has 1e-297, and one logit a weight of 1e-300 */
     int c, c_last;
     block_find(some && to > goal, some, S.red1, S.red2, &c, &c_last);

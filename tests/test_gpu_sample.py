@@ -296,3 +296,23 @@ def test_min_p_border_over_many_tokens(dev, kind):
         near = np.abs(w / min(m, 1.0) - 1)
         assert not ((near < 2.0 ** -40) & (near > 0) & (m < 1)).any()
     check(dev, l, par, rng.random(n, np.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("f", [dict(), dict(min_p=1e-12), dict(top_p=0.999999), dict(top_k=9000), dict(top_k=9000, top_p=0.999999)],
+                         ids=lambda f: "_".join(f) or "none")
+def test_from_one_on_the_last_token(dev, f):
+    """u of 1 and more takes the last kept token, however little it weighs: the last ones of each row weigh
+    less than the roundings of the row's sums."""
+    print(f"[case] sample u = 1 {f}", flush=True)
+    rng = np.random.default_rng(9)
+    n, vocab = 64, 2 * CHUNK + 1000
+    l = rng.standard_normal((n, vocab)).astype(np.float32)
+    for r in range(n):
+        if f:       # within reach of a filter, one token behind the others
+            l[r, -1] = l[r].max() - (26 if "min_p" in f else 0.5)
+        else:
+            l[r, -700 if r % 2 else -2:] = l[r].max() - 45
+    par = records(1, **f)
+    u = np.where(np.arange(n) % 3, 1.0, 2.0).astype(np.float32)
+    check(dev, l, par, u)

@@ -91,6 +91,20 @@ __device__ __forceinline__ float sample_unkey(uint32_t k) {
 }
 
 __device__ __forceinline__ double grid_pos(float x, double inv) { return (double)x * inv; }
+/* How far x lies above the lower edge fl of its bin (g = grid_pos, fl = floor(g)). g is off by 2^-52 of
+ * itself, which from SM_FAR bins on would cost a weight more than 2^-43: there what the product and inv
+ * left out is added (the result may leave [0, 1) by that much). Past 2^33 bins neighbouring floats are more
+ * than 256 bins apart, and only equal logits are ever compared. */
+constexpr double SM_FAR = 4096.0;
+__device__ __forceinline__ bool grid_far(double top) { return !(top < SM_FAR && top - SM_BINS > -SM_FAR); }
+/* what the rounding of inv = 8 / T left out */
+__device__ __forceinline__ double grid_rest(float T, double inv) {
+    return T < INFINITY ? __builtin_fma(-inv, (double)T, 8.0) / (double)T : 0.0;
+}
+__device__ __forceinline__ double grid_above(float x, double inv, double inv2, double g, double fl) {
+    const double fr = g - fl, a = fabs(fl);
+    return a >= SM_FAR && a < 0x1p33 ? fr + __builtin_fma((double)x, inv2, __builtin_fma((double)x, inv, -g)) : fr;
+}
 
 /* e^z for z <= 0, right to 2^-43 (2^(k + f), |f| <= 1/2, by the Taylor polynomial of degree 10 of
  * e^(f ln 2): the next term is below 2.1e-13 2^-1; the reduced argument's error is |z| 2^-52). What
@@ -142,9 +156,9 @@ struct BinPoly { /* the coefficients, in scalars: a lane's fma takes one from th
     }
     __device__ __forceinline__ unsigned long long at(double fr) const { return bits(fr) & 0xfffffffffffffull; }
 };
-__device__ __forceinline__ unsigned long long bin_mass(float x, double inv) {
+__device__ __forceinline__ unsigned long long bin_mass(float x, double inv, double inv2) {
     const double g = grid_pos(x, inv);
-    return BinPoly().at(g - floor(g));
+    return BinPoly().at(grid_above(x, inv, inv2, g, floor(g)));
 }
 
 __device__ __forceinline__ float block_max(float v, float *red, int waves) {
@@ -278,15 +292,29 @@ __global__ __launch_bounds__(SM_T1, 8) void sample_scan_k(const float *__restric
     const uint32_t copy = (lane & (SM_COPY - 1)) * 8;
     const BinPoly poly;
     uint32_t at[SM_PER]; /* byte offset of a copy's word << 12 | rank in it; all ones: no weight */
-#pragma unroll
-    for (int u = 0; u < SM_PER; u++) {
+    auto add = [&](int u, double fl, double above) {
         at[u] = 0xffffffffu;
-        const double g = grid_pos(v[u], p.inv), fl = floor(g), d = base - fl; /* inf for -inf */
+        const double d = base - fl; /* inf for -inf */
         if (d < (double)SM_BINS) {
             const uint32_t j = (uint32_t)(int)d * (SM_COPY * 8) + copy;
             unsigned long long *w = (unsigned long long *)((char *)bins + j);
-            const unsigned long long old = atomicAdd(w, poly.bits(g - fl) - (0x432ull << 52));
+            const unsigned long long old = atomicAdd(w, poly.bits(above) - (0x432ull << 52));
             at[u] = __builtin_amdgcn_alignbit(j, (uint32_t)(old >> 32), 20);
+        }
+    };
+    /* no bin of the chunk as far as SM_FAR: nothing to add, and three instructions a logit fewer */
+    if (!__builtin_amdgcn_readfirstlane(grid_far(base))) {
+#pragma unroll
+        for (int u = 0; u < SM_PER; u++) {
+            const double g = grid_pos(v[u], p.inv), fl = floor(g);
+            add(u, fl, g - fl);
+        }
+    } else {
+        const double inv2 = grid_rest(par[(size_t)row * par_step].temperature, p.inv);
+#pragma unroll
+        for (int u = 0; u < SM_PER; u++) {
+            const double g = grid_pos(v[u], p.inv), fl = floor(g);
+            add(u, fl, grid_above(v[u], p.inv, inv2, g, fl));
         }
     }
     __syncthreads();
@@ -363,7 +391,7 @@ struct Row {
     const Chunk *ch;
     const float *l;
     int C;
-    double inv, top; /* top: the row's top bin */
+    double inv, inv2, top; /* top: the row's top bin */
 };
 
 /* Member i of those in hand (S.seg, S.at): its chunk, its index there, its logit. */
@@ -441,7 +469,7 @@ __device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint
             if (k < klo || k > khi) continue;
             const uint32_t d = (khi - k) >> shift;
             atomicAdd(&S.digit[d], 1u);
-            if (!by_count) atomicAdd(&S.tally[d], bin_mass(sample_unkey(k), r.inv));
+            if (!by_count) atomicAdd(&S.tally[d], bin_mass(sample_unkey(k), r.inv, r.inv2));
         }
         __syncthreads();
         const uint32_t n = S.digit[tid];
@@ -473,7 +501,7 @@ __device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint
         if (k < klo || k > khi) continue;
         const uint32_t at = atomicAdd(&S.sel_n, 1u);
         S.small[at] = k; /* at < left <= SM_RANK */
-        S.small_mass[at] = by_count ? 0 : bin_mass(sample_unkey(k), r.inv);
+        S.small_mass[at] = by_count ? 0 : bin_mass(sample_unkey(k), r.inv, r.inv2);
     }
     __syncthreads();
     const uint32_t N = S.sel_n;
@@ -706,7 +734,8 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
         if (tid < C && mc > -INFINITY) mass = bc * weight(mc, mx, p.inv);
     } else {
         const double g_top = grid_pos(mx, p.inv), top = floor(g_top);
-        const Row r = {ch, l, C, p.inv, top};
+        const double inv2 = grid_far(top) ? grid_rest(par[(size_t)row * par_step].temperature, p.inv) : 0.0;
+        const Row r = {ch, l, C, p.inv, inv2, top};
         if (tid < C) {
             const double d = mc > -INFINITY ? top - bc : (double)SM_BINS;
             S.off[tid] = d < (double)SM_BINS ? (int)d : SM_BINS;
@@ -742,7 +771,8 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
             __syncthreads();
         }
         const double edge = S.edge[b];
-        const double unit = exp_neg((top - g_top) * 0.125) * 0x1p-40; /* a mass of the top bin, as a weight */
+        /* a mass of the top bin, as a weight */
+        const double unit = exp_neg(grid_above(mx, p.inv, inv2, g_top, top) * -0.125) * 0x1p-40;
         /* a bin that the kept tokens do not reach below: of top-k's or top-p's end, of min-p's border (one
          * lower, for its rounding). Few tokens down to it: they decide among themselves */
         uint32_t n_all;
@@ -793,10 +823,10 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
                 unsigned long long kept = 0, whole;
                 for (uint32_t i = tid; i < S.seg[C]; i += SM_T2) {
                     const uint32_t key = key_of(S, r, i);
-                    if (key > cut.key) kept += bin_mass(sample_unkey(key), p.inv);
+                    if (key > cut.key) kept += bin_mass(sample_unkey(key), p.inv, inv2);
                 }
                 block_scan(kept, S.red1, &whole);
-                k_mass = (double)whole + (double)cut.ties * (double)bin_mass(sample_unkey(cut.key), p.inv);
+                k_mass = (double)whole + (double)cut.ties * (double)bin_mass(sample_unkey(cut.key), p.inv, inv2);
             }
         }
         int opened = kb;
@@ -815,7 +845,7 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
             uint32_t above;
             double m_above;
             const uint32_t key = select_key(S, r, pb, false, 0, rest, pb == kb ? cut.key : 0, &above, &m_above);
-            const double need = ceil((rest - m_above) / (double)bin_mass(sample_unkey(key), p.inv));
+            const double need = ceil((rest - m_above) / (double)bin_mass(sample_unkey(key), p.inv, inv2));
             uint32_t ties = need < 1.0 ? 1u : need < 4e9 ? (uint32_t)need : 0xffffffffu;
             if (pb == kb && key == cut.key && cut.ties < ties) ties = cut.ties;
             cut.key = key, cut.ties = ties;
@@ -839,7 +869,7 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
                     if (total <= SM_LIST) key = S.list[i];
                     else key = sample_key(sample_value(l[(size_t)c * SM_CHUNK + ch[c].perm[S.at[c] + (i - S.seg[c])]]));
                     n += key == cut.key;
-                    if (key > cut.key) m += bin_mass(sample_unkey(key), p.inv);
+                    if (key > cut.key) m += bin_mass(sample_unkey(key), p.inv, inv2);
                 }
                 n = nmx_scan_wave(n), m = nmx_scan_wave(m);
                 if (lane == 63) S.ties[c] = n, S.cand[c] = m;
@@ -874,7 +904,7 @@ __global__ __launch_bounds__(SM_T2) void sample_pick_k(const float *__restrict__
             mass = S.chunk_mass[tid];
             if (cb < SM_BINS) {
                 double m = (double)S.cand[tid];
-                if (ties) m += (double)ties * (double)bin_mass(sample_unkey(cut.key), p.inv);
+                if (ties) m += (double)ties * (double)bin_mass(sample_unkey(cut.key), p.inv, inv2);
                 mass += m * S.edge[cb];
             }
             mass *= unit;

@@ -316,3 +316,28 @@ def test_from_one_on_the_last_token(dev, f):
     par = records(1, **f)
     u = np.where(np.arange(n) % 3, 1.0, 2.0).astype(np.float32)
     check(dev, l, par, u)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset,T", [(1e4, 0.002), (-1e4, 0.002), (1e6, 0.2), (3e4, 0.01), (1e30, 2e23)])
+def test_logits_far_from_zero(dev, offset, T):
+    """Logits about an offset, many temperatures away from 0: the weights are those of the differences to
+    the maximum. Eight values, 700 tokens each; top-p ends 2^-38 to 2^-32.5 of the mass from a token's
+    end, where weights right to 2^-40 of themselves decide alike and ones of 2^-31 do not."""
+    print(f"[case] sample offset {offset} T={T}", flush=True)
+    rng = np.random.default_rng(12)
+    T = float(np.float32(T))
+    values = np.sort((np.float32(offset) + np.spacing(np.float32(offset)) * rng.permutation(12)[:8]).astype(np.float32))[::-1]
+    w = np.exp((values.astype(np.float64) - float(values[0])) / T)
+    assert len(set(values)) == 8 and w[-1] > 1e-4
+    ends = np.cumsum(np.repeat(w, 700)) / (700 * w.sum())
+    p = ends.astype(np.float32)
+    off = np.abs(p - ends)
+    p = p[(off > 2.0 ** -38) & (off < 2.0 ** -32.5) & (p < 1)]
+    assert len(p) >= 10
+    l = np.full((len(p), CHUNK + 500), values[-1] - np.float32(400 * T), np.float32)
+    l[:, 1000:6600] = np.repeat(values, 700)
+    par = records(len(p))
+    par["temperature"], par["top_p"] = T, p
+    check(dev, l, par, np.ones(len(p), np.float32))
+    check(dev, l, par, rng.random(len(p), np.float32))

@@ -539,17 +539,21 @@ int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *m, const int32_t *par
     if ((uintptr_t)p.out % 16 || (uintptr_t)r.S % 16)
         return nmx_fail(ctx, "nmx_lin_mix_tree: pre.out or the state not 16-byte aligned");
     /* what is written overlaps nothing else that is read or written */
-    const size_t logw = (size_t)dk + dv + 1, vd = (size_t)heads * dv;
+    const size_t logw = (size_t)dk + dv + 1, vd = (size_t)heads * dv, gb = (size_t)heads * 4;
     struct Range {
         const void *p;
         size_t bytes;
     };
-    const Range w[] = {{p.out, (size_t)n * p.C * 4}, {p.xin, p.xin ? (size_t)n * p.C * 4 : 0}, {p.beta, (size_t)n * heads * 4},
-                       {p.decay, (size_t)n * heads * 4}, {r.S, vd * dk * 4}, {r.o, ((size_t)(n - 1) * r.o_stride + vd) * 4},
-                       {r.log, (size_t)n * heads * logw * 4}, {m->y, m->y ? ((size_t)(n - 1) * m->y_stride + vd) * 4 : 0}};
+    const Range w[] = {{p.out, (size_t)n * p.C * 4}, {p.xin, p.xin ? (size_t)n * p.C * 4 : 0}, {p.beta, n * gb},
+                       {p.decay, n * gb}, {r.S, vd * dk * 4}, {r.o, ((size_t)(n - 1) * r.o_stride + vd) * 4},
+                       {r.log, n * gb * logw}, {m->y, m->y ? ((size_t)(n - 1) * m->y_stride + vd) * 4 : 0},
+                       {m->a8.q, m->a8.q ? n * vd : 0}, {m->a8.d, m->a8.q ? n * vd / 8 : 0}, {m->a8.fs, m->a8.q ? n * vd / 8 : 0}};
     const Range in[] = {{p.raw, ((size_t)(n - 1) * p.raw_stride + p.C) * 4}, {p.state, (size_t)(p.conv_k - 1) * p.C * 4},
-                        {r.pend, (size_t)r.keep * heads * logw * 4}, {m->z, ((size_t)(n - 1) * m->z_stride + vd) * 4},
-                        {p.b_in, ((size_t)(n - 1) * p.g_stride + heads) * 4}, {p.a_in, ((size_t)(n - 1) * p.g_stride + heads) * 4}};
+                        {p.conv_w, (size_t)p.C * p.conv_k * 4}, {r.pend, r.keep * gb * logw},
+                        {m->z, ((size_t)(n - 1) * m->z_stride + vd) * 4}, {m->norm_w, (size_t)dv * 4},
+                        {p.b_in, (size_t)(n - 1) * p.g_stride * 4 + gb}, {p.a_in, (size_t)(n - 1) * p.g_stride * 4 + gb},
+                        {p.A_log, p.A_log ? gb : 0}, {p.A, p.A ? gb : 0}, {p.dt_bias, gb}, {parent, (size_t)n * 4},
+                        {r.keep_dev, r.keep_dev ? sizeof(int32_t) : 0}};
     for (size_t i = 0; i < sizeof w / sizeof *w; i++) {
         for (const Range &x : in)
             if (nmx_overlap(w[i].p, w[i].bytes, x.p, x.bytes))

@@ -375,3 +375,41 @@ def test_small_keys_and_queries(dev, dk, scale, kind):
     err, errd = np.abs(got["o"].reshape(o.shape) - o), np.abs(got["log"][:n, :, dk:dk + dv] - d)
     assert (err <= eo).all(), (err.max(), (err / eo).max(), np.abs(o).max())
     assert (errd <= ed).all(), (errd.max(), (errd / ed).max())
+
+
+@pytest.mark.gpu
+def test_outputs_inside_other_inputs_are_refused(dev):
+    """Every written range against the tree, the weights, the gates' vectors, the device's keep and the A8."""
+    print("[case] lin tree overlaps", flush=True)
+    rng = np.random.default_rng(8)
+    n, heads, dk, dv = 4, 2, 64, 64
+    r = Run(dev, make(rng, n, heads, 1, dk, dv, 4, 2), n, heads, 1, dk, dv, 4, 2, keep_dev=1)
+    r.b["parent"] = par = dev.to_device(tree(rng, n, "chain"))
+    p = {k: v.ptr for k, v in r.b.items()}
+    before = {k: v.numpy() for k, v in r.b.items()}
+    a8 = r.args.a8
+
+    def call(pre=None, rule=None, mix=None, parent=par.ptr):
+        a = LinMixArgs(LinPreArgs.from_buffer_copy(r.pre), LinArgs.from_buffer_copy(r.rule), r.args.z, r.args.z_stride,
+                       r.args.norm_w, r.args.eps, r.args.y, r.args.y_stride, r.args.a8)
+        for part, ch in ((a.pre, pre), (a.rule, rule), (a, mix)):
+            for k, v in (ch or {}).items():
+                setattr(part, k, v)
+        dev.lin_mix_tree(a, parent)
+
+    bad = [dict(parent=p[k]) for k in ("beta", "decay", "log", "cv", "o", "y", "rec", "xin", "aq", "ad", "afs")]
+    bad += [dict(rule=dict(keep_dev=p[k])) for k in ("beta", "decay", "log", "cv", "o", "y", "rec", "xin", "aq")]
+    bad += [dict(pre={f: p[k]}) for f in ("conv_w", "A_log", "dt_bias", "A") for k in ("cv", "beta", "log", "y", "aq")]
+    bad += [dict(mix=dict(norm_w=p[k])) for k in ("cv", "o", "log", "y", "aq")]
+    bad += [dict(mix=dict(a8=A8(p[k], a8.d, a8.fs))) for k in ("o", "y", "log", "cv", "rec", "z", "raw", "pend", "norm", "parent", "ad")]
+    bad += [dict(mix=dict(a8=A8(a8.q, p[k], a8.fs))) for k in ("o", "y", "log", "norm", "keep_dev", "afs")]
+    bad += [dict(mix=dict(a8=A8(a8.q, a8.d, p[k]))) for k in ("o", "y", "log", "norm", "conv_w", "aq")]
+    for b in bad:
+        with pytest.raises(NmxError, match="nmx_lin_mix_tree"):
+            call(**b)
+    dev.sync()
+    for k, v in r.b.items():
+        assert_bits_equal(v.numpy(), before[k], k)
+    call()      # and as it is: accepted
+    dev.sync()
+    r.free()

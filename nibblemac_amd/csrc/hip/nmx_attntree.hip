@@ -727,6 +727,17 @@ int launch_tree(nmx_ctx *ctx, const TreeAttn &a, const Plan &p) {
     return 0;
 }
 
+struct Range {
+    const void *p;
+    size_t bytes;
+};
+template <int N>
+bool hits(const Range (&in)[N], const void *out, size_t bytes) {
+    for (const Range &x : in)
+        if (x.p && nmx_overlap(out, bytes, x.p, x.bytes)) return true;
+    return false;
+}
+
 /* the arguments that both calls use */
 int tree_shape(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent, const char *what) {
     if (!p || !parent) return nmx_fail(ctx, "%s: NULL argument", what);
@@ -754,6 +765,12 @@ int nmx_attn_tree_prep(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *pare
     if (p->rot < 0 || p->rot % 2 || p->rot > p->hd || !p->k_in || !p->v_in || !p->q_norm || !p->k_norm ||
         (p->rot && (!p->rope_cos || !p->rope_sin)))
         return nmx_fail(ctx, "nmx_attn_tree_prep: bad arguments");
+    const size_t kb = nmx_kv_bytes(p->kv_dtype, p->nkv, p->max_ctx, p->hd), qb = (size_t)p->n * p->nh * 2 * p->hd * 4;
+    const size_t ib = (size_t)p->n * p->nkv * p->hd * 4, hb = (size_t)p->hd * 4, rb = (size_t)p->max_ctx * (p->rot / 2) * 4;
+    const Range in[] = {{p->k_in, ib}, {p->v_in, ib}, {p->q_norm, hb}, {p->k_norm, hb}, {p->rope_cos, rb},
+                        {p->rope_sin, rb}, {p->pos, 4}, {parent, (size_t)p->n * 4}};
+    if (hits(in, p->q, qb) || hits(in, p->kc, kb) || hits(in, p->vc, kb))
+        return nmx_fail(ctx, "nmx_attn_tree_prep: q or a cache overlaps an input");
     const nmx_attn_dev a{p->n, p->nh, p->nkv, p->hd, p->rot, p->max_ctx, p->q, p->k_in, p->v_in, p->q_norm,
                          p->k_norm, p->eps, p->scale, p->rope_cos, p->rope_sin, p->kc, p->vc, p->pos,
                          p->pos_off, nullptr, nullptr, nullptr, nullptr, p->n};
@@ -780,10 +797,15 @@ int nmx_attn_tree(nmx_ctx *ctx, const nmx_attn_args *p, const int32_t *parent, v
     if ((uintptr_t)work % 16) return nmx_fail(ctx, "nmx_attn_tree: work not 16-byte aligned");
     const Plan pl = make_plan(p->n, p->nh, p->nkv, p->hd);
     const size_t kb = nmx_kv_bytes(p->kv_dtype, p->nkv, p->max_ctx, p->hd), ob = (size_t)p->n * p->nh * p->hd * 4;
-    if (nmx_overlap(work, pl.bytes, p->q, 2 * ob) || nmx_overlap(work, pl.bytes, p->kc, kb) ||
-        nmx_overlap(work, pl.bytes, p->vc, kb) || nmx_overlap(work, pl.bytes, p->o, ob) ||
-        nmx_overlap(p->o, ob, p->q, 2 * ob) || nmx_overlap(p->o, ob, p->kc, kb) || nmx_overlap(p->o, ob, p->vc, kb))
-        return nmx_fail(ctx, "nmx_attn_tree: o, work and the inputs overlap");
+    const Range in[] = {{p->q, 2 * ob}, {p->kc, kb}, {p->vc, kb}, {p->pos, 4}, {parent, (size_t)p->n * 4}};
+    const size_t ab = p->a8.q ? ob : 0; /* a byte a value, a float to 32 each in d and fs */
+    const Range out[] = {{work, pl.bytes}, {p->o, ob}, {p->a8.q, ab / 4}, {p->a8.d, ab / 32}, {p->a8.fs, ab / 32}};
+    for (int i = 0; i < 5; i++) {
+        if (hits(in, out[i].p, out[i].bytes)) return nmx_fail(ctx, "nmx_attn_tree: an output or work overlaps an input");
+        for (int k = 0; k < i; k++)
+            if (nmx_overlap(out[i].p, out[i].bytes, out[k].p, out[k].bytes))
+                return nmx_fail(ctx, "nmx_attn_tree: outputs and work overlap");
+    }
     const TreeAttn a{p->n, p->nh, p->nkv, p->hd, p->max_ctx, p->q, p->kc, p->vc, p->pos, parent, p->pos_off,
                      p->scale, (float *)work, (float4 *)((char *)work + pl.part_bytes), pl.splits,
                      pl.jcols, p->o, p->a8.q, p->a8.d, p->a8.fs};

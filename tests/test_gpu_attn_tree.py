@@ -501,3 +501,43 @@ def test_zero_value_rows_beside_small_ones(dev, kv, n, nh, nkv, hd, pos):
         assert tol < 1e-3 * np.abs(V).max()
         got = run(dev, q, kc, vc, parent, pos, shape, kv)
         assert np.abs(got - want).max() <= tol, (vstd, np.abs(got - want).max(), tol)
+
+
+@pytest.mark.gpu
+def test_outputs_inside_inputs_are_refused(dev):
+    """The position, the tree, the A8 and the prep's inputs against everything that is written."""
+    print("[case] attn tree overlaps", flush=True)
+    n, nh, nkv, hd, ctx, rot = 4, 2, 1, 64, 32, 32
+    f = dict(q=(n, nh, 2 * hd), kc=(nkv, ctx, hd), vc=(nkv, ctx, hd), o=(n, nh * hd), ki=(n, hd), vi=(n, hd), qn=hd, kn=hd, cos=(ctx, rot // 2),
+             sin=(ctx, rot // 2), ad=n * nh * hd // 32, afs=n * nh * hd // 32, aq=n * nh * hd // 4)
+    b = {k: dev.zeros(s, np.float32) for k, s in f.items()}
+    b["pos"], b["par"] = dev.zeros(1, np.int32), dev.to_device(np.array([-1, 0, 0, 1], np.int32))
+    b["work"] = dev.zeros(dev.attn_tree_work_bytes(n, nh, nkv, hd), np.uint8)
+    p = {k: v.ptr for k, v in b.items()}
+    good = dict(n=n, nh=nh, nkv=nkv, hd=hd, rot=rot, max_ctx=ctx, q=p["q"], k_in=p["ki"], v_in=p["vi"], q_norm=p["qn"], k_norm=p["kn"],
+                rope_cos=p["cos"], rope_sin=p["sin"], kc=p["kc"], vc=p["vc"], pos=p["pos"], o=p["o"], a8=A8(p["aq"], p["ad"], p["afs"]))
+
+    def refused(call, name, par=p["par"], **bad):
+        with pytest.raises(NmxError, match=name):
+            call(AttnArgs(**{**good, **bad}), par, *([p["work"]] if call == dev.attn_tree else []))
+
+    for k in ("o", "aq", "ad", "afs", "work"):
+        refused(dev.attn_tree, "nmx_attn_tree", par=p[k])
+        refused(dev.attn_tree, "nmx_attn_tree", pos=p[k])
+    for k in ("q", "kc", "vc", "o", "work", "pos", "par"):
+        refused(dev.attn_tree, "nmx_attn_tree", a8=A8(p[k], p["ad"], p["afs"]))
+        refused(dev.attn_tree, "nmx_attn_tree", a8=A8(p["aq"], p[k], p["afs"]))
+        refused(dev.attn_tree, "nmx_attn_tree", a8=A8(p["aq"], p["ad"], p[k]))
+    refused(dev.attn_tree, "nmx_attn_tree", a8=A8(p["aq"], p["afs"], p["afs"]))
+    refused(dev.attn_tree, "nmx_attn_tree", a8=A8(p["aq"], p["aq"], p["afs"]))
+    for k in ("q", "kc", "vc"):
+        refused(dev.attn_tree_prep, "nmx_attn_tree_prep", par=p[k])
+        for what in ("pos", "k_in", "v_in", "q_norm", "k_norm", "rope_cos", "rope_sin"):
+            refused(dev.attn_tree_prep, "nmx_attn_tree_prep", **{what: p[k]})
+    dev.sync()
+    assert not any(b[k].numpy().any() for k in b if k != "par")
+    dev.attn_tree_prep(AttnArgs(**good), p["par"])      # and as they are: accepted
+    dev.attn_tree(AttnArgs(**good), p["par"], p["work"])
+    dev.sync()
+    for x in b.values():
+        x.free()

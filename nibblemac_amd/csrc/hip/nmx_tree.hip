@@ -136,6 +136,31 @@ __global__ __launch_bounds__(256) void tree_commit_k(Commit a) {
     }
 }
 
+/* Whether anything that the call writes overlaps anything else that it reads or writes (shapes checked). A
+ * cache's rows and an array's may move within themselves; vt may be tok, whose first is never read. */
+bool overlaps(const nmx_tree_commit_args &p) {
+    struct Range {
+        const void *p;
+        size_t bytes;
+    };
+    const size_t nb = (size_t)p.n * 4, rows = (size_t)p.layers * p.cap, lb = rows * p.row * 4;
+    const bool lin = p.layers > 0, conv = lin && p.conv_k > 1, kvs = p.caches > 0;
+    Range w[5 + NMX_TREE_KV_MAX] = {{p.out, nb + 8}, {p.ctl ? p.ctl + 1 : nullptr, p.ctl ? 8u : 0u}, {p.vt, p.vt ? 4u : 0u},
+                                    {p.state, conv ? (size_t)p.layers * (p.conv_k - 1) * p.C * 4 : 0}, {p.pend, lin ? lb : 0}};
+    const Range in[] = {{p.parent, nb}, {p.tok, nb}, {p.choice, nb}, {p.pos, kvs ? 4u : 0u}, {p.log, lin ? lb : 0},
+                        {p.xin, conv ? rows * p.C * 4 : 0}, {p.ctl, p.ctl ? 4u : 0u}};
+    int nw = 5;
+    const size_t kb = kvs ? nmx_kv_bytes(p.kv_dtype, p.nkv, p.max_ctx, p.hd) : 0;
+    for (int i = 0; i < p.caches; i++) w[nw++] = {p.kv[i], kb};
+    for (int i = 0; i < nw; i++) {
+        for (const Range &x : in)
+            if (nmx_overlap(w[i].p, w[i].bytes, x.p, x.bytes) && !(w[i].p == p.vt && x.p == p.tok && p.vt == p.tok)) return true;
+        for (int k = 0; k < i; k++)
+            if (nmx_overlap(w[i].p, w[i].bytes, w[k].p, w[k].bytes)) return true;
+    }
+    return false;
+}
+
 } // namespace
 
 extern "C" {
@@ -145,13 +170,6 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p) {
     if (!p) return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
     if (p->n < 1 || p->n > NMX_TREE_MAX) return nmx_fail(ctx, "nmx_tree_commit: n=%d", p->n);
     if (!p->parent || !p->tok || !p->choice || !p->out) return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
-    const size_t nb = (size_t)p->n * 4, ob = nb + 8;
-    if (nmx_overlap(p->out, ob, p->parent, nb) || nmx_overlap(p->out, ob, p->tok, nb) || nmx_overlap(p->out, ob, p->choice, nb) ||
-        (p->ctl && (nmx_overlap(p->out, ob, p->ctl, 12) || nmx_overlap(p->ctl + 1, 8, p->parent, nb) ||
-                    nmx_overlap(p->ctl + 1, 8, p->tok, nb) || nmx_overlap(p->ctl + 1, 8, p->choice, nb))) ||
-        (p->vt && (nmx_overlap(p->out, ob, p->vt, 4) || nmx_overlap(p->vt, 4, p->parent, nb) ||
-                   nmx_overlap(p->vt, 4, p->choice, nb) || (p->vt != p->tok && nmx_overlap(p->vt, 4, p->tok, nb)))))
-        return nmx_fail(ctx, "nmx_tree_commit: out, ctl, vt and the tree overlap");
     Commit a{};
     a.n = p->n, a.parent = p->parent, a.tok = p->tok, a.choice = p->choice;
     a.out = p->out, a.ctl = p->ctl, a.vt = p->vt;
@@ -162,12 +180,6 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p) {
                             p->conv_k, p->cap, p->row);
         if (!p->log || !p->pend || (p->conv_k > 1 && (!p->state || !p->xin)))
             return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
-        const size_t lb = (size_t)p->layers * p->cap * p->row * 4, xb = (size_t)p->layers * p->cap * p->C * 4,
-                     sb = (size_t)p->layers * (p->conv_k - 1) * p->C * 4;
-        if (nmx_overlap(p->log, lb, p->pend, lb) || nmx_overlap(p->state, sb, p->xin, xb) ||
-            nmx_overlap(p->state, sb, p->pend, lb) || nmx_overlap(p->state, sb, p->log, lb) ||
-            nmx_overlap(p->pend, lb, p->xin, xb))
-            return nmx_fail(ctx, "nmx_tree_commit: the layers' arrays overlap");
         a.layers = p->layers, a.C = p->C, a.S = p->conv_k - 1;
         a.state = p->state, a.xin = p->xin, a.log = p->log, a.pend = p->pend, a.cap = p->cap, a.row = p->row;
         a.conv_wgs = a.S ? (p->C + 255) / 256 : 0;
@@ -179,14 +191,8 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p) {
             return nmx_fail(ctx, "nmx_tree_commit: bad caches %d nkv=%d max_ctx=%d hd=%d kv_dtype=%d", p->caches, p->nkv,
                             p->max_ctx, p->hd, p->kv_dtype);
         if (!p->kv || !p->pos) return nmx_fail(ctx, "nmx_tree_commit: NULL argument");
-        if (nmx_overlap(p->out, ob, p->pos, 4) || (p->ctl && nmx_overlap(p->ctl + 1, 8, p->pos, 4)) ||
-            (p->vt && nmx_overlap(p->vt, 4, p->pos, 4)))
-            return nmx_fail(ctx, "nmx_tree_commit: pos overlaps an output");
-        const size_t kb = nmx_kv_bytes(p->kv_dtype, p->nkv, p->max_ctx, p->hd);
         for (int i = 0; i < p->caches; i++) {
             if (!p->kv[i] || (uintptr_t)p->kv[i] % 4) return nmx_fail(ctx, "nmx_tree_commit: cache %d", i);
-            for (int k = 0; k < i; k++)
-                if (nmx_overlap(p->kv[i], kb, p->kv[k], kb)) return nmx_fail(ctx, "nmx_tree_commit: caches overlap");
             a.kv[i] = p->kv[i];
         }
         a.caches = p->caches, a.nkv = p->nkv, a.max_ctx = p->max_ctx, a.pos = p->pos, a.pos_off = p->pos_off;
@@ -195,6 +201,7 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p) {
         a.scale_at = (size_t)p->nkv * p->max_ctx * p->hd;
         a.kv_wgs = (a.row_bytes / 4 + a.scales + 255) / 256;
     }
+    if (overlaps(*p)) return nmx_fail(ctx, "nmx_tree_commit: what is written overlaps something else");
     const nmx_on_device on(ctx);
     const size_t wgs = 1 + (size_t)a.layers * (a.conv_wgs + a.log_wgs) + (size_t)a.caches * a.nkv * a.kv_wgs;
     tree_commit_k<<<(unsigned)wgs, 256, 0, ctx->stream>>>(a);

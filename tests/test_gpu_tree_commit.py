@@ -346,3 +346,42 @@ def test_captured_call(dev):
         for x, y in zip(got, outputs()):
             assert_bits_equal(x, y, "replay")
     dev.graph_destroy(g)
+
+
+@pytest.mark.gpu
+def test_overlaps_are_refused(dev):
+    """Everything that is written (out, ctl, vt, states, pending rows, caches) against everything else."""
+    print("[case] tree commit overlaps", flush=True)
+    n = 4
+    i = {k: dev.zeros(32, np.int32) for k in ("parent", "tok", "choice", "out", "ctl", "vt")}
+    f = {k: dev.zeros(4096, np.float32) for k in ("state", "xin", "log", "pend")}
+    kv = [dev.zeros((1, 16, 64), np.float32) for _ in range(2)]
+    lin = dict(layers=1, C=32, conv_k=4, cap=4, row=33, **f)
+    kvs = dict(caches=kv, nkv=1, max_ctx=16, hd=64, kv_dtype=0, pos=i["ctl"])
+
+    def call(lin_=None, kv_=None, **ch):
+        g = {**dict(n=n, **i), **ch}
+        dev.tree_commit(tree_commit_args(g["n"], g["parent"], g["tok"], g["choice"], g["out"], ctl=g["ctl"], vt=g["vt"],
+                                         lin={**lin, **(lin_ or {})}, kv={**kvs, **(kv_ or {})}))
+
+    p = {k: v.ptr for k, v in {**i, **f, "kv0": kv[0], "kv1": kv[1]}.items()}
+    arrays = ("state", "xin", "log", "pend", "kv0", "kv1")
+    bad = [{k: p[a]} for k in ("out", "vt", "ctl") for a in arrays]
+    bad += [{k: p[a]} for k in ("parent", "tok", "choice") for a in ("state", "pend", "kv0", "kv1")]
+    bad += [dict(vt=p["ctl"] + 4), dict(vt=p["ctl"] + 8), dict(vt=p["ctl"]), dict(ctl=p["vt"] - 4), dict(vt=p["out"] + 4)]
+    bad += [dict(kv_=dict(pos=p[a])) for a in ("state", "pend", "kv0", "kv1")]
+    bad += [dict(lin_={k: p[a]}) for k in ("state", "pend", "log", "xin") for a in ("kv0", "kv1")]
+    bad += [dict(lin_={k: p[a]}) for k in ("state", "pend") for a in ("parent", "tok", "choice", "out", "vt", "ctl")]
+    bad += [dict(lin_=dict(xin=p["pend"])), dict(kv_=dict(caches=[kv[0], kv[0]])), dict(kv_=dict(caches=[kv[0], f["pend"]])),
+            dict(kv_=dict(caches=[i["out"]])), dict(kv_=dict(caches=[f["log"]]))]
+    for b in bad:
+        with pytest.raises(NmxError, match="nmx_tree_commit"):
+            call(**b)
+    dev.sync()
+    assert not any(x.numpy().any() for x in (*i.values(), *f.values(), *kv))
+    call()                                  # as they are, the tokens' own first as vt, no layers or caches
+    call(vt=i["tok"])
+    dev.tree_commit(tree_commit_args(n, i["parent"], i["tok"], i["choice"], i["out"], ctl=i["ctl"], vt=i["tok"]))
+    dev.sync()
+    for x in (*i.values(), *f.values(), *kv):
+        x.free()

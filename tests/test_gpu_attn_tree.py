@@ -541,3 +541,112 @@ def test_outputs_inside_inputs_are_refused(dev):
     dev.sync()
     for x in b.values():
         x.free()
+
+
+def held(x):
+    """What is left of rows of x without the low halves: 11 bits of each element."""
+    x = np.asarray(x, np.float64)
+    m, e = np.frexp(x)
+    return np.ldexp(np.rint(m * 2048), e - 11)
+
+
+def off_grid(rng, shape):
+    """Values in [1, 2) that lie 0.45 of a step above what 11 bits hold."""
+    return (1 + (rng.integers(0, 1023, shape) + 0.45) / 1024).astype(np.float32)
+
+
+def on_grid(rng, shape):
+    return (1 + rng.integers(0, 1023, shape) / 1024).astype(np.float32)
+
+
+def attend(q, K, V, parent, pos, shape, kv, less=""):
+    """64-bit attention of every node and what each element may be off by. less: the context's part with the
+    low halves of q, k, w (the weights) or v left out, mistakes to be noticed.
+
+    Per context position: q's and an fp32 row's elements are two binary16 parts, the low one rounded (2^-22
+    of the element), low times low left out (2^-22 more); a matrix instruction adds 32 products
+    and drops from each what lies below 2^-26 of the sum, then rounds (2^-23): 1.25 2^-21 of the sum of
+    magnitudes for each of the hd / 32 times 2 (fp32 rows 3) chained ones. The score is rounded 5 times on its
+    way to the exponential, which adds 2^-23 and 2^-24 of its distance to the maximum. These errors move o by p |v -
+    o|. The weights have 21 bits (the first part towards zero) and their low part times fp32 values' low part
+    is left out: 2^-21, fp32 values 2^-22 + 2^-21 more; a tile adds 2 (3) instructions' 1.25 2^-21 and a
+    rescale of 2^-23, the join at most 64 roundings, quotient and gate 2^-21: these move o by p |v|. What is
+    below 2^-24 of the largest scaled part is lost: 2^-36 of the row's, or tile's, largest for each term."""
+    n, nh, nkv, hd, ctx = shape
+    u22 = 2.0 ** -22
+    f32, hp = kv == KV_F32, 64 if hd <= 64 else 128 if hd <= 128 else 256 if hd <= 256 else 512
+    mfma = 1.25 * 2.0 ** -21
+    tiles = -(-pos // 32)
+    halves, mt = (2, 4) if hp == 512 else (1, 8)
+    splits = max(1, min(256, 256 // (nkv * (-(-(-(-n * (nh // nkv) // 16)) // mt)) * halves)))
+    T = -(-tiles // splits)
+    seen, scale = ancestors(parent), float(np.float32(1 / np.sqrt(hd)))
+    o, tol = np.zeros((n, nh, hd)), np.zeros((n, nh, hd))
+    for t in range(n):
+        at = np.concatenate([np.arange(pos), pos + np.flatnonzero(seen[t])])
+        c = np.arange(len(at)) < pos
+        for h in range(nh):
+            g = h // (nh // nkv)
+            x, k, v = q[t, h, :hd].astype(np.float64), K[g, at], V[g, at]
+            s = np.where(c, (held(k) if "k" in less else k) @ (held(x) if "q" in less else x), k @ x) * scale
+            w = np.exp(s - s.max())
+            wv = w
+            if "w" in less:     # towards zero, of the weight times an int8 row's scale
+                f = np.abs(v).max(1) / 127 if kv == KV_I8 else np.ones(len(at))
+                m, e = np.frexp(w * f)
+                wv = np.where(c, np.ldexp(np.floor(m * 2048), e - 11) / f, w)
+            y = np.where(c[:, None], held(v), v) if "v" in less else v
+            out = wv @ y / w.sum()
+            gate = 1 / (1 + np.exp(-q[t, h, hd:].astype(np.float64)))
+            o[t, h] = out * gate
+            mag = np.abs(k) @ np.abs(x)
+            ds = scale * (mag * ((3 if f32 else 1) * u22 + hp / 32 * (3 if f32 else 2) * mfma) +
+                          2.0 ** -36 * (np.abs(x).max() * np.abs(k).sum(1) + np.abs(x).sum() * np.abs(k).max(1)))
+            p = w / w.sum()
+            e1 = ds + 5 * 2.0 ** -24 * np.abs(s) + 2.0 ** -23 + 2.0 ** -24 * np.abs(s - s.max())
+            e2 = 2 * u22 + (3 * u22 if f32 else 0) + T * ((3 if f32 else 2) * mfma + 2.0 ** -23) + 64 * 2.0 ** -24 + 2 * u22
+            lost = len(at) * 2.0 ** -36 * (p * np.abs(v).max(1)).max()
+            tol[t, h] = ((p * e1) @ np.abs(v - out) + e2 * (p @ np.abs(v)) + lost) * gate
+    return o.reshape(n, nh * hd), tol.reshape(n, nh * hd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_F16, KV_I8])
+@pytest.mark.parametrize("n,nh,nkv,hd,pos", [(1, 2, 1, 64, 150), (9, 4, 2, 128, 333), (5, 4, 1, 192, 95), (1, 8, 2, 256, 3000), (64, 4, 1, 256, 200),
+                                             (7, 4, 2, 320, 130), (6, 4, 1, 512, 250), (33, 2, 1, 512, 64)])
+def test_every_operand_is_held_to_22_bits(dev, n, nh, nkv, hd, pos, kv):
+    """Inputs whose 11-bit halves are all off to the same side: leaving out the low half of the queries, of
+    fp32 keys, of the weights or of fp32 values moves o by far more than what it may be off by."""
+    print(f"[case] attn tree parts n={n} hd={hd} kv={kv}", flush=True)
+    rng = np.random.default_rng(n + hd + kv)
+    ctx, shape, rep = pos + n, (n, nh, nkv, hd, pos + n), nh // nkv
+    parent, half, scale = tree(rng, n, "random"), hd // 2, 1 / np.sqrt(hd)
+    sign = np.where(rng.random((nkv, hd)) < 0.5, -1, 1).astype(np.float32)
+    q = np.empty((n, nh, 2 * hd), np.float32)
+    q[..., :half], q[..., half:hd] = off_grid(rng, (n, nh, half)), on_grid(rng, (n, nh, hd - half))
+    q[..., :hd] *= sign.repeat(rep, 0)
+    q[..., hd:] = rng.standard_normal((n, nh, hd))
+
+    def device_and_bounds(k, v, *less):
+        (kc, K), (vc, V) = encode(k, kv), encode(v, kv)
+        want, tol = attend(q, K, V, parent, pos, shape, kv)
+        for part in less:
+            off = np.abs(attend(q, K, V, parent, pos, shape, kv, part)[0] - want)
+            assert (off > 2 * tol).any(), (part, (off / tol).max())
+        got = run(dev, q, kc, vc, parent, pos, shape, kv)
+        assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / tol).max()
+
+    # scores about 12: of one half of the positions from the columns where q is off the grid, of the other from
+    # those where (fp32) k is; values of +-1 by half
+    first = rng.random((nkv, ctx)) < 0.5
+    cols = np.where(first[..., None], np.arange(hd) < half, np.arange(hd) >= half)
+    size = np.float32(12 / (scale * 1.5 * half))
+    top = np.float32(2.0 ** np.floor(np.log2(size)))    # a power of two: the grid's steps stay where they are
+    lift = (1 + rng.integers(0, 64, (nkv, ctx, 1)) / 1024).astype(np.float32)
+    k = np.where(first[..., None], lift, lift + np.float32(0.45 / 1024) if kv == KV_F32 else lift) * top * cols * sign[:, None]
+    v = np.where(first, 1, -1)[..., None] * on_grid(rng, (nkv, ctx, hd))
+    device_and_bounds(k.astype(np.float32), v.astype(np.float32), *("qk" if kv == KV_F32 else "q"))
+    # weights of all sizes, values above 0
+    k = rng.standard_normal((nkv, ctx, hd)).astype(np.float32) * np.float32(0.25)
+    v = (off_grid if kv == KV_F32 else on_grid)(rng, (nkv, ctx, hd)) * np.float32(0.5)
+    device_and_bounds(k, v, *("wv" if kv == KV_F32 else "w"))

@@ -413,3 +413,69 @@ def test_outputs_inside_other_inputs_are_refused(dev):
     call()      # and as it is: accepted
     dev.sync()
     r.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk,rep,keep", [(32, 1, 0), (64, 2, 3), (128, 1, 5), (256, 1, 1)])
+def test_bushes_within_element_bounds(dev, dk, rep, keep):
+    """o and delta of shallow trees of 64 nodes from a state, element by element; products of nodes without
+    their rests would be noticed."""
+    print(f"[case] lin tree bounds dk={dk}", flush=True)
+    rng = np.random.default_rng(dk + 1)
+    n, heads, dv = 64, 2, 96
+    parent, kd = bushes(rng, n), heads // rep * dk
+    host = make(rng, n, heads, rep, dk, dv, 4, keep)
+    host["rec"] *= np.float32(0.05)
+    host["pend"][:, :, dk:dk + dv] *= np.float32(0.05)
+    host["b"][:] = 2
+    r = Run(dev, host, n, heads, rep, dk, dv, 4, keep)
+    got = r(parent)
+    r.free()
+    args = (got["cv"], got["beta"], got["decay"], got["rec"].astype(np.float64)[at_index(heads, dk, dv)], parent, heads, rep, dk, dv, kd)
+    o, d, eo, ed = bounded(*args)
+    off = bounded(*args, rests=False)
+    assert eo.max() <= 1e-3 * np.abs(o).max() and (np.abs(off[0] - o) > 2 * eo).any() and (np.abs(off[1] - d) > ed).any()
+    err, errd = np.abs(got["o"].reshape(o.shape) - o), np.abs(got["log"][:n, :, dk:dk + dv] - d)
+    assert (err <= eo).all() and (errd <= ed).all(), ((err / eo).max(), (errd / ed).max())
+
+
+def plain32(cv, beta, decay, S0, parent, heads, rep, dk, dv, kd):
+    """The recurrence node by node in 32 bits."""
+    n = len(parent)
+    q, k = (cv[:, a:a + kd].reshape(n, -1, dk).repeat(rep, 1) for a in (0, kd))
+    v = cv[:, 2 * kd:].reshape(n, heads, dv)
+    S, o, d = [], np.zeros((n, heads, dv), np.float32), np.zeros((n, heads, dv), np.float32)
+    for t in range(n):
+        R = (S[parent[t]] if 0 <= parent[t] < t else S0) * decay[t][:, None, None]
+        d[t] = (v[t] - (R @ k[t][:, :, None])[..., 0]) * beta[t][:, None]
+        R = R + d[t][:, :, None] * k[t][:, None, :]
+        o[t] = (R @ q[t][:, :, None])[..., 0]
+        S.append(R)
+    return o, d
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["chain", "random", "forest"])
+@pytest.mark.parametrize("dk,dv", [(32, 64), (64, 128), (128, 128), (256, 64)])
+def test_deep_trees_beside_plain_32_bits(dev, dk, dv, kind):
+    """Errors of o and delta over 64 nodes, root mean square and largest, against those of the plain
+    recurrence in 32 bits on the same inputs. A product of nodes lacks those of two rests: sqrt(dk) / 12 2^-24
+    of the rows' norms, 0.5 to 1.3 units of 32-bit rounding; the plain form rounds its state's elements at each
+    node, about one such unit a level of a product, and its sums. So the two are of one size: at most 8
+    times the plain one's passes (16 for the largest), a product without rests, 2^-13.3 of the norms, is 1000 times it."""
+    print(f"[case] lin tree 32 bits dk={dk} {kind}", flush=True)
+    rng = np.random.default_rng(dk + 2)
+    n, heads = 64, 2
+    parent, kd = tree(rng, n, kind), heads * dk
+    host = make(rng, n, heads, 1, dk, dv, 4, 2)
+    r = Run(dev, host, n, heads, 1, dk, dv, 4, 2)
+    got = r(parent)
+    r.free()
+    S0 = got["rec"][at_index(heads, dk, dv)]
+    args = (got["cv"], got["beta"], got["decay"], S0, parent, heads, 1, dk, dv, kd)
+    o, d, _ = recurrence(*args[:3], S0.astype(np.float64), *args[4:])
+    for name, x, want, plain in zip("od", (got["o"].reshape(o.shape), got["log"][:n, :, dk:dk + dv]), (o, d), plain32(*args)):
+        err, ref = x - want, plain - want
+        rms, rms32 = (float(np.sqrt((e * e).mean())) for e in (err, ref))
+        print(f"[case]   {name}: rms {rms:.2e} ({rms32:.2e} plain), largest {np.abs(err).max():.2e} ({np.abs(ref).max():.2e})", flush=True)
+        assert rms <= 8 * rms32 and np.abs(err).max() <= 16 * np.abs(ref).max()

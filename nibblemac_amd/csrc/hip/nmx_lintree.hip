@@ -209,8 +209,9 @@ __device__ __forceinline__ void tree_tables(TreeTables &s, int n, unsigned long 
  * whole number and the rest, both binary16. Products of whole numbers add up to no more than about 2^24: exact in
  * the accumulator. The products of a whole number and a rest are 2^-12 of that and have an accumulator of
  * their own: beside a larger sum the matrix instruction drops what lies below 2^-26 of it from every
- * product, which was the largest error of o where q.k nearly cancels. The products of two rests, random
- * and 2^-24, are left out. Three 16-bit instructions per 32 keys in place of 32 32-bit ones. */
+ * product, which was the largest error of o where q.k nearly cancels. The products of two rests go there
+ * too: 2^-24 and random between different rows, but of rows alike (a token repeated) they add up to dk / 12
+ * of that in every product. Four 16-bit instructions per 32 keys in place of 32 32-bit ones. */
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mfma16(half8 a, half8 b, f32x4 c) {
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
             const _Float16 *ar = kh2 + an * HS + 8 * gq, *tr = kh2 + (16 * X + c) * HS + 8 * gq, *ur = qh2 + (16 * X + c) * HS + 8 * gq;
             const int lo = n16 * HS;
             const float q_up = QL ? 0.0f : inverse_pow2(down[16 * X + c].y);
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x, xr = x, yr = x;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x, xr = x, yr = x, xs = x, ys = x;
 #pragma unroll
             for (int k = 0; k < DK; k += 32) {
                 const half8 ah = *(const half8 *)(ar + k), al = *(const half8 *)(ar + lo + k);
@@ -409,9 +410,10 @@ __global__ __launch_bounds__(256 + 64 * tree_wave<DK4>()) void lin_tree_rule_k(T
                 }
                 x = mfma16(th, ah, x), y = mfma16(uh, ah, y);
                 xr = mfma16(tl, ah, xr), yr = mfma16(ul, ah, yr);
-                xr = mfma16(th, al, xr), yr = mfma16(uh, al, yr);
+                xs = mfma16(th, al, xs), ys = mfma16(uh, al, ys);
+                xr = mfma16(tl, al, xr), yr = mfma16(ul, al, yr);
             }
-            x += xr, y += yr;
+            x += xr + xs, y += yr + ys;
             const int dp = tt.depth[an];
             const float down_a = down[an].x;
 #pragma unroll

@@ -650,3 +650,47 @@ def test_every_operand_is_held_to_22_bits(dev, n, nh, nkv, hd, pos, kv):
     k = rng.standard_normal((nkv, ctx, hd)).astype(np.float32) * np.float32(0.25)
     v = (off_grid if kv == KV_F32 else on_grid)(rng, (nkv, ctx, hd)) * np.float32(0.5)
     device_and_bounds(k, v, *("wv" if kv == KV_F32 else "w"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_F16, KV_I8])
+@pytest.mark.parametrize("zero", ["queries", "keys", "values", "some_of_each"])
+def test_rows_of_zeros(dev, kv, zero):
+    """Zero queries or keys weigh every position alike; zero values give zeros."""
+    print(f"[case] attn tree zeros {zero} kv={kv}", flush=True)
+    rng = np.random.default_rng(17 + kv)
+    n, nh, nkv, hd, ctx, pos = 10, 4, 2, 128, 300, 280
+    q = rng.standard_normal((n, nh, 2 * hd)).astype(np.float32)
+    k, v = (rng.standard_normal((nkv, ctx, hd)).astype(np.float32) for _ in range(2))
+    some = lambda x: x[..., 0] * 0 + (rng.random(x.shape[:-1]) < 0.5)  # noqa: E731
+    if zero in ("queries", "some_of_each"):
+        q[..., :hd] *= 0 if zero == "queries" else some(q)[..., None]
+    if zero in ("keys", "some_of_each"):
+        k *= 0 if zero == "keys" else some(k)[..., None]
+    if zero in ("values", "some_of_each"):
+        v *= 0 if zero == "values" else some(v)[..., None]
+    parent = tree(rng, n, "random")
+    (kc, K), (vc, V) = encode(k.astype(np.float32), kv), encode(v.astype(np.float32), kv)
+    want, tol = reference(q, K, V, parent, pos, (n, nh, nkv, hd, ctx))
+    got = run(dev, q, kc, vc, parent, pos, (n, nh, nkv, hd, ctx), kv)
+    assert np.abs(got - want).max() <= tol
+    if zero == "values":
+        assert not got.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_I8])
+@pytest.mark.parametrize("big", [1e18, 1e30, 1e-18, 1e-30])
+def test_queries_and_keys_of_opposite_magnitudes(dev, kv, big):
+    """Queries of 1e30 against keys of 1e-30 and the other way round: scores are ordinary."""
+    print(f"[case] attn tree magnitudes {big} kv={kv}", flush=True)
+    rng = np.random.default_rng(18 + kv)
+    n, nh, nkv, hd, ctx, pos = 10, 4, 2, 128, 300, 280
+    q = rng.standard_normal((n, nh, 2 * hd)).astype(np.float32)
+    q[..., :hd] *= np.float32(big)
+    kc, K = make_cache(rng, kv, nkv, ctx, hd, 1 / big)
+    vc, V = make_cache(rng, kv, nkv, ctx, hd)
+    parent = tree(rng, n, "random")
+    want, tol = reference(q, K, V, parent, pos, (n, nh, nkv, hd, ctx))
+    got = run(dev, q, kc, vc, parent, pos, (n, nh, nkv, hd, ctx), kv)
+    assert np.abs(got - want).max() <= tol, (np.abs(got - want).max(), tol)

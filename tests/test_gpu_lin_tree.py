@@ -297,9 +297,10 @@ def bounded(cv, beta, decay, S0, parent, heads, rep, dk, dv, kd, rests=True):
     two chains, each off by at most two roundings of its sum: (dk / 4 + 2) u of the sum of magnitudes. A
     product of nodes: rows scaled to a norm of at least 2^11 (q 2^11.5), an element as a whole number of 11
     bits and a rest of at most 1/2 + 2^-11 of the element in 11 bits, so with s = sqrt(dk) / 2 the rests
-    have a norm of at most s + 1 for every 2^11 of the row's: without the products of two rests it is
-    off by ((s + 1)^2 + 2 (s + 1) + 1) 2^-22 of the norms' product. A factor of decays has one rounding a level; every
-    product and sum one more. rests False: the same sums with the rests left out (a mistake to be noticed)."""
+    have a norm of at most s + 1 for every 2^11 of the row's and are themselves off by 2^-11 of that: the
+    product is off by (2 (s + 1) + 2) 2^-22 of the norms' product, its sums counted as one such unit. A factor of
+    decays has one rounding a level; every product and sum one more. rests False: the same sums with the rests left out
+    (a mistake to be noticed)."""
     n, u = len(parent), 2.0 ** -24
     q = cv[:, :kd].reshape(n, -1, dk).astype(np.float64).repeat(rep, 1)
     k = cv[:, kd:2 * kd].reshape(n, -1, dk).astype(np.float64).repeat(rep, 1)
@@ -311,7 +312,7 @@ def bounded(cv, beta, decay, S0, parent, heads, rep, dk, dv, kd, rests=True):
         qq, kk = (np.rint(x * up(x, nx)) / up(x, nx) for x, nx in ((q, nq), (k, nk)))
     KK, QK = (np.einsum("thd,ahd->tah", x, kk) for x in (kk, qq))
     s = np.sqrt(dk) / 2
-    eta = ((s + 1) ** 2 + 2 * (s + 1) + 1) * 2.0 ** -22
+    eta = (2 * (s + 1) + 2) * 2.0 ** -22
     o, d, eo, ed = (np.zeros((n, heads, dv)) for _ in range(4))
     for t in range(n):
         g, D, a, path = np.ones(heads), {}, t, []
@@ -459,16 +460,121 @@ def plain32(cv, beta, decay, S0, parent, heads, rep, dk, dv, kd):
 @pytest.mark.parametrize("dk,dv", [(32, 64), (64, 128), (128, 128), (256, 64)])
 def test_deep_trees_beside_plain_32_bits(dev, dk, dv, kind):
     """Errors of o and delta over 64 nodes, root mean square and largest, against those of the plain
-    recurrence in 32 bits on the same inputs. A product of nodes lacks those of two rests: sqrt(dk) / 12 2^-24
-    of the rows' norms, 0.5 to 1.3 units of 32-bit rounding; the plain form rounds its state's elements at each
-    node, about one such unit a level of a product, and its sums. So the two are of one size: at most 8
-    times the plain one's passes (16 for the largest), a product without rests, 2^-13.3 of the norms, is 1000 times it."""
+    recurrence in 32 bits on the same inputs. A product of nodes is off by about 2^-24 of its rows' norms, and
+    its sums over a node's ancestors are rounded as often as these are many; the plain form rounds its
+    state's elements at each node, about one such unit a level of a product, and its sums. So the two are of one
+    size: at most 8 times the plain one's passes (16 for the largest), a product without rests, 2^-13.3 of the
+    norms, is 1000 times it."""
     print(f"[case] lin tree 32 bits dk={dk} {kind}", flush=True)
     rng = np.random.default_rng(dk + 2)
     n, heads = 64, 2
     parent, kd = tree(rng, n, kind), heads * dk
     host = make(rng, n, heads, 1, dk, dv, 4, 2)
     r = Run(dev, host, n, heads, 1, dk, dv, 4, 2)
+    got = r(parent)
+    r.free()
+    S0 = got["rec"][at_index(heads, dk, dv)]
+    args = (got["cv"], got["beta"], got["decay"], S0, parent, heads, 1, dk, dv, kd)
+    o, d, _ = recurrence(*args[:3], S0.astype(np.float64), *args[4:])
+    for name, x, want, plain in zip("od", (got["o"].reshape(o.shape), got["log"][:n, :, dk:dk + dv]), (o, d), plain32(*args)):
+        err, ref = x - want, plain - want
+        rms, rms32 = (float(np.sqrt((e * e).mean())) for e in (err, ref))
+        print(f"[case]   {name}: rms {rms:.2e} ({rms32:.2e} plain), largest {np.abs(err).max():.2e} ({np.abs(ref).max():.2e})", flush=True)
+        assert rms <= 8 * rms32 and np.abs(err).max() <= 16 * np.abs(ref).max()
+
+
+@pytest.mark.gpu
+def test_optional_arguments(dev):
+    """y alone, the A8 alone, no xin, A in place of A_log: what is given equals the full call's, bit for bit."""
+    print("[case] lin tree optional arguments", flush=True)
+    rng = np.random.default_rng(13)
+    n, heads, dk, dv = 21, 2, 64, 64
+    host = make(rng, n, heads, 1, dk, dv, 4, 2)
+    host["A"] = -np.exp(host["A_log"].astype(np.float64)).astype(np.float32)
+    parent = tree(rng, n, "random")
+
+    def call(change=lambda a: None):
+        r = Run(dev, host, n, heads, 1, dk, dv, 4, 2)
+        change(r)
+        got = r(parent)
+        r.free()
+        return got
+
+    full = call()
+    outs = ("y", "aq", "ad", "afs", "o", "log", "rec", "xin", "cv")
+
+    def same(got, but):
+        for k in outs:
+            if k not in but:
+                assert_bits_equal(got[k], full[k], k)
+
+    def no_a8(r):
+        r.args.a8 = A8(None, None, None)
+
+    def no_y(r):
+        r.args.y = None
+
+    def no_xin(r):
+        r.args.pre.xin = None
+
+    got = call(no_a8)
+    same(got, ("aq", "ad", "afs"))
+    assert not got["aq"].any() and (got["ad"] == 7).all()
+    got = call(no_y)
+    same(got, ("y",))
+    assert (got["y"] == 7).all()
+    got = call(no_xin)
+    same(got, ("xin",))
+    assert (got["xin"] == 7).all()
+
+    def given_A(r):
+        r.args.pre.A, r.args.pre.A_log = r.b["A"].ptr, None
+
+    got = call(given_A)     # A may differ from the device's -exp(A_log) in the last place: an exponent of at most 1
+    assert np.abs(got["decay"] - full["decay"]).max() <= 2.0 ** -22
+    same(got, outs[:7])
+
+
+@pytest.mark.gpu
+def test_replays_that_advance_the_state(dev):
+    """A captured call with pending rows folds them in at every replay, as eager calls do."""
+    print("[case] lin tree replays", flush=True)
+    rng = np.random.default_rng(14)
+    n, heads, dk, dv = 40, 2, 128, 64
+    host = make(rng, n, heads, 1, dk, dv, 4, 9)
+    parent = tree(rng, n, "random")
+    a, b = (Run(dev, host, n, heads, 1, dk, dv, 4, 9, keep_dev=9) for _ in range(2))
+    par = dev.to_device(parent)
+    dev.graph_begin()
+    dev.lin_mix_tree(a.args, par)
+    g = dev.graph_end()
+    for keep in (3, 0, 9, 5):
+        for r in (a, b):
+            dev.upload(r.b["keep_dev"], np.array([keep], np.int32))
+        dev.graph_launch(g)
+        dev.lin_mix_tree(b.args, par)
+        dev.sync()
+        for k in ("y", "o", "log", "rec"):
+            assert_bits_equal(a.b[k].numpy(), b.b[k].numpy(), f"keep {keep} {k}")
+    dev.graph_destroy(g)
+    for x in (a, b):
+        x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("decay", [0.999, 0.5])
+def test_one_key_for_every_node(dev, decay):
+    """A chain of 64 tokens alike: every product of keys is that of a row with itself, which the deltas'
+    triangular system is hardest on; held as in the deep trees above."""
+    print(f"[case] lin tree one key decay={decay}", flush=True)
+    rng = np.random.default_rng(15)
+    n, heads, dk, dv = 64, 2, 128, 64
+    parent, kd = tree(rng, n, "chain"), heads * dk
+    host = make(rng, n, heads, 1, dk, dv, 4, 0)
+    host["raw"][:, :2 * kd] = host["raw"][:1, :2 * kd]
+    host["b"][:] = 3
+    host["a"][:] = np.log(np.expm1(-np.log(decay) / np.exp(host["A_log"]))) - host["dt"]
+    r = Run(dev, host, n, heads, 1, dk, dv, 4, 0)
     got = r(parent)
     r.free()
     S0 = got["rec"][at_index(heads, dk, dv)]

@@ -538,19 +538,21 @@ __device__ uint32_t select_key(Pick &S, const Row &r, int b, bool by_count, uint
 }
 
 /* The least logit whose weight is at least min_p of the largest: its key. Weights grow with the key, so a
- * wave cuts the span of keys that the border may lie in to a 64th at a time: 6 rounds for 32 bits, where
- * weights are alike over millions of keys too (logits next to 0, a high temperature, min_p of 1). The
- * upper end always holds a key that is in. */
+ * wave looks at 64 keys about the logarithm's border first, where it nearly always is, and else cuts the span of
+ * keys that it may lie in to a 64th at a time: 6 rounds for 32 bits, also where weights are alike over
+ * millions of keys (logits next to 0, a high temperature, min_p of 1). The upper end is always in. */
 __device__ uint32_t min_p_key(float mx, double inv, double min_p) {
     const uint32_t lane = threadIdx.x & 63;
     uint32_t lo = sample_key(-3.40282347e+38f), hi = sample_key(mx);
-    for (int round = 0; lo < hi && round < 7; round++) {
-        const uint32_t step = (hi - lo + 63) >> 6;
-        const uint32_t k = lo + lane * step < hi ? lo + lane * step : hi;
+    uint32_t step = 1, from = sample_key(sample_value((float)fmax((double)mx + 8.0 * log(min_p) / inv, -3.40282346638528859e+38)));
+    from = from < lo + 32 ? lo : from - 32 < hi ? from - 32 : hi;
+    for (int round = 0; lo < hi && round < 8; round++) {
+        const uint32_t k = from + lane * step < hi ? from + lane * step : hi;
         const unsigned long long in = __ballot(k == hi || weight(sample_unkey(k), mx, inv) >= min_p);
         const int f = in ? __ffsll((long long)in) - 1 : 64; /* the first key that is in */
-        if (f < 64) hi = lo + f * step < hi ? lo + f * step : hi;
-        if (f > 0) lo += (f - 1) * step + 1;
+        if (f < 64) hi = from + f * step < hi ? from + f * step : hi;
+        if (f > 0) lo = from + (f - 1) * step + 1;
+        from = lo, step = (hi - lo + 63) >> 6;
     }
     return hi;
 }

@@ -457,7 +457,8 @@ int nmx_attn_fused_chunk(nmx_ctx *ctx, const nmx_attn_args *p, int score_rows);
  * cache row is at slot *pos + pos_off + t, its position *pos + pos_off + depth(t); a node whose slot
  * lies outside the cache has no row (its caller keeps *pos + n <= max_ctx).
  * Results are right to 32-bit rounding but not equal bit for bit to those of a chain's calls, which
- * add in the reference's order. */
+ * add in the reference's order. (Attention multiplies operands of 22 bits and adds in 32; fp32 and int8 value
+ * rows with nothing above 2^-100 keep fewer. A DeltaNet node's sums have a term for each ancestor.) */
 #define NMX_TREE_MAX 64
 
 /* nmx_attn_prep for a tree: q and k rows normed, RoPE at the node's position, K and V stored at its
@@ -485,8 +486,9 @@ int nmx_lin_mix_tree(nmx_ctx *ctx, const nmx_lin_mix_args *a, const int32_t *par
 
 /* The end of a tree round: from node 0 on, the child whose token tok[child] equals the choice made
  * after its parent (choice[node]: the argmax of nmx_head_accept, or the token of nmx_sample, at the
- * node's logits) is accepted, the first one of several; a negative choice accepts none. With
- * e >= 1 nodes on that path (node 0 among them):
+ * node's logits) is accepted, the first one of several; a negative choice accepts none, and where the path
+ * ends with it (a row without a finite logit) out and vt hold it as it is: no token, and no row of an
+ * embedding. With e >= 1 nodes on that path (node 0 among them):
  *   out [2 + n]: e - 1 (accepted drafts), the choice after the last node (the next round's node 0),
  *     the path's nodes, -1 behind them; ctl (may be NULL): ctl[1] = ctl[2] = e, ctl[0] as it is
  *     (nmx_ctl_advance adds e to it); vt (may be NULL, may be tok): vt[0] = that choice;
@@ -529,7 +531,8 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p);
  * infinite temperature every finite logit). u
  * below 0 or NaN counts as 0, from 1 on the last kept token is taken. A logit of -inf or NaN is
  * never chosen, +inf is the largest finite value; a row that has nothing else gives token -1 and
- * prob 0. Tokens 32 nats below the maximum of a filtered row have no mass (less than 2^-46 each).
+ * prob 0. Tokens 32 nats below the maximum of a filtered row have no mass (less than 2^-46 each), nor has
+ * a weight below 1e-300 in any.
  * params and u are on the device (a captured call reads them at each replay): one record for all
  * rows (per_row 0) or n of them. work: device scratch of nmx_sample_work_bytes(n, vocab) bytes (0
  * for a shape that is refused), 16-byte aligned, used by one call at a time. n <= 4096, vocab <=

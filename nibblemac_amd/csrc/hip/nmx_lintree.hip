@@ -14,11 +14,12 @@
  * A node's sums run over its own ancestors alone (no product with a masked zero), so whatever
  * another branch holds, NaN or infinity, does not reach it.
  *
- * On MI355X, 16 heads of 128 x 128: 9 nodes 15.5 us (3.0 MB, 0.6 us as a copy), 64 nodes 26 us (7.6 MB,
- * 1.5 us; pre 5.5, rule 19.7, post 4.5). Both are chains of phases behind barriers, not bytes; of the rule's
- * at 64 nodes the requests take 2.1 us, parts of the rows 1.6, 5 pending rows 2.2, the state's products
- * and the tree's tables 2.2, the products of nodes 2.3, 15 levels 3.5. The whole mixer of a head in one
- * workgroup, for up to 16 nodes, took longer (9 nodes 18.0, 16 nodes 20.8 against 16.9 us). */
+ * On MI355X, 16 heads of 128 x 128: 9 nodes 15.7 us (3.0 MB, 0.6 us as a copy), 64 nodes 26.0 to 26.5 us (7.6 MB,
+ * 1.5 us; traced: pre 5.8, rule 19.9, post 4.2). Both are chains of phases behind barriers, not bytes; of the rule's
+ * at 64 nodes (before rows had powers of two of their own, about 0.2 us) the requests take 2.1 us, parts of the
+ * rows 1.6, 5 pending rows 2.2, the state's products and the tree's tables 2.2, the products of nodes
+ * 2.3, 15 levels 3.5. A level costs a barrier: a chain of 64 nodes takes 49 us. The whole mixer of a head
+ * in one workgroup, for up to 16 nodes, took longer (9 nodes 18.0, 16 nodes 20.8 against 17.0 us). */
 #include "nmx_internal.h"
 #include "nmx_a8.h"
 #include "nmx_lanes.h"

@@ -22,9 +22,10 @@
  * order. Each weight is thereby right to 2^-40 of itself (half a unit of rounding, and the polynomial's
  * next term).
  *
- * On MI355X (scan + pick): a row of 248320 with top-k and top-p 16.3 us (6.2 + 10.1), of 32768 with min-p
- * 13.4 (5.9 + 7.5), 5 rows at the temperature alone 12.1 (5.5 + 7.9), 64 rows of 248320 with top-p
- * 0.95 and no peaks 51 (26.6 + 25): 63.6 MB, 12.3 us as a copy. The scan of 64 rows issues 40 vector
+ * On MI355X (scan + pick): a row of 248320 with top-k and top-p 16.4 us (6.0 + 10.1), of 32768 with min-p
+ * 13.6 (5.7 + 7.7), 5 rows at the temperature alone 12.2 (5.5 + 8.0), 64 rows of 248320 with top-p
+ * 0.95 and no peaks 51 (27 + 27): 63.6 MB, 12.3 us as a copy; greedy, a row 7 to 8.6 and 64 rows 14.5. The scan
+ * of 64 rows issues 40 vector
  * instructions a logit, the weight's polynomial and the bin among them (81 % of its cycles; neither more
  * copies of the bins nor two additions for one changed it). A pick is one workgroup's chain of phases. */
 #include "nmx_internal.h"

@@ -1,9 +1,10 @@
 /* The commit of a verified tree (include/nmx.h nmx_tree_commit): the walk from the root along the
  * drafts that were chosen, and the move of what it accepted to where a chain's pass would have left
  * it. One launch: every workgroup redoes the walk (64 nodes: six shuffles and a ballot), so no second
- * launch waits for it; the rest is a copy of a few rows, bound by the round trip to memory: three rows of
- * 18 layers and 14 caches 5.1 us (5.2 MB, 1.0 us as a copy), nine of them 6.7 us (8.8 MB, 1.7 us). One row
- * at a time, each behind the last one's store, took 6.4 and 11.4 us. */
+ * launch waits for it; the rest is a copy of a few rows, bound by round trips to memory that wait for each
+ * other: the parents, tokens and choices, then the position, then rows, then their stores. A path of four nodes (three
+ * drafts) over 18 layers and 14 caches 5.0 us (5.2 MB, 1.0 us as a copy), one of ten 6.7 us (8.8 MB,
+ * 1.7 us). One row at a time, each behind the last one's store, took 6.4 and 11.4 us. */
 #include "nmx_internal.h"
 #include "nmx_lanes.h"
 #include "nmx_tree.h"

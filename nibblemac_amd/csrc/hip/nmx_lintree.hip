@@ -8,8 +8,8 @@
  * unrolls to sums over a node's ancestors:
  *     delta_t = beta_t (v_t - g_t S^T k_t - sum_{a above t} D(t, a) (k_t . k_a) delta_a)
  *     o_t     = g_t S^T q_t + sum_{a above t, t} D(t, a) (q_t . k_a) delta_a
- * so the state is read once, S^T k, S^T q and the products of nodes are 32-bit matrix instructions,
- * and only the deltas remain to be solved, one level of the tree after the other.
+ * so the state is read once, S^T k and S^T q are 32-bit matrix instructions, the products of nodes 16-bit
+ * ones of two parts each, and only the deltas remain to be solved, one level of the tree after the other.
  *
  * A node's sums run over its own ancestors alone (no product with a masked zero), so whatever
  * another branch holds, NaN or infinity, does not reach it.

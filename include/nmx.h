@@ -517,6 +517,136 @@ typedef struct {
 } nmx_tree_commit_args;
 int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p);
 
+/* ---- a batch of sequences -------------------------------------------------------------------
+ * One step of up to NMX_BATCH_MAX sequences with up to NMX_CHUNK_ROWS rows in all: sequence s has the
+ * rows row0[s] .. row0[s + 1] (device int32 [seqs + 1], from 0 on and not falling; values outside [0, n]
+ * are taken as the nearer end; lists that fall leave results unspecified): one row where it decodes, many where it reads a prompt, none where it
+ * waits. Rows past row0[seqs] (a padded batch) are left alone: not read, not written. The reference serves one sequence
+ * (engine/include/pinfer.h). The other calls of a step (products, norms, heads, nmx_sample) take rows
+ * of whatever sequence as they are.
+ *
+ * KV rows lie in pages: a cache is [npages] blocks of nmx_kv_bytes(kv_dtype, nkv, page, hd) bytes, each laid
+ * out as a cache of `page` positions, and position p of sequence s is row p % page of the block
+ * table[s][p / page]. All caches of a model (K and V of each layer) share one table. page is a power of
+ * two from 16 to 256. Entries behind a sequence's last page are never read. */
+#define NMX_BATCH_MAX 256
+typedef struct {
+    int seqs, npages, page, max_pages;
+    int32_t *table;        /* device [seqs][max_pages] */
+    int32_t *len;          /* device [seqs]: rows of each sequence, those of this step among them */
+    int nkv, hd, kv_dtype; /* hd a multiple of 64 up to 512 */
+} nmx_pages;
+
+/* A step's pages: sequence s becomes the first keep[s] rows of sequence from[s] (itself: it goes on, or is
+ * cut back; another one: a fork; anything outside [0, seqs): none, its pages are freed) with room for
+ * add[s] more. All of it happens at once, every source as it was before the call. keep is taken as at
+ * most the source's length, add as at least 0. The rows' pages are shared where sequences keep the same
+ * ones; a partly filled page that another sequence holds too is copied before a sequence adds rows to it
+ * (of several that would add to one that nobody else holds, the first keeps it). Pages are taken from the
+ * lowest free number on, in the sequences' order: for each its copy first, then those of its new rows.
+ *   len[s] = keep + add; table[s]: its pages, -1 behind them where the sequence had some; refs [npages]
+ *   (device): how many sequences hold a page, 0 for a free one. A cache starts with len and refs of zeros.
+ * pack != 0: afterwards the used pages from number U = (how many are used) on move to the free ones below
+ * U, the i-th to the i-th, and tables and refs follow: pages from U on are all free.
+ *   out [4] (device): 0 when done, U' > 0: U' pages are missing, -1 - s: sequence s would have more than
+ *   max_pages; in both cases nothing else is changed; the pages taken; U (pack, else 0); pages moved.
+ * caches (0: none): host array of device pointers, [npages] blocks each, 16-byte aligned: rows are copied
+ * and moved in all of them. work: device scratch of nmx_pages_work_bytes bytes (0 for a shape that is
+ * refused), 16-byte aligned, used by one call at a time. npages <= 2^20, max_pages <= 2^16. Table entries in use have to name pages of the cache. */
+#define NMX_BATCH_KV_MAX 64
+typedef struct {
+    nmx_pages pages;
+    int32_t *refs;
+    const int32_t *from, *keep, *add; /* device [seqs] each */
+    int pack;
+    int caches;
+    void *const *kv;
+    int32_t *out;
+} nmx_pages_args;
+size_t nmx_pages_work_bytes(int npages, int seqs, int max_pages);
+int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work);
+
+/* nmx_attn_prep for a batch: the q rows [n][nh][2 hd] normed and turned in place, the k rows normed,
+ * turned and stored with the v rows at the last positions of their sequences: row row0[s] + i at
+ * len[s] - (row0[s + 1] - row0[s]) + i. Rotary positions have `axes` axes (1 to 4: text has one; time,
+ * height and width of a picture three): frequency i of rot / 2 turns by row rope_pos[row][axis[i]], column
+ * i, of the tables [rope_rows][rot / 2] (values outside are taken as the nearer end). rope_pos: device
+ * int32 [n][axes], or NULL: a row's position in its sequence on every axis. axis: host array [rot / 2],
+ * read by the call, or NULL: axis 0. A row without a place (a negative position, past max_pages, a table entry
+ * that is no page) is turned but not stored. One axis: rows equal nmx_attn_prep's bit for bit.
+ *
+ * nmx_attn for a batch: row row0[s] + i sees the positions of its sequence up to its own; o *= sigmoid(gate);
+ * + A8 of the n rows. Group j, sequences group0[j] .. group0[j + 1] (device int32 [groups + 1], not falling),
+ * begins with shared[j] rows (device [groups]) that are the same in all of them: they are read once for
+ * the whole group, by the table of its first sequence that has rows (no more than come before the rows of
+ * any of its sequences count). groups 0: nothing shared. A row that sees nothing gives 0. Sums and softmax
+ * statistics are 32 bits; results are right to 32-bit rounding (operands of 22 bits where more than 16 query
+ * rows of a KV head meet the same keys) and do not depend on the other rows. Rows of pages that a row sees hold finite
+ * values; what lies behind the last position of a page may be anything. work: device scratch of
+ * nmx_attn_batch_work_bytes bytes (0 for a shape that is refused; enough for all lengths), 16-byte aligned,
+ * used by one call at a time. nh <= 1024, q, the caches and o 16-byte aligned. */
+typedef struct {
+    nmx_pages pages;
+    int n;
+    const int32_t *row0;
+    int nh, rot;
+    float *q;                           /* [n][nh][2 hd] query | gate */
+    const float *k_in, *v_in;           /* [n][nkv hd] */
+    const float *q_norm, *k_norm;
+    float eps, scale;
+    const float *rope_cos, *rope_sin;
+    int rope_rows, axes;
+    const uint8_t *axis;
+    const int32_t *rope_pos;
+    void *kc, *vc;
+    int groups;
+    const int32_t *group0, *shared;
+    float *o;                           /* [n][nh hd] */
+    nmx_a8 a8;
+} nmx_attn_batch_args;
+int nmx_attn_batch_prep(nmx_ctx *ctx, const nmx_attn_batch_args *p);
+size_t nmx_attn_batch_work_bytes(int n, int seqs, int groups, int nh, int nkv, int hd);
+int nmx_attn_batch(nmx_ctx *ctx, const nmx_attn_batch_args *p, void *work);
+
+/* nmx_lin_mix for a batch, without a log: sequence s starts from slot from[s] of state [seqs][3][C] and
+ * S [seqs][heads dv dk] (device int32 [seqs], or NULL: its own; a value outside [0, seqs): zeros, a new
+ * sequence), and what its rows leave goes to slot s of state_out and S_out. With from NULL these may be
+ * state and S themselves (in place); else they overlap neither. A sequence without rows has its slot copied. Rows as in
+ * row0; `most`: no sequence has more (what one has above it is not read and its state is that of the
+ * rows below). y and the A8 have n rows. Results equal nmx_lin_mix's on each sequence bit for bit.
+ * Of a: pre.out, pre.beta, pre.decay, pre.xin, rule.qkv, .decay, .beta, .o, .log, .pend, .keep, .log0 and
+ * .keep_dev are not used (pre.xin and rule.log have to be NULL, keep 0). conv_k 4, dk 64 or 128, dv a
+ * multiple of 32 with dk <= dv <= 128 and 2 dk + dv <= 4 dv - 64, rep 1 in place; most <= 64. */
+typedef struct {
+    int seqs, most;
+    const int32_t *row0;
+    const int32_t *from;
+    float *state_out, *S_out;
+} nmx_lin_batch;
+int nmx_lin_mix_batch(nmx_ctx *ctx, const nmx_lin_mix_args *a, const nmx_lin_batch *b);
+
+/* Low-rank adapters of many requests beside the projections that share x: for each row t with adapter
+ * m = adapter[t] (device int32 [n]; a value outside [0, adapters): none, the row is left alone), Y[s][t] += scale[m]
+ * B[s][m] (A[s][m] x[t]) for each of the count matrices; A[s] is [adapters][rank][cols] and B[s]
+ * [adapters][rows[s]][rank], both of w_dtype 0 fp32, 1 binary16 or 2 bfloat16. ranks (device [adapters],
+ * may be NULL): an adapter's own rank where it is less, what lies behind it in A and B is not used and may be
+ * anything. Y is what nmx_q4k_matmul* left there (or the residual). Products and sums are 32 bits, in an
+ * order that depends on the shapes alone. n <= NMX_CHUNK_ROWS, cols a multiple of 32 up to 32768, rank <= 256,
+ * rows <= 2^20; x 16-byte aligned rows; A and B 16-byte aligned. work: device scratch of nmx_lora_work_bytes bytes
+ * (0 for a shape that is refused), 16-byte aligned, used by one call at a time. */
+typedef struct {
+    int n, cols, x_stride, count;
+    const float *x;
+    int adapters, rank, w_dtype;
+    const int32_t *adapter, *ranks;
+    const float *scale;
+    const void *A[NMX_MAX_SEGS], *B[NMX_MAX_SEGS];
+    int rows[NMX_MAX_SEGS], y_stride[NMX_MAX_SEGS];
+    float *Y[NMX_MAX_SEGS];
+} nmx_lora_args;
+size_t nmx_lora_work_bytes(int n, int count, int rank);
+int nmx_lora(nmx_ctx *ctx, const nmx_lora_args *p, void *work);
+
 /* ---- sampling -----------------------------------------------------------------------------
  * A token for each of n rows of logits (row r at logits + r stride, vocab values), from a uniform
  * number per row. The reference decodes greedily only; this stands where a program that samples has

@@ -1,0 +1,826 @@
+/* Gated attention of a batch of sequences over paged KV caches (include/nmx.h nmx_attn_batch_prep,
+ * nmx_attn_batch): o = softmax(q K^T scale) V sigmoid(gate) of every row over its own sequence up to its
+ * own position, prefixes that a group of sequences shares read once for the group.
+ *
+ * The work is a list of segments: for each group the rows of all its sequences against the shared prefix,
+ * for each sequence its rows against what follows. A segment has units (KV head, tile of query rows), a
+ * unit steps of 32 positions, and the steps of all units in a row are cut into equal shares, one for each
+ * workgroup, whatever the lengths: a share may end one unit and begin others. Lengths are on the device,
+ * so every workgroup makes the list itself (a scan over at most 512 segments). What a workgroup finds of a
+ * unit is a part (weighted values, maximum, sum); attn_batch_join_k adds a row's parts in order.
+ *
+ * Two inner products. Up to 16 query rows (a token of each sequence: the heads of a KV group): fp32
+ * vector instructions, a wave streaming rows from memory into registers, 16 columns a lane, the keys of the
+ * next positions requested while the values of the current ones are added and the other way round; no LDS and no
+ * barrier on the way. More rows: the matrix cores over tiles in LDS (nmx_attnmx.h). */
+#include "nmx_internal.h"
+#include "nmx_a8.h"
+#include "nmx_attn.h"
+#include "nmx_attnmx.h"
+#include "nmx_batch.h"
+#include "nmx_lanes.h"
+#include "nmx_math.h"
+#include "nmx_rms.h"
+
+namespace {
+
+/* ---- norms, rotary positions, rows into pages ------------------------------------------------ */
+struct PrepBatch {
+    PageDev pg;
+    int n, nh, rot;
+    const int32_t *row0;
+    float *q;
+    const float *k_in, *v_in, *q_norm, *k_norm;
+    float eps;
+    const float *rcos, *rsin;
+    int rope_rows, axes;
+    const int32_t *rope_pos;
+    void *kc, *vc;
+    uint32_t axis[16]; /* two bits for each frequency */
+};
+
+template <int KVT>
+__global__ __launch_bounds__(512) void attn_batch_prep_k(PrepBatch a) {
+    extern __shared__ float sq[];
+    __shared__ float buf[512];
+    __shared__ float red[8];
+    const int t = blockIdx.y, u = blockIdx.x, i = threadIdx.x, hd = a.pg.hd, h2 = a.rot / 2, nkv = a.pg.nkv;
+    const bool is_k = u < nkv;
+    float v = is_k ? a.k_in[(size_t)t * nkv * hd + u * hd + i] : a.q[((size_t)t * a.nh + (u - nkv)) * 2 * hd + i];
+    const float w = is_k ? a.k_norm[i] : a.q_norm[i];
+    const float val = is_k ? a.v_in[(size_t)t * nkv * hd + u * hd + i] : 0.0f;
+    const int f = i < h2 ? i : i - h2; /* the frequency of columns below rot */
+    const bool turns = i < 2 * h2;
+    int at = 0;
+    if (turns && a.rope_pos) at = a.rope_pos[t * a.axes + (a.axis[f >> 4] >> 2 * (f & 15) & 3)];
+    const int s = seq_of_row(a.row0, a.pg.seqs, t);
+    if (s < 0) return; /* uniform over the workgroup */
+    const SeqRows rows = seq_rows(a.row0, s, a.n);
+    if (t >= rows.r0 + rows.count) return;
+    const int p = seq_len(a.pg, s) - rows.count + t - rows.r0;
+    if (!a.rope_pos) at = p;
+    at = at < 0 ? 0 : at < a.rope_rows ? at : a.rope_rows - 1;
+    float c = 0.0f, sn = 0.0f;
+    if (turns) c = a.rcos[(size_t)at * h2 + f], sn = a.rsin[(size_t)at * h2 + f];
+    int id = -1;
+    if (is_k && p >= 0) id = a.pg.table[(size_t)s * a.pg.max_pages + (p >> a.pg.shift)];
+    sq[i] = v * v;
+    __syncthreads();
+    const float ss = ordered_sum4(sq, hd, red);
+    const float r = 1.0f / sqrtf(ss / (float)hd + a.eps);
+    v = (v * r) * w;
+    buf[i] = v;
+    __syncthreads();
+    if (i < h2) v = buf[i] * c - buf[i + h2] * sn;
+    else if (turns) v = buf[i] * c + buf[i - h2] * sn;
+    if (!is_k) {
+        a.q[((size_t)t * a.nh + (u - nkv)) * 2 * hd + i] = v;
+    } else if ((uint32_t)id < (uint32_t)a.pg.npages) { /* uniform per workgroup */
+        nmx_attn_dev d{}; /* a block is a cache of `page` positions */
+        d.nkv = nkv, d.hd = hd, d.max_ctx = 1 << a.pg.shift;
+        const size_t R = ((size_t)u << a.pg.shift) + (p & (d.max_ctx - 1));
+        kv_store<KVT>((char *)a.kc + id * a.pg.block, d, R, i, v, red);
+        kv_store<KVT>((char *)a.vc + id * a.pg.block, d, R, i, val, red);
+    }
+}
+
+/* ---- the list of segments ---------------------------------------------------------------------- */
+constexpr int AB_SEGS = 2 * NMX_BATCH_MAX; /* a prefix for each group, the rest of each sequence */
+constexpr int AB_WGS = 256;                /* shares: a workgroup to a CU */
+constexpr int AB_VR = 16;                  /* query rows that the vector instructions take */
+/* a step of 32 positions costs a workgroup about as long by either product, tiles of many rows half as much again */
+constexpr int AB_COST_V = 2, AB_COST_M = 3;
+
+struct Seg {
+    unsigned long long c0; /* cost of all steps before this segment */
+    uint32_t unit;         /* the cost of one unit: all its steps; 0: nothing to do */
+    uint32_t u0;           /* units of its kind (vector, matrix) before it */
+    int m;                 /* query rows: rows times heads of a KV group */
+    int p0, p1;            /* positions */
+    int r0, seq;           /* first row; the sequence whose table is read */
+    int last;              /* the first row sees positions below last + 1, the next ones one more each (a prefix: all) */
+    int group;             /* of a sequence: its group, -1 none */
+};
+struct Plan {
+    unsigned long long per; /* the cost of a share */
+    Seg seg[AB_SEGS];       /* the groups, then the sequences */
+};
+
+struct BatchAttn {
+    PageDev pg;
+    int n, nh, groups;
+    const int32_t *row0, *group0, *shared;
+    const float *q;
+    const void *kc, *vc;
+    float scale;
+    Plan *plan;
+    float *part_v, *part_m; /* parts of the vector kind [slot][16][hd], of the matrix kind [slot][tile][columns] */
+    float4 *stat_v, *stat_m;
+    int jcols;
+    float *o;
+    int8_t *aq;
+    float *ad, *afs;
+};
+
+template <int HDP>
+constexpr int tile_rows() { /* of the matrix kind */
+    return 16 * ctx_waves<HDP>();
+}
+template <int HDP>
+constexpr int halves() { /* of 512 columns, a unit makes 256 */
+    return HDP > 256 ? 2 : 1;
+}
+
+/* The list, by every thread of the workgroup: seg[0 .. groups + seqs) in LDS, the cost of a share returned. */
+template <int HDP>
+__device__ unsigned long long make_list(const BatchAttn &a, Seg *seg) {
+    constexpr int TH = 64 * ctx_waves<HDP>(), PER = AB_SEGS / TH;
+    __shared__ int ctx_s[NMX_BATCH_MAX], first_s[NMX_BATCH_MAX], g0_s[NMX_BATCH_MAX + 1];
+    __shared__ unsigned long long sum_s[2][TH / 64];
+    const int tid = threadIdx.x, S = a.pg.seqs, G = a.groups, rep = a.nh / a.pg.nkv, lane = tid & 63, wave = tid >> 6;
+    /* sequences: their rows and the positions before them */
+    SeqRows rows{0, 0};
+    int len = 0, share = 0;
+    bool falls = false;
+    if (tid < S) rows = seq_rows(a.row0, tid, a.n), len = seq_len(a.pg, tid), falls = rows.count < 0;
+    if (tid < G) {
+        share = a.shared[tid], ctx_s[tid] = 0x7fffffff, first_s[tid] = S;
+        falls |= a.group0[tid] > a.group0[tid + 1];
+    }
+    for (int g = tid; G && g <= G; g += TH) g0_s[g] = a.group0[g];
+    /* a list that falls has no rows: the workspace holds the parts of lists that do not */
+    if (__syncthreads_or(falls)) rows = {0, 0};
+    int group = -1;
+    if (tid < S && G) { /* the last group that begins at or before it */
+        int lo = -1, hi = G; /* g0[lo] <= tid < g0[hi] */
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (g0_s[mid] <= tid) lo = mid;
+            else hi = mid;
+        }
+        if (lo >= 0 && tid < g0_s[lo + 1]) group = lo;
+        if (group >= 0 && rows.count) atomicMin(&ctx_s[group], len - rows.count), atomicMin(&first_s[group], tid);
+    }
+    if (tid < S) {
+        Seg &x = seg[G + tid];
+        x.r0 = rows.r0, x.m = rows.count, x.p1 = len, x.group = group;
+    }
+    __syncthreads();
+    if (tid < G) {
+        Seg &x = seg[tid];
+        const int first = first_s[tid];
+        x.m = 0, x.r0 = 0, x.p0 = 0, x.p1 = 0, x.seq = 0, x.last = 0x7ffffffe, x.group = -1;
+        if (first < S) {
+            const int end = g0_s[tid + 1] < S ? g0_s[tid + 1] : S; /* the group's last row */
+            const Seg &l = seg[G + end - 1];
+            x.r0 = seg[G + first].r0, x.m = (l.r0 + l.m - x.r0) * rep, x.seq = first;
+            x.p1 = share < ctx_s[tid] ? share : ctx_s[tid];
+            if (x.p1 < 0) x.p1 = 0;
+        }
+    }
+    __syncthreads();
+    if (tid < S) {
+        Seg &x = seg[G + tid];
+        x.seq = tid, x.last = len - rows.count, x.m = rows.count * rep;
+        x.p0 = group >= 0 && rows.count ? seg[group].p1 : 0;
+    }
+    __syncthreads();
+    /* costs and units before each segment; a thread has PER segments in a row */
+    unsigned long long cost = 0, units = 0; /* units: vector kind in the lower half */
+    auto measure = [&](const Seg &x, unsigned long long &unit, unsigned long long &count) {
+        const bool mx = x.m > AB_VR;
+        const int steps = x.m > 0 && x.p1 > x.p0 ? (x.p1 - x.p0 + AT_P - 1) / AT_P : 0;
+        const int tiles = mx ? (x.m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
+        unit = (unsigned long long)steps * (mx ? AB_COST_M : AB_COST_V);
+        count = steps ? (unsigned long long)tiles * a.pg.nkv : 0;
+        return mx;
+    };
+    for (int k = 0; k < PER; k++) {
+        const int j = tid * PER + k;
+        if (j >= G + S) break;
+        unsigned long long unit, count;
+        const bool mx = measure(seg[j], unit, count);
+        cost += unit * count, units += mx ? count << 32 : count;
+    }
+    const unsigned long long ci = nmx_scan_wave(cost), ui = nmx_scan_wave(units);
+    if (lane == 63) sum_s[0][wave] = ci, sum_s[1][wave] = ui;
+    __syncthreads();
+    unsigned long long cb = ci - cost, ub = ui - units, all = 0;
+    for (int w = 0; w < TH / 64; w++) {
+        if (w < wave) cb += sum_s[0][w], ub += sum_s[1][w];
+        all += sum_s[0][w];
+    }
+    for (int k = 0; k < PER; k++) {
+        const int j = tid * PER + k;
+        if (j >= G + S) break;
+        Seg &x = seg[j];
+        unsigned long long unit, count;
+        const bool mx = measure(x, unit, count);
+        x.c0 = cb, x.unit = count ? (uint32_t)unit : 0, x.u0 = (uint32_t)(mx ? ub >> 32 : ub);
+        cb += unit * count, ub += mx ? count << 32 : count;
+    }
+    __syncthreads();
+    return (all + AB_WGS - 1) / AB_WGS;
+}
+
+/* ---- the shares ---------------------------------------------------------------------------------- */
+/* One KV head of a paged cache as a sequence sees it. */
+template <int KVT>
+struct PagedHead {
+    const char *cache;
+    const int32_t *table;
+    size_t block;
+    int npages, shift, mask, hd;
+    uint32_t row, scales; /* the head's first row and first scale in a block, bytes */
+    static constexpr int SIZE = KVT == KV_F32 ? 4 : KVT == KV_F16 ? 2 : 1;
+    __device__ __forceinline__ PagedHead(const PageDev &pg, const void *cache, int seq, int g)
+        : cache((const char *)cache), table(pg.table + (size_t)seq * pg.max_pages), block(pg.block), npages(pg.npages),
+          shift(pg.shift), mask((1 << pg.shift) - 1), hd(pg.hd), row(((uint32_t)g << pg.shift) * pg.hd * SIZE),
+          scales((((uint32_t)pg.nkv << pg.shift) * pg.hd) + ((uint32_t)g << pg.shift) * 4) {}
+    /* an entry that is no page of the cache: any page stands for it */
+    __device__ __forceinline__ int page_of(int p) const {
+        const int id = table[p >> shift];
+        return (uint32_t)id < (uint32_t)npages ? id : 0;
+    }
+    __device__ __forceinline__ const char *at(int id, int p, int col) const {
+        return cache + (size_t)id * block + (row + (uint32_t)((p & mask) * hd + col) * SIZE);
+    }
+    __device__ __forceinline__ Raw8<KVT> load8(int id, int p, int col) const {
+        Raw8<KVT> r;
+        const char *s = at(id, p, col);
+        if constexpr (KVT == KV_F32) r.a = *(const uint4 *)s, r.b = *(const uint4 *)(s + 16);
+        else if constexpr (KVT == KV_F16) r.a = *(const uint4 *)s;
+        else r.a = *(const uint2 *)s;
+        return r;
+    }
+    __device__ __forceinline__ float scale(int id, int p) const {
+        if constexpr (KVT == KV_I8) return *(const float *)(cache + (size_t)id * block + scales + (uint32_t)(p & mask) * 4);
+        return 1.0f;
+    }
+};
+
+/* acc + sum over i of 8 values times x[i] */
+__device__ __forceinline__ float widen(const Raw8<KV_F32> &r, int i) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    return __uint_as_float(w[i]);
+}
+__device__ __forceinline__ float widen(const Raw8<KV_F16> &r, int i) {
+    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+    return kv_half_value(w[i >> 1] >> 16 * (i & 1));
+}
+__device__ __forceinline__ float widen(const Raw8<KV_I8> &r, int i) {
+    return (float)(int8_t)((i < 4 ? r.a.x : r.a.y) >> 8 * (i & 3));
+}
+
+/* the sum over W neighbouring lanes, in each of them */
+template <int W>
+__device__ __forceinline__ float sum_group(float v) {
+    auto with = [&](int o) { v += __int_as_float(o); };
+    if (W >= 2) with(nmx_dpp<NMX_DPP_XOR1>(__float_as_int(v)));
+    if (W >= 4) with(nmx_dpp<NMX_DPP_XOR2>(__float_as_int(v)));
+    if (W >= 8) with(nmx_dpp<NMX_DPP_HALF_MIRROR>(__float_as_int(v)));
+    if (W >= 16) with(nmx_dpp<NMX_DPP_MIRROR>(__float_as_int(v)));
+    if (W >= 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    return v;
+}
+/* v of this lane and of the lanes W, 2 W, ... on, combined by f, in all of them */
+template <int W, typename F>
+__device__ __forceinline__ float across_groups(float v, F f) {
+    if (W <= 4) v = f(v, __int_as_float(nmx_dpp<0x124>(__float_as_int(v)))); /* rows of 16 turned by 4 and by 8 */
+    if (W <= 8) v = f(v, __int_as_float(nmx_dpp<0x128>(__float_as_int(v))));
+    if (W <= 16) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+/* What a share finds of a unit of few rows: positions [p0, p1) of segment x's KV head g, to part and stat.
+ * A lane holds 16 columns (two chunks of 8) of 4 query rows; HDP / 16 lanes a position, so a wave has
+ * LG positions at once, VP times. Waves: groups of 4 rows first, then positions, in turns. */
+template <int HDP, int KVT>
+__device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, int g, int p0, int p1, float *part, float4 *stat,
+                                             uint4 *smem) {
+    constexpr int WV = ctx_waves<HDP>(), LPP = HDP / 16, LG = 64 / LPP, VP = KVT == KV_F32 ? 2 : 4;
+    const int lane = lane_id(), wave = wave_id(), l = lane % LPP, lg = lane / LPP, hd = a.pg.hd, rep = a.nh / a.pg.nkv;
+    const int quads = x.m > 8 ? 4 : x.m > 4 ? 2 : 1, rq = wave % quads, ws = wave / quads, NS = WV / quads;
+    const PagedHead<KVT> kh(a.pg, a.kc, x.seq, g), vh(a.pg, a.vc, x.seq, g);
+    int col[2];
+    bool in[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) col[j] = (l + LPP * j) * 8, in[j] = col[j] < hd, col[j] = in[j] ? col[j] : 0;
+    /* the positions of a turn: VP times NS LG neighbours, so that few positions spread over all waves */
+    const int turn = NS * LG * VP, mine = ws * LG + lg;
+    int pg[VP];
+    Raw8<KVT> rk[VP][2], rv[VP][2];
+    float sk[VP], sv[VP];
+    auto place = [&](int base, int v) {
+        const int p = base + v * NS * LG + mine;
+        return p < p1 ? p : p1 - 1;
+    };
+    auto ask = [&](int base) {
+#pragma unroll
+        for (int v = 0; v < VP; v++) pg[v] = kh.page_of(place(base, v));
+    };
+    auto fetch = [&](const PagedHead<KVT> &h, int base, Raw8<KVT>(&r)[VP][2], float(&s)[VP]) {
+#pragma unroll
+        for (int v = 0; v < VP; v++) {
+            const int p = place(base, v);
+#pragma unroll
+            for (int j = 0; j < 2; j++) r[v][j] = h.load8(pg[v], p, col[j]);
+            s[v] = h.scale(pg[v], p);
+        }
+    };
+    ask(p0);
+    /* query rows to LDS, in the order in which the lanes of a position read them: [row][chunk][half][lane][4] */
+    float *qs = (float *)smem;
+    constexpr int Q4 = HDP / 4, QU = (AB_VR * Q4 + 64 * WV - 1) / (64 * WV);
+    float4 qv[QU];
+#pragma unroll
+    for (int u = 0; u < QU; u++) {
+        const int e = u * 64 * WV + 64 * wave + lane, rr = e / Q4, at = rr < x.m ? rr : 0;
+        const int c = (e % LPP + LPP * (e % Q4 / (2 * LPP))) * 8 + e / LPP % 2 * 4;
+        const float *qp = a.q + ((size_t)(x.r0 + at / rep) * a.nh + g * rep + at % rep) * 2 * hd;
+        qv[u] = *(const float4 *)(qp + (c < hd ? c : 0));
+        if (c >= hd || rr >= x.m) qv[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    int lim[4]; /* a row sees positions below it; a row past the last one none */
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int rr = rq * 4 + r, more = rr / rep;
+        lim[r] = rr >= x.m ? 0 : x.last >= p1 ? p1 : x.last + 1 + more < p1 ? x.last + 1 + more : p1;
+    }
+    fetch(kh, p0, rk, sk);
+    fetch(vh, p0, rv, sv);
+#pragma unroll
+    for (int u = 0; u < QU; u++) {
+        const int e = u * 64 * WV + 64 * wave + lane;
+        if (e < AB_VR * Q4) *(float4 *)(qs + 4 * e) = qv[u];
+    }
+    nmx_lds_sync();
+    int q_at = rq * 4 * HDP + 4 * l;
+    ask(p0 + turn);
+    float acc[4][16], m[4], sum[4], lost[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        m[r] = -INFINITY, sum[r] = 0.0f, lost[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[r][i] = 0.0f;
+    }
+    const float qf = a.scale * AT_LOG2E;
+    for (int base = p0; base < p1; base += turn) {
+        asm volatile("" : "+v"(q_at)); /* the rows are read anew each turn: they have no registers to stay in */
+        const float *qr = qs + q_at;
+        float w[VP][4];
+#pragma unroll
+        for (int v = 0; v < VP; v++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) w[v][r] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) { /* 4 columns of the rows and of every position */
+            float4 q[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) q[r] = *(const float4 *)(qr + r * HDP + e * 4 * LPP);
+#pragma unroll
+            for (int v = 0; v < VP; v++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float k = widen(rk[v][e >> 1], 4 * (e & 1) + i);
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        w[v][r] = __builtin_fmaf(k, i == 0 ? q[r].x : i == 1 ? q[r].y : i == 2 ? q[r].z : q[r].w, w[v][r]);
+                }
+        }
+        float f[VP], fv[VP];
+#pragma unroll
+        for (int v = 0; v < VP; v++) f[v] = KVT == KV_I8 ? qf * sk[v] : qf, fv[v] = sv[v];
+        fetch(kh, base + turn, rk, sk); /* behind the last turn the last position again */
+        bool grows = false;
+        float top[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            top[r] = m[r];
+#pragma unroll
+            for (int v = 0; v < VP; v++) {
+                const int p = base + v * NS * LG + mine;
+                const float s = sum_group<LPP>(w[v][r]) * f[v];
+                w[v][r] = p < lim[r] ? s : -INFINITY;
+                top[r] = fmaxf(top[r], w[v][r]);
+            }
+            grows |= top[r] > m[r];
+        }
+        if (__any(grows)) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float down = __builtin_amdgcn_exp2f(m[r] - (top[r] == -INFINITY ? 0.0f : top[r]));
+                m[r] = top[r], sum[r] *= down, lost[r] *= down;
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[r][i] *= down;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float ref = m[r] == -INFINITY ? 0.0f : m[r];
+            float all = 0.0f;
+#pragma unroll
+            for (int v = 0; v < VP; v++) {
+                w[v][r] = __builtin_amdgcn_exp2f(w[v][r] - ref);
+                all += w[v][r];
+                if (KVT == KV_I8) w[v][r] *= fv[v];
+            }
+            const float add = all - lost[r], now = sum[r] + add; /* the roundings of a long share's sum are kept */
+            lost[r] = (now - sum[r]) - add, sum[r] = now;
+        }
+#pragma unroll
+        for (int v = 0; v < VP; v++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = widen(rv[v][j], i);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc[r][8 * j + i] = __builtin_fmaf(y, w[v][r], acc[r][8 * j + i]);
+                }
+        fetch(vh, base + turn, rv, sv);
+        ask(base + 2 * turn);
+    }
+    nmx_lds_sync(); /* the query rows have been read */
+    /* the wave's groups of lanes together, then the waves through LDS */
+    float *vals = (float *)smem;                  /* [WV][4][HDP] */
+    float2 *ml = (float2 *)(vals + WV * 4 * HDP); /* [WV][4]: maximum, sum */
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const float top = across_groups<LPP>(m[r], [](float u, float v) { return fmaxf(u, v); });
+        const float down = __builtin_amdgcn_exp2f(m[r] - (top == -INFINITY ? 0.0f : top));
+        auto add = [](float u, float v) { return u + v; };
+        const float all = across_groups<LPP>((sum[r] - lost[r]) * down, add);
+        if (lane == 0) ml[wave * 4 + r] = make_float2(top, all);
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[r][i] = across_groups<LPP>(acc[r][i] * down, add);
+        if (lg == 0) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float *y = vals + (wave * 4 + r) * HDP + (l + LPP * j) * 8;
+                *(float4 *)y = make_float4(acc[r][8 * j], acc[r][8 * j + 1], acc[r][8 * j + 2], acc[r][8 * j + 3]);
+                *(float4 *)(y + 4) = make_float4(acc[r][8 * j + 4], acc[r][8 * j + 5], acc[r][8 * j + 6], acc[r][8 * j + 7]);
+            }
+        }
+    }
+    __syncthreads();
+    const int c4 = hd / 4;
+    for (int e = 64 * wave + lane; e < x.m * c4; e += 64 * WV) {
+        const int rr = e / c4, c = e % c4 * 4, r = rr & 3, first = rr >> 2;
+        float top = -INFINITY;
+        for (int w = first; w < WV; w += quads) top = fmaxf(top, ml[w * 4 + r].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float all = 0.0f;
+        for (int w = first; w < WV; w += quads) {
+            const float2 y = ml[w * 4 + r];
+            const float f = __builtin_amdgcn_exp2f(y.x - ref);
+            const float4 z = *(const float4 *)(vals + (w * 4 + r) * HDP + c);
+            all = __builtin_fmaf(y.y, f, all);
+            v.x = __builtin_fmaf(z.x, f, v.x), v.y = __builtin_fmaf(z.y, f, v.y);
+            v.z = __builtin_fmaf(z.z, f, v.z), v.w = __builtin_fmaf(z.w, f, v.w);
+        }
+        *(float4 *)(part + (size_t)rr * hd + c) = v;
+        if (c == 0) stat[rr] = make_float4(top, 12.0f, all, 0.0f); /* as the matrix kind's 2^12 high values */
+    }
+}
+
+/* What a share finds of a unit of many rows, one tile of them. */
+template <int HDP, int KVT>
+__device__ __forceinline__ void matrix_piece(const BatchAttn &a, const Seg &x, int g, int tile, int half, int p0, int p1,
+                                             float *part, float4 *stat, uint4 *smem) {
+    constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32;
+    const int lane = lane_id(), wave = wave_id(), c = lane & 15, gq = lane >> 4, hd = a.pg.hd, rep = a.nh / a.pg.nkv;
+    const int row0 = tile * tile_rows<HDP>() + wave * 16, rr = row0 + c, d0 = half * OD;
+    const bool live = rr < x.m;
+    const int i = (live ? rr : 0) / rep, h = g * rep + (live ? rr : 0) % rep;
+    QueryRow<KS> qr(a.q + ((size_t)(x.r0 + i) * a.nh + h) * 2 * hd, live, hd, gq);
+    const PagedHead<KVT> kh(a.pg, a.kc, x.seq, g), vh(a.pg, a.vc, x.seq, g);
+    const int lim = x.last >= p1 ? p1 : x.last + 1 + i < p1 ? x.last + 1 + i : p1;
+    Running<OD / 16> r;
+    attend_tiles<HDP, KVT>(r, qr, a.scale, kh, vh, p0, p1, lim, d0, row0 < x.m, smem);
+    r.l -= r.lc;
+    r.l = nmx_sum_quarters(r.l);
+    if (!live) return;
+    const int at = wave * 16 + c;
+#pragma unroll
+    for (int d = 0; d < OD / 16; d++)
+        if (d0 + 16 * d < hd) *(float4v *)(part + (size_t)at * OD + 16 * d + 4 * gq) = r.o[d];
+    if (gq == 0) stat[at] = make_float4(r.m, (float)r.ve, r.l, 0.0f);
+}
+
+template <int HDP, int KVT>
+__global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(BatchAttn a) {
+    constexpr int TH = 64 * ctx_waves<HDP>(), OD = HDP > 256 ? 256 : HDP;
+    extern __shared__ uint4 smem[];
+    __shared__ Seg seg[AB_SEGS];
+    __shared__ int found_s;
+    const int tid = threadIdx.x, segs = a.groups + a.pg.seqs, w = blockIdx.x;
+    const unsigned long long per = make_list<HDP>(a, seg);
+    if (w == 0) { /* the join's */
+        for (int j = tid; j < segs; j += TH) a.plan->seg[j] = seg[j];
+        if (tid == 0) a.plan->per = per;
+    }
+    unsigned long long c = w * per;
+    const unsigned long long end = c + per;
+    while (c < end) {
+        if (tid == 0) found_s = -1;
+        __syncthreads();
+        for (int j = tid; j < segs; j += TH) {
+            const Seg &x = seg[j];
+            const unsigned long long next = j + 1 < segs ? seg[j + 1].c0 : per * AB_WGS;
+            if (x.unit && c >= x.c0 && c < next) found_s = j; /* the last one's range may pass the whole cost */
+        }
+        __syncthreads();
+        const int j = __builtin_amdgcn_readfirstlane(found_s);
+        if (j < 0) return;
+        const Seg x = seg[j];
+        const bool mx = x.m > AB_VR;
+        const int nkv = a.pg.nkv, tiles = mx ? (x.m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
+        const uint32_t u = (uint32_t)((c - x.c0) / x.unit);
+        if (u >= (uint32_t)(tiles * nkv)) return; /* past the whole cost */
+        const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit, cn = cu + x.unit < end ? cu + x.unit : end;
+        const int each = mx ? AB_COST_M : AB_COST_V;
+        const int s0 = (int)((c - cu + each - 1) / each), s1 = (int)((cn - cu + each - 1) / each);
+        const int p0 = x.p0 + s0 * AT_P, p1 = x.p0 + s1 * AT_P < x.p1 ? x.p0 + s1 * AT_P : x.p1;
+        const int tile = u / nkv, g = u % nkv;
+        const size_t slot = (size_t)w + x.u0 + u;
+        if (mx) {
+            float4 *stat = a.stat_m + slot * tile_rows<HDP>();
+            if (p0 < p1) matrix_piece<HDP, KVT>(a, x, g, tile / halves<HDP>(), tile % halves<HDP>(), p0, p1,
+                                                a.part_m + slot * tile_rows<HDP>() * (HDP > 256 ? OD : HDP), stat, smem);
+            else if (tid < tile_rows<HDP>()) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        } else {
+            float4 *stat = a.stat_v + slot * AB_VR;
+            if (p0 < p1) vector_piece<HDP, KVT>(a, x, g, p0, p1, a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
+            else if (tid < AB_VR) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        }
+        c = cn;
+        __syncthreads();
+    }
+}
+
+/* ---- the join -------------------------------------------------------------------------------------- */
+constexpr int JB = 256;              /* threads */
+constexpr int JB_PARTS = 2 * AB_WGS + 2;
+
+/* Workgroup: a row and head, blockIdx.y a group of a.jcols columns of it (of one half). */
+template <int HDP>
+__global__ __launch_bounds__(JB) void attn_batch_join_k(BatchAttn a) {
+    constexpr int OD = HDP > 256 ? 256 : HDP;
+    __shared__ float red[2][JB / 64], acc_s[JB * 4], w_s[JB_PARTS];
+    __shared__ const float *at_s[JB_PARTS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.x / a.nh, h = blockIdx.x % a.nh;
+    const int hd = a.pg.hd, nkv = a.pg.nkv, rep = a.nh / nkv, g = h / rep, c0 = blockIdx.y * a.jcols, half = c0 / OD;
+    const float gate = a.q[((size_t)t * a.nh + h) * 2 * hd + hd + c0 + (tid < a.jcols ? tid : 0)];
+    const unsigned long long per = a.plan->per;
+    const int s = seq_of_row(a.row0, a.pg.seqs, t);
+    if (s < 0) return; /* uniform over the workgroup */
+    const SeqRows rows = seq_rows(a.row0, s, a.n);
+    if (t >= rows.r0 + rows.count) return; /* a row of no sequence is left as it is */
+    const Seg own = a.plan->seg[a.groups + s];
+    Seg pre = own;
+    pre.unit = 0;
+    if (own.group >= 0) pre = a.plan->seg[own.group];
+    /* the parts of this row and half: those of the prefix, then the sequence's own */
+    int count[2];
+    const float *val[2];
+    const float4 *st[2];
+    size_t vstep[2], sstep[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const Seg &x = k ? own : pre;
+        const int rr = (t - x.r0) * rep + h % rep;
+        count[k] = 0, val[k] = nullptr, st[k] = nullptr, vstep[k] = sstep[k] = 0;
+        if (!x.unit || rr < 0 || rr >= x.m) continue;
+        const bool mx = x.m > AB_VR;
+        const int tr = mx ? tile_rows<HDP>() : AB_VR, width = mx ? OD : hd;
+        const uint32_t u = (mx ? rr / tr * halves<HDP>() + half : 0) * nkv + g;
+        const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit;
+        const uint32_t w0 = (uint32_t)(cu / per), w1 = (uint32_t)((cu + x.unit - 1) / per);
+        const size_t slot = (size_t)w0 + x.u0 + u;
+        count[k] = (int)(w1 - w0) + 1;
+        val[k] = (mx ? a.part_m : a.part_v) + (slot * tr + rr % tr) * width + (mx ? c0 - half * OD : c0);
+        st[k] = (mx ? a.stat_m : a.stat_v) + slot * tr + rr % tr;
+        vstep[k] = (size_t)tr * width, sstep[k] = tr;
+    }
+    const int parts = count[0] + count[1];
+    constexpr int PT = (JB_PARTS + JB - 1) / JB;
+    float4 y[PT];
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < PT; k++) {
+        const int i = tid + JB * k, b = i >= count[0], at = b ? i - count[0] : i;
+        y[k] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        if (i < parts) y[k] = st[b][at * sstep[b]], at_s[i] = val[b] + at * vstep[b];
+        top = fmaxf(top, y[k].x);
+    }
+    top = nmx_max_f32_wave(top);
+    if (lane == 0) red[0][wave] = top;
+    nmx_lds_sync();
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float all = 0.0f;
+#pragma unroll
+    for (int k = 0; k < PT; k++) {
+        const int i = tid + JB * k;
+        if (i >= parts) continue;
+        const float f = __builtin_amdgcn_exp2f(y[k].x - ref);
+        all += y[k].z * f;
+        w_s[i] = y[k].x == -INFINITY ? 0.0f : ldexpf(f, (int)y[k].y - 12);
+    }
+    all = sum_lanes(all);
+    if (lane == 0) red[1][wave] = all;
+    nmx_lds_sync();
+    all = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    /* slots of jcols / 4 threads: a thread takes 4 columns of every slots-th part */
+    const int per_slot = a.jcols >> 2, slots = JB / per_slot, slot = tid / per_slot, col = tid % per_slot * 4;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (slot < slots) {
+        constexpr int PB = 8;
+        for (int i0 = slot; i0 < parts; i0 += PB * slots) {
+            float4 v[PB];
+            float f[PB];
+#pragma unroll
+            for (int k = 0; k < PB; k++) {
+                const int i = i0 + k * slots, j = i < parts ? i : i0;
+                f[k] = i < parts ? w_s[j] : 0.0f;
+                v[k] = *(const float4 *)(at_s[j] + col);
+            }
+#pragma unroll
+            for (int k = 0; k < PB; k++)
+                if (f[k] != 0.0f) { /* a part without a visible position was never written */
+                    acc.x = __builtin_fmaf(f[k], v[k].x, acc.x), acc.y = __builtin_fmaf(f[k], v[k].y, acc.y);
+                    acc.z = __builtin_fmaf(f[k], v[k].z, acc.z), acc.w = __builtin_fmaf(f[k], v[k].w, acc.w);
+                }
+        }
+        *(float4 *)(acc_s + slot * a.jcols + col) = acc;
+    }
+    nmx_lds_sync();
+    if (tid < a.jcols) {
+        float v = 0.0f;
+        for (int k = 0; k < slots; k++) v += acc_s[k * a.jcols + tid];
+        v = all > 0.0f || !(all == all) ? v / all : 0.0f; /* nothing in sight: 0 */
+        v = v * nmx_sigmoid(gate);
+        const int at = h * hd + c0 + tid;
+        a.o[(size_t)t * a.nh * hd + at] = v;
+        if (a.aq) a8_block(v, at >> 5, t, a.n, a.aq, a.ad, a.afs); /* jcols % 64 == 0: whole blocks */
+    }
+}
+
+/* ---- the workspace ----------------------------------------------------------------------------------- */
+struct Room {
+    int hdp, jcols;
+    size_t stat_v, part_m, stat_m, plan, bytes; /* part_v at 0 */
+};
+
+Room make_room(int n, int seqs, int groups, int nh, int nkv, int hd) {
+    Room r;
+    r.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
+    const size_t tr = r.hdp > 256 ? 64 : 128, od = r.hdp > 256 ? 256 : r.hdp, hv = r.hdp > 256 ? 2 : 1;
+    const size_t qr = (size_t)n * (nh / nkv); /* query rows of a KV head */
+    const size_t sv = AB_WGS + (size_t)(seqs + groups) * nkv;
+    /* segments of more than 16 query rows, each a tile more than its whole ones; every row in two of them */
+    const size_t some = qr / (AB_VR + 1);
+    const size_t big = (some < (size_t)seqs ? some : seqs) + (some < (size_t)groups ? some : groups);
+    const size_t sm = big ? AB_WGS + (2 * (qr / tr) + big) * hv * nkv : 0;
+    size_t at = sv * AB_VR * hd * 4;
+    r.stat_v = at, at += sv * AB_VR * sizeof(float4);
+    r.part_m = at, at += sm * tr * od * 4;
+    r.stat_m = at, at += sm * tr * sizeof(float4);
+    r.plan = at, at += (sizeof(Plan) + 15) / 16 * 16;
+    r.bytes = at;
+    /* columns of a join's workgroup: of one half; few rows share their columns out too */
+    int cols = hd;
+    if (hd > 256)
+        for (cols = 256; hd % cols; cols /= 2) {}
+    while ((size_t)n * nh * (hd / cols) < 256 && cols % 128 == 0) cols /= 2;
+    r.jcols = cols;
+    return r;
+}
+
+bool shape_ok(int n, int seqs, int groups, int nh, int nkv, int hd) {
+    return n >= 1 && n <= NMX_CHUNK_ROWS && seqs >= 1 && seqs <= NMX_BATCH_MAX && groups >= 0 && groups <= seqs && nkv >= 1 &&
+           nh >= nkv && nh % nkv == 0 && nh <= 1024 && hd >= 64 && hd <= 512 && hd % 64 == 0;
+}
+
+template <int HDP, int KVT>
+int launch(nmx_ctx *ctx, const BatchAttn &a) {
+    static std::atomic<uint64_t> set0;
+    constexpr int vec = ctx_waves<HDP>() * 4 * (HDP * 4 + 8), mat = ctx_lds<HDP, KVT>();
+    constexpr int lds = vec > mat ? vec : mat;
+    if (nmx_dyn_lds(ctx, (const void *)attn_batch_k<HDP, KVT>, lds, set0)) return -1;
+    attn_batch_k<HDP, KVT><<<AB_WGS, 64 * ctx_waves<HDP>(), lds, ctx->stream>>>(a);
+    NMX_LAUNCHED(ctx, "attn_batch");
+    attn_batch_join_k<HDP><<<dim3((unsigned)(a.n * a.nh), (unsigned)(a.pg.hd / a.jcols)), JB, 0, ctx->stream>>>(a);
+    NMX_LAUNCHED(ctx, "attn_batch_join");
+    return 0;
+}
+template <int KVT>
+int launch_hd(nmx_ctx *ctx, const BatchAttn &a, int hdp) {
+    return hdp == 64 ? launch<64, KVT>(ctx, a) : hdp == 128 ? launch<128, KVT>(ctx, a) :
+           hdp == 256 ? launch<256, KVT>(ctx, a) : launch<512, KVT>(ctx, a);
+}
+
+/* the arguments that both calls use, and their byte ranges */
+struct Sizes {
+    size_t q, cache, table, len, row0;
+};
+int batch_shape(nmx_ctx *ctx, const nmx_attn_batch_args *p, const char *what, PageDev *pg, Sizes *z) {
+    if (!p) return nmx_fail(ctx, "%s: NULL argument", what);
+    if (nmx_pages_check(ctx, p->pages, what, pg)) return -1;
+    if (!shape_ok(p->n, pg->seqs, 0, p->nh, pg->nkv, pg->hd))
+        return nmx_fail(ctx, "%s: bad shape n=%d nh=%d nkv=%d", what, p->n, p->nh, pg->nkv);
+    if (!p->row0 || !p->q || !p->kc || !p->vc) return nmx_fail(ctx, "%s: NULL argument", what);
+    if ((uintptr_t)p->q % 16 || (uintptr_t)p->kc % 16 || (uintptr_t)p->vc % 16)
+        return nmx_fail(ctx, "%s: q or a cache not 16-byte aligned", what);
+    *z = Sizes{(size_t)p->n * p->nh * 2 * pg->hd * 4, pg->block * pg->npages, (size_t)pg->seqs * pg->max_pages * 4,
+               (size_t)pg->seqs * 4, (size_t)(pg->seqs + 1) * 4};
+    if (nmx_overlap(p->q, z->q, p->kc, z->cache) || nmx_overlap(p->q, z->q, p->vc, z->cache) ||
+        nmx_overlap(p->kc, z->cache, p->vc, z->cache))
+        return nmx_fail(ctx, "%s: q and the caches overlap", what);
+    return 0;
+}
+
+} // namespace
+
+extern "C" {
+
+int nmx_attn_batch_prep(nmx_ctx *ctx, const nmx_attn_batch_args *p) {
+    if (!ctx) return -1;
+    PrepBatch a{};
+    Sizes z;
+    if (batch_shape(ctx, p, "nmx_attn_batch_prep", &a.pg, &z)) return -1;
+    const int hd = a.pg.hd, h2 = p->rot / 2;
+    if (!p->k_in || !p->v_in || !p->q_norm || !p->k_norm) return nmx_fail(ctx, "nmx_attn_batch_prep: NULL argument");
+    if (p->rot < 0 || p->rot % 2 || p->rot > hd || (p->rot && (!p->rope_cos || !p->rope_sin || p->rope_rows < 1)))
+        return nmx_fail(ctx, "nmx_attn_batch_prep: rot=%d rope_rows=%d", p->rot, p->rope_rows);
+    if (p->axes < 1 || p->axes > 4) return nmx_fail(ctx, "nmx_attn_batch_prep: axes=%d", p->axes);
+    for (int i = 0; i < h2 && p->axis; i++) {
+        if (p->axis[i] >= p->axes) return nmx_fail(ctx, "nmx_attn_batch_prep: frequency %d on axis %d of %d", i, p->axis[i], p->axes);
+        a.axis[i >> 4] |= (uint32_t)p->axis[i] << 2 * (i & 15);
+    }
+    const size_t ib = (size_t)p->n * a.pg.nkv * hd * 4, hb = (size_t)hd * 4, rb = (size_t)p->rope_rows * h2 * 4;
+    const NmxRange in[] = {{p->k_in, ib}, {p->v_in, ib}, {p->q_norm, hb}, {p->k_norm, hb}, {p->rope_cos, p->rot ? rb : 0},
+                           {p->rope_sin, p->rot ? rb : 0}, {p->rope_pos, p->rope_pos ? (size_t)p->n * p->axes * 4 : 0},
+                           {p->row0, z.row0}, {a.pg.len, z.len}, {a.pg.table, z.table}};
+    if (nmx_hits(in, p->q, z.q) || nmx_hits(in, p->kc, z.cache) || nmx_hits(in, p->vc, z.cache))
+        return nmx_fail(ctx, "nmx_attn_batch_prep: q or a cache overlaps an input");
+    a.n = p->n, a.nh = p->nh, a.rot = p->rot, a.row0 = p->row0, a.q = p->q, a.k_in = p->k_in, a.v_in = p->v_in;
+    a.q_norm = p->q_norm, a.k_norm = p->k_norm, a.eps = p->eps, a.rcos = p->rope_cos, a.rsin = p->rope_sin;
+    a.rope_rows = p->rope_rows, a.axes = p->axes, a.rope_pos = p->rope_pos, a.kc = p->kc, a.vc = p->vc;
+    const nmx_on_device on(ctx);
+    const dim3 grid((unsigned)(a.pg.nkv + p->nh), (unsigned)p->n);
+    const size_t lds = (size_t)hd * 4;
+    const int kv = p->pages.kv_dtype;
+    if (kv == KV_F16) attn_batch_prep_k<KV_F16><<<grid, (unsigned)hd, lds, ctx->stream>>>(a);
+    else if (kv == KV_I8) attn_batch_prep_k<KV_I8><<<grid, (unsigned)hd, lds, ctx->stream>>>(a);
+    else attn_batch_prep_k<KV_F32><<<grid, (unsigned)hd, lds, ctx->stream>>>(a);
+    NMX_LAUNCHED(ctx, "attn_batch_prep");
+    return 0;
+}
+
+size_t nmx_attn_batch_work_bytes(int n, int seqs, int groups, int nh, int nkv, int hd) {
+    return shape_ok(n, seqs, groups, nh, nkv, hd) ? make_room(n, seqs, groups, nh, nkv, hd).bytes : 0;
+}
+
+int nmx_attn_batch(nmx_ctx *ctx, const nmx_attn_batch_args *p, void *work) {
+    if (!ctx) return -1;
+    BatchAttn a{};
+    Sizes z;
+    if (batch_shape(ctx, p, "nmx_attn_batch", &a.pg, &z)) return -1;
+    const int hd = a.pg.hd, seqs = a.pg.seqs, kv = p->pages.kv_dtype;
+    if (p->groups < 0 || p->groups > seqs) return nmx_fail(ctx, "nmx_attn_batch: groups=%d of %d sequences", p->groups, seqs);
+    if (!p->o || !work || (p->a8.q && (!p->a8.d || !p->a8.fs)) || (p->groups && (!p->group0 || !p->shared)))
+        return nmx_fail(ctx, "nmx_attn_batch: NULL argument");
+    if ((uintptr_t)work % 16 || (uintptr_t)p->o % 16) return nmx_fail(ctx, "nmx_attn_batch: work or o not 16-byte aligned");
+    const Room r = make_room(p->n, seqs, p->groups, p->nh, a.pg.nkv, hd);
+    const size_t ob = z.q / 2, ab = p->a8.q ? ob : 0; /* a byte a value, a float to 32 each in d and fs */
+    const NmxRange in[] = {{p->q, z.q}, {p->kc, z.cache}, {p->vc, z.cache}, {p->row0, z.row0}, {a.pg.len, z.len},
+                           {a.pg.table, z.table}, {p->group0, p->groups ? (size_t)(p->groups + 1) * 4 : 0},
+                           {p->shared, (size_t)p->groups * 4}};
+    const NmxRange out[] = {{work, r.bytes}, {p->o, ob}, {p->a8.q, ab / 4}, {p->a8.d, ab / 32}, {p->a8.fs, ab / 32}};
+    for (int i = 0; i < 5; i++) {
+        if (nmx_hits(in, out[i].p, out[i].bytes)) return nmx_fail(ctx, "nmx_attn_batch: an output or work overlaps an input");
+        for (int k = 0; k < i; k++)
+            if (nmx_overlap(out[i].p, out[i].bytes, out[k].p, out[k].bytes))
+                return nmx_fail(ctx, "nmx_attn_batch: outputs and work overlap");
+    }
+    char *ws = (char *)work;
+    a.n = p->n, a.nh = p->nh, a.groups = p->groups, a.row0 = p->row0, a.group0 = p->group0, a.shared = p->shared;
+    a.q = p->q, a.kc = p->kc, a.vc = p->vc, a.scale = p->scale, a.plan = (Plan *)(ws + r.plan);
+    a.part_v = (float *)ws, a.stat_v = (float4 *)(ws + r.stat_v), a.part_m = (float *)(ws + r.part_m);
+    a.stat_m = (float4 *)(ws + r.stat_m), a.jcols = r.jcols, a.o = p->o, a.aq = p->a8.q, a.ad = p->a8.d, a.afs = p->a8.fs;
+    const nmx_on_device on(ctx);
+    return kv == KV_F16 ? launch_hd<KV_F16>(ctx, a, r.hdp) : kv == KV_I8 ? launch_hd<KV_I8>(ctx, a, r.hdp) :
+           launch_hd<KV_F32>(ctx, a, r.hdp);
+}
+
+} /* extern "C" */

@@ -53,6 +53,13 @@ struct LinMix {
     float *ad, *afs;
 };
 
+/* Of a batch (nmx_lin_mix_batch), blockIdx.y the sequence: its rows and slots; all rows of the batch. */
+struct LinMixBatch {
+    int rows, seqs, most;
+    const int32_t *row0, *from;
+    float *state_out, *S_out;
+};
+
 __host__ __device__ constexpr int mix_lds_floats(int n, int dk, int dv) {
     /* q, k (rule layout [n][4][dk/4 + 4]), v, o [n][dv], pending keys [MIX_TB][4][dk/4 + 4],
      * pending deltas [MIX_TB][dv], z of the first tokens [MIX_TB][dv], norm weight [dv],
@@ -61,28 +68,60 @@ __host__ __device__ constexpr int mix_lds_floats(int n, int dk, int dv) {
            dv + 5 * n;
 }
 
-template <int DK4>
-__global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
+template <int DK4, bool BATCH>
+__global__ __launch_bounds__(MIX_MAX_THREADS, BATCH ? 4 : 1) void lin_mix_k(
     const float *__restrict__ raw, const float *__restrict__ z_in, const float *__restrict__ a_in,
     const float *__restrict__ b_in, int raw_stride, int z_stride, int g_stride, int kdim, int rep,
-    int dv_, int n_, LinMix a) {
+    int dv_, int n_, LinMix a, LinMixBatch bt) {
     extern __shared__ __align__(16) float sm[];
     __shared__ float red[8 * 64];
     __shared__ float spdec[MIX_TB]; /* decays of the pending batch (red serves the L2 norms) */
     __shared__ uint64_t sx2[32];    /* the gate exp's 2^(i/32) table */
     __shared__ float sgh[2];        /* the head's A (or A_log) and dt_bias */
     constexpr int DK = DK4 * 4, PAD = DK4 + 4, ROW = 4 * PAD;
-    const int n = n_, dv = dv_, heads = a.heads;
+    int n = n_;
+    const int dv = dv_, heads = a.heads;
     const int h = blockIdx.x, tid = threadIdx.x, T = 4 * dv, c = tid & 3; /* the launch's size */
     const int j = tid >> 2; /* value column of the quad (T = 4 dv) */
     const int kh = h / rep, kd = kdim;
     const size_t logw = (size_t)DK + dv + 1;
-    const bool logged = a.log != nullptr;
+    const bool logged = !BATCH && a.log != nullptr;
+    /* the rows of this sequence, the slot that its state comes from (none: zeros), its own slot */
+    int first = 0;
+    bool fresh = false;
+    float *Sto = a.S, *cto = a.state;
+    if constexpr (BATCH) {
+        const int s = blockIdx.y;
+        const size_t cs = (size_t)3 * a.C, ss = (size_t)heads * dv * DK;
+        const int from = bt.from ? bt.from[s] : s;
+        const int r0 = bt.row0[s], r1 = bt.row0[s + 1];
+        first = r0 < 0 ? 0 : r0 > bt.rows ? bt.rows : r0;
+        n = (r1 > bt.rows ? bt.rows : r1) - first;
+        n = n < 0 ? 0 : n > bt.most ? bt.most : n;
+        fresh = from < 0 || from >= bt.seqs;
+        a.S += (fresh ? 0 : from) * ss, a.state += (fresh ? 0 : from) * cs;
+        Sto = bt.S_out + s * ss, cto = bt.state_out + s * cs;
+        raw += (size_t)first * raw_stride, z_in += (size_t)first * z_stride;
+        a_in += (size_t)first * g_stride, b_in += (size_t)first * g_stride;
+        if (a.y) a.y += (size_t)first * a.y_stride;
+    }
+    /* a key head's channels are its first value head's to write */
+    const bool conv_own = !BATCH || tid >= 2 * DK || h % rep == 0;
+    if (BATCH && n == 0) { /* nothing to add: the slot goes on as it is */
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        const size_t at = (size_t)h * dv * DK;
+        for (int x = 4 * tid; x < dv * DK; x += 4 * T) *(float4 *)(Sto + at + x) = fresh ? zero : *(const float4 *)(a.S + at + x);
+        const int ci = tid, gc = ci < DK ? kh * DK + ci : ci < 2 * DK ? kd + kh * DK + (ci - DK) : 2 * kd + h * dv + (ci - 2 * DK);
+        if (ci < 2 * DK + dv && conv_own)
+            for (int r = 0; r < 3; r++) cto[(size_t)r * a.C + gc] = fresh ? 0.0f : a.state[(size_t)r * a.C + gc];
+        return;
+    }
     float *sq = sm, *sk = sq + n * ROW, *sv = sk + n * ROW, *so = sv + n * dv;
     float *sp = so + n * dv, *spd = sp + MIX_TB * ROW, *sz = spd + MIX_TB * dv;
     float *sw = sz + MIX_TB * dv, *sbet = sw + dv, *sdec = sbet + n, *srn = sdec + n;
     auto kidx = [](int i) { return (i / DK4) * PAD + i % DK4; }; /* rule layout of key i */
-    const int n0 = n < MIX_TB ? n : MIX_TB; /* tokens whose inputs are requested at entry */
+    constexpr int TB = BATCH ? 4 : MIX_TB; /* of a batch fewer: two workgroups share a CU's registers */
+    const int n0 = n < TB ? n : TB; /* tokens whose inputs are requested at entry */
 
     /* ==== every input of the first batch is requested here, before any of it is used; the
      * recurrence state last, since loads complete in order and the state is needed only by
@@ -92,29 +131,29 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
     const int pb0 = a.keep < MIX_TB ? a.keep : MIX_TB;
     float pkey[2], pdel[2], pdec = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
+    for (int e = 0; e < 2 && !BATCH; e++) {
         const int x = e * T + tid, uk = x / DK, ik = x - uk * DK, ud = x / dv, jd = x - ud * dv;
         pkey[e] = 0.0f, pdel[e] = 0.0f;
         if (uk < pb0) pkey[e] = a.pend[((size_t)uk * heads + h) * logw + ik];
         if (ud < pb0) pdel[e] = a.pend[((size_t)ud * heads + h) * logw + DK + jd];
     }
-    if (tid < pb0) pdec = a.pend[((size_t)tid * heads + h) * logw + DK + dv];
+    if (!BATCH && tid < pb0) pdec = a.pend[((size_t)tid * heads + h) * logw + DK + dv];
     /* conv: thread tid < nch owns channel tid (K = 4: 3 state rows, the taps as one float4) */
     const int nch = 2 * DK + dv, ci = tid;
     const bool conv_on = ci < nch;
     const int gc = ci < DK ? kh * DK + ci : ci < 2 * DK ? kd + kh * DK + (ci - DK)
                                                         : 2 * kd + h * dv + (ci - 2 * DK);
-    float cwin[3], cx[MIX_TB];
+    float cwin[3], cx[TB];
     float4 cw = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int r = 0; r < 3; r++) cwin[r] = 0.0f;
     if (conv_on) {
 #pragma unroll
-        for (int r = 0; r < 3; r++) cwin[r] = a.state[(size_t)r * a.C + gc];
+        for (int r = 0; r < 3; r++) cwin[r] = fresh ? 0.0f : a.state[(size_t)r * a.C + gc];
         cw = *(const float4 *)(a.conv_w + (size_t)gc * 4);
     }
 #pragma unroll
-    for (int u = 0; u < MIX_TB; u++) {
+    for (int u = 0; u < TB; u++) {
         cx[u] = 0.0f;
         if (conv_on && u < n0) cx[u] = raw[(size_t)u * raw_stride + gc];
     }
@@ -139,30 +178,30 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
     }
     if (w_on) wq = *(const float4 *)(a.w + 4 * tid);
     /* recurrence state of the quad's keys */
-    float *Sp = a.S + state_lane(h, j, c, DK, dv);
+    const float *Sf = a.S + state_lane(h, j, c, DK, dv);
+    float *Sp = Sto + state_lane(h, j, c, DK, dv);
     const int SS = state_slot(j, dv); /* a wave's loads: one contiguous 1 KB run each */
     float s[DK4];
 #pragma unroll
     for (int r = 0; r < DK4; r += 4) {
-        const float4 x = *(const float4 *)(Sp + (r >> 2) * SS);
+        const float4 x = *(const float4 *)(Sf + (r >> 2) * SS);
         s[r] = x.x, s[r + 1] = x.y, s[r + 2] = x.z, s[r + 3] = x.w;
     }
-
     /* pending rows to replay: the host's bound, or fewer from the device control block */
-    int keep = a.keep;
-    if (a.keep_dev) {
+    int keep = BATCH ? 0 : a.keep;
+    if (!BATCH && a.keep_dev) {
         const int kd_ = *a.keep_dev;
         keep = kd_ < keep ? kd_ : keep;
     }
 
     /* ---- requested values that later phases read from LDS ---- */
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
+    for (int e = 0; e < 2 && !BATCH; e++) {
         const int x = e * T + tid, uk = x / DK, ik = x - uk * DK, ud = x / dv;
         if (uk < pb0) sp[uk * ROW + kidx(ik)] = pkey[e];
         if (ud < pb0) spd[x] = pdel[e];
     }
-    if (tid < pb0) spdec[tid] = pdec;
+    if (!BATCH && tid < pb0) spdec[tid] = pdec;
     if (z_on) *(float4 *)(sz + 4 * tid) = zq;
     if (w_on) *(float4 *)(sw + 4 * tid) = wq;
     if (tid < 32) sx2[tid] = x2v;
@@ -175,18 +214,18 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
         const float wc[4] = {cw.x, cw.y, cw.z, cw.w};
 #pragma unroll
         for (int r = 0; r < 3; r++) win[r] = cwin[r];
-        for (int t0 = 0; t0 < n; t0 += MIX_TB) {
-            const int nb = n - t0 < MIX_TB ? n - t0 : MIX_TB;
-            float xt[MIX_TB];
+        for (int t0 = 0; t0 < n; t0 += TB) {
+            const int nb = n - t0 < TB ? n - t0 : TB;
+            float xt[TB];
 #pragma unroll
-            for (int u = 0; u < MIX_TB; u++) xt[u] = cx[u];
+            for (int u = 0; u < TB; u++) xt[u] = cx[u];
             if (t0 > 0) {
 #pragma unroll
-                for (int u = 0; u < MIX_TB; u++)
+                for (int u = 0; u < TB; u++)
                     xt[u] = u < nb ? raw[(size_t)(t0 + u) * raw_stride + gc] : 0.0f;
             }
 #pragma unroll
-            for (int u = 0; u < MIX_TB; u++) {
+            for (int u = 0; u < TB; u++) {
                 if (u >= nb) continue;
                 const int t = t0 + u;
                 /* taps in order over [state rows (oldest first), x_t] */
@@ -195,20 +234,20 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
                 acc = acc + wc[2] * win[2];
                 acc = acc + wc[3] * xt[u];
                 win[0] = win[1], win[1] = win[2], win[2] = xt[u];
-                if (t == 0 && a.xin) { /* logged pass: token 0 is committed in place */
+                if (!BATCH && t == 0 && a.xin) { /* logged pass: token 0 is committed in place */
 #pragma unroll
                     for (int q = 0; q < 3; q++) a.state[(size_t)q * a.C + gc] = win[q];
                 }
-                if (t > 0 && a.xin) a.xin[(size_t)t * a.C + gc] = xt[u];
+                if (!BATCH && t > 0 && a.xin) a.xin[(size_t)t * a.C + gc] = xt[u];
                 const float yv = nmx_silu(acc);
                 if (ci < DK) sq[t * ROW + kidx(ci)] = yv;
                 else if (ci < 2 * DK) sk[t * ROW + kidx(ci - DK)] = yv;
                 else sv[t * dv + (ci - 2 * DK)] = yv;
             }
         }
-        if (!a.xin) {
+        if (BATCH ? conv_own : !a.xin) {
 #pragma unroll
-            for (int q = 0; q < 3; q++) a.state[(size_t)q * a.C + gc] = win[q];
+            for (int q = 0; q < 3; q++) cto[(size_t)q * a.C + gc] = win[q];
         }
     }
     /* meanwhile the last wave computes the gates, beta = sigmoid(b) and
@@ -322,12 +361,16 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
             }
         }
     }
-    const bool store_now = a.log0 && keep > 0;
+    const bool store_now = !BATCH && a.log0 && keep > 0;
     if (store_now) {
 #pragma unroll
         for (int r = 0; r < DK4; r += 4) *(float4 *)(Sp + (r >> 2) * SS) = make_float4(s[r], s[r + 1], s[r + 2], s[r + 3]);
     }
 
+    if (BATCH && fresh) { /* a new sequence: what was read stands for nothing */
+#pragma unroll
+        for (int r = 0; r < DK4; r++) s[r] = 0.0f;
+    }
     /* ---- recurrence over the tokens (nmx_lin_rule arithmetic) ---- */
     for (int t = 0; t < n; t++) {
         const float *kk = sk + t * ROW + c * PAD, *qq = sq + t * ROW + c * PAD;
@@ -390,7 +433,7 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
         const int col = h * dv + jj;
         if (a.y) a.y[(size_t)t * a.y_stride + col] = yv;
         if (a.aq) {
-            const size_t u = (size_t)(col >> 5) * n + t;
+            const size_t u = (size_t)(col >> 5) * (BATCH ? bt.rows : n) + first + t;
             nmx_a8_store(yv, a.aq + u * 32, a.ad + u, a.afs + u);
         }
     };
@@ -410,7 +453,8 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
             a.y[(size_t)t2 * a.y_stride + c2] = y2;
         }
         if (a.aq) {
-            const size_t u1 = (size_t)(c1 >> 5) * n + t1, u2 = (size_t)(c2 >> 5) * n + t2;
+            const int all = BATCH ? bt.rows : n;
+            const size_t u1 = (size_t)(c1 >> 5) * all + first + t1, u2 = (size_t)(c2 >> 5) * all + first + t2;
             nmx_a8_store2(y1, a.aq + u1 * 32, a.ad + u1, a.afs + u1, y2, a.aq + u2 * 32,
                           a.ad + u2, a.afs + u2);
         }
@@ -428,12 +472,13 @@ __global__ __launch_bounds__(MIX_MAX_THREADS) void lin_mix_k(
     }
 }
 
-template <int DK4>
-int launch_mix(nmx_ctx *ctx, const LinMix &m, size_t lds) {
+template <int DK4, bool BATCH = false>
+int launch_mix(nmx_ctx *ctx, const LinMix &m, size_t lds, const LinMixBatch &b = {}) {
     static std::atomic<uint64_t> lds_set;
-    if (nmx_dyn_lds(ctx, (const void *)lin_mix_k<DK4>, MIX_LDS, lds_set)) return -1;
-    lin_mix_k<DK4><<<dim3((unsigned)m.heads), dim3((unsigned)(4 * m.dv)), lds, ctx->stream>>>(
-        m.raw, m.z, m.a_in, m.b_in, m.raw_stride, m.z_stride, m.g_stride, m.kd, m.rep, m.dv, m.n, m);
+    if (nmx_dyn_lds(ctx, (const void *)lin_mix_k<DK4, BATCH>, MIX_LDS, lds_set)) return -1;
+    const dim3 grid((unsigned)m.heads, BATCH ? (unsigned)b.seqs : 1u);
+    lin_mix_k<DK4, BATCH><<<grid, dim3((unsigned)(4 * m.dv)), lds, ctx->stream>>>(
+        m.raw, m.z, m.a_in, m.b_in, m.raw_stride, m.z_stride, m.g_stride, m.kd, m.rep, m.dv, m.n, m, b);
     NMX_LAUNCHED(ctx, "lin_mix");
     return 0;
 }
@@ -556,6 +601,63 @@ int nmx_lin_mix(nmx_ctx *ctx, const nmx_lin_mix_args *a) { return lin_mix(ctx, a
 
 int nmx_lin_mix_chunk(nmx_ctx *ctx, const nmx_lin_mix_args *a) {
     return lin_mix(ctx, a, true);
+}
+
+int nmx_lin_mix_batch(nmx_ctx *ctx, const nmx_lin_mix_args *a, const nmx_lin_batch *b) {
+    if (!ctx) return -1;
+    if (!a || !b) return nmx_fail(ctx, "nmx_lin_mix_batch: NULL args");
+    const nmx_lin_pre_args &p = a->pre;
+    const nmx_lin_args &r = a->rule;
+    const int n = p.n, dk = p.dk, dv = r.dv, heads = r.heads;
+    if (n < 1 || n > NMX_CHUNK_ROWS || b->seqs < 1 || b->seqs > NMX_BATCH_MAX || b->most < 1 || b->most > 64)
+        return nmx_fail(ctx, "nmx_lin_mix_batch: n=%d seqs=%d most=%d", n, b->seqs, b->most);
+    if (n != r.n || dk != r.dk || p.heads != heads || p.conv_k != 4 || (dk != 64 && dk != 128) || dv < dk ||
+        dv > MIX_MAX_THREADS / 4 || dv % 32 || 2 * dk + dv > 4 * dv - 64 || r.rep < 1 || heads < 1 || heads > 1024 ||
+        heads % r.rep || p.kd != heads / r.rep * dk || p.C != 2 * p.kd + heads * dv)
+        return nmx_fail(ctx, "nmx_lin_mix_batch: shape heads=%d rep=%d dk=%d dv=%d conv_k=%d C=%d kd=%d", heads, r.rep, dk,
+                        dv, p.conv_k, p.C, p.kd);
+    if (!p.raw || !p.state || !p.conv_w || !p.b_in || !p.a_in || !p.dt_bias || (!p.A_log && !p.A) || !r.S || !a->z ||
+        !a->norm_w || !b->row0 || !b->state_out || !b->S_out || (!a->y && !a->a8.q) ||
+        (a->a8.q && (!a->a8.d || !a->a8.fs)))
+        return nmx_fail(ctx, "nmx_lin_mix_batch: NULL argument");
+    if (p.xin || r.log || r.keep || r.log0) return nmx_fail(ctx, "nmx_lin_mix_batch: a log or pending rows");
+    const int vd = heads * dv;
+    if (p.raw_stride < p.C || p.g_stride < heads || a->z_stride < vd || a->z_stride % 4 || (a->y && a->y_stride < vd))
+        return nmx_fail(ctx, "nmx_lin_mix_batch: strides raw=%d gates=%d z=%d y=%d", p.raw_stride, p.g_stride, a->z_stride,
+                        a->y_stride);
+    auto odd = [](const void *q) { return ((uintptr_t)q & 15) != 0; };
+    if (odd(p.conv_w) || odd(a->z) || odd(a->norm_w) || odd(r.S) || odd(b->S_out))
+        return nmx_fail(ctx, "nmx_lin_mix_batch: taps, z, norm weight or a state not 16-byte aligned");
+    const size_t lds = (size_t)mix_lds_floats(b->most, dk, dv) * 4;
+    if (lds > (size_t)MIX_LDS) return nmx_fail(ctx, "nmx_lin_mix_batch: most=%d needs too much LDS", b->most);
+    const bool in_place = r.S == b->S_out && p.state == b->state_out;
+    if (in_place && (b->from || r.rep != 1))
+        return nmx_fail(ctx, "nmx_lin_mix_batch: from and shared key heads need other slots to write");
+    const size_t N = (size_t)n, sb = (size_t)b->seqs * vd * dk * 4, cb = (size_t)b->seqs * 3 * p.C * 4;
+    struct Span {
+        const void *p;
+        size_t b;
+    };
+    const Span out[] = {{b->state_out, cb}, {b->S_out, sb}, {a->y, a->y ? ((N - 1) * a->y_stride + vd) * 4 : 0},
+                        {a->a8.q, a->a8.q ? N * vd : 0}, {a->a8.d, a->a8.q ? N * vd / 8 : 0}, {a->a8.fs, a->a8.q ? N * vd / 8 : 0}},
+               in[] = {{p.state, in_place ? 0 : cb}, {r.S, in_place ? 0 : sb}, {p.raw, ((N - 1) * p.raw_stride + p.C) * 4},
+                       {p.conv_w, (size_t)p.C * 16}, {p.b_in, ((N - 1) * p.g_stride + heads) * 4},
+                       {p.a_in, ((N - 1) * p.g_stride + heads) * 4}, {p.A, p.A ? (size_t)heads * 4 : 0},
+                       {p.A_log, p.A_log ? (size_t)heads * 4 : 0}, {p.dt_bias, (size_t)heads * 4},
+                       {a->z, ((N - 1) * a->z_stride + vd) * 4}, {a->norm_w, (size_t)dv * 4},
+                       {b->row0, (size_t)(b->seqs + 1) * 4}, {b->from, b->from ? (size_t)b->seqs * 4 : 0}};
+    for (const Span &w : out) {
+        for (const Span &x : in)
+            if (nmx_overlap(w.p, w.b, x.p, x.b)) return nmx_fail(ctx, "nmx_lin_mix_batch: an output overlaps an input");
+        for (const Span &x : out)
+            if (&x != &w && nmx_overlap(w.p, w.b, x.p, x.b)) return nmx_fail(ctx, "nmx_lin_mix_batch: outputs overlap");
+    }
+    const LinMix m{n, p.C, p.conv_k, p.kd, p.raw, p.raw_stride, p.state, p.conv_w, nullptr, p.qscale, p.l2eps, p.b_in,
+                   p.a_in, p.g_stride, p.A_log, p.A, p.dt_bias, heads, r.rep, dv, r.S, nullptr, nullptr, 0, 0, nullptr,
+                   a->z, a->z_stride, a->norm_w, a->eps, a->y, a->y_stride, a->a8.q, a->a8.d, a->a8.fs};
+    const LinMixBatch mb{n, b->seqs, b->most, b->row0, b->from, b->state_out, b->S_out};
+    const nmx_on_device on(ctx);
+    return dk == 64 ? launch_mix<16, true>(ctx, m, lds, mb) : launch_mix<32, true>(ctx, m, lds, mb);
 }
 
 int nmx_lin_chunk_ok(int dk, int dv, int conv_k, int heads) {

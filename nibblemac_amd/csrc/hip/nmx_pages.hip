@@ -1,0 +1,326 @@
+/* The pages of a step (include/nmx.h nmx_pages_update): sequences go on, are cut back, fork from each other or
+ * end, and take pages for their new rows.
+ *
+ * pages_plan_k, one workgroup, does everything but move rows, so that no phase waits for another
+ * workgroup: it counts the holders of every page as they will be (additions to refs, exact in any order),
+ * decides which partly filled pages have to be copied before their sequence writes into them, takes the lowest
+ * free pages by running sums over the page counts, and writes tables and lengths; a step that does not fit is
+ * taken back by the opposite additions. A fork's entries go through the workspace, so sequences may
+ * exchange places. pages_copy_k and, with pack, pages_move_k then copy what the plan lists, in all
+ * caches at once. */
+#include "nmx_internal.h"
+#include "nmx_batch.h"
+#include "nmx_lanes.h"
+
+namespace {
+
+constexpr int PP = 1024;          /* threads of the plan */
+constexpr int PP_EACH = 16;       /* pages of a thread in a turn of a search */
+constexpr int PC = 256;           /* threads of a copy */
+constexpr int PC_CHUNK = PC * 64; /* bytes of a workgroup's item: four 16-byte units a thread */
+
+struct Lists { /* in the workspace, then the arrays below */
+    int copies, moves;
+    int4 copy[NMX_BATCH_MAX]; /* from, to, rows */
+};
+struct PagesDev {
+    PageDev pg;
+    int32_t *refs;
+    const int32_t *from, *keep, *add;
+    int pack;
+    int32_t *out;
+    Lists *lists;
+    int32_t *fresh, *holes, *movers, *to; /* [npages] each */
+    int32_t *rows;                        /* [seqs][max_pages]: the entries of sequences that fork */
+};
+
+__device__ __forceinline__ int read_refs(const int32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void add_refs(int32_t *refs, int npages, int page, int v) {
+    if ((uint32_t)page < (uint32_t)npages) (void)__hip_atomic_fetch_add(refs + page, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+/* Running sum over the workgroup, the total in *all (sum_s: PP / 64 words; two barriers). */
+__device__ __forceinline__ uint32_t scan_all(uint32_t v, uint32_t *sum_s, uint32_t *all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t inc = nmx_scan_wave(v);
+    __syncthreads();
+    if (lane == 63) sum_s[wave] = inc;
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+    for (int w = 0; w < PP / 64; w++) {
+        if (w < wave) before += sum_s[w];
+        total += sum_s[w];
+    }
+    *all = total;
+    return before + inc - v;
+}
+
+/* Calls hit(page, rank) for the pages in [0, npages) of which want(refs) is true, in order, while the rank is
+ * below `most`; returns how many there are (all of them where it is less than most). */
+template <typename Want, typename Hit>
+__device__ uint32_t search(const int32_t *refs, int begin, int npages, uint32_t most, uint32_t *sum_s, Want want, Hit hit) {
+    uint32_t found = 0;
+    for (int base = begin; base < npages && found < most; base += PP * PP_EACH) {
+        int v[PP_EACH];
+        const int at = base + (int)threadIdx.x * PP_EACH;
+#pragma unroll
+        for (int i = 0; i < PP_EACH; i++) v[i] = read_refs(refs + (at + i < npages ? at + i : npages - 1));
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < PP_EACH; i++)
+            if (at + i < npages && want(v[i])) mask |= 1u << i;
+        uint32_t all, rank = found + scan_all(__popc(mask), sum_s, &all);
+        for (; mask; mask &= mask - 1, rank++)
+            if (rank < most) hit(at + __ffs(mask) - 1, rank);
+        found += all;
+    }
+    return found;
+}
+
+__global__ __launch_bounds__(PP) void pages_plan_k(PagesDev a) {
+    __shared__ int src_s[NMX_BATCH_MAX], kept_s[NMX_BATCH_MAX], old_s[NMX_BATCH_MAX], all_s[NMX_BATCH_MAX],
+        last_s[NMX_BATCH_MAX], copy_s[NMX_BATCH_MAX];
+    __shared__ uint32_t base_s[NMX_BATCH_MAX], sum_s[PP / 64];
+    __shared__ int wide_s, some_s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.pg.seqs, npages = a.pg.npages, mp = a.pg.max_pages;
+    const int page = 1 << a.pg.shift, shift = a.pg.shift;
+    auto pages_of = [&](long long r) { return (int)((r + page - 1) >> shift); };
+    if (tid == 0) wide_s = S, some_s = 0;
+    __syncthreads();
+    int total = 0, part = 0, last = -1;
+    if (tid < S) {
+        const int f = a.from[tid], old = seq_len(a.pg, tid);
+        int keep = a.keep[tid], add = a.add[tid], src = f >= 0 && f < S ? f : -1;
+        const int most = src < 0 ? 0 : seq_len(a.pg, src);
+        keep = keep < 0 ? 0 : keep < most ? keep : most, add = add < 0 ? 0 : add;
+        const long long len = (long long)keep + add;
+        const bool wide = len > (long long)mp << shift;
+        if (wide) atomicMin(&wide_s, tid);
+        total = wide ? keep : (int)len, part = add > 0 ? keep & (page - 1) : 0;
+        src_s[tid] = src, kept_s[tid] = pages_of(keep), old_s[tid] = pages_of(old), all_s[tid] = pages_of(total);
+        if (part) last = a.pg.table[(size_t)src * mp + kept_s[tid] - 1];
+        if ((uint32_t)last >= (uint32_t)npages) last = -1;
+        if (src != tid || kept_s[tid] < old_s[tid]) some_s = 1; /* entries that change hands */
+    }
+    if (tid < NMX_BATCH_MAX) last_s[tid] = last;
+    __syncthreads();
+    const int wide = wide_s;
+    if (wide < S) {
+        if (tid < 4) a.out[tid] = tid ? 0 : -1 - wide;
+        if (tid == 0) a.lists->copies = 0, a.lists->moves = 0;
+        return;
+    }
+    /* who holds what after the step: a wave for each sequence whose entries change hands. sign -1 takes it back */
+    auto recount = [&](int sign) {
+        for (int s = wave; s < S; s += PP / 64) {
+            const int src = src_s[s], kept = kept_s[s], old = old_s[s];
+            const int32_t *mine = a.pg.table + (size_t)s * mp;
+            for (int e = (src == s ? kept : 0) + lane; e < old; e += 64) add_refs(a.refs, npages, mine[e], -sign);
+            if (src == s || src < 0) continue;
+            const int32_t *theirs = a.pg.table + (size_t)src * mp;
+            for (int e = lane; e < kept; e += 64) {
+                const int p = theirs[e];
+                add_refs(a.refs, npages, p, sign);
+                a.rows[(size_t)s * mp + e] = p;
+            }
+        }
+    };
+    if (some_s) { /* uniform */
+        recount(1);
+        __threadfence();
+        __syncthreads();
+    }
+    /* a page that its sequence would add rows to is copied where another one holds it; where all who hold it
+     * would, the first of them keeps it */
+    bool copy = false;
+    if (tid < S && last >= 0) {
+        const int held = read_refs(a.refs + last);
+        if (held > 1) {
+            int same = 0, before = 0;
+            for (int s = 0; s < S; s++) same += last_s[s] == last, before += s < tid && last_s[s] == last;
+            copy = !(held == same && before == 0);
+        }
+    }
+    if (tid < S) copy_s[tid] = copy;
+    const uint32_t need = tid < S ? (uint32_t)(all_s[tid] - kept_s[tid] + copy) : 0;
+    uint32_t needed, copies;
+    const uint32_t base = scan_all(need, sum_s, &needed), nth = scan_all(copy, sum_s, &copies);
+    if (tid < S) base_s[tid] = base;
+    if (needed) {
+        const uint32_t found = search(a.refs, 0, npages, needed, sum_s, [](int r) { return r == 0; },
+                                      [&](int p, uint32_t i) { a.fresh[i] = p; });
+        if (found < needed) {
+            if (some_s) recount(-1);
+            if (tid < 4) a.out[tid] = tid ? 0 : (int)(needed - found);
+            if (tid == 0) a.lists->copies = 0, a.lists->moves = 0;
+            return;
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    if (copy) {
+        a.lists->copy[nth] = make_int4(last, a.fresh[base], part, 0);
+        add_refs(a.refs, npages, last, -1);
+    }
+    if (tid < S) a.pg.len[tid] = total;
+    /* tables: what a fork keeps, the fresh pages, -1 where there were more */
+    for (int s = wave; s < S; s += PP / 64) {
+        const int src = src_s[s], all = all_s[s], own = kept_s[s] - copy_s[s];
+        int32_t *t = a.pg.table + (size_t)s * mp;
+        if (src != s && src >= 0)
+            for (int e = lane; e < own; e += 64) t[e] = a.rows[(size_t)s * mp + e];
+        for (int e = own + lane; e < all; e += 64) {
+            const int p = a.fresh[base_s[s] + e - own];
+            t[e] = p, a.refs[p] = 1;
+        }
+        for (int e = all + lane; e < old_s[s]; e += 64) t[e] = -1;
+    }
+    if (tid < 4) a.out[tid] = tid == 1 ? (int)needed : 0;
+    if (tid == 0) a.lists->copies = (int)copies, a.lists->moves = 0;
+    if (!a.pack) return;
+    /* the used pages from their number on move to the free ones below it */
+    __threadfence();
+    __syncthreads();
+    const uint32_t used = search(a.refs, 0, npages, ~0u, sum_s, [](int r) { return r != 0; }, [](int, uint32_t) {});
+    const uint32_t moves = search(a.refs, (int)used, npages, ~0u, sum_s, [](int r) { return r != 0; },
+                                  [&](int p, uint32_t i) { a.movers[i] = p; });
+    if (moves)
+        (void)search(a.refs, 0, (int)used, moves, sum_s, [](int r) { return r == 0; }, [&](int p, uint32_t i) { a.holes[i] = p; });
+    __threadfence();
+    __syncthreads();
+    for (uint32_t i = tid; i < moves; i += PP) {
+        const int p = a.movers[i], h = a.holes[i];
+        a.to[p] = h;
+        a.refs[h] = read_refs(a.refs + p), a.refs[p] = 0;
+    }
+    if (tid == 0) a.lists->moves = (int)moves;
+    if (tid == 2 || tid == 3) a.out[tid] = (int)(tid == 2 ? used : moves);
+    if (!moves) return;
+    __threadfence();
+    __syncthreads();
+    for (int s = wave; s < S; s += PP / 64) {
+        int32_t *t = a.pg.table + (size_t)s * mp;
+        for (int e = lane; e < all_s[s]; e += 64) {
+            const int p = t[e];
+            if ((uint32_t)p >= used && (uint32_t)p < (uint32_t)npages) t[e] = a.to[p];
+        }
+    }
+}
+
+struct CopyDev {
+    const Lists *lists;
+    const int32_t *movers, *holes;
+    int caches, nkv, page, row_bytes; /* of one KV head */
+    int scales;
+    size_t block;
+    int chunks; /* items of a head (a copy), of a block (a move) */
+    void *kv[NMX_BATCH_KV_MAX];
+};
+
+/* n bytes (a multiple of 16), at most a chunk */
+__device__ __forceinline__ void copy_chunk(char *dst, const char *src, size_t n) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const size_t at = (size_t)(i * PC + (int)threadIdx.x) * 16;
+        v[i] = *(const u32x4 *)(src + (at < n ? at : 0));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const size_t at = (size_t)(i * PC + (int)threadIdx.x) * 16;
+        if (at < n) *(u32x4 *)(dst + at) = v[i];
+    }
+}
+
+/* The first rows of pages, head by head, in every cache. */
+__global__ __launch_bounds__(PC) void pages_copy_k(CopyDev a) {
+    const long long items = (long long)a.lists->copies * a.caches * a.nkv * a.chunks;
+    for (long long i = blockIdx.x; i < items; i += gridDim.x) {
+        const int chunk = (int)(i % a.chunks), g = (int)(i / a.chunks % a.nkv);
+        const int cache = (int)(i / a.chunks / a.nkv % a.caches);
+        const int4 c = a.lists->copy[i / a.chunks / a.nkv / a.caches];
+        const char *src = (const char *)a.kv[cache] + c.x * a.block;
+        char *dst = (char *)a.kv[cache] + c.y * a.block;
+        const size_t head = (size_t)g * a.page * a.row_bytes, n = (size_t)c.z * a.row_bytes, at = (size_t)chunk * PC_CHUNK;
+        if (at < n) copy_chunk(dst + head + at, src + head + at, n - at < PC_CHUNK ? n - at : PC_CHUNK);
+        if (a.scales && chunk == 0 && (int)threadIdx.x < c.z) { /* a page has at most 256 rows */
+            const size_t s = (size_t)a.nkv * a.page * a.row_bytes + ((size_t)g * a.page + threadIdx.x) * 4;
+            *(float *)(dst + s) = *(const float *)(src + s);
+        }
+    }
+}
+
+/* Whole pages, in every cache. */
+__global__ __launch_bounds__(PC) void pages_move_k(CopyDev a) {
+    const long long items = (long long)a.lists->moves * a.caches * a.chunks;
+    for (long long i = blockIdx.x; i < items; i += gridDim.x) {
+        const int chunk = (int)(i % a.chunks), cache = (int)(i / a.chunks % a.caches), m = (int)(i / a.chunks / a.caches);
+        const size_t at = (size_t)chunk * PC_CHUNK, n = a.block - at;
+        copy_chunk((char *)a.kv[cache] + a.holes[m] * a.block + at, (const char *)a.kv[cache] + a.movers[m] * a.block + at,
+                   n < PC_CHUNK ? n : PC_CHUNK);
+    }
+}
+
+size_t up16(size_t x) { return (x + 15) / 16 * 16; }
+
+} // namespace
+
+extern "C" {
+
+size_t nmx_pages_work_bytes(int npages, int seqs, int max_pages) {
+    if (npages < 1 || npages > (1 << 20) || seqs < 1 || seqs > NMX_BATCH_MAX || max_pages < 1 || max_pages > (1 << 16)) return 0;
+    return up16(sizeof(Lists)) + 4 * up16((size_t)npages * 4) + up16((size_t)seqs * max_pages * 4);
+}
+
+int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work) {
+    if (!ctx) return -1;
+    if (!p) return nmx_fail(ctx, "nmx_pages_update: NULL argument");
+    PagesDev a{};
+    if (nmx_pages_check(ctx, p->pages, "nmx_pages_update", &a.pg)) return -1;
+    if (!p->refs || !p->from || !p->keep || !p->add || !p->out || !work) return nmx_fail(ctx, "nmx_pages_update: NULL argument");
+    if ((uintptr_t)work % 16) return nmx_fail(ctx, "nmx_pages_update: work not 16-byte aligned");
+    if (p->caches < 0 || p->caches > NMX_BATCH_KV_MAX || (p->caches && !p->kv))
+        return nmx_fail(ctx, "nmx_pages_update: caches=%d", p->caches);
+    const int S = a.pg.seqs, np = a.pg.npages, mp = a.pg.max_pages;
+    const size_t cb = a.pg.block * np, sb = (size_t)S * 4, wb = nmx_pages_work_bytes(np, S, mp);
+    const NmxRange in[] = {{p->from, sb}, {p->keep, sb}, {p->add, sb}};
+    NmxRange out[5 + NMX_BATCH_KV_MAX] = {{work, wb}, {a.pg.table, (size_t)S * mp * 4}, {a.pg.len, sb}, {p->refs, (size_t)np * 4},
+                                          {p->out, 16}};
+    CopyDev c{};
+    int no = 5;
+    for (int i = 0; i < p->caches; i++) {
+        if (!p->kv[i] || (uintptr_t)p->kv[i] % 16) return nmx_fail(ctx, "nmx_pages_update: cache %d", i);
+        c.kv[i] = p->kv[i];
+        out[no++] = {p->kv[i], cb};
+    }
+    for (int i = 0; i < no; i++) {
+        if (nmx_hits(in, out[i].p, out[i].bytes)) return nmx_fail(ctx, "nmx_pages_update: what is written overlaps an input");
+        for (int k = 0; k < i; k++)
+            if (nmx_overlap(out[i].p, out[i].bytes, out[k].p, out[k].bytes))
+                return nmx_fail(ctx, "nmx_pages_update: two of the tables, caches, out and work overlap");
+    }
+    char *w = (char *)work;
+    const size_t nb = up16((size_t)np * 4);
+    a.refs = p->refs, a.from = p->from, a.keep = p->keep, a.add = p->add, a.pack = p->pack != 0, a.out = p->out;
+    a.lists = (Lists *)w, w += up16(sizeof(Lists));
+    a.fresh = (int32_t *)w, a.holes = (int32_t *)(w + nb), a.movers = (int32_t *)(w + 2 * nb), a.to = (int32_t *)(w + 3 * nb);
+    a.rows = (int32_t *)(w + 4 * nb);
+    const nmx_on_device on(ctx);
+    pages_plan_k<<<1, PP, 0, ctx->stream>>>(a);
+    NMX_LAUNCHED(ctx, "pages_plan");
+    if (!p->caches) return 0;
+    const int kv = p->pages.kv_dtype, page = p->pages.page;
+    c.lists = a.lists, c.movers = a.movers, c.holes = a.holes, c.caches = p->caches, c.nkv = a.pg.nkv, c.page = page;
+    c.row_bytes = a.pg.hd * (kv == KV_F32 ? 4 : kv == KV_F16 ? 2 : 1), c.scales = kv == KV_I8, c.block = a.pg.block;
+    c.chunks = (page * c.row_bytes + PC_CHUNK - 1) / PC_CHUNK;
+    pages_copy_k<<<1024, PC, 0, ctx->stream>>>(c);
+    NMX_LAUNCHED(ctx, "pages_copy");
+    if (!p->pack) return 0;
+    c.chunks = (int)((c.block + PC_CHUNK - 1) / PC_CHUNK);
+    pages_move_k<<<2048, PC, 0, ctx->stream>>>(c);
+    NMX_LAUNCHED(ctx, "pages_move");
+    return 0;
+}
+
+} /* extern "C" */

@@ -122,6 +122,70 @@ def tree_commit_args(n: int, parent, tok, choice, out, *, ctl=None, vt=None, lin
     return a
 
 
+class Pages(ctypes.Structure):
+    """Mirror of nmx_pages (the layout of a paged cache and its tables)."""
+
+    _fields_ = [("seqs", _i), ("npages", _i), ("page", _i), ("max_pages", _i), ("table", _vp),
+                ("len", _vp), ("nkv", _i), ("hd", _i), ("kv_dtype", _i)]
+
+
+class PagesArgs(ctypes.Structure):
+    """Mirror of nmx_pages_args (src: its `from`)."""
+
+    _fields_ = [("pages", Pages), ("refs", _vp), ("src", _vp), ("keep", _vp), ("add", _vp),
+                ("pack", _i), ("caches", _i), ("kv", _vp), ("out", _vp)]
+
+
+def pages_args(pages: Pages, refs, src, keep, add, caches, out, *, pack: int = 0) -> PagesArgs:
+    """The arguments of Device.pages_update; caches: the device pointers of every paged cache."""
+    a = PagesArgs(pages=pages, refs=_p(refs), src=_p(src), keep=_p(keep), add=_p(add), pack=int(pack),
+                  caches=len(caches), out=_p(out))
+    ptrs = (ctypes.c_void_p * max(1, len(caches)))(*[_p(x) for x in caches])
+    a.kv = ctypes.addressof(ptrs)
+    a.keep_kv = ptrs  # the array lives as long as the arguments
+    return a
+
+
+class AttnBatchArgs(ctypes.Structure):
+    """Mirror of nmx_attn_batch_args."""
+
+    _fields_ = [("pages", Pages), ("n", _i), ("row0", _vp), ("nh", _i), ("rot", _i), ("q", _vp),
+                ("k_in", _vp), ("v_in", _vp), ("q_norm", _vp), ("k_norm", _vp),
+                ("eps", ctypes.c_float), ("scale", ctypes.c_float), ("rope_cos", _vp),
+                ("rope_sin", _vp), ("rope_rows", _i), ("axes", _i), ("axis", _vp),
+                ("rope_pos", _vp), ("kc", _vp), ("vc", _vp), ("groups", _i), ("group0", _vp),
+                ("shared", _vp), ("o", _vp), ("a8", A8)]
+
+
+class LinBatch(ctypes.Structure):
+    """Mirror of nmx_lin_batch (src: its `from`)."""
+
+    _fields_ = [("seqs", _i), ("most", _i), ("row0", _vp), ("src", _vp), ("state_out", _vp),
+                ("S_out", _vp)]
+
+
+class LoraArgs(ctypes.Structure):
+    """Mirror of nmx_lora_args."""
+
+    _fields_ = [("n", _i), ("cols", _i), ("x_stride", _i), ("count", _i), ("x", _vp),
+                ("adapters", _i), ("rank", _i), ("w_dtype", _i), ("adapter", _vp), ("ranks", _vp),
+                ("scale", _vp), ("A", _vp * NMX_MAX_SEGS), ("B", _vp * NMX_MAX_SEGS),
+                ("rows", _i * NMX_MAX_SEGS), ("y_stride", _i * NMX_MAX_SEGS),
+                ("Y", _vp * NMX_MAX_SEGS)]
+
+
+def lora_args(n: int, cols: int, x, x_stride: int, adapters: int, rank: int, w_dtype: int, adapter,
+              scale, segs, *, ranks=None) -> LoraArgs:
+    """The arguments of Device.lora; segs: (rows, A, B, Y, y_stride) of each matrix beside x."""
+    if len(segs) > NMX_MAX_SEGS:
+        raise NmxError(f"lora_args: {len(segs)} matrices, at most {NMX_MAX_SEGS}")
+    a = LoraArgs(n=n, cols=cols, x_stride=x_stride, count=len(segs), x=_p(x), adapters=adapters,
+                 rank=rank, w_dtype=w_dtype, adapter=_p(adapter), ranks=_p(ranks), scale=_p(scale))
+    for i, (rows, A, B, Y, stride) in enumerate(segs):
+        a.rows[i], a.A[i], a.B[i], a.Y[i], a.y_stride[i] = rows, _p(A), _p(B), _p(Y), stride
+    return a
+
+
 _SIGS: dict[str, tuple[object, list[object]]] = {
     "nmx_create": (_vp, [_i]),
     "nmx_create_error": (ctypes.c_char_p, []),
@@ -196,6 +260,14 @@ _SIGS: dict[str, tuple[object, list[object]]] = {
     "nmx_attn_tree": (_i, [_vp, ctypes.POINTER(AttnArgs), _vp, _vp]),
     "nmx_lin_mix_tree": (_i, [_vp, ctypes.POINTER(LinMixArgs), _vp]),
     "nmx_tree_commit": (_i, [_vp, ctypes.POINTER(TreeCommitArgs)]),
+    "nmx_pages_work_bytes": (_sz, [_i, _i, _i]),
+    "nmx_pages_update": (_i, [_vp, ctypes.POINTER(PagesArgs), _vp]),
+    "nmx_attn_batch_prep": (_i, [_vp, ctypes.POINTER(AttnBatchArgs)]),
+    "nmx_attn_batch_work_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "nmx_attn_batch": (_i, [_vp, ctypes.POINTER(AttnBatchArgs), _vp]),
+    "nmx_lin_mix_batch": (_i, [_vp, ctypes.POINTER(LinMixArgs), ctypes.POINTER(LinBatch)]),
+    "nmx_lora_work_bytes": (_sz, [_i, _i, _i]),
+    "nmx_lora": (_i, [_vp, ctypes.POINTER(LoraArgs), _vp]),
     "nmx_sample_work_bytes": (_sz, [_i, _i]),
     "nmx_sample": (_i, [_vp, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp]),
     "nmx_top1_gate": (_i, [_vp, _vp, _i, ctypes.c_float, _vp]),
@@ -515,6 +587,38 @@ class Device:
     def tree_commit(self, args: "TreeCommitArgs") -> None:
         """nmx_tree_commit: the accepted branch of a tree and the move of its rows."""
         self.check(self.lib.nmx_tree_commit(self.ctx, ctypes.byref(args)), "tree_commit")
+
+    def pages_work_bytes(self, npages: int, seqs: int, max_pages: int) -> int:
+        return int(self.lib.nmx_pages_work_bytes(npages, seqs, max_pages))
+
+    def pages_update(self, args: "PagesArgs", work) -> None:
+        """nmx_pages_update: the pages of a step (sequences go on, fork, are cut back or end)."""
+        self.check(self.lib.nmx_pages_update(self.ctx, ctypes.byref(args), _p(work)),
+                   "pages_update")
+
+    def attn_batch_prep(self, args: "AttnBatchArgs") -> None:
+        """nmx_attn_batch_prep: norms, rotary positions of several axes, K and V into pages."""
+        self.check(self.lib.nmx_attn_batch_prep(self.ctx, ctypes.byref(args)), "attn_batch_prep")
+
+    def attn_batch_work_bytes(self, n: int, seqs: int, groups: int, nh: int, nkv: int,
+                              hd: int) -> int:
+        return int(self.lib.nmx_attn_batch_work_bytes(n, seqs, groups, nh, nkv, hd))
+
+    def attn_batch(self, args: "AttnBatchArgs", work) -> None:
+        """nmx_attn_batch: attention of a batch's rows over paged caches, shared prefixes once."""
+        self.check(self.lib.nmx_attn_batch(self.ctx, ctypes.byref(args), _p(work)), "attn_batch")
+
+    def lin_mix_batch(self, args: "LinMixArgs", batch: "LinBatch") -> None:
+        """nmx_lin_mix_batch: the DeltaNet mixer over the rows and states of many sequences."""
+        self.check(self.lib.nmx_lin_mix_batch(self.ctx, ctypes.byref(args), ctypes.byref(batch)),
+                   "lin_mix_batch")
+
+    def lora_work_bytes(self, n: int, count: int, rank: int) -> int:
+        return int(self.lib.nmx_lora_work_bytes(n, count, rank))
+
+    def lora(self, args: "LoraArgs", work) -> None:
+        """nmx_lora: y += scale B (A x) of each row's adapter, for matrices that share x."""
+        self.check(self.lib.nmx_lora(self.ctx, ctypes.byref(args), _p(work)), "lora")
 
     def lin_apply(self, S, log, keep: int, heads: int, dk: int, dv: int) -> None:
         self.check(self.lib.nmx_lin_apply(self.ctx, _p(S), _p(log), keep, heads, dk, dv),

@@ -90,6 +90,10 @@ constexpr int AB_WGS = 256;                /* shares: a workgroup to a CU */
 constexpr int AB_VR = 16;                  /* query rows that the vector instructions take */
 /* a step of 32 positions costs a workgroup about as long by either product, tiles of many rows half as much again */
 constexpr int AB_COST_V = 2, AB_COST_M = 3;
+#ifndef OVERHEAD
+#define OVERHEAD 6
+#endif
+constexpr int AB_COST_UNIT = OVERHEAD; /* to begin a unit: round trips that no other work hides */
 
 struct Seg {
     unsigned long long c0; /* cost of all steps before this segment */
@@ -131,96 +135,130 @@ constexpr int halves() { /* of 512 columns, a unit makes 256 */
     return HDP > 256 ? 2 : 1;
 }
 
-/* The list, by every thread of the workgroup: seg[0 .. groups + seqs) in LDS, the cost of a share returned. */
+/* What a kernel asks for first: arguments of their own, which are in registers when it begins. */
+struct Head0 {
+    const int32_t *row0, *len;
+    int seqs, n, groups, room; /* room: positions of a table */
+};
+
+/* The list, by one wave: seg[0 .. groups + seqs) in LDS, the cost of a share returned. Loops of 64 sequences, not
+ * unrolled: most batches take one turn, and code that runs once is bound by its fetching. */
 template <int HDP>
-__device__ unsigned long long make_list(const BatchAttn &a, Seg *seg) {
-    constexpr int TH = 64 * ctx_waves<HDP>(), PER = AB_SEGS / TH;
+__device__ __forceinline__ unsigned long long make_list(const Head0 &b, const BatchAttn &a, Seg *seg) {
     __shared__ int ctx_s[NMX_BATCH_MAX], first_s[NMX_BATCH_MAX], g0_s[NMX_BATCH_MAX + 1];
-    __shared__ unsigned long long sum_s[2][TH / 64];
-    const int tid = threadIdx.x, S = a.pg.seqs, G = a.groups, rep = a.nh / a.pg.nkv, lane = tid & 63, wave = tid >> 6;
-    /* sequences: their rows and the positions before them */
-    SeqRows rows{0, 0};
-    int len = 0, share = 0;
+    const int lane = lane_id(), S = b.seqs, G = b.groups;
     bool falls = false;
-    if (tid < S) rows = seq_rows(a.row0, tid, a.n), len = seq_len(a.pg, tid), falls = rows.count < 0;
-    if (tid < G) {
-        share = a.shared[tid], ctx_s[tid] = 0x7fffffff, first_s[tid] = S;
-        falls |= a.group0[tid] > a.group0[tid + 1];
+#pragma unroll 1
+    for (int s = lane; s < S; s += 64) {
+        const SeqRows rows = seq_rows(b.row0, s, b.n);
+        const int l = b.len[s], len = l < 0 ? 0 : l < b.room ? l : b.room;
+        Seg &x = seg[G + s];
+        x.r0 = rows.r0, x.m = rows.count, x.p0 = 0, x.p1 = len, x.seq = s, x.last = len - rows.count, x.group = -1;
+        falls |= rows.count < 0;
     }
-    for (int g = tid; G && g <= G; g += TH) g0_s[g] = a.group0[g];
-    /* a list that falls has no rows: the workspace holds the parts of lists that do not */
-    if (__syncthreads_or(falls)) rows = {0, 0};
-    int group = -1;
-    if (tid < S && G) { /* the last group that begins at or before it */
-        int lo = -1, hi = G; /* g0[lo] <= tid < g0[hi] */
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (g0_s[mid] <= tid) lo = mid;
-            else hi = mid;
+#pragma unroll 1
+    for (int g = lane; g < G; g += 64) {
+        const int begin = a.group0[g], end = a.group0[g + 1];
+        Seg &x = seg[g];
+        x.m = 0, x.r0 = 0, x.p0 = 0, x.p1 = a.shared[g], x.seq = 0, x.last = 0x7ffffffe, x.group = -1;
+        ctx_s[g] = 0x7fffffff, first_s[g] = S, g0_s[g] = begin;
+        if (g == G - 1) g0_s[G] = end;
+        falls |= begin > end;
+    }
+    nmx_lds_wave_sync();
+    if (__any(falls)) { /* a list that falls has no rows: the workspace holds the parts of lists that do not */
+        for (int s = lane; s < S; s += 64) seg[G + s].m = 0;
+        nmx_lds_wave_sync();
+    }
+    if (G) {
+#pragma unroll 1
+        for (int s = lane; s < S; s += 64) {
+            int lo = -1, hi = G; /* the last group that begins at or before s: g0[lo] <= s < g0[hi] */
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (g0_s[mid] <= s) lo = mid;
+                else hi = mid;
+            }
+            if (lo < 0 || s >= g0_s[lo + 1] || !seg[G + s].m) continue;
+            seg[G + s].group = lo;
+            atomicMin(&ctx_s[lo], seg[G + s].last), atomicMin(&first_s[lo], s);
         }
-        if (lo >= 0 && tid < g0_s[lo + 1]) group = lo;
-        if (group >= 0 && rows.count) atomicMin(&ctx_s[group], len - rows.count), atomicMin(&first_s[group], tid);
-    }
-    if (tid < S) {
-        Seg &x = seg[G + tid];
-        x.r0 = rows.r0, x.m = rows.count, x.p1 = len, x.group = group;
-    }
-    __syncthreads();
-    if (tid < G) {
-        Seg &x = seg[tid];
-        const int first = first_s[tid];
-        x.m = 0, x.r0 = 0, x.p0 = 0, x.p1 = 0, x.seq = 0, x.last = 0x7ffffffe, x.group = -1;
-        if (first < S) {
-            const int end = g0_s[tid + 1] < S ? g0_s[tid + 1] : S; /* the group's last row */
-            const Seg &l = seg[G + end - 1];
-            x.r0 = seg[G + first].r0, x.m = (l.r0 + l.m - x.r0) * rep, x.seq = first;
-            x.p1 = share < ctx_s[tid] ? share : ctx_s[tid];
-            if (x.p1 < 0) x.p1 = 0;
+        nmx_lds_wave_sync();
+#pragma unroll 1
+        for (int g = lane; g < G; g += 64) {
+            Seg &x = seg[g];
+            const int first = first_s[g], ctx = ctx_s[g], share = x.p1, end = g0_s[g + 1] < S ? g0_s[g + 1] : S;
+            x.p1 = 0;
+            if (first >= S) continue;
+            x.seq = first, x.r0 = seg[G + first].r0, x.m = seg[G + end - 1].r0 + seg[G + end - 1].m - x.r0;
+            x.p1 = share < 0 || ctx < 0 ? 0 : share < ctx ? share : ctx;
         }
+        nmx_lds_wave_sync();
     }
-    __syncthreads();
-    if (tid < S) {
-        Seg &x = seg[G + tid];
-        x.seq = tid, x.last = len - rows.count, x.m = rows.count * rep;
-        x.p0 = group >= 0 && rows.count ? seg[group].p1 : 0;
+    /* costs and units (vector kind in the lower half) before each segment */
+    unsigned long long cb = 0, ub = 0;
+    const int rep = a.nh / a.pg.nkv;
+#pragma unroll 1
+    for (int j0 = 0; j0 < G + S; j0 += 64) {
+        const int j = j0 + lane;
+        unsigned long long cost = 0, units = 0;
+        bool mx = false;
+        if (j < G + S) {
+            Seg &x = seg[j];
+            x.m *= rep;
+            if (x.group >= 0) x.p0 = seg[x.group].p1;
+            mx = x.m > AB_VR;
+            const uint32_t steps = x.m > 0 && x.p1 > x.p0 ? (uint32_t)(x.p1 - x.p0 + AT_P - 1) / AT_P : 0;
+            const uint32_t tiles = mx ? (uint32_t)(x.m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
+            const uint32_t count = steps ? tiles * a.pg.nkv : 0, unit = steps * (mx ? AB_COST_M : AB_COST_V) + AB_COST_UNIT;
+            x.unit = count ? unit : 0;
+            cost = (unsigned long long)count * unit, units = mx ? (unsigned long long)count << 32 : count;
+        }
+        const unsigned long long ci = nmx_scan_wave(cost), ui = nmx_scan_wave(units);
+        if (j < G + S) seg[j].c0 = cb + ci - cost, seg[j].u0 = (uint32_t)(mx ? (ub + ui - units) >> 32 : ub + ui - units);
+        cb += __shfl(ci, 63), ub += __shfl(ui, 63);
     }
-    __syncthreads();
-    /* costs and units before each segment; a thread has PER segments in a row */
-    unsigned long long cost = 0, units = 0; /* units: vector kind in the lower half */
-    auto measure = [&](const Seg &x, unsigned long long &unit, unsigned long long &count) {
-        const bool mx = x.m > AB_VR;
-        const int steps = x.m > 0 && x.p1 > x.p0 ? (x.p1 - x.p0 + AT_P - 1) / AT_P : 0;
-        const int tiles = mx ? (x.m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
-        unit = (unsigned long long)steps * (mx ? AB_COST_M : AB_COST_V);
-        count = steps ? (unsigned long long)tiles * a.pg.nkv : 0;
-        return mx;
-    };
-    for (int k = 0; k < PER; k++) {
-        const int j = tid * PER + k;
-        if (j >= G + S) break;
-        unsigned long long unit, count;
-        const bool mx = measure(seg[j], unit, count);
-        cost += unit * count, units += mx ? count << 32 : count;
-    }
-    const unsigned long long ci = nmx_scan_wave(cost), ui = nmx_scan_wave(units);
-    if (lane == 63) sum_s[0][wave] = ci, sum_s[1][wave] = ui;
-    __syncthreads();
-    unsigned long long cb = ci - cost, ub = ui - units, all = 0;
-    for (int w = 0; w < TH / 64; w++) {
-        if (w < wave) cb += sum_s[0][w], ub += sum_s[1][w];
-        all += sum_s[0][w];
-    }
-    for (int k = 0; k < PER; k++) {
-        const int j = tid * PER + k;
-        if (j >= G + S) break;
-        Seg &x = seg[j];
-        unsigned long long unit, count;
-        const bool mx = measure(x, unit, count);
-        x.c0 = cb, x.unit = count ? (uint32_t)unit : 0, x.u0 = (uint32_t)(mx ? ub >> 32 : ub);
-        cb += unit * count, ub += mx ? count << 32 : count;
-    }
-    __syncthreads();
-    return (all + AB_WGS - 1) / AB_WGS;
+    nmx_lds_wave_sync();
+    return (cb + AB_WGS - 1) / AB_WGS;
+}
+
+/* What a share does next: the part of a unit that begins at cost c, by one wave (x.unit 0: nothing more). */
+struct Piece {
+    Seg x;
+    int tile, g, p0, p1;
+    size_t slot;
+    unsigned long long next;
+};
+template <int HDP>
+__device__ __forceinline__ void find_piece(const BatchAttn &a, const Seg *seg, unsigned long long c, unsigned long long end, int w,
+                                           Piece *piece) {
+    const int lane = lane_id(), segs = a.groups + a.pg.seqs, nkv = a.pg.nkv;
+    if (lane == 0) piece->x.unit = 0;
+    nmx_lds_wave_sync();
+    if (c < end)
+#pragma unroll 1
+        for (int j = lane; j < segs; j += 64) {
+            const unsigned long long c0 = seg[j].c0;
+            const uint32_t unit = seg[j].unit;
+            if (!unit || c < c0) continue;
+            const bool mx = seg[j].m > AB_VR;
+            const int tiles = mx ? (seg[j].m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
+            if (c - c0 >= (unsigned long long)unit * (uint32_t)(tiles * nkv)) continue;
+            const unsigned long long off = c - c0; /* one lane comes here */
+            const uint32_t u = off >> 32 ? (uint32_t)(off / unit) : (uint32_t)off / unit;
+            const unsigned long long cu = c0 + (unsigned long long)u * unit, cn = cu + unit < end ? cu + unit : end;
+            const int each = mx ? AB_COST_M : AB_COST_V;
+            auto steps = [&](unsigned long long cost) { /* of a unit, begun by the first part of its cost */
+                return cost <= AB_COST_UNIT ? 0 : ((int)(uint32_t)cost - AB_COST_UNIT + each - 1) / each;
+            };
+            const Seg x = seg[j];
+            piece->x = x;
+            piece->tile = u / nkv, piece->g = u % nkv;
+            piece->p0 = x.p0 + steps(c - cu) * AT_P;
+            const int p1 = x.p0 + steps(cn - cu) * AT_P;
+            piece->p1 = p1 < x.p1 ? p1 : x.p1;
+            piece->slot = (size_t)w + x.u0 + u, piece->next = cn;
+        }
 }
 
 /* ---- the shares ---------------------------------------------------------------------------------- */
@@ -452,21 +490,46 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
     /* the wave's groups of lanes together, then the waves through LDS */
     float *vals = (float *)smem;                  /* [WV][4][HDP] */
     float2 *ml = (float2 *)(vals + WV * 4 * HDP); /* [WV][4]: maximum, sum */
+    auto add = [](float u, float v) { return u + v; };
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const float top = across_groups<LPP>(m[r], [](float u, float v) { return fmaxf(u, v); });
         const float down = __builtin_amdgcn_exp2f(m[r] - (top == -INFINITY ? 0.0f : top));
-        auto add = [](float u, float v) { return u + v; };
         const float all = across_groups<LPP>((sum[r] - lost[r]) * down, add);
         if (lane == 0) ml[wave * 4 + r] = make_float2(top, all);
 #pragma unroll
-        for (int i = 0; i < 16; i++) acc[r][i] = across_groups<LPP>(acc[r][i] * down, add);
-        if (lg == 0) {
+        for (int i = 0; i < 16; i++) {
+            acc[r][i] *= down;
+            if (LPP <= 4) acc[r][i] = add(acc[r][i], __int_as_float(nmx_dpp<0x124>(__float_as_int(acc[r][i]))));
+            if (LPP <= 8) acc[r][i] = add(acc[r][i], __int_as_float(nmx_dpp<0x128>(__float_as_int(acc[r][i]))));
+        }
+    }
+    /* halves of the wave, then (rows of HDP / 16 <= 16 lanes) its quarters exchange two rows and add: a lane
+     * keeps its columns of row 2 (its half), or of that and of its quarter */
+    float keep[2][16];
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[r][i]), __float_as_uint(acc[r + 2][i]), false, false);
+            keep[r][i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+        }
+    if constexpr (LPP <= 16) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(keep[0][i]), __float_as_uint(keep[1][i]), false, false);
+            keep[0][i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+        }
+    }
+    if (LPP >= 16 || lane % 16 < LPP) {
+#pragma unroll
+        for (int k = 0; k < (LPP <= 16 ? 1 : 2); k++) {
+            const int r = LPP <= 16 ? 2 * (lane >> 5) + (lane >> 4 & 1) : 2 * (lane >> 5) + k;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 float *y = vals + (wave * 4 + r) * HDP + (l + LPP * j) * 8;
-                *(float4 *)y = make_float4(acc[r][8 * j], acc[r][8 * j + 1], acc[r][8 * j + 2], acc[r][8 * j + 3]);
-                *(float4 *)(y + 4) = make_float4(acc[r][8 * j + 4], acc[r][8 * j + 5], acc[r][8 * j + 6], acc[r][8 * j + 7]);
+                *(float4 *)y = make_float4(keep[k][8 * j], keep[k][8 * j + 1], keep[k][8 * j + 2], keep[k][8 * j + 3]);
+                *(float4 *)(y + 4) = make_float4(keep[k][8 * j + 4], keep[k][8 * j + 5], keep[k][8 * j + 6], keep[k][8 * j + 7]);
             }
         }
     }
@@ -517,52 +580,40 @@ __device__ __forceinline__ void matrix_piece(const BatchAttn &a, const Seg &x, i
 }
 
 template <int HDP, int KVT>
-__global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(BatchAttn a) {
+__global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int32_t *row0, const int32_t *len, int seqs, int n,
+                                                                     int groups, int room, BatchAttn a) {
     constexpr int TH = 64 * ctx_waves<HDP>(), OD = HDP > 256 ? 256 : HDP;
     extern __shared__ uint4 smem[];
     __shared__ Seg seg[AB_SEGS];
-    __shared__ int found_s;
-    const int tid = threadIdx.x, segs = a.groups + a.pg.seqs, w = blockIdx.x;
-    const unsigned long long per = make_list<HDP>(a, seg);
-    if (w == 0) { /* the join's */
-        for (int j = tid; j < segs; j += TH) a.plan->seg[j] = seg[j];
-        if (tid == 0) a.plan->per = per;
+    __shared__ Piece piece_s;
+    const int tid = threadIdx.x, segs = groups + seqs, w = blockIdx.x;
+    unsigned long long end = 0;
+    if (wave_id() == 0) {
+        const unsigned long long per = make_list<HDP>({row0, len, seqs, n, groups, room}, a, seg);
+        end = (w + 1) * per;
+        find_piece<HDP>(a, seg, w * per, end, w, &piece_s);
+        if (w == 0 && tid == 0) a.plan->per = per;
     }
-    unsigned long long c = w * per;
-    const unsigned long long end = c + per;
-    while (c < end) {
-        if (tid == 0) found_s = -1;
-        __syncthreads();
-        for (int j = tid; j < segs; j += TH) {
-            const Seg &x = seg[j];
-            const unsigned long long next = j + 1 < segs ? seg[j + 1].c0 : per * AB_WGS;
-            if (x.unit && c >= x.c0 && c < next) found_s = j; /* the last one's range may pass the whole cost */
-        }
-        __syncthreads();
-        const int j = __builtin_amdgcn_readfirstlane(found_s);
-        if (j < 0) return;
-        const Seg x = seg[j];
-        const bool mx = x.m > AB_VR;
-        const int nkv = a.pg.nkv, tiles = mx ? (x.m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
-        const uint32_t u = (uint32_t)((c - x.c0) / x.unit);
-        if (u >= (uint32_t)(tiles * nkv)) return; /* past the whole cost */
-        const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit, cn = cu + x.unit < end ? cu + x.unit : end;
-        const int each = mx ? AB_COST_M : AB_COST_V;
-        const int s0 = (int)((c - cu + each - 1) / each), s1 = (int)((cn - cu + each - 1) / each);
-        const int p0 = x.p0 + s0 * AT_P, p1 = x.p0 + s1 * AT_P < x.p1 ? x.p0 + s1 * AT_P : x.p1;
-        const int tile = u / nkv, g = u % nkv;
-        const size_t slot = (size_t)w + x.u0 + u;
-        if (mx) {
-            float4 *stat = a.stat_m + slot * tile_rows<HDP>();
-            if (p0 < p1) matrix_piece<HDP, KVT>(a, x, g, tile / halves<HDP>(), tile % halves<HDP>(), p0, p1,
-                                                a.part_m + slot * tile_rows<HDP>() * (HDP > 256 ? OD : HDP), stat, smem);
+    __syncthreads();
+    if (w == 0) /* the join's */
+        for (int j = tid; j < segs; j += TH) a.plan->seg[j] = seg[j];
+    for (;;) {
+        const Piece pc = piece_s;
+        const Seg &x = pc.x;
+        if (!__builtin_amdgcn_readfirstlane(x.unit)) return;
+        const int p0 = __builtin_amdgcn_readfirstlane(pc.p0), p1 = __builtin_amdgcn_readfirstlane(pc.p1);
+        if (x.m > AB_VR) {
+            float4 *stat = a.stat_m + pc.slot * tile_rows<HDP>();
+            if (p0 < p1) matrix_piece<HDP, KVT>(a, x, pc.g, pc.tile / halves<HDP>(), pc.tile % halves<HDP>(), p0, p1,
+                                                a.part_m + pc.slot * tile_rows<HDP>() * OD, stat, smem);
             else if (tid < tile_rows<HDP>()) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         } else {
-            float4 *stat = a.stat_v + slot * AB_VR;
-            if (p0 < p1) vector_piece<HDP, KVT>(a, x, g, p0, p1, a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
+            float4 *stat = a.stat_v + pc.slot * AB_VR;
+            if (p0 < p1) vector_piece<HDP, KVT>(a, x, pc.g, p0, p1, a.part_v + pc.slot * AB_VR * a.pg.hd, stat, smem);
             else if (tid < AB_VR) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         }
-        c = cn;
+        if (p0 >= p1) __syncthreads(); /* the others pass a barrier with the piece in their hands */
+        if (wave_id() == 0) find_piece<HDP>(a, seg, pc.next, end, w, &piece_s);
         __syncthreads();
     }
 }
@@ -717,7 +768,8 @@ int launch(nmx_ctx *ctx, const BatchAttn &a) {
     constexpr int vec = ctx_waves<HDP>() * 4 * (HDP * 4 + 8), mat = ctx_lds<HDP, KVT>();
     constexpr int lds = vec > mat ? vec : mat;
     if (nmx_dyn_lds(ctx, (const void *)attn_batch_k<HDP, KVT>, lds, set0)) return -1;
-    attn_batch_k<HDP, KVT><<<AB_WGS, 64 * ctx_waves<HDP>(), lds, ctx->stream>>>(a);
+    attn_batch_k<HDP, KVT><<<AB_WGS, 64 * ctx_waves<HDP>(), lds, ctx->stream>>>(a.row0, a.pg.len, a.pg.seqs, a.n, a.groups,
+                                                                              a.pg.max_pages << a.pg.shift, a);
     NMX_LAUNCHED(ctx, "attn_batch");
     attn_batch_join_k<HDP><<<dim3((unsigned)(a.n * a.nh), (unsigned)(a.pg.hd / a.jcols)), JB, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "attn_batch_join");

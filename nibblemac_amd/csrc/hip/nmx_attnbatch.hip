@@ -13,6 +13,8 @@
  * vector instructions, a wave streaming rows from memory into registers, 16 columns a lane, the keys of the
  * next positions requested while the values of the current ones are added and the other way round; no LDS and no
  * barrier on the way. More rows: the matrix cores over tiles in LDS (nmx_attnmx.h). */
+#include <type_traits>
+
 #include "nmx_internal.h"
 #include "nmx_a8.h"
 #include "nmx_attn.h"
@@ -226,7 +228,7 @@ __device__ __forceinline__ unsigned long long make_list(const Head0 &b, const Ba
 struct Piece {
     Seg x;
     int tile, g, p0, p1;
-    size_t slot;
+    uint32_t slot;
     unsigned long long next;
 };
 template <int HDP>
@@ -257,7 +259,7 @@ __device__ __forceinline__ void find_piece(const BatchAttn &a, const Seg *seg, u
             piece->p0 = x.p0 + steps(c - cu) * AT_P;
             const int p1 = x.p0 + steps(cn - cu) * AT_P;
             piece->p1 = p1 < x.p1 ? p1 : x.p1;
-            piece->slot = (size_t)w + x.u0 + u, piece->next = cn;
+            piece->slot = w + x.u0 + u, piece->next = cn;
         }
 }
 
@@ -310,199 +312,251 @@ __device__ __forceinline__ float widen(const Raw8<KV_I8> &r, int i) {
     return (float)(int8_t)((i < 4 ? r.a.x : r.a.y) >> 8 * (i & 3));
 }
 
-/* the sum over W neighbouring lanes, in each of them */
-template <int W>
-__device__ __forceinline__ float sum_group(float v) {
-    auto with = [&](int o) { v += __int_as_float(o); };
-    if (W >= 2) with(nmx_dpp<NMX_DPP_XOR1>(__float_as_int(v)));
-    if (W >= 4) with(nmx_dpp<NMX_DPP_XOR2>(__float_as_int(v)));
-    if (W >= 8) with(nmx_dpp<NMX_DPP_HALF_MIRROR>(__float_as_int(v)));
-    if (W >= 16) with(nmx_dpp<NMX_DPP_MIRROR>(__float_as_int(v)));
-    if (W >= 32) {
-        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    }
-    return v;
+/* v of lane r of each four neighbours, in all four */
+template <int R>
+__device__ __forceinline__ float of_quad(float v) {
+    return __int_as_float(nmx_dpp<0x55 * R>(__float_as_int(v)));
 }
-/* v of this lane and of the lanes W, 2 W, ... on, combined by f, in all of them */
-template <int W, typename F>
-__device__ __forceinline__ float across_groups(float v, F f) {
-    if (W <= 4) v = f(v, __int_as_float(nmx_dpp<0x124>(__float_as_int(v)))); /* rows of 16 turned by 4 and by 8 */
-    if (W <= 8) v = f(v, __int_as_float(nmx_dpp<0x128>(__float_as_int(v))));
-    if (W <= 16) {
-        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    }
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+__device__ __forceinline__ float quad_row(float v, int r) { /* r constant where it is unrolled */
+    return r == 0 ? of_quad<0>(v) : r == 1 ? of_quad<1>(v) : r == 2 ? of_quad<2>(v) : of_quad<3>(v);
 }
 
-/* What a share finds of a unit of few rows: positions [p0, p1) of segment x's KV head g, to part and stat.
- * A lane holds 16 columns (two chunks of 8) of 4 query rows; HDP / 16 lanes a position, so a wave has
- * LG positions at once, VP times. Waves: groups of 4 rows first, then positions, in turns. */
+/* What a share finds of a unit of few rows: positions [p0, p1) of segment x's KV head g, to part and stat. A wave
+ * takes 4 query rows; waves: groups of 4 rows first, then positions, in turns.
+ *
+ * Scores on the matrix cores, 16 positions at a time and keys straight from memory: as first operand they lie in
+ * a lane as they lie in a row. The second operand has 16 columns for 4 query rows: with 16-bit keys the
+ * rows' high and low parts stand in columns 4 apart and one product makes both; fp32 keys take the fp32
+ * instruction. Lane (quarter gq, column c) then holds the scores of row c mod 4 at the positions 4 gq .. 4 gq + 3, and
+ * the same quarter adds those positions' values, 16 columns (two chunks of 8) a lane, by vector instructions: a
+ * row's weight comes from a lane of the quad. (All by vector instructions a turn took 3.4 us of issue for 128 positions
+ * and CU, this 1.3.) */
 template <int HDP, int KVT>
 __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, int g, int p0, int p1, float *part, float4 *stat,
                                              uint4 *smem) {
-    constexpr int WV = ctx_waves<HDP>(), LPP = HDP / 16, LG = 64 / LPP, VP = KVT == KV_F32 ? 2 : 4;
-    const int lane = lane_id(), wave = wave_id(), l = lane % LPP, lg = lane / LPP, hd = a.pg.hd, rep = a.nh / a.pg.nkv;
+    constexpr int WV = ctx_waves<HDP>(), LPP = HDP / 16;   /* lanes of a position's values */
+    constexpr int NT = HDP < 256 ? 256 / HDP : 1;          /* tiles of 16 positions a turn */
+    constexpr int VP = HDP > 256 ? 8 : 4;                  /* positions whose values a lane adds in a turn */
+    constexpr int KW = KVT == KV_F32 ? 16 : 32, KN = HDP / KW; /* columns of a key's chunk (over the quarters), chunks */
+    constexpr int KH = KVT != KV_F32 ? 1 : HDP == 64 ? 4 : 2, KP = KN / KH; /* parts that a key comes in: fp32 rows have no room whole */
+    const int lane = lane_id(), wave = wave_id(), l = lane % LPP, c = lane & 15, gq = lane >> 4, hd = a.pg.hd, rep = a.nh / a.pg.nkv;
     const int quads = x.m > 8 ? 4 : x.m > 4 ? 2 : 1, rq = wave % quads, ws = wave / quads, NS = WV / quads;
     const PagedHead<KVT> kh(a.pg, a.kc, x.seq, g), vh(a.pg, a.vc, x.seq, g);
     int col[2];
-    bool in[2];
 #pragma unroll
-    for (int j = 0; j < 2; j++) col[j] = (l + LPP * j) * 8, in[j] = col[j] < hd, col[j] = in[j] ? col[j] : 0;
-    /* the positions of a turn: VP times NS LG neighbours, so that few positions spread over all waves */
-    const int turn = NS * LG * VP, mine = ws * LG + lg;
-    int pg[VP];
-    Raw8<KVT> rk[VP][2], rv[VP][2];
-    float sk[VP], sv[VP];
-    auto place = [&](int base, int v) {
-        const int p = base + v * NS * LG + mine;
-        return p < p1 ? p : p1 - 1;
-    };
+    for (int j = 0; j < 2; j++) col[j] = (l + LPP * j) * 8, col[j] = col[j] < hd ? col[j] : 0;
+    /* the positions of a turn: position v of quarter q in tile n is 4 NS (4 n + v) + 4 ws + q, so that few positions
+     * spread over all waves; behind the end the last one stands in and has no weight */
+    const int turn = 16 * NT * NS;
+    auto at = [&](int base, int n, int q, int v) { return base + 4 * NS * (4 * n + v) + 4 * ws + q; };
+    auto in = [&](int p) { return p < p1 ? p : p1 - 1; };
+    /* a lane's values: those of its quarter in the tile that its LPP lanes have (HDP 512: of two quarters) */
+    const int vt = LPP < 16 ? lane / LPP % (16 / LPP) : 0;
+    auto at_v = [&](int base, int v) { return HDP > 256 ? at(base, 0, (gq & 2) + (v >> 2), v & 3) : at(base, vt, gq, v); };
+    int pk[NT], pv[VP];
     auto ask = [&](int base) {
 #pragma unroll
-        for (int v = 0; v < VP; v++) pg[v] = kh.page_of(place(base, v));
+        for (int n = 0; n < NT; n++) pk[n] = kh.page_of(in(at(base, n, c >> 2, c & 3)));
+#pragma unroll
+        for (int v = 0; v < VP; v++) pv[v] = vh.page_of(in(at_v(base, v)));
     };
-    auto fetch = [&](const PagedHead<KVT> &h, int base, Raw8<KVT>(&r)[VP][2], float(&s)[VP]) {
+    typedef typename std::conditional<KVT == KV_I8, uint2, uint4>::type KeyChunk;
+    KeyChunk rk[NT][KP];
+    const char *row[NT];
+    Raw8<KVT> rv[VP][2];
+    float sk[NT], sv[NT]; /* int8: scales of position c of a tile (four of them are those of the lane's scores) */
+    auto find_k = [&](int base) {
 #pragma unroll
-        for (int v = 0; v < VP; v++) {
-            const int p = place(base, v);
-#pragma unroll
-            for (int j = 0; j < 2; j++) r[v][j] = h.load8(pg[v], p, col[j]);
-            s[v] = h.scale(pg[v], p);
+        for (int n = 0; n < NT; n++) {
+            const int p = in(at(base, n, c >> 2, c & 3));
+            row[n] = kh.at(pk[n], p, KW / 4 * gq);
+            if (KVT == KV_I8) sk[n] = kh.scale(pk[n], p), sv[n] = vh.scale(pk[n], p);
         }
+    };
+    auto fetch_k = [&](int part) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int k = 0; k < KP; k++) {
+                const int cc = KW * (part * KP + k);
+                if (cc < HDP / 2 + 64 || cc < hd) rk[n][k] = *(const KeyChunk *)(row[n] + cc * PagedHead<KVT>::SIZE);
+                else rk[n][k] = KeyChunk{}; /* columns behind hd */
+            }
+    };
+    auto fetch_v = [&](int base) {
+#pragma unroll
+        for (int v = 0; v < VP; v++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) rv[v][j] = vh.load8(pv[v], in(at_v(base, v)), col[j]);
     };
     ask(p0);
-    /* query rows to LDS, in the order in which the lanes of a position read them: [row][chunk][half][lane][4] */
-    float *qs = (float *)smem;
+    /* the query rows: row c mod 4 of this wave's; rows past the last one are of no use to anyone */
+    const int rr = rq * 4 + (c & 3), ri = rr < x.m ? rr : 0;
+    const float *qp = a.q + ((size_t)(x.r0 + ri / rep) * a.nh + g * rep + ri % rep) * 2 * hd;
+    half8 qx[KVT == KV_F32 ? 1 : KN];
+    float qf = a.scale * AT_LOG2E;
+    float *qs = (float *)smem; /* fp32: [16 rows][HDP] in LDS, they have no registers to stay in */
     constexpr int Q4 = HDP / 4, QU = (AB_VR * Q4 + 64 * WV - 1) / (64 * WV);
-    float4 qv[QU];
+    if constexpr (KVT == KV_F32) {
+        float4 qv[QU];
 #pragma unroll
-    for (int u = 0; u < QU; u++) {
-        const int e = u * 64 * WV + 64 * wave + lane, rr = e / Q4, at = rr < x.m ? rr : 0;
-        const int c = (e % LPP + LPP * (e % Q4 / (2 * LPP))) * 8 + e / LPP % 2 * 4;
-        const float *qp = a.q + ((size_t)(x.r0 + at / rep) * a.nh + g * rep + at % rep) * 2 * hd;
-        qv[u] = *(const float4 *)(qp + (c < hd ? c : 0));
-        if (c >= hd || rr >= x.m) qv[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    int lim[4]; /* a row sees positions below it; a row past the last one none */
+        for (int u = 0; u < QU; u++) {
+            const int e = u * 64 * WV + 64 * wave + lane, r = e / Q4 < x.m ? e / Q4 : 0, q4 = e % Q4 * 4;
+            qv[u] = *(const float4 *)(a.q + ((size_t)(x.r0 + r / rep) * a.nh + g * rep + r % rep) * 2 * hd + (q4 < hd ? q4 : 0));
+            if (q4 >= hd) qv[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        find_k(p0);
+        fetch_k(0);
+        fetch_v(p0);
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const int rr = rq * 4 + r, more = rr / rep;
-        lim[r] = rr >= x.m ? 0 : x.last >= p1 ? p1 : x.last + 1 + more < p1 ? x.last + 1 + more : p1;
-    }
-    fetch(kh, p0, rk, sk);
-    fetch(vh, p0, rv, sv);
+        for (int u = 0; u < QU; u++) {
+            /* 16-byte pieces of a row moved by its number, so that four rows' reads meet no bank twice */
+            const int e = u * 64 * WV + 64 * wave + lane;
+            if (e < AB_VR * Q4) *(float4 *)(qs + e / Q4 * HDP + ((e % Q4) ^ (e / Q4 % 4)) * 4) = qv[u];
+        }
+        nmx_lds_sync();
+    } else {
+        QueryRow<KN> qr(qp, true, hd, gq);
+        find_k(p0);
+        fetch_k(0);
+        fetch_v(p0);
+        half8 ql[KN];
+        qf = qr.split(a.scale, qx, ql);
 #pragma unroll
-    for (int u = 0; u < QU; u++) {
-        const int e = u * 64 * WV + 64 * wave + lane;
-        if (e < AB_VR * Q4) *(float4 *)(qs + 4 * e) = qv[u];
+        for (int k = 0; k < KN; k++) qx[k] = c & 4 ? ql[k] : qx[k];
     }
-    nmx_lds_sync();
-    int q_at = rq * 4 * HDP + 4 * l;
+    const int past = x.last + 1 + ri / rep; /* a row sees positions below it */
+    const int lim = rr >= x.m ? 0 : x.last >= p1 ? p1 : past < p1 ? past : p1;
     ask(p0 + turn);
-    float acc[4][16], m[4], sum[4], lost[4];
+    float acc[4][16], m = -INFINITY, sum = 0.0f, lost = 0.0f; /* m is the wave's, sum this lane's */
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        m[r] = -INFINITY, sum[r] = 0.0f, lost[r] = 0.0f;
+    for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[r][i] = 0.0f;
-    }
-    const float qf = a.scale * AT_LOG2E;
+    int q_at = (rq * 4 + (c & 3)) * HDP;
     for (int base = p0; base < p1; base += turn) {
-        asm volatile("" : "+v"(q_at)); /* the rows are read anew each turn: they have no registers to stay in */
-        const float *qr = qs + q_at;
-        float w[VP][4];
+        float4v s4[NT];
 #pragma unroll
-        for (int v = 0; v < VP; v++)
+        for (int n = 0; n < NT; n++) s4[n] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        if (KVT == KV_F32) asm volatile("" : "+v"(q_at)); /* the rows are read anew each turn */
 #pragma unroll
-            for (int r = 0; r < 4; r++) w[v][r] = 0.0f;
+        for (int part = 0; part < KH; part++) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) { /* 4 columns of the rows and of every position */
-            float4 q[4];
+            for (int kp = 0; kp < KP; kp++) {
+                const int k = part * KP + kp;
+                if constexpr (KVT == KV_F32) {
+                    if (k % 4 == 0) __builtin_amdgcn_sched_barrier(0); /* four pieces of a row in registers at once, not all */
+                    const float4 q = *(const float4 *)(qs + q_at + ((4 * k + gq) ^ (c & 3)) * 4);
 #pragma unroll
-            for (int r = 0; r < 4; r++) q[r] = *(const float4 *)(qr + r * HDP + e * 4 * LPP);
+                    for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int v = 0; v < VP; v++)
+                        for (int n = 0; n < NT; n++) {
+                            const uint4 y = rk[n][kp];
+                            s4[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(i == 0 ? y.x : i == 1 ? y.y : i == 2 ? y.z : y.w),
+                                                                         i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w, s4[n], 0, 0, 0);
+                        }
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float k = widen(rk[v][e >> 1], 4 * (e & 1) + i);
+                    for (int n = 0; n < NT; n++) {
+                        half8 y;
+                        if constexpr (KVT == KV_F16) y = __builtin_bit_cast(half8, rk[n][kp]);
+                        else y = codes8(rk[n][kp]);
+                        s4[n] = mfma16(y, qx[k], s4[n]);
+                    }
+                }
+            }
+            if (part + 1 < KH) fetch_k(part + 1);
+        }
+        float fv[NT][4];
+        if constexpr (KVT == KV_I8) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        w[v][r] = __builtin_fmaf(k, i == 0 ? q[r].x : i == 1 ? q[r].y : i == 2 ? q[r].z : q[r].w, w[v][r]);
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const int from = (lane & 48) + 4 * gq + v;
+                    s4[n][v] *= __shfl(sk[n], from), fv[n][v] = __shfl(sv[n], from);
                 }
         }
-        float f[VP], fv[VP];
+        find_k(base + turn); /* behind the last turn the last position again */
+        fetch_k(0);
+        float w[NT][4], top = m;
 #pragma unroll
-        for (int v = 0; v < VP; v++) f[v] = KVT == KV_I8 ? qf * sk[v] : qf, fv[v] = sv[v];
-        fetch(kh, base + turn, rk, sk); /* behind the last turn the last position again */
-        bool grows = false;
-        float top[4];
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            top[r] = m[r];
-#pragma unroll
-            for (int v = 0; v < VP; v++) {
-                const int p = base + v * NS * LG + mine;
-                const float s = sum_group<LPP>(w[v][r]) * f[v];
-                w[v][r] = p < lim[r] ? s : -INFINITY;
-                top[r] = fmaxf(top[r], w[v][r]);
+            for (int v = 0; v < 4; v++) {
+                float s = s4[n][v];
+                if (KVT != KV_F32) s += __int_as_float(nmx_dpp<0x124>(__float_as_int(s))); /* high and low: 4 columns on */
+                s *= qf;
+                w[n][v] = at(base, n, gq, v) < lim ? s : -INFINITY;
+                top = fmaxf(top, w[n][v]);
             }
-            grows |= top[r] > m[r];
-        }
-        if (__any(grows)) {
+        top = max_quarters(top);
+        if (__any(top > m)) {
+            const float down = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+            m = top, sum *= down, lost *= down;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float down = __builtin_amdgcn_exp2f(m[r] - (top[r] == -INFINITY ? 0.0f : top[r]));
-                m[r] = top[r], sum[r] *= down, lost[r] *= down;
+                const float d = quad_row(down, r);
 #pragma unroll
-                for (int i = 0; i < 16; i++) acc[r][i] *= down;
+                for (int i = 0; i < 16; i++) acc[r][i] *= d;
+            }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float all = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                w[n][v] = __builtin_amdgcn_exp2f(w[n][v] - ref);
+                all += w[n][v];
+                if (KVT == KV_I8) w[n][v] *= fv[n][v];
+            }
+        const float more = all - lost, now = sum + more; /* the roundings of a long share's sum are kept */
+        lost = (now - sum) - more, sum = now;
+        /* the weights of the positions whose values this lane adds */
+        float u[VP];
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            if constexpr (HDP > 256) { /* of both quarters of its half */
+                const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(w[0][v]), __float_as_uint(w[0][v]), false, false);
+                u[v] = __uint_as_float(y[0]), u[v + 4] = __uint_as_float(y[1]);
+            } else {
+                u[v] = w[0][v];
+#pragma unroll
+                for (int n = 1; n < NT; n++) u[v] = vt == n ? w[n][v] : u[v];
             }
         }
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const float ref = m[r] == -INFINITY ? 0.0f : m[r];
-            float all = 0.0f;
+        for (int v = 0; v < VP; v++) {
+            float wr[4];
 #pragma unroll
-            for (int v = 0; v < VP; v++) {
-                w[v][r] = __builtin_amdgcn_exp2f(w[v][r] - ref);
-                all += w[v][r];
-                if (KVT == KV_I8) w[v][r] *= fv[v];
-            }
-            const float add = all - lost[r], now = sum[r] + add; /* the roundings of a long share's sum are kept */
-            lost[r] = (now - sum[r]) - add, sum[r] = now;
-        }
-#pragma unroll
-        for (int v = 0; v < VP; v++)
+            for (int r = 0; r < 4; r++) wr[r] = quad_row(u[v], r);
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const float y = widen(rv[v][j], i);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) acc[r][8 * j + i] = __builtin_fmaf(y, w[v][r], acc[r][8 * j + i]);
+                    for (int r = 0; r < 4; r++) acc[r][8 * j + i] = __builtin_fmaf(y, wr[r], acc[r][8 * j + i]);
                 }
-        fetch(vh, base + turn, rv, sv);
+        }
+        fetch_v(base + turn);
         ask(base + 2 * turn);
     }
     nmx_lds_sync(); /* the query rows have been read */
     /* the wave's groups of lanes together, then the waves through LDS */
     float *vals = (float *)smem;                  /* [WV][4][HDP] */
     float2 *ml = (float2 *)(vals + WV * 4 * HDP); /* [WV][4]: maximum, sum */
-    auto add = [](float u, float v) { return u + v; };
+    const float total = nmx_sum_quarters(sum - lost);
+    if (lane < 4) ml[wave * 4 + lane] = make_float2(m, total);
+    if (LPP < 16) { /* within a quarter first: rows of 16 lanes turned by 4 and by 8 */
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const float top = across_groups<LPP>(m[r], [](float u, float v) { return fmaxf(u, v); });
-        const float down = __builtin_amdgcn_exp2f(m[r] - (top == -INFINITY ? 0.0f : top));
-        const float all = across_groups<LPP>((sum[r] - lost[r]) * down, add);
-        if (lane == 0) ml[wave * 4 + r] = make_float2(top, all);
+        for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            acc[r][i] *= down;
-            if (LPP <= 4) acc[r][i] = add(acc[r][i], __int_as_float(nmx_dpp<0x124>(__float_as_int(acc[r][i]))));
-            if (LPP <= 8) acc[r][i] = add(acc[r][i], __int_as_float(nmx_dpp<0x128>(__float_as_int(acc[r][i]))));
-        }
+            for (int i = 0; i < 16; i++) {
+                if (LPP <= 4) acc[r][i] += __int_as_float(nmx_dpp<0x124>(__float_as_int(acc[r][i])));
+                acc[r][i] += __int_as_float(nmx_dpp<0x128>(__float_as_int(acc[r][i])));
+            }
     }
     /* halves of the wave, then (rows of HDP / 16 <= 16 lanes) its quarters exchange two rows and add: a lane
      * keeps its columns of row 2 (its half), or of that and of its quarter */
@@ -598,22 +652,25 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
     if (w == 0) /* the join's */
         for (int j = tid; j < segs; j += TH) a.plan->seg[j] = seg[j];
     for (;;) {
-        const Piece pc = piece_s;
-        const Seg &x = pc.x;
-        if (!__builtin_amdgcn_readfirstlane(x.unit)) return;
-        const int p0 = __builtin_amdgcn_readfirstlane(pc.p0), p1 = __builtin_amdgcn_readfirstlane(pc.p1);
+        auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); }; /* into scalars */
+        if (!same(piece_s.x.unit)) return;
+        Seg x{};
+        x.m = same(piece_s.x.m), x.r0 = same(piece_s.x.r0), x.seq = same(piece_s.x.seq), x.last = same(piece_s.x.last);
+        const int p0 = same(piece_s.p0), p1 = same(piece_s.p1), g = same(piece_s.g), tile = same(piece_s.tile);
+        const size_t slot = (uint32_t)same(piece_s.slot);
+        const unsigned long long next = piece_s.next;
         if (x.m > AB_VR) {
-            float4 *stat = a.stat_m + pc.slot * tile_rows<HDP>();
-            if (p0 < p1) matrix_piece<HDP, KVT>(a, x, pc.g, pc.tile / halves<HDP>(), pc.tile % halves<HDP>(), p0, p1,
-                                                a.part_m + pc.slot * tile_rows<HDP>() * OD, stat, smem);
+            float4 *stat = a.stat_m + slot * tile_rows<HDP>();
+            if (p0 < p1) matrix_piece<HDP, KVT>(a, x, g, tile / halves<HDP>(), tile % halves<HDP>(), p0, p1,
+                                                a.part_m + slot * tile_rows<HDP>() * OD, stat, smem);
             else if (tid < tile_rows<HDP>()) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         } else {
-            float4 *stat = a.stat_v + pc.slot * AB_VR;
-            if (p0 < p1) vector_piece<HDP, KVT>(a, x, pc.g, p0, p1, a.part_v + pc.slot * AB_VR * a.pg.hd, stat, smem);
+            float4 *stat = a.stat_v + slot * AB_VR;
+            if (p0 < p1) vector_piece<HDP, KVT>(a, x, g, p0, p1, a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
             else if (tid < AB_VR) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         }
         if (p0 >= p1) __syncthreads(); /* the others pass a barrier with the piece in their hands */
-        if (wave_id() == 0) find_piece<HDP>(a, seg, pc.next, end, w, &piece_s);
+        if (wave_id() == 0) find_piece<HDP>(a, seg, next, end, w, &piece_s);
         __syncthreads();
     }
 }

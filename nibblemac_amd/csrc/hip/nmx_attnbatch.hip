@@ -9,7 +9,7 @@
  * so every workgroup makes the list itself (a scan over at most 512 segments). What a workgroup finds of a
  * unit is a part (weighted values, maximum, sum); attn_batch_join_k adds a row's parts in order.
  *
- * Two inner products. Up to 16 query rows (a token of each sequence: the heads of a KV group): fp32
+ * Two inner products. Up to 8 query rows (a token of each sequence: the heads of a KV group): fp32
  * vector instructions, a wave streaming rows from memory into registers, 16 columns a lane, the keys of the
  * next positions requested while the values of the current ones are added and the other way round; no LDS and no
  * barrier on the way. More rows: the matrix cores over tiles in LDS (nmx_attnmx.h). */
@@ -89,16 +89,29 @@ __global__ __launch_bounds__(512) void attn_batch_prep_k(PrepBatch a) {
 /* ---- the list of segments ---------------------------------------------------------------------- */
 constexpr int AB_SEGS = 2 * NMX_BATCH_MAX; /* a prefix for each group, the rest of each sequence */
 constexpr int AB_WGS = 256;                /* shares: a workgroup to a CU */
-constexpr int AB_VR = 16;                  /* query rows that the vector instructions take */
-/* a step of 32 positions costs a workgroup about as long by either product, tiles of many rows half as much again */
-constexpr int AB_COST_V = 2, AB_COST_M = 3;
-#ifndef OVERHEAD
-#define OVERHEAD 6
+constexpr int AB_VR = 8;                   /* query rows that the vector kind takes: 4 a wave */
+/* a step of 32 positions costs a workgroup about as long by either product, tiles of many rows half as much again;
+ * a unit's beginning is round trips that its workgroup (or its wave, beside others) waits for */
+#ifndef COSTM
+#define COSTM 20
 #endif
-constexpr int AB_COST_UNIT = OVERHEAD; /* to begin a unit: round trips that no other work hides */
+#ifndef COSTV
+#define COSTV 8
+#endif
+constexpr int AB_COST_V = COSTV, AB_COST_M = COSTM;
+#ifndef OVERHEAD
+#define OVERHEAD 8
+#endif
+#ifndef OVERHEADM
+#define OVERHEADM 80
+#endif
+constexpr int AB_BEGIN_V = OVERHEAD, AB_BEGIN_M = OVERHEADM;
+
+/* of a segment of m query rows */
+__device__ __forceinline__ int step_cost(int m) { return m > AB_VR ? AB_COST_M : m > 4 ? 2 * AB_COST_V : AB_COST_V; }
 
 struct Seg {
-    unsigned long long c0; /* cost of all steps before this segment */
+    unsigned long long c0; /* cost of all steps of its kind before this segment */
     uint32_t unit;         /* the cost of one unit: all its steps; 0: nothing to do */
     uint32_t u0;           /* units of its kind (vector, matrix) before it */
     int m;                 /* query rows: rows times heads of a KV group */
@@ -107,10 +120,18 @@ struct Seg {
     int last;              /* the first row sees positions below last + 1, the next ones one more each (a prefix: all) */
     int group;             /* of a sequence: its group, -1 none */
 };
-struct Plan {
-    unsigned long long per; /* the cost of a share */
-    Seg seg[AB_SEGS];       /* the groups, then the sequences */
+/* Who takes what: of AB_WGS workgroups the first mx take the matrix kind's steps, the others the vector kind's.
+ * A workgroup of those either lies within one unit, and its 8 waves take that part together, or its waves
+ * take an eighth of its share each, by themselves. */
+struct Shares {
+    unsigned long long per_m, per_w; /* the cost of a workgroup's share, of a wave's */
+    int mx;
 };
+struct Plan {
+    Shares sh;
+    Seg seg[AB_SEGS]; /* the groups, then the sequences */
+};
+constexpr int AB_PARTS = 8; /* shares of a vector workgroup */
 
 struct BatchAttn {
     PageDev pg;
@@ -143,10 +164,10 @@ struct Head0 {
     int seqs, n, groups, room; /* room: positions of a table */
 };
 
-/* The list, by one wave: seg[0 .. groups + seqs) in LDS, the cost of a share returned. Loops of 64 sequences, not
+/* The list, by one wave: seg[0 .. groups + seqs) in LDS. Loops of 64 sequences, not
  * unrolled: most batches take one turn, and code that runs once is bound by its fetching. */
 template <int HDP>
-__device__ __forceinline__ unsigned long long make_list(const Head0 &b, const BatchAttn &a, Seg *seg) {
+__device__ __forceinline__ Shares make_list(const Head0 &b, const BatchAttn &a, Seg *seg) {
     __shared__ int ctx_s[NMX_BATCH_MAX], first_s[NMX_BATCH_MAX], g0_s[NMX_BATCH_MAX + 1];
     const int lane = lane_id(), S = b.seqs, G = b.groups;
     bool falls = false;
@@ -197,8 +218,8 @@ __device__ __forceinline__ unsigned long long make_list(const Head0 &b, const Ba
         }
         nmx_lds_wave_sync();
     }
-    /* costs and units (vector kind in the lower half) before each segment */
-    unsigned long long cb = 0, ub = 0;
+    /* costs and units of its kind before each segment */
+    unsigned long long cb[2] = {0, 0}, ub = 0; /* vector, matrix; units: vector in the lower half */
     const int rep = a.nh / a.pg.nkv;
 #pragma unroll 1
     for (int j0 = 0; j0 < G + S; j0 += 64) {
@@ -212,29 +233,44 @@ __device__ __forceinline__ unsigned long long make_list(const Head0 &b, const Ba
             mx = x.m > AB_VR;
             const uint32_t steps = x.m > 0 && x.p1 > x.p0 ? (uint32_t)(x.p1 - x.p0 + AT_P - 1) / AT_P : 0;
             const uint32_t tiles = mx ? (uint32_t)(x.m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
-            const uint32_t count = steps ? tiles * a.pg.nkv : 0, unit = steps * (mx ? AB_COST_M : AB_COST_V) + AB_COST_UNIT;
-            x.unit = count ? unit : 0;
-            cost = (unsigned long long)count * unit, units = mx ? (unsigned long long)count << 32 : count;
+            const uint32_t count = steps ? tiles * a.pg.nkv : 0;
+            x.unit = count ? steps * step_cost(x.m) + (mx ? AB_BEGIN_M : AB_BEGIN_V) : 0;
+            cost = (unsigned long long)count * x.unit, units = mx ? (unsigned long long)count << 32 : count;
         }
-        const unsigned long long ci = nmx_scan_wave(cost), ui = nmx_scan_wave(units);
-        if (j < G + S) seg[j].c0 = cb + ci - cost, seg[j].u0 = (uint32_t)(mx ? (ub + ui - units) >> 32 : ub + ui - units);
-        cb += __shfl(ci, 63), ub += __shfl(ui, 63);
+        const unsigned long long ui = nmx_scan_wave(units);
+        unsigned long long mine = 0;
+#pragma unroll 1
+        for (int k = 0; k < 2; k++) {
+            if (k && !__any(mx)) break;
+            const unsigned long long own = mx == (k == 1) ? cost : 0, ci = nmx_scan_wave(own);
+            if (mx == (k == 1)) mine = cb[k] + ci - own;
+            cb[k] += __shfl(ci, 63);
+        }
+        if (j < G + S) seg[j].c0 = mine, seg[j].u0 = (uint32_t)(mx ? (ub + ui - units) >> 32 : ub + ui - units);
+        ub += __shfl(ui, 63);
     }
     nmx_lds_wave_sync();
-    return (cb + AB_WGS - 1) / AB_WGS;
+    /* workgroups in the proportion of the costs, one at least for each kind */
+    Shares sh;
+    const float part = (float)cb[1] / ((float)cb[0] + (float)cb[1] + 1.0f) * AB_WGS;
+    sh.mx = !cb[1] ? 0 : !cb[0] ? AB_WGS : part < 1.0f ? 1 : part > AB_WGS - 1 ? AB_WGS - 1 : (int)part;
+    const uint32_t waves = (uint32_t)(AB_WGS - sh.mx) * AB_PARTS;
+    auto over = [](unsigned long long c, uint32_t n) { return n ? c >> 32 ? (c + n - 1) / n : ((uint32_t)c + (unsigned long long)n - 1) >> 32 ? (c + n - 1) / n : ((uint32_t)c + n - 1) / n : 0; };
+    sh.per_m = over(cb[1], sh.mx), sh.per_w = over(cb[0], waves);
+    return sh;
 }
 
 /* What a share does next: the part of a unit that begins at cost c, by one wave (x.unit 0: nothing more). */
 struct Piece {
     Seg x;
     int tile, g, p0, p1;
-    uint32_t slot;
+    uint32_t unit; /* units of its kind before this one */
     unsigned long long next;
 };
 template <int HDP>
-__device__ __forceinline__ void find_piece(const BatchAttn &a, const Seg *seg, unsigned long long c, unsigned long long end, int w,
-                                           Piece *piece) {
-    const int lane = lane_id(), segs = a.groups + a.pg.seqs, nkv = a.pg.nkv;
+__device__ __forceinline__ void find_piece(const BatchAttn &a, int segs, const Seg *seg, bool matrix, unsigned long long c,
+                                           unsigned long long end, Piece *piece) {
+    const int lane = lane_id(), nkv = a.pg.nkv;
     if (lane == 0) piece->x.unit = 0;
     nmx_lds_wave_sync();
     if (c < end)
@@ -242,16 +278,16 @@ __device__ __forceinline__ void find_piece(const BatchAttn &a, const Seg *seg, u
         for (int j = lane; j < segs; j += 64) {
             const unsigned long long c0 = seg[j].c0;
             const uint32_t unit = seg[j].unit;
-            if (!unit || c < c0) continue;
             const bool mx = seg[j].m > AB_VR;
+            if (!unit || mx != matrix || c < c0) continue;
             const int tiles = mx ? (seg[j].m + tile_rows<HDP>() - 1) / tile_rows<HDP>() * halves<HDP>() : 1;
             if (c - c0 >= (unsigned long long)unit * (uint32_t)(tiles * nkv)) continue;
             const unsigned long long off = c - c0; /* one lane comes here */
             const uint32_t u = off >> 32 ? (uint32_t)(off / unit) : (uint32_t)off / unit;
             const unsigned long long cu = c0 + (unsigned long long)u * unit, cn = cu + unit < end ? cu + unit : end;
-            const int each = mx ? AB_COST_M : AB_COST_V;
+            const int each = step_cost(seg[j].m), begin = mx ? AB_BEGIN_M : AB_BEGIN_V;
             auto steps = [&](unsigned long long cost) { /* of a unit, begun by the first part of its cost */
-                return cost <= AB_COST_UNIT ? 0 : ((int)(uint32_t)cost - AB_COST_UNIT + each - 1) / each;
+                return cost <= (uint32_t)begin ? 0 : ((int)(uint32_t)cost - begin + each - 1) / each;
             };
             const Seg x = seg[j];
             piece->x = x;
@@ -259,8 +295,9 @@ __device__ __forceinline__ void find_piece(const BatchAttn &a, const Seg *seg, u
             piece->p0 = x.p0 + steps(c - cu) * AT_P;
             const int p1 = x.p0 + steps(cn - cu) * AT_P;
             piece->p1 = p1 < x.p1 ? p1 : x.p1;
-            piece->slot = w + x.u0 + u, piece->next = cn;
+            piece->unit = x.u0 + u, piece->next = cn;
         }
+    nmx_lds_wave_sync();
 }
 
 /* ---- the shares ---------------------------------------------------------------------------------- */
@@ -312,6 +349,20 @@ __device__ __forceinline__ float widen(const Raw8<KV_I8> &r, int i) {
     return (float)(int8_t)((i < 4 ? r.a.x : r.a.y) >> 8 * (i & 3));
 }
 
+/* the sum over W neighbouring lanes, in each of them */
+template <int W>
+__device__ __forceinline__ float sum_group(float v) {
+    auto with = [&](int o) { v += __int_as_float(o); };
+    if (W >= 2) with(nmx_dpp<NMX_DPP_XOR1>(__float_as_int(v)));
+    if (W >= 4) with(nmx_dpp<NMX_DPP_XOR2>(__float_as_int(v)));
+    if (W >= 8) with(nmx_dpp<NMX_DPP_HALF_MIRROR>(__float_as_int(v)));
+    if (W >= 16) with(nmx_dpp<NMX_DPP_MIRROR>(__float_as_int(v)));
+    if (W >= 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    }
+    return v;
+}
 /* v of lane r of each four neighbours, in all four */
 template <int R>
 __device__ __forceinline__ float of_quad(float v) {
@@ -321,67 +372,70 @@ __device__ __forceinline__ float quad_row(float v, int r) { /* r constant where 
     return r == 0 ? of_quad<0>(v) : r == 1 ? of_quad<1>(v) : r == 2 ? of_quad<2>(v) : of_quad<3>(v);
 }
 
-/* What a share finds of a unit of few rows: positions [p0, p1) of segment x's KV head g, to part and stat. A wave
- * takes 4 query rows; waves: groups of 4 rows first, then positions, in turns.
+/* What a wave finds of a unit of few rows: 4 query rows, the rq-th, of segment x's KV head g over the ws-th of NS
+ * shares of the positions [p0, p1), which change hands every 4 positions; to part and stat, where `together` is set with the
+ * workgroup's other waves.
  *
- * Scores on the matrix cores, 16 positions at a time and keys straight from memory: as first operand they lie in
- * a lane as they lie in a row. The second operand has 16 columns for 4 query rows: with 16-bit keys the
- * rows' high and low parts stand in columns 4 apart and one product makes both; fp32 keys take the fp32
- * instruction. Lane (quarter gq, column c) then holds the scores of row c mod 4 at the positions 4 gq .. 4 gq + 3, and
- * the same quarter adds those positions' values, 16 columns (two chunks of 8) a lane, by vector instructions: a
- * row's weight comes from a lane of the quad. (All by vector instructions a turn took 3.4 us of issue for 128 positions
- * and CU, this 1.3.) */
+ * Values: a lane adds 16 columns (two chunks of 8) of its positions' rows by vector instructions, a row's weight comes
+ * from a lane of its quad: lane (quarter gq, column c) has the weights of row c mod 4.
+ * Scores of 16-bit keys on the matrix cores, 16 positions at a time and straight from memory: as first operand keys lie in
+ * a lane as they lie in a row. The second operand has 16 columns for 4 query rows, so their high and low parts
+ * stand in columns 4 apart and one product makes both. (By vector instructions a turn took 3.4 us of issue for 128
+ * positions and CU, this 1.3.) fp32 keys are loaded as values are and take vector instructions too: they come at half
+ * the positions a second, and the matrix cores' fp32 products, 16 columns for 4 rows, took 20.5 against 14.9 us over
+ * 4 x 500 positions. */
 template <int HDP, int KVT>
-__device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, int g, int p0, int p1, float *part, float4 *stat,
-                                             uint4 *smem) {
+__device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, int g, int p0, int p1, int rq, int ws, int NS,
+                                             bool together, float *part, float4 *stat, uint4 *smem) {
     constexpr int WV = ctx_waves<HDP>(), LPP = HDP / 16;   /* lanes of a position's values */
     constexpr int NT = HDP < 256 ? 256 / HDP : 1;          /* tiles of 16 positions a turn */
-    constexpr int VP = HDP > 256 ? 8 : 4;                  /* positions whose values a lane adds in a turn */
-    constexpr int KW = KVT == KV_F32 ? 16 : 32, KN = HDP / KW; /* columns of a key's chunk (over the quarters), chunks */
-    constexpr int KH = KVT != KV_F32 ? 1 : HDP == 64 ? 4 : 2, KP = KN / KH; /* parts that a key comes in: fp32 rows have no room whole */
+    constexpr bool F32 = KVT == KV_F32;
+    constexpr int VT = !F32 ? 4 : HDP > 256 ? 1 : 2;       /* positions of a quarter in a tile (fp32: no room for four) */
+    constexpr int VP = HDP > 256 ? 2 * VT : VT;            /* positions whose values a lane adds in a turn */
+    constexpr int KN = F32 ? 1 : HDP / 32;                 /* a key's chunks of 32 columns over the quarters */
+    constexpr int NW = F32 ? VP : NT * VT;                 /* scores of a lane in a turn */
     const int lane = lane_id(), wave = wave_id(), l = lane % LPP, c = lane & 15, gq = lane >> 4, hd = a.pg.hd, rep = a.nh / a.pg.nkv;
-    const int quads = x.m > 8 ? 4 : x.m > 4 ? 2 : 1, rq = wave % quads, ws = wave / quads, NS = WV / quads;
     const PagedHead<KVT> kh(a.pg, a.kc, x.seq, g), vh(a.pg, a.vc, x.seq, g);
     int col[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) col[j] = (l + LPP * j) * 8, col[j] = col[j] < hd ? col[j] : 0;
-    /* the positions of a turn: position v of quarter q in tile n is 4 NS (4 n + v) + 4 ws + q, so that few positions
+    /* the positions of a turn: position v of quarter q in tile n is 4 NS (VT n + v) + 4 ws + q, so that few positions
      * spread over all waves; behind the end the last one stands in and has no weight */
-    const int turn = 16 * NT * NS;
-    auto at = [&](int base, int n, int q, int v) { return base + 4 * NS * (4 * n + v) + 4 * ws + q; };
+    const int turn = 4 * VT * NT * NS;
+    auto at = [&](int base, int n, int q, int v) { return base + 4 * NS * (VT * n + v) + 4 * ws + q; };
     auto in = [&](int p) { return p < p1 ? p : p1 - 1; };
     /* a lane's values: those of its quarter in the tile that its LPP lanes have (HDP 512: of two quarters) */
-    const int vt = LPP < 16 ? lane / LPP % (16 / LPP) : 0;
-    auto at_v = [&](int base, int v) { return HDP > 256 ? at(base, 0, (gq & 2) + (v >> 2), v & 3) : at(base, vt, gq, v); };
+    const int vt = lane / LPP % (LPP < 16 ? 16 / LPP : 1);
+    auto at_v = [&](int base, int v) { return HDP > 256 ? at(base, 0, (gq & 2) + v / VT, v % VT) : at(base, vt, gq, v); };
     int pk[NT], pv[VP];
     auto ask = [&](int base) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) pk[n] = kh.page_of(in(at(base, n, c >> 2, c & 3)));
+        for (int n = 0; n < NT && !F32; n++) pk[n] = kh.page_of(in(at(base, n, c >> 2, c & 3)));
 #pragma unroll
         for (int v = 0; v < VP; v++) pv[v] = vh.page_of(in(at_v(base, v)));
     };
     typedef typename std::conditional<KVT == KV_I8, uint2, uint4>::type KeyChunk;
-    KeyChunk rk[NT][KP];
-    const char *row[NT];
-    Raw8<KVT> rv[VP][2];
+    KeyChunk rk[NT][KN];
+    Raw8<KVT> rf[F32 ? VP : 1][2], rv[VP][2]; /* rf: fp32 keys */
     float sk[NT], sv[NT]; /* int8: scales of position c of a tile (four of them are those of the lane's scores) */
-    auto find_k = [&](int base) {
+    auto fetch_k = [&](int base) {
+        if constexpr (F32) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int p = in(at(base, n, c >> 2, c & 3));
-            row[n] = kh.at(pk[n], p, KW / 4 * gq);
-            if (KVT == KV_I8) sk[n] = kh.scale(pk[n], p), sv[n] = vh.scale(pk[n], p);
-        }
-    };
-    auto fetch_k = [&](int part) {
+            for (int v = 0; v < VP; v++)
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+                for (int j = 0; j < 2; j++) rf[v][j] = kh.load8(pv[v], in(at_v(base, v)), col[j]);
+        } else {
 #pragma unroll
-            for (int k = 0; k < KP; k++) {
-                const int cc = KW * (part * KP + k);
-                if (cc < HDP / 2 + 64 || cc < hd) rk[n][k] = *(const KeyChunk *)(row[n] + cc * PagedHead<KVT>::SIZE);
-                else rk[n][k] = KeyChunk{}; /* columns behind hd */
+            for (int n = 0; n < NT; n++) {
+                const int p = in(at(base, n, c >> 2, c & 3));
+                const char *row = kh.at(pk[n], p, 8 * gq);
+#pragma unroll
+                for (int k = 0; k < KN; k++)
+                    if (32 * k < HDP / 2 + 64 || 32 * k < hd) rk[n][k] = *(const KeyChunk *)(row + 32 * k * PagedHead<KVT>::SIZE);
+                    else rk[n][k] = KeyChunk{}; /* columns behind hd */
+                if (KVT == KV_I8) sk[n] = kh.scale(pk[n], p), sv[n] = vh.scale(pk[n], p);
             }
+        }
     };
     auto fetch_v = [&](int base) {
 #pragma unroll
@@ -393,32 +447,30 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
     /* the query rows: row c mod 4 of this wave's; rows past the last one are of no use to anyone */
     const int rr = rq * 4 + (c & 3), ri = rr < x.m ? rr : 0;
     const float *qp = a.q + ((size_t)(x.r0 + ri / rep) * a.nh + g * rep + ri % rep) * 2 * hd;
-    half8 qx[KVT == KV_F32 ? 1 : KN];
+    half8 qx[KN];
     float qf = a.scale * AT_LOG2E;
-    float *qs = (float *)smem; /* fp32: [16 rows][HDP] in LDS, they have no registers to stay in */
-    constexpr int Q4 = HDP / 4, QU = (AB_VR * Q4 + 64 * WV - 1) / (64 * WV);
-    if constexpr (KVT == KV_F32) {
+    float *qs = (float *)smem + wave * 4 * HDP; /* fp32: this wave's rows in LDS, they have no registers to stay in */
+    if constexpr (F32) {
+        constexpr int QU = HDP / 64;
         float4 qv[QU];
 #pragma unroll
-        for (int u = 0; u < QU; u++) {
-            const int e = u * 64 * WV + 64 * wave + lane, r = e / Q4 < x.m ? e / Q4 : 0, q4 = e % Q4 * 4;
-            qv[u] = *(const float4 *)(a.q + ((size_t)(x.r0 + r / rep) * a.nh + g * rep + r % rep) * 2 * hd + (q4 < hd ? q4 : 0));
+        for (int u = 0; u < QU; u++) { /* lane: row c mod 4, 16-byte pieces lane / 4 + 16 u of it */
+            const int q4 = (lane / 4 + 16 * u) * 4;
+            qv[u] = *(const float4 *)(qp + (q4 < hd ? q4 : 0));
             if (q4 >= hd) qv[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        find_k(p0);
-        fetch_k(0);
+        fetch_k(p0);
         fetch_v(p0);
+        nmx_lds_wave_sync();
 #pragma unroll
-        for (int u = 0; u < QU; u++) {
-            /* 16-byte pieces of a row moved by its number, so that four rows' reads meet no bank twice */
-            const int e = u * 64 * WV + 64 * wave + lane;
-            if (e < AB_VR * Q4) *(float4 *)(qs + e / Q4 * HDP + ((e % Q4) ^ (e / Q4 % 4)) * 4) = qv[u];
+        for (int u = 0; u < QU; u++) { /* [row][chunk][half][lane][4], as the lanes of a position read them */
+            const int piece = lane / 4 + 16 * u, chunk = piece / 2 / LPP;
+            *(float4 *)(qs + (c & 3) * HDP + ((chunk * 2 + piece % 2) * LPP + piece / 2 % LPP) * 4) = qv[u];
         }
-        nmx_lds_sync();
+        nmx_lds_wave_sync();
     } else {
         QueryRow<KN> qr(qp, true, hd, gq);
-        find_k(p0);
-        fetch_k(0);
+        fetch_k(p0);
         fetch_v(p0);
         half8 ql[KN];
         qf = qr.split(a.scale, qx, ql);
@@ -433,63 +485,73 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
     for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[r][i] = 0.0f;
-    int q_at = (rq * 4 + (c & 3)) * HDP;
+    int q_at = 4 * l;
     for (int base = p0; base < p1; base += turn) {
-        float4v s4[NT];
+        /* scores of row c mod 4 at this lane's positions: its quarter's in each tile, or (fp32) those of its values */
+        float w[NW], fv[NW];
+        if constexpr (F32) {
+            asm volatile("" : "+v"(q_at)); /* the query rows are read anew each turn: they have no registers to stay in */
+            float s[VP][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++) s4[n] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-        if (KVT == KV_F32) asm volatile("" : "+v"(q_at)); /* the rows are read anew each turn */
+            for (int v = 0; v < VP; v++)
 #pragma unroll
-        for (int part = 0; part < KH; part++) {
+                for (int r = 0; r < 4; r++) s[v][r] = 0.0f;
 #pragma unroll
-            for (int kp = 0; kp < KP; kp++) {
-                const int k = part * KP + kp;
-                if constexpr (KVT == KV_F32) {
-                    if (k % 4 == 0) __builtin_amdgcn_sched_barrier(0); /* four pieces of a row in registers at once, not all */
-                    const float4 q = *(const float4 *)(qs + q_at + ((4 * k + gq) ^ (c & 3)) * 4);
+            for (int e = 0; e < 4; e++) {
+                float4 q[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                for (int r = 0; r < 4; r++) q[r] = *(const float4 *)(qs + q_at + r * HDP + e * 4 * LPP);
 #pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            const uint4 y = rk[n][kp];
-                            s4[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(i == 0 ? y.x : i == 1 ? y.y : i == 2 ? y.z : y.w),
-                                                                         i == 0 ? q.x : i == 1 ? q.y : i == 2 ? q.z : q.w, s4[n], 0, 0, 0);
-                        }
-                } else {
+                for (int v = 0; v < VP; v++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        half8 y;
-                        if constexpr (KVT == KV_F16) y = __builtin_bit_cast(half8, rk[n][kp]);
-                        else y = codes8(rk[n][kp]);
-                        s4[n] = mfma16(y, qx[k], s4[n]);
+                    for (int i = 0; i < 4; i++) {
+                        const float k = widen(rf[v][e >> 1], 4 * (e & 1) + i);
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            s[v][r] = __builtin_fmaf(k, i == 0 ? q[r].x : i == 1 ? q[r].y : i == 2 ? q[r].z : q[r].w, s[v][r]);
                     }
-                }
             }
-            if (part + 1 < KH) fetch_k(part + 1);
-        }
-        float fv[NT][4];
-        if constexpr (KVT == KV_I8) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    const int from = (lane & 48) + 4 * gq + v;
-                    s4[n][v] *= __shfl(sk[n], from), fv[n][v] = __shfl(sv[n], from);
-                }
-        }
-        find_k(base + turn); /* behind the last turn the last position again */
-        fetch_k(0);
-        float w[NT][4], top = m;
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) {
-                float s = s4[n][v];
-                if (KVT != KV_F32) s += __int_as_float(nmx_dpp<0x124>(__float_as_int(s))); /* high and low: 4 columns on */
-                s *= qf;
-                w[n][v] = at(base, n, gq, v) < lim ? s : -INFINITY;
-                top = fmaxf(top, w[n][v]);
+            for (int v = 0; v < VP; v++) {
+                const float r0 = sum_group<LPP>(s[v][0]), r1 = sum_group<LPP>(s[v][1]);
+                const float r2 = sum_group<LPP>(s[v][2]), r3 = sum_group<LPP>(s[v][3]);
+                const float low = c & 1 ? r1 : r0, high = c & 1 ? r3 : r2;
+                w[v] = c & 2 ? high : low;
             }
+        } else {
+            float4v s4[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) s4[n] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < KN; k++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    half8 y;
+                    if constexpr (KVT == KV_F16) y = __builtin_bit_cast(half8, rk[n][k]);
+                    else y = codes8(rk[n][k]);
+                    s4[n] = mfma16(y, qx[k], s4[n]);
+                }
+#pragma unroll
+            for (int i = 0; i < NW; i++) {
+                float s = s4[i / VT][i % VT];
+                s += __int_as_float(nmx_dpp<0x124>(__float_as_int(s))); /* high and low: 4 columns on */
+                if (KVT == KV_I8) { /* the scales are with lane c = 4 quarter + v of a quarter */
+                    const int from = (lane & 48) + 4 * gq + i % VT;
+                    s *= __shfl(sk[i / VT], from), fv[i] = __shfl(sv[i / VT], from);
+                }
+                w[i] = s;
+            }
+        }
+        fetch_k(base + turn); /* behind the last turn the last position again */
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            const int p = F32 ? at_v(base, i) : at(base, i / VT, gq, i % VT);
+            w[i] = p < lim ? w[i] * qf : -INFINITY;
+            top = fmaxf(top, w[i]);
+        }
+        if (F32 && LPP <= 4) top = fmaxf(top, __int_as_float(nmx_dpp<0x124>(__float_as_int(top))));
+        if (F32 && LPP <= 8) top = fmaxf(top, __int_as_float(nmx_dpp<0x128>(__float_as_int(top))));
         top = max_quarters(top);
         if (__any(top > m)) {
             const float down = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
@@ -504,26 +566,27 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
         const float ref = m == -INFINITY ? 0.0f : m;
         float all = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int v = 0; v < 4; v++) {
-                w[n][v] = __builtin_amdgcn_exp2f(w[n][v] - ref);
-                all += w[n][v];
-                if (KVT == KV_I8) w[n][v] *= fv[n][v];
-            }
-        const float more = all - lost, now = sum + more; /* the roundings of a long share's sum are kept */
-        lost = (now - sum) - more, sum = now;
+        for (int i = 0; i < NW; i++) {
+            w[i] = __builtin_amdgcn_exp2f(w[i] - ref);
+            all += w[i];
+            if (KVT == KV_I8) w[i] *= fv[i];
+        }
+        const float gain = all - lost, now = sum + gain; /* the roundings of a long share's sum are kept */
+        lost = (now - sum) - gain, sum = now;
         /* the weights of the positions whose values this lane adds */
         float u[VP];
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
-            if constexpr (HDP > 256) { /* of both quarters of its half */
-                const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(w[0][v]), __float_as_uint(w[0][v]), false, false);
-                u[v] = __uint_as_float(y[0]), u[v + 4] = __uint_as_float(y[1]);
+        for (int v = 0; v < VT; v++) {
+            if constexpr (F32) {
+                u[v] = w[v];
+                if (HDP > 256) u[v + VT] = w[(v + VT) % NW];
+            } else if constexpr (HDP > 256) { /* of both quarters of its half */
+                const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(w[v]), __float_as_uint(w[v]), false, false);
+                u[v] = __uint_as_float(y[0]), u[v + VT] = __uint_as_float(y[1]);
             } else {
-                u[v] = w[0][v];
+                u[v] = w[v];
 #pragma unroll
-                for (int n = 1; n < NT; n++) u[v] = vt == n ? w[n][v] : u[v];
+                for (int n = 1; n < NT; n++) u[v] = vt == n ? w[VT * n + v] : u[v];
             }
         }
 #pragma unroll
@@ -543,12 +606,16 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
         fetch_v(base + turn);
         ask(base + 2 * turn);
     }
-    nmx_lds_sync(); /* the query rows have been read */
-    /* the wave's groups of lanes together, then the waves through LDS */
-    float *vals = (float *)smem;                  /* [WV][4][HDP] */
-    float2 *ml = (float2 *)(vals + WV * 4 * HDP); /* [WV][4]: maximum, sum */
-    const float total = nmx_sum_quarters(sum - lost);
-    if (lane < 4) ml[wave * 4 + lane] = make_float2(m, total);
+    /* a lane's sums over the wave's quarters */
+    float total = sum - lost;
+    if (F32 && LPP <= 4) total += __int_as_float(nmx_dpp<0x124>(__float_as_int(total)));
+    if (F32 && LPP <= 8) total += __int_as_float(nmx_dpp<0x128>(__float_as_int(total)));
+    if (F32 && LPP > 16) { /* the quarters of a half have the same positions */
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(total), __float_as_uint(total), false, false);
+        total = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+    } else {
+        total = nmx_sum_quarters(total);
+    }
     if (LPP < 16) { /* within a quarter first: rows of 16 lanes turned by 4 and by 8 */
 #pragma unroll
         for (int r = 0; r < 4; r++)
@@ -575,22 +642,30 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
             keep[0][i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
         }
     }
+    float *vals = (float *)smem;                  /* together: [WV][4][HDP] */
+    float2 *ml = (float2 *)(vals + WV * 4 * HDP); /* [WV][4]: maximum, sum */
+    if (together && lane < 4) ml[wave * 4 + lane] = make_float2(m, total);
+    if (!together && lane < 4 && rq * 4 + lane < x.m) stat[rq * 4 + lane] = make_float4(m, 12.0f, total, 0.0f); /* as 2^12 high values */
     if (LPP >= 16 || lane % 16 < LPP) {
 #pragma unroll
         for (int k = 0; k < (LPP <= 16 ? 1 : 2); k++) {
             const int r = LPP <= 16 ? 2 * (lane >> 5) + (lane >> 4 & 1) : 2 * (lane >> 5) + k;
+            if (!together && rq * 4 + r >= x.m) continue;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                float *y = vals + (wave * 4 + r) * HDP + (l + LPP * j) * 8;
+                const int c8 = (l + LPP * j) * 8;
+                if (!together && c8 >= hd) continue;
+                float *y = together ? vals + (wave * 4 + r) * HDP + c8 : part + (size_t)(rq * 4 + r) * hd + c8;
                 *(float4 *)y = make_float4(keep[k][8 * j], keep[k][8 * j + 1], keep[k][8 * j + 2], keep[k][8 * j + 3]);
                 *(float4 *)(y + 4) = make_float4(keep[k][8 * j + 4], keep[k][8 * j + 5], keep[k][8 * j + 6], keep[k][8 * j + 7]);
             }
         }
     }
+    if (!together) return;
     __syncthreads();
-    const int c4 = hd / 4;
+    const int c4 = hd / 4, quads = WV / NS;
     for (int e = 64 * wave + lane; e < x.m * c4; e += 64 * WV) {
-        const int rr = e / c4, c = e % c4 * 4, r = rr & 3, first = rr >> 2;
+        const int rr = e / c4, cc = e % c4 * 4, r = rr & 3, first = rr >> 2;
         float top = -INFINITY;
         for (int w = first; w < WV; w += quads) top = fmaxf(top, ml[w * 4 + r].x);
         const float ref = top == -INFINITY ? 0.0f : top;
@@ -599,13 +674,13 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
         for (int w = first; w < WV; w += quads) {
             const float2 y = ml[w * 4 + r];
             const float f = __builtin_amdgcn_exp2f(y.x - ref);
-            const float4 z = *(const float4 *)(vals + (w * 4 + r) * HDP + c);
+            const float4 z = *(const float4 *)(vals + (w * 4 + r) * HDP + cc);
             all = __builtin_fmaf(y.y, f, all);
             v.x = __builtin_fmaf(z.x, f, v.x), v.y = __builtin_fmaf(z.y, f, v.y);
             v.z = __builtin_fmaf(z.z, f, v.z), v.w = __builtin_fmaf(z.w, f, v.w);
         }
-        *(float4 *)(part + (size_t)rr * hd + c) = v;
-        if (c == 0) stat[rr] = make_float4(top, 12.0f, all, 0.0f); /* as the matrix kind's 2^12 high values */
+        *(float4 *)(part + (size_t)rr * hd + cc) = v;
+        if (cc == 0) stat[rr] = make_float4(top, 12.0f, all, 0.0f);
     }
 }
 
@@ -638,46 +713,85 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
                                                                      int groups, int room, BatchAttn a) {
     constexpr int TH = 64 * ctx_waves<HDP>(), OD = HDP > 256 ? 256 : HDP;
     extern __shared__ uint4 smem[];
+    constexpr int WV = ctx_waves<HDP>();
     __shared__ Seg seg[AB_SEGS];
-    __shared__ Piece piece_s;
-    const int tid = threadIdx.x, segs = groups + seqs, w = blockIdx.x;
-    unsigned long long end = 0;
-    if (wave_id() == 0) {
-        const unsigned long long per = make_list<HDP>({row0, len, seqs, n, groups, room}, a, seg);
-        end = (w + 1) * per;
-        find_piece<HDP>(a, seg, w * per, end, w, &piece_s);
-        if (w == 0 && tid == 0) a.plan->per = per;
+    __shared__ Piece piece_s[WV];
+    __shared__ Shares sh_s;
+    const int tid = threadIdx.x, segs = groups + seqs, w = blockIdx.x, wave = wave_id();
+    if (wave == 0) {
+        const Shares sh = make_list<HDP>({row0, len, seqs, n, groups, room}, a, seg);
+        const bool mx = w < sh.mx;
+        const unsigned long long per = mx ? sh.per_m : sh.per_w * AB_PARTS, c = (unsigned long long)(mx ? w : w - sh.mx) * per;
+        find_piece<HDP>(a, segs, seg, mx, c, c + per, piece_s);
+        if (tid == 0) sh_s = sh;
+        if (w == 0 && tid == 0) a.plan->sh = sh;
     }
     __syncthreads();
     if (w == 0) /* the join's */
         for (int j = tid; j < segs; j += TH) a.plan->seg[j] = seg[j];
-    for (;;) {
-        auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); }; /* into scalars */
-        if (!same(piece_s.x.unit)) return;
-        Seg x{};
-        x.m = same(piece_s.x.m), x.r0 = same(piece_s.x.r0), x.seq = same(piece_s.x.seq), x.last = same(piece_s.x.last);
-        const int p0 = same(piece_s.p0), p1 = same(piece_s.p1), g = same(piece_s.g), tile = same(piece_s.tile);
-        const size_t slot = (uint32_t)same(piece_s.slot);
-        const unsigned long long next = piece_s.next;
-        if (x.m > AB_VR) {
+    /* between pieces everything is in LDS: a piece has no registers to spare */
+    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    int p0, p1, g, tile;
+    size_t unit;
+    Seg x{};
+    auto take = [&](const Piece &p) {
+        x.m = same(p.x.m), x.r0 = same(p.x.r0), x.seq = same(p.x.seq), x.last = same(p.x.last);
+        p0 = same(p.p0), p1 = same(p.p1), g = same(p.g), tile = same(p.tile), unit = (uint32_t)same(p.unit);
+        return same(p.x.unit) != 0;
+    };
+    const int mxs = same(sh_s.mx);
+    if (w < mxs) {
+        while (take(piece_s[0])) {
+            const size_t slot = w + unit;
             float4 *stat = a.stat_m + slot * tile_rows<HDP>();
             if (p0 < p1) matrix_piece<HDP, KVT>(a, x, g, tile / halves<HDP>(), tile % halves<HDP>(), p0, p1,
                                                 a.part_m + slot * tile_rows<HDP>() * OD, stat, smem);
             else if (tid < tile_rows<HDP>()) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-        } else {
-            float4 *stat = a.stat_v + slot * AB_VR;
-            if (p0 < p1) vector_piece<HDP, KVT>(a, x, g, p0, p1, a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
-            else if (tid < AB_VR) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            __syncthreads();
+            if (wave == 0) find_piece<HDP>(a, segs, seg, true, piece_s[0].next, (w + 1) * sh_s.per_m, piece_s);
+            __syncthreads();
         }
-        if (p0 >= p1) __syncthreads(); /* the others pass a barrier with the piece in their hands */
-        if (wave_id() == 0) find_piece<HDP>(a, seg, next, end, w, &piece_s);
-        __syncthreads();
+        return;
+    }
+    if (!take(piece_s[0])) return;
+    /* together in one unit (4 waves: as if they were 8), or each share by a wave alone */
+    const bool together = same(piece_s[0].next == (unsigned long long)(w - mxs + 1) * AB_PARTS * sh_s.per_w);
+    const int quads = x.m > 4 ? 2 : 1;
+    if (together) {
+        const size_t slot = (size_t)(w - mxs) * AB_PARTS + unit;
+        float4 *stat = a.stat_v + slot * AB_VR;
+        if (p0 < p1) vector_piece<HDP, KVT>(a, x, g, p0, p1, wave % quads, wave / quads, WV / quads, true,
+                                            a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
+        else if (tid < AB_VR) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        return;
+    }
+    __syncthreads(); /* everyone has read the first piece */
+    /* the waves that a row's heads take (4 each) go over the same positions at the same time */
+    const int heads = a.nh / a.pg.nkv, team = heads > 4 ? 2 : 1;
+#pragma unroll 1
+    for (int share = (w - mxs) * AB_PARTS + wave / team; share < (w - mxs + 1) * AB_PARTS; share += WV / team) {
+        if (tid % 64 == 0) piece_s[wave].next = share * sh_s.per_w;
+        nmx_lds_wave_sync();
+#pragma unroll 1
+        for (;;) {
+            find_piece<HDP>(a, segs, seg, false, piece_s[wave].next, (share + 1) * sh_s.per_w, piece_s + wave);
+            if (!take(piece_s[wave])) break;
+            const size_t slot = share + unit;
+            float4 *stat = a.stat_v + slot * AB_VR;
+            if (p0 >= p1 && tid % 64 < AB_VR) stat[tid % 64] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+            for (int k = wave % team; 4 * k < x.m && p0 < p1; k += team) {
+                /* nothing of a pass is kept for the next one */
+                asm volatile("" : "+s"(p0), "+s"(p1), "+s"(g), "+s"(x.seq), "+s"(x.r0), "+s"(x.m), "+s"(x.last));
+                vector_piece<HDP, KVT>(a, x, g, p0, p1, k, 0, 1, false, a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
+            }
+        }
     }
 }
 
 /* ---- the join -------------------------------------------------------------------------------------- */
 constexpr int JB = 256;              /* threads */
-constexpr int JB_PARTS = 2 * AB_WGS + 2;
+constexpr int JB_PARTS = 2 * (AB_WGS + 2 * AB_PARTS);
 
 /* Workgroup: a row and head, blockIdx.y a group of a.jcols columns of it (of one half). */
 template <int HDP>
@@ -688,7 +802,7 @@ __global__ __launch_bounds__(JB) void attn_batch_join_k(BatchAttn a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.x / a.nh, h = blockIdx.x % a.nh;
     const int hd = a.pg.hd, nkv = a.pg.nkv, rep = a.nh / nkv, g = h / rep, c0 = blockIdx.y * a.jcols, half = c0 / OD;
     const float gate = a.q[((size_t)t * a.nh + h) * 2 * hd + hd + c0 + (tid < a.jcols ? tid : 0)];
-    const unsigned long long per = a.plan->per;
+    const Shares sh = a.plan->sh;
     const int s = seq_of_row(a.row0, a.pg.seqs, t);
     if (s < 0) return; /* uniform over the workgroup */
     const SeqRows rows = seq_rows(a.row0, s, a.n);
@@ -697,24 +811,32 @@ __global__ __launch_bounds__(JB) void attn_batch_join_k(BatchAttn a) {
     Seg pre = own;
     pre.unit = 0;
     if (own.group >= 0) pre = a.plan->seg[own.group];
-    /* the parts of this row and half: those of the prefix, then the sequence's own */
-    int count[2];
+    /* The parts of this row and half: those of the prefix, then the sequence's own. Of a unit of few rows: those of
+     * single waves, of workgroups whose share lies in it, of single waves. */
+    int count[2], solo[2], whole[2];
     const float *val[2];
     const float4 *st[2];
     size_t vstep[2], sstep[2];
-#pragma unroll
+    auto over = [](unsigned long long c, unsigned long long n) {
+        return c >> 32 || n >> 32 ? (uint32_t)(c / n) : (uint32_t)c / (uint32_t)n;
+    };
+#pragma unroll 1
     for (int k = 0; k < 2; k++) {
         const Seg &x = k ? own : pre;
         const int rr = (t - x.r0) * rep + h % rep;
-        count[k] = 0, val[k] = nullptr, st[k] = nullptr, vstep[k] = sstep[k] = 0;
+        count[k] = 0, solo[k] = whole[k] = 0, val[k] = nullptr, st[k] = nullptr, vstep[k] = sstep[k] = 0;
         if (!x.unit || rr < 0 || rr >= x.m) continue;
         const bool mx = x.m > AB_VR;
         const int tr = mx ? tile_rows<HDP>() : AB_VR, width = mx ? OD : hd;
         const uint32_t u = (mx ? rr / tr * halves<HDP>() + half : 0) * nkv + g;
-        const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit;
-        const uint32_t w0 = (uint32_t)(cu / per), w1 = (uint32_t)((cu + x.unit - 1) / per);
+        const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit, per = mx ? sh.per_m : sh.per_w;
+        const uint32_t w0 = over(cu, per), w1 = over(cu + x.unit - 1, per);
+        count[k] = solo[k] = (int)(w1 - w0) + 1;
+        if (!mx) {
+            const uint32_t f0 = (w0 * per == cu ? w0 + AB_PARTS - 1 : w0 + AB_PARTS) / AB_PARTS, f1 = over(cu + x.unit, per) / AB_PARTS;
+            if (f1 > f0) solo[k] = (int)(f0 * AB_PARTS - w0), whole[k] = (int)(f1 - f0), count[k] -= whole[k] * (AB_PARTS - 1);
+        }
         const size_t slot = (size_t)w0 + x.u0 + u;
-        count[k] = (int)(w1 - w0) + 1;
         val[k] = (mx ? a.part_m : a.part_v) + (slot * tr + rr % tr) * width + (mx ? c0 - half * OD : c0);
         st[k] = (mx ? a.stat_m : a.stat_v) + slot * tr + rr % tr;
         vstep[k] = (size_t)tr * width, sstep[k] = tr;
@@ -725,7 +847,9 @@ __global__ __launch_bounds__(JB) void attn_batch_join_k(BatchAttn a) {
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < PT; k++) {
-        const int i = tid + JB * k, b = i >= count[0], at = b ? i - count[0] : i;
+        const int i = tid + JB * k, b = i >= count[0], nth = b ? i - count[0] : i;
+        const int inner = nth - solo[b]; /* parts of whole workgroups stand AB_PARTS slots apart */
+        const int at = inner <= 0 ? nth : nth + (inner < whole[b] ? inner : whole[b]) * (AB_PARTS - 1);
         y[k] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         if (i < parts) y[k] = st[b][at * sstep[b]], at_s[i] = val[b] + at * vstep[b];
         top = fmaxf(top, y[k].x);
@@ -794,8 +918,8 @@ Room make_room(int n, int seqs, int groups, int nh, int nkv, int hd) {
     r.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 256 ? 256 : 512;
     const size_t tr = r.hdp > 256 ? 64 : 128, od = r.hdp > 256 ? 256 : r.hdp, hv = r.hdp > 256 ? 2 : 1;
     const size_t qr = (size_t)n * (nh / nkv); /* query rows of a KV head */
-    const size_t sv = AB_WGS + (size_t)(seqs + groups) * nkv;
-    /* segments of more than 16 query rows, each a tile more than its whole ones; every row in two of them */
+    const size_t sv = AB_WGS * AB_PARTS + (size_t)(seqs + groups) * nkv;
+    /* segments of the matrix kind, each a tile more than its whole ones; every row in two of them */
     const size_t some = qr / (AB_VR + 1);
     const size_t big = (some < (size_t)seqs ? some : seqs) + (some < (size_t)groups ? some : groups);
     const size_t sm = big ? AB_WGS + (2 * (qr / tr) + big) * hv * nkv : 0;

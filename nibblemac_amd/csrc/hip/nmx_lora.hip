@@ -1,12 +1,13 @@
 /* Low-rank adapters of many requests (include/nmx.h nmx_lora): y += scale B (A x), each row with its own
  * adapter, for the matrices that share x.
  *
- * Rows with one adapter are taken together, 16 at a time, so that A and B are read once for them: the first
- * of every 16 (counted over the rows by ballots) is the leader of its tile, and a workgroup whose row leads
- * none ends. lora_down_k: 16 ranks of A x, the columns shared out over the waves; lora_up_k: 16 rows of B at a
- * time, added to y. Products are fp32 matrix instructions (16 x 16 x 4): a lane takes 8 neighbouring
- * columns of a weight row and of a row of x, the sum over the 32 columns of a wave's step has no order to keep, so
- * weights go from 16-byte loads to the operand without passing through LDS. */
+ * Rows with one adapter are taken together, 16 at a time (a tile), so that A and B are read once for them. A row's rank
+ * among those of its adapter is counted by ballots over the adapters that 64 rows have; the rows of rank 0, 16, ..
+ * lead the tiles, which are numbered in the order of their leaders. lora_down_k makes the list in every workgroup, leaves it
+ * in the workspace, and makes 16 ranks of A x, the columns shared out over its waves; lora_up_k adds 16 rows of B at a
+ * time to y. Products are fp32 matrix instructions (16 x 16 x 4): a lane takes 8 neighbouring columns of a weight
+ * row and of a row of x, the sum over the 32 columns of a wave's step has no order to keep, so weights go from
+ * 16-byte loads to the operand without passing through LDS. */
 #include "nmx_internal.h"
 #include "nmx_attn.h"
 #include "nmx_batch.h"
@@ -27,7 +28,8 @@ struct Lora {
     int adapters, rank;
     const int32_t *adapter, *ranks;
     const float *scale;
-    float *low; /* [count][n][rank16]: A x */
+    float *low;         /* [count][n][rank16]: A x */
+    struct Tile *tiles; /* [tiles] */
     int rank16;
     const void *A[NMX_MAX_SEGS], *B[NMX_MAX_SEGS];
     int rows[NMX_MAX_SEGS], y_stride[NMX_MAX_SEGS];
@@ -35,42 +37,55 @@ struct Lora {
     int first[NMX_MAX_SEGS + 1]; /* of lora_up_k's workgroups */
 };
 
-/* The tile that row t leads: its adapter (-1: t leads none) and this lane's row (lane & 15; rows past the last one
- * repeat t, live false). Every lane of the wave active. */
+/* Rows of one adapter (adapter -1: no such tile); row -1: fewer rows. */
 struct Tile {
-    int adapter, row, rank;
-    bool live;
+    int adapter, rank, row[16], pad[14];
 };
-__device__ __forceinline__ Tile lead(const Lora &a, int t) {
-    const int lane = threadIdx.x & 63, c = lane & 15;
-    int id[NMX_CHUNK_ROWS / 64];
-    const int mine = a.adapter[t];
+/* Tile number `want`, by the whole workgroup (at least n threads). */
+__device__ __forceinline__ void find_tile(const Lora &a, int want, Tile *tile) {
+    constexpr int B = NMX_CHUNK_ROWS / 64;
+    __shared__ int leads_s[B], first_s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int id[B];
 #pragma unroll
-    for (int u = 0; u < NMX_CHUNK_ROWS / 64; u++) id[u] = 64 * u < a.n ? a.adapter[64 * u + lane < a.n ? 64 * u + lane : 0] : -1;
-    Tile r{-1, t, 0, false};
-    if (mine < 0 || mine >= a.adapters) return r;
-    int before = 0, at = 0;
-#pragma unroll
-    for (int u = 0; u < NMX_CHUNK_ROWS / 64; u++) {
-        unsigned long long m = __ballot(64 * u + lane < a.n && id[u] == mine);
-        const int split = t - 64 * u; /* rows of this 64 before t */
-        const unsigned long long early = split >= 64 ? ~0ull : split > 0 ? (1ull << split) - 1 : 0;
-        before += __popcll(m & early);
-        m &= ~early;
-        /* the c-th of the rows from t on */
-        const int have = __popcll(m);
-        if (c >= at && c < at + have) {
-            unsigned long long k = m;
-            for (int i = at; i < c; i++) k &= k - 1;
-            r.row = 64 * u + __ffsll((long long)k) - 1, r.live = true;
+    for (int u = 0; u < B; u++) {
+        id[u] = -1;
+        if (64 * u < a.n) { /* uniform */
+            const int v = a.adapter[64 * u + lane < a.n ? 64 * u + lane : 0];
+            id[u] = 64 * u + lane < a.n && v >= 0 && v < a.adapters ? v : -1;
         }
-        at += have;
     }
-    if (before % 16) return r;
-    r.adapter = mine;
-    const int rk = a.ranks ? a.ranks[mine] : a.rank;
-    r.rank = rk < 0 ? 0 : rk < a.rank ? rk : a.rank;
-    return r;
+    int mine = -1, rank = 0;
+#pragma unroll
+    for (int u = 0; u < B; u++) mine = u == wave ? id[u] : mine;
+    for (unsigned long long left = __ballot(mine >= 0); left;) { /* an adapter of this wave's rows */
+        const int m = __builtin_amdgcn_readlane(mine, __ffsll((long long)left) - 1);
+        const unsigned long long same = __ballot(mine == m);
+        int before = 0;
+        for (int u = 0; u < wave; u++) {
+            int v = id[0];
+#pragma unroll
+            for (int k = 1; k < B; k++) v = u == k ? id[k] : v;
+            before += __popcll(__ballot(v == m));
+        }
+        if (mine == m) rank = before + __popcll(same & ((1ull << lane) - 1));
+        left &= ~same;
+    }
+    const unsigned long long leads = __ballot(mine >= 0 && rank % 16 == 0);
+    if (lane == 0 && wave < B) leads_s[wave] = __popcll(leads);
+    if (tid < 16) tile->row[tid] = -1;
+    if (tid == 0) tile->adapter = -1;
+    __syncthreads();
+    int number = __popcll(leads & ((1ull << lane) - 1));
+    for (int w = 0; w < wave && w < B; w++) number += leads_s[w];
+    if (mine >= 0 && rank % 16 == 0 && number == want) {
+        const int rk = a.ranks ? a.ranks[mine] : a.rank;
+        tile->adapter = mine, tile->rank = rk < 0 ? 0 : rk < a.rank ? rk : a.rank;
+        first_s = rank;
+    }
+    __syncthreads();
+    if (mine >= 0 && mine == tile->adapter && rank >= first_s && rank < first_s + 16) tile->row[rank - first_s] = tid;
+    __syncthreads();
 }
 
 /* 8 weights as they lie in memory, widened */
@@ -107,14 +122,17 @@ __device__ __forceinline__ float4v mfma4(float a, float b, float4v c) {
 template <int WT>
 __global__ __launch_bounds__(64 * LD_WAVES) void lora_down_k(Lora a) {
     __shared__ float4 sum_s[LD_WAVES][64];
+    __shared__ Tile tile;
     constexpr int SIZE = WT == W_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, k = lane >> 4;
-    const Tile t = lead(a, blockIdx.x);
-    if (t.adapter < 0) return; /* uniform over the workgroup */
+    find_tile(a, blockIdx.x, &tile);
+    if (blockIdx.y == 0 && threadIdx.x < 18) ((int *)(a.tiles + blockIdx.x))[threadIdx.x] = ((int *)&tile)[threadIdx.x];
+    const int adapter = tile.adapter, own = tile.rank, row = tile.row[c];
+    if (adapter < 0) return; /* uniform over the workgroup */
     const int blocks = a.rank16 / 16, s = blockIdx.y / blocks, r0 = blockIdx.y % blocks * 16;
     const int r = r0 + c < a.rank ? r0 + c : a.rank - 1;
-    const char *wp = (const char *)a.A[s] + (((size_t)t.adapter * a.rank + r) * a.cols + 8 * k) * SIZE;
-    const float *xp = a.x + (size_t)t.row * a.x_stride + 8 * k;
+    const char *wp = (const char *)a.A[s] + (((size_t)adapter * a.rank + r) * a.cols + 8 * k) * SIZE;
+    const float *xp = a.x + (size_t)(row < 0 ? tile.row[0] : row) * a.x_stride + 8 * k;
     float4v acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
     constexpr int U = 4; /* steps of 32 columns requested at once */
     for (int c0 = wave * 32; c0 < a.cols; c0 += 32 * LD_WAVES * U) {
@@ -144,76 +162,103 @@ __global__ __launch_bounds__(64 * LD_WAVES) void lora_down_k(Lora a) {
         const float4 y = sum_s[w][lane];
         v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
     }
-    if (!t.live) return;
+    if (row < 0) return;
     /* ranks 4 k .. 4 k + 3 of row c; those that the adapter lacks are zeros, whatever A holds there */
     const int q = r0 + 4 * k;
-    if (q >= t.rank) v.x = 0.0f;
-    if (q + 1 >= t.rank) v.y = 0.0f;
-    if (q + 2 >= t.rank) v.z = 0.0f;
-    if (q + 3 >= t.rank) v.w = 0.0f;
-    *(float4 *)(a.low + ((size_t)s * a.n + t.row) * a.rank16 + q) = v;
+    if (q >= own) v.x = 0.0f;
+    if (q + 1 >= own) v.y = 0.0f;
+    if (q + 2 >= own) v.z = 0.0f;
+    if (q + 3 >= own) v.w = 0.0f;
+    *(float4 *)(a.low + ((size_t)s * a.n + row) * a.rank16 + q) = v;
 }
 
-/* Workgroup: a row, blockIdx.y a run of output rows of a matrix. VEC: rows of B are 16-byte aligned. */
+/* Workgroup: a tile, blockIdx.y a run of output rows of a matrix. VEC: rows of B are 16-byte aligned. */
 template <int WT, bool VEC>
 __global__ __launch_bounds__(64 * LU_WAVES) void lora_up_k(Lora a) {
     constexpr int SIZE = WT == W_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, k = lane >> 4;
-    const Tile t = lead(a, blockIdx.x);
-    if (t.adapter < 0) return;
+    const Tile *tile = a.tiles + blockIdx.x;
+    const int adapter = __builtin_amdgcn_readfirstlane(tile->adapter), own = __builtin_amdgcn_readfirstlane(tile->rank), row = tile->row[c];
+    if (adapter < 0) return;
     int s = 0;
     while (s + 1 < a.count && (int)blockIdx.y >= a.first[s + 1]) s++;
     const int rows = a.rows[s], o0 = (((int)blockIdx.y - a.first[s]) * LU_WAVES + wave) * 16 * LU_EACH;
     if (o0 >= rows) return;
-    const float scale = a.scale[t.adapter];
-    const float *lp = a.low + ((size_t)s * a.n + t.row) * a.rank16 + 8 * k;
+    const bool live = row >= 0;
+    const int any = live ? row : __builtin_amdgcn_readfirstlane(row); /* column 0 always has a row */
+    const float scale = a.scale[adapter];
+    const float *lp = a.low + ((size_t)s * a.n + any) * a.rank16 + 8 * k;
+    float *yp = a.Y[s] + (size_t)any * a.y_stride[s];
+    /* y is requested with the weights: four neighbouring rows of B are four neighbours in y */
+    const bool quads = a.y_stride[s] % 4 == 0 && ((uintptr_t)a.Y[s] & 15) == 0;
+    float4 y[LU_EACH];
+#pragma unroll
+    for (int e = 0; e < LU_EACH; e++) {
+        const int o = o0 + 16 * e + 4 * k;
+        y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (quads && o + 3 < rows && live) y[e] = *(const float4 *)(yp + o);
+    }
     float4v acc[LU_EACH];
 #pragma unroll
     for (int e = 0; e < LU_EACH; e++) acc[e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int q = 0; q < t.rank; q += 32) {
-        const int at = q + 8 * k; /* this lane's ranks */
-        float4 y0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), y1 = y0;
-        if (at < a.rank16) y0 = *(const float4 *)(lp + q), y1 = *(const float4 *)(lp + q + 4);
-        const float y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
-        float w[LU_EACH][8];
+    constexpr int U = 2; /* steps of 32 ranks requested at once */
+    for (int q = 0; q < own; q += 32 * U) {
+        float4 x[U][2];
+        float w[U][LU_EACH][8];
+        W8<WT> v[U][LU_EACH];
 #pragma unroll
-        for (int e = 0; e < LU_EACH; e++) {
-            const int o = o0 + 16 * e + c < rows ? o0 + 16 * e + c : rows - 1;
-            const size_t row = ((size_t)t.adapter * rows + o) * a.rank;
-            if constexpr (VEC) {
-                W8<WT> v;
-                v.load((const char *)a.B[s] + (row + (at < a.rank ? at : 0)) * SIZE);
+        for (int u = 0; u < U; u++) {
+            const int at = q + 32 * u + 8 * k; /* this lane's ranks */
+            x[u][0] = x[u][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (at < a.rank16) x[u][0] = *(const float4 *)(lp + q + 32 * u), x[u][1] = *(const float4 *)(lp + q + 32 * u + 4);
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[e][i] = at + i < t.rank ? v.at(i) : 0.0f;
-            } else {
+            for (int e = 0; e < LU_EACH; e++) {
+                const int o = o0 + 16 * e + c < rows ? o0 + 16 * e + c : rows - 1;
+                const size_t first = ((size_t)adapter * rows + o) * a.rank;
+                if constexpr (VEC) {
+                    v[u][e].load((const char *)a.B[s] + (first + (at < a.rank ? at : 0)) * SIZE);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float v = one_weight<WT>(a.B[s], row + (at + i < a.rank ? at + i : 0));
-                    w[e][i] = at + i < t.rank ? v : 0.0f;
+                    for (int i = 0; i < 8; i++) w[u][e][i] = one_weight<WT>(a.B[s], first + (at + i < a.rank ? at + i : 0));
                 }
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int u = 0; u < U; u++) {
+            if (q + 32 * u >= own) break; /* uniform */
+            const int at = q + 32 * u + 8 * k;
+            const float z[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
 #pragma unroll
-            for (int e = 0; e < LU_EACH; e++) acc[e] = mfma4(w[e][i], y[i], acc[e]);
-    }
-    if (!t.live) return;
-    float *yp = a.Y[s] + (size_t)t.row * a.y_stride[s];
+            for (int i = 0; i < 8; i++)
 #pragma unroll
-    for (int e = 0; e < LU_EACH; e++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int o = o0 + 16 * e + 4 * k + i;
-            if (o < rows) yp[o] = __builtin_fmaf(acc[e][i], scale, yp[o]);
+                for (int e = 0; e < LU_EACH; e++) {
+                    const float b = VEC ? v[u][e].at(i) : w[u][e][i]; /* behind the adapter's rank anything: not used */
+                    acc[e] = mfma4(at + i < own ? b : 0.0f, z[i], acc[e]);
+                }
         }
+    }
+    if (!live) return;
+#pragma unroll
+    for (int e = 0; e < LU_EACH; e++) {
+        const int o = o0 + 16 * e + 4 * k;
+        if (quads && o + 3 < rows) {
+            *(float4 *)(yp + o) = make_float4(__builtin_fmaf(acc[e][0], scale, y[e].x), __builtin_fmaf(acc[e][1], scale, y[e].y),
+                                              __builtin_fmaf(acc[e][2], scale, y[e].z), __builtin_fmaf(acc[e][3], scale, y[e].w));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (o + i < rows) yp[o + i] = __builtin_fmaf(acc[e][i], scale, yp[o + i]);
+        }
+    }
 }
 
 template <int WT>
 int launch(nmx_ctx *ctx, const Lora &a) {
-    lora_down_k<WT><<<dim3((unsigned)a.n, (unsigned)(a.count * a.rank16 / 16)), 64 * LD_WAVES, 0, ctx->stream>>>(a);
+    /* an adapter has at most one tile that is not full */
+    const int most = a.n / 16 + (a.adapters < a.n ? a.adapters : a.n), tiles = most < a.n ? most : a.n;
+    lora_down_k<WT><<<dim3((unsigned)tiles, (unsigned)(a.count * a.rank16 / 16)), 64 * LD_WAVES, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "lora_down");
-    const dim3 grid((unsigned)a.n, (unsigned)a.first[a.count]);
+    const dim3 grid((unsigned)tiles, (unsigned)a.first[a.count]);
     if (a.rank % 8 == 0) lora_up_k<WT, true><<<grid, 64 * LU_WAVES, 0, ctx->stream>>>(a);
     else lora_up_k<WT, false><<<grid, 64 * LU_WAVES, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "lora_up");
@@ -226,7 +271,7 @@ extern "C" {
 
 size_t nmx_lora_work_bytes(int n, int count, int rank) {
     if (n < 1 || n > NMX_CHUNK_ROWS || count < 1 || count > NMX_MAX_SEGS || rank < 1 || rank > 256) return 0;
-    return (size_t)count * n * ((rank + 15) / 16 * 16) * 4;
+    return (size_t)n * sizeof(Tile) + (size_t)count * n * ((rank + 15) / 16 * 16) * 4;
 }
 
 int nmx_lora(nmx_ctx *ctx, const nmx_lora_args *p, void *work) {
@@ -270,7 +315,8 @@ int nmx_lora(nmx_ctx *ctx, const nmx_lora_args *p, void *work) {
     }
     if (a.first[p->count] > 65535) return nmx_fail(ctx, "nmx_lora: too many rows in all");
     a.n = p->n, a.cols = p->cols, a.x_stride = p->x_stride, a.count = p->count, a.x = p->x, a.adapters = p->adapters;
-    a.rank = p->rank, a.adapter = p->adapter, a.ranks = p->ranks, a.scale = p->scale, a.low = (float *)work;
+    a.rank = p->rank, a.adapter = p->adapter, a.ranks = p->ranks, a.scale = p->scale;
+    a.tiles = (Tile *)work, a.low = (float *)((char *)work + N * sizeof(Tile));
     a.rank16 = (p->rank + 15) / 16 * 16;
     const nmx_on_device on(ctx);
     return p->w_dtype == W_F32 ? launch<W_F32>(ctx, a) : p->w_dtype == W_F16 ? launch<W_F16>(ctx, a) : launch<W_BF16>(ctx, a);

@@ -118,20 +118,14 @@ __device__ __forceinline__ float4v mfma4(float a, float b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-/* Workgroup: a row, blockIdx.y 16 ranks of a matrix. */
+/* Ranks r0 + 4 k .. + 3 of A x for the tile's row c in lane (k, c) of the first wave, zeros where the adapter has no such
+ * rank, whatever A holds there; by the whole workgroup. */
 template <int WT>
-__global__ __launch_bounds__(64 * LD_WAVES) void lora_down_k(Lora a) {
-    __shared__ float4 sum_s[LD_WAVES][64];
-    __shared__ Tile tile;
+__device__ __forceinline__ float4 down_block(const Lora &a, const Tile &tile, int s, int r0, float4 (*sum_s)[64]) {
     constexpr int SIZE = WT == W_F32 ? 4 : 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, k = lane >> 4;
-    find_tile(a, blockIdx.x, &tile);
-    if (blockIdx.y == 0 && threadIdx.x < 18) ((int *)(a.tiles + blockIdx.x))[threadIdx.x] = ((int *)&tile)[threadIdx.x];
-    const int adapter = tile.adapter, own = tile.rank, row = tile.row[c];
-    if (adapter < 0) return; /* uniform over the workgroup */
-    const int blocks = a.rank16 / 16, s = blockIdx.y / blocks, r0 = blockIdx.y % blocks * 16;
-    const int r = r0 + c < a.rank ? r0 + c : a.rank - 1;
-    const char *wp = (const char *)a.A[s] + (((size_t)adapter * a.rank + r) * a.cols + 8 * k) * SIZE;
+    const int row = tile.row[c], r = r0 + c < a.rank ? r0 + c : a.rank - 1;
+    const char *wp = (const char *)a.A[s] + (((size_t)tile.adapter * a.rank + r) * a.cols + 8 * k) * SIZE;
     const float *xp = a.x + (size_t)(row < 0 ? tile.row[0] : row) * a.x_stride + 8 * k;
     float4v acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
     constexpr int U = 4; /* steps of 32 columns requested at once */
@@ -155,111 +149,173 @@ __global__ __launch_bounds__(64 * LD_WAVES) void lora_down_k(Lora a) {
     const float4v mine = acc[0] + acc[1];
     sum_s[wave][lane] = make_float4(mine[0], mine[1], mine[2], mine[3]);
     __syncthreads();
-    if (wave) return;
     float4 v = sum_s[0][lane];
+    if (wave) return v;
 #pragma unroll
     for (int w = 1; w < LD_WAVES; w++) {
         const float4 y = sum_s[w][lane];
         v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
     }
-    if (row < 0) return;
-    /* ranks 4 k .. 4 k + 3 of row c; those that the adapter lacks are zeros, whatever A holds there */
-    const int q = r0 + 4 * k;
+    const int q = r0 + 4 * k, own = tile.rank;
     if (q >= own) v.x = 0.0f;
     if (q + 1 >= own) v.y = 0.0f;
     if (q + 2 >= own) v.z = 0.0f;
     if (q + 3 >= own) v.w = 0.0f;
-    *(float4 *)(a.low + ((size_t)s * a.n + row) * a.rank16 + q) = v;
+    return v;
+}
+
+/* Workgroup: a tile, blockIdx.y 16 ranks of a matrix. */
+template <int WT>
+__global__ __launch_bounds__(64 * LD_WAVES) void lora_down_k(Lora a) {
+    __shared__ float4 sum_s[LD_WAVES][64];
+    __shared__ Tile tile;
+    find_tile(a, blockIdx.x, &tile);
+    if (blockIdx.y == 0 && threadIdx.x < 18) ((int *)(a.tiles + blockIdx.x))[threadIdx.x] = ((int *)&tile)[threadIdx.x];
+    if (tile.adapter < 0) return; /* uniform over the workgroup */
+    const int blocks = a.rank16 / 16, s = blockIdx.y / blocks, r0 = blockIdx.y % blocks * 16, row = tile.row[threadIdx.x & 15];
+    const float4 v = down_block<WT>(a, tile, s, r0, sum_s);
+    if (threadIdx.x < 64 && row >= 0) *(float4 *)(a.low + ((size_t)s * a.n + row) * a.rank16 + r0 + 4 * (threadIdx.x >> 4)) = v;
+}
+
+/* 64 output rows of a wave: y, requested with the weights, and the products' accumulators. Four neighbouring rows of B are
+ * four neighbours in y. */
+template <int WT, bool VEC>
+struct Up {
+    static constexpr int SIZE = WT == W_F32 ? 4 : 2;
+    const Lora &a;
+    int s, o0, rows, adapter, own, c, k;
+    bool live, quads;
+    float *yp;
+    float4 y[LU_EACH];
+    float4v acc[LU_EACH];
+    W8<WT> v[LU_EACH];
+    float w[LU_EACH][8];
+    __device__ __forceinline__ Up(const Lora &a, int s, int o0, int adapter, int own, int row, int lane)
+        : a(a), s(s), o0(o0), rows(a.rows[s]), adapter(adapter), own(own), c(lane & 15), k(lane >> 4), live(row >= 0),
+          quads(a.y_stride[s] % 4 == 0 && ((uintptr_t)a.Y[s] & 15) == 0), yp(a.Y[s] + (size_t)(row < 0 ? 0 : row) * a.y_stride[s]) {
+#pragma unroll
+        for (int e = 0; e < LU_EACH; e++) {
+            const int o = o0 + 16 * e + 4 * k;
+            y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), acc[e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+            if (quads && o + 3 < rows && live) y[e] = *(const float4 *)(yp + o);
+        }
+    }
+    __device__ __forceinline__ void request(int q) { /* ranks q + 8 k .. + 7 */
+        const int at = q + 8 * k;
+#pragma unroll
+        for (int e = 0; e < LU_EACH; e++) {
+            const int o = o0 + 16 * e + c < rows ? o0 + 16 * e + c : rows - 1;
+            const size_t first = ((size_t)adapter * rows + o) * a.rank;
+            if constexpr (VEC) {
+                v[e].load((const char *)a.B[s] + (first + (at < a.rank ? at : 0)) * SIZE);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[e][i] = one_weight<WT>(a.B[s], first + (at + i < a.rank ? at + i : 0));
+            }
+        }
+    }
+    __device__ __forceinline__ void add(int q, const float4 (&x)[2]) {
+        const int at = q + 8 * k;
+        const float z[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int e = 0; e < LU_EACH; e++) {
+                const float b = VEC ? v[e].at(i) : w[e][i]; /* behind the adapter's rank anything: not used */
+                acc[e] = mfma4(at + i < own ? b : 0.0f, z[i], acc[e]);
+            }
+    }
+    __device__ __forceinline__ void store(float scale) {
+        if (!live) return;
+#pragma unroll
+        for (int e = 0; e < LU_EACH; e++) {
+            const int o = o0 + 16 * e + 4 * k;
+            if (quads && o + 3 < rows) {
+                *(float4 *)(yp + o) = make_float4(__builtin_fmaf(acc[e][0], scale, y[e].x), __builtin_fmaf(acc[e][1], scale, y[e].y),
+                                                  __builtin_fmaf(acc[e][2], scale, y[e].z), __builtin_fmaf(acc[e][3], scale, y[e].w));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (o + i < rows) yp[o + i] = __builtin_fmaf(acc[e][i], scale, yp[o + i]);
+            }
+        }
+    }
+};
+__device__ __forceinline__ int seg_of(const Lora &a, int y) {
+    int s = 0;
+    while (s + 1 < a.count && y >= a.first[s + 1]) s++;
+    return s;
 }
 
 /* Workgroup: a tile, blockIdx.y a run of output rows of a matrix. VEC: rows of B are 16-byte aligned. */
 template <int WT, bool VEC>
 __global__ __launch_bounds__(64 * LU_WAVES) void lora_up_k(Lora a) {
-    constexpr int SIZE = WT == W_F32 ? 4 : 2;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), c = lane & 15, k = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const Tile *tile = a.tiles + blockIdx.x;
-    const int adapter = __builtin_amdgcn_readfirstlane(tile->adapter), own = __builtin_amdgcn_readfirstlane(tile->rank), row = tile->row[c];
-    if (adapter < 0) return;
-    int s = 0;
-    while (s + 1 < a.count && (int)blockIdx.y >= a.first[s + 1]) s++;
-    const int rows = a.rows[s], o0 = (((int)blockIdx.y - a.first[s]) * LU_WAVES + wave) * 16 * LU_EACH;
-    if (o0 >= rows) return;
-    const bool live = row >= 0;
-    const int any = live ? row : __builtin_amdgcn_readfirstlane(row); /* column 0 always has a row */
+    const int adapter = __builtin_amdgcn_readfirstlane(tile->adapter), own = __builtin_amdgcn_readfirstlane(tile->rank);
+    const int row = tile->row[lane & 15];
+    if (adapter < 0 || own == 0) return; /* no ranks: the rows are left alone */
+    const int s = seg_of(a, blockIdx.y), o0 = (((int)blockIdx.y - a.first[s]) * LU_WAVES + wave) * 16 * LU_EACH;
+    if (o0 >= a.rows[s]) return;
     const float scale = a.scale[adapter];
-    const float *lp = a.low + ((size_t)s * a.n + any) * a.rank16 + 8 * k;
-    float *yp = a.Y[s] + (size_t)any * a.y_stride[s];
-    /* y is requested with the weights: four neighbouring rows of B are four neighbours in y */
-    const bool quads = a.y_stride[s] % 4 == 0 && ((uintptr_t)a.Y[s] & 15) == 0;
-    float4 y[LU_EACH];
-#pragma unroll
-    for (int e = 0; e < LU_EACH; e++) {
-        const int o = o0 + 16 * e + 4 * k;
-        y[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (quads && o + 3 < rows && live) y[e] = *(const float4 *)(yp + o);
+    Up<WT, VEC> up(a, s, o0, adapter, own, row, lane);
+    /* a column without a row takes the first one's: it is not stored */
+    const float *lp = a.low + ((size_t)s * a.n + (row < 0 ? __builtin_amdgcn_readfirstlane(row) : row)) * a.rank16 + 8 * up.k;
+    for (int q = 0; q < own; q += 32) {
+        float4 x[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+        up.request(q);
+        if (q + 8 * up.k < a.rank16) x[0] = *(const float4 *)(lp + q), x[1] = *(const float4 *)(lp + q + 4);
+        up.add(q, x);
     }
-    float4v acc[LU_EACH];
-#pragma unroll
-    for (int e = 0; e < LU_EACH; e++) acc[e] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int U = 2; /* steps of 32 ranks requested at once */
-    for (int q = 0; q < own; q += 32 * U) {
-        float4 x[U][2];
-        float w[U][LU_EACH][8];
-        W8<WT> v[U][LU_EACH];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int at = q + 32 * u + 8 * k; /* this lane's ranks */
-            x[u][0] = x[u][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (at < a.rank16) x[u][0] = *(const float4 *)(lp + q + 32 * u), x[u][1] = *(const float4 *)(lp + q + 32 * u + 4);
-#pragma unroll
-            for (int e = 0; e < LU_EACH; e++) {
-                const int o = o0 + 16 * e + c < rows ? o0 + 16 * e + c : rows - 1;
-                const size_t first = ((size_t)adapter * rows + o) * a.rank;
-                if constexpr (VEC) {
-                    v[u][e].load((const char *)a.B[s] + (first + (at < a.rank ? at : 0)) * SIZE);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) w[u][e][i] = one_weight<WT>(a.B[s], first + (at + i < a.rank ? at + i : 0));
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (q + 32 * u >= own) break; /* uniform */
-            const int at = q + 32 * u + 8 * k;
-            const float z[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int e = 0; e < LU_EACH; e++) {
-                    const float b = VEC ? v[u][e].at(i) : w[u][e][i]; /* behind the adapter's rank anything: not used */
-                    acc[e] = mfma4(at + i < own ? b : 0.0f, z[i], acc[e]);
-                }
-        }
-    }
-    if (!live) return;
-#pragma unroll
-    for (int e = 0; e < LU_EACH; e++) {
-        const int o = o0 + 16 * e + 4 * k;
-        if (quads && o + 3 < rows) {
-            *(float4 *)(yp + o) = make_float4(__builtin_fmaf(acc[e][0], scale, y[e].x), __builtin_fmaf(acc[e][1], scale, y[e].y),
-                                              __builtin_fmaf(acc[e][2], scale, y[e].z), __builtin_fmaf(acc[e][3], scale, y[e].w));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (o + i < rows) yp[o + i] = __builtin_fmaf(acc[e][i], scale, yp[o + i]);
-        }
-    }
+    up.store(scale);
 }
+
+/* Both in one launch, where the A of a matrix is small: every workgroup makes A x of its tile again, while its rows of B and
+ * y are on their way. */
+template <int WT, bool VEC>
+__global__ __launch_bounds__(64 * LD_WAVES) void lora_one_k(Lora a) {
+    __shared__ float4 sum_s[LD_WAVES][64];
+    __shared__ Tile tile;
+    __shared__ __align__(16) float low_s[16 * 20];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    find_tile(a, blockIdx.x, &tile);
+    const int adapter = tile.adapter, own = tile.rank, row = tile.row[lane & 15];
+    if (adapter < 0 || own == 0) return; /* uniform over the workgroup */
+    const int s = seg_of(a, blockIdx.y), o0 = (((int)blockIdx.y - a.first[s]) * LD_WAVES + wave) * 16 * LU_EACH;
+    const float scale = a.scale[adapter];
+    Up<WT, VEC> up(a, s, o0 < a.rows[s] ? o0 : 0, adapter, own, o0 < a.rows[s] ? row : -1, lane); /* no rows left: nothing is stored */
+    up.request(0);
+    const float4 v = down_block<WT>(a, tile, s, 0, sum_s);
+    if (wave == 0) *(float4 *)(low_s + up.c * 20 + 4 * up.k) = v;
+    __syncthreads();
+    float4 x[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+    const float *lp = low_s + up.c * 20 + 8 * up.k;
+    if (up.k < 2) x[0] = *(const float4 *)lp, x[1] = *(const float4 *)(lp + 4);
+    up.add(0, x);
+    up.store(scale);
+}
+
+/* One launch where every workgroup may make A x again: 16 ranks (more are one block of them after the other) of up to
+ * LO_BYTES. 8 requests, ranks of 16: 1024 binary16 columns 7.7 us against 9.7 in two launches, 3584 columns 11.6 against 13.7;
+ * 64 requests on 40 adapters of 25 ranks, bfloat16, 22.6 against 18.9. */
+constexpr size_t LO_BYTES = 128 * 1024;
+bool in_one(const Lora &a, int size) { return a.rank16 == 16 && (size_t)a.rank16 * a.cols * size <= LO_BYTES; }
 
 template <int WT>
 int launch(nmx_ctx *ctx, const Lora &a) {
     /* an adapter has at most one tile that is not full */
     const int most = a.n / 16 + (a.adapters < a.n ? a.adapters : a.n), tiles = most < a.n ? most : a.n;
+    const dim3 grid((unsigned)tiles, (unsigned)a.first[a.count]);
+    const bool vec = a.rank % 8 == 0;
+    if (in_one(a, WT == W_F32 ? 4 : 2)) {
+        if (vec) lora_one_k<WT, true><<<grid, 64 * LD_WAVES, 0, ctx->stream>>>(a);
+        else lora_one_k<WT, false><<<grid, 64 * LD_WAVES, 0, ctx->stream>>>(a);
+        NMX_LAUNCHED(ctx, "lora_one");
+        return 0;
+    }
     lora_down_k<WT><<<dim3((unsigned)tiles, (unsigned)(a.count * a.rank16 / 16)), 64 * LD_WAVES, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "lora_down");
-    const dim3 grid((unsigned)tiles, (unsigned)a.first[a.count]);
-    if (a.rank % 8 == 0) lora_up_k<WT, true><<<grid, 64 * LU_WAVES, 0, ctx->stream>>>(a);
+    if (vec) lora_up_k<WT, true><<<grid, 64 * LU_WAVES, 0, ctx->stream>>>(a);
     else lora_up_k<WT, false><<<grid, 64 * LU_WAVES, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "lora_up");
     return 0;
@@ -303,7 +359,6 @@ int nmx_lora(nmx_ctx *ctx, const nmx_lora_args *p, void *work) {
         in[ni++] = {p->B[s], mb * p->rows[s]};
         out[no++] = {p->Y[s], ((N - 1) * p->y_stride[s] + p->rows[s]) * 4};
         a.A[s] = p->A[s], a.B[s] = p->B[s], a.Y[s] = p->Y[s], a.rows[s] = p->rows[s], a.y_stride[s] = p->y_stride[s];
-        a.first[s + 1] = a.first[s] + (p->rows[s] + 16 * LU_EACH * LU_WAVES - 1) / (16 * LU_EACH * LU_WAVES);
     }
     for (int i = 0; i < no; i++) {
         for (int k = 0; k < ni; k++)
@@ -313,11 +368,13 @@ int nmx_lora(nmx_ctx *ctx, const nmx_lora_args *p, void *work) {
             if (nmx_overlap(out[i].p, out[i].bytes, out[k].p, out[k].bytes))
                 return nmx_fail(ctx, "nmx_lora: outputs and work overlap");
     }
+    a.rank16 = (p->rank + 15) / 16 * 16, a.cols = p->cols;
+    const int run = 16 * LU_EACH * (in_one(a, (int)ws) ? LD_WAVES : LU_WAVES); /* output rows of a workgroup */
+    for (int s = 0; s < p->count; s++) a.first[s + 1] = a.first[s] + (p->rows[s] + run - 1) / run;
     if (a.first[p->count] > 65535) return nmx_fail(ctx, "nmx_lora: too many rows in all");
-    a.n = p->n, a.cols = p->cols, a.x_stride = p->x_stride, a.count = p->count, a.x = p->x, a.adapters = p->adapters;
+    a.n = p->n, a.x_stride = p->x_stride, a.count = p->count, a.x = p->x, a.adapters = p->adapters;
     a.rank = p->rank, a.adapter = p->adapter, a.ranks = p->ranks, a.scale = p->scale;
     a.tiles = (Tile *)work, a.low = (float *)((char *)work + N * sizeof(Tile));
-    a.rank16 = (p->rank + 15) / 16 * 16;
     const nmx_on_device on(ctx);
     return p->w_dtype == W_F32 ? launch<W_F32>(ctx, a) : p->w_dtype == W_F16 ? launch<W_F16>(ctx, a) : launch<W_BF16>(ctx, a);
 }

@@ -2,12 +2,12 @@
  * end, and take pages for their new rows.
  *
  * pages_plan_k, one workgroup, does everything but move rows, so that no phase waits for another
- * workgroup: it counts the holders of every page as they will be (additions to refs, exact in any order),
- * decides which partly filled pages have to be copied before their sequence writes into them, takes the lowest
- * free pages by running sums over the page counts, and writes tables and lengths; a step that does not fit is
- * taken back by the opposite additions. A fork's entries go through the workspace, so sequences may
- * exchange places. pages_copy_k and, with pack, pages_move_k then copy what the plan lists, in all
- * caches at once. */
+ * workgroup: it counts the holders of every page as they will be (additions, exact in any order), decides which partly
+ * filled pages have to be copied before their sequence writes into them, takes the lowest free pages by running
+ * sums over the counts, and writes tables and lengths. Up to PP_LDS pages the counts stand in LDS meanwhile, and go back
+ * only if the step fits; of more pages they are changed where they are and a step that does not fit is taken back by the
+ * opposite additions. A fork's entries go through the workspace, so sequences may exchange places. pages_copy_k and, with
+ * pack, pages_move_k then copy what the plan lists, in all caches at once. */
 #include "nmx_internal.h"
 #include "nmx_batch.h"
 #include "nmx_lanes.h"
@@ -15,7 +15,8 @@
 namespace {
 
 constexpr int PP = 1024;          /* threads of the plan */
-constexpr int PP_EACH = 16;       /* pages of a thread in a turn of a search */
+constexpr int PP_LDS = 16384;     /* pages whose counts, and as many page numbers, have room in LDS */
+constexpr int PP_SEQS = 4;        /* sequences of a wave whose entries are requested together */
 constexpr int PC = 256;           /* threads of a copy */
 constexpr int PC_CHUNK = PC * 64; /* bytes of a workgroup's item: four 16-byte units a thread */
 
@@ -34,9 +35,25 @@ struct PagesDev {
     int32_t *rows;                        /* [seqs][max_pages]: the entries of sequences that fork */
 };
 
-__device__ __forceinline__ int read_refs(const int32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void add_refs(int32_t *refs, int npages, int page, int v) {
-    if ((uint32_t)page < (uint32_t)npages) (void)__hip_atomic_fetch_add(refs + page, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+/* The counts, in LDS or in memory. */
+template <bool LDS>
+struct Refs {
+    int32_t *p;
+    int npages;
+    __device__ __forceinline__ int get(int page) const {
+        return LDS ? p[page] : __hip_atomic_load(p + page, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ __forceinline__ void add(int page, int v) const {
+        if ((uint32_t)page >= (uint32_t)npages) return;
+        if (LDS) atomicAdd(p + page, v);
+        else (void)__hip_atomic_fetch_add(p + page, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+};
+/* What was written so far is seen by the whole workgroup. */
+template <bool LDS>
+__device__ __forceinline__ void settle() {
+    if (!LDS) __threadfence();
+    __syncthreads();
 }
 
 /* Running sum over the workgroup, the total in *all (sum_s: PP / 64 words; two barriers). */
@@ -55,20 +72,21 @@ __device__ __forceinline__ uint32_t scan_all(uint32_t v, uint32_t *sum_s, uint32
     return before + inc - v;
 }
 
-/* Calls hit(page, rank) for the pages in [0, npages) of which want(refs) is true, in order, while the rank is
+/* Calls hit(page, rank) for the pages from `begin` on whose count want() wants, in order, while the rank is
  * below `most`; returns how many there are (all of them where it is less than most). */
-template <typename Want, typename Hit>
-__device__ uint32_t search(const int32_t *refs, int begin, int npages, uint32_t most, uint32_t *sum_s, Want want, Hit hit) {
+template <bool LDS, typename Want, typename Hit>
+__device__ uint32_t search(const Refs<LDS> &refs, int begin, int end, uint32_t most, uint32_t *sum_s, Want want, Hit hit) {
+    constexpr int EACH = LDS ? 4 : 16; /* pages of a thread in a turn */
     uint32_t found = 0;
-    for (int base = begin; base < npages && found < most; base += PP * PP_EACH) {
-        int v[PP_EACH];
-        const int at = base + (int)threadIdx.x * PP_EACH;
+    for (int base = begin; base < end && found < most; base += PP * EACH) {
+        int v[EACH];
+        const int at = base + (int)threadIdx.x * EACH;
 #pragma unroll
-        for (int i = 0; i < PP_EACH; i++) v[i] = read_refs(refs + (at + i < npages ? at + i : npages - 1));
+        for (int i = 0; i < EACH; i++) v[i] = refs.get(at + i < end ? at + i : end - 1);
         uint32_t mask = 0;
 #pragma unroll
-        for (int i = 0; i < PP_EACH; i++)
-            if (at + i < npages && want(v[i])) mask |= 1u << i;
+        for (int i = 0; i < EACH; i++)
+            if (at + i < end && want(v[i])) mask |= 1u << i;
         uint32_t all, rank = found + scan_all(__popc(mask), sum_s, &all);
         for (; mask; mask &= mask - 1, rank++)
             if (rank < most) hit(at + __ffs(mask) - 1, rank);
@@ -77,21 +95,33 @@ __device__ uint32_t search(const int32_t *refs, int begin, int npages, uint32_t 
     return found;
 }
 
-__global__ __launch_bounds__(PP) void pages_plan_k(PagesDev a) {
+template <bool LDS>
+__global__ __launch_bounds__(PP) void pages_plan_k(const int32_t *from_, const int32_t *keep_, const int32_t *add_,
+                                                   const int32_t *len_, int seqs, int npages, PagesDev a) {
     __shared__ int src_s[NMX_BATCH_MAX], kept_s[NMX_BATCH_MAX], old_s[NMX_BATCH_MAX], all_s[NMX_BATCH_MAX],
-        last_s[NMX_BATCH_MAX], copy_s[NMX_BATCH_MAX];
+        last_s[NMX_BATCH_MAX], copy_s[NMX_BATCH_MAX], len_s[NMX_BATCH_MAX];
     __shared__ uint32_t base_s[NMX_BATCH_MAX], sum_s[PP / 64];
     __shared__ int wide_s, some_s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.pg.seqs, npages = a.pg.npages, mp = a.pg.max_pages;
+    extern __shared__ int32_t pages_s[]; /* LDS: the counts, then page numbers */
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = seqs, mp = a.pg.max_pages;
     const int page = 1 << a.pg.shift, shift = a.pg.shift;
+    const Refs<LDS> refs{LDS ? pages_s : a.refs, npages};
+    int32_t *fresh = LDS ? pages_s + npages : a.fresh;
     auto pages_of = [&](long long r) { return (int)((r + page - 1) >> shift); };
+    int f = -1, keep = 0, add = 0, old = 0;
+    if (tid < S) {
+        f = from_[tid], keep = keep_[tid], add = add_[tid], old = len_[tid];
+        const long long room = (long long)mp << shift;
+        old = old < 0 ? 0 : old > room ? (int)room : old;
+        len_s[tid] = old;
+    }
+    if (LDS)
+        for (int p = tid; p < npages; p += PP) pages_s[p] = a.refs[p];
     if (tid == 0) wide_s = S, some_s = 0;
     __syncthreads();
     int total = 0, part = 0, last = -1;
     if (tid < S) {
-        const int f = a.from[tid], old = seq_len(a.pg, tid);
-        int keep = a.keep[tid], add = a.add[tid], src = f >= 0 && f < S ? f : -1;
-        const int most = src < 0 ? 0 : seq_len(a.pg, src);
+        const int src = f >= 0 && f < S ? f : -1, most = src < 0 ? 0 : len_s[src];
         keep = keep < 0 ? 0 : keep < most ? keep : most, add = add < 0 ? 0 : add;
         const long long len = (long long)keep + add;
         const bool wide = len > (long long)mp << shift;
@@ -110,31 +140,47 @@ __global__ __launch_bounds__(PP) void pages_plan_k(PagesDev a) {
         if (tid == 0) a.lists->copies = 0, a.lists->moves = 0;
         return;
     }
-    /* who holds what after the step: a wave for each sequence whose entries change hands. sign -1 takes it back */
+    /* who holds what after the step: entries given up, entries that a fork keeps. sign -1 takes it back */
     auto recount = [&](int sign) {
-        for (int s = wave; s < S; s += PP / 64) {
-            const int src = src_s[s], kept = kept_s[s], old = old_s[s];
-            const int32_t *mine = a.pg.table + (size_t)s * mp;
-            for (int e = (src == s ? kept : 0) + lane; e < old; e += 64) add_refs(a.refs, npages, mine[e], -sign);
-            if (src == s || src < 0) continue;
-            const int32_t *theirs = a.pg.table + (size_t)src * mp;
-            for (int e = lane; e < kept; e += 64) {
-                const int p = theirs[e];
-                add_refs(a.refs, npages, p, sign);
-                a.rows[(size_t)s * mp + e] = p;
+        for (int s0 = wave; s0 < S; s0 += PP_SEQS * (PP / 64)) {
+            int begin[PP_SEQS], end[PP_SEQS], kept[PP_SEQS], src[PP_SEQS], longest = 0;
+#pragma unroll
+            for (int u = 0; u < PP_SEQS; u++) {
+                const int s = s0 + u * (PP / 64);
+                begin[u] = end[u] = kept[u] = src[u] = 0;
+                if (s >= S) continue;
+                const bool own = src_s[s] == s;
+                begin[u] = own ? kept_s[s] : 0, end[u] = old_s[s], src[u] = src_s[s];
+                kept[u] = own || src[u] < 0 ? 0 : kept_s[s];
+                const int n = end[u] - begin[u] > kept[u] ? end[u] - begin[u] : kept[u];
+                longest = n > longest ? n : longest;
+            }
+            for (int e0 = 0; e0 < longest; e0 += 64) {
+                int mine[PP_SEQS], theirs[PP_SEQS];
+#pragma unroll
+                for (int u = 0; u < PP_SEQS; u++) {
+                    const int s = s0 + u * (PP / 64), e = begin[u] + e0 + lane;
+                    mine[u] = theirs[u] = -1;
+                    if (e < end[u]) mine[u] = a.pg.table[(size_t)s * mp + e];
+                    if (e0 + lane < kept[u]) theirs[u] = a.pg.table[(size_t)src[u] * mp + e0 + lane];
+                }
+#pragma unroll
+                for (int u = 0; u < PP_SEQS; u++) {
+                    refs.add(mine[u], -sign), refs.add(theirs[u], sign);
+                    if (e0 + lane < kept[u]) a.rows[(size_t)(s0 + u * (PP / 64)) * mp + e0 + lane] = theirs[u];
+                }
             }
         }
     };
     if (some_s) { /* uniform */
         recount(1);
-        __threadfence();
-        __syncthreads();
+        settle<LDS>();
     }
     /* a page that its sequence would add rows to is copied where another one holds it; where all who hold it
      * would, the first of them keeps it */
     bool copy = false;
     if (tid < S && last >= 0) {
-        const int held = read_refs(a.refs + last);
+        const int held = refs.get(last);
         if (held > 1) {
             int same = 0, before = 0;
             for (int s = 0; s < S; s++) same += last_s[s] == last, before += s < tid && last_s[s] == last;
@@ -147,20 +193,19 @@ __global__ __launch_bounds__(PP) void pages_plan_k(PagesDev a) {
     const uint32_t base = scan_all(need, sum_s, &needed), nth = scan_all(copy, sum_s, &copies);
     if (tid < S) base_s[tid] = base;
     if (needed) {
-        const uint32_t found = search(a.refs, 0, npages, needed, sum_s, [](int r) { return r == 0; },
-                                      [&](int p, uint32_t i) { a.fresh[i] = p; });
+        const uint32_t found = search<LDS>(refs, 0, npages, needed, sum_s, [](int r) { return r == 0; },
+                                           [&](int p, uint32_t i) { fresh[i] = p; });
         if (found < needed) {
-            if (some_s) recount(-1);
+            if (!LDS && some_s) recount(-1);
             if (tid < 4) a.out[tid] = tid ? 0 : (int)(needed - found);
             if (tid == 0) a.lists->copies = 0, a.lists->moves = 0;
             return;
         }
     }
-    __threadfence();
-    __syncthreads();
+    settle<LDS>();
     if (copy) {
-        a.lists->copy[nth] = make_int4(last, a.fresh[base], part, 0);
-        add_refs(a.refs, npages, last, -1);
+        a.lists->copy[nth] = make_int4(last, fresh[base], part, 0);
+        refs.add(last, -1);
     }
     if (tid < S) a.pg.len[tid] = total;
     /* tables: what a fork keeps, the fresh pages, -1 where there were more */
@@ -170,40 +215,56 @@ __global__ __launch_bounds__(PP) void pages_plan_k(PagesDev a) {
         if (src != s && src >= 0)
             for (int e = lane; e < own; e += 64) t[e] = a.rows[(size_t)s * mp + e];
         for (int e = own + lane; e < all; e += 64) {
-            const int p = a.fresh[base_s[s] + e - own];
-            t[e] = p, a.refs[p] = 1;
+            const int p = fresh[base_s[s] + e - own];
+            t[e] = p, refs.p[p] = 1;
         }
         for (int e = all + lane; e < old_s[s]; e += 64) t[e] = -1;
     }
     if (tid < 4) a.out[tid] = tid == 1 ? (int)needed : 0;
     if (tid == 0) a.lists->copies = (int)copies, a.lists->moves = 0;
-    if (!a.pack) return;
-    /* the used pages from their number on move to the free ones below it */
-    __threadfence();
-    __syncthreads();
-    const uint32_t used = search(a.refs, 0, npages, ~0u, sum_s, [](int r) { return r != 0; }, [](int, uint32_t) {});
-    const uint32_t moves = search(a.refs, (int)used, npages, ~0u, sum_s, [](int r) { return r != 0; },
-                                  [&](int p, uint32_t i) { a.movers[i] = p; });
-    if (moves)
-        (void)search(a.refs, 0, (int)used, moves, sum_s, [](int r) { return r == 0; }, [&](int p, uint32_t i) { a.holes[i] = p; });
-    __threadfence();
-    __syncthreads();
-    for (uint32_t i = tid; i < moves; i += PP) {
-        const int p = a.movers[i], h = a.holes[i];
-        a.to[p] = h;
-        a.refs[h] = read_refs(a.refs + p), a.refs[p] = 0;
-    }
-    if (tid == 0) a.lists->moves = (int)moves;
-    if (tid == 2 || tid == 3) a.out[tid] = (int)(tid == 2 ? used : moves);
-    if (!moves) return;
-    __threadfence();
-    __syncthreads();
-    for (int s = wave; s < S; s += PP / 64) {
-        int32_t *t = a.pg.table + (size_t)s * mp;
-        for (int e = lane; e < all_s[s]; e += 64) {
-            const int p = t[e];
-            if ((uint32_t)p >= used && (uint32_t)p < (uint32_t)npages) t[e] = a.to[p];
+    if (a.pack) { /* the used pages from their number on move to the free ones below it */
+        settle<false>(); /* the tables too */
+        const uint32_t used = search<LDS>(refs, 0, npages, ~0u, sum_s, [](int r) { return r != 0; }, [](int, uint32_t) {});
+        const uint32_t moves = search<LDS>(refs, (int)used, npages, ~0u, sum_s, [](int r) { return r != 0; },
+                                           [&](int p, uint32_t i) { a.movers[i] = p; });
+        if (moves)
+            (void)search<LDS>(refs, 0, (int)used, moves, sum_s, [](int r) { return r == 0; }, [&](int p, uint32_t i) { a.holes[i] = p; });
+        int32_t *to = LDS ? fresh : a.to;
+        settle<false>();
+        for (uint32_t i = tid; i < moves; i += PP) {
+            const int p = a.movers[i], h = a.holes[i];
+            to[p] = h;
+            refs.p[h] = refs.get(p), refs.p[p] = 0;
         }
+        if (tid == 0) a.lists->moves = (int)moves;
+        if (tid == 2 || tid == 3) a.out[tid] = (int)(tid == 2 ? used : moves);
+        settle<LDS>();
+        if (moves) {
+            for (int s0 = wave; s0 < S; s0 += PP_SEQS * (PP / 64)) {
+                int longest = 0;
+#pragma unroll
+                for (int u = 0; u < PP_SEQS; u++) {
+                    const int s = s0 + u * (PP / 64);
+                    if (s < S && all_s[s] > longest) longest = all_s[s];
+                }
+                for (int e = lane; e < longest; e += 64) {
+                    int p[PP_SEQS];
+#pragma unroll
+                    for (int u = 0; u < PP_SEQS; u++) {
+                        const int s = s0 + u * (PP / 64);
+                        p[u] = s < S && e < all_s[s] ? a.pg.table[(size_t)s * mp + e] : -1;
+                    }
+#pragma unroll
+                    for (int u = 0; u < PP_SEQS; u++)
+                        if ((uint32_t)p[u] >= used && (uint32_t)p[u] < (uint32_t)npages)
+                            a.pg.table[(size_t)(s0 + u * (PP / 64)) * mp + e] = to[p[u]];
+                }
+            }
+        }
+    }
+    if (LDS) {
+        __syncthreads();
+        for (int p = tid; p < npages; p += PP) a.refs[p] = pages_s[p];
     }
 }
 
@@ -307,7 +368,13 @@ int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work) {
     a.fresh = (int32_t *)w, a.holes = (int32_t *)(w + nb), a.movers = (int32_t *)(w + 2 * nb), a.to = (int32_t *)(w + 3 * nb);
     a.rows = (int32_t *)(w + 4 * nb);
     const nmx_on_device on(ctx);
-    pages_plan_k<<<1, PP, 0, ctx->stream>>>(a);
+    if (np <= PP_LDS) {
+        static std::atomic<uint64_t> set0;
+        if (nmx_dyn_lds(ctx, (const void *)pages_plan_k<true>, (size_t)PP_LDS * 8, set0)) return -1;
+        pages_plan_k<true><<<1, PP, (size_t)np * 8, ctx->stream>>>(a.from, a.keep, a.add, a.pg.len, S, np, a);
+    } else {
+        pages_plan_k<false><<<1, PP, 0, ctx->stream>>>(a.from, a.keep, a.add, a.pg.len, S, np, a);
+    }
     NMX_LAUNCHED(ctx, "pages_plan");
     if (!p->caches) return 0;
     const int kv = p->pages.kv_dtype, page = p->pages.page;

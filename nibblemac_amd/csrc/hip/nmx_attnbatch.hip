@@ -791,7 +791,170 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
 
 /* ---- the join -------------------------------------------------------------------------------------- */
 constexpr int JB = 256;              /* threads */
+#ifndef JBW
+#define JBW 1024
+#endif
+constexpr int JB_WAVES = JBW; /* rows, heads and halves from which a wave takes one alone */
 constexpr int JB_PARTS = 2 * (AB_WGS + 2 * AB_PARTS);
+
+/* The parts of a row's head and half: those of the prefix, then the sequence's own. Of a unit of few rows: those of single
+ * waves, of workgroups whose share lies in it, of single waves. */
+template <int HDP>
+struct Parts {
+    int count[2], solo[2], whole[2];
+    const float *val[2]; /* of the half's first column */
+    const float4 *st[2];
+    uint32_t vstep[2], sstep[2];
+    bool any; /* the row belongs to a sequence */
+    __device__ __forceinline__ Parts(const BatchAttn &a, int t, int h, int half) {
+        constexpr int OD = HDP > 256 ? 256 : HDP;
+        const int hd = a.pg.hd, nkv = a.pg.nkv, rep = a.nh / nkv, g = h / rep;
+        const Shares sh = a.plan->sh;
+        const int s = seq_of_row(a.row0, a.pg.seqs, t);
+        any = false;
+        if (s < 0) return; /* uniform over the wave */
+        const SeqRows rows = seq_rows(a.row0, s, a.n);
+        if (t >= rows.r0 + rows.count) return;
+        any = true;
+        const Seg own = a.plan->seg[a.groups + s];
+        Seg pre = own;
+        pre.unit = 0;
+        if (own.group >= 0) pre = a.plan->seg[own.group];
+        auto over = [](unsigned long long c, unsigned long long n) {
+            return c >> 32 || n >> 32 ? (uint32_t)(c / n) : (uint32_t)c / (uint32_t)n;
+        };
+#pragma unroll 1
+        for (int k = 0; k < 2; k++) {
+            const Seg &x = k ? own : pre;
+            const int rr = (t - x.r0) * rep + h % rep;
+            int n = 0, so = 0, wh = 0;
+            const float *v = nullptr;
+            const float4 *f = nullptr;
+            uint32_t vs = 0, ss = 0;
+            if (x.unit && rr >= 0 && rr < x.m) {
+                const bool mx = x.m > AB_VR;
+                const int tr = mx ? tile_rows<HDP>() : AB_VR, width = mx ? OD : hd;
+                const uint32_t u = (mx ? rr / tr * halves<HDP>() + half : 0) * nkv + g;
+                const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit, per = mx ? sh.per_m : sh.per_w;
+                const uint32_t w0 = over(cu, per), w1 = over(cu + x.unit - 1, per);
+                n = so = (int)(w1 - w0) + 1;
+                if (!mx) {
+                    const uint32_t f0 = (w0 * per == cu ? w0 + AB_PARTS - 1 : w0 + AB_PARTS) / AB_PARTS, f1 = over(cu + x.unit, per) / AB_PARTS;
+                    if (f1 > f0) so = (int)(f0 * AB_PARTS - w0), wh = (int)(f1 - f0), n -= wh * (AB_PARTS - 1);
+                }
+                const size_t slot = (size_t)w0 + x.u0 + u;
+                v = (mx ? a.part_m : a.part_v) + (slot * tr + rr % tr) * width + (mx ? 0 : half * OD);
+                f = (mx ? a.stat_m : a.stat_v) + slot * tr + rr % tr;
+                vs = tr * width, ss = tr;
+            }
+            if (k) count[1] = n, solo[1] = so, whole[1] = wh, val[1] = v, st[1] = f, vstep[1] = vs, sstep[1] = ss;
+            else count[0] = n, solo[0] = so, whole[0] = wh, val[0] = v, st[0] = f, vstep[0] = vs, sstep[0] = ss;
+        }
+    }
+    __device__ __forceinline__ int all() const { return count[0] + count[1]; }
+    /* slots from the first one to part i */
+    __device__ __forceinline__ int step(int i) const {
+        const bool b = i >= count[0];
+        const int nth = b ? i - count[0] : i, inner = nth - (b ? solo[1] : solo[0]), w = b ? whole[1] : whole[0];
+        return inner <= 0 ? nth : nth + (inner < w ? inner : w) * (AB_PARTS - 1);
+    }
+    __device__ __forceinline__ const float *values(int i) const {
+        return i >= count[0] ? val[1] + (size_t)step(i) * vstep[1] : val[0] + (size_t)step(i) * vstep[0];
+    }
+    __device__ __forceinline__ float4 stat(int i) const { return i >= count[0] ? st[1][step(i) * sstep[1]] : st[0][step(i) * sstep[0]]; }
+};
+
+/* A wave for each row, head and half, where there are many of them: its parts' numbers stay in its lanes. */
+template <int HDP>
+__global__ __launch_bounds__(JB) void attn_batch_join_waves_k(BatchAttn a) {
+    constexpr int OD = HDP > 256 ? 256 : HDP, HV = halves<HDP>(), PT = (JB_PARTS + 63) / 64;
+    const int lane = lane_id(), item = __builtin_amdgcn_readfirstlane((int)blockIdx.x * (JB / 64) + wave_id());
+    if (item >= a.n * a.nh * HV) return;
+    const int hd = a.pg.hd, half = item % HV, h = item / HV % a.nh, t = item / HV / a.nh;
+    const int col = half * OD + 4 * lane, cols = hd - half * OD < OD ? hd - half * OD : OD;
+    const bool in = 4 * lane < cols;
+    const float *qp = a.q + ((size_t)t * a.nh + h) * 2 * hd + hd;
+    const float4 gate = *(const float4 *)(qp + (in ? col : 0));
+    const Parts<HDP> p(a, t, h, half);
+    if (!p.any) return; /* a row of no sequence is left as it is */
+    const int parts = p.all();
+    float top = -INFINITY, w[PT], sum[PT];
+    int ex[PT];
+#pragma unroll
+    for (int k = 0; k < PT; k++) {
+        w[k] = -INFINITY, sum[k] = 0.0f, ex[k] = 0;
+        if (64 * k >= parts) continue;
+        const int i = 64 * k + lane;
+        if (i < parts) {
+            const float4 y = p.stat(i);
+            w[k] = y.x, sum[k] = y.z, ex[k] = (int)y.y;
+        }
+        top = fmaxf(top, w[k]);
+    }
+    top = nmx_max_f32_wave(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float all = 0.0f;
+#pragma unroll
+    for (int k = 0; k < PT; k++) {
+        if (64 * k >= parts) continue;
+        const float f = __builtin_amdgcn_exp2f(w[k] - ref);
+        all += sum[k] * f;
+        w[k] = w[k] == -INFINITY ? 0.0f : ldexpf(f, ex[k] - 12);
+    }
+    all = sum_lanes(all);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int PB = 8;
+#pragma unroll
+    for (int k = 0; k < PT; k++) {
+        for (int i0 = 64 * k; i0 < parts && i0 < 64 * k + 64; i0 += PB) {
+            float4 v[PB];
+            float f[PB];
+#pragma unroll
+            for (int b = 0; b < PB; b++) {
+                const int i = i0 + b < parts ? i0 + b : i0;
+                f[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w[k]), i - 64 * k));
+                if (i0 + b >= parts) f[b] = 0.0f;
+                v[b] = *(const float4 *)(p.values(i) + (in ? 4 * lane : 0));
+            }
+#pragma unroll
+            for (int b = 0; b < PB; b++)
+                if (f[b] != 0.0f) { /* a part without a visible position was never written */
+                    acc.x = __builtin_fmaf(f[b], v[b].x, acc.x), acc.y = __builtin_fmaf(f[b], v[b].y, acc.y);
+                    acc.z = __builtin_fmaf(f[b], v[b].z, acc.z), acc.w = __builtin_fmaf(f[b], v[b].w, acc.w);
+                }
+        }
+    }
+    const bool some = all > 0.0f || !(all == all); /* nothing in sight: 0 */
+    const float x[4] = {some ? acc.x / all : 0.0f, some ? acc.y / all : 0.0f, some ? acc.z / all : 0.0f, some ? acc.w / all : 0.0f};
+    const float gx[4] = {gate.x, gate.y, gate.z, gate.w};
+    float o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = x[i] * nmx_sigmoid(gx[i]);
+    const int at = h * hd + col;
+    if (in) *(float4 *)(a.o + (size_t)t * a.nh * hd + at) = make_float4(o[0], o[1], o[2], o[3]);
+    if (a.aq) { /* blocks of 32 columns: 8 lanes of 4 */
+        float m = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
+        m = max_lanes<8>(m);
+        const float id = m > 0.0f ? 127.0f / m : 0.0f;
+        int c[4], n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            c[i] = (int)rintf(o[i] * id), n += c[i];
+            c[i] = c[i] > 127 ? 127 : c[i] < -128 ? -128 : c[i];
+        }
+        n += nmx_dpp<NMX_DPP_XOR1>(n);
+        n += nmx_dpp<NMX_DPP_XOR2>(n);
+        n += nmx_dpp<NMX_DPP_HALF_MIRROR>(n);
+        if (in) {
+            const size_t u = (size_t)(at >> 5) * a.n + t;
+            *(uint32_t *)(a.aq + u * 32 + (at & 31)) = (uint32_t)(c[0] & 255) | (uint32_t)(c[1] & 255) << 8 | (uint32_t)(c[2] & 255) << 16 | (uint32_t)c[3] << 24;
+            if (lane % 8 == 0) {
+                const float d = m / 127.0f;
+                a.ad[u] = d, a.afs[u] = d * (float)n;
+            }
+        }
+    }
+}
 
 /* Workgroup: a row and head, blockIdx.y a group of a.jcols columns of it (of one half). */
 template <int HDP>
@@ -800,58 +963,19 @@ __global__ __launch_bounds__(JB) void attn_batch_join_k(BatchAttn a) {
     __shared__ float red[2][JB / 64], acc_s[JB * 4], w_s[JB_PARTS];
     __shared__ const float *at_s[JB_PARTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.x / a.nh, h = blockIdx.x % a.nh;
-    const int hd = a.pg.hd, nkv = a.pg.nkv, rep = a.nh / nkv, g = h / rep, c0 = blockIdx.y * a.jcols, half = c0 / OD;
+    const int hd = a.pg.hd, c0 = blockIdx.y * a.jcols, half = c0 / OD;
     const float gate = a.q[((size_t)t * a.nh + h) * 2 * hd + hd + c0 + (tid < a.jcols ? tid : 0)];
-    const Shares sh = a.plan->sh;
-    const int s = seq_of_row(a.row0, a.pg.seqs, t);
-    if (s < 0) return; /* uniform over the workgroup */
-    const SeqRows rows = seq_rows(a.row0, s, a.n);
-    if (t >= rows.r0 + rows.count) return; /* a row of no sequence is left as it is */
-    const Seg own = a.plan->seg[a.groups + s];
-    Seg pre = own;
-    pre.unit = 0;
-    if (own.group >= 0) pre = a.plan->seg[own.group];
-    /* The parts of this row and half: those of the prefix, then the sequence's own. Of a unit of few rows: those of
-     * single waves, of workgroups whose share lies in it, of single waves. */
-    int count[2], solo[2], whole[2];
-    const float *val[2];
-    const float4 *st[2];
-    size_t vstep[2], sstep[2];
-    auto over = [](unsigned long long c, unsigned long long n) {
-        return c >> 32 || n >> 32 ? (uint32_t)(c / n) : (uint32_t)c / (uint32_t)n;
-    };
-#pragma unroll 1
-    for (int k = 0; k < 2; k++) {
-        const Seg &x = k ? own : pre;
-        const int rr = (t - x.r0) * rep + h % rep;
-        count[k] = 0, solo[k] = whole[k] = 0, val[k] = nullptr, st[k] = nullptr, vstep[k] = sstep[k] = 0;
-        if (!x.unit || rr < 0 || rr >= x.m) continue;
-        const bool mx = x.m > AB_VR;
-        const int tr = mx ? tile_rows<HDP>() : AB_VR, width = mx ? OD : hd;
-        const uint32_t u = (mx ? rr / tr * halves<HDP>() + half : 0) * nkv + g;
-        const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit, per = mx ? sh.per_m : sh.per_w;
-        const uint32_t w0 = over(cu, per), w1 = over(cu + x.unit - 1, per);
-        count[k] = solo[k] = (int)(w1 - w0) + 1;
-        if (!mx) {
-            const uint32_t f0 = (w0 * per == cu ? w0 + AB_PARTS - 1 : w0 + AB_PARTS) / AB_PARTS, f1 = over(cu + x.unit, per) / AB_PARTS;
-            if (f1 > f0) solo[k] = (int)(f0 * AB_PARTS - w0), whole[k] = (int)(f1 - f0), count[k] -= whole[k] * (AB_PARTS - 1);
-        }
-        const size_t slot = (size_t)w0 + x.u0 + u;
-        val[k] = (mx ? a.part_m : a.part_v) + (slot * tr + rr % tr) * width + (mx ? c0 - half * OD : c0);
-        st[k] = (mx ? a.stat_m : a.stat_v) + slot * tr + rr % tr;
-        vstep[k] = (size_t)tr * width, sstep[k] = tr;
-    }
-    const int parts = count[0] + count[1];
+    const Parts<HDP> p(a, t, h, half);
+    if (!p.any) return; /* a row of no sequence is left as it is; uniform over the workgroup */
+    const int parts = p.all();
     constexpr int PT = (JB_PARTS + JB - 1) / JB;
     float4 y[PT];
     float top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < PT; k++) {
-        const int i = tid + JB * k, b = i >= count[0], nth = b ? i - count[0] : i;
-        const int inner = nth - solo[b]; /* parts of whole workgroups stand AB_PARTS slots apart */
-        const int at = inner <= 0 ? nth : nth + (inner < whole[b] ? inner : whole[b]) * (AB_PARTS - 1);
+        const int i = tid + JB * k;
         y[k] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-        if (i < parts) y[k] = st[b][at * sstep[b]], at_s[i] = val[b] + at * vstep[b];
+        if (i < parts) y[k] = p.stat(i), at_s[i] = p.values(i) + c0 - half * OD;
         top = fmaxf(top, y[k].x);
     }
     top = nmx_max_f32_wave(top);
@@ -952,7 +1076,9 @@ int launch(nmx_ctx *ctx, const BatchAttn &a) {
     attn_batch_k<HDP, KVT><<<AB_WGS, 64 * ctx_waves<HDP>(), lds, ctx->stream>>>(a.row0, a.pg.len, a.pg.seqs, a.n, a.groups,
                                                                               a.pg.max_pages << a.pg.shift, a);
     NMX_LAUNCHED(ctx, "attn_batch");
-    attn_batch_join_k<HDP><<<dim3((unsigned)(a.n * a.nh), (unsigned)(a.pg.hd / a.jcols)), JB, 0, ctx->stream>>>(a);
+    const int items = a.n * a.nh * halves<HDP>();
+    if (items >= JB_WAVES) attn_batch_join_waves_k<HDP><<<(items + JB / 64 - 1) / (JB / 64), JB, 0, ctx->stream>>>(a);
+    else attn_batch_join_k<HDP><<<dim3((unsigned)(a.n * a.nh), (unsigned)(a.pg.hd / a.jcols)), JB, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "attn_batch_join");
     return 0;
 }

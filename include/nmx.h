@@ -580,8 +580,9 @@ int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work);
  * begins with shared[j] rows (device [groups]) that are the same in all of them: they are read once for
  * the whole group, by the table of its first sequence that has rows (no more than come before the rows of
  * any of its sequences count). groups 0: nothing shared. A row that sees nothing gives 0. Sums and softmax
- * statistics are 32 bits; results are right to 32-bit rounding (operands of 22 bits where more than 16 query
- * rows of a KV head meet the same keys) and do not depend on the other rows. Rows of pages that a row sees hold finite
+ * statistics are 32 bits; operands are held to 22 bits of their row's largest (two binary16 parts) and results are right to
+ * 32-bit rounding. A row's result depends on how the batch's positions are divided, within that rounding; the same call
+ * gives the same bits. Rows of pages that a row sees hold finite
  * values; what lies behind the last position of a page may be anything. work: device scratch of
  * nmx_attn_batch_work_bytes bytes (0 for a shape that is refused; enough for all lengths), 16-byte aligned,
  * used by one call at a time. nh <= 1024, q, the caches and o 16-byte aligned. */

@@ -4,15 +4,21 @@
  *
  * The work is a list of segments: for each group the rows of all its sequences against the shared prefix,
  * for each sequence its rows against what follows. A segment has units (KV head, tile of query rows), a
- * unit steps of 32 positions, and the steps of all units in a row are cut into equal shares, one for each
- * workgroup, whatever the lengths: a share may end one unit and begin others. Lengths are on the device,
- * so every workgroup makes the list itself (a scan over at most 512 segments). What a workgroup finds of a
- * unit is a part (weighted values, maximum, sum); attn_batch_join_k adds a row's parts in order.
+ * unit steps of 32 positions. Lengths are on the device, so every workgroup makes the list itself (one wave, a scan
+ * over at most 512 segments) and takes its share of the steps, whatever the lengths: a share may end one unit and
+ * begin others. What a share finds of a unit is a part (weighted values, maximum, sum); the join adds a row's parts in
+ * order.
  *
- * Two inner products. Up to 8 query rows (a token of each sequence: the heads of a KV group): fp32
- * vector instructions, a wave streaming rows from memory into registers, 16 columns a lane, the keys of the
- * next positions requested while the values of the current ones are added and the other way round; no LDS and no
- * barrier on the way. More rows: the matrix cores over tiles in LDS (nmx_attnmx.h). */
+ * Two kinds of segments. Up to 8 query rows (a token of a sequence: the heads of a KV group) are bound by the cache's bytes:
+ * a wave streams rows from memory into its registers, the keys of the next positions requested while the values of the
+ * current ones are added and the other way round, without a barrier on the way; shares are a wave's, so that
+ * the round trips at which a short sequence begins and ends hide behind other waves' work (with a workgroup's, each piece
+ * of one kept the CU for 12 us, and 48 sequences of 50 to 6000 positions took 40 instead of 32.5). More rows are bound by the
+ * matrix cores: tiles in LDS that the workgroup shares (nmx_attnmx.h).
+ *
+ * Times of both kernels on MI355X, 8 heads on 2 of 256, and of the attention kernel in a trace: 4 sequences of 300 to 700 fp32
+ * positions 14.4 us (9.3), 48 of 50 to 6000 binary16 32.5 (27; 118 MB, 23 as a copy), 64 of 1500 binary16 43 and fp32 81 (393 MB, 76
+ * as a copy), 64 with 30000 binary16 positions in common 71.5 (69), 20 of up to 90 rows with 700 int8 ones in common 47 (37). */
 #include <type_traits>
 
 #include "nmx_internal.h"
@@ -41,48 +47,106 @@ struct PrepBatch {
     uint32_t axis[16]; /* two bits for each frequency */
 };
 
-template <int KVT>
-__global__ __launch_bounds__(512) void attn_batch_prep_k(PrepBatch a) {
-    extern __shared__ float sq[];
-    __shared__ float buf[512];
-    __shared__ float red[8];
-    const int t = blockIdx.y, u = blockIdx.x, i = threadIdx.x, hd = a.pg.hd, h2 = a.rot / 2, nkv = a.pg.nkv;
+/* A wave for each row and head (attn_prep_k's operations: its sum of squares runs in four chains, here of four lanes over the
+ * wave's own LDS). Workgroups of a head and row, a thread a column, took 8.6 us for 460 rows of 8 + 2 heads, this 6.4; 8 rows 4.2
+ * and 4.8. E: 64 columns each, at least hd / 64. */
+constexpr int PREP_WAVES = 2;
+template <int KVT, int E>
+__device__ __forceinline__ void store_row(char *block, int nkv, int hd, int page, int R, int lane, const float (&x)[E]) {
+    float inv = 0.0f, m = 0.0f;
+    if constexpr (KVT == KV_I8) {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (64 * e < hd) m = fmaxf(m, fabsf(x[e]));
+        m = nmx_max_f32_wave(m);
+        inv = m > 127.0f / 3.40282347e+38f ? 127.0f / m : 0.0f; /* stays finite */
+        if (lane == 0) ((float *)(block + (size_t)nkv * page * hd))[R] = m / 127.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (64 * e >= hd) continue;
+        const size_t at = (size_t)R * hd + 64 * e + lane;
+        if constexpr (KVT == KV_F32) ((float *)block)[at] = x[e];
+        else if constexpr (KVT == KV_F16) ((unsigned short *)block)[at] = (unsigned short)kv_half_bits(x[e]);
+        else ((int8_t *)block)[at] = (int8_t)kv_i8_code(x[e], inv);
+    }
+}
+template <int KVT, int E>
+__global__ __launch_bounds__(64 * PREP_WAVES) void attn_batch_prep_k(const int32_t *row0, const int32_t *len, int seqs, int n,
+                                                                     int heads, PrepBatch a) {
+    __shared__ float row_s[PREP_WAVES][512], sum_s[PREP_WAVES][4];
+    const int lane = lane_id(), wave = wave_id(), item = blockIdx.x * PREP_WAVES + wave, t = item / heads, u = item % heads;
+    if (t >= n) return;
+    const int hd = a.pg.hd, h2 = a.rot / 2, nkv = a.pg.nkv;
     const bool is_k = u < nkv;
-    float v = is_k ? a.k_in[(size_t)t * nkv * hd + u * hd + i] : a.q[((size_t)t * a.nh + (u - nkv)) * 2 * hd + i];
-    const float w = is_k ? a.k_norm[i] : a.q_norm[i];
-    const float val = is_k ? a.v_in[(size_t)t * nkv * hd + u * hd + i] : 0.0f;
-    const int f = i < h2 ? i : i - h2; /* the frequency of columns below rot */
-    const bool turns = i < 2 * h2;
-    int at = 0;
-    if (turns && a.rope_pos) at = a.rope_pos[t * a.axes + (a.axis[f >> 4] >> 2 * (f & 15) & 3)];
-    const int s = seq_of_row(a.row0, a.pg.seqs, t);
-    if (s < 0) return; /* uniform over the workgroup */
-    const SeqRows rows = seq_rows(a.row0, s, a.n);
+    const float *in = is_k ? a.k_in + ((size_t)t * nkv + u) * hd : a.q + ((size_t)t * a.nh + (u - nkv)) * 2 * hd;
+    const float *w = is_k ? a.k_norm : a.q_norm, *vi = a.v_in + ((size_t)t * nkv + (is_k ? u : 0)) * hd;
+    float x[E], wt[E], val[E], cs[E], sn[E];
+    int at[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (64 * e >= hd) continue; /* uniform */
+        const int i = 64 * e + lane, f = i < h2 ? i : i - h2; /* the frequency of columns below rot */
+        x[e] = in[i], wt[e] = w[i], val[e] = is_k ? vi[i] : 0.0f, at[e] = 0;
+        if (i < 2 * h2 && a.rope_pos) at[e] = a.rope_pos[t * a.axes + (a.axis[f >> 4] >> 2 * (f & 15) & 3)];
+    }
+    const int s = seq_of_row(row0, seqs, t);
+    if (s < 0) return; /* uniform over the wave */
+    const SeqRows rows = seq_rows(row0, s, n);
     if (t >= rows.r0 + rows.count) return;
     const int p = seq_len(a.pg, s) - rows.count + t - rows.r0;
-    if (!a.rope_pos) at = p;
-    at = at < 0 ? 0 : at < a.rope_rows ? at : a.rope_rows - 1;
-    float c = 0.0f, sn = 0.0f;
-    if (turns) c = a.rcos[(size_t)at * h2 + f], sn = a.rsin[(size_t)at * h2 + f];
     int id = -1;
     if (is_k && p >= 0) id = a.pg.table[(size_t)s * a.pg.max_pages + (p >> a.pg.shift)];
-    sq[i] = v * v;
-    __syncthreads();
-    const float ss = ordered_sum4(sq, hd, red);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (64 * e >= hd) continue;
+        const int i = 64 * e + lane, f = i < h2 ? i : i - h2;
+        cs[e] = sn[e] = 0.0f;
+        if (i < 2 * h2) {
+            int r = a.rope_pos ? at[e] : p;
+            r = r < 0 ? 0 : r < a.rope_rows ? r : a.rope_rows - 1;
+            cs[e] = a.rcos[(size_t)r * h2 + f], sn[e] = a.rsin[(size_t)r * h2 + f];
+        }
+    }
+    float *buf = row_s[wave];
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (64 * e < hd) buf[64 * e + lane] = x[e] * x[e];
+    nmx_lds_wave_sync();
+    if (lane < 4) { /* ordered_sum4's chains */
+        float c = 0.0f;
+        for (int m0 = 0; m0 < hd / 4; m0 += 16) {
+            float b[16];
+#pragma unroll
+            for (int k = 0; k < 16; k++) b[k] = buf[4 * (m0 + k) + lane];
+#pragma unroll
+            for (int k = 0; k < 16; k++) c = c + b[k];
+        }
+        sum_s[wave][lane] = c;
+    }
+    nmx_lds_wave_sync();
+    const float *c4 = sum_s[wave];
+    const float ss = ((c4[0] + c4[1]) + (c4[2] + c4[3])) + 0.0f;
     const float r = 1.0f / sqrtf(ss / (float)hd + a.eps);
-    v = (v * r) * w;
-    buf[i] = v;
-    __syncthreads();
-    if (i < h2) v = buf[i] * c - buf[i + h2] * sn;
-    else if (turns) v = buf[i] * c + buf[i - h2] * sn;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        if (64 * e < hd) buf[64 * e + lane] = x[e] = (x[e] * r) * wt[e];
+    nmx_lds_wave_sync();
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        if (64 * e >= hd) continue;
+        const int i = 64 * e + lane;
+        if (i < h2) x[e] = buf[i] * cs[e] - buf[i + h2] * sn[e];
+        else if (i < 2 * h2) x[e] = buf[i] * cs[e] + buf[i - h2] * sn[e];
+    }
     if (!is_k) {
-        a.q[((size_t)t * a.nh + (u - nkv)) * 2 * hd + i] = v;
-    } else if ((uint32_t)id < (uint32_t)a.pg.npages) { /* uniform per workgroup */
-        nmx_attn_dev d{}; /* a block is a cache of `page` positions */
-        d.nkv = nkv, d.hd = hd, d.max_ctx = 1 << a.pg.shift;
-        const size_t R = ((size_t)u << a.pg.shift) + (p & (d.max_ctx - 1));
-        kv_store<KVT>((char *)a.kc + id * a.pg.block, d, R, i, v, red);
-        kv_store<KVT>((char *)a.vc + id * a.pg.block, d, R, i, val, red);
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (64 * e < hd) a.q[((size_t)t * a.nh + (u - nkv)) * 2 * hd + 64 * e + lane] = x[e];
+    } else if ((uint32_t)id < (uint32_t)a.pg.npages) { /* uniform over the wave */
+        const int page = 1 << a.pg.shift, R = (u << a.pg.shift) + (p & (page - 1));
+        store_row<KVT, E>((char *)a.kc + id * a.pg.block, nkv, hd, page, R, lane, x);
+        store_row<KVT, E>((char *)a.vc + id * a.pg.block, nkv, hd, page, R, lane, val);
     }
 }
 
@@ -90,22 +154,11 @@ __global__ __launch_bounds__(512) void attn_batch_prep_k(PrepBatch a) {
 constexpr int AB_SEGS = 2 * NMX_BATCH_MAX; /* a prefix for each group, the rest of each sequence */
 constexpr int AB_WGS = 256;                /* shares: a workgroup to a CU */
 constexpr int AB_VR = 8;                   /* query rows that the vector kind takes: 4 a wave */
-/* a step of 32 positions costs a workgroup about as long by either product, tiles of many rows half as much again;
- * a unit's beginning is round trips that its workgroup (or its wave, beside others) waits for */
-#ifndef COSTM
-#define COSTM 20
-#endif
-#ifndef COSTV
-#define COSTV 8
-#endif
-constexpr int AB_COST_V = COSTV, AB_COST_M = COSTM;
-#ifndef OVERHEAD
-#define OVERHEAD 8
-#endif
-#ifndef OVERHEADM
-#define OVERHEADM 80
-#endif
-constexpr int AB_BEGIN_V = OVERHEAD, AB_BEGIN_M = OVERHEADM;
+/* A step of 32 positions costs a workgroup this much: of the vector kind (4 query rows) what its bytes take at a CU's share of
+ * the memory's rate, of the matrix kind 2.5 times as long (64 questions about 30000 shared rows, binary16: 71.5 us; at 2 times 74.9,
+ * at 3 times 71.1, and pieces of prompts among tokens slower). A unit's beginning is round trips that its workgroup waits for, or
+ * its wave beside others. Eight units of cost a step, so that a share of the smallest batches is one step. */
+constexpr int AB_COST_V = 8, AB_COST_M = 20, AB_BEGIN_V = 8, AB_BEGIN_M = 80;
 
 /* of a segment of m query rows */
 __device__ __forceinline__ int step_cost(int m) { return m > AB_VR ? AB_COST_M : m > 4 ? 2 * AB_COST_V : AB_COST_V; }
@@ -791,10 +844,9 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
 
 /* ---- the join -------------------------------------------------------------------------------------- */
 constexpr int JB = 256;              /* threads */
-#ifndef JBW
-#define JBW 1024
-#endif
-constexpr int JB_WAVES = JBW; /* rows, heads and halves from which a wave takes one alone */
+/* rows, heads and halves from which a wave takes one alone (423 rows of 8 heads: 47.1 us against 52.6, 64 rows: 74.0 against
+ * 71.5) */
+constexpr int JB_WAVES = 1024;
 constexpr int JB_PARTS = 2 * (AB_WGS + 2 * AB_PARTS);
 
 /* The parts of a row's head and half: those of the prefix, then the sequence's own. Of a unit of few rows: those of single
@@ -1136,12 +1188,18 @@ int nmx_attn_batch_prep(nmx_ctx *ctx, const nmx_attn_batch_args *p) {
     a.q_norm = p->q_norm, a.k_norm = p->k_norm, a.eps = p->eps, a.rcos = p->rope_cos, a.rsin = p->rope_sin;
     a.rope_rows = p->rope_rows, a.axes = p->axes, a.rope_pos = p->rope_pos, a.kc = p->kc, a.vc = p->vc;
     const nmx_on_device on(ctx);
-    const dim3 grid((unsigned)(a.pg.nkv + p->nh), (unsigned)p->n);
-    const size_t lds = (size_t)hd * 4;
-    const int kv = p->pages.kv_dtype;
-    if (kv == KV_F16) attn_batch_prep_k<KV_F16><<<grid, (unsigned)hd, lds, ctx->stream>>>(a);
-    else if (kv == KV_I8) attn_batch_prep_k<KV_I8><<<grid, (unsigned)hd, lds, ctx->stream>>>(a);
-    else attn_batch_prep_k<KV_F32><<<grid, (unsigned)hd, lds, ctx->stream>>>(a);
+    const int heads = a.pg.nkv + p->nh, kv = p->pages.kv_dtype;
+    const unsigned wgs = (unsigned)(((size_t)p->n * heads + PREP_WAVES - 1) / PREP_WAVES);
+    auto go = [&](auto kernel) { kernel<<<wgs, 64 * PREP_WAVES, 0, ctx->stream>>>(a.row0, a.pg.len, a.pg.seqs, a.n, heads, a); };
+    auto go_kv = [&](auto e) {
+        if (kv == KV_F16) go(attn_batch_prep_k<KV_F16, e.value>);
+        else if (kv == KV_I8) go(attn_batch_prep_k<KV_I8, e.value>);
+        else go(attn_batch_prep_k<KV_F32, e.value>);
+    };
+    if (hd <= 64) go_kv(std::integral_constant<int, 1>{});
+    else if (hd <= 128) go_kv(std::integral_constant<int, 2>{});
+    else if (hd <= 256) go_kv(std::integral_constant<int, 4>{});
+    else go_kv(std::integral_constant<int, 8>{});
     NMX_LAUNCHED(ctx, "attn_batch_prep");
     return 0;
 }

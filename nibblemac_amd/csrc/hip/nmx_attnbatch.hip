@@ -194,9 +194,9 @@ struct BatchAttn {
     const void *kc, *vc;
     float scale;
     Plan *plan;
-    float *part_v, *part_m; /* parts of the vector kind [slot][16][hd], of the matrix kind [slot][tile][columns] */
+    float *part_v, *part_m; /* parts of the vector kind [slot][vrows][hd], of the matrix kind [slot][tile][columns] */
     float4 *stat_v, *stat_m;
-    int jcols;
+    int jcols, vrows; /* vrows: AB_VR, or the query rows of a KV head if there are fewer */
     float *o;
     int8_t *aq;
     float *ad, *afs;
@@ -812,10 +812,10 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
     const int quads = x.m > 4 ? 2 : 1;
     if (together) {
         const size_t slot = (size_t)(w - mxs) * AB_PARTS + unit;
-        float4 *stat = a.stat_v + slot * AB_VR;
+        float4 *stat = a.stat_v + slot * a.vrows;
         if (p0 < p1) vector_piece<HDP, KVT>(a, x, g, p0, p1, wave % quads, wave / quads, WV / quads, true,
-                                            a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
-        else if (tid < AB_VR) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+                                            a.part_v + slot * a.vrows * a.pg.hd, stat, smem);
+        else if (tid < a.vrows) stat[tid] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         return;
     }
     __syncthreads(); /* everyone has read the first piece */
@@ -830,13 +830,13 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
             find_piece<HDP>(a, segs, seg, false, piece_s[wave].next, (share + 1) * sh_s.per_w, piece_s + wave);
             if (!take(piece_s[wave])) break;
             const size_t slot = share + unit;
-            float4 *stat = a.stat_v + slot * AB_VR;
-            if (p0 >= p1 && tid % 64 < AB_VR) stat[tid % 64] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            float4 *stat = a.stat_v + slot * a.vrows;
+            if (p0 >= p1 && tid % 64 < a.vrows) stat[tid % 64] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
             for (int k = wave % team; 4 * k < x.m && p0 < p1; k += team) {
                 /* nothing of a pass is kept for the next one */
                 asm volatile("" : "+s"(p0), "+s"(p1), "+s"(g), "+s"(x.seq), "+s"(x.r0), "+s"(x.m), "+s"(x.last));
-                vector_piece<HDP, KVT>(a, x, g, p0, p1, k, 0, 1, false, a.part_v + slot * AB_VR * a.pg.hd, stat, smem);
+                vector_piece<HDP, KVT>(a, x, g, p0, p1, k, 0, 1, false, a.part_v + slot * a.vrows * a.pg.hd, stat, smem);
             }
         }
     }
@@ -885,7 +885,7 @@ struct Parts {
             uint32_t vs = 0, ss = 0;
             if (x.unit && rr >= 0 && rr < x.m) {
                 const bool mx = x.m > AB_VR;
-                const int tr = mx ? tile_rows<HDP>() : AB_VR, width = mx ? OD : hd;
+                const int tr = mx ? tile_rows<HDP>() : a.vrows, width = mx ? OD : hd;
                 const uint32_t u = (mx ? rr / tr * halves<HDP>() + half : 0) * nkv + g;
                 const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit, per = mx ? sh.per_m : sh.per_w;
                 const uint32_t w0 = over(cu, per), w1 = over(cu + x.unit - 1, per);
@@ -1085,7 +1085,7 @@ __global__ __launch_bounds__(JB) void attn_batch_join_k(BatchAttn a) {
 
 /* ---- the workspace ----------------------------------------------------------------------------------- */
 struct Room {
-    int hdp, jcols;
+    int hdp, jcols, vrows;
     size_t stat_v, part_m, stat_m, plan, bytes; /* part_v at 0 */
 };
 
@@ -1099,8 +1099,9 @@ Room make_room(int n, int seqs, int groups, int nh, int nkv, int hd) {
     const size_t some = qr / (AB_VR + 1);
     const size_t big = (some < (size_t)seqs ? some : seqs) + (some < (size_t)groups ? some : groups);
     const size_t sm = big ? AB_WGS + (2 * (qr / tr) + big) * hv * nkv : 0;
-    size_t at = sv * AB_VR * hd * 4;
-    r.stat_v = at, at += sv * AB_VR * sizeof(float4);
+    r.vrows = qr < AB_VR ? (int)qr : AB_VR; /* the clamped rows of all sequences are n at most */
+    size_t at = sv * r.vrows * hd * 4;
+    r.stat_v = at, at += sv * r.vrows * sizeof(float4);
     r.part_m = at, at += sm * tr * od * 4;
     r.stat_m = at, at += sm * tr * sizeof(float4);
     r.plan = at, at += (sizeof(Plan) + 15) / 16 * 16;
@@ -1129,7 +1130,7 @@ int launch(nmx_ctx *ctx, const BatchAttn &a) {
                                                                               a.pg.max_pages << a.pg.shift, a);
     NMX_LAUNCHED(ctx, "attn_batch");
     const int items = a.n * a.nh * halves<HDP>();
-    if (items >= JB_WAVES) attn_batch_join_waves_k<HDP><<<(items + JB / 64 - 1) / (JB / 64), JB, 0, ctx->stream>>>(a);
+    if (items >= JB_WAVES && (uintptr_t)a.aq % 4 == 0) attn_batch_join_waves_k<HDP><<<(items + JB / 64 - 1) / (JB / 64), JB, 0, ctx->stream>>>(a);
     else attn_batch_join_k<HDP><<<dim3((unsigned)(a.n * a.nh), (unsigned)(a.pg.hd / a.jcols)), JB, 0, ctx->stream>>>(a);
     NMX_LAUNCHED(ctx, "attn_batch_join");
     return 0;
@@ -1234,7 +1235,7 @@ int nmx_attn_batch(nmx_ctx *ctx, const nmx_attn_batch_args *p, void *work) {
     a.n = p->n, a.nh = p->nh, a.groups = p->groups, a.row0 = p->row0, a.group0 = p->group0, a.shared = p->shared;
     a.q = p->q, a.kc = p->kc, a.vc = p->vc, a.scale = p->scale, a.plan = (Plan *)(ws + r.plan);
     a.part_v = (float *)ws, a.stat_v = (float4 *)(ws + r.stat_v), a.part_m = (float *)(ws + r.part_m);
-    a.stat_m = (float4 *)(ws + r.stat_m), a.jcols = r.jcols, a.o = p->o, a.aq = p->a8.q, a.ad = p->a8.d, a.afs = p->a8.fs;
+    a.stat_m = (float4 *)(ws + r.stat_m), a.jcols = r.jcols, a.vrows = r.vrows, a.o = p->o, a.aq = p->a8.q, a.ad = p->a8.d, a.afs = p->a8.fs;
     const nmx_on_device on(ctx);
     return kv == KV_F16 ? launch_hd<KV_F16>(ctx, a, r.hdp) : kv == KV_I8 ? launch_hd<KV_I8>(ctx, a, r.hdp) :
            launch_hd<KV_F32>(ctx, a, r.hdp);

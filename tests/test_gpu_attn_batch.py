@@ -229,6 +229,45 @@ def test_long_sequences(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_F16, KV_I8])
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 4, 64), (8, 1, 64), (6, 2, 128), (4, 1, 192), (8, 2, 256), (8, 1, 256), (4, 1, 320), (8, 1, 512)])
+def test_shares_of_waves_and_workgroups(dev, nh, nkv, hd, kv):
+    """Short sequences that single waves take beside long ones whose parts whole workgroups take, several turns each,
+    with 3 to 8 query rows."""
+    rng = np.random.default_rng(hd + kv)
+    ctx = [6000, 10, 40, 300, 1, 0, 700, 33, 15, 2000, 64, 100, 31, 32, 129, 5, 5, 900]
+    check(dev, Case(rng, [1] * len(ctx), ctx, nh, nkv, hd, 16, kv, [(4, 0), (6, 10)] if hd == 128 else ()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,kv", [(256, KV_F16), (64, KV_F32), (320, KV_I8)])
+def test_many_rows(dev, hd, kv):
+    """Joins by waves: 300 rows of 8 heads, padded, and their A8."""
+    c = Case(np.random.default_rng(hd), [1] * 100 + [0, 150, 49, 1], [7] * 90 + [100] * 14, 8, 2, hd, 32, kv, [(0, 5)], pad=3)
+    check(dev, c)
+    o, q, d, fs = attend(dev, c, a8=True)
+    live, nb = int(c.row0[-1]), c.nh * c.hd // 32
+    x = dev.to_device(o[:live])
+    a = (dev.zeros((nb, live, 32), np.int8), dev.zeros((nb, live), np.float32), dev.zeros((nb, live), np.float32))
+    dev.quant_a8(x, live, c.nh * c.hd, *a)
+    dev.sync()
+    for got, want in zip((q, d, fs), a):
+        assert_bits_equal(got[:, :live], want.numpy(), "A8")
+        assert not got[:, live:].any()
+    for b in (x, *a):
+        b.free()
+
+
+@pytest.mark.gpu
+def test_most_sequences(dev):
+    """256 sequences and groups."""
+    rng = np.random.default_rng(15)
+    ctx = rng.integers(0, 60, 256)
+    check(dev, Case(rng, [1] * 255 + [0], ctx, 4, 2, 64, 16, KV_F16, [(s, int(ctx[s])) for s in range(256)]))
+    check(dev, Case(rng, [1] * 256, [40] * 256, 4, 2, 64, 16, KV_I8, [(0, 33), (100, 20)]))
+
+
+@pytest.mark.gpu
 def test_caches_past_4_gib(dev):
     """Pages whose bytes lie past 2^32 in the cache."""
     page, nkv, hd = 256, 4, 512

@@ -631,7 +631,7 @@ int nmx_lin_mix_batch(nmx_ctx *ctx, const nmx_lin_mix_args *a, const nmx_lin_bat
  * B[s][m] (A[s][m] x[t]) for each of the count matrices; A[s] is [adapters][rank][cols] and B[s]
  * [adapters][rows[s]][rank], both of w_dtype 0 fp32, 1 binary16 or 2 bfloat16. ranks (device [adapters],
  * may be NULL): an adapter's own rank where it is less, what lies behind it in A and B is not used and may be
- * anything. Y is what nmx_q4k_matmul* left there (or the residual). Products and sums are 32 bits, in an
+ * anything. Y is what nmx_q4k_matmul* left there (or the residual); several may be columns of the same rows. Products and sums are 32 bits, in an
  * order that depends on the shapes alone. n <= NMX_CHUNK_ROWS, cols a multiple of 32 up to 32768, rank <= 256,
  * rows <= 2^20; x 16-byte aligned rows; A and B 16-byte aligned. work: device scratch of nmx_lora_work_bytes bytes
  * (0 for a shape that is refused), 16-byte aligned, used by one call at a time. */

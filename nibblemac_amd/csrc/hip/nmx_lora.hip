@@ -321,6 +321,14 @@ int launch(nmx_ctx *ctx, const Lora &a) {
     return 0;
 }
 
+/* Matrices i and k write columns of their own of the same rows. */
+bool side_by_side(const nmx_lora_args &p, int i, int k) {
+    const intptr_t by = (intptr_t)p.Y[k] - (intptr_t)p.Y[i], row = (intptr_t)p.y_stride[i] * 4;
+    if (p.y_stride[i] != p.y_stride[k] || by % 4) return false;
+    const intptr_t at = (by % row + row) % row; /* of k's first column from i's, within a row */
+    return at >= (intptr_t)p.rows[i] * 4 && at + (intptr_t)p.rows[k] * 4 <= row;
+}
+
 } // namespace
 
 extern "C" {
@@ -365,7 +373,7 @@ int nmx_lora(nmx_ctx *ctx, const nmx_lora_args *p, void *work) {
             if (nmx_overlap(out[i].p, out[i].bytes, in[k].p, in[k].bytes))
                 return nmx_fail(ctx, "nmx_lora: an output or work overlaps an input");
         for (int k = 0; k < i; k++)
-            if (nmx_overlap(out[i].p, out[i].bytes, out[k].p, out[k].bytes))
+            if (nmx_overlap(out[i].p, out[i].bytes, out[k].p, out[k].bytes) && !(k > 0 && side_by_side(*p, i - 1, k - 1)))
                 return nmx_fail(ctx, "nmx_lora: outputs and work overlap");
     }
     a.rank16 = (p->rank + 15) / 16 * 16, a.cols = p->cols;

@@ -183,6 +183,26 @@ def test_replayed_with_other_adapters(dev):
         free(ds[0])
 
 
+@pytest.mark.gpu
+def test_matrices_side_by_side(dev):
+    """Outputs that are columns of the same rows."""
+    rng = np.random.default_rng(5)
+    c = Case(rng, 11, 128, [40, 24, 30], 3, 12, 1)
+    d, Y = c.upload(dev), dev.to_device(np.concatenate([y for y in c.y] + [c.y[0][:, :2]], 1))
+    wide, at = 40 + 24 + 30 + 2, 0
+    segs = []
+    for r, A, B in zip(c.rows, d["A"], d["B"]):
+        segs.append((r, A, B, Y.ptr + 4 * at, wide))
+        at += r
+    dev.lora(lora_args(11, 128, d["x"], c.xs, 3, 12, 1, d["ids"], d["scale"], segs[::-1]), d["work"])
+    dev.sync()
+    want, tol = c.reference()
+    got = Y.numpy()
+    assert (np.abs(got[:, :94] - np.concatenate(want, 1)) <= np.concatenate(tol, 1)).all() and (got[:, 94:] == c.y[0][:, :2]).all()
+    Y.free()
+    free(d)
+
+
 def test_refusals():
     at = iter(range(1 << 36, 1 << 45, 1 << 36))
     P = {k: next(at) for k in ("x", "ids", "ranks", "scale", "A", "B", "Y", "A2", "B2", "Y2", "work")}
@@ -201,7 +221,8 @@ def test_refusals():
     bad += [args(one(**k)) for k in (dict(r=0), dict(r=(1 << 20) + 1, s=1 << 21), dict(s=31), dict(A=None), dict(B=None), dict(Y=None),
                                      dict(A=P["A"] + 8), dict(B=P["B"] + 2), dict(Y=P["Y"] + 2), dict(Y=P["x"]), dict(Y=P["A"] + 64),
                                      dict(Y=P["B"]), dict(Y=P["ids"]), dict(Y=P["ranks"] + 8), dict(Y=P["scale"]), dict(Y=P["work"]))]
-    bad += [args([(32, P["A"], P["B"], P["Y"], 32), (16, P["A2"], P["B2"], P["Y"] + 64, 32)])]
+    bad += [args([(32, P["A"], P["B"], P["Y"], s), (16, P["A2"], P["B2"], P["Y"] + 4 * at, t)])
+            for s, t, at in ((32, 32, 16), (48, 48, 31), (48, 48, 33), (48, 64, 32), (47, 47, 32), (48, 48, 48 + 31), (48, 48, 0))]
     for i, a in enumerate(bad):
         refuses("nmx_lora", i, a, P["work"])
     refuses("nmx_lora", "no work", args(), None)

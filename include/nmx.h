@@ -520,10 +520,10 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p);
 /* ---- a batch of sequences -------------------------------------------------------------------
  * One step of up to NMX_BATCH_MAX sequences with up to NMX_CHUNK_ROWS rows in all: sequence s has the
  * rows row0[s] .. row0[s + 1] (device int32 [seqs + 1], from 0 on and not falling; values outside [0, n]
- * are taken as the nearer end; lists that fall leave results unspecified): one row where it decodes, many where it reads a prompt, none where it
- * waits. Rows past row0[seqs] (a padded batch) are left alone: not read, not written. The reference serves one sequence
- * (engine/include/pinfer.h). The other calls of a step (products, norms, heads, nmx_sample) take rows
- * of whatever sequence as they are.
+ * are taken as the nearer end; lists that fall leave results unspecified): one row where it decodes, many
+ * where it reads a prompt, none where it waits. Rows past row0[seqs] (a padded batch) are left alone: not read,
+ * not written. The reference serves one sequence (engine/include/pinfer.h). The other calls of a step
+ * (products, norms, heads, nmx_sample) take rows of whatever sequence as they are.
  *
  * KV rows lie in pages: a cache is [npages] blocks of nmx_kv_bytes(kv_dtype, nkv, page, hd) bytes, each laid
  * out as a cache of `page` positions, and position p of sequence s is row p % page of the block
@@ -552,7 +552,8 @@ typedef struct {
  *   max_pages; in both cases nothing else is changed; the pages taken; U (pack, else 0); pages moved.
  * caches (0: none): host array of device pointers, [npages] blocks each, 16-byte aligned: rows are copied
  * and moved in all of them. work: device scratch of nmx_pages_work_bytes bytes (0 for a shape that is
- * refused), 16-byte aligned, used by one call at a time. npages <= 2^20, max_pages <= 2^16. Table entries in use have to name pages of the cache. */
+ * refused), 16-byte aligned, used by one call at a time. npages <= 2^20, max_pages <= 2^16. Table entries in
+ * use have to name pages of the cache. */
 #define NMX_BATCH_KV_MAX 64
 typedef struct {
     nmx_pages pages;
@@ -580,10 +581,10 @@ int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work);
  * begins with shared[j] rows (device [groups]) that are the same in all of them: they are read once for
  * the whole group, by the table of its first sequence that has rows (no more than come before the rows of
  * any of its sequences count). groups 0: nothing shared. A row that sees nothing gives 0. Sums and softmax
- * statistics are 32 bits; operands are held to 22 bits of their row's largest (two binary16 parts) and results are right to
- * 32-bit rounding. A row's result depends on how the batch's positions are divided, within that rounding; the same call
- * gives the same bits. Rows of pages that a row sees hold finite
- * values; what lies behind the last position of a page may be anything. work: device scratch of
+ * statistics are 32 bits; operands are held to 22 bits of their row's largest (two binary16 parts) and results
+ * are right to 32-bit rounding. A row's result depends on how the batch's positions are divided, within that
+ * rounding; the same call gives the same bits. A sequence's positions hold finite values; what its pages hold behind
+ * its last position may be anything. work: device scratch of
  * nmx_attn_batch_work_bytes bytes (0 for a shape that is refused; enough for all lengths), 16-byte aligned,
  * used by one call at a time. nh <= 1024, q, the caches and o 16-byte aligned. */
 typedef struct {
@@ -631,9 +632,9 @@ int nmx_lin_mix_batch(nmx_ctx *ctx, const nmx_lin_mix_args *a, const nmx_lin_bat
  * B[s][m] (A[s][m] x[t]) for each of the count matrices; A[s] is [adapters][rank][cols] and B[s]
  * [adapters][rows[s]][rank], both of w_dtype 0 fp32, 1 binary16 or 2 bfloat16. ranks (device [adapters],
  * may be NULL): an adapter's own rank where it is less, what lies behind it in A and B is not used and may be
- * anything. Y is what nmx_q4k_matmul* left there (or the residual); several may be columns of the same rows. Products and sums are 32 bits, in an
- * order that depends on the shapes alone. n <= NMX_CHUNK_ROWS, cols a multiple of 32 up to 32768, rank <= 256,
- * rows <= 2^20; x 16-byte aligned rows; A and B 16-byte aligned. work: device scratch of nmx_lora_work_bytes bytes
+ * anything. Y is what nmx_q4k_matmul* left there (or the residual); several may be columns of
+ * the same rows. Products and sums are 32 bits, in an order that depends on the shapes alone.
+ * n <= NMX_CHUNK_ROWS, cols a multiple of 32 up to 32768, rank <= 256, rows <= 2^20; x 16-byte aligned rows; A and B 16-byte aligned. work: device scratch of nmx_lora_work_bytes bytes
  * (0 for a shape that is refused), 16-byte aligned, used by one call at a time. */
 typedef struct {
     int n, cols, x_stride, count;

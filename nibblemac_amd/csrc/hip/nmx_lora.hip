@@ -260,7 +260,8 @@ __global__ __launch_bounds__(64 * LU_WAVES) void lora_up_k(Lora a) {
     const float scale = a.scale[adapter];
     Up<WT, VEC> up(a, s, o0, adapter, own, row, lane);
     /* a column without a row takes the first one's: it is not stored */
-    const float *lp = a.low + ((size_t)s * a.n + (row < 0 ? __builtin_amdgcn_readfirstlane(row) : row)) * a.rank16 + 8 * up.k;
+    const int first = tile->row[0];
+    const float *lp = a.low + ((size_t)s * a.n + (row < 0 ? first : row)) * a.rank16 + 8 * up.k;
     for (int q = 0; q < own; q += 32) {
         float4 x[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
         up.request(q);

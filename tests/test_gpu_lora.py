@@ -156,6 +156,32 @@ def test_rows_do_not_depend_on_each_other(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,rank", [(1, 256), (2, 200), (3, 32), (7, 256)])
+def test_few_rows_of_large_ranks(dev, n, rank):
+    """Tiles that are mostly empty, the workspace's rows longer than its list of tiles."""
+    check(dev, Case(np.random.default_rng(n + rank), n, 128, [100, 24], 2, rank, 1, ids=[1] * n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank", [8, 48])
+def test_what_one_row_holds_stays_in_it(dev, rank):
+    """NaN and infinities in a row, in its adapter and in rows without one: the others' bits are as without them."""
+    rng = np.random.default_rng(rank)
+    c = Case(rng, 24, 96, [80, 33], 4, rank, 0, ids=[0, 1, 2, -1] * 6)
+    want = run(dev, c)
+    c.x[4], c.x[8, 5], c.x[3::4] = np.nan, np.inf, np.nan
+    for B in c.B:
+        B[2] = np.inf
+    got = run(dev, c)
+    for g, w in zip(got, want):
+        for t in range(24):
+            if t in (4, 8):
+                assert not np.isfinite(g[t]).any()
+            elif c.ids[t] != 2:
+                assert (g[t].view(np.uint32) == w[t].view(np.uint32)).all()
+
+
+@pytest.mark.gpu
 def test_replayed_with_other_adapters(dev):
     """Adapters, ranks and scales are the device's; a replay adds to y again. Two contexts at once."""
     rng = np.random.default_rng(4)

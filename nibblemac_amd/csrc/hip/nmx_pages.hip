@@ -7,7 +7,11 @@
  * sums over the counts, and writes tables and lengths. Up to PP_LDS pages the counts stand in LDS meanwhile, and go back
  * only if the step fits; of more pages they are changed where they are and a step that does not fit is taken back by the
  * opposite additions. A fork's entries go through the workspace, so sequences may exchange places. pages_copy_k and, with
- * pack, pages_move_k then copy what the plan lists, in all caches at once. */
+ * pack, pages_move_k then copy what the plan lists, in all caches at once.
+ *
+ * Times on MI355X: a token of 64 chats in 640 pages 11.2 us, of which the plan 7.6 and the copy of five pages in 14 caches 4 in
+ * a trace, both chains of round trips (the bytes take 0.8); 16 of 64 chats end and the others are packed, 1200 pages, 17.5 + 4.3
+ * + 21.2 in a trace, 26 as a copy. With the counts in memory, an atomic's round trip each, the plans took 15.8 and 34.5. */
 #include "nmx_internal.h"
 #include "nmx_batch.h"
 #include "nmx_lanes.h"

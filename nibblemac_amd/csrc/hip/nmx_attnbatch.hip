@@ -18,7 +18,7 @@
  *
  * Times of both kernels on MI355X, 8 heads on 2 of 256, and of the attention kernel in a trace: 4 sequences of 300 to 700 fp32
  * positions 14.4 us (9.3), 48 of 50 to 6000 binary16 32.5 (27; 118 MB, 23 as a copy), 64 of 1500 binary16 43 and fp32 81 (393 MB, 76
- * as a copy), 64 with 30000 binary16 positions in common 71.5 (69), 20 of up to 90 rows with 700 int8 ones in common 47 (37). */
+ * as a copy), 64 with 30000 binary16 positions in common 60, 20 of up to 90 rows with 700 int8 ones in common 43. */
 #include <type_traits>
 
 #include "nmx_internal.h"
@@ -155,8 +155,8 @@ constexpr int AB_SEGS = 2 * NMX_BATCH_MAX; /* a prefix for each group, the rest 
 constexpr int AB_WGS = 256;                /* shares: a workgroup to a CU */
 constexpr int AB_VR = 8;                   /* query rows that the vector kind takes: 4 a wave */
 /* A step of 32 positions costs a workgroup this much: of the vector kind (4 query rows) what its bytes take at a CU's share of
- * the memory's rate, of the matrix kind 2.5 times as long (64 questions about 30000 shared rows, binary16: 71.5 us; at 2 times 74.9,
- * at 3 times 71.1, and pieces of prompts among tokens slower). A unit's beginning is round trips that its workgroup waits for, or
+ * the memory's rate, of the matrix kind 2.5 times as long (pieces of prompts among tokens 42.6 us, 64 questions about 30000
+ * shared rows, binary16, 60.2; at 2 times 43.7 and 59.6, at 1.75 times 43.8 and 60.2). A unit's beginning is round trips that its workgroup waits for, or
  * its wave beside others. Eight units of cost a step, so that a share of the smallest batches is one step. */
 constexpr int AB_COST_V = 8, AB_COST_M = 20, AB_BEGIN_V = 8, AB_BEGIN_M = 80;
 
@@ -359,32 +359,34 @@ template <int KVT>
 struct PagedHead {
     const char *cache;
     const int32_t *table;
-    size_t block;
+    uint32_t block; /* bytes, at most 2^29 and some scales */
     int npages, shift, mask, hd;
     uint32_t row, scales; /* the head's first row and first scale in a block, bytes */
     static constexpr int SIZE = KVT == KV_F32 ? 4 : KVT == KV_F16 ? 2 : 1;
     __device__ __forceinline__ PagedHead(const PageDev &pg, const void *cache, int seq, int g)
-        : cache((const char *)cache), table(pg.table + (size_t)seq * pg.max_pages), block(pg.block), npages(pg.npages),
+        : cache((const char *)cache), table(pg.table + (size_t)seq * pg.max_pages), block((uint32_t)pg.block), npages(pg.npages),
           shift(pg.shift), mask((1 << pg.shift) - 1), hd(pg.hd), row(((uint32_t)g << pg.shift) * pg.hd * SIZE),
           scales((((uint32_t)pg.nkv << pg.shift) * pg.hd) + ((uint32_t)g << pg.shift) * 4) {}
-    /* an entry that is no page of the cache: any page stands for it */
-    __device__ __forceinline__ int page_of(int p) const {
-        const int id = table[p >> shift];
-        return (uint32_t)id < (uint32_t)npages ? id : 0;
+    /* An entry as it stands in the table. It is looked at when its rows are requested, a turn later: here that would wait for the
+     * entry, and for everything that was requested before it (a tile of many rows 2.4 instead of 2.1 us). */
+    __device__ __forceinline__ int page_of(int p) const { return table[p >> shift]; }
+    __device__ __forceinline__ unsigned long long page(int id) const { /* no page of the cache: any page stands for it */
+        return (unsigned long long)((uint32_t)id < (uint32_t)npages ? (uint32_t)id : 0) * block;
     }
-    __device__ __forceinline__ const char *at(int id, int p, int col) const {
-        return cache + (size_t)id * block + (row + (uint32_t)((p & mask) * hd + col) * SIZE);
+    __device__ __forceinline__ unsigned long long where(int id, int p, int col) const {
+        return page(id) + (row + (uint32_t)((p & mask) * hd + col) * SIZE);
     }
-    __device__ __forceinline__ Raw8<KVT> load8(int id, int p, int col) const {
+    __device__ __forceinline__ const char *at(int id, int p, int col) const { return cache + where(id, p, col); }
+    __device__ __forceinline__ Raw8<KVT> load8(unsigned long long where) const {
         Raw8<KVT> r;
-        const char *s = at(id, p, col);
+        const char *s = cache + where;
         if constexpr (KVT == KV_F32) r.a = *(const uint4 *)s, r.b = *(const uint4 *)(s + 16);
         else if constexpr (KVT == KV_F16) r.a = *(const uint4 *)s;
         else r.a = *(const uint2 *)s;
         return r;
     }
     __device__ __forceinline__ float scale(int id, int p) const {
-        if constexpr (KVT == KV_I8) return *(const float *)(cache + (size_t)id * block + scales + (uint32_t)(p & mask) * 4);
+        if constexpr (KVT == KV_I8) return *(const float *)(cache + page(id) + (scales + (uint32_t)(p & mask) * 4));
         return 1.0f;
     }
 };
@@ -476,7 +478,7 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
 #pragma unroll
             for (int v = 0; v < VP; v++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) rf[v][j] = kh.load8(pv[v], in(at_v(base, v)), col[j]);
+                for (int j = 0; j < 2; j++) rf[v][j] = kh.load8(kh.where(pv[v], in(at_v(base, v)), col[j]));
         } else {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -494,7 +496,7 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
 #pragma unroll
         for (int v = 0; v < VP; v++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) rv[v][j] = vh.load8(pv[v], in(at_v(base, v)), col[j]);
+            for (int j = 0; j < 2; j++) rv[v][j] = vh.load8(vh.where(pv[v], in(at_v(base, v)), col[j]));
     };
     ask(p0);
     /* the query rows: row c mod 4 of this wave's; rows past the last one are of no use to anyone */

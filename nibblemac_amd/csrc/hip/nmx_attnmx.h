@@ -76,15 +76,15 @@ __device__ __forceinline__ half4 lds_tr(const _Float16 *p) {
     return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(uintptr_t)p));
 }
 
-/* A row's 16-byte chunks of binary16 in LDS, moved by an XOR so that the operands' reads (16
- * positions of one chunk for the keys, 4 positions of two chunks for the values) meet no bank twice. */
+/* A row's 16-byte chunks of binary16 in LDS, moved by an XOR so that the operands' reads (16 positions of one chunk
+ * for the keys, 8 positions of two chunks for the values, 256 bytes a cycle) meet no bank twice. */
 template <int W>
 __device__ __forceinline__ int k_at(int p, int chunk) {
-    return p * W + ((chunk ^ (p & 7)) << 3);
+    return p * W + ((chunk ^ (W >= 128 ? p & 15 : p >> 1 & 7)) << 3);
 }
 template <int W>
 __device__ __forceinline__ int v_at(int p, int chunk) {
-    return p * W + ((chunk ^ ((p & 3) << 1)) << 3);
+    return p * W + ((chunk ^ (W >= 128 ? p & 7 : p >> 1 & 3) << 1) << 3);
 }
 
 /* 8 values of a cache row as they lie in it */
@@ -194,7 +194,7 @@ struct Running {
  * the low parts. */
 template <int OD, int KVT>
 __device__ __forceinline__ void add_tile(Running<OD / 16> &r, const float (&x)[8], const int (&e)[8], const float (&f)[8],
-                                         const _Float16 *const (&vb)[4], int plane) {
+                                         const _Float16 *const (&vb)[8], int plane) {
     constexpr int DT = OD / 16;
     float mx = x[0];
 #pragma unroll
@@ -232,29 +232,47 @@ __device__ __forceinline__ void add_tile(Running<OD / 16> &r, const float (&x)[8
     r.lc = (all - r.l) - more, r.l = all;
 #pragma unroll
     for (int i = 0; i < 8; i += 2) split2(wv[i], wv[i + 1], ph, pl, i);
-#pragma unroll
-    for (int d = 0; d < DT; d++) {
-        /* values of column c of the tile's 16, positions in the weights' order */
-        const _Float16 *at = vb[d & 3] + 16 * d;
-        half8 y;
+    /* values of column c of the tile's 16, positions in the weights' order: those of the next G column tiles are on
+     * their way while the products of these run */
+    constexpr int G = KVT == KV_F32 ? 1 : 2; /* fp32: no registers for more */
+    half8 y[2][G], z[2][G];
+    auto read = [&](int d, half8 &to, int at_plane) {
+        const _Float16 *at = vb[d & 7] + 16 * d + at_plane;
         const half4 y0 = lds_tr(at), y1 = lds_tr(at + 16 * OD);
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[i] = y0[i], y[4 + i] = y1[i];
-        r.o[d] = mfma16(y, ph, r.o[d]);
-        r.o[d] = mfma16(y, pl, r.o[d]);
-        if constexpr (KVT == KV_F32) {
-            const half4 z0 = lds_tr(at + plane), z1 = lds_tr(at + plane + 16 * OD);
-            half8 z;
+        for (int i = 0; i < 4; i++) to[i] = y0[i], to[4 + i] = y1[i];
+    };
+    auto ask = [&](int d0, int b) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) z[i] = z0[i], z[4 + i] = z1[i];
-            r.o[d] = mfma16(z, ph, r.o[d]);
+        for (int g = 0; g < G; g++) {
+            read(d0 + g, y[b][g], 0);
+            if constexpr (KVT == KV_F32) read(d0 + g, z[b][g], plane);
         }
+    };
+    ask(0, 0);
+#pragma unroll
+    for (int d = 0; d < DT; d += G) {
+        const int b = d / G & 1;
+        if (d + G < DT) ask(d + G, b ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < G; g++) r.o[d + g] = mfma16(y[b][g], ph, r.o[d + g]);
+#pragma unroll
+        for (int g = 0; g < G; g++) r.o[d + g] = mfma16(y[b][g], pl, r.o[d + g]);
+        if constexpr (KVT == KV_F32)
+#pragma unroll
+            for (int g = 0; g < G; g++) r.o[d + g] = mfma16(z[b][g], ph, r.o[d + g]);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-/* 8 waves of 16 rows (4 where a row has 512 columns) share a tile of 32 positions. The next tile is on its
+/* 8 waves of 16 rows (4 where a row has 512 columns) share a tile of 32 positions. The tile after the next one is on its
  * way into registers while the matrix cores work on the current one, with two tiles in LDS (one for
- * 512 columns of fp32, which have neither the registers nor the room). The same kernel serves few rows,
+ * 512 columns of fp32, which have neither the registers nor the room). Half of the waves, one on each SIMD, bring the next
+ * tile to LDS before they work on the current one, the others afterwards, so that a SIMD's two waves need
+ * its matrix core and its vector unit at different times. A tile of 128 rows, 256 columns, binary16 / int8 / fp32 takes
+ * 1.8 / 2.2 / 4.2 us (0.85 / 0.85 / 1.3 on the matrix cores alone); with all waves in step 1.9 / 2.3 / 4.8, with each
+ * operand waited for by itself 2.1 / 2.8 / 5.0. The same kernel serves few rows,
  * whose waves without rows only bring tiles: waves with tiles of their own, each staging for itself, took
  * as long over 20000 binary16 positions and much longer otherwise (5 nodes over 30000 fp32 positions 86
  * against 41 us, 2 over 16 int8 17 against 12). */
@@ -301,7 +319,7 @@ __device__ __forceinline__ void attend_tiles(Running<(HDP > 256 ? 256 : HDP) / 1
             pk[u] = kh.page_of(pt + p < p1 ? pt + p : p1 - 1);
         }
 #pragma unroll
-        for (int u = 0; u < VU; u++) {
+        for (int u = 0; u < VU && HDP > 256; u++) {
             const int p = (u * TH + tid) / VC & (AT_P - 1);
             pv[u] = vh.page_of(pt + p < p1 ? pt + p : p1 - 1);
         }
@@ -311,16 +329,18 @@ __device__ __forceinline__ void attend_tiles(Running<(HDP > 256 ? 256 : HDP) / 1
         for (int u = 0; u < KU; u++) {
             const int f = u * TH + tid, p = f / KC & (AT_P - 1), col = f % KC * 8;
             const int at = pt + p < p1 ? pt + p : p1 - 1;
-            rk[u] = kh.load8(pk[u], at, col < hd ? col : 0);
+            const auto row = kh.where(pk[u], at, col < hd ? col : 0);
+            rk[u] = kh.load8(row);
+            if (HDP <= 256) rv[u] = vh.load8(row), sv[u] = vh.scale(pk[u], at);
             sk[u] = kh.scale(pk[u], at);
         }
     };
     auto fetch_v = [&](int pt) {
 #pragma unroll
-        for (int u = 0; u < VU; u++) {
+        for (int u = 0; u < VU && HDP > 256; u++) {
             const int f = u * TH + tid, p = f / VC & (AT_P - 1), col = d0 + f % VC * 8;
             const int at = pt + p < p1 ? pt + p : p1 - 1;
-            rv[u] = vh.load8(pv[u], at, col < hd ? col : 0);
+            rv[u] = vh.load8(vh.where(pv[u], at, col < hd ? col : 0));
             sv[u] = vh.scale(pv[u], at);
         }
     };
@@ -380,18 +400,28 @@ __device__ __forceinline__ void attend_tiles(Running<(HDP > 256 ? 256 : HDP) / 1
     if constexpr (NB == 2) fetch_k(p0), fetch_v(p0), ask(p0 + AT_P);
     half8 qh[KS], ql[KS];
     const float qfac = qr.split(scale, qh, ql);
-    if (NB == 2) put_k(0), put_v(0);
-    /* this lane's operand addresses in a tile: the XORs leave two bases for the keys (chunk 4 k + gq by
-     * k's parity) and four for the values (by d mod 4), the rest is constant */
-    const int vp = 4 * gq + (c >> 2);
+    if (NB == 2) {
+        put_k(0), put_v(0);
+        fetch_k(p0 + AT_P), fetch_v(p0 + AT_P), ask(p0 + 2 * AT_P);
+    }
+    /* this lane's operand addresses in a tile: the XORs leave four bases for the keys (chunk 4 k + gq by
+     * k mod 4) and eight for the values (by d mod 8), the rest is constant; the second half of them are the first with
+     * the bit of 8 chunks, which the lane's position flips or not */
+    const int vp = 4 * gq + (c >> 2), kflip = 128 * (c >> 3), vflip = 128 * (vp >> 2 & 1);
     int kb[2], vo[4];
 #pragma unroll
     for (int i = 0; i < 2; i++) kb[i] = k_at<HDP>(c, 4 * i + gq) - 32 * i;
 #pragma unroll
     for (int i = 0; i < 4; i++) vo[i] = PL * AT_P * HDP + v_at<OD>(vp, 2 * i + ((c & 3) >> 1)) + 4 * (c & 1) - 16 * i;
+    auto stage = [&](int pt, int to) {
+        if (NB == 2 && pt + AT_P < p1) {
+            put_k(to), put_v(to);
+            if (pt + 2 * AT_P < p1) fetch_k(pt + 2 * AT_P), fetch_v(pt + 2 * AT_P), ask(pt + 3 * AT_P);
+        }
+    };
+    const bool late = wave_id() < ctx_waves<HDP>() / 2;
     int buf = 0;
     for (int pt = p0; pt < p1; pt += AT_P) {
-        const bool more = NB == 2 && pt + AT_P < p1;
         if (NB == 1) { /* one tile: no registers to hold the next one either */
             __syncthreads();
             fetch_k(pt), put_k(0);
@@ -399,7 +429,7 @@ __device__ __forceinline__ void attend_tiles(Running<(HDP > 256 ? 256 : HDP) / 1
             ask(pt + AT_P);
         }
         __syncthreads();
-        if (more) fetch_k(pt + AT_P), fetch_v(pt + AT_P), ask(pt + 2 * AT_P);
+        if (!late) stage(pt, buf ^ 1);
         if (busy) {
             const _Float16 *tk = tiles + buf * TILE;
             const float *kf = aux + buf * 3 * AT_P, *vf = kf + AT_P;
@@ -407,20 +437,40 @@ __device__ __forceinline__ void attend_tiles(Running<(HDP > 256 ? 256 : HDP) / 1
             float4v sc[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) sc[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < KS; k++)
+            /* the keys of the next 32 columns are on their way while the products of these run */
+            half8 key[2][2], low[2]; /* fp32: no registers for the next low parts */
+            auto ask_keys = [&](int k) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const _Float16 *at = tk + kb[k & 1] + 16 * i * HDP + 32 * k;
-                    const half8 x = *(const half8 *)at;
-                    sc[i] = mfma16(x, qh[k], sc[i]);
-                    sc[i] = mfma16(x, ql[k], sc[i]);
-                    if constexpr (KVT == KV_F32) sc[i] = mfma16(*(const half8 *)(at + AT_P * HDP), qh[k], sc[i]);
+                    const _Float16 *at = (k & 2 ? tk - kflip : tk) + kb[k & 1] + 16 * i * HDP + 32 * k;
+                    key[k & 1][i] = *(const half8 *)at;
                 }
+            };
+            auto ask_low = [&](int k) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    low[i] = *(const half8 *)((k & 2 ? tk - kflip : tk) + kb[k & 1] + (16 * i + AT_P) * HDP + 32 * k);
+            };
+            ask_keys(0);
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                if (KVT == KV_F32) ask_low(k);
+                if (k + 1 < KS) ask_keys(k + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < 2; i++) sc[i] = mfma16(key[k & 1][i], qh[k], sc[i]);
+#pragma unroll
+                for (int i = 0; i < 2; i++) sc[i] = mfma16(key[k & 1][i], ql[k], sc[i]);
+                if constexpr (KVT == KV_F32)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) sc[i] = mfma16(low[i], qh[k], sc[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const int left = lim - pt - 4 * gq;
             float x[8], f[8];
             int e[8];
 #pragma unroll
-            for (int h = 0; h < 2; h++) { /* positions 16 h + 4 gq + j */
+            for (int h = 0; h < 2; h++) { /* positions 16 h + 4 gq + j, seen below left */
                 const int p = 16 * h + 4 * gq;
                 float4v k4{1.0f, 1.0f, 1.0f, 1.0f}, f4 = k4;
                 int4 e4 = make_int4(0, 0, 0, 0);
@@ -430,13 +480,14 @@ __device__ __forceinline__ void attend_tiles(Running<(HDP > 256 ? 256 : HDP) / 1
                 for (int j = 0; j < 4; j++) {
                     float y = sc[h][j] * qfac;
                     if constexpr (KVT != KV_F16) y *= k4[j];
-                    x[4 * h + j] = pt + p + j < lim ? y : -INFINITY, f[4 * h + j] = f4[j], e[4 * h + j] = ej[j];
+                    x[4 * h + j] = j < left - 16 * h ? y : -INFINITY, f[4 * h + j] = f4[j], e[4 * h + j] = ej[j];
                 }
             }
-            const _Float16 *const vb[4] = {tk + vo[0], tk + vo[1], tk + vo[2], tk + vo[3]};
+            const _Float16 *const tf = tk - vflip, *const vb[8] = {tk + vo[0], tk + vo[1], tk + vo[2], tk + vo[3],
+                                                                   tf + vo[0], tf + vo[1], tf + vo[2], tf + vo[3]};
             add_tile<OD, KVT>(r, x, e, f, vb, AT_P * OD);
         }
-        if (more) put_k(buf ^ 1), put_v(buf ^ 1);
+        if (late) stage(pt, buf ^ 1);
         if (NB == 2) buf ^= 1;
     }
 }

@@ -122,9 +122,10 @@ struct Head {
           scales((const float *)((const char *)cache + (size_t)a.nkv * a.max_ctx * a.hd) + (size_t)g * a.max_ctx), hd(a.hd) {}
     __device__ __forceinline__ const char *at(int p, int col) const { return rows + (uint32_t)(p * hd + col) * SIZE; }
     __device__ __forceinline__ int page_of(int) const { return 0; } /* one block */
-    __device__ __forceinline__ Raw8<KVT> load8(int, int p, int col) const {
+    __device__ __forceinline__ uint32_t where(int, int p, int col) const { return (uint32_t)(p * hd + col) * SIZE; }
+    __device__ __forceinline__ Raw8<KVT> load8(uint32_t where) const {
         Raw8<KVT> r;
-        const char *s = at(p, col);
+        const char *s = rows + where;
         if constexpr (KVT == KV_F32) r.a = *(const uint4 *)s, r.b = *(const uint4 *)(s + 16);
         else if constexpr (KVT == KV_F16) r.a = *(const uint4 *)s;
         else r.a = *(const uint2 *)s;

@@ -268,6 +268,19 @@ def test_most_sequences(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,ctx,nh,nkv,hd,page,kv,groups", [
+    ([1, 1], [70, 5], 1024, 1, 64, 16, KV_F16, ()),           # most heads, on one KV head
+    ([2], [40], 1024, 1024, 64, 256, KV_I8, ()),              # and each on its own
+    ([512], [0], 16, 2, 64, 32, KV_F32, ()),                  # a chunk of a prompt, nothing before it
+    ([511, 1], [33, 600], 4, 1, 384, 64, KV_F16, ()),
+    ([200, 1, 1, 100], [100, 64, 31, 32], 4, 2, 448, 16, KV_I8, [(0, 31)]),
+    ([1] * 9, [3000] * 9, 8, 1, 256, 64, KV_F32, [(0, 2999), (5, 17)]),
+])
+def test_largest_shapes(dev, rows, ctx, nh, nkv, hd, page, kv, groups):
+    check(dev, Case(np.random.default_rng(nh + hd), rows, ctx, nh, nkv, hd, page, kv, groups))
+
+
+@pytest.mark.gpu
 def test_caches_past_4_gib(dev):
     """Pages whose bytes lie past 2^32 in the cache."""
     page, nkv, hd = 256, 4, 512

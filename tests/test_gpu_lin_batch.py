@@ -115,6 +115,9 @@ CASES = [
     ([1, 2, 1], 4, 2, 64, 96, [2, 1, 0], 0),              # shared key heads
     ([17] * 3, 2, 1, 64, 128, [0, 0, 0], 0),
     ([1] * 256, 2, 1, 64, 64, None, 3),
+    ([0], 1, 1, 64, 64, [-1], 1),                         # a new sequence that waits
+    ([64] * 8, 1, 1, 128, 128, [7] * 8, 0),
+    ([1, 2], 6, 3, 128, 128, [1, -1], 0),
 ]
 
 

@@ -259,6 +259,42 @@ def test_many_rows(dev, hd, kv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_F16, KV_I8])
+def test_queries_of_different_sizes(dev, kv):
+    """Rows and heads that share a wave or a tile: near-uniform weights beside a single position that takes all, and zeros."""
+    rng = np.random.default_rng(8 + kv)
+    c = Case(rng, [1, 1, 2, 20], [400, 90, 33, 300], 8, 2, 128, 16, kv)
+    c.q[..., :128] *= np.exp(rng.uniform(-8, 3, c.q.shape[:2])).astype(np.float32)[..., None]
+    c.q[0, 3, :128] = c.q[7, 2, :128] = 0
+    check(dev, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [KV_F32, KV_F16, KV_I8])
+def test_what_one_row_holds_stays_in_it(dev, kv):
+    """NaN and infinities in a row's query, in its gate and in a sequence's cache: all other rows' bits are as without them."""
+    c = Case(np.random.default_rng(5), [1, 1, 30, 1, 3, 1], [200, 300, 64, 70, 20, 500], 8, 2, 128, 16, kv, [(0, 48), (3, 0)])
+    want = attend(dev, c)
+    t = int(c.row0[2]) + 7
+    c.q[t, 3, 5], c.q[t, 4, 128 + 9], c.q[0, 1, :128] = np.nan, np.nan, np.inf
+    for p in range(c.len[4]):    # a sequence of its own pages
+        for b in (c.kb, c.vb):
+            page, off = c.table[4, p // 16], p % 16
+            if kv == KV_I8:
+                b[page, 2 * 16 * 128:].view(np.float32).reshape(2, 16)[:, off] = np.nan
+            else:
+                b[page].view((np.float32, np.float16)[kv]).reshape(2, 16, 128)[:, off] = np.nan
+    got = attend(dev, c)
+    same = np.ones((c.n, 8), bool)
+    same[t, [3, 4]] = same[0, 1] = False
+    same[c.row0[4]:c.row0[5]] = False
+    heads = lambda x: x.reshape(c.n, 8, 128)  # noqa: E731
+    assert (heads(got)[same].view(np.uint32) == heads(want)[same].view(np.uint32)).all()
+    assert np.isnan(heads(got)[t, 3]).all() and np.isnan(heads(got)[t, 4, 9]) and np.isnan(heads(got)[0, 1]).all()
+    assert np.isnan(heads(got)[c.row0[4]:c.row0[5]]).all()
+
+
+@pytest.mark.gpu
 def test_most_sequences(dev):
     """256 sequences and groups."""
     rng = np.random.default_rng(15)

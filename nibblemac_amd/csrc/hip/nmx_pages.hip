@@ -35,7 +35,7 @@ struct PagesDev {
     int pack;
     int32_t *out;
     Lists *lists;
-    int32_t *fresh, *holes, *movers, *to; /* [npages] each */
+    int32_t *fresh, *holes, *movers;      /* [npages] each */
     int32_t *rows;                        /* [seqs][max_pages]: the entries of sequences that fork */
 };
 
@@ -229,17 +229,18 @@ __global__ __launch_bounds__(PP) void pages_plan_k(const int32_t *from_, const i
     if (a.pack) { /* the used pages from their number on move to the free ones below it */
         settle<false>(); /* the tables too */
         const uint32_t used = search<LDS>(refs, 0, npages, ~0u, sum_s, [](int r) { return r != 0; }, [](int, uint32_t) {});
-        const uint32_t moves = search<LDS>(refs, (int)used, npages, ~0u, sum_s, [](int r) { return r != 0; },
-                                           [&](int p, uint32_t i) { a.movers[i] = p; });
+        /* as many are free below it as used from it on, so holes' numbers never reach the pages that move: fresh[i] is the
+         * i-th hole and fresh[p] where p goes */
+        const uint32_t moves = search<LDS>(refs, 0, (int)used, ~0u, sum_s, [](int r) { return r == 0; },
+                                           [&](int p, uint32_t i) { fresh[i] = p; });
+        settle<LDS>();
         if (moves)
-            (void)search<LDS>(refs, 0, (int)used, moves, sum_s, [](int r) { return r == 0; }, [&](int p, uint32_t i) { a.holes[i] = p; });
-        int32_t *to = LDS ? fresh : a.to;
-        settle<false>();
-        for (uint32_t i = tid; i < moves; i += PP) {
-            const int p = a.movers[i], h = a.holes[i];
-            to[p] = h;
-            refs.p[h] = refs.get(p), refs.p[p] = 0;
-        }
+            (void)search<LDS>(refs, (int)used, npages, ~0u, sum_s, [](int r) { return r != 0; }, [&](int p, uint32_t i) {
+                const int h = fresh[i];
+                a.movers[i] = p, a.holes[i] = h, fresh[p] = h;
+                refs.p[h] = refs.get(p), refs.p[p] = 0;
+            });
+        const int32_t *to = fresh;
         if (tid == 0) a.lists->moves = (int)moves;
         if (tid == 2 || tid == 3) a.out[tid] = (int)(tid == 2 ? used : moves);
         settle<LDS>();
@@ -335,7 +336,7 @@ extern "C" {
 
 size_t nmx_pages_work_bytes(int npages, int seqs, int max_pages) {
     if (npages < 1 || npages > (1 << 20) || seqs < 1 || seqs > NMX_BATCH_MAX || max_pages < 1 || max_pages > (1 << 16)) return 0;
-    return up16(sizeof(Lists)) + 4 * up16((size_t)npages * 4) + up16((size_t)seqs * max_pages * 4);
+    return up16(sizeof(Lists)) + 3 * up16((size_t)npages * 4) + up16((size_t)seqs * max_pages * 4);
 }
 
 int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work) {
@@ -369,8 +370,8 @@ int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work) {
     const size_t nb = up16((size_t)np * 4);
     a.refs = p->refs, a.from = p->from, a.keep = p->keep, a.add = p->add, a.pack = p->pack != 0, a.out = p->out;
     a.lists = (Lists *)w, w += up16(sizeof(Lists));
-    a.fresh = (int32_t *)w, a.holes = (int32_t *)(w + nb), a.movers = (int32_t *)(w + 2 * nb), a.to = (int32_t *)(w + 3 * nb);
-    a.rows = (int32_t *)(w + 4 * nb);
+    a.fresh = (int32_t *)w, a.holes = (int32_t *)(w + nb), a.movers = (int32_t *)(w + 2 * nb);
+    a.rows = (int32_t *)(w + 3 * nb);
     const nmx_on_device on(ctx);
     if (np <= PP_LDS) {
         static std::atomic<uint64_t> set0;

@@ -300,19 +300,35 @@ __global__ __launch_bounds__(64 * LD_WAVES) void lora_one_k(Lora a) {
     up.store(scale);
 }
 
+/* an adapter has at most one tile that is not full */
+int tiles_of(const Lora &a) {
+    const int most = a.n / 16 + (a.adapters < a.n ? a.adapters : a.n);
+    return most < a.n ? most : a.n;
+}
+/* workgroups of a tile's output rows, `run` rows each */
+int runs_of(const nmx_lora_args &p, int run) {
+    int n = 0;
+    for (int s = 0; s < p.count; s++) n += (p.rows[s] + run - 1) / run;
+    return n;
+}
 /* One launch where every workgroup may make A x again: 16 ranks (more are one block of them after the other) of up to
- * LO_BYTES. 8 requests, ranks of 16: 1024 binary16 columns 7.7 us against 9.7 in two launches, 3584 columns 11.6 against 13.7;
- * 64 requests on 40 adapters of 25 ranks, bfloat16, 22.6 against 18.9. */
+ * LO_BYTES, in up to two workgroups a CU, or one where the list of the tiles is longer than a wave. Ranks of 16, binary16: 8
+ * requests to 4096 + 512 + 512 rows 7.7 us against 9.7 in two launches, from 3584 columns 11.6 against 13.7; 64 on 40 adapters
+ * (440 workgroups) 12.4 against 13.5, to 3584 + 3584 (616) 16.1 against 13.5; 512 on 4 (360) 18.7 against 16.1, from 3584 columns
+ * to 1024 rows (72) 17.8 against 18.9; 64 on 40 of 25 ranks, bfloat16, 22.6 against 18.9. */
 constexpr size_t LO_BYTES = 128 * 1024;
-bool in_one(const Lora &a, int size) { return a.rank16 == 16 && (size_t)a.rank16 * a.cols * size <= LO_BYTES; }
+constexpr int LO_RUN = 16 * LU_EACH * LD_WAVES;
+bool in_one(const Lora &a, const nmx_lora_args &p, int size) {
+    return a.rank16 == 16 && (size_t)a.rank16 * a.cols * size <= LO_BYTES &&
+           (long long)tiles_of(a) * runs_of(p, LO_RUN) <= (a.n <= 64 ? 512 : 256);
+}
 
 template <int WT>
-int launch(nmx_ctx *ctx, const Lora &a) {
-    /* an adapter has at most one tile that is not full */
-    const int most = a.n / 16 + (a.adapters < a.n ? a.adapters : a.n), tiles = most < a.n ? most : a.n;
+int launch(nmx_ctx *ctx, const Lora &a, bool one) {
+    const int tiles = tiles_of(a);
     const dim3 grid((unsigned)tiles, (unsigned)a.first[a.count]);
     const bool vec = a.rank % 8 == 0;
-    if (in_one(a, WT == W_F32 ? 4 : 2)) {
+    if (one) {
         if (vec) lora_one_k<WT, true><<<grid, 64 * LD_WAVES, 0, ctx->stream>>>(a);
         else lora_one_k<WT, false><<<grid, 64 * LD_WAVES, 0, ctx->stream>>>(a);
         NMX_LAUNCHED(ctx, "lora_one");
@@ -381,15 +397,16 @@ int nmx_lora(nmx_ctx *ctx, const nmx_lora_args *p, void *work) {
             if (nmx_overlap(out[i].p, out[i].bytes, out[k].p, out[k].bytes) && !(k > 0 && side_by_side(*p, i - 1, k - 1)))
                 return nmx_fail(ctx, "nmx_lora: outputs and work overlap");
     }
-    a.rank16 = (p->rank + 15) / 16 * 16, a.cols = p->cols;
-    const int run = 16 * LU_EACH * (in_one(a, (int)ws) ? LD_WAVES : LU_WAVES); /* output rows of a workgroup */
+    a.rank16 = (p->rank + 15) / 16 * 16, a.cols = p->cols, a.n = p->n, a.adapters = p->adapters;
+    const bool one = in_one(a, *p, (int)ws);
+    const int run = one ? LO_RUN : 16 * LU_EACH * LU_WAVES; /* output rows of a workgroup */
     for (int s = 0; s < p->count; s++) a.first[s + 1] = a.first[s] + (p->rows[s] + run - 1) / run;
     if (a.first[p->count] > 65535) return nmx_fail(ctx, "nmx_lora: too many rows in all");
-    a.n = p->n, a.x_stride = p->x_stride, a.count = p->count, a.x = p->x, a.adapters = p->adapters;
+    a.x_stride = p->x_stride, a.count = p->count, a.x = p->x;
     a.rank = p->rank, a.adapter = p->adapter, a.ranks = p->ranks, a.scale = p->scale;
     a.tiles = (Tile *)work, a.low = (float *)((char *)work + N * sizeof(Tile));
     const nmx_on_device on(ctx);
-    return p->w_dtype == W_F32 ? launch<W_F32>(ctx, a) : p->w_dtype == W_F16 ? launch<W_F16>(ctx, a) : launch<W_BF16>(ctx, a);
+    return p->w_dtype == W_F32 ? launch<W_F32>(ctx, a, one) : p->w_dtype == W_F16 ? launch<W_F16>(ctx, a, one) : launch<W_BF16>(ctx, a, one);
 }
 
 } /* extern "C" */

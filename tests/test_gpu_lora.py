@@ -125,6 +125,9 @@ CASES = [
     (512, 512, [256], 1, 256, 1, None, None, 0, 0),
     (512, 32, [64] * 6, 512, 8, 2, list(range(512)), None, 0, 0),
     (5, 32768, [16], 2, 5, 0, None, None, 0, 0),
+    (64, 1024, [3584, 3584], 40, 16, 1, None, None, 0, 0),         # small ranks, many workgroups: two launches
+    (200, 64, [512, 40], 9, 12, 2, None, "ragged", 0, 0),          # in one
+    (200, 64, [4096, 4096], 9, 12, 2, None, "ragged", 0, 0),       # in two
 ]
 
 

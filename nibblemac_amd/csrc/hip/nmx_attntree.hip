@@ -16,17 +16,16 @@
  * two parts itself: three products, the low-low one left out (2^-22 of the row).
  *
  * Times of both kernels on MI355X, 8 heads on 2 of 256 (and of each in a kernel trace, context + join): 64 nodes
- * over 100000 binary16 positions 124 to 128 us, 415 TFLOP/s of the definition's products and twice that of
- * the matrix cores', which a large binary16 product runs at 1068 (traced 124 at least and 151 at the median + 14,
- * longer than the whole untraced pass); 37 nodes over 4001 int8 25.7 us (17.8 + 8.8); 9 nodes over 600
- * fp32 16.1 us (11.2 + 5.7) and one node over 20000 binary16 17.5 us (13.0 + 5.7): the latter 41 MB, 8 us
+ * over 100000 binary16 positions 122 us (the same ones again and again 113), 428 TFLOP/s of the definition's products and twice that of
+ * the matrix cores', which a large binary16 product runs at 1106 (traced 111 at least and 120 at the median + 14);
+ * 37 nodes over 4001 int8 25.3 us (17.3 + 8.9); 9 nodes over 600
+ * fp32 15.1 us (10.3 + 5.6) and one node over 20000 binary16 16.8 us (11.2 + 6.1): the latter 41 MB, 8 us
  * as a copy; the others are chains of round trips to memory (position, rows, barrier, parts, position, parts,
- * rows). Long fp32 and int8 contexts: 5 nodes over 30000 fp32 40 us (123 MB, 24 as a copy), 64 of them 87;
- * 9 over 100000 int8 58 us (104 MB, 20), 64 of them 143.
+ * rows). Long fp32 and int8 contexts (before the tiles' waves worked a phase apart): 5 nodes over 30000 fp32 40 us (123 MB, 24 as
+ * a copy), 64 of them 87; 9 over 100000 int8 58 us (104 MB, 20), 64 of them 143.
  *
- * The largest case is bound by two things alike: a wave's 16 rows read the whole tile from LDS, 8 x 32 KiB
- * for 32 positions, 2048 cycles at 128 bytes each and as long as its matrix instructions (counted: LDS
- * active in 49 % of the CUs' busy cycles, 22 % of them bank conflicts, matrix cores in 43 %). */
+ * The largest case is bound by the matrix cores and the vector unit together (counted: either is active in 51 % of the CUs'
+ * busy cycles, LDS in 32 % without a bank conflict): two waves of a SIMD leave the one idle while both need the other. */
 #include "nmx_internal.h"
 #include "nmx_a8.h"
 #include "nmx_attn.h"

@@ -10,7 +10,7 @@
  * 16-byte loads to the operand without passing through LDS.
  *
  * Times on MI355X: 8 requests, 5 adapters of 16 ranks, 1024 columns to 4096 + 512 + 512 rows 7.7 us (one launch); 64 requests, 40
- * adapters of up to 64 ranks, 1024 to 3584 + 3584 21 (10.0 + 11.8 in a trace, 5.1 as a copy): most tiles have one or two
+ * adapters of up to 64 ranks, 1024 to 3584 + 3584 21 (9.7 + 12.4 in a trace, 5.1 as a copy): most tiles have one or two
  * rows, and each launch is a chain of round trips; 512 requests of one adapter of 64 ranks 24. */
 #include "nmx_internal.h"
 #include "nmx_attn.h"

@@ -9,9 +9,9 @@
  * opposite additions. A fork's entries go through the workspace, so sequences may exchange places. pages_copy_k and, with
  * pack, pages_move_k then copy what the plan lists, in all caches at once.
  *
- * Times on MI355X: a token of 64 chats in 640 pages 11.2 us, of which the plan 7.6 and the copy of five pages in 14 caches 4 in
- * a trace, both chains of round trips (the bytes take 0.8); 16 of 64 chats end and the others are packed, 1200 pages, 17.5 + 4.3
- * + 21.2 in a trace, 26 as a copy. With the counts in memory, an atomic's round trip each, the plans took 15.8 and 34.5. */
+ * Times on MI355X: a token of 64 chats in 640 pages 11.4 us, of which the plan 7.8 and the copy of five pages in 14 caches 3.5 in
+ * a trace, both chains of round trips (the bytes take 0.8); 16 of 64 chats end and the others are packed, 1200 pages, 12.8 + 4.6
+ * + 21.3 in a trace, 26 as a copy. With the counts in memory, an atomic's round trip each, the first plan took 15.8. */
 #include "nmx_internal.h"
 #include "nmx_batch.h"
 #include "nmx_lanes.h"

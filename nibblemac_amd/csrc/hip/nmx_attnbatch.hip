@@ -196,6 +196,7 @@ struct BatchAttn {
     Plan *plan;
     float *part_v, *part_m; /* parts of the vector kind [slot][vrows][hd], of the matrix kind [slot][tile][columns] */
     float4 *stat_v, *stat_m;
+    int rep;          /* heads of a KV head */
     int jcols, vrows; /* vrows: AB_VR, or the query rows of a KV head if there are fewer */
     float *o;
     int8_t *aq;
@@ -273,7 +274,7 @@ __device__ __forceinline__ Shares make_list(const Head0 &b, const BatchAttn &a, 
     }
     /* costs and units of its kind before each segment */
     unsigned long long cb[2] = {0, 0}, ub = 0; /* vector, matrix; units: vector in the lower half */
-    const int rep = a.nh / a.pg.nkv;
+    const int rep = a.rep;
 #pragma unroll 1
     for (int j0 = 0; j0 < G + S; j0 += 64) {
         const int j = j0 + lane;
@@ -449,7 +450,7 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
     constexpr int VP = HDP > 256 ? 2 * VT : VT;            /* positions whose values a lane adds in a turn */
     constexpr int KN = F32 ? 1 : HDP / 32;                 /* a key's chunks of 32 columns over the quarters */
     constexpr int NW = F32 ? VP : NT * VT;                 /* scores of a lane in a turn */
-    const int lane = lane_id(), wave = wave_id(), l = lane % LPP, c = lane & 15, gq = lane >> 4, hd = a.pg.hd, rep = a.nh / a.pg.nkv;
+    const int lane = lane_id(), wave = wave_id(), l = lane % LPP, c = lane & 15, gq = lane >> 4, hd = a.pg.hd, rep = a.rep;
     const PagedHead<KVT> kh(a.pg, a.kc, x.seq, g), vh(a.pg, a.vc, x.seq, g);
     int col[2];
 #pragma unroll
@@ -744,7 +745,7 @@ template <int HDP, int KVT>
 __device__ __forceinline__ void matrix_piece(const BatchAttn &a, const Seg &x, int g, int tile, int half, int p0, int p1,
                                              float *part, float4 *stat, uint4 *smem) {
     constexpr int OD = HDP > 256 ? 256 : HDP, KS = HDP / 32;
-    const int lane = lane_id(), wave = wave_id(), c = lane & 15, gq = lane >> 4, hd = a.pg.hd, rep = a.nh / a.pg.nkv;
+    const int lane = lane_id(), wave = wave_id(), c = lane & 15, gq = lane >> 4, hd = a.pg.hd, rep = a.rep;
     const int row0 = tile * tile_rows<HDP>() + wave * 16, rr = row0 + c, d0 = half * OD;
     const bool live = rr < x.m;
     const int i = (live ? rr : 0) / rep, h = g * rep + (live ? rr : 0) % rep;
@@ -822,7 +823,7 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
     }
     __syncthreads(); /* everyone has read the first piece */
     /* the waves that a row's heads take (4 each) go over the same positions at the same time */
-    const int heads = a.nh / a.pg.nkv, team = heads > 4 ? 2 : 1;
+    const int heads = a.rep, team = heads > 4 ? 2 : 1;
 #pragma unroll 1
     for (int share = (w - mxs) * AB_PARTS + wave / team; share < (w - mxs + 1) * AB_PARTS; share += WV / team) {
         if (tid % 64 == 0) piece_s[wave].next = share * sh_s.per_w;
@@ -862,7 +863,7 @@ struct Parts {
     bool any; /* the row belongs to a sequence */
     __device__ __forceinline__ Parts(const BatchAttn &a, int t, int h, int half) {
         constexpr int OD = HDP > 256 ? 256 : HDP;
-        const int hd = a.pg.hd, nkv = a.pg.nkv, rep = a.nh / nkv, g = h / rep;
+        const int hd = a.pg.hd, nkv = a.pg.nkv, rep = a.rep, g = h / rep;
         const Shares sh = a.plan->sh;
         const int s = seq_of_row(a.row0, a.pg.seqs, t);
         any = false;
@@ -887,18 +888,19 @@ struct Parts {
             uint32_t vs = 0, ss = 0;
             if (x.unit && rr >= 0 && rr < x.m) {
                 const bool mx = x.m > AB_VR;
-                const int tr = mx ? tile_rows<HDP>() : a.vrows, width = mx ? OD : hd;
-                const uint32_t u = (mx ? rr / tr * halves<HDP>() + half : 0) * nkv + g;
+                constexpr int TR = tile_rows<HDP>(); /* few rows: one tile */
+                const int tr = mx ? TR : a.vrows, tile = mx ? rr / TR : 0, in = mx ? rr % TR : rr, width = mx ? OD : hd;
+                const uint32_t u = (mx ? tile * halves<HDP>() + half : 0) * nkv + g;
                 const unsigned long long cu = x.c0 + (unsigned long long)u * x.unit, per = mx ? sh.per_m : sh.per_w;
                 const uint32_t w0 = over(cu, per), w1 = over(cu + x.unit - 1, per);
                 n = so = (int)(w1 - w0) + 1;
                 if (!mx) {
-                    const uint32_t f0 = (w0 * per == cu ? w0 + AB_PARTS - 1 : w0 + AB_PARTS) / AB_PARTS, f1 = over(cu + x.unit, per) / AB_PARTS;
+                    const uint32_t f0 = (w0 * per == cu ? w0 + AB_PARTS - 1 : w0 + AB_PARTS) / AB_PARTS, f1 = (w1 + (cu + x.unit == (w1 + 1) * per)) / AB_PARTS;
                     if (f1 > f0) so = (int)(f0 * AB_PARTS - w0), wh = (int)(f1 - f0), n -= wh * (AB_PARTS - 1);
                 }
                 const size_t slot = (size_t)w0 + x.u0 + u;
-                v = (mx ? a.part_m : a.part_v) + (slot * tr + rr % tr) * width + (mx ? 0 : half * OD);
-                f = (mx ? a.stat_m : a.stat_v) + slot * tr + rr % tr;
+                v = (mx ? a.part_m : a.part_v) + (slot * tr + in) * width + (mx ? 0 : half * OD);
+                f = (mx ? a.stat_m : a.stat_v) + slot * tr + in;
                 vs = tr * width, ss = tr;
             }
             if (k) count[1] = n, solo[1] = so, whole[1] = wh, val[1] = v, st[1] = f, vstep[1] = vs, sstep[1] = ss;
@@ -1234,7 +1236,7 @@ int nmx_attn_batch(nmx_ctx *ctx, const nmx_attn_batch_args *p, void *work) {
                 return nmx_fail(ctx, "nmx_attn_batch: outputs and work overlap");
     }
     char *ws = (char *)work;
-    a.n = p->n, a.nh = p->nh, a.groups = p->groups, a.row0 = p->row0, a.group0 = p->group0, a.shared = p->shared;
+    a.n = p->n, a.nh = p->nh, a.rep = p->nh / a.pg.nkv, a.groups = p->groups, a.row0 = p->row0, a.group0 = p->group0, a.shared = p->shared;
     a.q = p->q, a.kc = p->kc, a.vc = p->vc, a.scale = p->scale, a.plan = (Plan *)(ws + r.plan);
     a.part_v = (float *)ws, a.stat_v = (float4 *)(ws + r.stat_v), a.part_m = (float *)(ws + r.part_m);
     a.stat_m = (float4 *)(ws + r.stat_m), a.jcols = r.jcols, a.vrows = r.vrows, a.o = p->o, a.aq = p->a8.q, a.ad = p->a8.d, a.afs = p->a8.fs;

@@ -180,9 +180,16 @@ struct Shares {
     unsigned long long per_m, per_w; /* the cost of a workgroup's share, of a wave's */
     int mx;
 };
+/* What the join asks for: the shares, and for each row its sequence's segment and its group's prefix (r0 below 0: the row
+ * belongs to nobody), at an address that the row's number gives. */
+struct RowSeg {
+    unsigned long long c0;
+    uint32_t unit, u0;
+    int m, r0;
+};
 struct Plan {
     Shares sh;
-    Seg seg[AB_SEGS]; /* the groups, then the sequences */
+    RowSeg row[NMX_CHUNK_ROWS][2]; /* the prefix, the rest */
 };
 constexpr int AB_PARTS = 8; /* shares of a vector workgroup */
 
@@ -767,7 +774,7 @@ __device__ __forceinline__ void matrix_piece(const BatchAttn &a, const Seg &x, i
 template <int HDP, int KVT>
 __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int32_t *row0, const int32_t *len, int seqs, int n,
                                                                      int groups, int room, BatchAttn a) {
-    constexpr int TH = 64 * ctx_waves<HDP>(), OD = HDP > 256 ? 256 : HDP;
+    constexpr int OD = HDP > 256 ? 256 : HDP;
     extern __shared__ uint4 smem[];
     constexpr int WV = ctx_waves<HDP>();
     __shared__ Seg seg[AB_SEGS];
@@ -783,8 +790,22 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
         if (w == 0 && tid == 0) a.plan->sh = sh;
     }
     __syncthreads();
-    if (w == 0) /* the join's */
-        for (int j = tid; j < segs; j += TH) a.plan->seg[j] = seg[j];
+    if (wave == WV - 1) /* the join's rows, each by one workgroup */
+#pragma unroll 1
+        for (int t = w; t < n; t += AB_WGS) {
+            auto put = [&](int k, const Seg &x, uint32_t unit) { a.plan->row[t][k] = RowSeg{x.c0, unit, x.u0, x.m, x.r0}; };
+            bool found = false;
+#pragma unroll 1
+            for (int s = tid % 64; s < seqs; s += 64) {
+                const Seg &x = seg[groups + s];
+                if (t < x.r0 || (t - x.r0) * a.rep >= x.m) continue; /* a row has one sequence */
+                found = true;
+                put(1, x, x.unit);
+                const Seg &y = seg[x.group < 0 ? groups + s : x.group];
+                put(0, y, x.group < 0 ? 0 : y.unit);
+            }
+            if (!__any(found) && tid % 64 == 0) a.plan->row[t][1].r0 = -1;
+        }
     /* between pieces everything is in LDS: a piece has no registers to spare */
     auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
     int p0, p1, g, tile;
@@ -865,22 +886,15 @@ struct Parts {
         constexpr int OD = HDP > 256 ? 256 : HDP;
         const int hd = a.pg.hd, nkv = a.pg.nkv, rep = a.rep, g = h / rep;
         const Shares sh = a.plan->sh;
-        const int s = seq_of_row(a.row0, a.pg.seqs, t);
-        any = false;
-        if (s < 0) return; /* uniform over the wave */
-        const SeqRows rows = seq_rows(a.row0, s, a.n);
-        if (t >= rows.r0 + rows.count) return;
-        any = true;
-        const Seg own = a.plan->seg[a.groups + s];
-        Seg pre = own;
-        pre.unit = 0;
-        if (own.group >= 0) pre = a.plan->seg[own.group];
+        const RowSeg pre = a.plan->row[t][0], own = a.plan->row[t][1];
+        any = own.r0 >= 0;
+        if (!any) return; /* uniform over the wave */
         auto over = [](unsigned long long c, unsigned long long n) {
             return c >> 32 || n >> 32 ? (uint32_t)(c / n) : (uint32_t)c / (uint32_t)n;
         };
 #pragma unroll 1
         for (int k = 0; k < 2; k++) {
-            const Seg &x = k ? own : pre;
+            const RowSeg &x = k ? own : pre;
             const int rr = (t - x.r0) * rep + h % rep;
             int n = 0, so = 0, wh = 0;
             const float *v = nullptr;

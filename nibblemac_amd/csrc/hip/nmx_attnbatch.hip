@@ -17,8 +17,9 @@
  * matrix cores: tiles in LDS that the workgroup shares (nmx_attnmx.h).
  *
  * Times of both kernels on MI355X, 8 heads on 2 of 256, and of the attention kernel in a trace: 4 sequences of 300 to 700 fp32
- * positions 14.4 us (9.7), 48 of 50 to 6000 binary16 32 (27, inputs out of the caches 37 in all; 118 MB, 23 as a copy), 64 of 1500 binary16 43 and fp32 81 (393 MB, 76
- * as a copy), 64 with 30000 binary16 positions in common 60 (57, out of the caches 69), 20 of up to 90 rows with 700 int8 ones in common 43. */
+ * positions 13.8 us (9.6), 48 of 50 to 6000 binary16 31 (27; inputs out of the caches 37 in all; 118 MB, 23 as a copy), 64 of
+ * 1500 binary16 42 and fp32 81 (393 MB, 76 as a copy), 64 with 30000 binary16 positions in common 60 (56; out of the caches
+ * 69), 20 of up to 90 rows with 700 int8 ones in common 42 (32). */
 #include <type_traits>
 
 #include "nmx_internal.h"

@@ -574,9 +574,10 @@ int nmx_pages_update(nmx_ctx *ctx, const nmx_pages_args *p, void *work);
  * i, of the tables [rope_rows][rot / 2] (values outside are taken as the nearer end). rope_pos: device
  * int32 [n][axes], or NULL: a row's position in its sequence on every axis. axis: host array [rot / 2],
  * read by the call, or NULL: axis 0. A row without a place (a negative position, past max_pages, a table entry
- * that is no page) is turned but not stored. One axis: rows equal nmx_attn_prep's bit for bit.
+ * that is no page) is turned but not stored; len may be more than a table holds, the rows before keep their
+ * places. One axis: rows equal nmx_attn_prep's bit for bit.
  *
- * nmx_attn for a batch: row row0[s] + i sees the positions of its sequence up to its own; o *= sigmoid(gate);
+ * nmx_attn for a batch: row row0[s] + i sees the positions of its sequence up to its own, as far as the table goes; o *= sigmoid(gate);
  * + A8 of the n rows. Group j, sequences group0[j] .. group0[j + 1] (device int32 [groups + 1], not falling),
  * begins with shared[j] rows (device [groups]) that are the same in all of them: they are read once for
  * the whole group, by the table of its first sequence that has rows (no more than come before the rows of

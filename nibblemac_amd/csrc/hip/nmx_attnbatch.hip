@@ -95,9 +95,9 @@ __global__ __launch_bounds__(64 * PREP_WAVES) void attn_batch_prep_k(const int32
     if (s < 0) return; /* uniform over the wave */
     const SeqRows rows = seq_rows(row0, s, n);
     if (t >= rows.r0 + rows.count) return;
-    const int p = seq_len(a.pg, s) - rows.count + t - rows.r0;
+    const int p = seq_len(a.pg.len, s) - (rows.count - (t - rows.r0)); /* may be past the table */
     int id = -1;
-    if (is_k && p >= 0) id = a.pg.table[(size_t)s * a.pg.max_pages + (p >> a.pg.shift)];
+    if (is_k && p >= 0 && p >> a.pg.shift < a.pg.max_pages) id = a.pg.table[(size_t)s * a.pg.max_pages + (p >> a.pg.shift)];
 #pragma unroll
     for (int e = 0; e < E; e++) {
         if (64 * e >= hd) continue;
@@ -236,9 +236,10 @@ __device__ __forceinline__ Shares make_list(const Head0 &b, const BatchAttn &a, 
 #pragma unroll 1
     for (int s = lane; s < S; s += 64) {
         const SeqRows rows = seq_rows(b.row0, s, b.n);
-        const int l = b.len[s], len = l < 0 ? 0 : l < b.room ? l : b.room;
+        const int len = seq_len(b.len, s);
         Seg &x = seg[G + s];
-        x.r0 = rows.r0, x.m = rows.count, x.p0 = 0, x.p1 = len, x.seq = s, x.last = len - rows.count, x.group = -1;
+        x.r0 = rows.r0, x.m = rows.count, x.p0 = 0, x.p1 = len < b.room ? len : b.room, x.seq = s, x.group = -1;
+        x.last = rows.count < 0 ? 0 : len - rows.count;
         falls |= rows.count < 0;
     }
 #pragma unroll 1
@@ -272,7 +273,7 @@ __device__ __forceinline__ Shares make_list(const Head0 &b, const BatchAttn &a, 
 #pragma unroll 1
         for (int g = lane; g < G; g += 64) {
             Seg &x = seg[g];
-            const int first = first_s[g], ctx = ctx_s[g], share = x.p1, end = g0_s[g + 1] < S ? g0_s[g + 1] : S;
+            const int first = first_s[g], ctx = ctx_s[g] < b.room ? ctx_s[g] : b.room, share = x.p1, end = g0_s[g + 1] < S ? g0_s[g + 1] : S;
             x.p1 = 0;
             if (first >= S) continue;
             x.seq = first, x.r0 = seg[G + first].r0, x.m = seg[G + end - 1].r0 + seg[G + end - 1].m - x.r0;

@@ -24,12 +24,8 @@ __device__ __forceinline__ SeqRows seq_rows(const int32_t *row0, int s, int n) {
     const int r0 = a < 0 ? 0 : a > n ? n : a, r1 = b < 0 ? 0 : b > n ? n : b;
     return {r0, r1 - r0};
 }
-/* The length of sequence s, within what its table can hold. */
-__device__ __forceinline__ int seq_len(const PageDev &pg, int s) {
-    const long long most = (long long)pg.max_pages << pg.shift; /* at most 2^24 */
-    const int l = pg.len[s];
-    return l < 0 ? 0 : l > most ? (int)most : l;
-}
+/* The length of sequence s: its positions past max_pages << shift have no place in the table. */
+__device__ __forceinline__ int seq_len(const int32_t *len, int s) { return len[s] < 0 ? 0 : len[s]; }
 /* The sequence of row t: the last one that begins at or before it (every lane of the wave active). */
 __device__ __forceinline__ int seq_of_row(const int32_t *row0, int seqs, int t) {
     const int lane = threadIdx.x & 63;

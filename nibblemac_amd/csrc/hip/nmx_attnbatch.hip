@@ -30,6 +30,7 @@
 #include "nmx_lanes.h"
 #include "nmx_math.h"
 #include "nmx_rms.h"
+#include "nmx_rowpos.h"
 
 namespace {
 
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(64 * PREP_WAVES) void attn_batch_prep_k(const int32
     if (s < 0) return; /* uniform over the wave */
     const SeqRows rows = seq_rows(row0, s, n);
     if (t >= rows.r0 + rows.count) return;
-    const int p = seq_len(a.pg.len, s) - (rows.count - (t - rows.r0)); /* may be past the table */
+    const int p = row_position(seq_len(a.pg.len, s), rows.count, t - rows.r0); /* may be past the table */
     int id = -1;
     if (is_k && p >= 0 && p >> a.pg.shift < a.pg.max_pages) id = a.pg.table[(size_t)s * a.pg.max_pages + (p >> a.pg.shift)];
 #pragma unroll
@@ -171,7 +172,7 @@ struct Seg {
     int m;                 /* query rows: rows times heads of a KV group */
     int p0, p1;            /* positions */
     int r0, seq;           /* first row; the sequence whose table is read */
-    int last;              /* the first row sees positions below last + 1, the next ones one more each (a prefix: all) */
+    int last;              /* what its rows see (positions_seen) */
     int group;             /* of a sequence: its group, -1 none */
 };
 /* Who takes what: of AB_WGS workgroups the first mx take the matrix kind's steps, the others the vector kind's.
@@ -239,14 +240,14 @@ __device__ __forceinline__ Shares make_list(const Head0 &b, const BatchAttn &a, 
         const int len = seq_len(b.len, s);
         Seg &x = seg[G + s];
         x.r0 = rows.r0, x.m = rows.count, x.p0 = 0, x.p1 = len < b.room ? len : b.room, x.seq = s, x.group = -1;
-        x.last = rows.count < 0 ? 0 : len - rows.count;
+        x.last = rows.count < 0 ? 0 : row_position(len, rows.count, 0);
         falls |= rows.count < 0;
     }
 #pragma unroll 1
     for (int g = lane; g < G; g += 64) {
         const int begin = a.group0[g], end = a.group0[g + 1];
         Seg &x = seg[g];
-        x.m = 0, x.r0 = 0, x.p0 = 0, x.p1 = a.shared[g], x.seq = 0, x.last = 0x7ffffffe, x.group = -1;
+        x.m = 0, x.r0 = 0, x.p0 = 0, x.p1 = a.shared[g], x.seq = 0, x.last = ROWS_SEE_ALL, x.group = -1;
         ctx_s[g] = 0x7fffffff, first_s[g] = S, g0_s[g] = begin;
         if (g == G - 1) g0_s[G] = end;
         falls |= begin > end;
@@ -542,8 +543,7 @@ __device__ __forceinline__ void vector_piece(const BatchAttn &a, const Seg &x, i
 #pragma unroll
         for (int k = 0; k < KN; k++) qx[k] = c & 4 ? ql[k] : qx[k];
     }
-    const int past = x.last + 1 + ri / rep; /* a row sees positions below it */
-    const int lim = rr >= x.m ? 0 : x.last >= p1 ? p1 : past < p1 ? past : p1;
+    const int lim = rr >= x.m ? 0 : positions_seen(x.last, ri / rep, p1);
     ask(p0 + turn);
     float acc[4][16], m = -INFINITY, sum = 0.0f, lost = 0.0f; /* m is the wave's, sum this lane's */
 #pragma unroll
@@ -760,7 +760,7 @@ __device__ __forceinline__ void matrix_piece(const BatchAttn &a, const Seg &x, i
     const int i = (live ? rr : 0) / rep, h = g * rep + (live ? rr : 0) % rep;
     QueryRow<KS> qr(a.q + ((size_t)(x.r0 + i) * a.nh + h) * 2 * hd, live, hd, gq);
     const PagedHead<KVT> kh(a.pg, a.kc, x.seq, g), vh(a.pg, a.vc, x.seq, g);
-    const int lim = x.last >= p1 ? p1 : x.last + 1 + i < p1 ? x.last + 1 + i : p1;
+    const int lim = positions_seen(x.last, i, p1);
     Running<OD / 16> r;
     attend_tiles<HDP, KVT>(r, qr, a.scale, kh, vh, p0, p1, lim, d0, row0 < x.m, smem);
     r.l -= r.lc;

@@ -521,9 +521,10 @@ int nmx_tree_commit(nmx_ctx *ctx, const nmx_tree_commit_args *p);
  * One step of up to NMX_BATCH_MAX sequences with up to NMX_CHUNK_ROWS rows in all: sequence s has the
  * rows row0[s] .. row0[s + 1] (device int32 [seqs + 1], from 0 on and not falling; values outside [0, n]
  * are taken as the nearer end; lists that fall leave results unspecified): one row where it decodes, many
- * where it reads a prompt, none where it waits. Rows past row0[seqs] (a padded batch) are left alone: not read,
- * not written. The reference serves one sequence (engine/include/pinfer.h). The other calls of a step
- * (products, norms, heads, nmx_sample) take rows of whatever sequence as they are.
+ * where it reads a prompt, none where it waits. Rows past row0[seqs] (a padded batch) are left alone: every
+ * array has its n rows, but what theirs hold does not matter and nothing of them is written. The reference
+ * serves one sequence (engine/include/pinfer.h). The other calls of a step (products, norms, heads,
+ * nmx_sample) take rows of whatever sequence as they are.
  *
  * KV rows lie in pages: a cache is [npages] blocks of nmx_kv_bytes(kv_dtype, nkv, page, hd) bytes, each laid
  * out as a cache of `page` positions, and position p of sequence s is row p % page of the block

@@ -17,9 +17,14 @@
  * matrix cores: tiles in LDS that the workgroup shares (nmx_attnmx.h).
  *
  * Times of both kernels on MI355X, 8 heads on 2 of 256, and of the attention kernel in a trace: 4 sequences of 300 to 700 fp32
- * positions 13.8 us (9.6), 48 of 50 to 6000 binary16 31 (27; inputs out of the caches 37 in all; 118 MB, 23 as a copy), 64 of
- * 1500 binary16 42 and fp32 81 (393 MB, 76 as a copy), 64 with 30000 binary16 positions in common 60 (56; out of the caches
- * 69), 20 of up to 90 rows with 700 int8 ones in common 42 (32). */
+ * positions 13.7 us (9.6), 48 of 50 to 6000 binary16 31 (27; inputs out of the caches 37 in all; 118 MB, 23 as a copy), 64 of
+ * 1500 binary16 42 (37) and fp32 78 (73; 393 MB, 76 as a copy), 64 with 30000 binary16 positions in common 60 (56; out of the caches
+ * 69), 20 of up to 90 rows with 700 int8 ones in common 42 (32).
+ *
+ * Where the last two go, by clocks read in the kernel (medians of the workgroups of the matrix kind): 2.1 / 2.1 us until a workgroup
+ * begins, 5.0 / 4.2 for the list, 5.6 / 6.4 until the first tile of a share lies in LDS, 18 / 4.7 tiles of 2.0 / 2.1, 1.9 / 1.8 to
+ * store a part, 1.9 / 1.8 for the search of the next share; together 52.1 / 27.5. The last workgroup, whose share touches two units, ends
+ * 4 us after them. Shares of few rows: 2.9 for the list; then 5.6 at least in fp32, 10.6 in binary16. */
 #include <type_traits>
 
 #include "nmx_internal.h"
@@ -158,8 +163,9 @@ constexpr int AB_WGS = 256;                /* shares: a workgroup to a CU */
 constexpr int AB_VR = 8;                   /* query rows that the vector kind takes: 4 a wave */
 /* A step of 32 positions costs a workgroup this much: of the vector kind (4 query rows) what its bytes take at a CU's share of
  * the memory's rate, of the matrix kind 2.5 times as long (pieces of prompts among tokens 42.6 us, 64 questions about 30000
- * shared rows, binary16, 60.2; at 2 times 43.7 and 59.6, at 1.75 times 43.8 and 60.2). A unit's beginning is round trips that its workgroup waits for, or
- * its wave beside others. Eight units of cost a step, so that a share of the smallest batches is one step. */
+ * shared rows, binary16, 60.2; at 2 times 43.7 and 59.6, at 1.75 times 43.8 and 60.2; other heads and types take the same). A unit's beginning is round trips that its workgroup waits for, or
+ * its wave beside others. Eight units of cost a step, so that a share of the smallest batches is one step.
+ * A part's end (its store, and what the join reads of it) has no cost here. */
 constexpr int AB_COST_V = 8, AB_COST_M = 20, AB_BEGIN_V = 8, AB_BEGIN_M = 80;
 
 /* of a segment of m query rows */
@@ -871,7 +877,7 @@ __global__ __launch_bounds__(64 * ctx_waves<HDP>()) void attn_batch_k(const int3
 /* ---- the join -------------------------------------------------------------------------------------- */
 constexpr int JB = 256;              /* threads */
 /* rows, heads and halves from which a wave takes one alone (423 rows of 8 heads: 47.1 us against 52.6, 64 rows: 74.0 against
- * 71.5) */
+ * 71.5; nothing between 512 and 3384 items is measured) */
 constexpr int JB_WAVES = 1024;
 constexpr int JB_PARTS = 2 * (AB_WGS + 2 * AB_PARTS);
 

@@ -15,7 +15,9 @@
  *
  * BATCH (nmx_lin_mix_batch): the same for many sequences, a row of the grid each, from one slot of the states to another.
  * With few sequences it is a chain of phases (4 of one row 7.5 us), with many bound by the states' bytes: 64 of
- * 16 heads of 128 x 128 32.8 us for 146 MB, 28.5 as a copy. */
+ * 16 heads of 128 x 128 32.8 us for 146 MB, 28.5 as a copy (inputs in turn out of several sets; one set again and again 26.7).
+ * The rows of a sequence lie in LDS, so it has 64 at most, and the longest one's room is every workgroup's. 32 bytes of a
+ * lane are in scratch memory. */
 #include "nmx_internal.h"
 #include "nmx_linc.h"
 #include "nmx_math.h"

@@ -10,8 +10,9 @@
  * 16-byte loads to the operand without passing through LDS.
  *
  * Times on MI355X: 8 requests, 5 adapters of 16 ranks, 1024 columns to 4096 + 512 + 512 rows 7.7 us (one launch); 64 requests, 40
- * adapters of up to 64 ranks, 1024 to 3584 + 3584 21 (9.7 + 12.4 in a trace, 5.1 as a copy): most tiles have one or two
- * rows, and each launch is a chain of round trips; 512 requests of one adapter of 64 ranks 24. */
+ * adapters of up to 64 ranks, 1024 to 3584 + 3584 21 (9.7 + 12.4 in a trace, 5.1 as a copy); 512 requests of one adapter of 64
+ * ranks 25 (11.4 + 14.9, 5.7 as a copy). Two launches, each a chain of round trips: lora_up_k waits for each 32 ranks in turn
+ * and asks for half of a 128-byte line of 64 16-bit ranks at a time; every tile of 16 rows asks for its adapter again. */
 #include "nmx_internal.h"
 #include "nmx_attn.h"
 #include "nmx_batch.h"
